@@ -379,6 +379,157 @@ typedef struct tcbnn_avgpool_fc_desc {
 } tcbnn_avgpool_fc_desc;
 int tcbnn_avgpool_fc_forward(const tcbnn_avgpool_fc_desc* d, void* stream);
 
+/* ------------------------------------------------ float head of a network */
+/* What a network computes in floating point after (or between) its binary layers, forward and backward: linear layers,
+ * layer norms, and the log probabilities of its answers.  The library has no optimizer: a step on the gradients is the
+ * caller's.  NO counterpart in the reference.
+ *
+ * Matrices are row major, `*_ld` elements from one row to the next (0: rows without gaps); pointers need the alignment of
+ * one element.  Activations, weights and logits have the type `dtype` names; bias, gamma, beta, statistics, log
+ * probabilities and the gradients of bias, gamma and beta are fp32.  Sums are held in fp32 and every output is rounded
+ * once.  A call with rows = 0 launches nothing (the gradients of parameters become 0); other sizes are positive.
+ * Outputs may not overlap inputs or each other except where noted.  Results do not depend on what else runs: no atomics,
+ * the same sums in the same order in every call of the same sizes. */
+#define TCBNN_F32 0
+#define TCBNN_BF16 1
+#define TCBNN_F16 2
+
+#define TCBNN_ACT_NONE 0
+#define TCBNN_ACT_RELU 1 /* max(z, 0)                                     */
+#define TCBNN_ACT_GELU 2 /* z * (1 + erf(z / sqrt(2))) / 2                */
+#define TCBNN_ACT_SILU 3 /* z / (1 + exp(-z))                             */
+
+/* z = input * weight^T + bias;  output = act(z) + residual.  `output` may be `residual` (same pointer and stride).
+ * `preact` receives z, rounded to dtype: what tcbnn_linear_backward needs of a layer with an activation.
+ * `workspace` (tcbnn_linear_workspace_bytes; may be NULL) lets products of few rows and outputs share a long sum over
+ * inputs among workgroups.  in_features <= 1048576. */
+typedef struct tcbnn_linear_desc {
+    const void* input;     /* [rows][in_features]                     */
+    const void* weight;    /* [out_features][in_features]             */
+    const float* bias;     /* [out_features], or NULL                 */
+    const void* residual;  /* [rows][out_features], or NULL           */
+    void* output;          /* [rows][out_features]                    */
+    void* preact;          /* [rows][out_features], or NULL           */
+    int rows, in_features, out_features;
+    int dtype;             /* TCBNN_F32 / BF16 / F16                  */
+    int activation;        /* TCBNN_ACT_*                             */
+    long long input_ld, weight_ld, residual_ld, output_ld, preact_ld;
+    void* workspace;
+    size_t workspace_bytes;
+} tcbnn_linear_desc;
+size_t tcbnn_linear_workspace_bytes(int rows, int in_features, int out_features, int dtype);
+int tcbnn_linear_forward(const tcbnn_linear_desc* d, void* stream);
+
+/* With dz = grad_output * act'(z):  grad_input = dz * weight, grad_weight = dz^T * input, grad_bias = sums of dz over the
+ * rows (the gradient of `residual` is grad_output itself).  Each of the three may be NULL; what is given is overwritten.
+ * `preact` is z as the forward call wrote it (NULL without an activation); relu'(0) = 0.  In 16-bit types dz is rounded
+ * to dtype before the two products, as their results are after them; grad_bias sums it unrounded.
+ * `workspace` holds tcbnn_linear_grad_workspace_bytes (a NULL one is refused where that is not 0). */
+typedef struct tcbnn_linear_grad_desc {
+    const void* input;        /* [rows][in_features]; NULL where grad_weight is         */
+    const void* weight;       /* [out_features][in_features]; NULL where grad_input is  */
+    const void* preact;       /* [rows][out_features]                                   */
+    const void* grad_output;  /* [rows][out_features]                                   */
+    void* grad_input;         /* [rows][in_features]                                    */
+    void* grad_weight;        /* [out_features][in_features]                            */
+    float* grad_bias;         /* [out_features]                                         */
+    int rows, in_features, out_features;
+    int dtype;
+    int activation;
+    long long input_ld, weight_ld, preact_ld, grad_output_ld, grad_input_ld, grad_weight_ld;
+    void* workspace;
+    size_t workspace_bytes;
+} tcbnn_linear_grad_desc;
+size_t tcbnn_linear_grad_workspace_bytes(int rows, int in_features, int out_features, int dtype);
+int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stream);
+
+/* mean and rstd = 1 / sqrt(variance + eps) of every row (the variance about the mean, over all features);
+ * output = (input - mean) * rstd * gamma + beta.  `output` may be `input` (same pointer and stride).  `mean` and `rstd`
+ * may be NULL; tcbnn_layernorm_backward needs them.  features <= 65536. */
+typedef struct tcbnn_layernorm_desc {
+    const void* input;   /* [rows][features]          */
+    const float* gamma;  /* [features], or NULL (1)   */
+    const float* beta;   /* [features], or NULL (0)   */
+    void* output;        /* [rows][features]          */
+    float* mean;         /* [rows], or NULL           */
+    float* rstd;         /* [rows], or NULL           */
+    int rows, features;
+    int dtype;
+    float eps;           /* >= 0                      */
+    long long input_ld, output_ld;
+} tcbnn_layernorm_desc;
+int tcbnn_layernorm_forward(const tcbnn_layernorm_desc* d, void* stream);
+
+/* With xh = (input - mean) * rstd and g = grad_output * gamma:
+ * grad_input = rstd * (g - mean of g - xh * mean of g * xh) (means over a row's features), grad_gamma = sums of
+ * grad_output * xh over the rows, grad_beta = sums of grad_output.  Each of the three may be NULL.  `grad_input` may be
+ * `grad_output` (same pointer and stride).  `workspace` holds tcbnn_layernorm_grad_workspace_bytes where grad_gamma or
+ * grad_beta is asked for. */
+typedef struct tcbnn_layernorm_grad_desc {
+    const void* input;        /* [rows][features]         */
+    const float* gamma;       /* [features], or NULL (1)  */
+    const float* mean;        /* [rows]                   */
+    const float* rstd;        /* [rows]                   */
+    const void* grad_output;  /* [rows][features]         */
+    void* grad_input;         /* [rows][features]         */
+    float* grad_gamma;        /* [features]               */
+    float* grad_beta;         /* [features]               */
+    int rows, features;
+    int dtype;
+    long long input_ld, grad_output_ld, grad_input_ld;
+    void* workspace;
+    size_t workspace_bytes;
+} tcbnn_layernorm_grad_desc;
+size_t tcbnn_layernorm_grad_workspace_bytes(int rows, int features);
+int tcbnn_layernorm_backward(const tcbnn_layernorm_grad_desc* d, void* stream);
+
+/* Of every row of logits x: logsumexp = log(sum exp(x_j)); logprob = x_t - logsumexp of the given class t = targets[row];
+ * entropy = -sum p_j log p_j with p_j = exp(x_j - logsumexp) (in nats); rank = the number of classes before t in the order
+ * "larger logit first, lower index among equals" (0: t is the best); top_index, top_logprob = the first `top` classes of
+ * that order.  Any output may be NULL; targets only where logprob and rank are.
+ *   t < 0        : a row without a given class: logprob 0, rank -1.   t >= classes: logprob NaN, rank -1.
+ *   x_j = -inf   : a forbidden class: p_j = 0, no share in the entropy, log probability -inf.
+ *   all -inf     : logsumexp -inf, every log probability -inf, entropy 0.
+ *   NaN, +inf    : the row's logsumexp, log probabilities and entropy are NaN; NaN goes before every number in the order.
+ * top <= 64 and <= classes.  `workspace` (tcbnn_logprobs_workspace_bytes; a NULL one is refused where that is not 0) joins
+ * rows that several workgroups share. */
+typedef struct tcbnn_logprobs_desc {
+    const void* logits;      /* [rows][classes]           */
+    const int32_t* targets;  /* [rows]                    */
+    float* logprob;          /* [rows]                    */
+    float* entropy;          /* [rows]                    */
+    float* logsumexp;        /* [rows]                    */
+    int32_t* rank;           /* [rows]                    */
+    int32_t* top_index;      /* [rows][top]               */
+    float* top_logprob;      /* [rows][top]               */
+    int rows, classes, top;
+    int dtype;
+    long long logits_ld;
+    void* workspace;
+    size_t workspace_bytes;
+} tcbnn_logprobs_desc;
+size_t tcbnn_logprobs_workspace_bytes(int rows, int classes, int top, int dtype);
+int tcbnn_logprobs_forward(const tcbnn_logprobs_desc* d, void* stream);
+
+/* The gradient of sum over rows of grad_logprob * logprob + grad_entropy * entropy:
+ * grad_logits_j = grad_logprob * ([j = t] - p_j) - grad_entropy * p_j * (log p_j + entropy).  `logsumexp` and `entropy`
+ * are the forward call's; grad_logprob or grad_entropy may be NULL (0).  Without a given class (t < 0) grad_logprob
+ * counts as 0; with t >= classes the row is NaN unless grad_logprob is NULL; a row whose classes are all forbidden gets 0.
+ * The mean cross entropy of n rows is grad_logprob = -1 / n.  `grad_logits` may be `logits` (same pointer and stride). */
+typedef struct tcbnn_logprobs_grad_desc {
+    const void* logits;         /* [rows][classes]           */
+    const int32_t* targets;     /* [rows]; NULL where grad_logprob is */
+    const float* logsumexp;     /* [rows]                    */
+    const float* entropy;       /* [rows]; NULL where grad_entropy is */
+    const float* grad_logprob;  /* [rows], or NULL           */
+    const float* grad_entropy;  /* [rows], or NULL           */
+    void* grad_logits;          /* [rows][classes]           */
+    int rows, classes;
+    int dtype;
+    long long logits_ld, grad_logits_ld;
+} tcbnn_logprobs_grad_desc;
+int tcbnn_logprobs_backward(const tcbnn_logprobs_grad_desc* d, void* stream);
+
 /* ------------------------------------------------ standalone GEMM / conv */
 /* C[m][n] = K - 2*popc(A[m,:] xor B[n,:]), int32 row major [M][N].  A: [K/32][M]
  * (tcbnn_pack_rows output), B: [N][K/32] (tcbnn_pack_cols output: each column of the

@@ -82,6 +82,50 @@ class AvgPoolFcDesc(C.Structure):
                 ("out_features", c_int), ("residual_format", c_int)]
 
 
+class LinearDesc(C.Structure):
+    _fields_ = [("input", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("residual", c_void_p),
+                ("output", c_void_p), ("preact", c_void_p), ("rows", c_int), ("in_features", c_int),
+                ("out_features", c_int), ("dtype", c_int), ("activation", c_int), ("input_ld", C.c_longlong),
+                ("weight_ld", C.c_longlong), ("residual_ld", C.c_longlong), ("output_ld", C.c_longlong),
+                ("preact_ld", C.c_longlong), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class LinearGradDesc(C.Structure):
+    _fields_ = [("input", c_void_p), ("weight", c_void_p), ("preact", c_void_p), ("grad_output", c_void_p),
+                ("grad_input", c_void_p), ("grad_weight", c_void_p), ("grad_bias", c_void_p), ("rows", c_int),
+                ("in_features", c_int), ("out_features", c_int), ("dtype", c_int), ("activation", c_int),
+                ("input_ld", C.c_longlong), ("weight_ld", C.c_longlong), ("preact_ld", C.c_longlong),
+                ("grad_output_ld", C.c_longlong), ("grad_input_ld", C.c_longlong), ("grad_weight_ld", C.c_longlong),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class LayerNormDesc(C.Structure):
+    _fields_ = [("input", c_void_p), ("gamma", c_void_p), ("beta", c_void_p), ("output", c_void_p),
+                ("mean", c_void_p), ("rstd", c_void_p), ("rows", c_int), ("features", c_int), ("dtype", c_int),
+                ("eps", C.c_float), ("input_ld", C.c_longlong), ("output_ld", C.c_longlong)]
+
+
+class LayerNormGradDesc(C.Structure):
+    _fields_ = [("input", c_void_p), ("gamma", c_void_p), ("mean", c_void_p), ("rstd", c_void_p),
+                ("grad_output", c_void_p), ("grad_input", c_void_p), ("grad_gamma", c_void_p),
+                ("grad_beta", c_void_p), ("rows", c_int), ("features", c_int), ("dtype", c_int),
+                ("input_ld", C.c_longlong), ("grad_output_ld", C.c_longlong), ("grad_input_ld", C.c_longlong),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class LogProbsDesc(C.Structure):
+    _fields_ = [("logits", c_void_p), ("targets", c_void_p), ("logprob", c_void_p), ("entropy", c_void_p),
+                ("logsumexp", c_void_p), ("rank", c_void_p), ("top_index", c_void_p), ("top_logprob", c_void_p),
+                ("rows", c_int), ("classes", c_int), ("top", c_int), ("dtype", c_int), ("logits_ld", C.c_longlong),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class LogProbsGradDesc(C.Structure):
+    _fields_ = [("logits", c_void_p), ("targets", c_void_p), ("logsumexp", c_void_p), ("entropy", c_void_p),
+                ("grad_logprob", c_void_p), ("grad_entropy", c_void_p), ("grad_logits", c_void_p), ("rows", c_int),
+                ("classes", c_int), ("dtype", c_int), ("logits_ld", C.c_longlong), ("grad_logits_ld", C.c_longlong)]
+
+
 # name -> (restype, argtypes); the complete list of symbols include/tcbnn_hip.h declares.
 ABI = {
     "tcbnn_abi_version": (c_int, []),
@@ -132,6 +176,16 @@ ABI = {
     "tcbnn_out128_kernel_name": (c_int, [C.POINTER(Out128Desc), C.c_char_p, c_size_t]),
     "tcbnn_inconv128_kernel_name": (c_int, [C.POINTER(InConv128Desc), C.c_char_p, c_size_t]),
     "tcbnn_shader_clock_probe": (c_int, [c_void_p, c_int, C.POINTER(c_int), c_void_p]),
+    "tcbnn_linear_workspace_bytes": (c_size_t, [c_int] * 4),
+    "tcbnn_linear_forward": (c_int, [C.POINTER(LinearDesc), c_void_p]),
+    "tcbnn_linear_grad_workspace_bytes": (c_size_t, [c_int] * 4),
+    "tcbnn_linear_backward": (c_int, [C.POINTER(LinearGradDesc), c_void_p]),
+    "tcbnn_layernorm_forward": (c_int, [C.POINTER(LayerNormDesc), c_void_p]),
+    "tcbnn_layernorm_grad_workspace_bytes": (c_size_t, [c_int] * 2),
+    "tcbnn_layernorm_backward": (c_int, [C.POINTER(LayerNormGradDesc), c_void_p]),
+    "tcbnn_logprobs_workspace_bytes": (c_size_t, [c_int] * 4),
+    "tcbnn_logprobs_forward": (c_int, [C.POINTER(LogProbsDesc), c_void_p]),
+    "tcbnn_logprobs_backward": (c_int, [C.POINTER(LogProbsGradDesc), c_void_p]),
     "tcbnn_bmm": (c_int, [c_void_p] * 3 + [c_int] * 4 + [c_void_p]),
     "tcbnn_bconv": (c_int, [c_void_p] * 3 + [c_int] * 14 + [c_void_p]),
     "tcbnn_unpack_fc_output": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
@@ -153,6 +207,8 @@ VARIANT_AUTO, VARIANT_POPC, VARIANT_MFMA_I8, VARIANT_MFMA_F4 = 0, 1, 2, 3
 VARIANTS = {"auto": 0, "popc": 1, "mfma_i8": 2, "mfma_f4": 3}
 RES_I32, RES_I16, RES_I12 = 0, 1, 2
 INCONV_INPUT_NCHW, INCONV_INPUT_PACKED = 0, 1
+DTYPES = {"f32": 0, "bf16": 1, "f16": 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 INT32_MAX = 2 ** 31 - 1
 
 

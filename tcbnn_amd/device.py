@@ -59,6 +59,27 @@ class DeviceBuffer:
             pass
 
 
+class DeviceView:
+    """Device memory that something else owns, as a layer's input or output: `nbytes` at `ptr`, rows of a matrix `ld`
+    elements apart (0: without gaps).  `owner` is kept alive with the view; free() leaves the memory alone."""
+
+    def __init__(self, ptr, nbytes, ld=0, owner=None):
+        self.ptr, self.nbytes, self.ld, self.owner = ptr, int(nbytes), int(ld), owner
+
+    @classmethod
+    def of(cls, tensor):
+        """A torch tensor of one or two dimensions whose rows are contiguous."""
+        if tensor.dim() > 2 or (tensor.shape[-1] > 1 and tensor.stride(-1) != 1):
+            raise _lib.TcbnnError("a layer takes vectors and matrices with contiguous rows")
+        ld = tensor.stride(0) if tensor.dim() == 2 and tensor.shape[0] > 1 else 0
+        return cls(tensor.data_ptr(), tensor.numel() * tensor.element_size(), ld, tensor)
+
+    to_numpy = DeviceBuffer.to_numpy
+
+    def free(self):
+        self.ptr = self.owner = None
+
+
 class PinnedBuffer:
     """Owning handle on pinned host memory."""
 

@@ -1,0 +1,268 @@
+"""The floating point end of a network: linear layers, layer norms and log probabilities, forward and backward.
+
+The layers are objects like those of layers.py: a constructor with the sizes, `initialize` with parameters and buffers,
+`forward(stream)` and `backward(stream)` as stream-ordered launches that allocate nothing, `download_*` and `release`.
+Buffers are DeviceBuffer or DeviceView (memory of another library, with a stride between rows); a parameter may also be
+a numpy array, which is uploaded in the layer's type.  What is not given and not asked for is not computed.
+All compute goes through the C ABI of libtcbnn_hip.so.  The reference has no counterpart.
+"""
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+from ._lib import check, lib
+from .device import DeviceBuffer
+from .layers import _stream_handle
+
+
+def encode(values, dtype):
+    """fp32 values in the bits of `dtype` ("f32", "bf16", "f16"), rounded to nearest even."""
+    x = np.ascontiguousarray(values, dtype=np.float32)
+    if dtype == "f32":
+        return x
+    if dtype == "f16":
+        return x.astype(np.float16)
+    u = x.view(np.uint32).astype(np.uint64)
+    bits = ((u + 0x7fff + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(x), np.uint16(0x7fc0), bits)
+
+
+def decode(bits, dtype):
+    """What encode() made, as fp32."""
+    if dtype == "bf16":
+        return (bits.astype(np.uint32) << 16).view(np.float32)
+    return bits.astype(np.float32)
+
+
+def storage(dtype):
+    """The numpy type that holds `dtype`."""
+    return {"f32": np.float32, "bf16": np.uint16, "f16": np.float16}[dtype]
+
+
+def _ptr(buf):
+    return None if buf is None else buf.ptr
+
+
+def _ld(buf):
+    return getattr(buf, "ld", 0)
+
+
+class _HeadLayer:
+    def __init__(self, name, dtype):
+        if dtype not in _lib.DTYPES:
+            raise _lib.TcbnnError("Error: %s: unknown dtype %r" % (name, dtype))
+        self.name, self.dtype = name, dtype
+        self._owned = []
+        self._desc = self._grad_desc = None
+
+    def _itemsize(self):
+        return 4 if self.dtype == "f32" else 2
+
+    def _buffer(self, nbytes):
+        buf = DeviceBuffer(nbytes)
+        self._owned.append(buf)
+        return buf
+
+    def _parameter(self, p, dtype, shape):
+        """A parameter's device buffer: what the caller holds, or an upload of a host array."""
+        if p is None or hasattr(p, "ptr"):
+            return p
+        buf = DeviceBuffer.from_numpy(encode(np.asarray(p, np.float32).reshape(shape), dtype))
+        self._owned.append(buf)
+        return buf
+
+    def _sized(self, buf, what, count, itemsize):
+        if buf is not None and buf.nbytes < count * itemsize:
+            raise _lib.TcbnnError("Error: %s: %s holds %d bytes, %d needed" % (self.name, what, buf.nbytes, count * itemsize))
+        return buf
+
+    def _required(self, buf, what):
+        if buf is None:
+            raise _lib.TcbnnError("Error: NULL pointer (%s: %s)" % (self.name, what))
+        return buf
+
+    def _run(self, entry, desc, stream):
+        if desc is None:
+            raise _lib.TcbnnError("Error: %s: not initialized" % self.name)
+        check(entry(C.byref(desc), _stream_handle(stream)))
+
+    def release(self):
+        for buf in self._owned:
+            buf.free()
+        self._owned = []
+        self._desc = self._grad_desc = None
+
+
+class LinearLayerParam(_HeadLayer):
+    """output = act(input * weight^T + bias) + residual; input [rows][in_features], weight [out_features][in_features]."""
+
+    def __init__(self, name, rows, in_features, out_features, dtype="f32", activation="none"):
+        super().__init__(name, dtype)
+        if activation not in _lib.ACTIVATIONS:
+            raise _lib.TcbnnError("Error: %s: unknown activation %r" % (name, activation))
+        self.rows, self.in_features, self.out_features, self.activation = rows, in_features, out_features, activation
+
+    def initialize(self, weight, bias, input_gpu, residual_gpu=None, output_gpu=None, preact_gpu=None, save_preact=False):
+        """save_preact: keep the values before the activation, which backward() of a layer with one needs, in a buffer of
+        the layer's own (or give `preact_gpu`)."""
+        m, k, n, size = self.rows, self.in_features, self.out_features, self._itemsize()
+        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", m * k, size)
+        self.weight_gpu = self._sized(self._parameter(self._required(weight, "weight"), self.dtype, (n, k)), "weight", n * k, size)
+        self.bias_gpu = self._sized(self._parameter(bias, "f32", (n,)), "bias", n, 4)
+        self.residual_gpu = self._sized(residual_gpu, "residual", m * n, size)
+        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * size), "output", m * n, size)
+        if preact_gpu is None and save_preact:
+            preact_gpu = self._buffer(m * n * size)
+        self.preact_gpu = self._sized(preact_gpu, "preact", m * n, size)
+        nbytes = lib.tcbnn_linear_workspace_bytes(m, k, n, _lib.DTYPES[self.dtype])
+        ws = self._buffer(nbytes) if nbytes else None
+        self._desc = _lib.LinearDesc(
+            self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), _ptr(self.residual_gpu), self.output_gpu.ptr,
+            _ptr(self.preact_gpu), m, k, n, _lib.DTYPES[self.dtype], _lib.ACTIVATIONS[self.activation], _ld(self.input_gpu),
+            _ld(self.weight_gpu), _ld(self.residual_gpu), _ld(self.output_gpu), _ld(self.preact_gpu), _ptr(ws), nbytes)
+        return self
+
+    def initialize_backward(self, grad_output_gpu, grad_input_gpu=None, grad_weight_gpu=None, grad_bias_gpu=None):
+        """After initialize().  Gradients are written where a buffer is given."""
+        m, k, n, size = self.rows, self.in_features, self.out_features, self._itemsize()
+        if self.activation != "none":
+            self._required(self.preact_gpu, "preact")
+        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", m * n, size)
+        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", m * k, size)
+        self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", n * k, size)
+        self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", n, 4)
+        nbytes = lib.tcbnn_linear_grad_workspace_bytes(m, k, n, _lib.DTYPES[self.dtype])
+        ws = self._buffer(nbytes) if nbytes else None
+        self._grad_desc = _lib.LinearGradDesc(
+            self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.preact_gpu), self.grad_output_gpu.ptr, _ptr(grad_input_gpu),
+            _ptr(grad_weight_gpu), _ptr(grad_bias_gpu), m, k, n, _lib.DTYPES[self.dtype], _lib.ACTIVATIONS[self.activation],
+            _ld(self.input_gpu), _ld(self.weight_gpu), _ld(self.preact_gpu), _ld(grad_output_gpu), _ld(grad_input_gpu),
+            _ld(grad_weight_gpu), _ptr(ws), nbytes)
+        return self
+
+    def get_output_gpu(self):
+        return self.output_gpu
+
+    def forward(self, stream=None):
+        self._run(lib.tcbnn_linear_forward, self._desc, stream)
+
+    def backward(self, stream=None):
+        self._run(lib.tcbnn_linear_backward, self._grad_desc, stream)
+
+    def download_output(self):
+        """fp32 [rows][out_features] of a buffer without gaps between rows."""
+        return decode(self.output_gpu.to_numpy(storage(self.dtype), (self.rows, self.out_features)), self.dtype)
+
+
+class LayerNormLayerParam(_HeadLayer):
+    """output = (input - mean) / sqrt(variance + eps) * gamma + beta over the features of each row."""
+
+    def __init__(self, name, rows, features, dtype="f32", eps=1e-5):
+        super().__init__(name, dtype)
+        self.rows, self.features, self.eps = rows, features, eps
+
+    def initialize(self, gamma, beta, input_gpu, output_gpu=None, mean_gpu=None, rstd_gpu=None):
+        m, n, size = self.rows, self.features, self._itemsize()
+        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", m * n, size)
+        self.gamma_gpu = self._sized(self._parameter(gamma, "f32", (n,)), "gamma", n, 4)
+        self.beta_gpu = self._sized(self._parameter(beta, "f32", (n,)), "beta", n, 4)
+        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * size), "output", m * n, size)
+        self.mean_gpu = self._sized(mean_gpu if mean_gpu is not None else self._buffer(4 * m), "mean", m, 4)
+        self.rstd_gpu = self._sized(rstd_gpu if rstd_gpu is not None else self._buffer(4 * m), "rstd", m, 4)
+        self._desc = _lib.LayerNormDesc(
+            self.input_gpu.ptr, _ptr(self.gamma_gpu), _ptr(self.beta_gpu), self.output_gpu.ptr, self.mean_gpu.ptr, self.rstd_gpu.ptr,
+            m, n, _lib.DTYPES[self.dtype], self.eps, _ld(self.input_gpu), _ld(self.output_gpu))
+        return self
+
+    def initialize_backward(self, grad_output_gpu, grad_input_gpu=None, grad_gamma_gpu=None, grad_beta_gpu=None):
+        """After initialize().  Gradients are written where a buffer is given; mean and rstd are those of forward()."""
+        m, n, size = self.rows, self.features, self._itemsize()
+        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", m * n, size)
+        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", m * n, size)
+        self.grad_gamma_gpu = self._sized(grad_gamma_gpu, "grad_gamma", n, 4)
+        self.grad_beta_gpu = self._sized(grad_beta_gpu, "grad_beta", n, 4)
+        nbytes = lib.tcbnn_layernorm_grad_workspace_bytes(m, n)
+        ws = self._buffer(nbytes) if nbytes else None
+        self._grad_desc = _lib.LayerNormGradDesc(
+            self.input_gpu.ptr, _ptr(self.gamma_gpu), self.mean_gpu.ptr, self.rstd_gpu.ptr, self.grad_output_gpu.ptr,
+            _ptr(grad_input_gpu), _ptr(grad_gamma_gpu), _ptr(grad_beta_gpu), m, n, _lib.DTYPES[self.dtype], _ld(self.input_gpu),
+            _ld(grad_output_gpu), _ld(grad_input_gpu), _ptr(ws), nbytes)
+        return self
+
+    def get_output_gpu(self):
+        return self.output_gpu
+
+    def forward(self, stream=None):
+        self._run(lib.tcbnn_layernorm_forward, self._desc, stream)
+
+    def backward(self, stream=None):
+        self._run(lib.tcbnn_layernorm_backward, self._grad_desc, stream)
+
+    def download_output(self):
+        """fp32 [rows][features] of a buffer without gaps between rows."""
+        return decode(self.output_gpu.to_numpy(storage(self.dtype), (self.rows, self.features)), self.dtype)
+
+
+class LogProbsLayerParam(_HeadLayer):
+    """Of every row of logits: log probability and rank of a given class, entropy, the `top` best classes."""
+
+    def __init__(self, name, rows, classes, top=0, dtype="f32"):
+        super().__init__(name, dtype)
+        self.rows, self.classes, self.top = rows, classes, top
+
+    def initialize(self, logits_gpu, targets_gpu=None, logprob_gpu=None, entropy_gpu=None, logsumexp_gpu=None, rank_gpu=None,
+                   top_index_gpu=None, top_logprob_gpu=None):
+        """Without `targets_gpu` (int32, -1: none) no log probabilities and ranks of given classes are computed."""
+        m, n, k = self.rows, self.classes, self.top
+        self.logits_gpu = self._sized(self._required(logits_gpu, "logits"), "logits", m * n, self._itemsize())
+        self.targets_gpu = self._sized(targets_gpu, "targets", m, 4)
+
+        def out(buf, what, count, wanted=True):
+            return self._sized(buf if buf is not None or not wanted else self._buffer(4 * count), what, count, 4)
+
+        given = targets_gpu is not None
+        self.logprob_gpu = out(logprob_gpu, "logprob", m, given)
+        self.entropy_gpu = out(entropy_gpu, "entropy", m)
+        self.logsumexp_gpu = out(logsumexp_gpu, "logsumexp", m)
+        self.rank_gpu = out(rank_gpu, "rank", m, given)
+        self.top_index_gpu = out(top_index_gpu, "top_index", m * k, k > 0)
+        self.top_logprob_gpu = out(top_logprob_gpu, "top_logprob", m * k, k > 0)
+        nbytes = lib.tcbnn_logprobs_workspace_bytes(m, n, k, _lib.DTYPES[self.dtype])
+        ws = self._buffer(nbytes) if nbytes else None
+        self._desc = _lib.LogProbsDesc(
+            self.logits_gpu.ptr, _ptr(targets_gpu), _ptr(self.logprob_gpu), _ptr(self.entropy_gpu), _ptr(self.logsumexp_gpu),
+            _ptr(self.rank_gpu), _ptr(self.top_index_gpu), _ptr(self.top_logprob_gpu), m, n, k, _lib.DTYPES[self.dtype],
+            _ld(self.logits_gpu), _ptr(ws), nbytes)
+        return self
+
+    def initialize_backward(self, grad_logprob_gpu, grad_entropy_gpu, grad_logits_gpu):
+        """After initialize(); either of the first two may be None.  logsumexp and entropy are those of forward()."""
+        m, n = self.rows, self.classes
+        if grad_logprob_gpu is not None:
+            self._required(self.targets_gpu, "targets")
+        self.grad_logprob_gpu = self._sized(grad_logprob_gpu, "grad_logprob", m, 4)
+        self.grad_entropy_gpu = self._sized(grad_entropy_gpu, "grad_entropy", m, 4)
+        self.grad_logits_gpu = self._sized(self._required(grad_logits_gpu, "grad_logits"), "grad_logits", m * n, self._itemsize())
+        self._grad_desc = _lib.LogProbsGradDesc(
+            self.logits_gpu.ptr, _ptr(self.targets_gpu), self.logsumexp_gpu.ptr, self.entropy_gpu.ptr, _ptr(grad_logprob_gpu),
+            _ptr(grad_entropy_gpu), grad_logits_gpu.ptr, m, n, _lib.DTYPES[self.dtype], _ld(self.logits_gpu), _ld(grad_logits_gpu))
+        return self
+
+    def forward(self, stream=None):
+        self._run(lib.tcbnn_logprobs_forward, self._desc, stream)
+
+    def backward(self, stream=None):
+        self._run(lib.tcbnn_logprobs_backward, self._grad_desc, stream)
+
+    def download_output(self):
+        """dict of the host arrays of what forward() wrote."""
+        m, k = self.rows, self.top
+        out = {"entropy": self.entropy_gpu.to_numpy(np.float32, (m,)), "logsumexp": self.logsumexp_gpu.to_numpy(np.float32, (m,))}
+        if self.targets_gpu is not None:
+            out["logprob"] = self.logprob_gpu.to_numpy(np.float32, (m,))
+            out["rank"] = self.rank_gpu.to_numpy(np.int32, (m,))
+        if k:
+            out["top_index"] = self.top_index_gpu.to_numpy(np.int32, (m, k))
+            out["top_logprob"] = self.top_logprob_gpu.to_numpy(np.float32, (m, k))
+        return out

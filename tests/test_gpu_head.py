@@ -1,0 +1,492 @@
+"""The float head on the GPU against definitions in 64 bits: linear layers, layer norms, log probabilities, and the
+gradient of each; sizes around those where the kernels change, odd sizes, strides, empty and degenerate inputs."""
+import numpy as np
+import pytest
+
+from tests import headops as ho
+
+pytestmark = pytest.mark.gpu
+
+GAPS = {"f32": 1, "bf16": 3, "f16": 5}
+
+
+def rng(*seed):
+    return np.random.default_rng([abs(int(s)) for s in seed])
+
+
+# --------------------------------------------------------------------------- linear
+# (rows, inputs, outputs): one value; one row; the widths of matrix instructions and one to each side; whole and ragged
+# tiles; few rows with long sums; more rows than a tile
+LINEAR = [(1, 1, 1), (1, 16, 10), (1, 4096, 512), (1, 1025, 33), (2, 8, 3), (3, 17, 5), (5, 1032, 264), (7, 33, 1000),
+          (8, 512, 64), (15, 31, 65), (16, 64, 16), (17, 72, 130), (31, 2048, 96), (32, 256, 129), (33, 100, 127),
+          (64, 4096, 48), (65, 65, 65), (77, 1023, 129), (127, 200, 128), (128, 128, 128), (129, 136, 257),
+          (256, 512, 1000), (300, 64, 8), (255, 1000, 511), (513, 96, 300), (1000, 24, 1030)]
+
+
+def _linear(gpu, m, k, n, dtype, activation, bias=True, residual=True, preact=True, gap=0, in_place=False, stream=None):
+    from tcbnn_amd import head
+    r = rng(m, k, n, len(dtype), len(activation))
+    x = ho.Matrix(r.standard_normal((m, k)), dtype, gap)
+    w = ho.Matrix(r.standard_normal((n, k)) / np.sqrt(k), dtype, gap)
+    b = r.standard_normal(n).astype(np.float32) if bias else None
+    res = ho.Matrix(r.standard_normal((m, n)), dtype, gap) if residual else None
+    rv = res.values if residual else 0.0
+    y = res if in_place else ho.Matrix(None, dtype, gap, m, n)
+    z = ho.Matrix(None, dtype, gap, m, n) if preact else None
+    layer = head.LinearLayerParam("linear", m, k, n, dtype, activation)
+    layer.initialize(w.view, b, x.view, residual_gpu=res.view if residual else None, output_gpu=y.view,
+                     preact_gpu=z.view if preact else None)
+    layer.forward(stream)
+    ho.sync()
+    zw = x.values @ w.values.T + (b.astype(np.float64) if bias else 0.0)
+    zerr = (k + 1) * ho.U32 * (np.abs(x.values) @ np.abs(w.values).T + (np.abs(b) if bias else 0.0))
+    if preact:
+        ho.check(z.get(), zw, zerr + ho.U[dtype] * (np.abs(zw) + zerr) + ho.TINY[dtype], "preact")
+    yw = ho.act(activation, zw) + rv
+    # slopes are below 1.13; the activation itself is good to a few units in the last place of its argument
+    yerr = 1.13 * zerr + 8 * ho.U32 * (np.abs(zw) + np.abs(rv))
+    ho.check(y.get(), yw, yerr + ho.U[dtype] * (np.abs(yw) + yerr) + ho.TINY[dtype], "output")
+    layer.release()
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n", LINEAR)
+def test_linear(gpu, m, k, n, dtype):
+    _linear(gpu, m, k, n, dtype, ["none", "relu", "gelu", "silu"][(m + k + n) % 4])
+
+
+@pytest.mark.parametrize("activation", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("m,k,n", [(2, 40, 24), (33, 129, 65), (200, 264, 136)])
+def test_linear_epilogues(gpu, m, k, n, activation):
+    for dtype in ho.DTYPES:
+        for bias, residual, preact in [(False, False, False), (True, False, True), (False, True, False)]:
+            _linear(gpu, m, k, n, dtype, activation, bias, residual, preact)
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 64, 40), (19, 128, 72), (130, 264, 136), (300, 61, 77)])
+def test_linear_strides_and_output_over_residual(gpu, m, k, n, dtype):
+    _linear(gpu, m, k, n, dtype, "gelu", gap=GAPS[dtype])
+    _linear(gpu, m, k, n, dtype, "silu", gap=8, in_place=True)
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n", [(3, 4096, 24), (140, 96, 136)])
+def test_linear_rows_do_not_mix(gpu, m, k, n, dtype):
+    """A NaN row of the input, an infinite row of the weight: one row and one column of the output, nothing else."""
+    from tcbnn_amd import head
+    r = rng(m, k, n)
+    xv, wv = r.standard_normal((m, k)), r.standard_normal((n, k))
+    xv[1, k - 1] = np.nan
+    wv[2, 0] = np.inf
+    x, w, y = ho.Matrix(xv, dtype), ho.Matrix(wv, dtype), ho.Matrix(None, dtype, 0, m, n)
+    head.LinearLayerParam("linear", m, k, n, dtype).initialize(w.view, None, x.view, output_gpu=y.view).forward()
+    ho.sync()
+    finite = np.isfinite(y.get())
+    want = np.ones((m, n), bool)
+    want[1] = False
+    want[:, 2] = False
+    np.testing.assert_array_equal(finite, want)
+
+
+def _linear_grad(gpu, m, k, n, dtype, activation, gap=0, want=("x", "w", "b")):
+    from tcbnn_amd import head
+    r = rng(m, k, n, len(dtype), len(activation), 1)
+    x = ho.Matrix(r.standard_normal((m, k)), dtype, gap)
+    w = ho.Matrix(r.standard_normal((n, k)) / np.sqrt(k), dtype, gap)
+    z = ho.Matrix(r.standard_normal((m, n)) * 2, dtype, gap)
+    dy = ho.Matrix(r.standard_normal((m, n)), dtype, gap)
+    dx, dw, db = ho.Matrix(None, dtype, gap, m, k), ho.Matrix(None, dtype, gap, n, k), ho.empty(n)
+    layer = head.LinearLayerParam("linear", m, k, n, dtype, activation)
+    layer.initialize(w.view, None, x.view, preact_gpu=z.view if activation != "none" else None)
+    layer.initialize_backward(dy.view, dx.view if "x" in want else None, dw.view if "w" in want else None,
+                              db if "b" in want else None)
+    layer.backward()
+    ho.sync()
+    g = dy.values * ho.slope(activation, z.values)
+    gerr = 8 * ho.U32 * np.abs(dy.values) * (0 if activation == "none" else 1)  # the slope, good to a few units of 1
+    used = gerr + (ho.U[dtype] * (np.abs(g) + gerr) + ho.TINY[dtype] if activation != "none" else 0.0)  # as the products read it
+    if "x" in want:
+        exact, terms = g @ w.values, np.abs(g) @ np.abs(w.values)
+        err = used @ np.abs(w.values) + n * ho.U32 * 1.01 * terms
+        ho.check(dx.get(), exact, err + ho.U[dtype] * (np.abs(exact) + err) + ho.TINY[dtype], "grad_input")
+    if "w" in want:
+        exact, terms = g.T @ x.values, np.abs(g).T @ np.abs(x.values)
+        err = used.T @ np.abs(x.values) + m * ho.U32 * 1.01 * terms
+        ho.check(dw.get(), exact, err + ho.U[dtype] * (np.abs(exact) + err) + ho.TINY[dtype], "grad_weight")
+    if "b" in want:
+        ho.check(db.to_numpy(np.float32, (n,)), g.sum(0), gerr.sum(0) + m * ho.U32 * 1.01 * np.abs(g).sum(0), "grad_bias")
+    layer.release()
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n", LINEAR)
+def test_linear_grad(gpu, m, k, n, dtype):
+    _linear_grad(gpu, m, k, n, dtype, ["none", "relu", "gelu", "silu"][(m + k + n) % 4])
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 64, 40), (19, 130, 72), (130, 264, 136), (700, 61, 77)])
+def test_linear_grad_strides_and_single_outputs(gpu, m, k, n, dtype):
+    _linear_grad(gpu, m, k, n, dtype, "gelu", gap=GAPS[dtype])
+    _linear_grad(gpu, m, k, n, dtype, "none", gap=8)
+    for want in (("x",), ("w",), ("b",), ("w", "b")):
+        _linear_grad(gpu, m, k, n, dtype, "silu", want=want)
+        _linear_grad(gpu, m, k, n, dtype, "none", want=want)
+
+
+def test_linear_without_rows(gpu):
+    from tcbnn_amd import head
+    x, w = ho.Matrix(None, "bf16", 0, 0, 24), ho.Matrix(np.ones((16, 24)), "bf16")
+    y, dw, db = ho.Matrix(None, "bf16", 0, 0, 16), ho.Matrix(None, "bf16", 0, 16, 24), ho.empty(16)
+    layer = head.LinearLayerParam("linear", 0, 24, 16, "bf16", "gelu")
+    layer.initialize(w.view, None, x.view, output_gpu=y.view, save_preact=True)
+    layer.initialize_backward(y.view, x.view, dw.view, db)
+    layer.forward()
+    layer.backward()
+    ho.sync()
+    assert not dw.get().any() and not db.to_numpy(np.float32, (16,)).any()
+
+
+# --------------------------------------------------------------------------- layer norm
+NORM = [(1, 1), (3, 2), (5, 7), (70, 64), (4, 100), (300, 128), (2, 512), (9, 513), (33, 1000), (65, 1023), (3, 1024),
+        (1, 4096), (17, 4097), (3, 8192), (2, 8195), (5, 16384), (2, 20001), (1, 65536)]
+EPS = 1e-5
+
+
+def _norm_inputs(m, n, dtype, gap, offset=0.5):
+    r = rng(m, n, len(dtype))
+    x = ho.Matrix(2.0 * r.standard_normal((m, n)) + offset, dtype, gap)
+    gamma, beta = (1 + 0.2 * r.standard_normal(n)).astype(np.float32), r.standard_normal(n).astype(np.float32)
+    return r, x, gamma, beta
+
+
+def _check_norm(x, gamma, beta, y, mean, rstd, dtype):
+    n = x.shape[1]
+    yw, mw, rw = ho.norm(x, gamma, beta, EPS)
+    # sums of n terms over at least 64 lanes: n / 64 terms in a row at most, and the steps that join the lanes
+    depth = n / 64 + 24
+    merr = depth * ho.U32 * np.abs(x).mean(1)
+    ho.check(mean, mw, merr, "mean")
+    # the variance's own relative error, and what the mean's adds (its square, and nothing in first order)
+    verr = (2 * depth + 6) * ho.U32 + (merr * rw) ** 2
+    ho.check(rstd, rw, rw * (0.5 * verr + 4 * ho.U32), "rstd")
+    xh = (x - mw[:, None]) * rw[:, None]
+    err = (np.abs(gamma) * (np.abs(xh) * (0.5 * verr + 8 * ho.U32)[:, None] + ((merr + ho.U32 * np.abs(x).max(1)) * rw)[:, None])
+           + 2 * ho.U32 * np.abs(yw))
+    ho.check(y, yw, err + ho.U[dtype] * (np.abs(yw) + err) + ho.TINY[dtype], "output")
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,n", NORM)
+def test_layernorm(gpu, m, n, dtype):
+    from tcbnn_amd import head
+    for gap in (0, GAPS[dtype], 8):
+        r, x, gamma, beta = _norm_inputs(m, n, dtype, gap)
+        y = ho.Matrix(None, dtype, gap, m, n)
+        layer = head.LayerNormLayerParam("norm", m, n, dtype, EPS).initialize(gamma, beta, x.view, output_gpu=y.view)
+        layer.forward()
+        ho.sync()
+        _check_norm(x.values, gamma.astype(np.float64), beta.astype(np.float64), y.get(), layer.mean_gpu.to_numpy(np.float32, (m,)),
+                    layer.rstd_gpu.to_numpy(np.float32, (m,)), dtype)
+        layer.release()
+
+
+@pytest.mark.parametrize("n", [64, 1000, 5000])
+def test_layernorm_far_from_zero_and_in_place(gpu, n):
+    """A variance that is small beside the mean's square, as only sums about the mean hold it; output over input; no
+    parameters; a row of equal values."""
+    from tcbnn_amd import head
+    m = 6
+    r = rng(n)
+    v = 1000.0 + r.standard_normal((m, n))
+    v[2] = 3.0
+    x = ho.Matrix(v, "f32")
+    layer = head.LayerNormLayerParam("norm", m, n, "f32", EPS).initialize(None, None, x.view, output_gpu=x.view)
+    layer.forward()
+    ho.sync()
+    _check_norm(x.values, np.ones(n), np.zeros(n), x.get(), layer.mean_gpu.to_numpy(np.float32, (m,)),
+                layer.rstd_gpu.to_numpy(np.float32, (m,)), "f32")
+
+
+def _norm_grad(m, n, dtype, gap=0, want=("x", "g", "b"), in_place=False, affine=True):
+    from tcbnn_amd import head
+    r, x, gamma, _ = _norm_inputs(m, n, dtype, gap)
+    if not affine:
+        gamma = None
+    gv = gamma.astype(np.float64) if affine else np.ones(n)
+    dy = ho.Matrix(r.standard_normal((m, n)), dtype, gap)
+    dyv = dy.values
+    _, mean, rstd = ho.norm(x.values, 1.0, 0.0, EPS)
+    mean, rstd = mean.astype(np.float32), rstd.astype(np.float32)
+    dx, dg, db = dy if in_place else ho.Matrix(None, dtype, gap, m, n), ho.empty(n), ho.empty(n)
+    layer = head.LayerNormLayerParam("norm", m, n, dtype, EPS)
+    layer.initialize(gamma, None, x.view, mean_gpu=ho.vector(mean), rstd_gpu=ho.vector(rstd))
+    layer.initialize_backward(dy.view, dx.view if "x" in want else None, dg if "g" in want else None, db if "b" in want else None)
+    layer.backward()
+    ho.sync()
+    mean, rstd = mean.astype(np.float64)[:, None], rstd.astype(np.float64)[:, None]
+    xh, g = (x.values - mean) * rstd, dyv * gv
+    xerr = 3 * ho.U32 * np.abs(xh) + ho.U32 * np.abs(x.values) * rstd
+    if "x" in want:
+        mg, mgx = g.mean(1, keepdims=True), (g * xh).mean(1, keepdims=True)
+        exact = (g - mg - xh * mgx) * rstd
+        depth = (n / 64 + 24) * ho.U32
+        e1 = depth * np.abs(g).mean(1, keepdims=True)
+        e2 = depth * np.abs(g * xh).mean(1, keepdims=True) + (np.abs(g) * xerr).mean(1, keepdims=True)
+        err = rstd * (e1 + np.abs(xh) * e2 + xerr * np.abs(mgx) + 6 * ho.U32 * (np.abs(g) + np.abs(mg) + np.abs(xh * mgx)))
+        ho.check(dx.get(), exact, err + ho.U[dtype] * (np.abs(exact) + err) + ho.TINY[dtype], "grad_input")
+    if "g" in want:
+        err = (m + 2) * ho.U32 * np.abs(dyv * xh).sum(0) + (np.abs(dyv) * xerr).sum(0)
+        ho.check(dg.to_numpy(np.float32, (n,)), (dyv * xh).sum(0), err, "grad_gamma")
+    if "b" in want:
+        ho.check(db.to_numpy(np.float32, (n,)), dyv.sum(0), m * ho.U32 * np.abs(dyv).sum(0), "grad_beta")
+    layer.release()
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,n", NORM + [(2000, 24), (3001, 130), (600, 1000)])
+def test_layernorm_grad(gpu, m, n, dtype):
+    _norm_grad(m, n, dtype)
+    _norm_grad(m, n, dtype, GAPS[dtype], affine=False)
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,n", [(5, 72), (130, 1001)])
+def test_layernorm_grad_single_outputs_and_in_place(gpu, m, n, dtype):
+    for want in (("x",), ("g",), ("b",), ("x", "b")):
+        _norm_grad(m, n, dtype, want=want)
+    _norm_grad(m, n, dtype, 8, in_place=True)
+
+
+def test_layernorm_without_rows(gpu):
+    from tcbnn_amd import head
+    x, dg, db, one = ho.Matrix(None, "f32", 0, 0, 40), ho.empty(40), ho.empty(40), ho.empty(1)
+    layer = head.LayerNormLayerParam("norm", 0, 40).initialize(None, None, x.view, output_gpu=x.view, mean_gpu=one, rstd_gpu=one)
+    layer.initialize_backward(x.view, x.view, dg, db)
+    layer.forward()
+    layer.backward()
+    ho.sync()
+    assert not dg.to_numpy(np.float32, (40,)).any() and not db.to_numpy(np.float32, (40,)).any()
+
+
+# --------------------------------------------------------------------------- log probabilities
+# (rows, classes, top): one class; around a wavefront, a workgroup's share and several of them; few rows of many classes
+# and many rows of few
+LOGPROBS = [(3, 1, 1), (5, 2, 2), (700, 10, 5), (9, 63, 5), (4, 64, 64), (7, 65, 20), (33, 257, 8), (256, 1000, 5), (3, 1025, 32),
+            (2, 4095, 64), (5, 4097, 0), (2, 8192, 5), (3, 16385, 20), (1, 32003, 20), (2, 50257, 1), (1, 131072, 20),
+            (300, 2050, 3), (1, 262147, 64)]
+
+
+def _logits(r, m, n, kind):
+    x = 3.0 * r.standard_normal((m, n))
+    if kind == "ties":
+        x = np.round(x * 2) / 2
+    elif kind == "equal":
+        x[:] = np.round(x[:, :1], 1)
+    elif kind == "sorted":
+        x = np.sort(x, 1)
+        x[::2] = x[::2, ::-1]
+    elif kind == "cluster":  # the best classes lie side by side
+        x[:, n // 3:n // 3 + 80] += 30.0
+    elif kind == "stride":  # ... or a power of two apart
+        x[:, ::64] += 30.0
+    elif kind == "masked":
+        x[r.random((m, n)) < 0.5] = -np.inf
+        x[0] = -np.inf
+        x[-1] = -np.inf
+        x[-1, n // 2] = 0.25
+    elif kind == "lowest":  # masks of the type's lowest value
+        low = np.finfo(np.float16).min
+        x[r.random((m, n)) < 0.7] = low
+        x[0] = low
+    elif kind == "special":
+        x[0, n // 2] = np.nan
+        x[m // 2, n - 1] = np.inf
+        x[-1, 0] = -0.0
+        x[-1, n - 1] = 0.0
+    return x
+
+
+def _logprobs(m, n, top, dtype, kind="plain", gap=0, stream=None):
+    from tcbnn_amd import head
+    r = rng(m, n, top, len(kind))
+    x = ho.Matrix(_logits(r, m, n, kind), dtype, gap)
+    t = r.integers(0, n, m).astype(np.int32)
+    t[::5] = x.values[::5].argmax(1)
+    t[3::7] = -1
+    t[4::50] = n + 3
+    layer = head.LogProbsLayerParam("logprobs", m, n, top, dtype).initialize(x.view, ho.vector(t, np.int32))
+    layer.forward(stream)
+    ho.sync()
+    got = layer.download_output()
+    xs = x.values
+    want = [ho.logprobs(xs[i], int(t[i]), top) for i in range(m)]
+    np.testing.assert_array_equal(got["rank"], [w[3] for w in want])
+    if top:
+        np.testing.assert_array_equal(got["top_index"], np.stack([w[4] for w in want]))
+    # exp is good to 2 units of its result and 1.5 of its argument, terms of large arguments being small: |d| exp(d) < 0.4;
+    # sums over at least 64 lanes; the logarithm, and roundings of the size of the largest logit
+    big = np.array([np.abs(row[np.isfinite(row)]).max(initial=0.0) if row.max() < 100 else 0.0 for row in xs])
+    depth = n / 64 + 24
+    with np.errstate(invalid="ignore"):
+        m_ = np.array([row.max() for row in xs])
+    top_size = np.where(np.isfinite(m_), np.abs(np.where(np.isfinite(m_), m_, 0)), 0)
+    lerr = (depth + 8) * ho.U32 + 4 * ho.U32 * (top_size + np.log(n) + 1)
+    ho.check(got["logsumexp"], [w[2] for w in want], lerr, "logsumexp")
+    lp = np.array([w[0] for w in want])
+    ho.check(got["logprob"], lp, lerr + 2 * ho.U32 * (np.abs(np.where(np.isfinite(lp), lp, 0)) + top_size), "logprob")
+    ent = np.array([w[1] for w in want])
+    eerr = (2 * depth + 24) * ho.U32 * (np.log(n) + 2 + np.where(np.isfinite(ent), ent, 0))
+    ho.check(got["entropy"], ent, eerr, "entropy")
+    if top:
+        lp = np.stack([w[5] for w in want])
+        ho.check(got["top_logprob"], lp, lerr[:, None] + 2 * ho.U32 * (np.abs(np.where(np.isfinite(lp), lp, 0)) + top_size[:, None]),
+                 "top_logprob")
+    layer.release()
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,n,top", LOGPROBS)
+def test_logprobs(gpu, m, n, top, dtype):
+    _logprobs(m, n, top, dtype)
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("kind", ["ties", "equal", "sorted", "cluster", "stride", "masked", "lowest", "special"])
+@pytest.mark.parametrize("m,n,top", [(4, 100, 64), (3, 1000, 20), (2, 4099, 64), (3, 33001, 33), (2, 140000, 64)])
+def test_logprobs_of_rows_that_are_hard_to_rank(gpu, m, n, top, kind, dtype):
+    _logprobs(m, n, top, dtype, kind, gap=GAPS[dtype] if n % 2 else 8)
+
+
+def test_logprobs_outputs_are_optional(gpu):
+    """What is not asked for is not needed: entropy alone, the best classes alone."""
+    import ctypes as C
+    from tcbnn_amd import _lib
+    r = rng(5)
+    x = ho.Matrix(r.standard_normal((4, 300)), "f32")
+    want = [ho.logprobs(v, -1, 3) for v in x.values]
+    entropy, index = ho.empty(4), ho.empty(12, np.int32)
+    ws_bytes = _lib.lib.tcbnn_logprobs_workspace_bytes(4, 300, 3, 0)
+    ws = ho.DeviceBuffer(ws_bytes)
+    d = _lib.LogProbsDesc(logits=x.view.ptr, entropy=entropy.ptr, rows=4, classes=300, dtype=0, workspace=ws.ptr,
+                          workspace_bytes=ws_bytes)
+    _lib.check(_lib.lib.tcbnn_logprobs_forward(C.byref(d), None))
+    d = _lib.LogProbsDesc(logits=x.view.ptr, top_index=index.ptr, rows=4, classes=300, top=3, dtype=0, workspace=ws.ptr,
+                          workspace_bytes=ws_bytes)
+    _lib.check(_lib.lib.tcbnn_logprobs_forward(C.byref(d), None))
+    ho.sync()
+    ho.check(entropy.to_numpy(np.float32, (4,)), [w[1] for w in want], 1e-5)
+    np.testing.assert_array_equal(index.to_numpy(np.int32, (4, 3)), np.stack([w[4] for w in want]))
+
+
+def _logprobs_grad(m, n, dtype, kind="plain", gap=0, entropy=True, logprob=True, in_place=False):
+    from tcbnn_amd import head
+    r = rng(m, n, len(kind), 2)
+    x = ho.Matrix(_logits(r, m, n, kind), dtype, gap)
+    xs = x.values
+    t = r.integers(0, n, m).astype(np.int32)
+    t[3::7] = -1
+    t[4::50] = n
+    with np.errstate(invalid="ignore", divide="ignore"):
+        rows = [ho.logprobs(v, -1, 0) for v in xs]
+    lse, ent = np.array([w[2] for w in rows], np.float32), np.array([w[1] for w in rows], np.float32)
+    g, ge = r.standard_normal(m).astype(np.float32), r.standard_normal(m).astype(np.float32)
+    dx = x if in_place else ho.Matrix(None, dtype, gap, m, n)
+    layer = head.LogProbsLayerParam("logprobs", m, n, 0, dtype)
+    layer.initialize(x.view, ho.vector(t, np.int32), logsumexp_gpu=ho.vector(lse), entropy_gpu=ho.vector(ent))
+    layer.initialize_backward(ho.vector(g) if logprob else None, ho.vector(ge) if entropy else None, dx.view)
+    layer.backward()
+    ho.sync()
+    got = dx.get()
+    for i in range(m):
+        gi = 0.0 if not logprob or t[i] < 0 else (np.nan if t[i] >= n else float(g[i]))
+        gei = float(ge[i]) if entropy else 0.0
+        if lse[i] == -np.inf:
+            want, err = np.full(n, np.nan if np.isnan(gi) else 0.0), 0.0
+        else:
+            with np.errstate(invalid="ignore"):
+                lp = xs[i] - np.float64(lse[i])
+                p = np.exp(lp)
+                hot = np.zeros(n)
+                if 0 <= t[i] < n:
+                    hot[t[i]] = 1.0
+                l0 = np.where(p > 0, lp, 0.0)
+                want = gi * (hot - p) - gei * p * (l0 + ent[i])
+                # exp: a rounding of its argument's size, and its own
+                perr = p * ho.U32 * (4 + 3 * np.abs(l0) + 2 * np.abs(lse[i]))
+                err = (abs(gi) * (perr + 3 * ho.U32 * (hot + p)) + abs(gei) * (perr * np.abs(l0 + ent[i])
+                       + p * ho.U32 * (6 * np.abs(l0) + 4 * abs(ent[i]) + 2 * np.abs(lse[i]))))
+        with np.errstate(invalid="ignore"):
+            tol = err + ho.U[dtype] * (np.abs(want) + err) + ho.TINY[dtype]
+        ho.check(got[i], want, tol, "row %d" % i)
+    layer.release()
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,n", [(3, 1), (60, 10), (9, 64), (5, 1000), (3, 1025), (2, 4097), (2, 32003), (1, 131072)])
+def test_logprobs_grad(gpu, m, n, dtype):
+    _logprobs_grad(m, n, dtype)
+    _logprobs_grad(m, n, dtype, gap=GAPS[dtype], entropy=False)
+    _logprobs_grad(m, n, dtype, gap=8, logprob=False)
+    _logprobs_grad(m, n, dtype, in_place=True)
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("kind", ["equal", "masked", "lowest", "special"])
+@pytest.mark.parametrize("m,n", [(4, 100), (3, 2051)])
+def test_logprobs_grad_of_special_rows(gpu, m, n, kind, dtype):
+    _logprobs_grad(m, n, dtype, kind)
+
+
+# --------------------------------------------------------------------------- gradients against differences
+def _slope_along(f, x, v):
+    h = 1e-5
+    return (f(x + h * v) - f(x - h * v)) / (2 * h)
+
+
+def test_gradients_against_differences(gpu):
+    """Norm -> linear (GELU, residual) -> log probabilities in fp32 on the GPU, forward and backward through the layers,
+    against central differences of the definition in 64 bits along random directions."""
+    from tcbnn_amd import head
+    m, k, n = 21, 40, 30
+    r = rng(11)
+    x, wt = r.standard_normal((m, k)), r.standard_normal((n, k)) / np.sqrt(k)
+    gamma, beta, b = 1 + 0.1 * r.standard_normal(k), 0.1 * r.standard_normal(k), 0.1 * r.standard_normal(n)
+    res = r.standard_normal((m, n))
+    t = r.integers(0, n, m).astype(np.int32)
+    g, ge = r.standard_normal(m), r.standard_normal(m)
+    x, wt, gamma, beta, b, res, g, ge = (a.astype(np.float32).astype(np.float64) for a in (x, wt, gamma, beta, b, res, g, ge))
+
+    def loss(x, gamma, beta, wt, b, res):
+        y, _, _ = ho.norm(x, gamma, beta, EPS)
+        z = ho.act("gelu", y @ wt.T + b) + res
+        rows = [ho.logprobs(z[i], int(t[i]), 0) for i in range(m)]
+        return sum(g[i] * rows[i][0] + ge[i] * rows[i][1] for i in range(m))
+
+    mx = {name: ho.Matrix(a, "f32") for name, a in dict(x=x, w=wt, res=res).items()}
+    out = {name: ho.Matrix(None, "f32", 0, *s) for name, s in dict(y=(m, k), z=(m, n), dz=(m, n), dy=(m, k), dx=(m, k), dw=(n, k)).items()}
+    vec = {name: ho.empty(s) for name, s in dict(dgamma=k, dbeta=k, db=n).items()}
+    norm = head.LayerNormLayerParam("norm", m, k).initialize(gamma, beta, mx["x"].view, output_gpu=out["y"].view)
+    lin = head.LinearLayerParam("linear", m, k, n, activation="gelu").initialize(
+        mx["w"].view, b, out["y"].view, residual_gpu=mx["res"].view, output_gpu=out["z"].view, save_preact=True)
+    lps = head.LogProbsLayerParam("logprobs", m, n).initialize(out["z"].view, ho.vector(t, np.int32))
+    lps.initialize_backward(ho.vector(g), ho.vector(ge), out["dz"].view)
+    lin.initialize_backward(out["dz"].view, out["dy"].view, out["dw"].view, vec["db"])
+    norm.initialize_backward(out["dy"].view, out["dx"].view, vec["dgamma"], vec["dbeta"])
+    for layer in (norm, lin, lps):
+        layer.forward()
+    for layer in (lps, lin, norm):
+        layer.backward()
+    ho.sync()
+    args = dict(x=x, gamma=gamma, beta=beta, wt=wt, b=b, res=res)
+    grads = dict(x=out["dx"].get(), gamma=vec["dgamma"].to_numpy(np.float32, (k,)), beta=vec["dbeta"].to_numpy(np.float32, (k,)),
+                 wt=out["dw"].get(), b=vec["db"].to_numpy(np.float32, (n,)), res=out["dz"].get())
+    for name, grad in grads.items():
+        for _ in range(3):
+            v = r.standard_normal(args[name].shape)
+            want = _slope_along(lambda a: loss(**{**args, name: a}), args[name], v)
+            # a few hundred fp32 roundings of terms of the gradient's own size
+            assert abs((grad * v).sum() - want) <= 200 * ho.U32 * np.abs(grad * v).sum() + 1e-6, name
+    for layer in (norm, lin, lps):
+        layer.release()

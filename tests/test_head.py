@@ -1,0 +1,187 @@
+"""The float head without a GPU: what its entry points refuse (nothing is launched), what its layers refuse, the rounding of
+parameters, and the definitions that the GPU tests compare with, against differences."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from tests import headops as ho
+
+EINVAL, ENULL = -1, -2
+P = 0x1000  # a pointer that no refused call follows
+
+
+def _lib():
+    from tcbnn_amd import _lib
+    return _lib
+
+
+def _linear(**kw):
+    d = dict(input=P, weight=P, output=P, rows=4, in_features=8, out_features=8, dtype=1, activation=0)
+    return "tcbnn_linear_forward", _lib().LinearDesc(**{**d, **kw})
+
+
+def _linear_grad(**kw):
+    d = dict(input=P, weight=P, preact=P, grad_output=P, grad_input=P, grad_weight=P, grad_bias=P, rows=4, in_features=8,
+             out_features=8, dtype=1, activation=2, workspace=P, workspace_bytes=1 << 30)
+    return "tcbnn_linear_backward", _lib().LinearGradDesc(**{**d, **kw})
+
+
+def _norm(**kw):
+    d = dict(input=P, output=P, rows=4, features=8, dtype=1, eps=1e-5)
+    return "tcbnn_layernorm_forward", _lib().LayerNormDesc(**{**d, **kw})
+
+
+def _norm_grad(**kw):
+    d = dict(input=P, mean=P, rstd=P, grad_output=P, grad_input=P, grad_gamma=P, rows=4, features=8, dtype=1, workspace=P,
+             workspace_bytes=1 << 30)
+    return "tcbnn_layernorm_backward", _lib().LayerNormGradDesc(**{**d, **kw})
+
+
+def _logprobs(**kw):
+    d = dict(logits=P, targets=P, logprob=P, top_index=P, rows=4, classes=80, top=5, dtype=1, workspace=P, workspace_bytes=1 << 30)
+    return "tcbnn_logprobs_forward", _lib().LogProbsDesc(**{**d, **kw})
+
+
+def _logprobs_grad(**kw):
+    d = dict(logits=P, targets=P, logsumexp=P, entropy=P, grad_logprob=P, grad_entropy=P, grad_logits=P, rows=4, classes=80, dtype=1)
+    return "tcbnn_logprobs_backward", _lib().LogProbsGradDesc(**{**d, **kw})
+
+
+@pytest.mark.parametrize("make,change,code,message", [
+    (_linear, dict(dtype=3), EINVAL, "dtype"), (_linear, dict(dtype=-1), EINVAL, "dtype"),
+    (_linear, dict(activation=4), EINVAL, "activation"), (_linear, dict(rows=-1), EINVAL, "shape"),
+    (_linear, dict(in_features=0), EINVAL, "shape"), (_linear, dict(out_features=0), EINVAL, "shape"),
+    (_linear, dict(in_features=(1 << 20) + 1), EINVAL, "inputs"), (_linear, dict(input_ld=7), EINVAL, "overlap"),
+    (_linear, dict(weight_ld=7), EINVAL, "overlap"), (_linear, dict(output_ld=7), EINVAL, "overlap"),
+    (_linear, dict(residual_ld=-8), EINVAL, "overlap"), (_linear, dict(preact_ld=1), EINVAL, "overlap"),
+    (_linear, dict(input=0), ENULL, "input"), (_linear, dict(weight=0), ENULL, "weight"), (_linear, dict(output=0), ENULL, "output"),
+    (_linear, dict(residual=P, residual_ld=16), EINVAL, "stride"),
+    (_linear_grad, dict(dtype=9), EINVAL, "dtype"), (_linear_grad, dict(activation=-1), EINVAL, "activation"),
+    (_linear_grad, dict(rows=-4), EINVAL, "shape"), (_linear_grad, dict(grad_output=0), ENULL, "grad_output"),
+    (_linear_grad, dict(preact=0), ENULL, "preact"), (_linear_grad, dict(input=0), ENULL, "input"),
+    (_linear_grad, dict(weight=0), ENULL, "weight"), (_linear_grad, dict(workspace=0), ENULL, "workspace"),
+    (_linear_grad, dict(workspace_bytes=1), EINVAL, "workspace"), (_linear_grad, dict(grad_weight_ld=4), EINVAL, "overlap"),
+    (_norm, dict(dtype=3), EINVAL, "dtype"), (_norm, dict(features=0), EINVAL, "shape"), (_norm, dict(features=65537), EINVAL, "features"),
+    (_norm, dict(eps=-1.0), EINVAL, "eps"), (_norm, dict(eps=float("nan")), EINVAL, "eps"), (_norm, dict(input=0), ENULL, "input"),
+    (_norm, dict(output=0), ENULL, "output"), (_norm, dict(input_ld=7), EINVAL, "overlap"),
+    (_norm, dict(output_ld=16), EINVAL, "stride"),
+    (_norm_grad, dict(rows=-1), EINVAL, "shape"), (_norm_grad, dict(mean=0), ENULL, "mean"), (_norm_grad, dict(rstd=0), ENULL, "rstd"),
+    (_norm_grad, dict(input=0), ENULL, "input"), (_norm_grad, dict(grad_output=0), ENULL, "grad_output"),
+    (_norm_grad, dict(grad_input_ld=3), EINVAL, "overlap"), (_norm_grad, dict(features=1 << 17), EINVAL, "features"),
+    (_logprobs, dict(classes=0), EINVAL, "shape"), (_logprobs, dict(top=65), EINVAL, "top"), (_logprobs, dict(top=-1), EINVAL, "top"),
+    (_logprobs, dict(classes=4), EINVAL, "top"), (_logprobs, dict(logits=0), ENULL, "logits"),
+    (_logprobs, dict(targets=0), ENULL, "targets"), (_logprobs, dict(logprob=0, rank=P, targets=0), ENULL, "targets"),
+    (_logprobs, dict(logits_ld=79), EINVAL, "overlap"), (_logprobs, dict(dtype=4), EINVAL, "dtype"),
+    (_logprobs_grad, dict(classes=-2), EINVAL, "shape"), (_logprobs_grad, dict(logits=0), ENULL, "logits"),
+    (_logprobs_grad, dict(logsumexp=0), ENULL, "logsumexp"), (_logprobs_grad, dict(entropy=0), ENULL, "entropy"),
+    (_logprobs_grad, dict(targets=0), ENULL, "targets"), (_logprobs_grad, dict(grad_logits=0), ENULL, "grad_logits"),
+    (_logprobs_grad, dict(grad_logits=P, grad_logits_ld=96), EINVAL, "stride"),
+])
+def test_refusals(make, change, code, message):
+    if make is _linear and "residual" in change:
+        change = dict(change, output=P)
+    if make is _norm and "output_ld" in change:
+        change = dict(change, output=P)
+    entry, d = make(**change)
+    lib = _lib().lib
+    assert getattr(lib, entry)(C.byref(d), None) == code
+    assert message in lib.tcbnn_last_error().decode()
+
+
+def test_no_rows_and_null_descriptors():
+    lib = _lib().lib
+    for entry, d in (_linear(rows=0, input=0, output=0), _norm(rows=0, input=0, output=0), _logprobs(rows=0, logits=0),
+                     _logprobs_grad(rows=0, logits=0)):
+        assert getattr(lib, entry)(C.byref(d), None) == 0
+    for entry in ("tcbnn_linear_forward", "tcbnn_linear_backward", "tcbnn_layernorm_forward", "tcbnn_layernorm_backward",
+                  "tcbnn_logprobs_forward", "tcbnn_logprobs_backward"):
+        assert getattr(lib, entry)(None, None) == ENULL
+
+
+def test_workspaces_of_refused_sizes_are_empty():
+    lib = _lib().lib
+    assert lib.tcbnn_linear_workspace_bytes(0, 8, 8, 0) == lib.tcbnn_linear_workspace_bytes(4, -1, 8, 0) == 0
+    assert lib.tcbnn_linear_grad_workspace_bytes(4, 8, 0, 0) == lib.tcbnn_linear_grad_workspace_bytes(4, 8, 8, 7) == 0
+    assert lib.tcbnn_layernorm_grad_workspace_bytes(0, 8) == lib.tcbnn_layernorm_grad_workspace_bytes(4, -8) == 0
+    assert lib.tcbnn_logprobs_workspace_bytes(-1, 8, 0, 0) == lib.tcbnn_logprobs_workspace_bytes(4, 8, 99, 0) == 0
+
+
+def test_layers_refuse():
+    from tcbnn_amd import head
+    from tcbnn_amd.device import DeviceView
+    E = _lib().TcbnnError
+    buf = DeviceView(P, 4 * 64)
+    with pytest.raises(E, match="dtype"):
+        head.LinearLayerParam("l", 4, 8, 8, "f64")
+    with pytest.raises(E, match="activation"):
+        head.LinearLayerParam("l", 4, 8, 8, "f32", "tanh")
+    with pytest.raises(E, match="NULL pointer"):
+        head.LinearLayerParam("l", 4, 8, 8).initialize(buf, None, None, output_gpu=buf)
+    with pytest.raises(E, match="input holds"):
+        head.LinearLayerParam("l", 9, 8, 8).initialize(buf, None, buf, output_gpu=buf)
+    with pytest.raises(E, match="weight holds"):
+        head.LinearLayerParam("l", 1, 8, 9).initialize(buf, None, buf, output_gpu=buf)
+    with pytest.raises(E, match="preact"):
+        head.LinearLayerParam("l", 1, 8, 8, activation="silu").initialize(buf, None, buf, output_gpu=buf).initialize_backward(buf)
+    with pytest.raises(E, match="not initialized"):
+        head.LayerNormLayerParam("n", 4, 8).forward()
+    with pytest.raises(E, match="gamma holds"):
+        head.LayerNormLayerParam("n", 1, 64).initialize(DeviceView(P, 60), None, buf, output_gpu=buf)
+    with pytest.raises(E, match="targets"):
+        head.LogProbsLayerParam("p", 4, 8).initialize(buf, entropy_gpu=buf, logsumexp_gpu=buf).initialize_backward(buf, None, buf)
+
+
+def test_views_of_tensors():
+    torch = pytest.importorskip("torch")
+    from tcbnn_amd.device import DeviceView
+    wide = torch.zeros((5, 12))
+    v = DeviceView.of(wide[:, 2:9])
+    assert (v.ptr, v.ld, v.nbytes) == (wide.data_ptr() + 8, 12, 4 * 35)
+    assert DeviceView.of(wide[1]).ld == 0 and DeviceView.of(wide[:1, :7]).ld == 0
+    for bad in (wide.t(), wide[:, ::2], wide.reshape(5, 3, 4)):
+        with pytest.raises(_lib().TcbnnError):
+            DeviceView.of(bad)
+
+
+def test_encode_rounds_to_nearest_even():
+    from tcbnn_amd import head
+    torch = pytest.importorskip("torch")
+    r = np.random.default_rng(3)
+    x = np.concatenate([r.integers(0, 2 ** 32, 20000, dtype=np.uint64).astype(np.uint32).view(np.float32),
+                        np.array([0.0, -0.0, np.inf, -np.inf, 1.00390625, 1.01171875, 3.4e38], np.float32)])
+    for dtype, t in (("bf16", torch.bfloat16), ("f16", torch.float16), ("f32", torch.float32)):
+        want = torch.from_numpy(x).to(t).float().numpy()
+        with np.errstate(over="ignore", invalid="ignore"):
+            np.testing.assert_array_equal(head.decode(head.encode(x, dtype), dtype), want)
+
+
+def _differences(f, x, v):
+    h = 1e-5
+    return (f(x + h * v) - f(x - h * v)) / (2 * h)
+
+
+@pytest.mark.parametrize("name", ["none", "relu", "gelu", "silu"])
+def test_slopes_of_activations(name):
+    z = np.linspace(-6, 6, 241) + 0.01234
+    np.testing.assert_allclose(_differences(lambda a: ho.act(name, a), z, 1.0), ho.slope(name, z), atol=1e-8)
+
+
+def test_gradient_formulas_of_norm_and_log_probabilities():
+    r = np.random.default_rng(9)
+    m, n = 5, 12
+    x, gamma, dy, v = (r.standard_normal(s) for s in ((m, n), (n,), (m, n), (m, n)))
+    _, mean, rstd = ho.norm(x, gamma, 0.0, 1e-5)
+    xh, g = (x - mean[:, None]) * rstd[:, None], dy * gamma
+    dx = (g - g.mean(1, keepdims=True) - xh * (g * xh).mean(1, keepdims=True)) * rstd[:, None]
+    assert abs(_differences(lambda a: (dy * ho.norm(a, gamma, 0.0, 1e-5)[0]).sum(), x, v) - (dx * v).sum()) < 1e-7
+    t, c, ce = 3, 0.7, -0.4
+    logprob, entropy, lse, *_ = ho.logprobs(x[0], t, 0)
+    p = np.exp(x[0] - lse)
+    dx = c * ((np.arange(n) == t) - p) - ce * p * (x[0] - lse + entropy)
+
+    def f(a):
+        lp, h, *_ = ho.logprobs(a, t, 0)
+        return c * lp + ce * h
+
+    assert abs(_differences(f, x[0], v[0]) - (dx * v[0]).sum()) < 1e-8
