@@ -2,7 +2,8 @@
 // any alignment, sums over wavefronts and workgroups, activations, and the choice of a kernel by type.
 #pragma once
 
-#include <utility>
+#include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -54,17 +55,39 @@ auto by_dtype(int dtype, F&& f) {
 // The distance between rows: 0 stands for rows without gaps.  A negative result is a row that overlaps the next.
 inline long long row_stride(long long ld, long long length) { return ld == 0 ? length : (ld < length ? -1 : ld); }
 
-// ---- sums and maxima over the 64 lanes; every lane gets the result.  The order is the same in every call.
+// ---- sums and maxima over the 64 lanes, by DPP within 16 lanes and lane swaps beyond (a shuffle through LDS takes ten times
+// as long).  Every lane gets the same bits, and the order is the same in every call.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int kSwapPairs = 0xb1, kSwapTwos = 0x4e, kMirrorHalf = 0x141, kMirrorRow = 0x140;
+// f(v, v of the lane 16 or 32 away)
+template <typename F>
+__device__ __forceinline__ uint32_t across_rows(uint32_t v, F f) {
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f((uint32_t)a[0], (uint32_t)a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f((uint32_t)b[0], (uint32_t)b[1]);
+}
+template <typename F>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t v, F f) {
+    v = f(v, dpp<kSwapPairs>(v));
+    v = f(v, dpp<kSwapTwos>(v));
+    v = f(v, dpp<kMirrorHalf>(v));
+    v = f(v, dpp<kMirrorRow>(v));
+    return across_rows(v, f);
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+    return __uint_as_float(wave_reduce(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+    return __uint_as_float(wave_reduce(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
 }
+
+// What grids are sized for.  A constant, not the device's own count: how work is split decides the order of sums, and the size
+// of a workspace is asked for before a device is chosen.
+constexpr int kComputeUnits = 256;
 
 }  // namespace head
 }  // namespace tcbnn

@@ -3,6 +3,10 @@
 //   mean = sum x / N,  var = sum (x - mean)^2 / N,  rstd = 1 / sqrt(var + eps),  y = (x - mean) rstd gamma + beta
 //   xh = (x - mean) rstd,  g = dy gamma,  dx = rstd (g - mean(g) - xh mean(g xh)),
 //   dgamma = sum over rows of dy xh,  dbeta = sum over rows of dy
+//
+// Bound by memory: every value is read once and kept in registers as fp32 (the variance is summed about the mean, which one
+// pass over the memory allows because the row is still there).  A row belongs to a team of W wavefronts whose lanes hold R
+// vectors of 16 bytes each; teams go from row to row, so gamma, beta and the gradient's sums over rows stay in registers too.
 #include "head.h"
 
 namespace tcbnn {
@@ -10,91 +14,341 @@ namespace {
 
 using namespace head;
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
 constexpr int kMaxFeatures = 65536;
 
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.0f;
+// R vectors of a row, 64 W lanes side by side; what lies past the row becomes `pad`
+template <typename T, int W, int R>
+struct RowSlice {
+    static constexpr int V = Elem<T>::kVec;
+    static constexpr int kStep = 64 * W * V;  // elements that one vector of every lane covers
+    float v[R][V];
+
+    __device__ __forceinline__ void load(const T* __restrict__ row, int lane, int n, float pad) {
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) v += lds[w];
+        for (int r = 0; r < R; ++r) {
+            const int i = r * kStep + lane * V;
+            if ((r + 1) * kStep <= n || i + V <= n) {  // (the first test is the same for all lanes: whole slices have no branch)
+                const Vec<T> x = load_vec(row + i);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[r][e] = (float)x[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[r][e] = i + e < n ? (float)row[i + e] : pad;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* __restrict__ row, int lane, int n) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = r * kStep + lane * V;
+            if ((r + 1) * kStep <= n || i + V <= n) {
+                Vec<T> x;
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[e] = (T)v[r][e];
+                store_vec(row + i, x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (i + e < n) row[i + e] = (T)v[r][e];
+            }
+        }
+    }
+    // the lane's part of a vector of parameters, or `fill` where there is none
+    __device__ __forceinline__ void load_param(const float* __restrict__ p, int lane, int n, float fill) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const int i = r * kStep + lane * V + e;
+                v[r][e] = p == nullptr ? fill : (i < n ? p[i] : 0.0f);
+            }
+    }
+};
+
+// The sum over a team's wavefronts.  Two alternating slots: whoever writes a slot again has passed the barrier after its last
+// reading, so one barrier a sum is enough.
+template <int W>
+__device__ __forceinline__ float team_sum(float v, float* slot, int wave) {
+    v = wave_sum(v);
+    if constexpr (W > 1) {
+        slot[wave] = v;  // (all lanes of a wavefront write the same value)
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v += slot[w];
+    }
     return v;
 }
 
+constexpr int forward_threads(int w) { return w > 4 ? 64 * w : 256; }
+
+// All teams of a workgroup take the same number of steps; one without a row of its own computes on row 0 and keeps nothing.
+template <typename T, int W, int R>
+__global__ __launch_bounds__(forward_threads(W)) void layernorm_kernel(const T* x, const float* __restrict__ gamma,
+                                                                       const float* __restrict__ beta, T* y,
+                                                                       float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                                                                       int rows, int n, float eps, long long x_ld, long long y_ld) {
+    constexpr int kTeams = forward_threads(W) / (64 * W);
+    using Slice = RowSlice<T, W, R>;
+    constexpr int V = Slice::V;
+    __shared__ float slots[2][kTeams][W];
+    const int lane = threadIdx.x % (64 * W), wave = lane >> 6, team = threadIdx.x / (64 * W);
+    Slice g, b, s;
+    g.load_param(gamma, lane, n, 1.0f);
+    b.load_param(beta, lane, n, 0.0f);
+    const float inv = 1.0f / (float)n;
+    for (long long first = (long long)blockIdx.x * kTeams; first < rows; first += (long long)gridDim.x * kTeams) {
+        const bool mine = first + team < rows;
+        const long long row = mine ? first + team : first;
+        s.load(x + row * x_ld, lane, n, 0.0f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum += s.v[r][e];
+        const float mean = team_sum<W>(sum, slots[0][team], wave) * inv;
+        float sq = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                // what lies past the row (the last slices' lanes alone) has no share in the variance
+                const bool in = (r + 1) * Slice::kStep <= n || r * Slice::kStep + lane * V + e < n;
+                const float d = in ? s.v[r][e] - mean : 0.0f;
+                s.v[r][e] = d;
+                sq = __builtin_fmaf(d, d, sq);
+            }
+        const float rstd = 1.0f / sqrtf(__builtin_fmaf(team_sum<W>(sq, slots[1][team], wave), inv, eps));
+        if (!mine) continue;
+        if (lane == 0) {
+            if (mean_out) mean_out[row] = mean;
+            if (rstd_out) rstd_out[row] = rstd;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s.v[r][e] = __builtin_fmaf(s.v[r][e] * rstd, g.v[r][e], b.v[r][e]);
+        s.store(y + row * y_ld, lane, n);
+    }
+}
+
+// Rows that a workgroup's registers do not hold: a workgroup a row, which is read three times (twice from the cache).
+constexpr int kLongThreads = 1024;
+__device__ __forceinline__ float long_sum(float v, float* slot) { return team_sum<kLongThreads / 64>(v, slot, threadIdx.x >> 6); }
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void layernorm_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
-                                                             const float* __restrict__ beta, T* __restrict__ y,
-                                                             float* __restrict__ mean_out, float* __restrict__ rstd_out, int n,
-                                                             float eps, long long x_ld, long long y_ld) {
-    __shared__ float lds[kWaves];
+__global__ __launch_bounds__(kLongThreads) void layernorm_long_kernel(const T* x, const float* __restrict__ gamma,
+                                                                      const float* __restrict__ beta, T* y,
+                                                                      float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                                                                      int n, float eps, long long x_ld, long long y_ld) {
+    __shared__ float slots[2][kLongThreads / 64];
     const long long row = blockIdx.x;
     x += row * x_ld;
     y += row * y_ld;
     float s = 0.0f;
-    for (int i = threadIdx.x; i < n; i += kThreads) s += (float)x[i];
-    const float mean = block_sum(s, lds) / (float)n;
+    for (int i = threadIdx.x; i < n; i += kLongThreads) s += (float)x[i];
+    const float mean = long_sum(s, slots[0]) / (float)n;
     s = 0.0f;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += kLongThreads) {
         const float d = (float)x[i] - mean;
         s = __builtin_fmaf(d, d, s);
     }
-    const float rstd = 1.0f / sqrtf(block_sum(s, lds) / (float)n + eps);
+    const float rstd = 1.0f / sqrtf(long_sum(s, slots[1]) / (float)n + eps);
     if (threadIdx.x == 0) {
         if (mean_out) mean_out[row] = mean;
         if (rstd_out) rstd_out[row] = rstd;
     }
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const float xh = ((float)x[i] - mean) * rstd;
-        y[i] = (T)__builtin_fmaf(xh, gamma ? gamma[i] : 1.0f, beta ? beta[i] : 0.0f);
+    for (int i = threadIdx.x; i < n; i += kLongThreads)
+        y[i] = (T)__builtin_fmaf(((float)x[i] - mean) * rstd, gamma ? gamma[i] : 1.0f, beta ? beta[i] : 0.0f);
+}
+
+// ---- gradient.  A workgroup of 16 wavefronts is 16 / W teams; all of them take the same number of steps (a team without a
+// row of its own computes on row 0 of what there is and keeps nothing).  PARAMS: sums over the workgroup's rows of dy xh and
+// dy, one row of `partial` a workgroup: [2][n] each.
+constexpr int kGradThreads = 1024;
+
+template <typename T, int W, int R, bool PARAMS>
+__global__ __launch_bounds__(kGradThreads) void layernorm_grad_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
+                                                                      const float* __restrict__ mean_in,
+                                                                      const float* __restrict__ rstd_in, const T* dy, T* dx,
+                                                                      float* __restrict__ partial, int rows, int n, long long x_ld,
+                                                                      long long dy_ld, long long dx_ld) {
+    constexpr int kTeams = kGradThreads / (64 * W);
+    using Slice = RowSlice<T, W, R>;
+    constexpr int V = Slice::V;
+    __shared__ float slots[2][kTeams][2][W];
+    __shared__ float sums[PARAMS && kTeams > 1 ? kTeams * 64 * W * V : 1];
+    const int lane = threadIdx.x % (64 * W), wave = lane >> 6, team = threadIdx.x / (64 * W);
+    Slice g, s, d, dg, db;
+    g.load_param(gamma, lane, n, 1.0f);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) dg.v[r][e] = db.v[r][e] = 0.0f;
+    const float inv = 1.0f / (float)n;
+    const long long stride = (long long)gridDim.x * kTeams;
+    int parity = 0;
+    for (long long first = (long long)blockIdx.x * kTeams; first < rows; first += stride, parity ^= 1) {
+        const bool mine = first + team < rows;
+        const long long row = mine ? first + team : 0;
+        s.load(x + row * x_ld, lane, n, 0.0f);
+        d.load(dy + row * dy_ld, lane, n, 0.0f);
+        const float mean = mean_in[row], rstd = rstd_in[row];
+        float sg = 0.0f, sgx = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float xh = (s.v[r][e] - mean) * rstd;  // (past the row dy is 0, and so is every product)
+                s.v[r][e] = xh;
+                if constexpr (PARAMS) {
+                    const float dv = mine ? d.v[r][e] : 0.0f;
+                    db.v[r][e] += dv;
+                    dg.v[r][e] = __builtin_fmaf(dv, xh, dg.v[r][e]);
+                }
+                const float gv = d.v[r][e] * g.v[r][e];
+                d.v[r][e] = gv;
+                sg += gv;
+                sgx = __builtin_fmaf(gv, xh, sgx);
+            }
+        if (dx) {
+            sg = wave_sum(sg);
+            sgx = wave_sum(sgx);
+            if constexpr (W > 1) {
+                slots[parity][team][0][wave] = sg;
+                slots[parity][team][1][wave] = sgx;
+                __syncthreads();
+                sg = sgx = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    sg += slots[parity][team][0][w];
+                    sgx += slots[parity][team][1][w];
+                }
+            }
+            sg *= inv;
+            sgx *= inv;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int e = 0; e < V; ++e) d.v[r][e] = (d.v[r][e] - sg - s.v[r][e] * sgx) * rstd;
+            if (mine) d.store(dx + row * dx_ld, lane, n);
+        }
+    }
+    if constexpr (PARAMS) {
+        float* out = partial + (size_t)blockIdx.x * 2 * n;
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const Slice& a = which == 0 ? dg : db;
+                if constexpr (kTeams == 1) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (r * Slice::kStep + lane * V + e < n) out[(size_t)which * n + r * Slice::kStep + lane * V + e] = a.v[r][e];
+                } else {
+                    __syncthreads();
+#pragma unroll
+                    for (int e = 0; e < V; ++e) sums[(team * V + e) * 64 * W + lane] = a.v[r][e];  // (lanes side by side: no bank twice)
+                    __syncthreads();
+                    for (int c = threadIdx.x; c < Slice::kStep; c += kGradThreads) {
+                        const int e = c / (64 * W), l = c % (64 * W), i = r * Slice::kStep + l * V + e;
+                        float t = 0.0f;
+                        for (int k = 0; k < kTeams; ++k) t += sums[(k * V + e) * 64 * W + l];
+                        if (i < n) out[(size_t)which * n + i] = t;
+                    }
+                }
+            }
     }
 }
 
+// Rows that a workgroup's registers do not hold: the gradient of the input, a workgroup a row ...
 template <typename T>
-__global__ __launch_bounds__(kThreads) void layernorm_dx_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
-                                                                const float* __restrict__ mean_in,
-                                                                const float* __restrict__ rstd_in, const T* dy, T* dx, int n,
-                                                                long long x_ld, long long dy_ld, long long dx_ld) {
-    __shared__ float lds[kWaves];
+__global__ __launch_bounds__(kLongThreads) void layernorm_long_grad_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
+                                                                           const float* __restrict__ mean_in,
+                                                                           const float* __restrict__ rstd_in, const T* dy, T* dx,
+                                                                           int n, long long x_ld, long long dy_ld, long long dx_ld) {
+    __shared__ float slots[2][kLongThreads / 64];
     const long long row = blockIdx.x;
     x += row * x_ld;
     dy += row * dy_ld;
     dx += row * dx_ld;
     const float mean = mean_in[row], rstd = rstd_in[row];
     float sg = 0.0f, sgx = 0.0f;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += kLongThreads) {
         const float g = (float)dy[i] * (gamma ? gamma[i] : 1.0f);
         sg += g;
         sgx = __builtin_fmaf(g, ((float)x[i] - mean) * rstd, sgx);
     }
-    sg = block_sum(sg, lds) / (float)n;
-    sgx = block_sum(sgx, lds) / (float)n;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    sg = long_sum(sg, slots[0]) / (float)n;
+    sgx = long_sum(sgx, slots[1]) / (float)n;
+    for (int i = threadIdx.x; i < n; i += kLongThreads) {
         const float g = (float)dy[i] * (gamma ? gamma[i] : 1.0f);
-        const float xh = ((float)x[i] - mean) * rstd;
-        dx[i] = (T)((g - sg - xh * sgx) * rstd);
+        dx[i] = (T)((g - sg - ((float)x[i] - mean) * rstd * sgx) * rstd);
     }
 }
 
-// a thread a feature, all rows in order
+// ... and the parameters' sums: 256 features a workgroup, every so manieth row, sums as above.
+constexpr int kColumnThreads = 256;
 template <typename T>
-__global__ __launch_bounds__(kThreads) void layernorm_params_kernel(const T* __restrict__ x, const float* __restrict__ mean,
-                                                                    const float* __restrict__ rstd, const T* __restrict__ dy,
-                                                                    float* __restrict__ dgamma, float* __restrict__ dbeta,
-                                                                    int rows, int n, long long x_ld, long long dy_ld) {
-    const int i = blockIdx.x * kThreads + threadIdx.x;
+__global__ __launch_bounds__(kColumnThreads) void layernorm_columns_kernel(const T* __restrict__ x, const float* __restrict__ mean,
+                                                                           const float* __restrict__ rstd, const T* __restrict__ dy,
+                                                                           float* __restrict__ partial, int rows, int n,
+                                                                           long long x_ld, long long dy_ld) {
+    const int i = blockIdx.x * kColumnThreads + threadIdx.x;
     if (i >= n) return;
     float sg = 0.0f, sb = 0.0f;
-    for (long long r = 0; r < rows; ++r) {
+    for (long long r = blockIdx.y; r < rows; r += gridDim.y) {
         const float d = (float)dy[r * dy_ld + i];
         sb += d;
         sg = __builtin_fmaf(d, ((float)x[r * x_ld + i] - mean[r]) * rstd[r], sg);
     }
-    if (dgamma) dgamma[i] = sg;
-    if (dbeta) dbeta[i] = sb;
+    partial[((size_t)blockIdx.y * 2) * n + i] = sg;
+    partial[((size_t)blockIdx.y * 2 + 1) * n + i] = sb;
+}
+
+// The sums of all workgroups: 16 features a workgroup, 16 threads to a feature.
+constexpr int kJoinThreads = 256, kJoinFeatures = 16;
+__global__ __launch_bounds__(kJoinThreads) void layernorm_join_kernel(const float* __restrict__ partial, float* __restrict__ dgamma,
+                                                                      float* __restrict__ dbeta, int parts, int n) {
+    __shared__ float lds[kJoinThreads / kJoinFeatures][kJoinFeatures];
+    const int c = threadIdx.x % kJoinFeatures, part = threadIdx.x / kJoinFeatures, i = blockIdx.x * kJoinFeatures + c;
+    float* out = blockIdx.y == 0 ? dgamma : dbeta;
+    if (out == nullptr) return;
+    float s = 0.0f;
+    if (i < n)
+        for (int k = part; k < parts; k += kJoinThreads / kJoinFeatures) s += partial[((size_t)k * 2 + blockIdx.y) * n + i];
+    lds[part][c] = s;
+    __syncthreads();
+    if (part == 0 && i < n) {
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kJoinThreads / kJoinFeatures; ++k) s += lds[k][c];
+        out[i] = s;
+    }
+}
+
+// The team of wavefronts that keeps a row of so many vectors of 16 bytes: one vector a lane, two in the longest.
+inline int row_vectors(int n, int per_vector) { return (n + per_vector - 1) / per_vector; }
+constexpr int kMaxVectors = 2 * 16 * 64;
+template <typename F>
+void by_team(int vectors, F&& f) {
+    using std::integral_constant;
+    if (vectors <= 64) return f(integral_constant<int, 1>(), integral_constant<int, 1>());
+    if (vectors <= 128) return f(integral_constant<int, 2>(), integral_constant<int, 1>());
+    if (vectors <= 256) return f(integral_constant<int, 4>(), integral_constant<int, 1>());
+    if (vectors <= 512) return f(integral_constant<int, 8>(), integral_constant<int, 1>());
+    if (vectors <= 1024) return f(integral_constant<int, 16>(), integral_constant<int, 1>());
+    return f(integral_constant<int, 16>(), integral_constant<int, 2>());
+}
+
+// workgroups whose sums over rows are joined afterwards
+inline int grad_parts(int rows) { return std::max(1, std::min(rows, kComputeUnits)); }
+
+int check_norm(int rows, int features, int dtype) {
+    TCBNN_REQUIRE(dtype_known(dtype), "layernorm: unknown dtype");
+    TCBNN_REQUIRE(rows >= 0 && features > 0, "layernorm: bad shape");
+    TCBNN_REQUIRE(features <= kMaxFeatures, "layernorm: at most %d features", kMaxFeatures);
+    return TCBNN_OK;
 }
 
 }  // namespace
@@ -105,9 +359,7 @@ using namespace tcbnn::head;
 
 extern "C" int tcbnn_layernorm_forward(const tcbnn_layernorm_desc* d, void* stream) {
     TCBNN_NOTNULL(d);
-    TCBNN_REQUIRE(dtype_known(d->dtype), "layernorm: unknown dtype");
-    TCBNN_REQUIRE(d->rows >= 0 && d->features > 0, "layernorm: bad shape");
-    TCBNN_REQUIRE(d->features <= kMaxFeatures, "layernorm: at most %d features", kMaxFeatures);
+    if (int rc = check_norm(d->rows, d->features, d->dtype)) return rc;
     TCBNN_REQUIRE(d->eps >= 0.0f, "layernorm: eps must be 0 or more");
     const long long x_ld = row_stride(d->input_ld, d->features), y_ld = row_stride(d->output_ld, d->features);
     TCBNN_REQUIRE(x_ld > 0 && y_ld > 0, "layernorm: rows overlap");
@@ -117,42 +369,87 @@ extern "C" int tcbnn_layernorm_forward(const tcbnn_layernorm_desc* d, void* stre
     TCBNN_REQUIRE(d->output != d->input || d->rows == 1 || x_ld == y_ld, "layernorm: an output over its input has the input's stride");
     by_dtype(d->dtype, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(layernorm_kernel<T>, dim3((unsigned)d->rows), dim3(kThreads), 0, (hipStream_t)stream, (const T*)d->input,
-                           d->gamma, d->beta, (T*)d->output, d->mean, d->rstd, d->features, d->eps, x_ld, y_ld);
+        const int vectors = row_vectors(d->features, Elem<T>::kVec);
+        if (vectors > kMaxVectors) {
+            hipLaunchKernelGGL(layernorm_long_kernel<T>, dim3((unsigned)d->rows), dim3(kLongThreads), 0, (hipStream_t)stream,
+                               (const T*)d->input, d->gamma, d->beta, (T*)d->output, d->mean, d->rstd, d->features, d->eps, x_ld, y_ld);
+            return;
+        }
+        by_team(vectors, [&](auto w, auto r) {
+            constexpr int W = w.value, R = r.value;
+            const int teams = forward_threads(W) / (64 * W);
+            // the registers of 2048 threads a compute unit, more where rows are left
+            const int blocks = std::min((d->rows + teams - 1) / teams, kComputeUnits * 2048 / forward_threads(W));
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(layernorm_kernel<T, W, R>), dim3((unsigned)blocks), dim3(forward_threads(W)), 0,
+                               (hipStream_t)stream, (const T*)d->input, d->gamma, d->beta, (T*)d->output, d->mean, d->rstd, d->rows,
+                               d->features, d->eps, x_ld, y_ld);
+        });
     });
     TCBNN_LAUNCH_CHECK("layernorm_kernel");
     return TCBNN_OK;
 }
 
-extern "C" size_t tcbnn_layernorm_grad_workspace_bytes(int rows, int features) { return 0; }
+extern "C" size_t tcbnn_layernorm_grad_workspace_bytes(int rows, int features) {
+    if (rows <= 0 || features <= 0 || features > kMaxFeatures) return 0;
+    return (size_t)grad_parts(rows) * 2 * features * sizeof(float);
+}
 
 extern "C" int tcbnn_layernorm_backward(const tcbnn_layernorm_grad_desc* d, void* stream) {
     TCBNN_NOTNULL(d);
-    TCBNN_REQUIRE(dtype_known(d->dtype), "layernorm: unknown dtype");
-    TCBNN_REQUIRE(d->rows >= 0 && d->features > 0, "layernorm: bad shape");
-    TCBNN_REQUIRE(d->features <= kMaxFeatures, "layernorm: at most %d features", kMaxFeatures);
+    if (int rc = check_norm(d->rows, d->features, d->dtype)) return rc;
     const long long x_ld = row_stride(d->input_ld, d->features), dy_ld = row_stride(d->grad_output_ld, d->features),
                     dx_ld = row_stride(d->grad_input_ld, d->features);
     TCBNN_REQUIRE(x_ld > 0 && dy_ld > 0 && dx_ld > 0, "layernorm: rows overlap");
+    const bool params = d->grad_gamma || d->grad_beta;
     if (d->rows > 0) {
         TCBNN_NOTNULL(d->input);
         TCBNN_NOTNULL(d->mean);
         TCBNN_NOTNULL(d->rstd);
         TCBNN_NOTNULL(d->grad_output);
+        if (params) {
+            TCBNN_NOTNULL(d->workspace);
+            TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_layernorm_grad_workspace_bytes(d->rows, d->features), "layernorm: workspace too small");
+        }
     }
     TCBNN_REQUIRE(d->grad_input != d->grad_output || d->grad_input == nullptr || d->rows <= 1 || dx_ld == dy_ld,
                   "layernorm: a gradient over another has its stride");
-    by_dtype(d->dtype, [&](auto t) {
-        using T = decltype(t);
-        if (d->grad_gamma || d->grad_beta)
-            hipLaunchKernelGGL(layernorm_params_kernel<T>, dim3((unsigned)((d->features + kThreads - 1) / kThreads)), dim3(kThreads), 0,
-                               (hipStream_t)stream, (const T*)d->input, d->mean, d->rstd, (const T*)d->grad_output, d->grad_gamma,
-                               d->grad_beta, d->rows, d->features, x_ld, dy_ld);
-        if (d->grad_input && d->rows > 0)
-            hipLaunchKernelGGL(layernorm_dx_kernel<T>, dim3((unsigned)d->rows), dim3(kThreads), 0, (hipStream_t)stream,
-                               (const T*)d->input, d->gamma, d->mean, d->rstd, (const T*)d->grad_output, (T*)d->grad_input,
-                               d->features, x_ld, dy_ld, dx_ld);
-    });
-    TCBNN_LAUNCH_CHECK("layernorm_dx_kernel");
+    float* partial = (float*)d->workspace;
+    int parts = 0;
+    if (d->rows > 0)
+        by_dtype(d->dtype, [&](auto t) {
+            using T = decltype(t);
+            const int vectors = row_vectors(d->features, Elem<T>::kVec);
+            if (vectors > kMaxVectors) {
+                if (params) {
+                    parts = grad_parts(d->rows);
+                    hipLaunchKernelGGL(layernorm_columns_kernel<T>,
+                                       dim3((unsigned)((d->features + kColumnThreads - 1) / kColumnThreads), (unsigned)parts),
+                                       dim3(kColumnThreads), 0, (hipStream_t)stream, (const T*)d->input, d->mean, d->rstd,
+                                       (const T*)d->grad_output, partial, d->rows, d->features, x_ld, dy_ld);
+                }
+                if (d->grad_input)
+                    hipLaunchKernelGGL(layernorm_long_grad_kernel<T>, dim3((unsigned)d->rows), dim3(kLongThreads), 0, (hipStream_t)stream,
+                                       (const T*)d->input, d->gamma, d->mean, d->rstd, (const T*)d->grad_output, (T*)d->grad_input,
+                                       d->features, x_ld, dy_ld, dx_ld);
+                return;
+            }
+            by_team(vectors, [&](auto w, auto r) {
+                constexpr int W = w.value, R = r.value, kTeams = kGradThreads / (64 * W);
+                parts = std::min((d->rows + kTeams - 1) / kTeams, grad_parts(d->rows));
+                auto launch = [&](auto kernel) {
+                    hipLaunchKernelGGL(kernel, dim3((unsigned)parts), dim3(kGradThreads), 0, (hipStream_t)stream, (const T*)d->input,
+                                       d->gamma, d->mean, d->rstd, (const T*)d->grad_output, (T*)d->grad_input, partial, d->rows,
+                                       d->features, x_ld, dy_ld, dx_ld);
+                };
+                if (params)
+                    launch(layernorm_grad_kernel<T, W, R, true>);
+                else if (d->grad_input)
+                    launch(layernorm_grad_kernel<T, W, R, false>);
+            });
+        });
+    if (params)
+        hipLaunchKernelGGL(layernorm_join_kernel, dim3((unsigned)((d->features + kJoinFeatures - 1) / kJoinFeatures), 2), dim3(kJoinThreads),
+                           0, (hipStream_t)stream, partial, d->grad_gamma, d->grad_beta, parts, d->features);
+    TCBNN_LAUNCH_CHECK("layernorm_grad_kernel");
     return TCBNN_OK;
 }
