@@ -16,26 +16,32 @@ using namespace head;
 
 constexpr int kMaxFeatures = 65536;
 
-// R vectors of a row, 64 W lanes side by side; what lies past the row becomes `pad`
+// R vectors of a row, 64 W lanes side by side
 template <typename T, int W, int R>
 struct RowSlice {
     static constexpr int V = Elem<T>::kVec;
     static constexpr int kStep = 64 * W * V;  // elements that one vector of every lane covers
     float v[R][V];
 
-    __device__ __forceinline__ void load(const T* __restrict__ row, int lane, int n, float pad) {
+    // A row's vectors are requested a step before they are taken up: what lies past the row is 0.
+    using Raw = Vec<T>[R];
+    static __device__ __forceinline__ void request(const T* __restrict__ row, int lane, int n, Raw& raw) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int i = r * kStep + lane * V;
-            if ((r + 1) * kStep <= n || i + V <= n) {  // (the first test is the same for all lanes: whole slices have no branch)
-                const Vec<T> x = load_vec(row + i);
-#pragma unroll
-                for (int e = 0; e < V; ++e) v[r][e] = (float)x[e];
+            if ((r + 1) * kStep <= n || i + V <= n) {
+                raw[r] = load_vec(row + i);
             } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[r][e] = i + e < n ? (float)row[i + e] : pad;
+                for (int e = 0; e < V; ++e) raw[r][e] = i + e < n ? row[i + e] : (T)0.0f;
             }
         }
+    }
+    __device__ __forceinline__ void take(const Raw& raw) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[r][e] = (float)raw[r][e];
     }
     __device__ __forceinline__ void store(T* __restrict__ row, int lane, int n) const {
 #pragma unroll
@@ -56,12 +62,23 @@ struct RowSlice {
     // the lane's part of a vector of parameters, or `fill` where there is none
     __device__ __forceinline__ void load_param(const float* __restrict__ p, int lane, int n, float fill) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+            const int i = r * kStep + lane * V;
+            if (p == nullptr) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int i = r * kStep + lane * V + e;
-                v[r][e] = p == nullptr ? fill : (i < n ? p[i] : 0.0f);
+                for (int e = 0; e < V; ++e) v[r][e] = fill;
+            } else if ((r + 1) * kStep <= n || i + V <= n) {
+#pragma unroll
+                for (int e = 0; e < V; e += 4) {
+                    const Vec<float> x = load_vec(p + i + e);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[r][e + k] = x[k];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[r][e] = i + e < n ? p[i + e] : 0.0f;
             }
+        }
     }
 };
 
@@ -82,7 +99,8 @@ __device__ __forceinline__ float team_sum(float v, float* slot, int wave) {
 
 constexpr int forward_threads(int w) { return w > 4 ? 64 * w : 256; }
 
-// All teams of a workgroup take the same number of steps; one without a row of its own computes on row 0 and keeps nothing.
+// All teams of a workgroup take the same number of steps; one without a row of its own computes on the last one
+// and keeps nothing.
 template <typename T, int W, int R>
 __global__ __launch_bounds__(forward_threads(W)) void layernorm_kernel(const T* x, const float* __restrict__ gamma,
                                                                        const float* __restrict__ beta, T* y,
@@ -94,13 +112,18 @@ __global__ __launch_bounds__(forward_threads(W)) void layernorm_kernel(const T* 
     __shared__ float slots[2][kTeams][W];
     const int lane = threadIdx.x % (64 * W), wave = lane >> 6, team = threadIdx.x / (64 * W);
     Slice g, b, s;
+    typename Slice::Raw raw;
+    const long long stride = (long long)gridDim.x * kTeams;
+    auto request = [&](long long first) { Slice::request(x + min(first + team, (long long)rows - 1) * x_ld, lane, n, raw); };
+    request((long long)blockIdx.x * kTeams);
     g.load_param(gamma, lane, n, 1.0f);
     b.load_param(beta, lane, n, 0.0f);
     const float inv = 1.0f / (float)n;
-    for (long long first = (long long)blockIdx.x * kTeams; first < rows; first += (long long)gridDim.x * kTeams) {
+    for (long long first = (long long)blockIdx.x * kTeams; first < rows; first += stride) {
         const bool mine = first + team < rows;
-        const long long row = mine ? first + team : first;
-        s.load(x + row * x_ld, lane, n, 0.0f);
+        const long long row = first + team;
+        s.take(raw);
+        if (first + stride < rows) request(first + stride);
         float sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -163,7 +186,7 @@ __global__ __launch_bounds__(kLongThreads) void layernorm_long_kernel(const T* x
 }
 
 // ---- gradient.  A workgroup of 16 wavefronts is 16 / W teams; all of them take the same number of steps (a team without a
-// row of its own computes on row 0 of what there is and keeps nothing).  PARAMS: sums over the workgroup's rows of dy xh and
+// row of its own computes on the last one and keeps nothing).  PARAMS: sums over the workgroup's rows of dy xh and
 // dy, one row of `partial` a workgroup: [2][n] each.
 constexpr int kGradThreads = 1024;
 
@@ -180,19 +203,27 @@ __global__ __launch_bounds__(kGradThreads) void layernorm_grad_kernel(const T* _
     __shared__ float sums[PARAMS && kTeams > 1 ? kTeams * 64 * W * V : 1];
     const int lane = threadIdx.x % (64 * W), wave = lane >> 6, team = threadIdx.x / (64 * W);
     Slice g, s, d, dg, db;
+    typename Slice::Raw raw_x, raw_dy;
+    const long long stride = (long long)gridDim.x * kTeams;
+    auto request = [&](long long first) {
+        const long long row = min(first + team, (long long)rows - 1);
+        Slice::request(x + row * x_ld, lane, n, raw_x);
+        Slice::request(dy + row * dy_ld, lane, n, raw_dy);
+    };
+    request((long long)blockIdx.x * kTeams);
     g.load_param(gamma, lane, n, 1.0f);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int e = 0; e < V; ++e) dg.v[r][e] = db.v[r][e] = 0.0f;
     const float inv = 1.0f / (float)n;
-    const long long stride = (long long)gridDim.x * kTeams;
     int parity = 0;
     for (long long first = (long long)blockIdx.x * kTeams; first < rows; first += stride, parity ^= 1) {
         const bool mine = first + team < rows;
-        const long long row = mine ? first + team : 0;
-        s.load(x + row * x_ld, lane, n, 0.0f);
-        d.load(dy + row * dy_ld, lane, n, 0.0f);
+        const long long row = min(first + team, (long long)rows - 1);
+        s.take(raw_x);
+        d.take(raw_dy);
+        if (first + stride < rows) request(first + stride);
         const float mean = mean_in[row], rstd = rstd_in[row];
         float sg = 0.0f, sgx = 0.0f;
 #pragma unroll
@@ -315,8 +346,17 @@ __global__ __launch_bounds__(kJoinThreads) void layernorm_join_kernel(const floa
     float* out = blockIdx.y == 0 ? dgamma : dbeta;
     if (out == nullptr) return;
     float s = 0.0f;
-    if (i < n)
-        for (int k = part; k < parts; k += kJoinThreads / kJoinFeatures) s += partial[((size_t)k * 2 + blockIdx.y) * n + i];
+    if (i < n) {
+        const float* p = partial + (size_t)blockIdx.y * n + i;
+        constexpr int kStep = kJoinThreads / kJoinFeatures;
+        for (int k = part; k < parts; k += 8 * kStep) {
+            float v[8];  // (requests of their own, one wait)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = k + u * kStep < parts ? p[(size_t)(k + u * kStep) * 2 * n] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+    }
     lds[part][c] = s;
     __syncthreads();
     if (part == 0 && i < n) {
