@@ -10,9 +10,8 @@ namespace {
 
 using namespace head;
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;
+constexpr float kLog2e = 1.44269504088896341f;
 
 // The order of classes as one number: larger logits first (NaN before all, -0 with +0), lower indices first among equals.
 // Larger keys come first; 0 is below every class's key.
@@ -22,116 +21,495 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ uint64_t key_of(float x, int j) { return ((uint64_t)ordered(x) << 32) | (uint32_t)~j; }
-
+__device__ __forceinline__ int class_of(uint64_t key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float logit_of(uint64_t key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return u == 0xffffffffu ? NAN : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
 __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint64_t o = (uint64_t)__shfl_xor((unsigned long long)v, d);
-        if (o > v) v = o;
-    }
+    for (int d = 32; d > 0; d >>= 1) v = max(v, (uint64_t)__shfl_xor((unsigned long long)v, d));
     return v;
+}
+__device__ __forceinline__ int wave_sum_int(int v) { return (int)wave_reduce((uint32_t)v, [](uint32_t a, uint32_t b) { return a + b; }); }
+
+// 16 bytes of logits as they lie in memory, -inf in the place of those past the end.  They are kept as words: the compiler
+// keeps elements that come out of a branch in a register each.
+typedef int Words __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ Words load_words(const T* x, int j, int n, bool whole) {
+    constexpr int V = Elem<T>::kVec;
+    if (whole || j + V <= n) return __builtin_bit_cast(Words, load_vec(x + j));
+    Vec<T> v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = j + e < n ? x[j + e] : (T)-INFINITY;
+    return __builtin_bit_cast(Words, v);
+}
+template <typename T>
+__device__ __forceinline__ float value(const Words& w, int e) {
+    return (float)__builtin_bit_cast(Vec<T>, w)[e];
 }
 
-template <typename V, typename F>
-__device__ __forceinline__ V block_reduce(V v, V* lds, F f) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = lds[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) v = f(v, lds[w]);
-    return v;
+// What is known of a set of logits: the largest, sums of exp(x - m) and of (x - m) exp(x - m), how many go before the given
+// class.  A NaN or infinite logit leaves s NaN; no allowed class leaves m = -inf and s = 0.
+struct Part {
+    float m, s, sx;
+    int before;
+};
+__device__ __forceinline__ void rescale(Part& p, float m) {
+    const float d = p.m - m, f = p.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(d * kLog2e);
+    p.sx = f == 0.0f ? p.s * 0.0f : __builtin_fmaf(d, p.s, p.sx) * f;  // (keeps a NaN)
+    p.s *= f;
+    p.m = m;
 }
+struct Answer {
+    float m, logsum, logsumexp, entropy;
+    bool none;  // no allowed class
+    __device__ __forceinline__ explicit Answer(const Part& p) {
+        none = p.m == -INFINITY && p.s == 0.0f;
+        m = p.m;
+        logsum = logf(p.s);
+        logsumexp = none ? -INFINITY : m + logsum;
+        entropy = none ? 0.0f : logsum - p.sx / p.s;
+    }
+    __device__ __forceinline__ float log_prob(float x) const { return none ? -INFINITY : (x - m) - logsum; }
+};
 
 struct LogProbsParams {
     const int32_t* targets;
     float *logprob, *entropy, *logsumexp, *top_logprob;
     int32_t *rank, *top_index;
-    int classes, top;
+    int rows, classes, top, chunks;
     long long ld;
+    // rows in several chunks: a Part and `top` keys of each, best first
+    Part* parts;    // [rows][chunks]
+    uint64_t* keys; // [rows][chunks][top]
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ x, const LogProbsParams p) {
-    __shared__ float lds_f[kWaves];
-    __shared__ uint64_t lds_k[kWaves];
-    const long long row = blockIdx.x;
-    x += row * p.ld;
-    const int n = p.classes, tid = threadIdx.x;
-    auto add = [](float a, float b) { return a + b; };
-    // the largest key has the largest value (or NaN)
-    uint64_t best = 0;
-    for (int j = tid; j < n; j += kThreads) best = max(best, key_of((float)x[j], j));
-    best = block_reduce(wave_max_key(best), lds_k, [](uint64_t a, uint64_t b) { return max(a, b); });
-    const float m = (float)x[(int)~(uint32_t)best];
-    const float shift = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f, sx = 0.0f;
-    for (int j = tid; j < n; j += kThreads) {
-        const float d = (float)x[j] - shift;
-        const float e = expf(d);
-        s += e;
-        if (e != 0.0f) sx = __builtin_fmaf(e, d, sx);
-    }
-    s = block_reduce(wave_sum(s), lds_f, add);
-    sx = block_reduce(wave_sum(sx), lds_f, add);
-    const float lse = m == -INFINITY ? m : m + logf(s);
+__device__ __forceinline__ void write_row(const LogProbsParams& p, long long row, const Part& part, const Answer& a, bool given, float xt) {
     const int t = p.targets ? p.targets[row] : -1;
-    const bool given = t >= 0 && t < n;
-    const float xt = given ? (float)x[t] : 0.0f;
-    int before = 0;
-    if (p.rank && given) {
-        const uint64_t kt = key_of(xt, t);
-        for (int j = tid; j < n; j += kThreads) before += key_of((float)x[j], j) > kt;
-        float c = wave_sum((float)before);
-        before = (int)block_reduce(c, lds_f, add);
-    }
-    auto log_prob = [&](float v) { return m == -INFINITY ? m : v - lse; };
-    if (tid == 0) {
-        if (p.logprob) p.logprob[row] = given ? log_prob(xt) : (t < 0 ? 0.0f : NAN);
-        if (p.entropy) p.entropy[row] = m == -INFINITY ? 0.0f : logf(s) - sx / s;
-        if (p.logsumexp) p.logsumexp[row] = lse;
-        if (p.rank) p.rank[row] = given ? before : -1;
-    }
-    for (int k = 0; k < p.top; ++k) {
-        if (tid == 0) {
-            const int j = (int)~(uint32_t)best;
-            if (p.top_index) p.top_index[row * p.top + k] = j;
-            if (p.top_logprob) p.top_logprob[row * p.top + k] = log_prob((float)x[j]);
-        }
-        uint64_t next = 0;
-        for (int j = tid; j < n; j += kThreads) {
-            const uint64_t key = key_of((float)x[j], j);
-            if (key < best) next = max(next, key);
-        }
-        best = block_reduce(wave_max_key(next), lds_k, [](uint64_t a, uint64_t b) { return max(a, b); });
+    if (p.logprob) p.logprob[row] = given ? a.log_prob(xt) : (t < 0 ? 0.0f : NAN);
+    if (p.entropy) p.entropy[row] = a.entropy;
+    if (p.logsumexp) p.logsumexp[row] = a.logsumexp;
+    if (p.rank) p.rank[row] = given ? part.before : -1;
+}
+__device__ __forceinline__ void write_top(const LogProbsParams& p, long long row, const Answer& a, int place, uint64_t key) {
+    if (p.top_index) p.top_index[row * p.top + place] = class_of(key);
+    if (p.top_logprob) p.top_logprob[row * p.top + place] = a.log_prob(logit_of(key));
+}
+
+// A chunk of a row (the whole row, if it fits) belongs to a team of W wavefronts and stays in their registers, R vectors of 16
+// bytes a lane, while it is looked at: for its largest logit, for the sums, for what goes before the given class, for the best
+// classes.  Every lane number is a group of logits, and the k-th largest of the 64 groups' maxima bounds the k-th largest
+// logit from below: what reaches the bound (little more than k, for logits in any usual order) is gathered in LDS and ordered
+// by counting.  Many equal logits or a cluster in one group can be too much for the list: then the ones above the bound are
+// taken with the first of those equal to it, and if that is too much still, or the chunk holds a NaN, the best classes are
+// found one after the other.
+constexpr int kList = 256;
+constexpr int team_threads(int w) { return w == 1 ? 256 : 64 * w; }
+
+template <int W>
+__device__ __forceinline__ void team_sync() {
+    if constexpr (W == 1) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_grad_kernel(const T* x, const int32_t* __restrict__ targets,
-                                                                 const float* __restrict__ logsumexp,
-                                                                 const float* __restrict__ entropy,
-                                                                 const float* __restrict__ g_logprob,
-                                                                 const float* __restrict__ g_entropy, T* dx, int n,
-                                                                 long long x_ld, long long dx_ld) {
-    const long long row = blockIdx.x;
-    x += row * x_ld;
-    dx += row * dx_ld;
-    const float lse = logsumexp[row];
-    const int t = g_logprob ? targets[row] : -1;
-    const float g = t >= n ? NAN : (t >= 0 ? g_logprob[row] : 0.0f);
-    const float ge = g_entropy ? g_entropy[row] : 0.0f, h = g_entropy ? entropy[row] : 0.0f;
-    for (int j = threadIdx.x; j < n; j += kThreads) {
-        float out = 0.0f;
-        if (lse != -INFINITY) {
-            const float lp = (float)x[j] - lse;
-            const float p = expf(lp);
-            out = g * ((j == t ? 1.0f : 0.0f) - p);
-            if (p != 0.0f) out -= ge * p * (lp + h);
-        } else if (g != g) {
-            out = g;
+template <int W>
+struct TeamLds {
+    uint64_t list[kList];
+    uint64_t best[W];
+    Part part[W];
+    float lane_max[W][64];
+    int count, waves[W];
+};
+
+template <typename T, int W, int R, bool SPLIT>
+__global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __restrict__ x, const LogProbsParams p) {
+    constexpr int V = Elem<T>::kVec, kTeam = 64 * W, kTeams = team_threads(W) / kTeam, kStep = kTeam * V, kChunk = R * kStep;
+    __shared__ TeamLds<W> lds_all[kTeams];
+    const int lane = threadIdx.x & 63, tid = threadIdx.x % kTeam, wave = tid >> 6, team = threadIdx.x / kTeam;
+    TeamLds<W>& lds = lds_all[team];
+    const long long unit = (long long)blockIdx.x * kTeams + team;
+    const long long row = SPLIT ? unit / p.chunks : unit;
+    const int chunk = SPLIT ? (int)(unit - row * p.chunks) : 0;
+    if (row >= p.rows) return;  // (a team alone in its workgroup always has a row)
+    const int base = chunk * kChunk, n = min(kChunk, p.classes - base), top = p.top;
+    x += row * p.ld + base;
+
+    Words raw[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) raw[r] = load_words(x, r * kStep + tid * V, n, (r + 1) * kStep <= n);
+    // Between the passes over the registers: the values as fp32 (twice the registers of the 16-bit types) are made anew.
+    auto again = [&]() {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) asm volatile("" : "+v"(raw[r]));
         }
-        dx[j] = (T)out;
+    };
+    const int target = p.targets ? p.targets[row] : -1;
+    const bool given = target >= 0 && target < p.classes;
+    const int t = target - base;  // within the chunk, before it or behind it
+    const float xt = given ? (float)x[t] : 0.0f;
+    if (tid == 0) lds.count = 0;
+
+    // ---- the largest logit of the lane and of the wavefront
+    float lane_max = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) lane_max = fmaxf(lane_max, value<T>(raw[r], e));
+    Part part = {wave_max(lane_max), 0.0f, 0.0f, 0};
+    // ---- sums about it.  exp(x - m) as 2^((x - m) log2 e): the difference first, which is exact or small beside the rounding
+    // of x; a product with m would cost digits.  (x - m) is held above -200, where exp is 0 anyway: 0 times -inf is NaN.
+    const float m = part.m == -INFINITY ? 0.0f : part.m;
+    again();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = value<T>(raw[r], e) - m;
+            const float ex = __builtin_amdgcn_exp2f(d * kLog2e);
+            part.s += ex;
+            part.sx = __builtin_fmaf(ex, fmaxf(d, -200.0f), part.sx);
+        }
+    // ---- what goes before the given class: larger logits, and equal ones of lower index.  A slice of all lanes' r-th vectors
+    // lies before the class (equal ones count: above the next lower number), behind it, or around it.
+    if (p.rank && given) {
+        uint32_t o = ordered(xt) - 1;
+        if (o == 0x7fffffffu) --o;  // (no class has the key of -0)
+        const float below = logit_of((uint64_t)o << 32);
+        again();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int first = r * kStep;
+            if ((first <= t && t < first + kStep) || !(xt > -INFINITY)) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const int j = first + tid * V + e;
+                    const float v = value<T>(raw[r], e);
+                    part.before += (v > xt || (v == xt && j < t)) && j < n;
+                }
+            } else {
+                const float bound = first < t ? below : xt;
+#pragma unroll
+                for (int e = 0; e < V; ++e) part.before += value<T>(raw[r], e) > bound;
+            }
+        }
+        part.before = wave_sum_int(part.before);
+    }
+    part.s = wave_sum(part.s);
+    part.sx = wave_sum(part.sx);
+    if (W > 1 || top > 0) {
+        if (lane == 0) lds.part[wave] = part;
+        lds.lane_max[wave][lane] = lane_max;
+        team_sync<W>();
+    }
+    if constexpr (W > 1) {
+        float most = lds.part[0].m;
+#pragma unroll
+        for (int w = 1; w < W; ++w) most = fmaxf(most, lds.part[w].m);
+        part = {most, 0.0f, 0.0f, 0};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            Part q = lds.part[w];
+            rescale(q, most);
+            part.s += q.s;
+            part.sx += q.sx;
+            part.before += q.before;
+        }
+    }
+    const bool odd = part.s != part.s;  // a NaN, or infinity
+    if (odd && p.rank && given) {
+        int before = 0;
+        const uint64_t kt = key_of(xt, target);
+#pragma unroll 1
+        for (int j = tid; j < n; j += kTeam) before += key_of((float)x[j], base + j) > kt;
+        before = wave_sum_int(before);
+        team_sync<W>();
+        lds.waves[wave] = before;
+        team_sync<W>();
+        part.before = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) part.before += lds.waves[w];
+    }
+    const Answer answer(part);
+    if (tid == 0) {
+        if constexpr (SPLIT)
+            p.parts[unit] = part;
+        else
+            write_row(p, row, part, answer, given, xt);
+    }
+    if (top == 0) return;
+    auto emit = [&](int place, uint64_t key) {  // (keys within the chunk count their classes from its first)
+        if constexpr (SPLIT)
+            p.keys[unit * top + place] = key == 0 ? 0 : key_of(logit_of(key), class_of(key) + base);
+        else
+            write_top(p, row, answer, place, key);
+    };
+
+    // ---- the best classes
+    int count = kList + 1;
+    if (!odd) {
+        float group = lds.lane_max[0][lane];
+#pragma unroll
+        for (int w = 1; w < W; ++w) group = fmaxf(group, lds.lane_max[w][lane]);
+        int larger = 0;
+#pragma unroll
+        for (int l = 0; l < 64; ++l) larger += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(group), l)) > group;
+        const float bound = -wave_max(larger < top ? -group : -INFINITY);
+        auto gather = [&](auto wanted) {
+            again();
+            if (__builtin_amdgcn_ballot_w64(wanted(lane_max)) != 0) {
+                constexpr int kBits = R * V < 32 ? R * V : 32;
+#pragma unroll
+                for (int i = 0; i < R * V / kBits; ++i) {
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int k = kBits - 1; k >= 0; --k) bits = (bits << 1) | (wanted(value<T>(raw[(i * kBits + k) / V], (i * kBits + k) % V)) ? 1u : 0u);
+                    while (bits != 0) {
+                        const int k = i * kBits + __builtin_ctz(bits), j = k / V * kStep + tid * V + k % V;
+                        bits &= bits - 1;
+                        if (j < n) {
+                            const int at = atomicAdd(&lds.count, 1);
+                            if (at < kList) lds.list[at] = key_of((float)x[j], j);
+                        }
+                    }
+                }
+            }
+            team_sync<W>();
+            count = lds.count;
+        };
+        gather([&](float v) { return v >= bound; });
+        if (count > kList) {
+            team_sync<W>();
+            if (tid == 0) lds.count = 0;
+            team_sync<W>();
+            gather([&](float v) { return v > bound; });
+            if (count <= kList - kMaxTop) {
+                // ... and the first `top` of those equal to the bound, slice by slice, lane by lane
+                int found = 0;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (found < top) {
+                        int mine = 0;
+#pragma unroll
+                        for (int e = 0; e < V; ++e) mine += value<T>(raw[r], e) == bound && r * kStep + tid * V + e < n;
+                        int place = mine;  // becomes the number in lanes up to this one
+#pragma unroll
+                        for (int d = 1; d < 64; d <<= 1) {
+                            const int o = __shfl_up(place, d);
+                            if (lane >= d) place += o;
+                        }
+                        team_sync<W>();
+                        if (lane == 63) lds.waves[wave] = place;
+                        team_sync<W>();
+                        place += found - mine;
+#pragma unroll
+                        for (int w = 0; w < W; ++w) {
+                            if (w < wave) place += lds.waves[w];
+                            found += lds.waves[w];
+                        }
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            const int j = r * kStep + tid * V + e;
+                            if (value<T>(raw[r], e) == bound && j < n) {
+                                if (place < top) lds.list[count + place] = key_of(bound, j);
+                                ++place;
+                            }
+                        }
+                    }
+                }
+                count += min(found, top);
+                team_sync<W>();
+            }
+        }
+    }
+    if (count <= kList) {
+        for (int i = tid; i < count; i += kTeam) {
+            const uint64_t key = lds.list[i];
+            int place = 0;
+            for (int k = 0; k < count; ++k) place += lds.list[k] > key;
+            if (place < top) emit(place, key);
+        }
+        if constexpr (SPLIT)
+            for (int i = count + tid; i < top; i += kTeam) emit(i, 0);
+        return;
+    }
+    uint64_t last = ~0ull;
+#pragma unroll 1
+    for (int i = 0; i < top; ++i) {
+        uint64_t best = 0;
+#pragma unroll 1
+        for (int j = tid; j < n; j += kTeam) {
+            const uint64_t key = key_of((float)x[j], j);
+            if (key < last) best = max(best, key);
+        }
+        best = wave_max_key(best);
+        if constexpr (W > 1) {
+            team_sync<W>();
+            lds.best[wave] = best;
+            team_sync<W>();
+#pragma unroll
+            for (int w = 0; w < W; ++w) best = max(best, lds.best[w]);
+        }
+        if (tid == 0) emit(i, best);
+        last = best;
+    }
+}
+
+// Rows in several chunks: a wavefront a row.  The same way to the best keys: the k-th largest of the lanes' largest bounds them.
+constexpr int kJoinRows = 4;
+template <typename T>
+__global__ __launch_bounds__(64 * kJoinRows) void logprobs_join_kernel(const T* __restrict__ x, const LogProbsParams p) {
+    __shared__ uint64_t lists[kJoinRows][kList];
+    __shared__ int counts[kJoinRows];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long row = (long long)blockIdx.x * kJoinRows + wave;
+    if (row >= p.rows) return;
+    const uint64_t* keys = p.keys + row * p.chunks * p.top;
+    const int total = p.chunks * p.top;
+    uint64_t best = 0;
+    for (int i = lane; i < total; i += 64) best = max(best, keys[i]);
+    Part part = {-INFINITY, 0.0f, 0.0f, 0};
+    for (int c = lane; c < p.chunks; c += 64) {
+        Part q = p.parts[row * p.chunks + c];
+        const float m = fmaxf(part.m, q.m);
+        rescale(part, m);
+        rescale(q, m);
+        part.s += q.s;
+        part.sx += q.sx;
+        part.before += q.before;
+    }
+    rescale(part, wave_max(part.m));
+    part.s = wave_sum(part.s);
+    part.sx = wave_sum(part.sx);
+    part.before = wave_sum_int(part.before);
+    const Answer answer(part);
+    if (lane == 0) {
+        const int t = p.targets ? p.targets[row] : -1;
+        const bool given = t >= 0 && t < p.classes;
+        write_row(p, row, part, answer, given, given ? (float)x[row * p.ld + t] : 0.0f);
+        counts[wave] = 0;
+    }
+    if (p.top == 0) return;
+    int larger = 0;
+#pragma unroll
+    for (int l = 0; l < 64; ++l) larger += lane_key(best, l) > best;
+    // (keys differ, but for those that stand for nothing: 0)
+    const uint64_t bound = max((uint64_t)1, ~wave_max_key(larger < p.top ? ~best : 0));
+    team_sync<1>();
+    for (int i = lane; i < total; i += 64) {
+        const uint64_t key = keys[i];
+        if (key >= bound) {
+            const int at = atomicAdd(&counts[wave], 1);
+            if (at < kList) lists[wave][at] = key;
+        }
+    }
+    team_sync<1>();
+    const int count = counts[wave];
+    if (count <= kList) {
+        for (int i = lane; i < count; i += 64) {
+            const uint64_t key = lists[wave][i];
+            int place = 0;
+            for (int k = 0; k < count; ++k) place += lists[wave][k] > key;
+            if (place < p.top) write_top(p, row, answer, place, key);
+        }
+        return;
+    }
+    uint64_t last = ~0ull;
+    for (int i = 0; i < p.top; ++i) {
+        best = 0;
+        for (int k = lane; k < total; k += 64)
+            if (keys[k] < last) best = max(best, keys[k]);
+        last = wave_max_key(best);
+        if (lane == 0) write_top(p, row, answer, i, last);
+    }
+}
+
+// How a row is shared: whole rows while a team's registers hold them; longer ones, and rows too few to fill the chip, in
+// chunks.
+struct Shape {
+    int w, r, chunks;
+};
+inline Shape shape_of(long long rows, int classes, int per_vector) {
+    const int vectors = (classes + per_vector - 1) / per_vector;
+    auto chunks = [&](int r) { return (vectors + 256 * r - 1) / (256 * r); };
+    if (vectors <= 64) return {1, 1, 1};
+    if (vectors <= 128) return {1, 2, 1};
+    if (vectors <= 256) return {1, 4, 1};
+    if (vectors <= 1024 || rows * chunks(16) < 2 * kComputeUnits) return {4, 4, chunks(4)};
+    if (vectors <= 2048) return {4, 8, 1};
+    return {4, 16, chunks(16)};
+}
+template <typename F>
+void by_shape(const Shape& s, F&& f) {
+    using std::integral_constant;
+    if (s.w == 1 && s.r == 1) return f(integral_constant<int, 1>(), integral_constant<int, 1>());
+    if (s.w == 1 && s.r == 2) return f(integral_constant<int, 1>(), integral_constant<int, 2>());
+    if (s.w == 1) return f(integral_constant<int, 1>(), integral_constant<int, 4>());
+    if (s.r == 4) return f(integral_constant<int, 4>(), integral_constant<int, 4>());
+    if (s.r == 8) return f(integral_constant<int, 4>(), integral_constant<int, 8>());
+    return f(integral_constant<int, 4>(), integral_constant<int, 16>());
+}
+
+// ---- gradient.  Bound by memory: a workgroup a piece of a row, four vectors of 16 bytes a thread, all requested first.
+constexpr int kGradThreads = 256, kGradVectors = 4;
+
+template <typename T>
+__global__ __launch_bounds__(kGradThreads) void logprobs_grad_kernel(const T* x, const int32_t* __restrict__ targets,
+                                                                     const float* __restrict__ logsumexp,
+                                                                     const float* __restrict__ entropy,
+                                                                     const float* __restrict__ g_logprob,
+                                                                     const float* __restrict__ g_entropy, T* dx, int n, int pieces,
+                                                                     long long x_ld, long long dx_ld) {
+    constexpr int V = Elem<T>::kVec, kStep = kGradThreads * V, kPiece = kGradVectors * kStep;
+    const long long row = blockIdx.x / (unsigned)pieces;
+    const int base = (int)(blockIdx.x - (unsigned)row * pieces) * kPiece, left = n - base;
+    x += row * x_ld + base;
+    dx += row * dx_ld + base;
+    Words raw[kGradVectors];
+#pragma unroll
+    for (int r = 0; r < kGradVectors; ++r) raw[r] = load_words((const T*)x, r * kStep + threadIdx.x * V, left, (r + 1) * kStep <= left);
+    const float lse = logsumexp[row];
+    const int target = g_logprob ? targets[row] : -1, t = target - base;
+    const float g = target >= n ? NAN : (target >= 0 ? g_logprob[row] : 0.0f);
+    const float ge = g_entropy ? g_entropy[row] : 0.0f, h = g_entropy ? entropy[row] : 0.0f;
+    const bool none = lse == -INFINITY;  // no allowed class: no distribution, no gradient
+    // -p (g + ge (log p + h)), and g for the given class.  log p is held above -200, where p is 0 anyway.
+    const float c0 = none ? (g != g ? g : 0.0f) : __builtin_fmaf(ge, h, g), c1 = none ? 0.0f : ge, shift = none ? 0.0f : lse;
+#pragma unroll
+    for (int r = 0; r < kGradVectors; ++r) {
+        const int j = r * kStep + threadIdx.x * V;
+        if (j >= left) break;
+        float out[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float lp = value<T>(raw[r], e) - shift;
+            const float prob = __builtin_amdgcn_exp2f(lp * kLog2e);
+            out[e] = -prob * __builtin_fmaf(c1, fmaxf(lp, -200.0f), c0);
+        }
+        if (j <= t && t < j + V) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (j + e == t && !none) out[e] += g;
+        }
+        if (j + V <= left) {
+            Vec<T> v;
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = (T)out[e];
+            store_vec(dx + j, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (j + e < left) dx[j + e] = (T)out[e];
+        }
     }
 }
 
@@ -141,7 +519,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_grad_kernel(const T* x, con
 using namespace tcbnn;
 using namespace tcbnn::head;
 
-extern "C" size_t tcbnn_logprobs_workspace_bytes(int rows, int classes, int top, int dtype) { return 0; }
+extern "C" size_t tcbnn_logprobs_workspace_bytes(int rows, int classes, int top, int dtype) {
+    if (rows <= 0 || classes <= 0 || top < 0 || top > kMaxTop || !dtype_known(dtype)) return 0;
+    const Shape s = shape_of(rows, classes, (int)(16 / dtype_bytes(dtype)));
+    return s.chunks == 1 ? 0 : (size_t)rows * s.chunks * (sizeof(Part) + top * sizeof(uint64_t));
+}
 
 extern "C" int tcbnn_logprobs_forward(const tcbnn_logprobs_desc* d, void* stream) {
     TCBNN_NOTNULL(d);
@@ -153,11 +535,35 @@ extern "C" int tcbnn_logprobs_forward(const tcbnn_logprobs_desc* d, void* stream
     if (d->rows == 0) return TCBNN_OK;
     TCBNN_NOTNULL(d->logits);
     if (d->logprob || d->rank) TCBNN_NOTNULL(d->targets);
-    const LogProbsParams p = {d->targets, d->logprob, d->entropy, d->logsumexp, d->top_logprob, d->rank, d->top_index, d->classes,
-                              d->top_index || d->top_logprob ? d->top : 0, ld};
-    by_dtype(d->dtype, [&](auto t) {
-        using T = decltype(t);
-        hipLaunchKernelGGL(logprobs_kernel<T>, dim3((unsigned)d->rows), dim3(kThreads), 0, (hipStream_t)stream, (const T*)d->logits, p);
+    const int top = d->top_index || d->top_logprob ? d->top : 0;
+    const Shape shape = shape_of(d->rows, d->classes, (int)(16 / dtype_bytes(d->dtype)));
+    const long long units = (long long)d->rows * shape.chunks;
+    TCBNN_REQUIRE(units <= 0x7fffffffLL, "logprobs: grid too large");
+    LogProbsParams p = {d->targets, d->logprob, d->entropy, d->logsumexp, d->top_logprob, d->rank, d->top_index, d->rows, d->classes, top,
+                        shape.chunks, ld, nullptr, nullptr};
+    if (shape.chunks > 1) {
+        TCBNN_NOTNULL(d->workspace);
+        TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_logprobs_workspace_bytes(d->rows, d->classes, top, d->dtype), "logprobs: workspace too small");
+        TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "logprobs: the workspace is not aligned to 16 bytes");
+        p.parts = (Part*)d->workspace;
+        p.keys = (uint64_t*)(p.parts + units);
+    }
+    by_dtype(d->dtype, [&](auto e) {
+        using T = decltype(e);
+        by_shape(shape, [&](auto w, auto r) {
+            constexpr int W = w.value, R = r.value, kTeams = team_threads(W) / (64 * W);
+            const dim3 grid((unsigned)((units + kTeams - 1) / kTeams));
+            if constexpr (W > 1)
+                if (shape.chunks > 1) {
+                    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_kernel<T, W, R, true>), grid, dim3(team_threads(W)), 0, (hipStream_t)stream,
+                                       (const T*)d->logits, p);
+                    hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)((d->rows + kJoinRows - 1) / kJoinRows)), dim3(64 * kJoinRows),
+                                       0, (hipStream_t)stream, (const T*)d->logits, p);
+                    return;
+                }
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_kernel<T, W, R, false>), grid, dim3(team_threads(W)), 0, (hipStream_t)stream,
+                               (const T*)d->logits, p);
+        });
     });
     TCBNN_LAUNCH_CHECK("logprobs_kernel");
     return TCBNN_OK;
@@ -176,11 +582,14 @@ extern "C" int tcbnn_logprobs_backward(const tcbnn_logprobs_grad_desc* d, void* 
     if (d->grad_logprob) TCBNN_NOTNULL(d->targets);
     if (d->grad_entropy) TCBNN_NOTNULL(d->entropy);
     TCBNN_REQUIRE(d->grad_logits != d->logits || d->rows == 1 || x_ld == dx_ld, "logprobs: a gradient over the logits has their stride");
+    const long long piece = kGradThreads * kGradVectors * (long long)(16 / dtype_bytes(d->dtype));
+    const long long pieces = (d->classes + piece - 1) / piece;
+    TCBNN_REQUIRE(pieces * d->rows <= 0x7fffffffLL, "logprobs: grid too large");
     by_dtype(d->dtype, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(logprobs_grad_kernel<T>, dim3((unsigned)d->rows), dim3(kThreads), 0, (hipStream_t)stream,
+        hipLaunchKernelGGL(logprobs_grad_kernel<T>, dim3((unsigned)(pieces * d->rows)), dim3(kGradThreads), 0, (hipStream_t)stream,
                            (const T*)d->logits, d->targets, d->logsumexp, d->entropy, d->grad_logprob, d->grad_entropy,
-                           (T*)d->grad_logits, d->classes, x_ld, dx_ld);
+                           (T*)d->grad_logits, d->classes, (int)pieces, x_ld, dx_ld);
     });
     TCBNN_LAUNCH_CHECK("logprobs_grad_kernel");
     return TCBNN_OK;
