@@ -11,7 +11,7 @@ namespace {
 using namespace head;
 
 constexpr int kMaxTop = 64;
-constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 
 // The order of classes as one number: larger logits first (NaN before all, -0 with +0), lower indices first among equals.
 // Larger keys come first; 0 is below every class's key.
@@ -36,21 +36,46 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
 }
 __device__ __forceinline__ int wave_sum_int(int v) { return (int)wave_reduce((uint32_t)v, [](uint32_t a, uint32_t b) { return a + b; }); }
 
-// 16 bytes of logits as they lie in memory, -inf in the place of those past the end.  They are kept as words: the compiler
-// keeps elements that come out of a branch in a register each.
+// 16 bytes of logits as they lie in memory (as words: the compiler keeps elements that come out of a branch in a register each).
 typedef int Words __attribute__((ext_vector_type(4)));
 template <typename T>
-__device__ __forceinline__ Words load_words(const T* x, int j, int n, bool whole) {
-    constexpr int V = Elem<T>::kVec;
-    if (whole || j + V <= n) return __builtin_bit_cast(Words, load_vec(x + j));
+__device__ __forceinline__ Words load_words(const T* x) {
+    return __builtin_bit_cast(Words, load_vec(x));
+}
+// n < V logits, -inf in the place of the others
+template <typename T>
+__device__ __forceinline__ Words load_rest(const T* x, int n) {
     Vec<T> v;
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = j + e < n ? x[j + e] : (T)-INFINITY;
+    for (int e = 0; e < Elem<T>::kVec; ++e) v[e] = e < n ? x[e] : (T)-INFINITY;
     return __builtin_bit_cast(Words, v);
+}
+// `kR` vectors of the n logits at x, the r-th one at (r * lanes + lane) V; -inf past the end.  Where the logits end within a
+// vector, all lanes read that one, and the lane that it belongs to takes it.
+template <typename T, int kR>
+__device__ __forceinline__ void load_slices(const T* x, int n, int lane, int lanes, Words (&raw)[kR]) {
+    constexpr int V = Elem<T>::kVec;
+    const Words none = load_rest(x, 0);
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+        const int j = (r * lanes + lane) * V;
+        raw[r] = none;
+        if ((r + 1) * lanes * V <= n || j + V <= n) raw[r] = load_words(x + j);
+    }
+    if (n % V != 0) {
+        const int last = n / V;
+        const Words rest = load_rest(x + last * V, n % V);
+#pragma unroll
+        for (int r = 0; r < kR; ++r)
+            if (r * lanes + lane == last) raw[r] = rest;
+    }
 }
 template <typename T>
 __device__ __forceinline__ float value(const Words& w, int e) {
-    return (float)__builtin_bit_cast(Vec<T>, w)[e];
+    if constexpr (std::is_same_v<T, __bf16>)  // (of a conversion the compiler makes maxima in bf16, which take four instructions)
+        return __uint_as_float(e & 1 ? (uint32_t)w[e / 2] & 0xffff0000u : (uint32_t)w[e / 2] << 16);
+    else
+        return (float)__builtin_bit_cast(Vec<T>, w)[e];
 }
 
 // What is known of a set of logits: the largest, sums of exp(x - m) and of (x - m) exp(x - m), how many go before the given
@@ -144,66 +169,67 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
     x += row * p.ld + base;
 
     Words raw[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) raw[r] = load_words(x, r * kStep + tid * V, n, (r + 1) * kStep <= n);
-    // Between the passes over the registers: the values as fp32 (twice the registers of the 16-bit types) are made anew.
-    auto again = [&]() {
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) asm volatile("" : "+v"(raw[r]));
-        }
-    };
+    load_slices<T, R>(x, n, tid, kTeam, raw);
     const int target = p.targets ? p.targets[row] : -1;
     const bool given = target >= 0 && target < p.classes;
     const int t = target - base;  // within the chunk, before it or behind it
     const float xt = given ? (float)x[t] : 0.0f;
     if (tid == 0) lds.count = 0;
 
-    // ---- the largest logit of the lane and of the wavefront
-    float lane_max = -INFINITY;
+    // ---- the largest logit of each vector, of the lane, of the wavefront
+    float vec_max[R], lane_max = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+        vec_max[r] = value<T>(raw[r], 0);
 #pragma unroll
-        for (int e = 0; e < V; ++e) lane_max = fmaxf(lane_max, value<T>(raw[r], e));
+        for (int e = 1; e < V; ++e) vec_max[r] = fmaxf(vec_max[r], value<T>(raw[r], e));
+        lane_max = fmaxf(lane_max, vec_max[r]);
+    }
     Part part = {wave_max(lane_max), 0.0f, 0.0f, 0};
-    // ---- sums about it.  exp(x - m) as 2^((x - m) log2 e): the difference first, which is exact or small beside the rounding
-    // of x; a product with m would cost digits.  (x - m) is held above -200, where exp is 0 anyway: 0 times -inf is NaN.
-    const float m = part.m == -INFINITY ? 0.0f : part.m;
-    again();
+    // ---- sums about it, and what goes before the given class.
+    // exp(x - m) = 2^u, u = x log2 e - c with c = m log2 e rounded: one fused multiply-add, as exact as a difference of x and
+    // m, but about c.  `off`, what c was rounded by, takes the sums back to m.  u is held above -250, where 2^u is 0 anyway: 0
+    // times -inf is NaN.
+    // Before the class go larger logits and equal ones of lower index: whole vectors below it compare with the next lower
+    // number, the equal ones in the class's own vector are counted afterwards.
+    const float m = part.m == -INFINITY ? 0.0f : part.m, c = m * kLog2e, off = __builtin_fmaf(m, kLog2e, -c);
+    uint32_t lower = ordered(xt) - 1;
+    if (lower == 0x7fffffffu) --lower;  // (no class has the key of -0)
+    const float below = logit_of((uint64_t)lower << 32);
+    uint32_t signs = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+        const float bound = r * kStep + tid * V + V <= t ? below : xt;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float d = value<T>(raw[r], e) - m;
-            const float ex = __builtin_amdgcn_exp2f(d * kLog2e);
+            const float v = value<T>(raw[r], e);
+            const float u = __builtin_fmaf(v, kLog2e, -c);
+            const float ex = __builtin_amdgcn_exp2f(u);
             part.s += ex;
-            part.sx = __builtin_fmaf(ex, fmaxf(d, -200.0f), part.sx);
+            part.sx = __builtin_fmaf(ex, fmaxf(u, -250.0f), part.sx);
+            // the sign of bound - v, shifted in from below (comparisons write a scalar, which the addition then waits for)
+            signs = __builtin_amdgcn_alignbit(signs, __float_as_uint(bound - v), 31);
         }
-    // ---- what goes before the given class: larger logits, and equal ones of lower index.  A slice of all lanes' r-th vectors
-    // lies before the class (equal ones count: above the next lower number), behind it, or around it.
-    if (p.rank && given) {
-        uint32_t o = ordered(xt) - 1;
-        if (o == 0x7fffffffu) --o;  // (no class has the key of -0)
-        const float below = logit_of((uint64_t)o << 32);
-        again();
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int first = r * kStep;
-            if ((first <= t && t < first + kStep) || !(xt > -INFINITY)) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const int j = first + tid * V + e;
-                    const float v = value<T>(raw[r], e);
-                    part.before += (v > xt || (v == xt && j < t)) && j < n;
-                }
-            } else {
-                const float bound = first < t ? below : xt;
-#pragma unroll
-                for (int e = 0; e < V; ++e) part.before += value<T>(raw[r], e) > bound;
-            }
-        }
-        part.before = wave_sum_int(part.before);
+        if ((r + 1) * V % 32 == 0 || r == R - 1) part.before += __popc(signs);
+        // Vector after vector, the values as fp32 made anew: all at once, as the compiler likes it, takes twice the registers.
+        asm volatile("" : "+v"(part.s), "+v"(part.sx), "+v"(signs));
+        if (r + 1 < R) asm volatile("" : "+v"(raw[r + 1]));
+        __builtin_amdgcn_sched_barrier(0);
     }
+    if (fabsf(m) > 1e38f) {  // log2 e times that is infinite; neighbours are so far apart that only equal logits count
+        const float one = m < INFINITY ? 1.0f : NAN;
+        part.s = part.sx = 0.0f;
+#pragma unroll 1
+        for (int j = tid; j < n; j += kTeam) {
+            const float v = (float)x[j];
+            part.s += v == m ? one : (v != v ? v : 0.0f);
+        }
+    } else {
+        part.sx = __builtin_fmaf(-off, part.s, part.sx) * kLn2;
+        part.s = __builtin_fmaf(-off * kLn2, part.s, part.s);
+    }
+    if (wave == 0 && t >= 0 && t < n && lane < t % V) part.before += (float)x[t - 1 - lane] == xt;
+    part.before = wave_sum_int(part.before);
     part.s = wave_sum(part.s);
     part.sx = wave_sum(part.sx);
     if (W > 1 || top > 0) {
@@ -226,7 +252,7 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
         }
     }
     const bool odd = part.s != part.s;  // a NaN, or infinity
-    if (odd && p.rank && given) {
+    if (given && (odd || !(below > -INFINITY))) {  // what differences of floats do not order
         int before = 0;
         const uint64_t kt = key_of(xt, target);
 #pragma unroll 1
@@ -264,67 +290,50 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
 #pragma unroll
         for (int l = 0; l < 64; ++l) larger += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(group), l)) > group;
         const float bound = -wave_max(larger < top ? -group : -INFINITY);
-        auto gather = [&](auto wanted) {
-            again();
-            if (__builtin_amdgcn_ballot_w64(wanted(lane_max)) != 0) {
-                constexpr int kBits = R * V < 32 ? R * V : 32;
-#pragma unroll
-                for (int i = 0; i < R * V / kBits; ++i) {
-                    uint32_t bits = 0;
-#pragma unroll
-                    for (int k = kBits - 1; k >= 0; --k) bits = (bits << 1) | (wanted(value<T>(raw[(i * kBits + k) / V], (i * kBits + k) % V)) ? 1u : 0u);
-                    while (bits != 0) {
-                        const int k = i * kBits + __builtin_ctz(bits), j = k / V * kStep + tid * V + k % V;
-                        bits &= bits - 1;
-                        if (j < n) {
-                            const int at = atomicAdd(&lds.count, 1);
-                            if (at < kList) lds.list[at] = key_of((float)x[j], j);
-                        }
-                    }
-                }
-            }
-            team_sync<W>();
-            count = lds.count;
+        auto push = [&](int j, float v) {
+            const int at = atomicAdd(&lds.count, 1);
+            if (at < kList) lds.list[at] = key_of(v, j);
         };
-        gather([&](float v) { return v >= bound; });
+        uint32_t hot = 0;  // the vectors that reach the bound: few, and read again (from the cache)
+#pragma unroll
+        for (int r = 0; r < R; ++r) hot |= vec_max[r] >= bound ? 1u << r : 0u;
+        while (hot != 0) {
+            const int j = __builtin_ctz(hot) * kStep + tid * V;
+            hot &= hot - 1;
+            const Words w = j + V <= n ? load_words(x + j) : load_rest(x + j, n - j);
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (value<T>(w, e) >= bound && j + e < n) push(j + e, value<T>(w, e));
+        }
+        team_sync<W>();
+        count = lds.count;
         if (count > kList) {
             team_sync<W>();
             if (tid == 0) lds.count = 0;
             team_sync<W>();
-            gather([&](float v) { return v > bound; });
+#pragma unroll 1
+            for (int j = tid; j < n; j += kTeam)
+                if ((float)x[j] > bound) push(j, (float)x[j]);
+            team_sync<W>();
+            count = lds.count;
             if (count <= kList - kMaxTop) {
-                // ... and the first `top` of those equal to the bound, slice by slice, lane by lane
+                // ... and the first `top` of those equal to the bound: 64 W in a row at a time
                 int found = 0;
+#pragma unroll 1
+                for (int first = 0; first < n && found < top; first += kTeam) {
+                    const int j = first + tid;
+                    const bool equal = j < n && (float)x[j] == bound;
+                    const uint64_t mask = __builtin_amdgcn_ballot_w64(equal);
+                    team_sync<W>();
+                    if (lane == 0) lds.waves[wave] = __popcll(mask);
+                    team_sync<W>();
+                    int place = found + __popcll(mask & ((1ull << lane) - 1));
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    if (found < top) {
-                        int mine = 0;
-#pragma unroll
-                        for (int e = 0; e < V; ++e) mine += value<T>(raw[r], e) == bound && r * kStep + tid * V + e < n;
-                        int place = mine;  // becomes the number in lanes up to this one
-#pragma unroll
-                        for (int d = 1; d < 64; d <<= 1) {
-                            const int o = __shfl_up(place, d);
-                            if (lane >= d) place += o;
-                        }
-                        team_sync<W>();
-                        if (lane == 63) lds.waves[wave] = place;
-                        team_sync<W>();
-                        place += found - mine;
-#pragma unroll
-                        for (int w = 0; w < W; ++w) {
-                            if (w < wave) place += lds.waves[w];
-                            found += lds.waves[w];
-                        }
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const int j = r * kStep + tid * V + e;
-                            if (value<T>(raw[r], e) == bound && j < n) {
-                                if (place < top) lds.list[count + place] = key_of(bound, j);
-                                ++place;
-                            }
-                        }
+                    for (int w = 0; w < W; ++w) {
+                        if (w < wave) place += lds.waves[w];
+                        found += lds.waves[w];
                     }
+                    if (equal && place < top) lds.list[count + place] = key_of(bound, j);
                 }
                 count += min(found, top);
                 team_sync<W>();
@@ -475,8 +484,7 @@ __global__ __launch_bounds__(kGradThreads) void logprobs_grad_kernel(const T* x,
     x += row * x_ld + base;
     dx += row * dx_ld + base;
     Words raw[kGradVectors];
-#pragma unroll
-    for (int r = 0; r < kGradVectors; ++r) raw[r] = load_words((const T*)x, r * kStep + threadIdx.x * V, left, (r + 1) * kStep <= left);
+    load_slices<T, kGradVectors>(x, min(left, kPiece), threadIdx.x, kGradThreads, raw);
     const float lse = logsumexp[row];
     const int target = g_logprob ? targets[row] : -1, t = target - base;
     const float g = target >= n ? NAN : (target >= 0 ? g_logprob[row] : 0.0f);
