@@ -1,5 +1,8 @@
 // Linear layers and their gradients (tcbnn_linear_forward / _backward):  z = x w^T + b,  y = act(z) + r;
 // dz = dy act'(z),  dx = dz w,  dw = dz^T x,  db = column sums of dz.
+//
+// All three products are one kernel: c[i][j] = sum over s of I(i, s) J(j, s), where an operand lies in memory either along the
+// sum (x and w of the forward product: rows of s) or across it (w of dx, dz and x of dw: a row for every s).
 #include "head.h"
 
 namespace tcbnn {
@@ -7,9 +10,9 @@ namespace {
 
 using namespace head;
 
-constexpr int kTile = 64, kDepth = 16, kThreads = 256;
-constexpr int kMaxIn = 1 << 20;
+constexpr int kMaxIn = 1 << 20, kMaxOut = 1 << 28;
 
+// ---- activations
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
     if constexpr (ACT == TCBNN_ACT_RELU) return z > 0.0f || z != z ? z : 0.0f;
@@ -29,65 +32,360 @@ __device__ __forceinline__ float slope(float z) {
     return 1.0f;
 }
 template <typename F>
-void by_activation(int act, F&& f) {
+__host__ __device__ __forceinline__ void by_activation(int act, F&& f) {
     if (act == TCBNN_ACT_RELU) return f(std::integral_constant<int, TCBNN_ACT_RELU>());
     if (act == TCBNN_ACT_GELU) return f(std::integral_constant<int, TCBNN_ACT_GELU>());
     if (act == TCBNN_ACT_SILU) return f(std::integral_constant<int, TCBNN_ACT_SILU>());
     return f(std::integral_constant<int, TCBNN_ACT_NONE>());
 }
 
-// c[i][j] = epilogue(sum over k of a(i, k) b(j, k)), operands anywhere: a(i, k) = a[i * a_i + k * a_k]
-struct ProductParams {
-    long long m, n, k, a_i, a_k, b_i, b_k;
-    const float* bias;
-    const void* residual;
-    void* out;
-    void* preact;
-    long long residual_ld, out_ld, preact_ld;
-};
-
-template <typename T, int ACT>
-__global__ __launch_bounds__(kThreads) void product_kernel(const T* __restrict__ a, const T* __restrict__ b, const ProductParams p) {
-    __shared__ float la[kDepth][kTile + 1], lb[kDepth][kTile + 1];
-    const int tid = threadIdx.x, ti = tid >> 4, tj = tid & 15;
-    const long long i0 = (long long)blockIdx.y * kTile, j0 = (long long)blockIdx.x * kTile;
-    float acc[4][4] = {};
-    for (long long k0 = 0; k0 < p.k; k0 += kDepth) {
-        __syncthreads();
-        for (int e = tid; e < kTile * kDepth; e += kThreads) {
-            const int ra = p.a_k == 1 ? e / kDepth : e % kTile, ka = p.a_k == 1 ? e % kDepth : e / kTile;
-            la[ka][ra] = i0 + ra < p.m && k0 + ka < p.k ? (float)a[(i0 + ra) * p.a_i + (k0 + ka) * p.a_k] : 0.0f;
-            const int rb = p.b_k == 1 ? e / kDepth : e % kTile, kb = p.b_k == 1 ? e % kDepth : e / kTile;
-            lb[kb][rb] = j0 + rb < p.n && k0 + kb < p.k ? (float)b[(j0 + rb) * p.b_i + (k0 + kb) * p.b_k] : 0.0f;
-        }
-        __syncthreads();
+// ---- matrix instructions.  16 bytes of a row or column of each operand are one instruction's share of a lane in the 16-bit types
+// (32 x 32, 16 of the sum) and four instructions' in fp32 (32 x 32, 2 of the sum each).  Lane l holds row l % 32 of its operand,
+// half l / 32 of the sum.  Accumulator register v of lane l is row 8 (v / 4) + 4 (l / 32) + v % 4 of the first operand and row
+// l % 32 of the second: with J first a lane holds runs of four neighbouring j.
+typedef int Words __attribute__((ext_vector_type(4)));
+typedef float Acc __attribute__((ext_vector_type(16)));
+template <typename T>
+__device__ __forceinline__ Acc mma(Words j, Words i, Acc c) {
+    if constexpr (std::is_same_v<T, __bf16>) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Vec<__bf16>, j), __builtin_bit_cast(Vec<__bf16>, i), c, 0, 0, 0);
+    } else if constexpr (std::is_same_v<T, _Float16>) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(Vec<_Float16>, j), __builtin_bit_cast(Vec<_Float16>, i), c, 0, 0, 0);
+    } else {
 #pragma unroll
-        for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) acc[u][v] = __builtin_fmaf(la[k][ti + 16 * u], lb[k][tj + 16 * v], acc[u][v]);
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__int_as_float(j[e]), __int_as_float(i[e]), c, 0, 0, 0);
+        return c;
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const long long i = i0 + ti + 16 * u, j = j0 + tj + 16 * v;
-            if (i >= p.m || j >= p.n) continue;
-            const float z = acc[u][v] + (p.bias ? p.bias[j] : 0.0f);
-            if (p.preact) ((T*)p.preact)[i * p.preact_ld + j] = (T)z;
-            float y = activate<ACT>(z);
-            if (p.residual) y += (float)((const T*)p.residual)[i * p.residual_ld + j];
-            ((T*)p.out)[i * p.out_ld + j] = (T)y;
-        }
 }
 
+// ---- an operand's tiles.  A step of the sum is 128 bytes of a row (64 elements of 16 bits, 32 of fp32); a tile is `ROWS` rows
+// (i or j) of a step, in LDS in pieces of 16 bytes as it lies in memory:
+//   along the sum:  [ROWS][8 pieces], piece c of row r at place c ^ (r % 8): the 64 lanes of a fragment read 32 rows at once;
+//   across the sum: [64 or 32 steps][ROWS elements], pieces exchanged so that the rows which one instruction reads lie in
+//                   different banks.  A fragment then is two transposing reads of four elements (16 bits), or four of one.
+typedef __attribute__((address_space(3))) void LdsVoid;
+constexpr int kStepBytes = 128;
+constexpr int kOutOfRange = (int)0x80000000u;  // (a request there touches no memory and returns 0)
+
+struct Operand {
+    const void* p;
+    long long ld;  // elements between rows in memory
+};
+
+template <typename T, int ROWS, bool ACROSS, bool ALIGNED, int THREADS>
+struct Tile {
+    static constexpr int V = Elem<T>::kVec, kSteps = kStepBytes / (int)sizeof(T);
+    static constexpr int kBytes = ROWS * kStepBytes, kPieces = kBytes / 16, kEach = kPieces / THREADS;
+    static constexpr int kRowPieces = ACROSS ? ROWS / V : 8;  // pieces of a row as LDS holds them
+    static_assert(kEach * THREADS == kPieces, "whole pieces a thread");
+
+    const T* base;
+    int offset[kEach];  // bytes from the tile's first element in memory, at the first step
+    Words held[ALIGNED ? 1 : kEach];
+    long long ld;
+    int valid;  // rows of the tile that exist
+
+    static __device__ __forceinline__ int swizzle(int row) {
+        if constexpr (!ACROSS) return row & 7;
+        if constexpr (sizeof(T) == 4) return ((row >> 2) & 1) << 3;
+        if constexpr (kRowPieces >= 16) return (row & 3) << 2;
+        return ((row >> 1) & 1) << 2;
+    }
+    // thread's e-th piece: its row and piece in memory
+    static __device__ __forceinline__ void where(int e, int& row, int& piece) {
+        const int at = e * THREADS + (int)threadIdx.x;
+        row = at / kRowPieces;
+        piece = (at % kRowPieces) ^ swizzle(row);
+    }
+    // rows first .. of `total` rows (i or j)
+    __device__ __forceinline__ void init(const Operand& o, long long first, long long total) {
+        ld = o.ld;
+        valid = (int)min((long long)ROWS, total - first);
+        base = (const T*)o.p + (ACROSS ? first : first * ld);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            int row, piece;
+            where(e, row, piece);
+            // what lies past the last row is some other row's: nothing of it is kept
+            if constexpr (ACROSS)
+                offset[e] = (int)(row * ld + (piece * V < valid ? piece * V : 0)) * (int)sizeof(T);
+            else
+                offset[e] = (int)(min(row, valid - 1) * ld + piece * V) * (int)sizeof(T);
+        }
+    }
+    // requests the tile of the step that begins at `s` of `sum` (into LDS at once, or into registers)
+    __device__ __forceinline__ void request(char* lds, int s, int sum) {
+        const bool whole = s + kSteps <= sum;
+        if constexpr (ALIGNED) {
+            const __amdgpu_buffer_rsrc_t r =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(ACROSS ? base + s * ld : base), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                int row, piece;
+                where(e, row, piece);
+                const bool there = whole || s + (ACROSS ? row : piece * V) < sum;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(lds + (e * THREADS + wave_first()) * 16), 16,
+                                                         there ? offset[e] : kOutOfRange, ACROSS ? 0 : s * (int)sizeof(T), 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                int row, piece;
+                where(e, row, piece);
+                held[e] = Words{0, 0, 0, 0};
+                if constexpr (ACROSS) {
+                    const T* p = base + (s + row) * ld + piece * V;
+                    if (s + row < sum) held[e] = take(p, valid - piece * V);
+                } else {
+                    const T* p = base + min(row, valid - 1) * ld + s + piece * V;
+                    held[e] = take(p, sum - (s + piece * V));
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ Words take(const T* p, int n) {
+        if (n >= V) return __builtin_bit_cast(Words, load_vec(p));
+        Vec<T> v;
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = k < n ? p[k] : (T)0.0f;
+        return __builtin_bit_cast(Words, v);
+    }
+    static __device__ __forceinline__ int wave_first() { return __builtin_amdgcn_readfirstlane(threadIdx.x & ~63); }
+    __device__ __forceinline__ void store(char* lds) const {
+        if constexpr (!ALIGNED) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) *reinterpret_cast<Words*>(lds + (e * THREADS + (int)threadIdx.x) * 16) = held[e];
+        }
+    }
+    // the fragment of rows `first` .. `first` + 31, the k-th quarter of the step
+    static __device__ __forceinline__ Words fragment(const char* lds, int first, int k) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        if constexpr (!ACROSS) {
+            const int row = first + (lane & 31);
+            return *reinterpret_cast<const Words*>(lds + row * 128 + (((2 * k + h) ^ (lane & 7)) << 4));
+        } else if constexpr (sizeof(T) == 2) {
+            typedef short S4 __attribute__((ext_vector_type(4)));
+            typedef int I2 __attribute__((ext_vector_type(2)));
+            I2 half[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int row = 16 * k + 8 * h + 4 * q + ((lane >> 2) & 3), col = first + (lane & 16) + 4 * (lane & 3);
+                const char* at = lds + row * (ROWS * 2) + (((col >> 3) ^ swizzle(row)) << 4) + (col & 7) * 2;
+                half[q] = __builtin_bit_cast(I2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)at));
+            }
+            return Words{half[0][0], half[0][1], half[1][0], half[1][1]};
+        } else {
+            Words w;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = 8 * k + 4 * h + q, col = first + (lane & 31);
+                w[q] = *reinterpret_cast<const int*>(lds + row * (ROWS * 4) + (((col >> 2) ^ swizzle(row)) << 4) + (col & 3) * 4);
+            }
+            return w;
+        }
+    }
+};
+
+struct ProductParams {
+    Operand i, j;
+    int rows, cols, sum;  // c is rows x cols
+    int tiles_i, tiles_j, splits, split_sum;
+    int activation;
+    const float* bias;     // [cols], or NULL
+    const void* residual;  // or NULL
+    void* out;
+    void* preact;          // or NULL
+    long long residual_ld, out_ld, preact_ld;
+    float* partial;        // splits > 1: [splits][rows][cols]
+};
+
+// z of `n` <= kVec neighbouring columns of a row -> the outputs
+template <typename T>
+__device__ __forceinline__ void finish(const ProductParams& p, long long i, int j, const float* bias, float* z, int n) {
+    constexpr int V = Elem<T>::kVec;
+#pragma unroll
+    for (int e = 0; e < V; ++e) z[e] += bias[e];
+    auto put = [&](void* base, long long ld) {
+        T* to = (T*)base + i * ld + j;
+        if (n == V) {
+            Vec<T> v;
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = (T)z[e];
+            store_vec(to, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (e < n) to[e] = (T)z[e];
+        }
+    };
+    if (p.preact) put(p.preact, p.preact_ld);
+    by_activation(p.activation, [&](auto act) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[e] = activate<act.value>(z[e]);
+    });
+    if (p.residual) {
+        const T* r = (const T*)p.residual + i * p.residual_ld + j;
+        if (n == V) {
+            const Vec<T> v = load_vec(r);
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[e] += (float)v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (e < n) z[e] += (float)r[e];
+        }
+    }
+    put(p.out, p.out_ld);
+}
+
+// A workgroup's tile of c is BI x BJ, WI x WJ wavefronts with 32 x 32 pieces of it each.  Two tiles of each operand in LDS: the
+// next step is requested before the present one is multiplied.
+template <typename T, int BI, int BJ, int WI, int WJ, bool ACROSS_I, bool ACROSS_J, bool ALIGNED>
+__global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductParams p) {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves the stub out where it instantiates a tile's requests twice)
+    constexpr int kThreads = 64 * WI * WJ, NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec;
+    using TileI = Tile<T, BI, ACROSS_I, ALIGNED, kThreads>;
+    using TileJ = Tile<T, BJ, ACROSS_J, ALIGNED, kThreads>;
+    constexpr int kStage = TileI::kBytes + TileJ::kBytes;
+    // a wavefront's 32 rows of c on their way out, 16 bytes between rows
+    constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
+    constexpr int kLds = 2 * kStage > kOutWave * WI * WJ ? 2 * kStage : kOutWave * WI * WJ;
+    __shared__ __align__(1024) char lds[kLds];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // Workgroups go to the 8 XCDs in turn: each XCD gets a run of tiles, and a run covers 8 tiles of i after 8 tiles of i, so that what
+    // runs at one time on an XCD shares its operands' tiles in that XCD's L2.
+    const int tiles = p.tiles_i * p.tiles_j, units = tiles * p.splits;
+    const int xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
+    const int unit = xcd * (units / 8) + min(xcd, units % 8) + nth;
+    const int split = unit / tiles, tile = unit % tiles;
+    const int band = tile / (8 * p.tiles_j), in_band = tile % (8 * p.tiles_j), high = min(8, p.tiles_i - 8 * band);
+    const long long i0 = (long long)(8 * band + in_band % high) * BI, j0 = (long long)(in_band / high) * BJ;
+
+    TileI ti;
+    TileJ tj;
+    ti.init(p.i, i0, p.rows);
+    tj.init(p.j, j0, p.cols);
+    const int s0 = split * p.split_sum, s1 = min(p.sum, s0 + p.split_sum);
+    const int wi = wave / WJ * (32 * NI), wj = wave % WJ * (32 * NJ);
+
+    Acc acc[NI][NJ];
+#pragma unroll
+    for (int a = 0; a < NI; ++a)
+#pragma unroll
+        for (int b = 0; b < NJ; ++b)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.0f;
+
+    auto request = [&](int stage, int s) {
+        ti.request(lds + stage * kStage, s, s1);
+        tj.request(lds + stage * kStage + TileI::kBytes, s, s1);
+    };
+    auto arrived = [&](int stage) {
+        ti.store(lds + stage * kStage);
+        tj.store(lds + stage * kStage + TileI::kBytes);
+        __syncthreads();
+    };
+    if (s0 < s1) {
+        request(0, s0);
+        arrived(0);
+    }
+    int stage = 0;
+    for (int s = s0; s < s1; s += TileI::kSteps, stage ^= 1) {
+        const bool more = s + TileI::kSteps < s1;
+        if (more) request(stage ^ 1, s + TileI::kSteps);
+        const char* li = lds + stage * kStage;
+        const char* lj = li + TileI::kBytes;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            Words fi[NI], fj[NJ];
+#pragma unroll
+            for (int a = 0; a < NI; ++a) fi[a] = TileI::fragment(li, wi + 32 * a, k);
+#pragma unroll
+            for (int b = 0; b < NJ; ++b) fj[b] = TileJ::fragment(lj, wj + 32 * b, k);
+#pragma unroll
+            for (int a = 0; a < NI; ++a)
+#pragma unroll
+                for (int b = 0; b < NJ; ++b) acc[a][b] = mma<T>(fj[b], fi[a], acc[a][b]);
+        }
+        if (more)
+            arrived(stage ^ 1);
+        else
+            __syncthreads();
+    }
+
+    // ---- out: 32 rows of the wavefront at a time through LDS, so that a row leaves in whole runs of 64 bytes or more
+    char* mine = lds + wave * kOutWave;
+    constexpr int kPerRow = 32 * NJ / V, kRowsAtOnce = 64 / kPerRow;  // lanes to a row, rows at once
+    const int col = (lane % kPerRow) * V, j = (int)j0 + wj + col, n = min(V, p.cols - j);
+    float bias[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) bias[e] = p.bias && e < n ? p.bias[j + e] : 0.0f;
+#pragma unroll
+    for (int a = 0; a < NI; ++a) {
+#pragma unroll
+        for (int b = 0; b < NJ; ++b)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4*>(mine + (lane & 31) * kOutRow + (32 * b + 8 * g + 4 * (lane >> 5)) * 4) =
+                    make_float4(acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int r = 0; r < 32; r += kRowsAtOnce) {
+            const int row = r + lane / kPerRow;
+            const long long i = i0 + wi + 32 * a + row;
+            float z[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(mine + row * kOutRow + (col + e) * 4);
+                z[e] = q.x, z[e + 1] = q.y, z[e + 2] = q.z, z[e + 3] = q.w;
+            }
+            if (i < p.rows && n > 0) {
+                if (p.splits > 1) {
+                    float* to = p.partial + ((size_t)split * p.rows + i) * p.cols + j;
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (e < n) to[e] = z[e];
+                } else {
+                    finish<T>(p, i, j, bias, z, n);
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#endif
+}
+
+// the sums of all splits and what follows them
+template <typename T>
+__global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p) {
+    constexpr int V = Elem<T>::kVec;
+    const int per_row = (p.cols + V - 1) / V;
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x, i = at / per_row;
+    if (i >= p.rows) return;
+    const int j = (int)(at - i * per_row) * V, n = min(V, p.cols - j);
+    float z[V], bias[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        z[e] = 0.0f;
+        bias[e] = p.bias && e < n ? p.bias[j + e] : 0.0f;
+    }
+    for (int k = 0; k < p.splits; ++k) {
+        const float* from = p.partial + ((size_t)k * p.rows + i) * p.cols + j;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (e < n) z[e] += from[e];
+    }
+    finish<T>(p, i, j, bias, z, n);
+}
+
+constexpr int kColumnThreads = 256;
 // dz = dy act'(z) in the operands' type (nothing to write without an activation) and its column sums in fp32: a thread a
 // column, all rows in order
 template <typename T, int ACT>
-__global__ __launch_bounds__(kThreads) void dz_kernel(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz,
+__global__ __launch_bounds__(kColumnThreads) void dz_kernel(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz,
                                                       float* __restrict__ db, int rows, int n, long long dy_ld, long long z_ld) {
-    const int j = blockIdx.x * kThreads + threadIdx.x;
+    const int j = blockIdx.x * kColumnThreads + threadIdx.x;
     if (j >= n) return;
     float s = 0.0f;
     for (long long r = 0; r < rows; ++r) {
@@ -101,10 +399,45 @@ __global__ __launch_bounds__(kThreads) void dz_kernel(const T* __restrict__ dy, 
     if (db) db[j] = s;
 }
 
-template <typename T, int ACT>
-void launch_product(const T* a, const T* b, const ProductParams& p, hipStream_t stream) {
-    const dim3 grid((unsigned)((p.n + kTile - 1) / kTile), (unsigned)((p.m + kTile - 1) / kTile));
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, ACT>), grid, dim3(kThreads), 0, stream, a, b, p);
+
+// The tile that a product is cut into, and its launch.
+template <typename T, bool ACROSS_I, bool ACROSS_J>
+int launch_product(ProductParams p, hipStream_t stream) {
+    auto aligned = [](const Operand& o, int rows, int sum, bool across) {
+        const int row = across ? rows : sum;
+        return (uintptr_t)o.p % 16 == 0 && o.ld * sizeof(T) % 16 == 0 && row % Elem<T>::kVec == 0 && o.ld * 256 * (long long)sizeof(T) <= 0x7fffffffLL;
+    };
+    const bool vectors = aligned(p.i, p.rows, p.sum, ACROSS_I) && aligned(p.j, p.cols, p.sum, ACROSS_J);
+    TCBNN_REQUIRE((long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) <= 0x7fffffffLL, "linear: grid too large");
+    auto go = [&](auto bi, auto bj, auto wi, auto wj, auto whole) {
+        constexpr int BI = bi.value, BJ = bj.value, WI = wi.value, WJ = wj.value;
+        p.tiles_i = (p.rows + BI - 1) / BI;
+        p.tiles_j = (p.cols + BJ - 1) / BJ;
+        p.splits = 1;
+        p.split_sum = p.sum;
+        const long long units = (long long)p.tiles_i * p.tiles_j;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, BI, BJ, WI, WJ, ACROSS_I, ACROSS_J, whole.value>), dim3((unsigned)units),
+                           dim3(64 * WI * WJ), 0, stream, p);
+    };
+    using std::integral_constant;
+    auto by_size = [&](auto whole) {
+        const long long large = (long long)((p.rows + 255) / 256) * ((p.cols + 255) / 256), middle = (long long)((p.rows + 127) / 128) * ((p.cols + 127) / 128);
+        integral_constant<int, 256> n256;
+        integral_constant<int, 128> n128;
+        integral_constant<int, 64> n64;
+        integral_constant<int, 2> two;
+        integral_constant<int, 4> four;
+        if constexpr (whole.value)
+            if (large >= kComputeUnits * 3 / 4) return go(n256, n256, two, four, whole);
+        if (middle >= kComputeUnits * 3 / 4) return go(n128, n128, two, two, whole);
+        go(n64, n64, two, two, whole);
+    };
+    if (vectors)
+        by_size(std::true_type());
+    else
+        by_size(std::false_type());
+    TCBNN_LAUNCH_CHECK("product_kernel");
+    return TCBNN_OK;
 }
 
 }  // namespace
@@ -118,6 +451,7 @@ static int check_linear(int rows, int in_features, int out_features, int dtype, 
     TCBNN_REQUIRE(activation >= TCBNN_ACT_NONE && activation <= TCBNN_ACT_SILU, "linear: unknown activation");
     TCBNN_REQUIRE(rows >= 0 && in_features > 0 && out_features > 0, "linear: bad shape");
     TCBNN_REQUIRE(in_features <= kMaxIn, "linear: at most %d inputs", kMaxIn);
+    TCBNN_REQUIRE(out_features <= kMaxOut, "linear: at most %d outputs", kMaxOut);
     return TCBNN_OK;
 }
 
@@ -135,15 +469,21 @@ extern "C" int tcbnn_linear_forward(const tcbnn_linear_desc* d, void* stream) {
     TCBNN_NOTNULL(d->weight);
     TCBNN_NOTNULL(d->output);
     TCBNN_REQUIRE(d->output != d->residual || d->rows == 1 || y_ld == r_ld, "linear: an output over its residual has the residual's stride");
-    ProductParams p = {d->rows, d->out_features, d->in_features, x_ld, 1, w_ld, 1, d->bias, d->residual, d->output, d->preact, r_ld, y_ld, z_ld};
-    by_dtype(d->dtype, [&](auto t) {
-        using T = decltype(t);
-        by_activation(d->activation, [&](auto act) {
-            launch_product<T, act.value>((const T*)d->input, (const T*)d->weight, p, (hipStream_t)stream);
-        });
-    });
-    TCBNN_LAUNCH_CHECK("product_kernel");
-    return TCBNN_OK;
+    ProductParams p = {};
+    p.i = {d->input, x_ld};
+    p.j = {d->weight, w_ld};
+    p.rows = d->rows;
+    p.cols = d->out_features;
+    p.sum = d->in_features;
+    p.activation = d->activation;
+    p.bias = d->bias;
+    p.residual = d->residual;
+    p.out = d->output;
+    p.preact = d->preact;
+    p.residual_ld = r_ld;
+    p.out_ld = y_ld;
+    p.preact_ld = z_ld;
+    return by_dtype(d->dtype, [&](auto t) { return launch_product<decltype(t), false, false>(p, (hipStream_t)stream); });
 }
 
 extern "C" size_t tcbnn_linear_grad_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
@@ -170,27 +510,37 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
                           "linear: workspace too small");
         }
     }
-    by_dtype(d->dtype, [&](auto t) {
+    return by_dtype(d->dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const T* dz = active ? (const T*)d->workspace : (const T*)d->grad_output;
-        const long long dz_ld = active ? d->out_features : dy_ld;
         by_activation(d->activation, [&](auto act) {
             if (active || d->grad_bias)
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<T, act.value>), dim3((unsigned)((d->out_features + kThreads - 1) / kThreads)),
-                                   dim3(kThreads), 0, (hipStream_t)stream, (const T*)d->grad_output, (const T*)d->preact,
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<T, act.value>), dim3((unsigned)((d->out_features + kColumnThreads - 1) / kColumnThreads)),
+                                   dim3(kColumnThreads), 0, (hipStream_t)stream, (const T*)d->grad_output, (const T*)d->preact,
                                    (T*)d->workspace, d->grad_bias, d->rows, d->out_features, dy_ld, z_ld);
         });
-        if (d->grad_input && d->rows > 0)
-            launch_product<T, TCBNN_ACT_NONE>(dz, (const T*)d->weight,
-                                              {d->rows, d->in_features, d->out_features, dz_ld, 1, 1, w_ld, nullptr, nullptr, d->grad_input,
-                                               nullptr, 0, dx_ld, 0},
-                                              (hipStream_t)stream);
-        if (d->grad_weight)
-            launch_product<T, TCBNN_ACT_NONE>(dz, (const T*)d->input,
-                                              {d->out_features, d->in_features, d->rows, 1, dz_ld, 1, x_ld, nullptr, nullptr, d->grad_weight,
-                                               nullptr, 0, dw_ld, 0},
-                                              (hipStream_t)stream);
+        TCBNN_LAUNCH_CHECK("dz_kernel");
+        ProductParams p = {};
+        const Operand dz = active ? Operand{d->workspace, d->out_features} : Operand{d->grad_output, dy_ld};
+        if (d->grad_input && d->rows > 0) {
+            p.i = dz;
+            p.j = {d->weight, w_ld};
+            p.rows = d->rows;
+            p.cols = d->in_features;
+            p.sum = d->out_features;
+            p.out = d->grad_input;
+            p.out_ld = dx_ld;
+            if (int rc = launch_product<T, false, true>(p, (hipStream_t)stream)) return rc;
+        }
+        if (d->grad_weight) {
+            p.i = dz;
+            p.j = {d->input, x_ld};
+            p.rows = d->out_features;
+            p.cols = d->in_features;
+            p.sum = d->rows;
+            p.out = d->grad_weight;
+            p.out_ld = dw_ld;
+            if (int rc = launch_product<T, true, true>(p, (hipStream_t)stream)) return rc;
+        }
+        return TCBNN_OK;
     });
-    TCBNN_LAUNCH_CHECK("product_kernel");
-    return TCBNN_OK;
 }
