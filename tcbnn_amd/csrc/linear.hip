@@ -12,22 +12,59 @@ using namespace head;
 
 constexpr int kMaxIn = 1 << 20, kMaxOut = 1 << 28;
 
-// ---- activations
-template <int ACT>
+// ---- activations.  fp32 uses the library's erf and exp.  In 16-bit types, whose rounding is 2^-9 or 2^-12 of a result, they
+// cost as much as a quarter of a large product; there exp is 2^x of the hardware, a quotient its reciprocal (each good to
+// one unit in the last place of fp32), and the normal distribution's tail
+//   h(z) = erfc(|z| / sqrt 2) / 2 = exp(-z^2 / 2) Q(1 / (1 + 0.3 |z|)),
+// Q a polynomial of degree 8 without a constant term, fitted here for the least relative error of h over 0 <= |z| <= 13 (a Lawson
+// iteration: least squares, weights multiplied by the errors): 1.2e-7, evaluated in fp32 4.5e-7.
+constexpr float kLog2e = 1.44269504088896341f;
+template <typename T>
+__device__ __forceinline__ float exp_of(float x) {
+    if constexpr (sizeof(T) == 4) return expf(x);
+    return __builtin_amdgcn_exp2f(x * kLog2e);
+}
+template <typename T>
+__device__ __forceinline__ float over(float a, float b) {
+    if constexpr (sizeof(T) == 4) return a / b;
+    return a * __builtin_amdgcn_rcpf(b);
+}
+// the normal distribution function of z, and exp(-z^2 / 2)
+template <typename T>
+__device__ __forceinline__ float normal(float z, float& e) {
+    e = exp_of<T>(-0.5f * z * z);
+    if constexpr (sizeof(T) == 4) return 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(z), 0.3f, 1.0f));
+    float q = 0.036194976f;
+    q = __builtin_fmaf(q, t, -0.15937878f);
+    q = __builtin_fmaf(q, t, 0.21011917f);
+    q = __builtin_fmaf(q, t, -0.05716805f);
+    q = __builtin_fmaf(q, t, 0.13041681f);
+    q = __builtin_fmaf(q, t, 0.09934702f);
+    q = __builtin_fmaf(q, t, 0.12084555f);
+    q = __builtin_fmaf(q, t, 0.11962326f);
+    const float h = q * t * e;
+    return z < 0.0f ? h : 1.0f - h;
+}
+template <typename T, int ACT>
 __device__ __forceinline__ float activate(float z) {
+    float e;
     if constexpr (ACT == TCBNN_ACT_RELU) return z > 0.0f || z != z ? z : 0.0f;
-    if constexpr (ACT == TCBNN_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    if constexpr (ACT == TCBNN_ACT_SILU) return z / (1.0f + expf(-z));
+    if constexpr (ACT == TCBNN_ACT_GELU) return z * normal<T>(z, e);
+    if constexpr (ACT == TCBNN_ACT_SILU) return over<T>(z, 1.0f + exp_of<T>(-z));
     return z;
 }
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float slope(float z) {
+    float e;
     if constexpr (ACT == TCBNN_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    if constexpr (ACT == TCBNN_ACT_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    if constexpr (ACT == TCBNN_ACT_GELU) {
+        const float phi = normal<T>(z, e);
+        return __builtin_fmaf(z * 0.39894228040143268f, e, phi);
+    }
     if constexpr (ACT == TCBNN_ACT_SILU) {
-        const float p = 1.0f / (1.0f + expf(-z));
-        return p * (1.0f + z * (1.0f - p));
+        const float p = over<T>(1.0f, 1.0f + exp_of<T>(-z));
+        return p * __builtin_fmaf(z, 1.0f - p, 1.0f);
     }
     return 1.0f;
 }
@@ -199,43 +236,48 @@ struct ProductParams {
     float* partial;        // splits > 1: [splits][rows][cols]
 };
 
-// z of `n` <= kVec neighbouring columns of a row -> the outputs
+// `n` <= kVec neighbouring columns of a row, 0 in the place of those that are not there
 template <typename T>
-__device__ __forceinline__ void finish(const ProductParams& p, long long i, int j, const float* bias, float* z, int n) {
+__device__ __forceinline__ Vec<T> get_columns(const void* base, long long ld, long long i, int j, int n) {
+    constexpr int V = Elem<T>::kVec;
+    const T* from = (const T*)base + i * ld + j;
+    if (n >= V) return load_vec(from);
+    Vec<T> v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = e < n ? from[e] : (T)0.0f;
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void put_columns(void* base, long long ld, long long i, int j, int n, const float* z) {
+    constexpr int V = Elem<T>::kVec;
+    T* to = (T*)base + i * ld + j;
+    Vec<T> v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (T)z[e];
+    if (n >= V) {
+        store_vec(to, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (e < n) to[e] = v[e];
+    }
+}
+// their z -> the outputs
+template <typename T>
+__device__ __forceinline__ void finish(const ProductParams& p, long long i, int j, int n, const float* bias, Vec<T> residual, float* z) {
     constexpr int V = Elem<T>::kVec;
 #pragma unroll
     for (int e = 0; e < V; ++e) z[e] += bias[e];
-    auto put = [&](void* base, long long ld) {
-        T* to = (T*)base + i * ld + j;
-        if (n == V) {
-            Vec<T> v;
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = (T)z[e];
-            store_vec(to, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (e < n) to[e] = (T)z[e];
-        }
-    };
-    if (p.preact) put(p.preact, p.preact_ld);
+    if (p.preact) put_columns<T>(p.preact, p.preact_ld, i, j, n, z);
     by_activation(p.activation, [&](auto act) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) z[e] = activate<act.value>(z[e]);
+        for (int e = 0; e < V; ++e) z[e] = activate<T, act.value>(z[e]);
     });
     if (p.residual) {
-        const T* r = (const T*)p.residual + i * p.residual_ld + j;
-        if (n == V) {
-            const Vec<T> v = load_vec(r);
 #pragma unroll
-            for (int e = 0; e < V; ++e) z[e] += (float)v[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (e < n) z[e] += (float)r[e];
-        }
+        for (int e = 0; e < V; ++e) z[e] += (float)residual[e];
     }
-    put(p.out, p.out_ld);
+    put_columns<T>(p.out, p.out_ld, i, j, n, z);
 }
 
 // A workgroup's tile of c is BI x BJ, WI x WJ wavefronts with 32 x 32 pieces of it each.  Two tiles of each operand in LDS: the
@@ -284,35 +326,47 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
     auto arrived = [&](int stage) {
         ti.store(lds + stage * kStage);
         tj.store(lds + stage * kStage + TileI::kBytes);
+        if constexpr (ALIGNED) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what this wavefront requested is in LDS
         __syncthreads();
+    };
+    // A step's fragments come a quarter ahead of their instructions, the first quarter's from the next step's tiles: so the barrier
+    // that hands these over, and the request for the step after it into the tiles that are done with, lie before the last quarter's
+    // instructions.
+    Words fi[2][NI], fj[2][NJ];
+    auto fragments = [&](int set, int stage, int k) {
+        const char* li = lds + stage * kStage;
+#pragma unroll
+        for (int b = 0; b < NJ; ++b) fj[set][b] = TileJ::fragment(li + TileI::kBytes, wj + 32 * b, k);
+#pragma unroll
+        for (int a = 0; a < NI; ++a) fi[set][a] = TileI::fragment(li, wi + 32 * a, k);
+    };
+    auto multiply = [&](int set) {
+#pragma unroll
+        for (int a = 0; a < NI; ++a)
+#pragma unroll
+            for (int b = 0; b < NJ; ++b) acc[a][b] = mma<T>(fj[set][b], fi[set][a], acc[a][b]);
     };
     if (s0 < s1) {
         request(0, s0);
         arrived(0);
+        if (s0 + TileI::kSteps < s1) request(1, s0 + TileI::kSteps);
+        fragments(0, 0, 0);
     }
     int stage = 0;
     for (int s = s0; s < s1; s += TileI::kSteps, stage ^= 1) {
-        const bool more = s + TileI::kSteps < s1;
-        if (more) request(stage ^ 1, s + TileI::kSteps);
-        const char* li = lds + stage * kStage;
-        const char* lj = li + TileI::kBytes;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            Words fi[NI], fj[NJ];
-#pragma unroll
-            for (int a = 0; a < NI; ++a) fi[a] = TileI::fragment(li, wi + 32 * a, k);
-#pragma unroll
-            for (int b = 0; b < NJ; ++b) fj[b] = TileJ::fragment(lj, wj + 32 * b, k);
-#pragma unroll
-            for (int a = 0; a < NI; ++a)
-#pragma unroll
-                for (int b = 0; b < NJ; ++b) acc[a][b] = mma<T>(fj[b], fi[a], acc[a][b]);
+        for (int k = 0; k < 3; ++k) {
+            fragments((k + 1) & 1, stage, k + 1);
+            multiply(k & 1);
         }
-        if (more)
+        if (s + TileI::kSteps < s1) {
             arrived(stage ^ 1);
-        else
-            __syncthreads();
+            if (s + 2 * TileI::kSteps < s1) request(stage, s + 2 * TileI::kSteps);
+            fragments(0, stage ^ 1, 0);
+        }
+        multiply(1);
     }
+    __syncthreads();
 
     // ---- out: 32 rows of the wavefront at a time through LDS, so that a row leaves in whole runs of 64 bytes or more
     char* mine = lds + wave * kOutWave;
@@ -321,33 +375,43 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
     float bias[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) bias[e] = p.bias && e < n ? p.bias[j + e] : 0.0f;
-#pragma unroll
+#pragma unroll 1
     for (int a = 0; a < NI; ++a) {
+        constexpr int kTimes = 32 / kRowsAtOnce;
+        const long long first = i0 + wi + 32 * a + lane / kPerRow;
+        Vec<T> residual[kTimes];
+        if (p.residual && p.splits == 1) {
 #pragma unroll
-        for (int b = 0; b < NJ; ++b)
+            for (int r = 0; r < kTimes; ++r)
+                if (first + r * kRowsAtOnce < p.rows) residual[r] = get_columns<T>(p.residual, p.residual_ld, first + r * kRowsAtOnce, j, n);
+        }
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<float4*>(mine + (lane & 31) * kOutRow + (32 * b + 8 * g + 4 * (lane >> 5)) * 4) =
-                    make_float4(acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]);
+        for (int k = 0; k < NI; ++k)  // (registers have no index: one of NI pieces of code)
+            if (k == a) {
+#pragma unroll
+                for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<float4*>(mine + (lane & 31) * kOutRow + (32 * b + 8 * g + 4 * (lane >> 5)) * 4) =
+                            make_float4(acc[k][b][4 * g], acc[k][b][4 * g + 1], acc[k][b][4 * g + 2], acc[k][b][4 * g + 3]);
+            }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int r = 0; r < 32; r += kRowsAtOnce) {
-            const int row = r + lane / kPerRow;
-            const long long i = i0 + wi + 32 * a + row;
+        for (int r = 0; r < kTimes; ++r) {
+            const long long i = first + r * kRowsAtOnce;
+            const char* from = mine + (r * kRowsAtOnce + lane / kPerRow) * kOutRow + col * 4;
             float z[V];
 #pragma unroll
             for (int e = 0; e < V; e += 4) {
-                const float4 q = *reinterpret_cast<const float4*>(mine + row * kOutRow + (col + e) * 4);
+                const float4 q = *reinterpret_cast<const float4*>(from + e * 4);
                 z[e] = q.x, z[e + 1] = q.y, z[e + 2] = q.z, z[e + 3] = q.w;
             }
             if (i < p.rows && n > 0) {
                 if (p.splits > 1) {
-                    float* to = p.partial + ((size_t)split * p.rows + i) * p.cols + j;
 #pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (e < n) to[e] = z[e];
+                    for (int e = 0; e < V; e += 4) put_columns<float>(p.partial + (size_t)split * p.rows * p.cols, p.cols, i, j + e, n - e, z + e);
                 } else {
-                    finish<T>(p, i, j, bias, z, n);
+                    finish<T>(p, i, j, n, bias, residual[r], z);
                 }
             }
         }
@@ -376,29 +440,117 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
         for (int e = 0; e < V; ++e)
             if (e < n) z[e] += from[e];
     }
-    finish<T>(p, i, j, bias, z, n);
+    Vec<T> residual;
+    if (p.residual) residual = get_columns<T>(p.residual, p.residual_ld, i, j, n);
+    finish<T>(p, i, j, n, bias, residual, z);
 }
 
-constexpr int kColumnThreads = 256;
-// dz = dy act'(z) in the operands' type (nothing to write without an activation) and its column sums in fp32: a thread a
-// column, all rows in order
+// ---- dz = dy act'(z) in the operands' type (nothing to write without an activation), and its column sums in fp32, unrounded.
+// Bound by memory: a thread has one vector of 16 bytes of columns and goes down its share of the rows, two rows requested at
+// a time; the workgroups' sums are joined afterwards, always in the same order.
+constexpr int kDzThreads = 256;
+// Rows that one thread takes, and the parts that a column's sum falls into (a part a workgroup).
+inline int dz_rows(int rows, int vectors) {
+    const long long threads = 1024LL * kComputeUnits;  // four workgroups a compute unit
+    return (int)std::max(8LL, ((long long)rows * vectors + threads - 1) / threads);
+}
+inline int dz_lanes(int vectors) { return vectors >= kDzThreads ? kDzThreads : vectors; }  // of a workgroup, side by side
+inline int dz_parts(int rows, int vectors) {
+    const int deep = kDzThreads / dz_lanes(vectors) * dz_rows(rows, vectors);
+    return (rows + deep - 1) / deep;
+}
+
 template <typename T, int ACT>
-__global__ __launch_bounds__(kColumnThreads) void dz_kernel(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz,
-                                                      float* __restrict__ db, int rows, int n, long long dy_ld, long long z_ld) {
-    const int j = blockIdx.x * kColumnThreads + threadIdx.x;
-    if (j >= n) return;
-    float s = 0.0f;
-    for (long long r = 0; r < rows; ++r) {
-        float g = (float)dy[r * dy_ld + j];
-        if constexpr (ACT != TCBNN_ACT_NONE) {
-            g *= slope<ACT>((float)z[r * z_ld + j]);
-            dz[r * n + j] = (T)g;
+__global__ __launch_bounds__(kDzThreads) void dz_kernel(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz,
+                                                        float* __restrict__ sums, int rows, int n, int lanes, int each,
+                                                        long long dy_ld, long long z_ld) {
+    constexpr int V = Elem<T>::kVec, kAtOnce = 4;
+    __shared__ float lds[kDzThreads * V];
+    const int deep = kDzThreads / lanes, lane = threadIdx.x % lanes, depth = threadIdx.x / lanes;
+    const int j = (blockIdx.x * lanes + lane) * V, left = n - j;
+    const long long first = (long long)blockIdx.y * deep * each;
+    const long long last = min((long long)rows, first + (long long)deep * each);
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = 0.0f;
+    if (depth < deep && left > 0) {
+        auto get = [&](const T* p) {
+            if (left >= V) return load_vec(p);
+            Vec<T> v;
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = e < left ? p[e] : (T)0.0f;
+            return v;
+        };
+        for (long long r = first + depth; r < last; r += kAtOnce * deep) {
+            Vec<T> g[kAtOnce], x[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const long long at = min(r + u * deep, last - 1);  // (rows past the end are read once more and not used)
+                g[u] = get(dy + at * dy_ld + j);
+                if constexpr (ACT != TCBNN_ACT_NONE) x[u] = get(z + at * z_ld + j);
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                if (r + u * deep >= last) break;
+                float d[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    d[e] = (float)g[u][e];
+                    if constexpr (ACT != TCBNN_ACT_NONE) d[e] *= slope<T, ACT>((float)x[u][e]);
+                    s[e] += d[e];
+                }
+                if constexpr (ACT != TCBNN_ACT_NONE) {
+                    T* to = dz + (r + u * deep) * n + j;
+                    if (left >= V) {
+                        Vec<T> v;
+#pragma unroll
+                        for (int e = 0; e < V; ++e) v[e] = (T)d[e];
+                        store_vec(to, v);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e)
+                            if (e < left) to[e] = (T)d[e];
+                    }
+                }
+            }
         }
-        s += g;
     }
-    if (db) db[j] = s;
+    if (sums == nullptr) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) lds[e * kDzThreads + threadIdx.x] = s[e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < lanes * V; c += kDzThreads) {
+        const int l = c / V, e = c % V, col = (blockIdx.x * lanes + l) * V + e;
+        float t = 0.0f;
+        for (int d = 0; d < deep; ++d) t += lds[e * kDzThreads + d * lanes + l];
+        if (col < n) sums[(size_t)blockIdx.y * n + col] = t;
+    }
 }
 
+// the sums of all parts: 16 columns a workgroup, 16 threads to a column
+constexpr int kJoinColumns = 16;
+__global__ __launch_bounds__(kDzThreads) void column_join_kernel(const float* __restrict__ sums, float* __restrict__ db, int parts, int n) {
+    constexpr int kStep = kDzThreads / kJoinColumns;
+    __shared__ float lds[kStep][kJoinColumns];
+    const int c = threadIdx.x % kJoinColumns, part = threadIdx.x / kJoinColumns, j = blockIdx.x * kJoinColumns + c;
+    float s = 0.0f;
+    if (j < n)
+        for (int k = part; k < parts; k += 8 * kStep) {
+            float v[8];  // (requests of their own, one wait)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = k + u * kStep < parts ? sums[(size_t)(k + u * kStep) * n + j] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+    lds[part][c] = s;
+    __syncthreads();
+    if (part == 0 && j < n) {
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) s += lds[k][c];
+        db[j] = s;
+    }
+}
 
 // The tile that a product is cut into, and its launch.
 template <typename T, bool ACROSS_I, bool ACROSS_J>
@@ -486,9 +638,15 @@ extern "C" int tcbnn_linear_forward(const tcbnn_linear_desc* d, void* stream) {
     return by_dtype(d->dtype, [&](auto t) { return launch_product<decltype(t), false, false>(p, (hipStream_t)stream); });
 }
 
+// What the gradients need of a workspace: dz in dtype, then the parts of the column sums (whole 256 bytes each).
+static size_t whole_lines(size_t bytes) { return (bytes + 255) / 256 * 256; }
+static size_t dz_bytes(int rows, int out_features, int dtype) { return whole_lines((size_t)rows * out_features * dtype_bytes(dtype)); }
+static int out_vectors(int out_features, int dtype) { return (out_features + (int)(16 / dtype_bytes(dtype)) - 1) / (int)(16 / dtype_bytes(dtype)); }
+
 extern "C" size_t tcbnn_linear_grad_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
     if (rows <= 0 || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
-    return (size_t)rows * out_features * dtype_bytes(dtype);
+    return dz_bytes(rows, out_features, dtype) +
+           whole_lines(sizeof(float) * dz_parts(rows, out_vectors(out_features, dtype)) * (size_t)out_features);
 }
 
 extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stream) {
@@ -504,20 +662,28 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
         if (active) TCBNN_NOTNULL(d->preact);
         if (d->grad_weight) TCBNN_NOTNULL(d->input);
         if (d->grad_input) TCBNN_NOTNULL(d->weight);
-        if (active && tcbnn_linear_grad_workspace_bytes(d->rows, d->in_features, d->out_features, d->dtype) > 0) {
+        if (active || d->grad_bias) {
             TCBNN_NOTNULL(d->workspace);
+            TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "linear: the workspace is not aligned to 16 bytes");
             TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_linear_grad_workspace_bytes(d->rows, d->in_features, d->out_features, d->dtype),
                           "linear: workspace too small");
         }
     }
     return by_dtype(d->dtype, [&](auto t) -> int {
         using T = decltype(t);
-        by_activation(d->activation, [&](auto act) {
-            if (active || d->grad_bias)
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<T, act.value>), dim3((unsigned)((d->out_features + kColumnThreads - 1) / kColumnThreads)),
-                                   dim3(kColumnThreads), 0, (hipStream_t)stream, (const T*)d->grad_output, (const T*)d->preact,
-                                   (T*)d->workspace, d->grad_bias, d->rows, d->out_features, dy_ld, z_ld);
-        });
+        if (active || d->grad_bias) {
+            const int vectors = out_vectors(d->out_features, d->dtype), lanes = dz_lanes(vectors), parts = dz_parts(d->rows, vectors);
+            float* sums = d->grad_bias ? (float*)((char*)d->workspace + dz_bytes(d->rows, d->out_features, d->dtype)) : nullptr;
+            if (d->rows > 0)
+                by_activation(d->activation, [&](auto act) {
+                    hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<T, act.value>), dim3((unsigned)((vectors + lanes - 1) / lanes), (unsigned)parts),
+                                       dim3(kDzThreads), 0, (hipStream_t)stream, (const T*)d->grad_output, (const T*)d->preact,
+                                       (T*)d->workspace, sums, d->rows, d->out_features, lanes, dz_rows(d->rows, vectors), dy_ld, z_ld);
+                });
+            if (d->grad_bias)
+                hipLaunchKernelGGL(column_join_kernel, dim3((unsigned)((d->out_features + kJoinColumns - 1) / kJoinColumns)), dim3(kDzThreads), 0,
+                                   (hipStream_t)stream, sums, d->grad_bias, d->rows > 0 ? parts : 0, d->out_features);
+        }
         TCBNN_LAUNCH_CHECK("dz_kernel");
         ProductParams p = {};
         const Operand dz = active ? Operand{d->workspace, d->out_features} : Operand{d->grad_output, dy_ld};
