@@ -113,6 +113,7 @@ template <typename T, int ROWS, bool ACROSS, bool ALIGNED, int THREADS>
 struct Tile {
     static constexpr int V = Elem<T>::kVec, kSteps = kStepBytes / (int)sizeof(T);
     static constexpr int kBytes = ROWS * kStepBytes, kPieces = kBytes / 16, kEach = kPieces / THREADS;
+    static constexpr int kReads = !ACROSS ? 1 : (sizeof(T) == 2 ? 2 : 4);  // LDS requests of a fragment
     static constexpr int kRowPieces = ACROSS ? ROWS / V : 8;  // pieces of a row as LDS holds them
     static_assert(kEach * THREADS == kPieces, "whole pieces a thread");
 
@@ -280,9 +281,15 @@ __device__ __forceinline__ void finish(const ProductParams& p, long long i, int 
     put_columns<T>(p.out, p.out_ld, i, j, n, z);
 }
 
-// A workgroup's tile of c is BI x BJ, WI x WJ wavefronts with 32 x 32 pieces of it each.  Two tiles of each operand in LDS: the
-// next step is requested before the present one is multiplied.
-template <typename T, int BI, int BJ, int WI, int WJ, bool ACROSS_I, bool ACROSS_J, bool ALIGNED>
+// all of the workgroup's wavefronts are here, with all but `N` of their requests done and nothing of LDS under way
+template <int N>
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// A workgroup's tile of c is BI x BJ, WI x WJ wavefronts with 32 x 32 pieces of it each.  STAGES steps of both operands lie in LDS
+// or are on their way there; unaligned operands go through registers, one step ahead.
+template <typename T, int BI, int BJ, int WI, int WJ, int STAGES, bool ACROSS_I, bool ACROSS_J, bool ALIGNED>
 __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductParams p) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves the stub out where it instantiates a tile's requests twice)
     constexpr int kThreads = 64 * WI * WJ, NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec;
@@ -291,7 +298,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
     constexpr int kStage = TileI::kBytes + TileJ::kBytes;
     // a wavefront's 32 rows of c on their way out, 16 bytes between rows
     constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
-    constexpr int kLds = 2 * kStage > kOutWave * WI * WJ ? 2 * kStage : kOutWave * WI * WJ;
+    static_assert(ALIGNED || STAGES == 2, "registers hold one step");
+    constexpr int kLds = STAGES * kStage > kOutWave * WI * WJ ? STAGES * kStage : kOutWave * WI * WJ;
     __shared__ __align__(1024) char lds[kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -323,11 +331,21 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
         ti.request(lds + stage * kStage, s, s1);
         tj.request(lds + stage * kStage + TileI::kBytes, s, s1);
     };
-    auto arrived = [&](int stage) {
-        ti.store(lds + stage * kStage);
-        tj.store(lds + stage * kStage + TileI::kBytes);
-        if constexpr (ALIGNED) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what this wavefront requested is in LDS
-        __syncthreads();
+    // the next step's tiles are in LDS, for all to read; `rest` steps after it have been requested
+    constexpr int kRequests = TileI::kEach + TileJ::kEach;
+    auto arrived = [&](int stage, int rest) {
+        if constexpr (ALIGNED) {
+            if (rest >= STAGES - 1)
+                meet<(STAGES - 1) * kRequests>();
+            else if (STAGES > 2 && rest == STAGES - 2)
+                meet<(STAGES - 2) * kRequests>();
+            else
+                meet<0>();
+        } else {
+            ti.store(lds + stage * kStage);
+            tj.store(lds + stage * kStage + TileI::kBytes);
+            __syncthreads();
+        }
     };
     // A step's fragments come a quarter ahead of their instructions, the first quarter's from the next step's tiles: so the barrier
     // that hands these over, and the request for the step after it into the tiles that are done with, lie before the last quarter's
@@ -346,25 +364,47 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
 #pragma unroll
             for (int b = 0; b < NJ; ++b) acc[a][b] = mma<T>(fj[set][b], fi[set][a], acc[a][b]);
     };
-    if (s0 < s1) {
-        request(0, s0);
-        arrived(0);
-        if (s0 + TileI::kSteps < s1) request(1, s0 + TileI::kSteps);
+    const int steps = (s1 - s0 + TileI::kSteps - 1) / TileI::kSteps;
+    if (steps > 0) {
+        if constexpr (ALIGNED) {
+#pragma unroll
+            for (int k = 0; k < STAGES; ++k)
+                if (k < steps) request(k, s0 + k * TileI::kSteps);
+            arrived(0, min(steps, STAGES) - 1);
+        } else {
+            request(0, s0);
+            arrived(0, 0);
+            if (steps > 1) request(1, s0 + TileI::kSteps);
+        }
         fragments(0, 0, 0);
     }
     int stage = 0;
-    for (int s = s0; s < s1; s += TileI::kSteps, stage ^= 1) {
+    for (int step = 0; step < steps; ++step) {
+        const int next = stage + 1 == STAGES ? 0 : stage + 1;
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
             fragments((k + 1) & 1, stage, k + 1);
             multiply(k & 1);
+            // a request or two of LDS to a matrix instruction: all at once, they hold both wavefronts of a SIMD
+            constexpr int kReads = NI * TileI::kReads + NJ * TileJ::kReads, kInstr = NI * NJ * (sizeof(T) == 4 ? 4 : 1);
+            constexpr int kPer = (kReads + kInstr - 1) / kInstr, kGroups = (kReads + kPer - 1) / kPer;
+#pragma unroll
+            for (int q = 0; q < kGroups; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
+            }
+            if constexpr (kInstr > kGroups) __builtin_amdgcn_sched_group_barrier(0x008, kInstr - kGroups, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (s + TileI::kSteps < s1) {
-            arrived(stage ^ 1);
-            if (s + 2 * TileI::kSteps < s1) request(stage, s + 2 * TileI::kSteps);
-            fragments(0, stage ^ 1, 0);
+        if (step + 1 < steps) {
+            arrived(next, min(steps - 1, step + STAGES - 1) - (step + 1));
+            if (step + STAGES < steps) request(stage, s0 + (step + STAGES) * TileI::kSteps);
+            fragments(0, next, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
         multiply(1);
+        __builtin_amdgcn_sched_barrier(0);
+        stage = next;
     }
     __syncthreads();
 
@@ -440,7 +480,7 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
         for (int e = 0; e < V; ++e)
             if (e < n) z[e] += from[e];
     }
-    Vec<T> residual;
+    Vec<T> residual = {};
     if (p.residual) residual = get_columns<T>(p.residual, p.residual_ld, i, j, n);
     finish<T>(p, i, j, n, bias, residual, z);
 }
@@ -552,42 +592,65 @@ __global__ __launch_bounds__(kDzThreads) void column_join_kernel(const float* __
     }
 }
 
-// The tile that a product is cut into, and its launch.
+// The tile that a product is cut into, how often its sum is split, and its launch.
+enum Cut : int { CUT_256, CUT_256_128, CUT_128, CUT_64 };
+struct Plan {
+    Cut cut;
+    int splits;
+};
+inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors) {
+    const long long large = (long long)((rows + 255) / 256) * ((cols + 255) / 256), middle = (long long)((rows + 127) / 128) * ((cols + 127) / 128);
+    if (vectors && large >= kComputeUnits * 3 / 4) return {CUT_256, 1};
+    if (middle >= kComputeUnits * 3 / 4) return {CUT_128, 1};
+    return {CUT_64, 1};
+}
+
 template <typename T, bool ACROSS_I, bool ACROSS_J>
-int launch_product(ProductParams p, hipStream_t stream) {
+int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
+    TCBNN_REQUIRE((long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) <= 0x7fffffffLL, "linear: grid too large");
     auto aligned = [](const Operand& o, int rows, int sum, bool across) {
         const int row = across ? rows : sum;
         return (uintptr_t)o.p % 16 == 0 && o.ld * sizeof(T) % 16 == 0 && row % Elem<T>::kVec == 0 && o.ld * 256 * (long long)sizeof(T) <= 0x7fffffffLL;
     };
     const bool vectors = aligned(p.i, p.rows, p.sum, ACROSS_I) && aligned(p.j, p.cols, p.sum, ACROSS_J);
-    TCBNN_REQUIRE((long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) <= 0x7fffffffLL, "linear: grid too large");
-    auto go = [&](auto bi, auto bj, auto wi, auto wj, auto whole) {
-        constexpr int BI = bi.value, BJ = bj.value, WI = wi.value, WJ = wj.value;
+    const size_t part = (size_t)p.rows * p.cols * sizeof(float);
+    Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), vectors);
+    if (plan.splits * part > workspace_bytes) plan.splits = 1;
+    auto go = [&](auto bi, auto bj, auto wi, auto wj, auto stages, auto whole) {
+        constexpr int BI = bi.value, BJ = bj.value, WI = wi.value, WJ = wj.value, S = stages.value;
+        constexpr int kSteps = kStepBytes / (int)sizeof(T);
         p.tiles_i = (p.rows + BI - 1) / BI;
         p.tiles_j = (p.cols + BJ - 1) / BJ;
-        p.splits = 1;
-        p.split_sum = p.sum;
-        const long long units = (long long)p.tiles_i * p.tiles_j;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, BI, BJ, WI, WJ, ACROSS_I, ACROSS_J, whole.value>), dim3((unsigned)units),
+        const int steps = (p.sum + kSteps - 1) / kSteps;
+        p.split_sum = std::max(1, (steps + plan.splits - 1) / plan.splits) * kSteps;
+        p.splits = std::max(1, (p.sum + p.split_sum - 1) / p.split_sum);
+        p.partial = workspace;
+        const long long units = (long long)p.tiles_i * p.tiles_j * p.splits;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, BI, BJ, WI, WJ, S, ACROSS_I, ACROSS_J, whole.value>), dim3((unsigned)units),
                            dim3(64 * WI * WJ), 0, stream, p);
+        if (p.splits > 1) {
+            const long long vectors_out = (long long)p.rows * ((p.cols + Elem<T>::kVec - 1) / Elem<T>::kVec);
+            hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)((vectors_out + 255) / 256)), dim3(256), 0, stream, p);
+        }
     };
-    using std::integral_constant;
-    auto by_size = [&](auto whole) {
-        const long long large = (long long)((p.rows + 255) / 256) * ((p.cols + 255) / 256), middle = (long long)((p.rows + 127) / 128) * ((p.cols + 127) / 128);
-        integral_constant<int, 256> n256;
-        integral_constant<int, 128> n128;
-        integral_constant<int, 64> n64;
-        integral_constant<int, 2> two;
-        integral_constant<int, 4> four;
-        if constexpr (whole.value)
-            if (large >= kComputeUnits * 3 / 4) return go(n256, n256, two, four, whole);
-        if (middle >= kComputeUnits * 3 / 4) return go(n128, n128, two, two, whole);
-        go(n64, n64, two, two, whole);
-    };
-    if (vectors)
-        by_size(std::true_type());
-    else
-        by_size(std::false_type());
+    constexpr std::integral_constant<int, 256> n256;
+    constexpr std::integral_constant<int, 128> n128;
+    constexpr std::integral_constant<int, 64> n64;
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 3> three;
+    constexpr std::integral_constant<int, 4> four;
+    if (vectors) {
+        switch (plan.cut) {
+            case CUT_256: go(n256, n256, two, four, two, std::true_type()); break;
+            case CUT_256_128: go(n256, n128, two, two, three, std::true_type()); break;
+            case CUT_128: go(n128, n128, two, two, two, std::true_type()); break;
+            case CUT_64: go(n64, n64, two, two, four, std::true_type()); break;
+        }
+    } else if (plan.cut == CUT_64) {
+        go(n64, n64, two, two, two, std::false_type());
+    } else {
+        go(n128, n128, two, two, two, std::false_type());
+    }
     TCBNN_LAUNCH_CHECK("product_kernel");
     return TCBNN_OK;
 }
@@ -607,7 +670,16 @@ static int check_linear(int rows, int in_features, int out_features, int dtype, 
     return TCBNN_OK;
 }
 
-extern "C" size_t tcbnn_linear_workspace_bytes(int rows, int in_features, int out_features, int dtype) { return 0; }
+// the partial sums of a split product
+static size_t split_bytes(int rows, int cols, int sum, int dtype) {
+    const int splits = plan_product(rows, cols, sum, (int)dtype_bytes(dtype), true).splits;
+    return splits > 1 ? (size_t)splits * rows * cols * sizeof(float) : 0;
+}
+
+extern "C" size_t tcbnn_linear_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
+    if (rows <= 0 || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
+    return split_bytes(rows, out_features, in_features, dtype);
+}
 
 extern "C" int tcbnn_linear_forward(const tcbnn_linear_desc* d, void* stream) {
     TCBNN_NOTNULL(d);
@@ -635,7 +707,7 @@ extern "C" int tcbnn_linear_forward(const tcbnn_linear_desc* d, void* stream) {
     p.residual_ld = r_ld;
     p.out_ld = y_ld;
     p.preact_ld = z_ld;
-    return by_dtype(d->dtype, [&](auto t) { return launch_product<decltype(t), false, false>(p, (hipStream_t)stream); });
+    return by_dtype(d->dtype, [&](auto t) { return launch_product<decltype(t), false, false>(p, (float*)d->workspace, d->workspace ? d->workspace_bytes : 0, (hipStream_t)stream); });
 }
 
 // What the gradients need of a workspace: dz in dtype, then the parts of the column sums (whole 256 bytes each).
@@ -643,10 +715,13 @@ static size_t whole_lines(size_t bytes) { return (bytes + 255) / 256 * 256; }
 static size_t dz_bytes(int rows, int out_features, int dtype) { return whole_lines((size_t)rows * out_features * dtype_bytes(dtype)); }
 static int out_vectors(int out_features, int dtype) { return (out_features + (int)(16 / dtype_bytes(dtype)) - 1) / (int)(16 / dtype_bytes(dtype)); }
 
+static size_t sum_bytes(int rows, int out_features, int dtype) {
+    return rows == 0 ? 0 : whole_lines(sizeof(float) * dz_parts(rows, out_vectors(out_features, dtype)) * (size_t)out_features);
+}
 extern "C" size_t tcbnn_linear_grad_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
     if (rows <= 0 || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
-    return dz_bytes(rows, out_features, dtype) +
-           whole_lines(sizeof(float) * dz_parts(rows, out_vectors(out_features, dtype)) * (size_t)out_features);
+    return dz_bytes(rows, out_features, dtype) + sum_bytes(rows, out_features, dtype) +
+           std::max(split_bytes(rows, in_features, out_features, dtype), split_bytes(out_features, in_features, rows, dtype));
 }
 
 extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stream) {
@@ -685,6 +760,9 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
                                    (hipStream_t)stream, sums, d->grad_bias, d->rows > 0 ? parts : 0, d->out_features);
         }
         TCBNN_LAUNCH_CHECK("dz_kernel");
+        const size_t before = dz_bytes(d->rows, d->out_features, d->dtype) + sum_bytes(d->rows, d->out_features, d->dtype);
+        float* partials = d->workspace && d->workspace_bytes > before ? (float*)((char*)d->workspace + before) : nullptr;
+        const size_t partial_bytes = partials ? d->workspace_bytes - before : 0;
         ProductParams p = {};
         const Operand dz = active ? Operand{d->workspace, d->out_features} : Operand{d->grad_output, dy_ld};
         if (d->grad_input && d->rows > 0) {
@@ -695,7 +773,7 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
             p.sum = d->out_features;
             p.out = d->grad_input;
             p.out_ld = dx_ld;
-            if (int rc = launch_product<T, false, true>(p, (hipStream_t)stream)) return rc;
+            if (int rc = launch_product<T, false, true>(p, partials, partial_bytes, (hipStream_t)stream)) return rc;
         }
         if (d->grad_weight) {
             p.i = dz;
@@ -705,7 +783,7 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
             p.sum = d->rows;
             p.out = d->grad_weight;
             p.out_ld = dw_ld;
-            if (int rc = launch_product<T, true, true>(p, (hipStream_t)stream)) return rc;
+            if (int rc = launch_product<T, true, true>(p, partials, partial_bytes, (hipStream_t)stream)) return rc;
         }
         return TCBNN_OK;
     });
