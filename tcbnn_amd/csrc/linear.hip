@@ -3,6 +3,8 @@
 //
 // All three products are one kernel: c[i][j] = sum over s of I(i, s) J(j, s), where an operand lies in memory either along the
 // sum (x and w of the forward product: rows of s) or across it (w of dx, dz and x of dw: a row for every s).
+#include <cmath>
+
 #include "head.h"
 
 namespace tcbnn {
@@ -125,9 +127,8 @@ struct Tile {
 
     static __device__ __forceinline__ int swizzle(int row) {
         if constexpr (!ACROSS) return row & 7;
-        if constexpr (sizeof(T) == 4) return ((row >> 2) & 1) << 3;
-        if constexpr (kRowPieces >= 16) return (row & 3) << 2;
-        return ((row >> 1) & 1) << 2;
+        if constexpr (sizeof(T) == 4) return kRowPieces >= 16 ? ((row >> 2) & 1) << 3 : 0;
+        return kRowPieces >= 16 ? (row & 3) << 2 : (kRowPieces == 8 ? ((row >> 1) & 1) << 2 : 0);
     }
     // thread's e-th piece: its row and piece in memory
     static __device__ __forceinline__ void where(int e, int& row, int& piece) {
@@ -237,48 +238,49 @@ struct ProductParams {
     float* partial;        // splits > 1: [splits][rows][cols]
 };
 
-// `n` <= kVec neighbouring columns of a row, 0 in the place of those that are not there
-template <typename T>
-__device__ __forceinline__ Vec<T> get_columns(const void* base, long long ld, long long i, int j, int n) {
-    constexpr int V = Elem<T>::kVec;
+// C neighbouring columns of a row, of which `n` exist; 0 in the place of the others
+template <typename T, int C>
+using Columns = T __attribute__((ext_vector_type(C)));
+template <typename T, int C>
+using ColumnsAnywhere = T __attribute__((ext_vector_type(C), aligned(sizeof(T))));
+template <typename T, int C>
+__device__ __forceinline__ Columns<T, C> get_columns(const void* base, long long ld, long long i, int j, int n) {
     const T* from = (const T*)base + i * ld + j;
-    if (n >= V) return load_vec(from);
-    Vec<T> v;
+    if (n >= C) return *reinterpret_cast<const ColumnsAnywhere<T, C>*>(from);
+    Columns<T, C> v;
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = e < n ? from[e] : (T)0.0f;
+    for (int e = 0; e < C; ++e) v[e] = e < n ? from[e] : (T)0.0f;
     return v;
 }
-template <typename T>
+template <typename T, int C>
 __device__ __forceinline__ void put_columns(void* base, long long ld, long long i, int j, int n, const float* z) {
-    constexpr int V = Elem<T>::kVec;
     T* to = (T*)base + i * ld + j;
-    Vec<T> v;
+    Columns<T, C> v;
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = (T)z[e];
-    if (n >= V) {
-        store_vec(to, v);
+    for (int e = 0; e < C; ++e) v[e] = (T)z[e];
+    if (n >= C) {
+        *reinterpret_cast<ColumnsAnywhere<T, C>*>(to) = v;
     } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e)
+        for (int e = 0; e < C; ++e)
             if (e < n) to[e] = v[e];
     }
 }
 // their z -> the outputs
-template <typename T>
-__device__ __forceinline__ void finish(const ProductParams& p, long long i, int j, int n, const float* bias, Vec<T> residual, float* z) {
-    constexpr int V = Elem<T>::kVec;
+template <typename T, int C>
+__device__ __forceinline__ void finish(const ProductParams& p, long long i, int j, int n, const float* bias, Columns<T, C> residual, float* z) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) z[e] += bias[e];
-    if (p.preact) put_columns<T>(p.preact, p.preact_ld, i, j, n, z);
+    for (int e = 0; e < C; ++e) z[e] += bias[e];
+    if (p.preact) put_columns<T, C>(p.preact, p.preact_ld, i, j, n, z);
     by_activation(p.activation, [&](auto act) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) z[e] = activate<T, act.value>(z[e]);
+        for (int e = 0; e < C; ++e) z[e] = activate<T, act.value>(z[e]);
     });
     if (p.residual) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) z[e] += (float)residual[e];
+        for (int e = 0; e < C; ++e) z[e] += (float)residual[e];
     }
-    put_columns<T>(p.out, p.out_ld, i, j, n, z);
+    put_columns<T, C>(p.out, p.out_ld, i, j, n, z);
 }
 
 // all of the workgroup's wavefronts are here, with all but `N` of their requests done and nothing of LDS under way
@@ -287,19 +289,20 @@ __device__ __forceinline__ void meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// A workgroup's tile of c is BI x BJ, WI x WJ wavefronts with 32 x 32 pieces of it each.  STAGES steps of both operands lie in LDS
-// or are on their way there; unaligned operands go through registers, one step ahead.
-template <typename T, int BI, int BJ, int WI, int WJ, int STAGES, bool ACROSS_I, bool ACROSS_J, bool ALIGNED>
-__global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductParams p) {
+// A workgroup's tile of c is BI x BJ, WI x WJ wavefronts with 32 x 32 pieces of it each, WS times over: those share the quarters of a
+// step, and their sums are added at the end.  STAGES steps of both operands lie in LDS or are on their way there; unaligned
+// operands go through registers, one step ahead.
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, bool ACROSS_I, bool ACROSS_J, bool ALIGNED>
+__global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const ProductParams p) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves the stub out where it instantiates a tile's requests twice)
-    constexpr int kThreads = 64 * WI * WJ, NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec;
+    constexpr int kThreads = 64 * WI * WJ * WS, NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec, kQuarters = 4 / WS;
     using TileI = Tile<T, BI, ACROSS_I, ALIGNED, kThreads>;
     using TileJ = Tile<T, BJ, ACROSS_J, ALIGNED, kThreads>;
     constexpr int kStage = TileI::kBytes + TileJ::kBytes;
     // a wavefront's 32 rows of c on their way out, 16 bytes between rows
     constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
     static_assert(ALIGNED || STAGES == 2, "registers hold one step");
-    constexpr int kLds = STAGES * kStage > kOutWave * WI * WJ ? STAGES * kStage : kOutWave * WI * WJ;
+    constexpr int kOut = kOutWave * WI * WJ * WS, kLds = STAGES * kStage > kOut ? STAGES * kStage : kOut;
     __shared__ __align__(1024) char lds[kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
     ti.init(p.i, i0, p.rows);
     tj.init(p.j, j0, p.cols);
     const int s0 = split * p.split_sum, s1 = min(p.sum, s0 + p.split_sum);
-    const int wi = wave / WJ * (32 * NI), wj = wave % WJ * (32 * NJ);
+    const int share = wave / (WI * WJ), wi = wave / WJ % WI * (32 * NI), wj = wave % WJ * (32 * NJ);
 
     Acc acc[NI][NJ];
 #pragma unroll
@@ -353,6 +356,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
     Words fi[2][NI], fj[2][NJ];
     auto fragments = [&](int set, int stage, int k) {
         const char* li = lds + stage * kStage;
+        k += share * kQuarters;
 #pragma unroll
         for (int b = 0; b < NJ; ++b) fj[set][b] = TileJ::fragment(li + TileI::kBytes, wj + 32 * b, k);
 #pragma unroll
@@ -382,7 +386,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
     for (int step = 0; step < steps; ++step) {
         const int next = stage + 1 == STAGES ? 0 : stage + 1;
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
+        for (int k = 0; k + 1 < kQuarters; ++k) {
             fragments((k + 1) & 1, stage, k + 1);
             multiply(k & 1);
             // a request or two of LDS to a matrix instruction: all at once, they hold both wavefronts of a SIMD
@@ -399,31 +403,40 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
         if (step + 1 < steps) {
             arrived(next, min(steps - 1, step + STAGES - 1) - (step + 1));
             if (step + STAGES < steps) request(stage, s0 + (step + STAGES) * TileI::kSteps);
-            fragments(0, next, 0);
+            fragments(kQuarters & 1, next, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-        multiply(1);
+        multiply((kQuarters - 1) & 1);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kQuarters == 1) {  // (registers have no index: the next step's fragments take the place of this one's)
+#pragma unroll
+            for (int a = 0; a < NI; ++a) fi[0][a] = fi[1][a];
+#pragma unroll
+            for (int b = 0; b < NJ; ++b) fj[0][b] = fj[1][b];
+        }
         stage = next;
     }
     __syncthreads();
 
-    // ---- out: 32 rows of the wavefront at a time through LDS, so that a row leaves in whole runs of 64 bytes or more
+    // ---- out: 32 rows of the wavefront at a time through LDS, so that a row leaves in whole runs of 64 bytes or more.  Wavefronts
+    // that shared the sum take a share of the rows each.
     char* mine = lds + wave * kOutWave;
-    constexpr int kPerRow = 32 * NJ / V, kRowsAtOnce = 64 / kPerRow;  // lanes to a row, rows at once
-    const int col = (lane % kPerRow) * V, j = (int)j0 + wj + col, n = min(V, p.cols - j);
+    const char* first_share = lds + wave % (WI * WJ) * kOutWave;
+    constexpr int kPerRow = 32 * NJ / V, kShareRows = 32 / WS;  // lanes to a row, rows of a wavefront
+    constexpr int kRowsAtOnce = 64 / kPerRow < kShareRows ? 64 / kPerRow : kShareRows, kTimes = kShareRows / kRowsAtOnce;
+    const int col = (lane % kPerRow) * V, j = (int)j0 + wj + col, n = lane / kPerRow < kRowsAtOnce ? min(V, p.cols - j) : 0;
     float bias[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) bias[e] = p.bias && e < n ? p.bias[j + e] : 0.0f;
 #pragma unroll 1
     for (int a = 0; a < NI; ++a) {
-        constexpr int kTimes = 32 / kRowsAtOnce;
-        const long long first = i0 + wi + 32 * a + lane / kPerRow;
+        const int row0 = share * kShareRows + lane / kPerRow % kRowsAtOnce;
+        const long long first = i0 + wi + 32 * a + row0;
         Vec<T> residual[kTimes];
         if (p.residual && p.splits == 1) {
 #pragma unroll
             for (int r = 0; r < kTimes; ++r)
-                if (first + r * kRowsAtOnce < p.rows) residual[r] = get_columns<T>(p.residual, p.residual_ld, first + r * kRowsAtOnce, j, n);
+                if (first + r * kRowsAtOnce < p.rows) residual[r] = get_columns<T, V>(p.residual, p.residual_ld, first + r * kRowsAtOnce, j, n);
         }
 #pragma unroll
         for (int k = 0; k < NI; ++k)  // (registers have no index: one of NI pieces of code)
@@ -435,27 +448,39 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const ProductPara
                         *reinterpret_cast<float4*>(mine + (lane & 31) * kOutRow + (32 * b + 8 * g + 4 * (lane >> 5)) * 4) =
                             make_float4(acc[k][b][4 * g], acc[k][b][4 * g + 1], acc[k][b][4 * g + 2], acc[k][b][4 * g + 3]);
             }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if constexpr (WS > 1)
+            __syncthreads();
+        else
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int r = 0; r < kTimes; ++r) {
             const long long i = first + r * kRowsAtOnce;
-            const char* from = mine + (r * kRowsAtOnce + lane / kPerRow) * kOutRow + col * 4;
+            const char* from = first_share + (row0 + r * kRowsAtOnce) * kOutRow + col * 4;
             float z[V];
 #pragma unroll
             for (int e = 0; e < V; e += 4) {
-                const float4 q = *reinterpret_cast<const float4*>(from + e * 4);
+                float4 q = *reinterpret_cast<const float4*>(from + e * 4);
+#pragma unroll
+                for (int w = 1; w < WS; ++w) {
+                    const float4 o = *reinterpret_cast<const float4*>(from + w * (WI * WJ * kOutWave) + e * 4);
+                    q.x += o.x, q.y += o.y, q.z += o.z, q.w += o.w;
+                }
                 z[e] = q.x, z[e + 1] = q.y, z[e + 2] = q.z, z[e + 3] = q.w;
             }
             if (i < p.rows && n > 0) {
                 if (p.splits > 1) {
 #pragma unroll
-                    for (int e = 0; e < V; e += 4) put_columns<float>(p.partial + (size_t)split * p.rows * p.cols, p.cols, i, j + e, n - e, z + e);
+                    for (int e = 0; e < V; e += 4) put_columns<float, 4>(p.partial + (size_t)split * p.rows * p.cols, p.cols, i, j + e, n - e, z + e);
                 } else {
-                    finish<T>(p, i, j, n, bias, residual[r], z);
+                    finish<T, V>(p, i, j, n, bias, residual[r], z);
                 }
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if constexpr (WS > 1) {
+            if (NI > 1) __syncthreads();
+        } else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
     }
 #endif
 }
@@ -481,8 +506,91 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
             if (e < n) z[e] += from[e];
     }
     Vec<T> residual = {};
-    if (p.residual) residual = get_columns<T>(p.residual, p.residual_ld, i, j, n);
-    finish<T>(p, i, j, n, bias, residual, z);
+    if (p.residual) residual = get_columns<T, V>(p.residual, p.residual_ld, i, j, n);
+    finish<T, V>(p, i, j, n, bias, residual, z);
+}
+
+
+// ---- few rows (16 NI at most): bound by the weights' bytes.  A workgroup has 16 outputs, its 8 wavefronts an eighth of the sum each;
+// 64 bytes of 16 weight rows are one request of a wavefront and one matrix instruction (four in fp32), and eight requests of each
+// operand are under way at a time.  Nothing goes through LDS but the wavefronts' sums, and rows may lie anywhere.
+constexpr int kFewRows = 32, kFewWaves = 8, kFewOutputs = 16, kFewAtOnce = 8;
+typedef float Acc4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ Acc4 mma16(Vec<T> j, Vec<T> i, Acc4 c) {
+    if constexpr (std::is_same_v<T, __bf16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(j, i, c, 0, 0, 0);
+    } else if constexpr (std::is_same_v<T, _Float16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(j, i, c, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(j[e], i[e], c, 0, 0, 0);
+        return c;
+    }
+}
+
+template <typename T, int NI>
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const ProductParams p) {
+    constexpr int V = Elem<T>::kVec, kChunk = 4 * V;
+    __shared__ Acc4 lds[kFewWaves][NI][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int j0 = blockIdx.x * kFewOutputs;
+    // rows past the last one are read as the last one; nothing of them is kept
+    const T* w = (const T*)p.j.p + (long long)min(j0 + (lane & 15), p.cols - 1) * p.j.ld + (lane >> 4) * V;
+    const T* x[NI];
+#pragma unroll
+    for (int a = 0; a < NI; ++a) x[a] = (const T*)p.i.p + (long long)min(16 * a + (lane & 15), p.rows - 1) * p.i.ld + (lane >> 4) * V;
+    const int chunks = (p.sum + kChunk - 1) / kChunk, each = (chunks + kFewWaves - 1) / kFewWaves;
+    const int c0 = wave * each, c1 = min(chunks, c0 + each);
+    Acc4 acc[NI];
+#pragma unroll
+    for (int a = 0; a < NI; ++a) acc[a] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
+    int c = c0;
+    for (; c + kFewAtOnce <= c1 && (c + kFewAtOnce) * kChunk <= p.sum; c += kFewAtOnce) {
+        Vec<T> fw[kFewAtOnce], fx[NI][kFewAtOnce];
+#pragma unroll
+        for (int u = 0; u < kFewAtOnce; ++u) fw[u] = load_vec(w + (c + u) * kChunk);
+#pragma unroll
+        for (int a = 0; a < NI; ++a)
+#pragma unroll
+            for (int u = 0; u < kFewAtOnce; ++u) fx[a][u] = load_vec(x[a] + (c + u) * kChunk);
+#pragma unroll
+        for (int u = 0; u < kFewAtOnce; ++u)
+#pragma unroll
+            for (int a = 0; a < NI; ++a) acc[a] = mma16<T>(fw[u], fx[a][u], acc[a]);
+    }
+    // what is left: single chunks, the last one perhaps not whole
+    for (; c < c1; ++c) {
+        const int left = p.sum - c * kChunk - (lane >> 4) * V;  // of the sum, from the lane's first element on
+        auto get = [&](const T* q) {
+            if (left >= V) return load_vec(q + c * kChunk);
+            Vec<T> v;
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = e < left ? q[c * kChunk + e] : (T)0.0f;
+            return v;
+        };
+        const Vec<T> fw = get(w);
+#pragma unroll
+        for (int a = 0; a < NI; ++a) acc[a] = mma16<T>(fw, get(x[a]), acc[a]);
+    }
+#pragma unroll
+    for (int a = 0; a < NI; ++a) lds[wave][a][lane] = acc[a];
+    __syncthreads();
+    if (wave >= NI) return;
+    const int i = 16 * wave + (lane & 15), j = j0 + 4 * (lane >> 4), n = min(4, p.cols - j);
+    if (i >= p.rows || n <= 0) return;
+    float z[4], bias[4];
+    Acc4 sum = lds[0][wave][lane];
+#pragma unroll
+    for (int k = 1; k < kFewWaves; ++k) sum += lds[k][wave][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        z[e] = sum[e];
+        bias[e] = p.bias && e < n ? p.bias[j + e] : 0.0f;
+    }
+    Columns<T, 4> residual = {};
+    if (p.residual) residual = get_columns<T, 4>(p.residual, p.residual_ld, i, j, n);
+    finish<T, 4>(p, i, j, n, bias, residual, z);
 }
 
 // ---- dz = dy act'(z) in the operands' type (nothing to write without an activation), and its column sums in fp32, unrounded.
@@ -593,16 +701,46 @@ __global__ __launch_bounds__(kDzThreads) void column_join_kernel(const float* __
 }
 
 // The tile that a product is cut into, how often its sum is split, and its launch.
-enum Cut : int { CUT_256, CUT_256_128, CUT_128, CUT_64 };
+//
+// The plan is the one with the shortest estimate, from what the tiles measured (us): a step of the sum takes `step` when a
+// compute unit has one tile to work on (latency, then), `more` for each when it has several at a time, and a launch `start` besides.
+// A split sum is joined by a kernel of its own: 4.5 and the partial sums' bytes, out and back in, at 4 TB/s.
+enum Cut : int { CUT_256, CUT_128, CUT_128_DEEP, CUT_64, CUT_32, CUTS };
+struct CutCost {
+    int size;
+    float start, step, more;
+};
+// 16-bit types: 8192 x 4096 x 4096 227 us in tiles of 256 and 273 in 128; 2048^3 57 / 29 / 27 (deep) / 36 in 256 / 128 / 128 / 64; 1024^3
+// 36 / 17 / 16 / 8.8 / 13.5 (32); 100 x 400 x 300 20 / 11.5 / - / 6.1 / 4.9.  fp32: 400 x 800 x 1600 64 / 59 / 20 / 22 in 128 / deep / 64 / 32,
+// 256 x 512 x 1000 45 / - / 16 / 8.2.  Unaligned rows: 77 x 1023 x 1537 26 / - / 14 / 11, 8192 x 4096 x 4096 390 / - / 609 / 999.
+constexpr CutCost kCuts16[CUTS] = {{256, 10.0f, 1.6f, 1.75f}, {128, 6.0f, 0.85f, 0.55f}, {128, 6.0f, 0.6f, 0.65f}, {64, 3.2f, 0.33f, 0.26f}, {32, 3.2f, 0.21f, 0.14f}};
+constexpr CutCost kCuts32[CUTS] = {{256, 12.0f, 7.5f, 7.5f}, {128, 6.0f, 2.2f, 2.0f}, {128, 6.0f, 2.1f, 2.1f}, {64, 3.2f, 0.66f, 0.57f}, {32, 3.2f, 0.31f, 0.26f}};
+constexpr CutCost kCutsAnywhere[CUTS] = {{0, 0, 0, 0}, {128, 6.0f, 1.27f, 0.75f}, {0, 0, 0, 0}, {64, 3.2f, 0.7f, 0.3f}, {32, 3.2f, 0.5f, 0.14f}};
 struct Plan {
     Cut cut;
     int splits;
 };
-inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors) {
-    const long long large = (long long)((rows + 255) / 256) * ((cols + 255) / 256), middle = (long long)((rows + 127) / 128) * ((cols + 127) / 128);
-    if (vectors && large >= kComputeUnits * 3 / 4) return {CUT_256, 1};
-    if (middle >= kComputeUnits * 3 / 4) return {CUT_128, 1};
-    return {CUT_64, 1};
+inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, size_t workspace_bytes) {
+    const int steps = (int)(((long long)sum * size + kStepBytes - 1) / kStepBytes);
+    Plan best = {CUT_32, 1};
+    float least = 0.0f;
+    for (int c = 0; c < CUTS; ++c) {
+        CutCost cost = vectors ? (size == 4 ? kCuts32[c] : kCuts16[c]) : kCutsAnywhere[c];
+        if (cost.size == 0) continue;
+        if (!vectors && size == 4) cost.step = std::max(cost.step, kCuts32[c].step), cost.more = std::max(cost.more, kCuts32[c].more);
+        const float tiles = (float)((rows + cost.size - 1) / cost.size) * (float)((cols + cost.size - 1) / cost.size);
+        for (int k = 1; k <= 8 && (k == 1 || steps >= 4 * k); k *= 2) {
+            const size_t partial = k > 1 ? (size_t)k * rows * cols * sizeof(float) : 0;
+            if (partial > workspace_bytes) break;
+            const float rounds = std::ceil(tiles * (float)k / (float)kComputeUnits), each = std::max(cost.step, rounds * cost.more);
+            const float time = cost.start + (float)((steps + k - 1) / k) * each + (k > 1 ? 4.5f + (float)partial * 2.0f / 4.0e6f : 0.0f);
+            if (least == 0.0f || time < least) {
+                least = time;
+                best = {(Cut)c, k};
+            }
+        }
+    }
+    return best;
 }
 
 template <typename T, bool ACROSS_I, bool ACROSS_J>
@@ -613,21 +751,30 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
         return (uintptr_t)o.p % 16 == 0 && o.ld * sizeof(T) % 16 == 0 && row % Elem<T>::kVec == 0 && o.ld * 256 * (long long)sizeof(T) <= 0x7fffffffLL;
     };
     const bool vectors = aligned(p.i, p.rows, p.sum, ACROSS_I) && aligned(p.j, p.cols, p.sum, ACROSS_J);
-    const size_t part = (size_t)p.rows * p.cols * sizeof(float);
-    Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), vectors);
-    if (plan.splits * part > workspace_bytes) plan.splits = 1;
-    auto go = [&](auto bi, auto bj, auto wi, auto wj, auto stages, auto whole) {
-        constexpr int BI = bi.value, BJ = bj.value, WI = wi.value, WJ = wj.value, S = stages.value;
+    if constexpr (!ACROSS_I && !ACROSS_J) {
+        if (p.rows <= kFewRows) {
+            const dim3 grid((unsigned)((p.cols + kFewOutputs - 1) / kFewOutputs));
+            if (p.rows <= 16)
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, 1>), grid, dim3(64 * kFewWaves), 0, stream, p);
+            else
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, 2>), grid, dim3(64 * kFewWaves), 0, stream, p);
+            TCBNN_LAUNCH_CHECK("few_rows_kernel");
+            return TCBNN_OK;
+        }
+    }
+    const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), vectors, workspace_bytes);
+    auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto whole) {
+        constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value;
         constexpr int kSteps = kStepBytes / (int)sizeof(T);
-        p.tiles_i = (p.rows + BI - 1) / BI;
-        p.tiles_j = (p.cols + BJ - 1) / BJ;
+        p.tiles_i = (p.rows + B - 1) / B;
+        p.tiles_j = (p.cols + B - 1) / B;
         const int steps = (p.sum + kSteps - 1) / kSteps;
         p.split_sum = std::max(1, (steps + plan.splits - 1) / plan.splits) * kSteps;
         p.splits = std::max(1, (p.sum + p.split_sum - 1) / p.split_sum);
         p.partial = workspace;
         const long long units = (long long)p.tiles_i * p.tiles_j * p.splits;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, BI, BJ, WI, WJ, S, ACROSS_I, ACROSS_J, whole.value>), dim3((unsigned)units),
-                           dim3(64 * WI * WJ), 0, stream, p);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, ACROSS_I, ACROSS_J, whole.value>), dim3((unsigned)units),
+                           dim3(64 * WI * WJ * WS), 0, stream, p);
         if (p.splits > 1) {
             const long long vectors_out = (long long)p.rows * ((p.cols + Elem<T>::kVec - 1) / Elem<T>::kVec);
             hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)((vectors_out + 255) / 256)), dim3(256), 0, stream, p);
@@ -636,20 +783,25 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
     constexpr std::integral_constant<int, 256> n256;
     constexpr std::integral_constant<int, 128> n128;
     constexpr std::integral_constant<int, 64> n64;
+    constexpr std::integral_constant<int, 32> n32;
+    constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;
-    constexpr std::integral_constant<int, 3> three;
     constexpr std::integral_constant<int, 4> four;
+    constexpr std::integral_constant<int, 8> eight;
     if (vectors) {
         switch (plan.cut) {
-            case CUT_256: go(n256, n256, two, four, two, std::true_type()); break;
-            case CUT_256_128: go(n256, n128, two, two, three, std::true_type()); break;
-            case CUT_128: go(n128, n128, two, two, two, std::true_type()); break;
-            case CUT_64: go(n64, n64, two, two, four, std::true_type()); break;
+            case CUT_256: go(n256, two, four, one, two, std::true_type()); break;
+            case CUT_128: go(n128, two, two, one, two, std::true_type()); break;
+            case CUT_128_DEEP: go(n128, two, two, two, four, std::true_type()); break;
+            case CUT_64: go(n64, two, two, two, four, std::true_type()); break;
+            default: go(n32, one, one, four, eight, std::true_type()); break;
         }
-    } else if (plan.cut == CUT_64) {
-        go(n64, n64, two, two, two, std::false_type());
     } else {
-        go(n128, n128, two, two, two, std::false_type());
+        switch (plan.cut) {
+            case CUT_128: go(n128, two, two, one, two, std::false_type()); break;
+            case CUT_64: go(n64, two, two, one, two, std::false_type()); break;
+            default: go(n32, one, one, four, two, std::false_type()); break;
+        }
     }
     TCBNN_LAUNCH_CHECK("product_kernel");
     return TCBNN_OK;
@@ -672,13 +824,13 @@ static int check_linear(int rows, int in_features, int out_features, int dtype, 
 
 // the partial sums of a split product
 static size_t split_bytes(int rows, int cols, int sum, int dtype) {
-    const int splits = plan_product(rows, cols, sum, (int)dtype_bytes(dtype), true).splits;
+    const int splits = plan_product(rows, cols, sum, (int)dtype_bytes(dtype), true, ~(size_t)0).splits;
     return splits > 1 ? (size_t)splits * rows * cols * sizeof(float) : 0;
 }
 
 extern "C" size_t tcbnn_linear_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
     if (rows <= 0 || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
-    return split_bytes(rows, out_features, in_features, dtype);
+    return rows <= kFewRows ? 0 : split_bytes(rows, out_features, in_features, dtype);
 }
 
 extern "C" int tcbnn_linear_forward(const tcbnn_linear_desc* d, void* stream) {
