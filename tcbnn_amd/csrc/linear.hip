@@ -111,7 +111,12 @@ struct Operand {
     long long ld;  // elements between rows in memory
 };
 
-template <typename T, int ROWS, bool ACROSS, bool ALIGNED, int THREADS>
+// How an operand's rows lie in memory: at whole pieces (requested into LDS), anywhere (through registers: the last piece of a row is
+// requested as the row's last 16 bytes and moved into place), or anywhere in rows shorter than a piece or further apart than 32
+// bits hold for a tile (element by element).
+enum Access : int { WHOLE_PIECES, ANYWHERE, ELEMENTS };
+
+template <typename T, int ROWS, bool ACROSS, Access ACCESS, int THREADS, int SLOTS>
 struct Tile {
     static constexpr int V = Elem<T>::kVec, kSteps = kStepBytes / (int)sizeof(T);
     static constexpr int kBytes = ROWS * kStepBytes, kPieces = kBytes / 16, kEach = kPieces / THREADS;
@@ -121,7 +126,7 @@ struct Tile {
 
     const T* base;
     int offset[kEach];  // bytes from the tile's first element in memory, at the first step
-    Words held[ALIGNED ? 1 : kEach];
+    Words held[SLOTS][ACCESS == WHOLE_PIECES ? 1 : kEach];
     long long ld;
     int valid;  // rows of the tile that exist
 
@@ -136,26 +141,31 @@ struct Tile {
         row = at / kRowPieces;
         piece = (at % kRowPieces) ^ swizzle(row);
     }
-    // rows first .. of `total` rows (i or j)
+    // rows first .. of `total` rows (i or j).  What lies past the last row is some other row's: nothing of it is kept.
     __device__ __forceinline__ void init(const Operand& o, long long first, long long total) {
         ld = o.ld;
         valid = (int)min((long long)ROWS, total - first);
-        base = (const T*)o.p + (ACROSS ? first : first * ld);
+        // Across the sum, a tile's last piece is read as the row's last 16 bytes, which begin before the tile where it has fewer
+        // columns than that: offsets count from there and are never negative.
+        const int lead = ACROSS && ACCESS == ANYWHERE ? max(0, V - valid) : 0;
+        base = (const T*)o.p + (ACROSS ? first - lead : first * ld);
+        if constexpr (ACCESS != ELEMENTS) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            int row, piece;
-            where(e, row, piece);
-            // what lies past the last row is some other row's: nothing of it is kept
-            if constexpr (ACROSS)
-                offset[e] = (int)(row * ld + (piece * V < valid ? piece * V : 0)) * (int)sizeof(T);
-            else
-                offset[e] = (int)(min(row, valid - 1) * ld + piece * V) * (int)sizeof(T);
+            for (int e = 0; e < kEach; ++e) {
+                int row, piece;
+                where(e, row, piece);
+                if constexpr (ACROSS)  // (pieces past the last column: the last one)
+                    offset[e] = (int)(row * ld + min(piece * V, valid - V) + lead) * (int)sizeof(T);
+                else
+                    offset[e] = (int)(min(row, valid - 1) * ld + piece * V) * (int)sizeof(T);
+            }
         }
     }
-    // requests the tile of the step that begins at `s` of `sum` (into LDS at once, or into registers)
+    // requests the tile of the step that begins at `s` of `sum`: into LDS at once, or into the registers of a slot
+    template <int SLOT>
     __device__ __forceinline__ void request(char* lds, int s, int sum) {
         const bool whole = s + kSteps <= sum;
-        if constexpr (ALIGNED) {
+        if constexpr (ACCESS == WHOLE_PIECES) {
             const __amdgpu_buffer_rsrc_t r =
                 __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(ACROSS ? base + s * ld : base), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
@@ -166,34 +176,77 @@ struct Tile {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(lds + (e * THREADS + wave_first()) * 16), 16,
                                                          there ? offset[e] : kOutOfRange, ACROSS ? 0 : s * (int)sizeof(T), 0, 0);
             }
+        } else if constexpr (ACCESS == ANYWHERE) {
+            // (no branches: then the requests of several steps can be told apart by their number)
+            const char* from = reinterpret_cast<const char*>(ACROSS ? base + s * ld : base);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                int row, piece;
+                where(e, row, piece);
+                int at = offset[e];
+                if constexpr (ACROSS) {
+                    at -= max(0, s + row - (sum - 1)) * (int)(ld * (int)sizeof(T));  // rows past the sum: the last one
+                } else {
+                    const int start = s + piece * V;
+                    at += (start >= sum ? -piece * V : min(s, sum - V - piece * V)) * (int)sizeof(T);
+                }
+                held[SLOT][e] = __builtin_bit_cast(Words, load_vec(reinterpret_cast<const T*>(from + (uint32_t)at)));
+            }
         } else {
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
                 int row, piece;
                 where(e, row, piece);
-                held[e] = Words{0, 0, 0, 0};
-                if constexpr (ACROSS) {
-                    const T* p = base + (s + row) * ld + piece * V;
-                    if (s + row < sum) held[e] = take(p, valid - piece * V);
-                } else {
-                    const T* p = base + min(row, valid - 1) * ld + s + piece * V;
-                    held[e] = take(p, sum - (s + piece * V));
-                }
+                const T* p = ACROSS ? base + (s + row) * ld + piece * V : base + min(row, valid - 1) * ld + s + piece * V;
+                const int n = ACROSS ? (s + row < sum ? valid - piece * V : 0) : sum - (s + piece * V);
+                Vec<T> v;
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[k] = k < n ? p[k] : (T)0.0f;
+                held[SLOT][e] = __builtin_bit_cast(Words, v);
             }
         }
     }
-    static __device__ __forceinline__ Words take(const T* p, int n) {
-        if (n >= V) return __builtin_bit_cast(Words, load_vec(p));
-        Vec<T> v;
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = k < n ? p[k] : (T)0.0f;
-        return __builtin_bit_cast(Words, v);
-    }
     static __device__ __forceinline__ int wave_first() { return __builtin_amdgcn_readfirstlane(threadIdx.x & ~63); }
-    __device__ __forceinline__ void store(char* lds) const {
-        if constexpr (!ALIGNED) {
+    // the last `n` elements of a piece in the place of its first, 0 behind them
+    static __device__ __forceinline__ Words last_first(Words w, int n) {
+        const int bits = (V - n) * 8 * (int)sizeof(T);
+        unsigned long long lo = ((unsigned long long)(uint32_t)w[1] << 32) | (uint32_t)w[0];
+        unsigned long long hi = ((unsigned long long)(uint32_t)w[3] << 32) | (uint32_t)w[2];
+        if (bits >= 64) {
+            lo = hi >> (bits - 64);
+            hi = 0;
+        } else {
+            lo = (lo >> bits) | (hi << 1 << (63 - bits));
+            hi >>= bits;
+        }
+        return Words{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+    }
+    // a slot, whose step began at `s`, into LDS
+    template <int SLOT>
+    __device__ __forceinline__ void store(char* lds, int s, int sum) {
+        if constexpr (ACCESS == ANYWHERE) {
+            if (ACROSS && valid < ROWS && valid % V != 0) {
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) *reinterpret_cast<Words*>(lds + (e * THREADS + (int)threadIdx.x) * 16) = held[e];
+                for (int e = 0; e < kEach; ++e) {
+                    int row, piece;
+                    where(e, row, piece);
+                    if (piece == valid / V) held[SLOT][e] = last_first(held[SLOT][e], valid % V);
+                }
+            }
+            if (s + kSteps > sum) {
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    int row, piece;
+                    where(e, row, piece);
+                    const int left = sum - s - (ACROSS ? row : piece * V);
+                    if (!ACROSS && left > 0 && left < V) held[SLOT][e] = last_first(held[SLOT][e], sum % V);
+                    if (left <= 0) held[SLOT][e] = Words{0, 0, 0, 0};
+                }
+            }
+        }
+        if constexpr (ACCESS != WHOLE_PIECES) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) *reinterpret_cast<Words*>(lds + (e * THREADS + (int)threadIdx.x) * 16) = held[SLOT][e];
         }
     }
     // the fragment of rows `first` .. `first` + 31, the k-th quarter of the step
@@ -290,18 +343,19 @@ __device__ __forceinline__ void meet() {
 }
 
 // A workgroup's tile of c is BI x BJ, WI x WJ wavefronts with 32 x 32 pieces of it each, WS times over: those share the quarters of a
-// step, and their sums are added at the end.  STAGES steps of both operands lie in LDS or are on their way there; unaligned
-// operands go through registers, one step ahead.
-template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, bool ACROSS_I, bool ACROSS_J, bool ALIGNED>
+// step, and their sums are added at the end.  STAGES steps of both operands lie in LDS or are on their way there;
+// what goes through registers does so HOLD steps ahead.
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool ACROSS_I, bool ACROSS_J>
 __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const ProductParams p) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves the stub out where it instantiates a tile's requests twice)
     constexpr int kThreads = 64 * WI * WJ * WS, NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec, kQuarters = 4 / WS;
-    using TileI = Tile<T, BI, ACROSS_I, ALIGNED, kThreads>;
-    using TileJ = Tile<T, BJ, ACROSS_J, ALIGNED, kThreads>;
+    constexpr bool ALIGNED = ACCESS == WHOLE_PIECES;
+    using TileI = Tile<T, BI, ACROSS_I, ACCESS, kThreads, HOLD>;
+    using TileJ = Tile<T, BJ, ACROSS_J, ACCESS, kThreads, HOLD>;
     constexpr int kStage = TileI::kBytes + TileJ::kBytes;
     // a wavefront's 32 rows of c on their way out, 16 bytes between rows
     constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
-    static_assert(ALIGNED || STAGES == 2, "registers hold one step");
+    static_assert(ALIGNED || STAGES == 2, "what registers hold needs two tiles");
     constexpr int kOut = kOutWave * WI * WJ * WS, kLds = STAGES * kStage > kOut ? STAGES * kStage : kOut;
     __shared__ __align__(1024) char lds[kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -330,13 +384,15 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const Produc
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.0f;
 
-    auto request = [&](int stage, int s) {
-        ti.request(lds + stage * kStage, s, s1);
-        tj.request(lds + stage * kStage + TileI::kBytes, s, s1);
+    using std::integral_constant;
+    auto request = [&](int stage, int step, auto slot) {
+        const int s = s0 + step * TileI::kSteps;
+        ti.template request<slot.value>(lds + stage * kStage, s, s1);
+        tj.template request<slot.value>(lds + stage * kStage + TileI::kBytes, s, s1);
     };
     // the next step's tiles are in LDS, for all to read; `rest` steps after it have been requested
     constexpr int kRequests = TileI::kEach + TileJ::kEach;
-    auto arrived = [&](int stage, int rest) {
+    auto arrived = [&](int stage, int step, int rest, auto slot) {
         if constexpr (ALIGNED) {
             if (rest >= STAGES - 1)
                 meet<(STAGES - 1) * kRequests>();
@@ -345,9 +401,10 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const Produc
             else
                 meet<0>();
         } else {
-            ti.store(lds + stage * kStage);
-            tj.store(lds + stage * kStage + TileI::kBytes);
-            __syncthreads();
+            const int s = s0 + step * TileI::kSteps;
+            ti.template store<slot.value>(lds + stage * kStage, s, s1);
+            tj.template store<slot.value>(lds + stage * kStage + TileI::kBytes, s, s1);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (requests into registers stay under way)
         }
     };
     // A step's fragments come a quarter ahead of their instructions, the first quarter's from the next step's tiles: so the barrier
@@ -369,22 +426,23 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const Produc
             for (int b = 0; b < NJ; ++b) acc[a][b] = mma<T>(fj[set][b], fi[set][a], acc[a][b]);
     };
     const int steps = (s1 - s0 + TileI::kSteps - 1) / TileI::kSteps;
-    if (steps > 0) {
-        if constexpr (ALIGNED) {
-#pragma unroll
-            for (int k = 0; k < STAGES; ++k)
-                if (k < steps) request(k, s0 + k * TileI::kSteps);
-            arrived(0, min(steps, STAGES) - 1);
-        } else {
-            request(0, s0);
-            arrived(0, 0);
-            if (steps > 1) request(1, s0 + TileI::kSteps);
+    // steps under way at a time: the tiles in LDS, or the slots of registers
+    constexpr int kAhead = ALIGNED ? STAGES : HOLD;
+    auto each = [&](auto f) {
+        f(integral_constant<int, 0>());
+        if constexpr (kAhead > 1) f(integral_constant<int, 1>());
+        if constexpr (kAhead > 2) f(integral_constant<int, 2>());
+        if constexpr (kAhead > 3) f(integral_constant<int, 3>());
+        if constexpr (kAhead > 4) {
+            static_assert(kAhead == 8, "");
+            f(integral_constant<int, 4>()), f(integral_constant<int, 5>()), f(integral_constant<int, 6>()), f(integral_constant<int, 7>());
         }
-        fragments(0, 0, 0);
-    }
+    };
     int stage = 0;
-    for (int step = 0; step < steps; ++step) {
+    // `slot` (unaligned operands): step % HOLD
+    auto advance = [&](int step, auto slot) {
         const int next = stage + 1 == STAGES ? 0 : stage + 1;
+        constexpr integral_constant<int, (slot.value + 1) % HOLD> next_slot;
 #pragma unroll
         for (int k = 0; k + 1 < kQuarters; ++k) {
             fragments((k + 1) & 1, stage, k + 1);
@@ -401,8 +459,12 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const Produc
             __builtin_amdgcn_sched_barrier(0);
         }
         if (step + 1 < steps) {
-            arrived(next, min(steps - 1, step + STAGES - 1) - (step + 1));
-            if (step + STAGES < steps) request(stage, s0 + (step + STAGES) * TileI::kSteps);
+            arrived(next, step + 1, min(steps - 1, step + kAhead - 1) - (step + 1), next_slot);
+            if constexpr (ALIGNED) {
+                if (step + STAGES < steps) request(stage, step + STAGES, slot);
+            } else {
+                if (step + 1 + HOLD < steps) request(0, step + 1 + HOLD, next_slot);
+            }
             fragments(kQuarters & 1, next, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -415,6 +477,29 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const Produc
             for (int b = 0; b < NJ; ++b) fj[0][b] = fj[1][b];
         }
         stage = next;
+    };
+    if (steps > 0) {
+        if constexpr (ALIGNED) {
+            each([&](auto k) {
+                if (k.value < steps) request(k.value, k.value, integral_constant<int, 0>());
+            });
+            arrived(0, 0, min(steps, STAGES) - 1, integral_constant<int, 0>());
+        } else {
+            each([&](auto k) {
+                if (k.value < steps) request(0, k.value, k);
+            });
+            arrived(0, 0, 0, integral_constant<int, 0>());
+            if (HOLD < steps) request(0, HOLD, integral_constant<int, 0>());
+        }
+        fragments(0, 0, 0);
+    }
+    if constexpr (ALIGNED) {
+        for (int step = 0; step < steps; ++step) advance(step, integral_constant<int, 0>());
+    } else {
+        for (int step = 0; step < steps; step += HOLD)
+            each([&](auto k) {
+                if (step + k.value < steps) advance(step + k.value, k);
+            });
     }
     __syncthreads();
 
@@ -530,7 +615,7 @@ __device__ __forceinline__ Acc4 mma16(Vec<T> j, Vec<T> i, Acc4 c) {
 }
 
 template <typename T, int NI>
-__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const ProductParams p) {
+__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 4))) void few_rows_kernel(const ProductParams p) {
     constexpr int V = Elem<T>::kVec, kChunk = 4 * V;
     __shared__ Acc4 lds[kFewWaves][NI][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -554,6 +639,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const ProductP
         for (int a = 0; a < NI; ++a)
 #pragma unroll
             for (int u = 0; u < kFewAtOnce; ++u) fx[a][u] = load_vec(x[a] + (c + u) * kChunk);
+        __builtin_amdgcn_sched_barrier(0);  // (all requests first: the compiler would rather save registers)
 #pragma unroll
         for (int u = 0; u < kFewAtOnce; ++u)
 #pragma unroll
@@ -746,11 +832,12 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
 template <typename T, bool ACROSS_I, bool ACROSS_J>
 int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
     TCBNN_REQUIRE((long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) <= 0x7fffffffLL, "linear: grid too large");
-    auto aligned = [](const Operand& o, int rows, int sum, bool across) {
+    auto access_of = [](const Operand& o, int rows, int sum, bool across) {
         const int row = across ? rows : sum;
-        return (uintptr_t)o.p % 16 == 0 && o.ld * sizeof(T) % 16 == 0 && row % Elem<T>::kVec == 0 && o.ld * 256 * (long long)sizeof(T) <= 0x7fffffffLL;
+        if (row < Elem<T>::kVec || o.ld * 256 * (long long)sizeof(T) > 0x7fffffffLL) return ELEMENTS;
+        return (uintptr_t)o.p % 16 == 0 && o.ld * sizeof(T) % 16 == 0 && row % Elem<T>::kVec == 0 ? WHOLE_PIECES : ANYWHERE;
     };
-    const bool vectors = aligned(p.i, p.rows, p.sum, ACROSS_I) && aligned(p.j, p.cols, p.sum, ACROSS_J);
+    const Access access = std::max(access_of(p.i, p.rows, p.sum, ACROSS_I), access_of(p.j, p.cols, p.sum, ACROSS_J));
     if constexpr (!ACROSS_I && !ACROSS_J) {
         if (p.rows <= kFewRows) {
             const dim3 grid((unsigned)((p.cols + kFewOutputs - 1) / kFewOutputs));
@@ -762,9 +849,9 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
             return TCBNN_OK;
         }
     }
-    const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), vectors, workspace_bytes);
-    auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto whole) {
-        constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value;
+    const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
+    auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold) {
+        constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value, H = hold.value;
         constexpr int kSteps = kStepBytes / (int)sizeof(T);
         p.tiles_i = (p.rows + B - 1) / B;
         p.tiles_j = (p.cols + B - 1) / B;
@@ -773,7 +860,7 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
         p.splits = std::max(1, (p.sum + p.split_sum - 1) / p.split_sum);
         p.partial = workspace;
         const long long units = (long long)p.tiles_i * p.tiles_j * p.splits;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, ACROSS_I, ACROSS_J, whole.value>), dim3((unsigned)units),
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, ACROSS_I, ACROSS_J>), dim3((unsigned)units),
                            dim3(64 * WI * WJ * WS), 0, stream, p);
         if (p.splits > 1) {
             const long long vectors_out = (long long)p.rows * ((p.cols + Elem<T>::kVec - 1) / Elem<T>::kVec);
@@ -788,20 +875,25 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
     constexpr std::integral_constant<int, 2> two;
     constexpr std::integral_constant<int, 4> four;
     constexpr std::integral_constant<int, 8> eight;
-    if (vectors) {
+    constexpr std::integral_constant<Access, WHOLE_PIECES> pieces;
+    constexpr std::integral_constant<Access, ANYWHERE> anywhere;
+    constexpr std::integral_constant<Access, ELEMENTS> elements;
+    if (access == WHOLE_PIECES) {
         switch (plan.cut) {
-            case CUT_256: go(n256, two, four, one, two, std::true_type()); break;
-            case CUT_128: go(n128, two, two, one, two, std::true_type()); break;
-            case CUT_128_DEEP: go(n128, two, two, two, four, std::true_type()); break;
-            case CUT_64: go(n64, two, two, two, four, std::true_type()); break;
-            default: go(n32, one, one, four, eight, std::true_type()); break;
+            case CUT_256: go(n256, two, four, one, two, pieces, one); break;
+            case CUT_128: go(n128, two, two, one, two, pieces, one); break;
+            case CUT_128_DEEP: go(n128, two, two, two, four, pieces, one); break;
+            case CUT_64: go(n64, two, two, two, four, pieces, one); break;
+            default: go(n32, one, one, four, eight, pieces, one); break;
+        }
+    } else if (access == ANYWHERE) {
+        switch (plan.cut) {
+            case CUT_128: go(n128, two, two, one, two, anywhere, one); break;
+            case CUT_64: go(n64, two, two, two, two, anywhere, four); break;
+            default: go(n32, one, one, four, two, anywhere, four); break;
         }
     } else {
-        switch (plan.cut) {
-            case CUT_128: go(n128, two, two, one, two, std::false_type()); break;
-            case CUT_64: go(n64, two, two, one, two, std::false_type()); break;
-            default: go(n32, one, one, four, two, std::false_type()); break;
-        }
+        go(n32, one, one, four, two, elements, one);
     }
     TCBNN_LAUNCH_CHECK("product_kernel");
     return TCBNN_OK;
