@@ -187,14 +187,15 @@ __global__ __launch_bounds__(kLongThreads) void layernorm_long_kernel(const T* x
 
 // ---- gradient.  A workgroup of 16 wavefronts is 16 / W teams; all of them take the same number of steps (a team without a
 // row of its own computes on the last one and keeps nothing).  PARAMS: sums over the workgroup's rows of dy xh and
-// dy, one row of `partial` a workgroup: [2][n] each.
+// dy, one row of `partial` a workgroup: [2][n] each; a workgroup that has all rows writes the gradients themselves.
 constexpr int kGradThreads = 1024;
 
 template <typename T, int W, int R, bool PARAMS>
 __global__ __launch_bounds__(kGradThreads) void layernorm_grad_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
                                                                       const float* __restrict__ mean_in,
                                                                       const float* __restrict__ rstd_in, const T* dy, T* dx,
-                                                                      float* __restrict__ partial, int rows, int n, long long x_ld,
+                                                                      float* __restrict__ partial, float* __restrict__ dgamma,
+                                                                      float* __restrict__ dbeta, int rows, int n, long long x_ld,
                                                                       long long dy_ld, long long dx_ld) {
     constexpr int kTeams = kGradThreads / (64 * W);
     using Slice = RowSlice<T, W, R>;
@@ -266,16 +267,16 @@ __global__ __launch_bounds__(kGradThreads) void layernorm_grad_kernel(const T* _
         }
     }
     if constexpr (PARAMS) {
-        float* out = partial + (size_t)blockIdx.x * 2 * n;
 #pragma unroll
-        for (int which = 0; which < 2; ++which)
+        for (int which = 0; which < 2; ++which) {
+            float* out = gridDim.x > 1 ? partial + ((size_t)blockIdx.x * 2 + which) * n : (which == 0 ? dgamma : dbeta);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const Slice& a = which == 0 ? dg : db;
                 if constexpr (kTeams == 1) {
 #pragma unroll
                     for (int e = 0; e < V; ++e)
-                        if (r * Slice::kStep + lane * V + e < n) out[(size_t)which * n + r * Slice::kStep + lane * V + e] = a.v[r][e];
+                        if (out && r * Slice::kStep + lane * V + e < n) out[r * Slice::kStep + lane * V + e] = a.v[r][e];
                 } else {
                     __syncthreads();
 #pragma unroll
@@ -285,10 +286,11 @@ __global__ __launch_bounds__(kGradThreads) void layernorm_grad_kernel(const T* _
                         const int e = c / (64 * W), l = c % (64 * W), i = r * Slice::kStep + l * V + e;
                         float t = 0.0f;
                         for (int k = 0; k < kTeams; ++k) t += sums[(k * V + e) * 64 * W + l];
-                        if (i < n) out[(size_t)which * n + i] = t;
+                        if (out && i < n) out[i] = t;
                     }
                 }
             }
+        }
     }
 }
 
@@ -381,8 +383,12 @@ void by_team(int vectors, F&& f) {
     return f(integral_constant<int, 16>(), integral_constant<int, 2>());
 }
 
-// workgroups whose sums over rows are joined afterwards
-inline int grad_parts(int rows) { return std::max(1, std::min(rows, kComputeUnits)); }
+// Workgroups whose sums over rows are joined afterwards.  Up to four rows a team they are one: the launch that joins them takes as
+// long as those rows (11 x 16 bf16: 6.4 us in two launches, 3.6 in one).
+inline int grad_parts(int rows, int teams) {
+    const int steps = (rows + teams - 1) / teams;
+    return steps <= 4 ? 1 : std::min(steps, kComputeUnits);
+}
 
 int check_norm(int rows, int features, int dtype) {
     TCBNN_REQUIRE(dtype_known(dtype), "layernorm: unknown dtype");
@@ -431,7 +437,7 @@ extern "C" int tcbnn_layernorm_forward(const tcbnn_layernorm_desc* d, void* stre
 
 extern "C" size_t tcbnn_layernorm_grad_workspace_bytes(int rows, int features) {
     if (rows <= 0 || features <= 0 || features > kMaxFeatures) return 0;
-    return (size_t)grad_parts(rows) * 2 * features * sizeof(float);
+    return (size_t)std::min(rows, kComputeUnits) * 2 * features * sizeof(float);
 }
 
 extern "C" int tcbnn_layernorm_backward(const tcbnn_layernorm_grad_desc* d, void* stream) {
@@ -455,13 +461,14 @@ extern "C" int tcbnn_layernorm_backward(const tcbnn_layernorm_grad_desc* d, void
                   "layernorm: a gradient over another has its stride");
     float* partial = (float*)d->workspace;
     int parts = 0;
+    bool joined = false;
     if (d->rows > 0)
         by_dtype(d->dtype, [&](auto t) {
             using T = decltype(t);
             const int vectors = row_vectors(d->features, Elem<T>::kVec);
             if (vectors > kMaxVectors) {
                 if (params) {
-                    parts = grad_parts(d->rows);
+                    parts = std::min(d->rows, kComputeUnits);
                     hipLaunchKernelGGL(layernorm_columns_kernel<T>,
                                        dim3((unsigned)((d->features + kColumnThreads - 1) / kColumnThreads), (unsigned)parts),
                                        dim3(kColumnThreads), 0, (hipStream_t)stream, (const T*)d->input, d->mean, d->rstd,
@@ -475,19 +482,20 @@ extern "C" int tcbnn_layernorm_backward(const tcbnn_layernorm_grad_desc* d, void
             }
             by_team(vectors, [&](auto w, auto r) {
                 constexpr int W = w.value, R = r.value, kTeams = kGradThreads / (64 * W);
-                parts = std::min((d->rows + kTeams - 1) / kTeams, grad_parts(d->rows));
+                parts = params ? grad_parts(d->rows, kTeams) : std::min((d->rows + kTeams - 1) / kTeams, kComputeUnits);
                 auto launch = [&](auto kernel) {
                     hipLaunchKernelGGL(kernel, dim3((unsigned)parts), dim3(kGradThreads), 0, (hipStream_t)stream, (const T*)d->input,
-                                       d->gamma, d->mean, d->rstd, (const T*)d->grad_output, (T*)d->grad_input, partial, d->rows,
-                                       d->features, x_ld, dy_ld, dx_ld);
+                                       d->gamma, d->mean, d->rstd, (const T*)d->grad_output, (T*)d->grad_input, partial, d->grad_gamma,
+                                       d->grad_beta, d->rows, d->features, x_ld, dy_ld, dx_ld);
                 };
+                joined = params && parts == 1;
                 if (params)
                     launch(layernorm_grad_kernel<T, W, R, true>);
                 else if (d->grad_input)
                     launch(layernorm_grad_kernel<T, W, R, false>);
             });
         });
-    if (params)
+    if (params && !joined)
         hipLaunchKernelGGL(layernorm_join_kernel, dim3((unsigned)((d->features + kJoinFeatures - 1) / kJoinFeatures), 2), dim3(kJoinThreads),
                            0, (hipStream_t)stream, partial, d->grad_gamma, d->grad_beta, parts, d->features);
     TCBNN_LAUNCH_CHECK("layernorm_grad_kernel");

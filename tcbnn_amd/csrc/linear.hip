@@ -345,9 +345,14 @@ __device__ __forceinline__ void meet() {
 // A workgroup's tile of c is BI x BJ, WI x WJ wavefronts with 32 x 32 pieces of it each, WS times over: those share the quarters of a
 // step, and their sums are added at the end.  STAGES steps of both operands lie in LDS or are on their way there;
 // what goes through registers does so HOLD steps ahead.
+template <int BI, int BJ, int WI, int WJ, int WS, int STAGES>
+constexpr int product_lds() {
+    constexpr int kStages = STAGES * (BI + BJ) * kStepBytes, kOut = 32 * (32 * (BJ / WJ / 32) * 4 + 16) * WI * WJ * WS;
+    return kStages > kOut ? kStages : kOut;
+}
 template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool ACROSS_I, bool ACROSS_J>
-__global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const ProductParams p) {
-#ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves the stub out where it instantiates a tile's requests twice)
+__device__ __forceinline__ void product(const ProductParams& p, int block, char* lds) {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
     constexpr int kThreads = 64 * WI * WJ * WS, NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec, kQuarters = 4 / WS;
     constexpr bool ALIGNED = ACCESS == WHOLE_PIECES;
     using TileI = Tile<T, BI, ACROSS_I, ACCESS, kThreads, HOLD>;
@@ -356,14 +361,13 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const Produc
     // a wavefront's 32 rows of c on their way out, 16 bytes between rows
     constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
     static_assert(ALIGNED || STAGES == 2, "what registers hold needs two tiles");
-    constexpr int kOut = kOutWave * WI * WJ * WS, kLds = STAGES * kStage > kOut ? STAGES * kStage : kOut;
-    __shared__ __align__(1024) char lds[kLds];
+    static_assert(ALIGNED || STAGES == 2, "what registers hold needs two tiles");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // Workgroups go to the 8 XCDs in turn: each XCD gets a run of tiles, and a run covers 8 tiles of i after 8 tiles of i, so that what
     // runs at one time on an XCD shares its operands' tiles in that XCD's L2.
     const int tiles = p.tiles_i * p.tiles_j, units = tiles * p.splits;
-    const int xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
+    const int xcd = block % 8, nth = block / 8;
     const int unit = xcd * (units / 8) + min(xcd, units % 8) + nth;
     const int split = unit / tiles, tile = unit % tiles;
     const int band = tile / (8 * p.tiles_j), in_band = tile % (8 * p.tiles_j), high = min(8, p.tiles_i - 8 * band);
@@ -569,6 +573,11 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const Produc
     }
 #endif
 }
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool ACROSS_I, bool ACROSS_J>
+__global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const ProductParams p) {
+    __shared__ __align__(1024) char lds[product_lds<BI, BJ, WI, WJ, WS, STAGES>()];
+    product<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, ACROSS_I, ACROSS_J>(p, blockIdx.x, lds);
+}
 
 // the sums of all splits and what follows them
 template <typename T>
@@ -684,11 +693,13 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
 // a time; the workgroups' sums are joined afterwards, always in the same order.
 constexpr int kDzThreads = 256;
 // Rows that one thread takes, and the parts that a column's sum falls into (a part a workgroup).
+inline int dz_lanes(int vectors) { return vectors >= kDzThreads ? kDzThreads : vectors; }  // of a workgroup, side by side
 inline int dz_rows(int rows, int vectors) {
     const long long threads = 1024LL * kComputeUnits;  // four workgroups a compute unit
-    return (int)std::max(8LL, ((long long)rows * vectors + threads - 1) / threads);
+    const int each = (int)std::max(8LL, ((long long)rows * vectors + threads - 1) / threads), deep = kDzThreads / dz_lanes(vectors);
+    // one part needs no join: 16 rows a thread take less time than that launch
+    return rows <= 16 * deep ? std::max(each, (rows + deep - 1) / deep) : each;
 }
-inline int dz_lanes(int vectors) { return vectors >= kDzThreads ? kDzThreads : vectors; }  // of a workgroup, side by side
 inline int dz_parts(int rows, int vectors) {
     const int deep = kDzThreads / dz_lanes(vectors) * dz_rows(rows, vectors);
     return (rows + deep - 1) / deep;
@@ -786,6 +797,17 @@ __global__ __launch_bounds__(kDzThreads) void column_join_kernel(const float* __
     }
 }
 
+// ---- both products of small gradients in one launch: the first workgroups have dx, the others dw.  A launch more takes as long as
+// these products do (102 x 24 -> 21 bf16: 15.9 us in three launches, 10.5 in two).
+template <typename T, Access ACCESS, int STAGES, int HOLD>
+__global__ __launch_bounds__(256) void small_gradients_kernel(const ProductParams dx, const ProductParams dw, int blocks_dx) {
+    __shared__ __align__(1024) char lds[product_lds<32, 32, 1, 1, 4, STAGES>()];
+    if ((int)blockIdx.x < blocks_dx)
+        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, false, true>(dx, blockIdx.x, lds);
+    else
+        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, true, true>(dw, blockIdx.x - blocks_dx, lds);
+}
+
 // The tile that a product is cut into, how often its sum is split, and its launch.
 //
 // The plan is the one with the shortest estimate, from what the tiles measured (us): a step of the sum takes `step` when a
@@ -830,14 +852,46 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
 }
 
 template <typename T, bool ACROSS_I, bool ACROSS_J>
-int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
-    TCBNN_REQUIRE((long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) <= 0x7fffffffLL, "linear: grid too large");
-    auto access_of = [](const Operand& o, int rows, int sum, bool across) {
+Access access_of(const ProductParams& p) {
+    auto of = [](const Operand& o, int rows, int sum, bool across) {
         const int row = across ? rows : sum;
         if (row < Elem<T>::kVec || o.ld * 256 * (long long)sizeof(T) > 0x7fffffffLL) return ELEMENTS;
         return (uintptr_t)o.p % 16 == 0 && o.ld * sizeof(T) % 16 == 0 && row % Elem<T>::kVec == 0 ? WHOLE_PIECES : ANYWHERE;
     };
-    const Access access = std::max(access_of(p.i, p.rows, p.sum, ACROSS_I), access_of(p.j, p.cols, p.sum, ACROSS_J));
+    return std::max(of(p.i, p.rows, p.sum, ACROSS_I), of(p.j, p.cols, p.sum, ACROSS_J));
+}
+inline void cut_product(ProductParams& p, int size, int steps_size, int splits, float* workspace) {
+    p.tiles_i = (p.rows + size - 1) / size;
+    p.tiles_j = (p.cols + size - 1) / size;
+    const int steps = (p.sum + steps_size - 1) / steps_size;
+    p.split_sum = std::max(1, (steps + splits - 1) / splits) * steps_size;
+    p.splits = std::max(1, (p.sum + p.split_sum - 1) / p.split_sum);
+    p.partial = workspace;
+}
+
+// dx and dw, where both are products of one row of 32 x 32 tiles a compute unit; false: nothing is launched
+template <typename T>
+bool launch_small_gradients(ProductParams dx, ProductParams dw, hipStream_t stream) {
+    const Access access = std::max(access_of<T, false, true>(dx), access_of<T, true, true>(dw));
+    auto small = [&](const ProductParams& p) {
+        const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0);
+        return plan.cut == CUT_32 && (long long)((p.rows + 31) / 32) * ((p.cols + 31) / 32) <= 4 * kComputeUnits;
+    };
+    if (access == ELEMENTS || !small(dx) || !small(dw)) return false;
+    cut_product(dx, 32, kStepBytes / (int)sizeof(T), 1, nullptr);
+    cut_product(dw, 32, kStepBytes / (int)sizeof(T), 1, nullptr);
+    const int blocks_dx = dx.tiles_i * dx.tiles_j, blocks = blocks_dx + dw.tiles_i * dw.tiles_j;
+    if (access == WHOLE_PIECES)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(small_gradients_kernel<T, WHOLE_PIECES, 8, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, dx, dw, blocks_dx);
+    else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(small_gradients_kernel<T, ANYWHERE, 2, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, dx, dw, blocks_dx);
+    return true;
+}
+
+template <typename T, bool ACROSS_I, bool ACROSS_J>
+int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
+    TCBNN_REQUIRE((long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) <= 0x7fffffffLL, "linear: grid too large");
+    const Access access = access_of<T, ACROSS_I, ACROSS_J>(p);
     if constexpr (!ACROSS_I && !ACROSS_J) {
         if (p.rows <= kFewRows) {
             const dim3 grid((unsigned)((p.cols + kFewOutputs - 1) / kFewOutputs));
@@ -852,13 +906,7 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
     const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
     auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold) {
         constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value, H = hold.value;
-        constexpr int kSteps = kStepBytes / (int)sizeof(T);
-        p.tiles_i = (p.rows + B - 1) / B;
-        p.tiles_j = (p.cols + B - 1) / B;
-        const int steps = (p.sum + kSteps - 1) / kSteps;
-        p.split_sum = std::max(1, (steps + plan.splits - 1) / plan.splits) * kSteps;
-        p.splits = std::max(1, (p.sum + p.split_sum - 1) / p.split_sum);
-        p.partial = workspace;
+        cut_product(p, B, kStepBytes / (int)sizeof(T), plan.splits, workspace);
         const long long units = (long long)p.tiles_i * p.tiles_j * p.splits;
         hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, ACROSS_I, ACROSS_J>), dim3((unsigned)units),
                            dim3(64 * WI * WJ * WS), 0, stream, p);
@@ -993,13 +1041,14 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
         if (active || d->grad_bias) {
             const int vectors = out_vectors(d->out_features, d->dtype), lanes = dz_lanes(vectors), parts = dz_parts(d->rows, vectors);
             float* sums = d->grad_bias ? (float*)((char*)d->workspace + dz_bytes(d->rows, d->out_features, d->dtype)) : nullptr;
+            if (d->grad_bias && parts == 1 && d->rows > 0) sums = d->grad_bias;
             if (d->rows > 0)
                 by_activation(d->activation, [&](auto act) {
                     hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<T, act.value>), dim3((unsigned)((vectors + lanes - 1) / lanes), (unsigned)parts),
                                        dim3(kDzThreads), 0, (hipStream_t)stream, (const T*)d->grad_output, (const T*)d->preact,
                                        (T*)d->workspace, sums, d->rows, d->out_features, lanes, dz_rows(d->rows, vectors), dy_ld, z_ld);
                 });
-            if (d->grad_bias)
+            if (d->grad_bias && sums != d->grad_bias)
                 hipLaunchKernelGGL(column_join_kernel, dim3((unsigned)((d->out_features + kJoinColumns - 1) / kJoinColumns)), dim3(kDzThreads), 0,
                                    (hipStream_t)stream, sums, d->grad_bias, d->rows > 0 ? parts : 0, d->out_features);
         }
@@ -1007,28 +1056,29 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
         const size_t before = dz_bytes(d->rows, d->out_features, d->dtype) + sum_bytes(d->rows, d->out_features, d->dtype);
         float* partials = d->workspace && d->workspace_bytes > before ? (float*)((char*)d->workspace + before) : nullptr;
         const size_t partial_bytes = partials ? d->workspace_bytes - before : 0;
-        ProductParams p = {};
         const Operand dz = active ? Operand{d->workspace, d->out_features} : Operand{d->grad_output, dy_ld};
-        if (d->grad_input && d->rows > 0) {
-            p.i = dz;
-            p.j = {d->weight, w_ld};
-            p.rows = d->rows;
-            p.cols = d->in_features;
-            p.sum = d->out_features;
-            p.out = d->grad_input;
-            p.out_ld = dx_ld;
-            if (int rc = launch_product<T, false, true>(p, partials, partial_bytes, (hipStream_t)stream)) return rc;
+        ProductParams dx = {}, dw = {};
+        dx.i = dw.i = dz;
+        dx.j = {d->weight, w_ld};
+        dx.rows = d->rows;
+        dx.cols = d->in_features;
+        dx.sum = d->out_features;
+        dx.out = d->grad_input;
+        dx.out_ld = dx_ld;
+        dw.j = {d->input, x_ld};
+        dw.rows = d->out_features;
+        dw.cols = d->in_features;
+        dw.sum = d->rows;
+        dw.out = d->grad_weight;
+        dw.out_ld = dw_ld;
+        if (d->grad_input && d->grad_weight && d->rows > 0 && launch_small_gradients<T>(dx, dw, (hipStream_t)stream)) {
+            TCBNN_LAUNCH_CHECK("small_gradients_kernel");
+            return TCBNN_OK;
         }
-        if (d->grad_weight) {
-            p.i = dz;
-            p.j = {d->input, x_ld};
-            p.rows = d->out_features;
-            p.cols = d->in_features;
-            p.sum = d->rows;
-            p.out = d->grad_weight;
-            p.out_ld = dw_ld;
-            if (int rc = launch_product<T, true, true>(p, partials, partial_bytes, (hipStream_t)stream)) return rc;
-        }
+        if (d->grad_input && d->rows > 0)
+            if (int rc = launch_product<T, false, true>(dx, partials, partial_bytes, (hipStream_t)stream)) return rc;
+        if (d->grad_weight)
+            if (int rc = launch_product<T, true, true>(dw, partials, partial_bytes, (hipStream_t)stream)) return rc;
         return TCBNN_OK;
     });
 }

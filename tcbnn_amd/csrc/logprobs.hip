@@ -169,7 +169,16 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
     x += row * p.ld + base;
 
     Words raw[R];
-    load_slices<T, R>(x, n, tid, kTeam, raw);
+    // Short rows are dealt to the lanes one by one: in vectors, most lanes would have none, and the groups' maxima bound little.
+    constexpr bool kDealt = W == 1 && R == 1;
+    if constexpr (kDealt) {
+        Vec<T> v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = e * 64 + tid < n ? x[e * 64 + tid] : (T)-INFINITY;
+        raw[0] = __builtin_bit_cast(Words, v);
+    } else {
+        load_slices<T, R>(x, n, tid, kTeam, raw);
+    }
     const int target = p.targets ? p.targets[row] : -1;
     const bool given = target >= 0 && target < p.classes;
     const int t = target - base;  // within the chunk, before it or behind it
@@ -199,7 +208,7 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
     uint32_t signs = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const float bound = r * kStep + tid * V + V <= t ? below : xt;
+        float bound = r * kStep + tid * V + V <= t ? below : xt;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const float v = value<T>(raw[r], e);
@@ -207,6 +216,7 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
             const float ex = __builtin_amdgcn_exp2f(u);
             part.s += ex;
             part.sx = __builtin_fmaf(ex, fmaxf(u, -250.0f), part.sx);
+            if constexpr (kDealt) bound = e * 64 + tid < t ? below : xt;
             // the sign of bound - v, shifted in from below (comparisons write a scalar, which the addition then waits for)
             signs = __builtin_amdgcn_alignbit(signs, __float_as_uint(bound - v), 31);
         }
@@ -228,7 +238,7 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
         part.sx = __builtin_fmaf(-off, part.s, part.sx) * kLn2;
         part.s = __builtin_fmaf(-off * kLn2, part.s, part.s);
     }
-    if (wave == 0 && t >= 0 && t < n && lane < t % V) part.before += (float)x[t - 1 - lane] == xt;
+    if (!kDealt && wave == 0 && t >= 0 && t < n && lane < t % V) part.before += (float)x[t - 1 - lane] == xt;
     part.before = wave_sum_int(part.before);
     part.s = wave_sum(part.s);
     part.sx = wave_sum(part.sx);
@@ -294,16 +304,22 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
             const int at = atomicAdd(&lds.count, 1);
             if (at < kList) lds.list[at] = key_of(v, j);
         };
-        uint32_t hot = 0;  // the vectors that reach the bound: few, and read again (from the cache)
-#pragma unroll
-        for (int r = 0; r < R; ++r) hot |= vec_max[r] >= bound ? 1u << r : 0u;
-        while (hot != 0) {
-            const int j = __builtin_ctz(hot) * kStep + tid * V;
-            hot &= hot - 1;
-            const Words w = j + V <= n ? load_words(x + j) : load_rest(x + j, n - j);
+        if constexpr (kDealt) {
 #pragma unroll
             for (int e = 0; e < V; ++e)
-                if (value<T>(w, e) >= bound && j + e < n) push(j + e, value<T>(w, e));
+                if (value<T>(raw[0], e) >= bound && e * 64 + tid < n) push(e * 64 + tid, value<T>(raw[0], e));
+        } else {
+            uint32_t hot = 0;  // the vectors that reach the bound: few, and read again (from the cache)
+#pragma unroll
+            for (int r = 0; r < R; ++r) hot |= vec_max[r] >= bound ? 1u << r : 0u;
+            while (hot != 0) {
+                const int j = __builtin_ctz(hot) * kStep + tid * V;
+                hot &= hot - 1;
+                const Words w = j + V <= n ? load_words(x + j) : load_rest(x + j, n - j);
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (value<T>(w, e) >= bound && j + e < n) push(j + e, value<T>(w, e));
+            }
         }
         team_sync<W>();
         count = lds.count;
@@ -344,6 +360,7 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
         for (int i = tid; i < count; i += kTeam) {
             const uint64_t key = lds.list[i];
             int place = 0;
+#pragma unroll 8
             for (int k = 0; k < count; ++k) place += lds.list[k] > key;
             if (place < top) emit(place, key);
         }
@@ -427,6 +444,7 @@ __global__ __launch_bounds__(64 * kJoinRows) void logprobs_join_kernel(const T* 
         for (int i = lane; i < count; i += 64) {
             const uint64_t key = lists[wave][i];
             int place = 0;
+#pragma unroll 8
             for (int k = 0; k < count; ++k) place += lists[wave][k] > key;
             if (place < p.top) write_top(p, row, answer, place, key);
         }

@@ -13,7 +13,6 @@ import numpy as np
 from . import _lib
 from ._lib import check, lib
 from .device import DeviceBuffer
-from .layers import _stream_handle
 
 
 def encode(values, dtype):
@@ -54,7 +53,11 @@ class _HeadLayer:
             raise _lib.TcbnnError("Error: %s: unknown dtype %r" % (name, dtype))
         self.name, self.dtype = name, dtype
         self._owned = []
-        self._desc = self._grad_desc = None
+        self._desc = self._grad_desc = None  # kept by the calls below
+        self._forward = self._backward = self._not_initialized
+
+    def _not_initialized(self, handle):
+        raise _lib.TcbnnError("Error: %s: not initialized" % self.name)
 
     def _itemsize(self):
         return 4 if self.dtype == "f32" else 2
@@ -82,16 +85,31 @@ class _HeadLayer:
             raise _lib.TcbnnError("Error: NULL pointer (%s: %s)" % (self.name, what))
         return buf
 
-    def _run(self, entry, desc, stream):
-        if desc is None:
-            raise _lib.TcbnnError("Error: %s: not initialized" % self.name)
-        check(entry(C.byref(desc), _stream_handle(stream)))
+    @staticmethod
+    def _call(entry, desc):
+        """A call of the entry point with this descriptor, on a stream's handle (what does not change is made once: a small
+        layer takes no longer on the GPU than its call does here)."""
+        ref = C.byref(desc)
+
+        def call(handle):
+            rc = entry(ref, handle)
+            if rc:
+                check(rc)
+
+        return call
+
+    def forward(self, stream=None):
+        self._forward(None if stream is None else stream.handle)
+
+    def backward(self, stream=None):
+        self._backward(None if stream is None else stream.handle)
 
     def release(self):
         for buf in self._owned:
             buf.free()
         self._owned = []
         self._desc = self._grad_desc = None
+        self._forward = self._backward = self._not_initialized
 
 
 class LinearLayerParam(_HeadLayer):
@@ -121,6 +139,7 @@ class LinearLayerParam(_HeadLayer):
             self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), _ptr(self.residual_gpu), self.output_gpu.ptr,
             _ptr(self.preact_gpu), m, k, n, _lib.DTYPES[self.dtype], _lib.ACTIVATIONS[self.activation], _ld(self.input_gpu),
             _ld(self.weight_gpu), _ld(self.residual_gpu), _ld(self.output_gpu), _ld(self.preact_gpu), _ptr(ws), nbytes)
+        self._forward = self._call(lib.tcbnn_linear_forward, self._desc)
         return self
 
     def initialize_backward(self, grad_output_gpu, grad_input_gpu=None, grad_weight_gpu=None, grad_bias_gpu=None):
@@ -139,16 +158,11 @@ class LinearLayerParam(_HeadLayer):
             _ptr(grad_weight_gpu), _ptr(grad_bias_gpu), m, k, n, _lib.DTYPES[self.dtype], _lib.ACTIVATIONS[self.activation],
             _ld(self.input_gpu), _ld(self.weight_gpu), _ld(self.preact_gpu), _ld(grad_output_gpu), _ld(grad_input_gpu),
             _ld(grad_weight_gpu), _ptr(ws), nbytes)
+        self._backward = self._call(lib.tcbnn_linear_backward, self._grad_desc)
         return self
 
     def get_output_gpu(self):
         return self.output_gpu
-
-    def forward(self, stream=None):
-        self._run(lib.tcbnn_linear_forward, self._desc, stream)
-
-    def backward(self, stream=None):
-        self._run(lib.tcbnn_linear_backward, self._grad_desc, stream)
 
     def download_output(self):
         """fp32 [rows][out_features] of a buffer without gaps between rows."""
@@ -173,6 +187,7 @@ class LayerNormLayerParam(_HeadLayer):
         self._desc = _lib.LayerNormDesc(
             self.input_gpu.ptr, _ptr(self.gamma_gpu), _ptr(self.beta_gpu), self.output_gpu.ptr, self.mean_gpu.ptr, self.rstd_gpu.ptr,
             m, n, _lib.DTYPES[self.dtype], self.eps, _ld(self.input_gpu), _ld(self.output_gpu))
+        self._forward = self._call(lib.tcbnn_layernorm_forward, self._desc)
         return self
 
     def initialize_backward(self, grad_output_gpu, grad_input_gpu=None, grad_gamma_gpu=None, grad_beta_gpu=None):
@@ -188,16 +203,11 @@ class LayerNormLayerParam(_HeadLayer):
             self.input_gpu.ptr, _ptr(self.gamma_gpu), self.mean_gpu.ptr, self.rstd_gpu.ptr, self.grad_output_gpu.ptr,
             _ptr(grad_input_gpu), _ptr(grad_gamma_gpu), _ptr(grad_beta_gpu), m, n, _lib.DTYPES[self.dtype], _ld(self.input_gpu),
             _ld(grad_output_gpu), _ld(grad_input_gpu), _ptr(ws), nbytes)
+        self._backward = self._call(lib.tcbnn_layernorm_backward, self._grad_desc)
         return self
 
     def get_output_gpu(self):
         return self.output_gpu
-
-    def forward(self, stream=None):
-        self._run(lib.tcbnn_layernorm_forward, self._desc, stream)
-
-    def backward(self, stream=None):
-        self._run(lib.tcbnn_layernorm_backward, self._grad_desc, stream)
 
     def download_output(self):
         """fp32 [rows][features] of a buffer without gaps between rows."""
@@ -234,6 +244,7 @@ class LogProbsLayerParam(_HeadLayer):
             self.logits_gpu.ptr, _ptr(targets_gpu), _ptr(self.logprob_gpu), _ptr(self.entropy_gpu), _ptr(self.logsumexp_gpu),
             _ptr(self.rank_gpu), _ptr(self.top_index_gpu), _ptr(self.top_logprob_gpu), m, n, k, _lib.DTYPES[self.dtype],
             _ld(self.logits_gpu), _ptr(ws), nbytes)
+        self._forward = self._call(lib.tcbnn_logprobs_forward, self._desc)
         return self
 
     def initialize_backward(self, grad_logprob_gpu, grad_entropy_gpu, grad_logits_gpu):
@@ -247,13 +258,8 @@ class LogProbsLayerParam(_HeadLayer):
         self._grad_desc = _lib.LogProbsGradDesc(
             self.logits_gpu.ptr, _ptr(self.targets_gpu), self.logsumexp_gpu.ptr, self.entropy_gpu.ptr, _ptr(grad_logprob_gpu),
             _ptr(grad_entropy_gpu), grad_logits_gpu.ptr, m, n, _lib.DTYPES[self.dtype], _ld(self.logits_gpu), _ld(grad_logits_gpu))
+        self._backward = self._call(lib.tcbnn_logprobs_backward, self._grad_desc)
         return self
-
-    def forward(self, stream=None):
-        self._run(lib.tcbnn_logprobs_forward, self._desc, stream)
-
-    def backward(self, stream=None):
-        self._run(lib.tcbnn_logprobs_backward, self._grad_desc, stream)
 
     def download_output(self):
         """dict of the host arrays of what forward() wrote."""
