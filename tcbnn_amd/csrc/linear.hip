@@ -99,7 +99,8 @@ __device__ __forceinline__ Acc mma(Words j, Words i, Acc c) {
 
 // ---- an operand's tiles.  A step of the sum is 128 bytes of a row (64 elements of 16 bits, 32 of fp32); a tile is `ROWS` rows
 // (i or j) of a step, in LDS in pieces of 16 bytes as it lies in memory:
-//   along the sum:  [ROWS][8 pieces], piece c of row r at place c ^ (r % 8): the 64 lanes of a fragment read 32 rows at once;
+//   along the sum:  [ROWS][8 pieces], piece c of row r at place c ^ (r / 2 % 8): 16 lanes read a piece of 16 rows at a time, and
+//                   two rows cover all banks;
 //   across the sum: [64 or 32 steps][ROWS elements], pieces exchanged so that the rows which one instruction reads lie in
 //                   different banks.  A fragment then is two transposing reads of four elements (16 bits), or four of one.
 typedef __attribute__((address_space(3))) void LdsVoid;
@@ -131,7 +132,7 @@ struct Tile {
     int valid;  // rows of the tile that exist
 
     static __device__ __forceinline__ int swizzle(int row) {
-        if constexpr (!ACROSS) return row & 7;
+        if constexpr (!ACROSS) return (row >> 1) & 7;
         if constexpr (sizeof(T) == 4) return kRowPieces >= 16 ? ((row >> 2) & 1) << 3 : 0;
         return kRowPieces >= 16 ? (row & 3) << 2 : (kRowPieces == 8 ? ((row >> 1) & 1) << 2 : 0);
     }
@@ -254,7 +255,7 @@ struct Tile {
         const int lane = threadIdx.x & 63, h = lane >> 5;
         if constexpr (!ACROSS) {
             const int row = first + (lane & 31);
-            return *reinterpret_cast<const Words*>(lds + row * 128 + (((2 * k + h) ^ (lane & 7)) << 4));
+            return *reinterpret_cast<const Words*>(lds + row * 128 + (((2 * k + h) ^ swizzle(lane)) << 4));
         } else if constexpr (sizeof(T) == 2) {
             typedef short S4 __attribute__((ext_vector_type(4)));
             typedef int I2 __attribute__((ext_vector_type(2)));
