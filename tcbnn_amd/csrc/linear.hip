@@ -165,7 +165,6 @@ struct Tile {
     // requests the tile of the step that begins at `s` of `sum`: into LDS at once, or into the registers of a slot
     template <int SLOT>
     __device__ __forceinline__ void request(char* lds, int s, int sum) {
-        const bool whole = s + kSteps <= sum;
         if constexpr (ACCESS == WHOLE_PIECES) {
             const __amdgpu_buffer_rsrc_t r =
                 __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(ACROSS ? base + s * ld : base), 0, 0x7fffffff, 0x00020000);
@@ -173,7 +172,7 @@ struct Tile {
             for (int e = 0; e < kEach; ++e) {
                 int row, piece;
                 where(e, row, piece);
-                const bool there = whole || s + (ACROSS ? row : piece * V) < sum;
+                const bool there = s + (ACROSS ? row : piece * V) < sum;
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(lds + (e * THREADS + wave_first()) * 16), 16,
                                                          there ? offset[e] : kOutOfRange, ACROSS ? 0 : s * (int)sizeof(T), 0, 0);
             }
@@ -390,27 +389,18 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
             for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.0f;
 
     using std::integral_constant;
-    auto request = [&](int stage, int step, auto slot) {
-        const int s = s0 + step * TileI::kSteps;
-        ti.template request<slot.value>(lds + stage * kStage, s, s1);
-        tj.template request<slot.value>(lds + stage * kStage + TileI::kBytes, s, s1);
+    constexpr integral_constant<int, 0> slot0;
+    const int steps = (s1 - s0 + TileI::kSteps - 1) / TileI::kSteps;
+    // (a step past the last one: requests that touch no memory)
+    auto request_i = [&](int stage, int step, auto slot) { ti.template request<slot.value>(lds + stage * kStage, s0 + step * TileI::kSteps, s1); };
+    auto request_j = [&](int stage, int step, auto slot) {
+        tj.template request<slot.value>(lds + stage * kStage + TileI::kBytes, s0 + step * TileI::kSteps, s1);
     };
-    // the next step's tiles are in LDS, for all to read; `rest` steps after it have been requested
-    constexpr int kRequests = TileI::kEach + TileJ::kEach;
-    auto arrived = [&](int stage, int step, int rest, auto slot) {
-        if constexpr (ALIGNED) {
-            if (rest >= STAGES - 1)
-                meet<(STAGES - 1) * kRequests>();
-            else if (STAGES > 2 && rest == STAGES - 2)
-                meet<(STAGES - 2) * kRequests>();
-            else
-                meet<0>();
-        } else {
-            const int s = s0 + step * TileI::kSteps;
-            ti.template store<slot.value>(lds + stage * kStage, s, s1);
-            tj.template store<slot.value>(lds + stage * kStage + TileI::kBytes, s, s1);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (requests into registers stay under way)
-        }
+    // (registers only) a slot's step goes to LDS, for all to read
+    auto hand_over = [&](int stage, int step, auto slot) {
+        ti.template store<slot.value>(lds + stage * kStage, s0 + step * TileI::kSteps, s1);
+        tj.template store<slot.value>(lds + stage * kStage + TileI::kBytes, s0 + step * TileI::kSteps, s1);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (requests into registers stay under way)
     };
     // A step's fragments come a quarter ahead of their instructions, the first quarter's from the next step's tiles: so the barrier
     // that hands these over, and the request for the step after it into the tiles that are done with, lie before the last quarter's
@@ -430,81 +420,108 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
 #pragma unroll
             for (int b = 0; b < NJ; ++b) acc[a][b] = mma<T>(fj[set][b], fi[set][a], acc[a][b]);
     };
-    const int steps = (s1 - s0 + TileI::kSteps - 1) / TileI::kSteps;
-    // steps under way at a time: the tiles in LDS, or the slots of registers
-    constexpr int kAhead = ALIGNED ? STAGES : HOLD;
-    auto each = [&](auto f) {
-        f(integral_constant<int, 0>());
-        if constexpr (kAhead > 1) f(integral_constant<int, 1>());
-        if constexpr (kAhead > 2) f(integral_constant<int, 2>());
-        if constexpr (kAhead > 3) f(integral_constant<int, 3>());
-        if constexpr (kAhead > 4) {
-            static_assert(kAhead == 8, "");
-            f(integral_constant<int, 4>()), f(integral_constant<int, 5>()), f(integral_constant<int, 6>()), f(integral_constant<int, 7>());
+    // One request of LDS after a matrix instruction, and one of memory after every other: a burst of either holds all wavefronts
+    // while the matrix cores wait.  `reads` and `requests` are those of the code up to here.
+    constexpr int kInstr = NI * NJ * (sizeof(T) == 4 ? 4 : 1);
+    auto interleave = [](auto reads, auto requests) {
+        constexpr int kPer = (reads.value + kInstr - 1) / kInstr, kEvery = requests.value > 0 ? std::max(1, kInstr / std::max(1, requests.value)) : kInstr + 1;
+        constexpr int kPerRequest = (requests.value + kInstr - 1) / kInstr;
+#pragma unroll
+        for (int q = 0; q < kInstr; ++q) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (q * kPer < reads.value) __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
+            if (requests.value > 0 && q % kEvery == 0) __builtin_amdgcn_sched_group_barrier(0x010, std::max(1, kPerRequest), 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
+    constexpr integral_constant<int, NI * TileI::kReads + NJ * TileJ::kReads> reads;
+    constexpr integral_constant<int, TileI::kEach> requests_i;
+    constexpr integral_constant<int, TileJ::kEach> requests_j;
+    constexpr int kRequests = TileI::kEach + TileJ::kEach;
     int stage = 0;
-    // `slot` (unaligned operands): step % HOLD
-    auto advance = [&](int step, auto slot) {
-        const int next = stage + 1 == STAGES ? 0 : stage + 1;
-        constexpr integral_constant<int, (slot.value + 1) % HOLD> next_slot;
-#pragma unroll
-        for (int k = 0; k + 1 < kQuarters; ++k) {
-            fragments((k + 1) & 1, stage, k + 1);
-            multiply(k & 1);
-            // a request or two of LDS to a matrix instruction: all at once, they hold both wavefronts of a SIMD
-            constexpr int kReads = NI * TileI::kReads + NJ * TileJ::kReads, kInstr = NI * NJ * (sizeof(T) == 4 ? 4 : 1);
-            constexpr int kPer = (kReads + kInstr - 1) / kInstr, kGroups = (kReads + kPer - 1) / kPer;
-#pragma unroll
-            for (int q = 0; q < kGroups; ++q) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
-            }
-            if constexpr (kInstr > kGroups) __builtin_amdgcn_sched_group_barrier(0x008, kInstr - kGroups, 0);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if (step + 1 < steps) {
-            arrived(next, step + 1, min(steps - 1, step + kAhead - 1) - (step + 1), next_slot);
-            if constexpr (ALIGNED) {
-                if (step + STAGES < steps) request(stage, step + STAGES, slot);
-            } else {
-                if (step + 1 + HOLD < steps) request(0, step + 1 + HOLD, next_slot);
-            }
-            fragments(kQuarters & 1, next, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        multiply((kQuarters - 1) & 1);
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (kQuarters == 1) {  // (registers have no index: the next step's fragments take the place of this one's)
-#pragma unroll
-            for (int a = 0; a < NI; ++a) fi[0][a] = fi[1][a];
-#pragma unroll
-            for (int b = 0; b < NJ; ++b) fj[0][b] = fj[1][b];
-        }
-        stage = next;
-    };
     if (steps > 0) {
         if constexpr (ALIGNED) {
-            each([&](auto k) {
-                if (k.value < steps) request(k.value, k.value, integral_constant<int, 0>());
-            });
-            arrived(0, 0, min(steps, STAGES) - 1, integral_constant<int, 0>());
+            // Step t + STAGES is requested into the tiles of step t as soon as these are done with: J's with the last quarter of step
+            // t, I's with the first of step t + 1 (where a wavefront has a quarter alone, both at once).
+            constexpr bool kApart = kQuarters > 1;
+#pragma unroll
+            for (int k = 0; k < STAGES; ++k) {
+                request_j(k, k, slot0);
+                if (!kApart || k + 1 < STAGES) request_i(k, k, slot0);
+            }
+            meet<(STAGES - 1) * kRequests - (kApart ? TileI::kEach : 0)>();
+            fragments(0, 0, 0);
+            for (int step = 0; step < steps; ++step) {
+                const int next = stage + 1 == STAGES ? 0 : stage + 1;
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k + 1 < kQuarters; ++k) {
+                    if (kApart && k == 0) request_i(stage == 0 ? STAGES - 1 : stage - 1, step + STAGES - 1, slot0);
+                    fragments((k + 1) & 1, stage, k + 1);
+                    multiply(k & 1);
+                    if (kApart && k == 0)
+                        interleave(reads, requests_i);
+                    else
+                        interleave(reads, slot0);
+                }
+                meet<(STAGES - 2) * kRequests>();
+                request_j(stage, step + STAGES, slot0);
+                if (!kApart) request_i(stage, step + STAGES, slot0);
+                fragments(kQuarters & 1, next, 0);
+                multiply((kQuarters - 1) & 1);
+                if constexpr (kApart) interleave(reads, requests_j);
+                if constexpr (kQuarters == 1) {  // (registers have no index: the next step's fragments take the place of this one's)
+#pragma unroll
+                    for (int a = 0; a < NI; ++a) fi[0][a] = fi[1][a];
+#pragma unroll
+                    for (int b = 0; b < NJ; ++b) fj[0][b] = fj[1][b];
+                }
+                stage = next;
+            }
+            meet<0>();
         } else {
+            auto each = [&](auto f) {
+                f(integral_constant<int, 0>());
+                if constexpr (HOLD == 4) f(integral_constant<int, 1>()), f(integral_constant<int, 2>()), f(integral_constant<int, 3>());
+            };
+            static_assert(HOLD == 1 || HOLD == 4, "");
             each([&](auto k) {
-                if (k.value < steps) request(0, k.value, k);
+                if (k.value < steps) request_i(0, k.value, k), request_j(0, k.value, k);
             });
-            arrived(0, 0, 0, integral_constant<int, 0>());
-            if (HOLD < steps) request(0, HOLD, integral_constant<int, 0>());
+            hand_over(0, 0, slot0);
+            if (HOLD < steps) request_i(0, HOLD, slot0), request_j(0, HOLD, slot0);
+            fragments(0, 0, 0);
+            // `slot`: step % HOLD
+            auto advance = [&](int step, auto slot) {
+                const int next = stage ^ 1;
+                constexpr integral_constant<int, (slot.value + 1) % HOLD> next_slot;
+#pragma unroll
+                for (int k = 0; k + 1 < kQuarters; ++k) {
+                    fragments((k + 1) & 1, stage, k + 1);
+                    multiply(k & 1);
+                    interleave(reads, slot0);
+                }
+                if (step + 1 < steps) {
+                    hand_over(next, step + 1, next_slot);
+                    if (step + 1 + HOLD < steps) request_i(0, step + 1 + HOLD, next_slot), request_j(0, step + 1 + HOLD, next_slot);
+                    fragments(kQuarters & 1, next, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                multiply((kQuarters - 1) & 1);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (kQuarters == 1) {
+#pragma unroll
+                    for (int a = 0; a < NI; ++a) fi[0][a] = fi[1][a];
+#pragma unroll
+                    for (int b = 0; b < NJ; ++b) fj[0][b] = fj[1][b];
+                }
+                stage = next;
+            };
+            for (int step = 0; step < steps; step += HOLD)
+                each([&](auto k) {
+                    if (step + k.value < steps) advance(step + k.value, k);
+                });
         }
-        fragments(0, 0, 0);
-    }
-    if constexpr (ALIGNED) {
-        for (int step = 0; step < steps; ++step) advance(step, integral_constant<int, 0>());
-    } else {
-        for (int step = 0; step < steps; step += HOLD)
-            each([&](auto k) {
-                if (step + k.value < steps) advance(step + k.value, k);
-            });
     }
     __syncthreads();
 
