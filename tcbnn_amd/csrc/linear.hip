@@ -117,7 +117,8 @@ struct Operand {
 // bits hold for a tile (element by element).
 enum Access : int { WHOLE_PIECES, ANYWHERE, ELEMENTS };
 
-template <typename T, int ROWS, bool ACROSS, Access ACCESS, int THREADS, int SLOTS>
+// HIDDEN: the compiler is not to know of requests into LDS (below).
+template <typename T, int ROWS, bool ACROSS, Access ACCESS, int THREADS, int SLOTS, bool HIDDEN>
 struct Tile {
     static constexpr int V = Elem<T>::kVec, kSteps = kStepBytes / (int)sizeof(T);
     static constexpr int kBytes = ROWS * kStepBytes, kPieces = kBytes / 16, kEach = kPieces / THREADS;
@@ -162,20 +163,35 @@ struct Tile {
             }
         }
     }
-    // requests the tile of the step that begins at `s` of `sum`: into LDS at once, or into the registers of a slot
+    // requests a piece of the step that begins at `s` of `sum` into LDS
+    __device__ __forceinline__ void request_piece(char* lds, int s, int sum, int e) {
+        int row, piece;
+        where(e, row, piece);
+        const int at = s + (ACROSS ? row : piece * V) < sum ? offset[e] : kOutOfRange;
+        char* to = lds + (e * THREADS + wave_first()) * 16;
+        const T* from = ACROSS ? base + s * ld : base;
+        if constexpr (HIDDEN) {
+            // The builtin makes the compiler wait for it before every transposing read of LDS, whichever tile that reads; what is in
+            // LDS is for meet() to wait for.  (m0: where in LDS; nothing comes back into registers.)
+            const unsigned long long address = (unsigned long long)(uintptr_t)from;
+            const Words r = {__builtin_amdgcn_readfirstlane((int)address), __builtin_amdgcn_readfirstlane((int)(address >> 32) & 0xffff), 0x7fffffff,
+                             0x00020000};
+            // Five wait states: a vector instruction may have written the descriptor's registers just before.  Never remove them.
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(
+                             __builtin_amdgcn_readfirstlane((int)(uintptr_t)(LdsVoid*)to)),
+                         "v"(at), "s"(r), "s"(ACROSS ? 0 : s * (int)sizeof(T))
+                         : "memory", "m0");
+        } else {
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(from), 0, 0x7fffffff, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)to, 16, at, ACROSS ? 0 : s * (int)sizeof(T), 0, 0);
+        }
+    }
+    // requests the tile of a step: into LDS at once, or into the registers of a slot
     template <int SLOT>
     __device__ __forceinline__ void request(char* lds, int s, int sum) {
         if constexpr (ACCESS == WHOLE_PIECES) {
-            const __amdgpu_buffer_rsrc_t r =
-                __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(ACROSS ? base + s * ld : base), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                int row, piece;
-                where(e, row, piece);
-                const bool there = s + (ACROSS ? row : piece * V) < sum;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(lds + (e * THREADS + wave_first()) * 16), 16,
-                                                         there ? offset[e] : kOutOfRange, ACROSS ? 0 : s * (int)sizeof(T), 0, 0);
-            }
+            for (int e = 0; e < kEach; ++e) request_piece(lds, s, sum, e);
         } else if constexpr (ACCESS == ANYWHERE) {
             // (no branches: then the requests of several steps can be told apart by their number)
             const char* from = reinterpret_cast<const char*>(ACROSS ? base + s * ld : base);
@@ -355,8 +371,9 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
     constexpr int kThreads = 64 * WI * WJ * WS, NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec, kQuarters = 4 / WS;
     constexpr bool ALIGNED = ACCESS == WHOLE_PIECES;
-    using TileI = Tile<T, BI, ACROSS_I, ACCESS, kThreads, HOLD>;
-    using TileJ = Tile<T, BJ, ACROSS_J, ACCESS, kThreads, HOLD>;
+    constexpr bool kHidden = ALIGNED && sizeof(T) == 2 && (ACROSS_I || ACROSS_J);  // transposing reads
+    using TileI = Tile<T, BI, ACROSS_I, ACCESS, kThreads, HOLD, kHidden>;
+    using TileJ = Tile<T, BJ, ACROSS_J, ACCESS, kThreads, HOLD, kHidden>;
     constexpr int kStage = TileI::kBytes + TileJ::kBytes;
     // a wavefront's 32 rows of c on their way out, 16 bytes between rows
     constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
@@ -420,6 +437,25 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
 #pragma unroll
             for (int b = 0; b < NJ; ++b) acc[a][b] = mma<T>(fj[set][b], fi[set][a], acc[a][b]);
     };
+    // (hidden requests are where they are written: after every other matrix instruction)
+    auto multiply_and = [&](int set, auto requests, auto request_piece) {
+        constexpr int kEvery = std::max(1, NI * NJ / requests.value), kAtOnce = (requests.value + NI * NJ - 1) / (NI * NJ);
+        int e = 0;
+#pragma unroll
+        for (int a = 0; a < NI; ++a)
+#pragma unroll
+            for (int b = 0; b < NJ; ++b) {
+                acc[a][b] = mma<T>(fj[set][b], fi[set][a], acc[a][b]);
+                if ((a * NJ + b) % kEvery == 0) {
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u)
+                        if (e < requests.value) request_piece(e++);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+#pragma unroll
+        for (; e < requests.value; ++e) request_piece(e);
+    };
     // One request of LDS after a matrix instruction, and one of memory after every other: a burst of either holds all wavefronts
     // while the matrix cores wait.  `reads` and `requests` are those of the code up to here.
     constexpr int kInstr = NI * NJ * (sizeof(T) == 4 ? 4 : 1);
@@ -456,20 +492,31 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int k = 0; k + 1 < kQuarters; ++k) {
-                    if (kApart && k == 0) request_i(stage == 0 ? STAGES - 1 : stage - 1, step + STAGES - 1, slot0);
+                    const int last = stage == 0 ? STAGES - 1 : stage - 1, s = s0 + (step + STAGES - 1) * TileI::kSteps;
+                    if (kApart && k == 0 && !kHidden) request_i(last, step + STAGES - 1, slot0);
                     fragments((k + 1) & 1, stage, k + 1);
-                    multiply(k & 1);
-                    if (kApart && k == 0)
-                        interleave(reads, requests_i);
-                    else
-                        interleave(reads, slot0);
+                    if (kApart && k == 0 && kHidden) {
+                        multiply_and(0, requests_i, [&](int e) { ti.request_piece(lds + last * kStage, s, s1, e); });
+                    } else {
+                        multiply(k & 1);
+                        if (kApart && k == 0)
+                            interleave(reads, requests_i);
+                        else
+                            interleave(reads, slot0);
+                    }
                 }
                 meet<(STAGES - 2) * kRequests>();
-                request_j(stage, step + STAGES, slot0);
+                if (!kHidden || !kApart) request_j(stage, step + STAGES, slot0);
                 if (!kApart) request_i(stage, step + STAGES, slot0);
                 fragments(kQuarters & 1, next, 0);
-                multiply((kQuarters - 1) & 1);
-                if constexpr (kApart) interleave(reads, requests_j);
+                if constexpr (kHidden && kApart) {
+                    multiply_and((kQuarters - 1) & 1, requests_j, [&](int e) {
+                        tj.request_piece(lds + stage * kStage + TileI::kBytes, s0 + (step + STAGES) * TileI::kSteps, s1, e);
+                    });
+                } else {
+                    multiply((kQuarters - 1) & 1);
+                    if constexpr (kApart) interleave(reads, requests_j);
+                }
                 if constexpr (kQuarters == 1) {  // (registers have no index: the next step's fragments take the place of this one's)
 #pragma unroll
                     for (int a = 0; a < NI; ++a) fi[0][a] = fi[1][a];
