@@ -876,19 +876,22 @@ __global__ __launch_bounds__(256) void small_gradients_kernel(const ProductParam
 // The tile that a product is cut into, how often its sum is split, and its launch.
 //
 // The plan is the one with the shortest estimate, from what the tiles measured (us): a step of the sum takes `step` when a
-// compute unit has one tile to work on (latency, then), `more` for each when it has several at a time, and a launch `start` besides.
-// A split sum is joined by a kernel of its own: 4.5 (6, where splits of rows that lie anywhere start) and the partial sums' bytes, out and back in, at 4 TB/s.
+// compute unit has one tile to work on (latency, then), `more` for each when it has several, `tile` besides for every tile after
+// the first, and a launch `start`.  A split sum is joined by a kernel of its own: 4.5 (6, where splits of rows that lie anywhere start)
+// and the partial sums' bytes, out and back in, at 4 TB/s.
 enum Cut : int { CUT_256, CUT_128, CUT_128_DEEP, CUT_64, CUT_32, CUTS };
 struct CutCost {
     int size;
-    float start, step, more;
+    float start, tile, step, more;
 };
-// 16-bit types: 8192 x 4096 x 4096 227 us in tiles of 256 and 273 in 128; 2048^3 57 / 29 / 27 (deep) / 36 in 256 / 128 / 128 / 64; 1024^3
-// 36 / 17 / 16 / 8.8 / 13.5 (32); 100 x 400 x 300 20 / 11.5 / - / 6.1 / 4.9.  fp32: 400 x 800 x 1600 64 / 59 / 20 / 22 in 128 / deep / 64 / 32,
-// 256 x 512 x 1000 45 / - / 16 / 8.2.  Rows that lie anywhere: 77 x 1023 x 1537 22 / - / 13 / 10, 8192 x 4096 x 4096 358 / - / 593 / 974.
-constexpr CutCost kCuts16[CUTS] = {{256, 10.0f, 1.6f, 1.75f}, {128, 6.0f, 0.85f, 0.55f}, {128, 6.0f, 0.6f, 0.65f}, {64, 3.2f, 0.33f, 0.26f}, {32, 3.2f, 0.21f, 0.14f}};
-constexpr CutCost kCuts32[CUTS] = {{256, 12.0f, 7.5f, 7.5f}, {128, 6.0f, 2.2f, 2.0f}, {128, 6.0f, 2.1f, 2.1f}, {64, 3.2f, 0.66f, 0.57f}, {32, 3.2f, 0.31f, 0.26f}};
-constexpr CutCost kCutsAnywhere[CUTS] = {{0, 0, 0, 0}, {128, 6.0f, 1.0f, 0.7f}, {0, 0, 0, 0}, {64, 3.2f, 0.6f, 0.29f}, {32, 3.2f, 0.45f, 0.17f}};
+// Measured in tiles of 256 / 128 / 128 deep / 64 / 32, rows x inputs x outputs, 16-bit types: 8192 x 4096 x 4096 220 / 274 / 310 / 458 / -,
+// 8192 x 4096 x 1024 108 / 79 / 86 / 127 / 216, 4096 x 8192 x 1024 195 / 113 / 78 / 121 / 204, 2048^3 51 / 29 / 23 / 32 / 62, 1024^3 34 / 18 / 14 / 8.5 /
+// 12.6, 64 x 4096 x 4096 69 / 44 / 29 / 19 / 11, 512^3 25 / 11 / 11 / 6.1 / 4.7.  fp32: 4000 x 2000 x 2000 482 / 259 / 266 / 280 / -, 1000^3 256 / 78 /
+// 72 / 25 / 30, 64 x 1024 x 1024 244 / 77 / 71 / 23 / 11.  Rows that lie anywhere: 8192 x 4096 x 4096 - / 358 / - / 593 / 974, 77 x 1023 x 1537 - /
+// 22 / - / 13 / 10.
+constexpr CutCost kCuts16[CUTS] = {{256, 9.0f, 4.0f, 1.4f, 1.6f}, {128, 6.0f, 1.5f, 0.8f, 0.52f}, {128, 6.0f, 3.0f, 0.4f, 0.55f}, {64, 3.5f, 1.0f, 0.27f, 0.21f}, {32, 3.2f, 0.5f, 0.135f, 0.11f}};
+constexpr CutCost kCuts32[CUTS] = {{256, 12.0f, 4.0f, 7.4f, 7.4f}, {128, 6.0f, 1.5f, 2.2f, 1.95f}, {128, 6.0f, 3.0f, 2.0f, 2.05f}, {64, 3.5f, 1.0f, 0.67f, 0.55f}, {32, 3.2f, 0.5f, 0.25f, 0.22f}};
+constexpr CutCost kCutsAnywhere[CUTS] = {{}, {128, 6.0f, 0.0f, 1.0f, 0.7f}, {}, {64, 3.2f, 0.0f, 0.6f, 0.29f}, {32, 3.2f, 0.0f, 0.45f, 0.17f}};
 struct Plan {
     Cut cut;
     int splits;
@@ -906,7 +909,7 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
             const size_t partial = k > 1 ? (size_t)k * rows * cols * sizeof(float) : 0;
             if (partial > workspace_bytes) break;
             const float rounds = std::ceil(tiles * (float)k / (float)kComputeUnits), each = std::max(cost.step, rounds * cost.more);
-            const float time = cost.start + (float)((steps + k - 1) / k) * each + (k > 1 ? (vectors ? 4.5f : 6.0f) + (float)partial * 2.0f / 4.0e6f : 0.0f);
+            const float time = cost.start + (rounds - 1.0f) * cost.tile + (float)((steps + k - 1) / k) * each + (k > 1 ? (vectors ? 4.5f : 6.0f) + (float)partial * 2.0f / 4.0e6f : 0.0f);
             if (least == 0.0f || time < least) {
                 least = time;
                 best = {(Cut)c, k};
