@@ -111,7 +111,7 @@ struct LogProbsParams {
     long long ld;
     // rows in several chunks: a Part and `top` keys of each, best first
     Part* parts;    // [rows][chunks]
-    uint64_t* keys; // [rows][chunks][top]
+    uint64_t* keys; // [rows][top][chunks]: what comes first in its chunk is side by side, and so spread over the lanes that join them
 };
 
 __device__ __forceinline__ void write_row(const LogProbsParams& p, long long row, const Part& part, const Answer& a, bool given, float xt) {
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
     if (top == 0) return;
     auto emit = [&](int place, uint64_t key) {  // (keys within the chunk count their classes from its first)
         if constexpr (SPLIT)
-            p.keys[unit * top + place] = key == 0 ? 0 : key_of(logit_of(key), class_of(key) + base);
+            p.keys[(row * top + place) * p.chunks + chunk] = key == 0 ? 0 : key_of(logit_of(key), class_of(key) + base);
         else
             write_top(p, row, answer, place, key);
     };
@@ -401,8 +401,18 @@ __global__ __launch_bounds__(64 * kJoinRows) void logprobs_join_kernel(const T* 
     if (row >= p.rows) return;
     const uint64_t* keys = p.keys + row * p.chunks * p.top;
     const int total = p.chunks * p.top;
-    uint64_t best = 0;
-    for (int i = lane; i < total; i += 64) best = max(best, keys[i]);
+    // the first keys are requested together and kept (all of them, in most calls), the others read as they are needed
+    constexpr int kKept = 8;
+    uint64_t kept[kKept], best = 0;
+#pragma unroll
+    for (int u = 0; u < kKept; ++u) kept[u] = lane + 64 * u < total ? keys[lane + 64 * u] : 0;
+    auto each_key = [&](auto f) {
+#pragma unroll
+        for (int u = 0; u < kKept; ++u) f(kept[u]);
+#pragma unroll 4
+        for (int i = lane + 64 * kKept; i < total; i += 64) f(keys[i]);
+    };
+    each_key([&](uint64_t key) { best = max(best, key); });
     Part part = {-INFINITY, 0.0f, 0.0f, 0};
     for (int c = lane; c < p.chunks; c += 64) {
         Part q = p.parts[row * p.chunks + c];
@@ -431,13 +441,12 @@ __global__ __launch_bounds__(64 * kJoinRows) void logprobs_join_kernel(const T* 
     // (keys differ, but for those that stand for nothing: 0)
     const uint64_t bound = max((uint64_t)1, ~wave_max_key(larger < p.top ? ~best : 0));
     team_sync<1>();
-    for (int i = lane; i < total; i += 64) {
-        const uint64_t key = keys[i];
+    each_key([&](uint64_t key) {
         if (key >= bound) {
             const int at = atomicAdd(&counts[wave], 1);
             if (at < kList) lists[wave][at] = key;
         }
-    }
+    });
     team_sync<1>();
     const int count = counts[wave];
     if (count <= kList) {
@@ -453,8 +462,9 @@ __global__ __launch_bounds__(64 * kJoinRows) void logprobs_join_kernel(const T* 
     uint64_t last = ~0ull;
     for (int i = 0; i < p.top; ++i) {
         best = 0;
-        for (int k = lane; k < total; k += 64)
-            if (keys[k] < last) best = max(best, keys[k]);
+        each_key([&](uint64_t key) {
+            if (key < last) best = max(best, key);
+        });
         last = wave_max_key(best);
         if (lane == 0) write_top(p, row, answer, i, last);
     }
