@@ -272,3 +272,88 @@ class LogProbsLayerParam(_HeadLayer):
             out["top_index"] = self.top_index_gpu.to_numpy(np.int32, (m, k))
             out["top_logprob"] = self.top_logprob_gpu.to_numpy(np.float32, (m, k))
         return out
+
+
+class FloatHead:
+    """A float head on `features` values a row, as on the last binary layer of a network:
+    norm -> linear (GELU), + the features where there are as many hidden values -> norm -> linear -> log probabilities of
+    `classes`.  The features are given (the network below them is frozen): they get no gradient.
+
+    forward() scores the rows' targets and ranks the best classes; backward() leaves the gradient of the mean cross
+    entropy in the layers' gradient buffers; step() takes a step of gradient descent on the parameters, which are kept
+    in fp32 on the host."""
+
+    def __init__(self, rows, features, hidden, classes, dtype="f32", top=5):
+        self.rows, self.features, self.hidden, self.classes, self.dtype = rows, features, hidden, classes, dtype
+        self.norm1 = LayerNormLayerParam("Norm1", rows, features, dtype)
+        self.linear1 = LinearLayerParam("Linear1", rows, features, hidden, dtype, "gelu")
+        self.norm2 = LayerNormLayerParam("Norm2", rows, hidden, dtype)
+        self.linear2 = LinearLayerParam("Linear2", rows, hidden, classes, dtype)
+        self.logprobs = LogProbsLayerParam("LogProbs", rows, classes, min(top, classes), dtype)
+        self.layers = [self.norm1, self.linear1, self.norm2, self.linear2, self.logprobs]
+
+    def initialize(self, features_gpu, targets, seed=0):
+        """features_gpu: [rows][features] in the head's dtype; targets: int32 [rows], -1 for rows without a class."""
+        rng = np.random.default_rng(seed)
+        k, h, c, m = self.features, self.hidden, self.classes, self.rows
+        self.params = {"gamma1": np.ones(k, np.float32), "beta1": np.zeros(k, np.float32),
+                       "w1": rng.normal(0, k ** -0.5, (h, k)).astype(np.float32), "b1": np.zeros(h, np.float32),
+                       "gamma2": np.ones(h, np.float32), "beta2": np.zeros(h, np.float32),
+                       "w2": rng.normal(0, h ** -0.5, (c, h)).astype(np.float32), "b2": np.zeros(c, np.float32)}
+        p, size = self.params, 4 if self.dtype == "f32" else 2
+        targets = np.ascontiguousarray(targets, np.int32)
+        n1, l1, n2, l2, lp = self.layers
+        n1.initialize(p["gamma1"], p["beta1"], features_gpu)
+        l1.initialize(p["w1"], p["b1"], n1.output_gpu, residual_gpu=features_gpu if h == k else None, save_preact=True)
+        n2.initialize(p["gamma2"], p["beta2"], l1.output_gpu)
+        l2.initialize(p["w2"], p["b2"], n2.output_gpu)
+        self._targets = DeviceBuffer.from_numpy(targets)
+        lp.initialize(l2.output_gpu, self._targets)
+        self._grads = {name: DeviceBuffer(a.size * (size if name[0] == "w" else 4)) for name, a in p.items()}
+        self._flows = [DeviceBuffer(m * n * size) for n in (c, h, h, k)]
+        g = self._grads
+        given = max(1, int((targets >= 0).sum()))
+        self._loss = DeviceBuffer.from_numpy(np.where(targets >= 0, np.float32(-1.0 / given), np.float32(0)))
+        self._given = given
+        lp.initialize_backward(self._loss, None, self._flows[0])
+        l2.initialize_backward(self._flows[0], self._flows[1], g["w2"], g["b2"])
+        n2.initialize_backward(self._flows[1], self._flows[2], g["gamma2"], g["beta2"])
+        l1.initialize_backward(self._flows[2], self._flows[3], g["w1"], g["b1"])
+        n1.initialize_backward(self._flows[3], None, g["gamma1"], g["beta1"])
+        self._devices = {"gamma1": n1.gamma_gpu, "beta1": n1.beta_gpu, "w1": l1.weight_gpu, "b1": l1.bias_gpu,
+                         "gamma2": n2.gamma_gpu, "beta2": n2.beta_gpu, "w2": l2.weight_gpu, "b2": l2.bias_gpu}
+        return self
+
+    def forward(self, stream=None):
+        for layer in self.layers:
+            layer.forward(stream)
+
+    def backward(self, stream=None):
+        """The gradients of all parameters, of the mean cross entropy of the last forward()."""
+        for layer in reversed(self.layers):
+            layer.backward(stream)
+
+    def loss(self):
+        """The mean cross entropy of the last forward()."""
+        _lib.device_synchronize()
+        return -float(self.logprobs.logprob_gpu.to_numpy(np.float32, (self.rows,)).astype(np.float64).sum()) / self._given
+
+    def gradients(self):
+        """fp32 host arrays of the last backward()'s gradients, by parameter."""
+        _lib.device_synchronize()
+        out = {}
+        for name, a in self.params.items():
+            dt = self.dtype if name[0] == "w" else "f32"
+            out[name] = decode(self._grads[name].to_numpy(storage(dt), a.shape), dt)
+        return out
+
+    def step(self, rate):
+        for name, g in self.gradients().items():
+            self.params[name] -= np.float32(rate) * g
+            self._devices[name].upload(encode(self.params[name], self.dtype if name[0] == "w" else "f32"))
+
+    def release(self):
+        for layer in self.layers:
+            layer.release()
+        for buf in [self._targets, self._loss] + self._flows + list(self._grads.values()):
+            buf.free()
