@@ -419,6 +419,8 @@ typedef struct tcbnn_linear_desc {
 } tcbnn_linear_desc;
 size_t tcbnn_linear_workspace_bytes(int rows, int in_features, int out_features, int dtype);
 int tcbnn_linear_forward(const tcbnn_linear_desc* d, void* stream);
+/* Name of the kernel that tcbnn_linear_forward launches for this descriptor; nothing is launched, no pointer followed. */
+int tcbnn_linear_kernel_name(const tcbnn_linear_desc* d, char* buf, size_t len);
 
 /* With dz = grad_output * act'(z):  grad_input = dz * weight, grad_weight = dz^T * input, grad_bias = sums of dz over the
  * rows (the gradient of `residual` is grad_output itself).  Each of the three may be NULL; what is given is overwritten.

@@ -178,6 +178,7 @@ ABI = {
     "tcbnn_shader_clock_probe": (c_int, [c_void_p, c_int, C.POINTER(c_int), c_void_p]),
     "tcbnn_linear_workspace_bytes": (c_size_t, [c_int] * 4),
     "tcbnn_linear_forward": (c_int, [C.POINTER(LinearDesc), c_void_p]),
+    "tcbnn_linear_kernel_name": (c_int, [C.POINTER(LinearDesc), C.c_char_p, c_size_t]),
     "tcbnn_linear_grad_workspace_bytes": (c_size_t, [c_int] * 4),
     "tcbnn_linear_backward": (c_int, [C.POINTER(LinearGradDesc), c_void_p]),
     "tcbnn_layernorm_forward": (c_int, [C.POINTER(LayerNormDesc), c_void_p]),

@@ -172,7 +172,7 @@ struct Tile {
         const T* from = ACROSS ? base + s * ld : base;
         if constexpr (HIDDEN) {
             // The builtin makes the compiler wait for it before every transposing read of LDS, whichever tile that reads; what is in
-            // LDS is for meet() to wait for.  (m0: where in LDS; nothing comes back into registers.)
+            // LDS is for meet() to wait for.  (m0, which the compiler sets itself right before each use of its own: where in LDS.  Nothing comes back into registers.)
             const unsigned long long address = (unsigned long long)(uintptr_t)from;
             const Words r = {__builtin_amdgcn_readfirstlane((int)address), __builtin_amdgcn_readfirstlane((int)(address >> 32) & 0xffff), 0x7fffffff,
                              0x00020000};
@@ -180,7 +180,7 @@ struct Tile {
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(
                              __builtin_amdgcn_readfirstlane((int)(uintptr_t)(LdsVoid*)to)),
                          "v"(at), "s"(r), "s"(ACROSS ? 0 : s * (int)sizeof(T))
-                         : "memory", "m0");
+                         : "memory");
         } else {
             const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(from), 0, 0x7fffffff, 0x00020000);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)to, 16, at, ACROSS ? 0 : s * (int)sizeof(T), 0, 0);
@@ -956,6 +956,25 @@ bool launch_small_gradients(ProductParams dx, ProductParams dw, hipStream_t stre
     return true;
 }
 
+// the kernel that launch_product takes for a forward product, as a profiler lists it
+template <typename T>
+void product_name(const ProductParams& p, size_t workspace_bytes, char* buf, size_t len) {
+    const char* type = std::is_same_v<T, float> ? "float" : (std::is_same_v<T, _Float16> ? "_Float16" : "__bf16");
+    if (p.rows <= kFewRows) {
+        snprintf(buf, len, "few_rows_kernel<%s, %d>", type, p.rows <= 16 ? 1 : 2);
+        return;
+    }
+    const Access access = access_of<T, false, false>(p);
+    const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
+    static const char* const shape[3][CUTS] = {
+        {"256, 256, 2, 4, 1, 2", "128, 128, 2, 2, 1, 2", "128, 128, 2, 2, 2, 4", "64, 64, 2, 2, 2, 4", "32, 32, 1, 1, 4, 8"},
+        {"", "128, 128, 2, 2, 1, 2", "", "64, 64, 2, 2, 2, 2", "32, 32, 1, 1, 4, 2"},
+        {"32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2"}};
+    const int hold = access == ANYWHERE && plan.cut != CUT_128 ? 4 : 1;
+    snprintf(buf, len, "product_kernel<%s, %s, (Access)%d, %d, false, false>%s", type, shape[access][plan.cut], (int)access, hold,
+             plan.splits > 1 && access != ELEMENTS ? " + product_join_kernel" : "");
+}
+
 template <typename T, bool ACROSS_I, bool ACROSS_J>
 int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
     TCBNN_REQUIRE((long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) <= 0x7fffffffLL, "linear: grid too large");
@@ -1041,6 +1060,32 @@ extern "C" size_t tcbnn_linear_workspace_bytes(int rows, int in_features, int ou
     return rows <= kFewRows ? 0 : split_bytes(rows, out_features, in_features, dtype);
 }
 
+static ProductParams forward_product(const tcbnn_linear_desc* d) {
+    ProductParams p = {};
+    p.i = {d->input, row_stride(d->input_ld, d->in_features)};
+    p.j = {d->weight, row_stride(d->weight_ld, d->in_features)};
+    p.rows = d->rows;
+    p.cols = d->out_features;
+    p.sum = d->in_features;
+    p.activation = d->activation;
+    p.bias = d->bias;
+    p.residual = d->residual;
+    p.out = d->output;
+    p.preact = d->preact;
+    p.residual_ld = row_stride(d->residual_ld, d->out_features);
+    p.out_ld = row_stride(d->output_ld, d->out_features);
+    p.preact_ld = row_stride(d->preact_ld, d->out_features);
+    return p;
+}
+
+extern "C" int tcbnn_linear_kernel_name(const tcbnn_linear_desc* d, char* buf, size_t len) {
+    TCBNN_NOTNULL(d);
+    TCBNN_NOTNULL(buf);
+    if (int rc = check_linear(d->rows, d->in_features, d->out_features, d->dtype, d->activation)) return rc;
+    by_dtype(d->dtype, [&](auto t) { product_name<decltype(t)>(forward_product(d), d->workspace ? d->workspace_bytes : 0, buf, len); });
+    return TCBNN_OK;
+}
+
 extern "C" int tcbnn_linear_forward(const tcbnn_linear_desc* d, void* stream) {
     TCBNN_NOTNULL(d);
     if (int rc = check_linear(d->rows, d->in_features, d->out_features, d->dtype, d->activation)) return rc;
@@ -1053,20 +1098,7 @@ extern "C" int tcbnn_linear_forward(const tcbnn_linear_desc* d, void* stream) {
     TCBNN_NOTNULL(d->weight);
     TCBNN_NOTNULL(d->output);
     TCBNN_REQUIRE(d->output != d->residual || d->rows == 1 || y_ld == r_ld, "linear: an output over its residual has the residual's stride");
-    ProductParams p = {};
-    p.i = {d->input, x_ld};
-    p.j = {d->weight, w_ld};
-    p.rows = d->rows;
-    p.cols = d->out_features;
-    p.sum = d->in_features;
-    p.activation = d->activation;
-    p.bias = d->bias;
-    p.residual = d->residual;
-    p.out = d->output;
-    p.preact = d->preact;
-    p.residual_ld = r_ld;
-    p.out_ld = y_ld;
-    p.preact_ld = z_ld;
+    const ProductParams p = forward_product(d);
     return by_dtype(d->dtype, [&](auto t) { return launch_product<decltype(t), false, false>(p, (float*)d->workspace, d->workspace ? d->workspace_bytes : 0, (hipStream_t)stream); });
 }
 

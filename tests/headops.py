@@ -22,22 +22,23 @@ def rounded(x, dtype):
 
 
 class Matrix:
-    """A matrix on the device, rows `gap` elements further apart than they are long, every gap element NaN."""
+    """A matrix on the device, rows `gap` elements further apart than they are long, every gap element NaN.  It begins `shift`
+    elements into its buffer: with one, rows of odd length start at every alignment there is; with none, rows whose length
+    and gap are multiples of 16 bytes lie at whole 16 bytes."""
 
-    def __init__(self, values, dtype, gap=0, rows=None, cols=None):
+    def __init__(self, values, dtype, gap=0, rows=None, cols=None, shift=1):
         if values is None:  # an output: NaN everywhere
             values = np.full((rows, cols), np.nan, np.float32)
-        self.shape, self.dtype, self.gap = values.shape, dtype, gap
+        self.shape, self.dtype, self.gap, self.shift = values.shape, dtype, gap, shift
         wide = np.full((values.shape[0], values.shape[1] + gap), np.nan, np.float32)
         wide[:, :values.shape[1]] = values
         bits = head.encode(wide, dtype)
         self.values = head.decode(bits, dtype).astype(np.float64)[:, :values.shape[1]]
-        # one element into the buffer: rows of odd length then start at every alignment there is
-        self.buf = DeviceBuffer.from_numpy(np.concatenate([np.zeros(1, bits.dtype), bits.ravel()]))
-        self.view = DeviceView(self.buf.ptr + bits.itemsize, bits.nbytes, wide.shape[1] if gap else 0, self.buf)
+        self.buf = DeviceBuffer.from_numpy(np.concatenate([np.zeros(shift, bits.dtype), bits.ravel()]))
+        self.view = DeviceView(self.buf.ptr + shift * bits.itemsize, bits.nbytes, wide.shape[1] if gap else 0, self.buf)
 
     def get(self):
-        wide = self.buf.to_numpy(head.storage(self.dtype), (1 + self.shape[0] * (self.shape[1] + self.gap),))[1:]
+        wide = self.buf.to_numpy(head.storage(self.dtype), (self.shift + self.shape[0] * (self.shape[1] + self.gap),))[self.shift:]
         wide = head.decode(wide, self.dtype).reshape(self.shape[0], -1)
         assert np.isnan(wide[:, self.shape[1]:]).all(), "a gap between rows was written"
         return wide[:, :self.shape[1]].astype(np.float64)
@@ -60,7 +61,7 @@ def check(got, want, tol, what=""):
     assert got.shape == want.shape, (what, got.shape, want.shape)
     special = ~np.isfinite(want)
     np.testing.assert_array_equal(got[special], want[special], err_msg=what)
-    err = np.abs(got - want)[~special]
+    err = np.abs(got[~special] - want[~special])
     bad = ~(err <= np.broadcast_to(tol, want.shape)[~special])
     assert not bad.any(), "%s: %d of %d off, by up to %g (allowed there %g)" % (
         what, bad.sum(), bad.size, err[bad].max(), np.broadcast_to(tol, want.shape)[~special][bad][err[bad].argmax()])

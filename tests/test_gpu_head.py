@@ -23,11 +23,11 @@ LINEAR = [(1, 1, 1), (1, 16, 10), (1, 4096, 512), (1, 1025, 33), (2, 8, 3), (3, 
           (256, 512, 1000), (300, 64, 8), (255, 1000, 511), (513, 96, 300), (1000, 24, 1030)]
 
 
-def _linear(gpu, m, k, n, dtype, activation, bias=True, residual=True, preact=True, gap=0, in_place=False, stream=None):
+def _linear(gpu, m, k, n, dtype, activation, bias=True, residual=True, preact=True, gap=0, in_place=False, stream=None, shift=1):
     from tcbnn_amd import head
     r = rng(m, k, n, len(dtype), len(activation))
-    x = ho.Matrix(r.standard_normal((m, k)), dtype, gap)
-    w = ho.Matrix(r.standard_normal((n, k)) / np.sqrt(k), dtype, gap)
+    x = ho.Matrix(r.standard_normal((m, k)), dtype, gap, shift=shift)
+    w = ho.Matrix(r.standard_normal((n, k)) / np.sqrt(k), dtype, gap, shift=shift)
     b = r.standard_normal(n).astype(np.float32) if bias else None
     res = ho.Matrix(r.standard_normal((m, n)), dtype, gap) if residual else None
     rv = res.values if residual else 0.0
@@ -89,13 +89,13 @@ def test_linear_rows_do_not_mix(gpu, m, k, n, dtype):
     np.testing.assert_array_equal(finite, want)
 
 
-def _linear_grad(gpu, m, k, n, dtype, activation, gap=0, want=("x", "w", "b")):
+def _linear_grad(gpu, m, k, n, dtype, activation, gap=0, want=("x", "w", "b"), shift=1):
     from tcbnn_amd import head
     r = rng(m, k, n, len(dtype), len(activation), 1)
-    x = ho.Matrix(r.standard_normal((m, k)), dtype, gap)
-    w = ho.Matrix(r.standard_normal((n, k)) / np.sqrt(k), dtype, gap)
+    x = ho.Matrix(r.standard_normal((m, k)), dtype, gap, shift=shift)
+    w = ho.Matrix(r.standard_normal((n, k)) / np.sqrt(k), dtype, gap, shift=shift)
     z = ho.Matrix(r.standard_normal((m, n)) * 2, dtype, gap)
-    dy = ho.Matrix(r.standard_normal((m, n)), dtype, gap)
+    dy = ho.Matrix(r.standard_normal((m, n)), dtype, gap, shift=shift)
     dx, dw, db = ho.Matrix(None, dtype, gap, m, k), ho.Matrix(None, dtype, gap, n, k), ho.empty(n)
     layer = head.LinearLayerParam("linear", m, k, n, dtype, activation)
     layer.initialize(w.view, None, x.view, preact_gpu=z.view if activation != "none" else None)
@@ -133,6 +133,146 @@ def test_linear_grad_strides_and_single_outputs(gpu, m, k, n, dtype):
     for want in (("x",), ("w",), ("b",), ("w", "b")):
         _linear_grad(gpu, m, k, n, dtype, "silu", want=want)
         _linear_grad(gpu, m, k, n, dtype, "none", want=want)
+
+
+def _kernel(m, k, n, dtype):
+    import ctypes as C
+    from tcbnn_amd import _lib
+    dt = _lib.DTYPES[dtype]
+    d = _lib.LinearDesc(input=1 << 20, weight=1 << 20, output=1 << 20, rows=m, in_features=k, out_features=n, dtype=dt, workspace=1 << 20,
+                        workspace_bytes=_lib.lib.tcbnn_linear_workspace_bytes(m, k, n, dt))
+    buf = C.create_string_buffer(160)
+    _lib.check(_lib.lib.tcbnn_linear_kernel_name(C.byref(d), buf, 160))
+    return buf.value.decode()
+
+
+# rows at whole 16 bytes: every tile, with whole tiles and ragged ones, whole steps of the sum and ragged ones, sums of one step, of fewer
+# than the tile keeps under way and of many; the bf16 plan of each
+WHOLE = [((1, 64, 64), "few_rows_kernel"), ((32, 1048, 72), "few_rows_kernel"), ((33, 8, 8), "32, 32"), ((40, 64, 64), "32, 32"),
+         ((100, 520, 304), "32, 32"), ((300, 256, 520), "32, 32"), ((64, 2048, 2048), "32, 32"), ((64, 16384, 64), "join"),
+         ((128, 4096, 136), "join"), ((1024, 512, 1024), "64, 64"), ((1000, 72, 3000), "64, 64"), ((1016, 1032, 1048), "64, 64"),
+         ((2040, 136, 2040), "128, 128, 2, 2, 2, 4"), ((2048, 512, 2048), "128, 128, 2, 2, 2, 4"), ((2040, 72, 4104), "128, 128, 2, 2, 1, 2"),
+         ((3000, 200, 3000), "128, 128, 2, 2, 1, 2"), ((4096, 64, 4096), "256, 256"), ((4000, 200, 4088), "256, 256")]
+
+
+@pytest.mark.parametrize("shape,kernel", WHOLE)
+def test_linear_of_whole_pieces(gpu, shape, kernel):
+    assert kernel in _kernel(*shape, "bf16")
+    for dtype, activation in (("bf16", "gelu"), ("f16", "none"), ("f32", "silu")):
+        _linear(gpu, *shape, dtype, activation, preact=False, shift=0)
+    _linear(gpu, *shape, "bf16", "relu", gap=8, in_place=True, shift=0)
+
+
+# the same tiles for the gradients: (rows, sum, columns) of grad_input, then of grad_weight
+WHOLE_GRADS = [((40, 64, 64), "32, 32"), ((100, 304, 520), "32, 32"), ((64, 2048, 2048), "32, 32"), ((64, 16384, 64), "join"), ((1000, 72, 3000), "64, 64"),
+               ((1016, 1032, 1048), "64, 64"), ((2040, 136, 2040), "128, 128, 2, 2, 2, 4"), ((2040, 72, 4104), "128, 128, 2, 2, 1, 2"),
+               ((4000, 72, 4088), "256, 256")]
+
+
+@pytest.mark.parametrize("shape,kernel", WHOLE_GRADS)
+def test_linear_grad_of_whole_pieces(gpu, shape, kernel):
+    assert kernel in _kernel(*shape, "bf16")
+    rows, total, cols = shape
+    for dtype, activation in (("bf16", "none"), ("f16", "gelu"), ("f32", "relu")):
+        _linear_grad(gpu, rows, cols, total, dtype, activation, want=("x",), shift=0)
+        _linear_grad(gpu, total, cols, rows, dtype, activation, want=("w",), shift=0)
+    _linear_grad(gpu, min(rows, 300), min(cols, 520), min(total, 200), "bf16", "silu", gap=8, shift=0)
+
+
+def test_linear_sums_in_one_order(gpu):
+    """The same bits in every call, whatever was in the workspace."""
+    from tcbnn_amd import head
+    r = rng(77)
+    m, k, n = 64, 16384, 64
+    x, w, z, dy = (ho.Matrix(r.standard_normal(s), "bf16", shift=0) for s in ((m, k), (n, k), (m, n), (m, n)))
+    y, dx, dw, db = (ho.Matrix(None, "bf16", 0, *s, shift=0) for s in ((m, n), (m, k), (n, k), (1, 2 * n)))
+    layer = head.LinearLayerParam("linear", m, k, n, "bf16", "gelu").initialize(w.view, None, x.view, output_gpu=y.view, preact_gpu=z.view)
+    layer.initialize_backward(dy.view, dx.view, dw.view, db.view)
+    first = None
+    for fill in (0, 0xFF, 0x3C):
+        for buf in layer._owned:
+            buf.fill(fill)
+        layer.backward()
+        layer.forward()
+        ho.sync()
+        bits = [a.buf.to_numpy(np.uint16, (a.shape[0] * a.shape[1],)) for a in (y, dx, dw, db)]
+        first = first or bits
+        for a, b in zip(bits, first):
+            np.testing.assert_array_equal(a, b)
+        z.buf.upload(head.encode(z.values.astype(np.float32), "bf16"))
+    layer.release()
+
+
+class _Apart:
+    """Rows so far apart that their offsets pass 32 bits, on the device."""
+
+    def __init__(self, values, dtype, ld):
+        from tcbnn_amd import _lib, head
+        self.rows, self.cols, self.ld, self.dtype = *values.shape, ld, dtype
+        self.size = 4 if dtype == "f32" else 2
+        self.buf = ho.DeviceBuffer(self.size * (ld * (self.rows - 1) + self.cols))
+        self.view = ho.DeviceView(self.buf.ptr, self.buf.nbytes, ld, self.buf)
+        bits = head.encode(values, dtype)
+        self.values = head.decode(bits, dtype).astype(np.float64)
+        for i in range(self.rows):
+            row = np.ascontiguousarray(bits[i])
+            _lib.hip_check(_lib.hip.hipMemcpy(self.buf.ptr + self.size * ld * i, row.ctypes.data, row.nbytes, _lib.H2D))
+
+    def get(self):
+        from tcbnn_amd import _lib, head
+        out = np.empty((self.rows, self.cols), head.storage(self.dtype))
+        for i in range(self.rows):
+            row = np.empty(self.cols, out.dtype)
+            _lib.hip_check(_lib.hip.hipMemcpy(row.ctypes.data, self.buf.ptr + self.size * self.ld * i, row.nbytes, _lib.D2H))
+            out[i] = row
+        return head.decode(out, self.dtype).astype(np.float64)
+
+
+@pytest.mark.parametrize("rows,ld", [(3, (1 << 30) + 8), (40, (1 << 26) + 4)])
+def test_offsets_past_32_bits(gpu, rows, ld):
+    """Rows 2 GiB (or 128 MiB, in more rows than the kernel for few rows takes) apart: each operator reads and writes them."""
+    from tcbnn_amd import head
+    r = rng(rows)
+    n = 72
+    x = _Apart(r.standard_normal((rows, n)).astype(np.float32), "bf16", ld)
+    gamma, beta = np.ones(n, np.float32), np.zeros(n, np.float32)
+    mean, rstd = ho.empty(rows), ho.empty(rows)
+    y = ho.Matrix(None, "bf16", 0, rows, n)
+    norm = head.LayerNormLayerParam("norm", rows, n, "bf16", EPS).initialize(gamma, beta, x.view, output_gpu=y.view, mean_gpu=mean, rstd_gpu=rstd)
+    norm.forward()
+    ho.sync()
+    _check_norm(x.values, gamma.astype(np.float64), beta.astype(np.float64), y.get(), mean.to_numpy(np.float32, (rows,)),
+                rstd.to_numpy(np.float32, (rows,)), "bf16")
+    w = ho.Matrix(r.standard_normal((24, n)), "bf16")
+    z = ho.Matrix(None, "bf16", 0, rows, 24)
+    head.LinearLayerParam("linear", rows, n, 24, "bf16").initialize(w.view, None, x.view, output_gpu=z.view).forward()
+    ho.sync()
+    exact, terms = x.values @ w.values.T, np.abs(x.values) @ np.abs(w.values).T
+    ho.check(z.get(), exact, n * ho.U32 * terms + ho.U["bf16"] * (np.abs(exact) + terms * n * ho.U32), "linear")
+    lin = head.LinearLayerParam("linear", rows, 24, n, "bf16").initialize(ho.Matrix(r.standard_normal((n, 24)), "bf16").view, None, z.view)
+    dw = ho.Matrix(None, "bf16", 0, n, 24)
+    lin.initialize_backward(x.view, None, dw.view, None)  # (the far rows as grad_output)
+    lin.backward()
+    ho.sync()
+    exact, terms = x.values.T @ z.get(), np.abs(x.values).T @ np.abs(z.get())
+    ho.check(dw.get(), exact, rows * ho.U32 * terms + ho.U["bf16"] * (np.abs(exact) + terms * rows * ho.U32), "grad_weight")
+    t = r.integers(0, n, rows).astype(np.int32)
+    lp = head.LogProbsLayerParam("logprobs", rows, n, 4, "bf16").initialize(x.view, ho.vector(t, np.int32))
+    lp.initialize_backward(ho.vector(np.ones(rows)), None, x.view)
+    lp.forward()
+    ho.sync()
+    want = [ho.logprobs(x.values[i], int(t[i]), 4) for i in range(rows)]
+    got = lp.download_output()
+    np.testing.assert_array_equal(got["top_index"], np.stack([v[4] for v in want]))
+    np.testing.assert_allclose(got["logprob"], [v[0] for v in want], atol=1e-5)
+    lp.backward()
+    ho.sync()
+    p = np.exp(x.values - np.array([v[2] for v in want])[:, None])
+    hot = (np.arange(n) == t[:, None]) - p
+    ho.check(x.get(), hot, 2 * ho.U["bf16"] * np.abs(hot) + 1e-6, "grad_logits")
+    for layer in (norm, lin, lp):
+        layer.release()
+    x.buf.free()
 
 
 def test_linear_without_rows(gpu):

@@ -107,6 +107,28 @@ def test_workspaces_of_refused_sizes_are_empty():
     assert lib.tcbnn_logprobs_workspace_bytes(-1, 8, 0, 0) == lib.tcbnn_logprobs_workspace_bytes(4, 8, 99, 0) == 0
 
 
+def test_kernel_names():
+    """The kernel of a forward call by sizes and alignment; a workspace lets few tiles share a long sum; nothing is followed."""
+    lib = _lib().lib
+
+    def name(**kw):
+        d = _linear(**{**dict(rows=64, in_features=16384, out_features=64), **kw})[1]
+        buf = C.create_string_buffer(160)
+        assert lib.tcbnn_linear_kernel_name(C.byref(d), buf, 160) == 0
+        return buf.value.decode()
+
+    need = lib.tcbnn_linear_workspace_bytes(64, 16384, 64, 1)
+    assert need > 0 and "join" in name(workspace=P, workspace_bytes=need)
+    assert "join" not in name() and "join" not in name(workspace=P, workspace_bytes=16)
+    assert name(rows=32) == "few_rows_kernel<__bf16, 2>" and name(rows=1, dtype=0) == "few_rows_kernel<float, 1>"
+    assert "(Access)0" in name() and "(Access)1" in name(input=P + 2) and "(Access)1" in name(input_ld=16387)
+    assert "(Access)2" in name(in_features=5) and "(Access)2" in name(weight_ld=1 << 24)
+    assert "256, 256" in name(rows=8192, in_features=4096, out_features=4096)
+    d = _linear(rows=-1)[1]
+    assert lib.tcbnn_linear_kernel_name(C.byref(d), C.create_string_buffer(8), 8) == EINVAL
+    assert lib.tcbnn_linear_kernel_name(None, C.create_string_buffer(8), 8) == ENULL
+
+
 def test_layers_refuse():
     from tcbnn_amd import head
     from tcbnn_amd.device import DeviceView
