@@ -3,6 +3,13 @@
 //
 // All three products are one kernel: c[i][j] = sum over s of I(i, s) J(j, s), where an operand lies in memory either along the
 // sum (x and w of the forward product: rows of s) or across it (w of dx, dz and x of dw: a row for every s).
+//
+// Large products are bound by the matrix instructions, as far as power and the barriers between steps let them run: 8192 x 4096 x
+// 4096 in bf16 takes 218 us (1.26 PFLOP/s), 250 with bias, GELU, residual and z kept, because 134 MB more of traffic and the
+// activations follow the tiles' last steps; 8192^3 815 us (1.35 PFLOP/s); fp32 4096^3 960 us (143 TFLOP/s).  Of the gradients
+// of 8192 x 4096 x 1024 dx takes 83 us and dw 86 (0.8 PFLOP/s): operands across the sum need twice the LDS requests.  Rows that lie
+// anywhere go through registers, 358 us instead of 218.  Small products are bound by a launch and the latency of their steps,
+// products of few rows by the weights' bytes.
 #include <cmath>
 
 #include "head.h"
@@ -670,10 +677,13 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
 }
 
 
-// ---- few rows (16 NI at most): bound by the weights' bytes.  A workgroup has 16 outputs, its 8 wavefronts an eighth of the sum each;
-// 64 bytes of 16 weight rows are one request of a wavefront and one matrix instruction (four in fp32), and eight requests of each
-// operand are under way at a time.  Nothing goes through LDS but the wavefronts' sums, and rows may lie anywhere.
-constexpr int kFewRows = 32, kFewWaves = 8, kFewOutputs = 16, kFewAtOnce = 8;
+// ---- few rows (16 at most): bound by the weights' bytes.  A wavefront has 16 outputs and a share of the sum; 64 bytes of 16 weight
+// rows are one request of it and one matrix instruction (four in fp32), and eight requests of each operand are under way at a
+// time.  A workgroup's 8 wavefronts are SHARES of the sum by 8 / SHARES groups of outputs: 8, or 2 where a sum is so short that eight
+// requests are half of it (1 x 512 x 32768 in 16 bits 8.2 us instead of 10.8, 1 x 128 x 65536 5.8 instead of 12.6).  Nothing goes
+// through LDS but the wavefronts' sums, and rows may lie anywhere.  1 x 4096 x 4096 bf16 8.3 us (33.6 MB, half of it the launch and the
+// first requests' latency), 1 x 8192 x 28672 77 us (6.1 TB/s).
+constexpr int kFewRows = 16, kFewWaves = 8, kFewOutputs = 16, kFewAtOnce = 8;
 typedef float Acc4 __attribute__((ext_vector_type(4)));
 template <typename T>
 __device__ __forceinline__ Acc4 mma16(Vec<T> j, Vec<T> i, Acc4 c) {
@@ -688,64 +698,57 @@ __device__ __forceinline__ Acc4 mma16(Vec<T> j, Vec<T> i, Acc4 c) {
     }
 }
 
-template <typename T, int NI>
+template <typename T, int SHARES>
 __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 4))) void few_rows_kernel(const ProductParams p) {
     constexpr int V = Elem<T>::kVec, kChunk = 4 * V;
-    __shared__ Acc4 lds[kFewWaves][NI][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int j0 = blockIdx.x * kFewOutputs;
+    __shared__ Acc4 lds[kFewWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = wave % SHARES, start = (lane >> 4) * V;
+    const int j0 = (blockIdx.x * (kFewWaves / SHARES) + wave / SHARES) * kFewOutputs;
     // rows past the last one are read as the last one; nothing of them is kept
-    const T* w = (const T*)p.j.p + (long long)min(j0 + (lane & 15), p.cols - 1) * p.j.ld + (lane >> 4) * V;
-    const T* x[NI];
-#pragma unroll
-    for (int a = 0; a < NI; ++a) x[a] = (const T*)p.i.p + (long long)min(16 * a + (lane & 15), p.rows - 1) * p.i.ld + (lane >> 4) * V;
-    const int chunks = (p.sum + kChunk - 1) / kChunk, each = (chunks + kFewWaves - 1) / kFewWaves;
-    const int c0 = wave * each, c1 = min(chunks, c0 + each);
-    Acc4 acc[NI];
-#pragma unroll
-    for (int a = 0; a < NI; ++a) acc[a] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
+    const T* w = (const T*)p.j.p + (long long)min(j0 + (lane & 15), p.cols - 1) * p.j.ld;
+    const T* x = (const T*)p.i.p + (long long)min(lane & 15, p.rows - 1) * p.i.ld;
+    const int chunks = (p.sum + kChunk - 1) / kChunk, each = (chunks + SHARES - 1) / SHARES;
+    const int c0 = share * each, c1 = min(chunks, c0 + each), whole = min(c1, p.sum / kChunk);
+    Acc4 acc = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
     int c = c0;
-    for (; c + kFewAtOnce <= c1 && (c + kFewAtOnce) * kChunk <= p.sum; c += kFewAtOnce) {
-        Vec<T> fw[kFewAtOnce], fx[NI][kFewAtOnce];
+    auto batch = [&](auto count) {
+        constexpr int N = count.value;
+        Vec<T> fw[N], fx[N];
 #pragma unroll
-        for (int u = 0; u < kFewAtOnce; ++u) fw[u] = load_vec(w + (c + u) * kChunk);
+        for (int u = 0; u < N; ++u) fw[u] = load_vec(w + (c + u) * kChunk + start);
 #pragma unroll
-        for (int a = 0; a < NI; ++a)
-#pragma unroll
-            for (int u = 0; u < kFewAtOnce; ++u) fx[a][u] = load_vec(x[a] + (c + u) * kChunk);
+        for (int u = 0; u < N; ++u) fx[u] = load_vec(x + (c + u) * kChunk + start);
         __builtin_amdgcn_sched_barrier(0);  // (all requests first: the compiler would rather save registers)
 #pragma unroll
-        for (int u = 0; u < kFewAtOnce; ++u)
-#pragma unroll
-            for (int a = 0; a < NI; ++a) acc[a] = mma16<T>(fw[u], fx[a][u], acc[a]);
-    }
-    // what is left: single chunks, the last one perhaps not whole
-    for (; c < c1; ++c) {
-        const int left = p.sum - c * kChunk - (lane >> 4) * V;  // of the sum, from the lane's first element on
+        for (int u = 0; u < N; ++u) acc = mma16<T>(fw[u], fx[u], acc);
+        c += N;
+    };
+    while (c + kFewAtOnce <= whole) batch(std::integral_constant<int, kFewAtOnce>());
+    if (c + 4 <= whole) batch(std::integral_constant<int, 4>());
+    if (c + 2 <= whole) batch(std::integral_constant<int, 2>());
+    if (c + 1 <= whole) batch(std::integral_constant<int, 1>());
+    if (c < c1) {  // the end of the sum, no whole chunk
+        const int k0 = c * kChunk + start;
         auto get = [&](const T* q) {
-            if (left >= V) return load_vec(q + c * kChunk);
+            if (k0 + V <= p.sum) return load_vec(q + k0);
             Vec<T> v;
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = e < left ? q[c * kChunk + e] : (T)0.0f;
+            for (int e = 0; e < V; ++e) v[e] = k0 + e < p.sum ? q[k0 + e] : (T)0.0f;
             return v;
         };
-        const Vec<T> fw = get(w);
-#pragma unroll
-        for (int a = 0; a < NI; ++a) acc[a] = mma16<T>(fw, get(x[a]), acc[a]);
+        acc = mma16<T>(get(w), get(x), acc);
     }
-#pragma unroll
-    for (int a = 0; a < NI; ++a) lds[wave][a][lane] = acc[a];
+    lds[wave][lane] = acc;
     __syncthreads();
-    if (wave >= NI) return;
-    const int i = 16 * wave + (lane & 15), j = j0 + 4 * (lane >> 4), n = min(4, p.cols - j);
+    if (share != 0) return;
+    const int i = lane & 15, j = j0 + 4 * (lane >> 4), n = min(4, p.cols - j);
     if (i >= p.rows || n <= 0) return;
     float z[4], bias[4];
-    Acc4 sum = lds[0][wave][lane];
 #pragma unroll
-    for (int k = 1; k < kFewWaves; ++k) sum += lds[k][wave][lane];
+    for (int k = 1; k < SHARES; ++k) acc += lds[wave + k][lane];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        z[e] = sum[e];
+        z[e] = acc[e];
         bias[e] = p.bias && e < n ? p.bias[j + e] : 0.0f;
     }
     Columns<T, 4> residual = {};
@@ -754,8 +757,10 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
 }
 
 // ---- dz = dy act'(z) in the operands' type (nothing to write without an activation), and its column sums in fp32, unrounded.
-// Bound by memory: a thread has one vector of 16 bytes of columns and goes down its share of the rows, two rows requested at
-// a time; the workgroups' sums are joined afterwards, always in the same order.
+// Bound by memory: a thread has one vector of 16 bytes of columns and goes down its share of the rows, four rows requested at
+// a time; the workgroups' sums are joined afterwards, always in the same order.  8192 x 4096 bf16 with GELU: 42 us for 201 MB (4.8 TB/s)
+// and 5 us for the join.  dz is rounded to the operands' type because that is what the matrix instructions of dx and dw take: each term
+// of theirs then has two roundings of its own in place of one, which in 16 bits are sqrt 2 of the error that dw would have otherwise.
 constexpr int kDzThreads = 256;
 // Rows that one thread takes, and the parts that a column's sum falls into (a part a workgroup).
 inline int dz_lanes(int vectors) { return vectors >= kDzThreads ? kDzThreads : vectors; }  // of a workgroup, side by side
@@ -863,7 +868,7 @@ __global__ __launch_bounds__(kDzThreads) void column_join_kernel(const float* __
 }
 
 // ---- both products of small gradients in one launch: the first workgroups have dx, the others dw.  A launch more takes as long as
-// these products do (102 x 24 -> 21 bf16: 15.9 us in three launches, 10.5 in two).
+// these products do (102 x 24 -> 21 f16 with its dz: 15.9 us in three launches, 9.8 in two).
 template <typename T, Access ACCESS, int STAGES, int HOLD>
 __global__ __launch_bounds__(256) void small_gradients_kernel(const ProductParams dx, const ProductParams dw, int blocks_dx) {
     __shared__ __align__(1024) char lds[product_lds<32, 32, 1, 1, 4, STAGES>()];
@@ -892,14 +897,16 @@ struct CutCost {
 constexpr CutCost kCuts16[CUTS] = {{256, 9.0f, 4.0f, 1.4f, 1.6f}, {128, 6.0f, 1.5f, 0.8f, 0.52f}, {128, 6.0f, 3.0f, 0.4f, 0.55f}, {64, 3.5f, 1.0f, 0.27f, 0.21f}, {32, 3.2f, 0.5f, 0.135f, 0.11f}};
 constexpr CutCost kCuts32[CUTS] = {{256, 12.0f, 4.0f, 7.4f, 7.4f}, {128, 6.0f, 1.5f, 2.2f, 1.95f}, {128, 6.0f, 3.0f, 2.0f, 2.05f}, {64, 3.5f, 1.0f, 0.67f, 0.55f}, {32, 3.2f, 0.5f, 0.25f, 0.22f}};
 constexpr CutCost kCutsAnywhere[CUTS] = {{}, {128, 6.0f, 0.0f, 1.0f, 0.7f}, {}, {64, 3.2f, 0.0f, 0.6f, 0.29f}, {32, 3.2f, 0.0f, 0.45f, 0.17f}};
+constexpr float kReadRate = 5.5e6f;  // bytes of operands in a us that no tile exceeds where they are read once
 struct Plan {
     Cut cut;
     int splits;
+    float time;
 };
 inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, size_t workspace_bytes) {
     const int steps = (int)(((long long)sum * size + kStepBytes - 1) / kStepBytes);
-    Plan best = {CUT_32, 1};
-    float least = 0.0f;
+    const float read = ((float)rows + (float)cols) * (float)sum * (float)size / kReadRate;
+    Plan best = {CUT_32, 1, 0.0f};
     for (int c = 0; c < CUTS; ++c) {
         CutCost cost = vectors ? (size == 4 ? kCuts32[c] : kCuts16[c]) : kCutsAnywhere[c];
         if (cost.size == 0) continue;
@@ -909,14 +916,25 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
             const size_t partial = k > 1 ? (size_t)k * rows * cols * sizeof(float) : 0;
             if (partial > workspace_bytes) break;
             const float rounds = std::ceil(tiles * (float)k / (float)kComputeUnits), each = std::max(cost.step, rounds * cost.more);
-            const float time = cost.start + (rounds - 1.0f) * cost.tile + (float)((steps + k - 1) / k) * each + (k > 1 ? (vectors ? 4.5f : 6.0f) + (float)partial * 2.0f / 4.0e6f : 0.0f);
-            if (least == 0.0f || time < least) {
-                least = time;
-                best = {(Cut)c, k};
-            }
+            const float time = cost.start + (rounds - 1.0f) * cost.tile + std::max((float)((steps + k - 1) / k) * each, read) + (k > 1 ? (vectors ? 4.5f : 6.0f) + (float)partial * 2.0f / 4.0e6f : 0.0f);
+            if (best.time == 0.0f || time < best.time) best = {(Cut)c, k, time};
         }
     }
     return best;
+}
+
+// The kernel for few rows instead: the wavefronts' shares of a sum, and the estimate to compare with a plan's.  A chunk of 64 bytes
+// costs a wavefront a latency, and the compute unit its requests where several workgroups have one; the rows of x are read again by every
+// workgroup.  Measured, this kernel / tiles, 16-bit types: 1 x 4096 x 4096 8.4 / 14.9, 16 x 4096 x 4096 10.4 / 10.8, 4 x 8192 x 28672 80 / 85,
+// 16 x 8192 x 28672 108 / 88, 1 x 2048 x 8192 9.8 / 8.2, 1 x 16384 x 512 20 / 16; fp32: 8 x 2048 x 1024 8.7 / 11.7, 8 x 16384 x 64 48 / 24;
+// rows that lie anywhere: 8 x 999 x 1001 6.2 / 8.7, 8 x 4095 x 4097 32 / 23, 4 x 8191 x 20001 184 / 109.
+inline int few_shares(int cols, int sum, int size) { return sum * size <= 1024 && cols > 64 * (kComputeUnits - 1) ? 2 : 8; }
+inline float few_time(int rows, int cols, int sum, int size, bool vectors) {
+    const int shares = few_shares(cols, sum, size), outputs = kFewOutputs * kFewWaves / shares;
+    const float blocks = (float)(cols / outputs + (cols % outputs != 0)) / (float)kComputeUnits;
+    const float chunks = std::ceil((float)sum * (float)size / (64.0f * (float)shares)), n = (float)rows;
+    const float latency = vectors ? 0.25f + 0.01f * n : 0.45f + 0.035f * n, more = vectors ? 0.2875f + 0.0095f * n : 0.85f + 0.1f * n;
+    return 2.4f + chunks * std::max(latency, blocks * more) + blocks * (shares == 2 ? 0.7f : 1.4f);
 }
 
 template <typename T, bool ACROSS_I, bool ACROSS_J>
@@ -937,7 +955,7 @@ inline void cut_product(ProductParams& p, int size, int steps_size, int splits, 
     p.partial = workspace;
 }
 
-// dx and dw, where both are products of one row of 32 x 32 tiles a compute unit; false: nothing is launched
+// dx and dw, where both are products of 32 x 32 tiles, four a compute unit at most; false: nothing is launched
 template <typename T>
 bool launch_small_gradients(ProductParams dx, ProductParams dw, hipStream_t stream) {
     const Access access = std::max(access_of<T, false, true>(dx), access_of<T, true, true>(dw));
@@ -956,16 +974,22 @@ bool launch_small_gradients(ProductParams dx, ProductParams dw, hipStream_t stre
     return true;
 }
 
+// (tiles of single elements are for memory where addresses do not fit; they are slower in any size)
+template <typename T>
+bool few_rows(const ProductParams& p, Access access, const Plan& plan) {
+    return p.rows <= kFewRows && (access == ELEMENTS || few_time(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES) < plan.time);
+}
+
 // the kernel that launch_product takes for a forward product, as a profiler lists it
 template <typename T>
 void product_name(const ProductParams& p, size_t workspace_bytes, char* buf, size_t len) {
     const char* type = std::is_same_v<T, float> ? "float" : (std::is_same_v<T, _Float16> ? "_Float16" : "__bf16");
-    if (p.rows <= kFewRows) {
-        snprintf(buf, len, "few_rows_kernel<%s, %d>", type, p.rows <= 16 ? 1 : 2);
-        return;
-    }
     const Access access = access_of<T, false, false>(p);
     const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
+    if (few_rows<T>(p, access, plan)) {
+        snprintf(buf, len, "few_rows_kernel<%s, %d>", type, few_shares(p.cols, p.sum, (int)sizeof(T)));
+        return;
+    }
     static const char* const shape[3][CUTS] = {
         {"256, 256, 2, 4, 1, 2", "128, 128, 2, 2, 1, 2", "128, 128, 2, 2, 2, 4", "64, 64, 2, 2, 2, 4", "32, 32, 1, 1, 4, 8"},
         {"", "128, 128, 2, 2, 1, 2", "", "64, 64, 2, 2, 2, 2", "32, 32, 1, 1, 4, 2"},
@@ -979,18 +1003,19 @@ template <typename T, bool ACROSS_I, bool ACROSS_J>
 int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
     TCBNN_REQUIRE((long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) <= 0x7fffffffLL, "linear: grid too large");
     const Access access = access_of<T, ACROSS_I, ACROSS_J>(p);
+    const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
     if constexpr (!ACROSS_I && !ACROSS_J) {
-        if (p.rows <= kFewRows) {
-            const dim3 grid((unsigned)((p.cols + kFewOutputs - 1) / kFewOutputs));
-            if (p.rows <= 16)
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, 1>), grid, dim3(64 * kFewWaves), 0, stream, p);
+        if (few_rows<T>(p, access, plan)) {
+            const int shares = few_shares(p.cols, p.sum, (int)sizeof(T)), outputs = kFewOutputs * kFewWaves / shares;
+            const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
+            if (shares == 8)
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, 8>), grid, dim3(64 * kFewWaves), 0, stream, p);
             else
                 hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, 2>), grid, dim3(64 * kFewWaves), 0, stream, p);
             TCBNN_LAUNCH_CHECK("few_rows_kernel");
             return TCBNN_OK;
         }
     }
-    const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
     auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold) {
         constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value, H = hold.value;
         cut_product(p, B, kStepBytes / (int)sizeof(T), plan.splits, workspace);
@@ -1050,14 +1075,19 @@ static int check_linear(int rows, int in_features, int out_features, int dtype, 
 }
 
 // the partial sums of a split product
-static size_t split_bytes(int rows, int cols, int sum, int dtype) {
-    const int splits = plan_product(rows, cols, sum, (int)dtype_bytes(dtype), true, ~(size_t)0).splits;
+static size_t split_bytes(int rows, int cols, int sum, int dtype, bool forward) {
+    const int size = (int)dtype_bytes(dtype);
+    int splits = 1;
+    for (bool vectors : {false, true}) {  // (where the operands will lie is not known here)
+        const Plan plan = plan_product(rows, cols, sum, size, vectors, ~(size_t)0);
+        if (!forward || rows > kFewRows || few_time(rows, cols, sum, size, vectors) >= plan.time) splits = std::max(splits, plan.splits);
+    }
     return splits > 1 ? (size_t)splits * rows * cols * sizeof(float) : 0;
 }
 
 extern "C" size_t tcbnn_linear_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
     if (rows <= 0 || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
-    return rows <= kFewRows ? 0 : split_bytes(rows, out_features, in_features, dtype);
+    return split_bytes(rows, out_features, in_features, dtype, true);
 }
 
 static ProductParams forward_product(const tcbnn_linear_desc* d) {
@@ -1113,7 +1143,7 @@ static size_t sum_bytes(int rows, int out_features, int dtype) {
 extern "C" size_t tcbnn_linear_grad_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
     if (rows <= 0 || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
     return dz_bytes(rows, out_features, dtype) + sum_bytes(rows, out_features, dtype) +
-           std::max(split_bytes(rows, in_features, out_features, dtype), split_bytes(out_features, in_features, rows, dtype));
+           std::max(split_bytes(rows, in_features, out_features, dtype, false), split_bytes(out_features, in_features, rows, dtype, false));
 }
 
 extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stream) {

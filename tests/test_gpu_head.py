@@ -20,7 +20,7 @@ def rng(*seed):
 LINEAR = [(1, 1, 1), (1, 16, 10), (1, 4096, 512), (1, 1025, 33), (2, 8, 3), (3, 17, 5), (5, 1032, 264), (7, 33, 1000),
           (8, 512, 64), (15, 31, 65), (16, 64, 16), (17, 72, 130), (31, 2048, 96), (32, 256, 129), (33, 100, 127),
           (64, 4096, 48), (65, 65, 65), (77, 1023, 129), (127, 200, 128), (128, 128, 128), (129, 136, 257),
-          (256, 512, 1000), (300, 64, 8), (255, 1000, 511), (513, 96, 300), (1000, 24, 1030)]
+          (256, 512, 1000), (300, 64, 8), (255, 1000, 511), (513, 96, 300), (1000, 24, 1030), (4, 1023, 4099), (8, 16385, 33)]
 
 
 def _linear(gpu, m, k, n, dtype, activation, bias=True, residual=True, preact=True, gap=0, in_place=False, stream=None, shift=1):
@@ -148,7 +148,8 @@ def _kernel(m, k, n, dtype):
 
 # rows at whole 16 bytes: every tile, with whole tiles and ragged ones, whole steps of the sum and ragged ones, sums of one step, of fewer
 # than the tile keeps under way and of many; the bf16 plan of each
-WHOLE = [((1, 64, 64), "few_rows_kernel"), ((32, 1048, 72), "few_rows_kernel"), ((33, 8, 8), "32, 32"), ((40, 64, 64), "32, 32"),
+WHOLE = [((1, 64, 64), "few_rows_kernel<__bf16, 8>"), ((16, 1048, 72), "few_rows_kernel<__bf16, 8>"), ((3, 264, 16408), "few_rows_kernel<__bf16, 2>"),
+         ((9, 512, 16392), "few_rows_kernel<__bf16, 2>"), ((16, 1032, 8200), "32, 32"), ((5, 16384, 64), "join"), ((17, 1048, 72), "32, 32"), ((33, 8, 8), "32, 32"), ((40, 64, 64), "32, 32"),
          ((100, 520, 304), "32, 32"), ((300, 256, 520), "32, 32"), ((64, 2048, 2048), "32, 32"), ((64, 16384, 64), "join"),
          ((128, 4096, 136), "join"), ((1024, 512, 1024), "64, 64"), ((1000, 72, 3000), "64, 64"), ((1016, 1032, 1048), "64, 64"),
          ((2040, 136, 2040), "128, 128, 2, 2, 2, 4"), ((2048, 512, 2048), "128, 128, 2, 2, 2, 4"), ((2040, 72, 4104), "128, 128, 2, 2, 1, 2"),
@@ -415,7 +416,7 @@ def test_layernorm_without_rows(gpu):
 # and many rows of few
 LOGPROBS = [(3, 1, 1), (5, 2, 2), (700, 10, 5), (9, 63, 5), (4, 64, 64), (7, 65, 20), (33, 257, 8), (256, 1000, 5), (3, 1025, 32),
             (2, 4095, 64), (5, 4097, 0), (2, 8192, 5), (3, 16385, 20), (1, 32003, 20), (2, 50257, 1), (1, 131072, 20),
-            (300, 2050, 3), (1, 262147, 64)]
+            (300, 2050, 3), (1, 262147, 64), (2, 24255, 9), (260, 32776, 7)]
 
 
 def _logits(r, m, n, kind):
@@ -494,7 +495,7 @@ def test_logprobs(gpu, m, n, top, dtype):
 
 @pytest.mark.parametrize("dtype", ho.DTYPES)
 @pytest.mark.parametrize("kind", ["ties", "equal", "sorted", "cluster", "stride", "masked", "lowest", "special"])
-@pytest.mark.parametrize("m,n,top", [(4, 100, 64), (3, 1000, 20), (2, 4099, 64), (3, 33001, 33), (2, 140000, 64)])
+@pytest.mark.parametrize("m,n,top", [(4, 100, 64), (3, 1000, 20), (2, 4099, 64), (2, 24255, 33), (3, 33001, 33), (2, 140000, 64)])
 def test_logprobs_of_rows_that_are_hard_to_rank(gpu, m, n, top, kind, dtype):
     _logprobs(m, n, top, dtype, kind, gap=GAPS[dtype] if n % 2 else 8)
 

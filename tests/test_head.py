@@ -120,7 +120,9 @@ def test_kernel_names():
     need = lib.tcbnn_linear_workspace_bytes(64, 16384, 64, 1)
     assert need > 0 and "join" in name(workspace=P, workspace_bytes=need)
     assert "join" not in name() and "join" not in name(workspace=P, workspace_bytes=16)
-    assert name(rows=32) == "few_rows_kernel<__bf16, 2>" and name(rows=1, dtype=0) == "few_rows_kernel<float, 1>"
+    assert name(rows=16, in_features=1024) == "few_rows_kernel<__bf16, 8>" and name(rows=1, dtype=0, in_features=256) == "few_rows_kernel<float, 8>"
+    assert name(rows=3, in_features=264, out_features=16408) == "few_rows_kernel<__bf16, 2>" and "32, 32" in name(rows=17, in_features=1024)
+    assert "few" in name(rows=1) and "join" in name(rows=1, workspace=P, workspace_bytes=need)
     assert "(Access)0" in name() and "(Access)1" in name(input=P + 2) and "(Access)1" in name(input_ld=16387)
     assert "(Access)2" in name(in_features=5) and "(Access)2" in name(weight_ld=1 << 24)
     assert "256, 256" in name(rows=8192, in_features=4096, out_features=4096)
