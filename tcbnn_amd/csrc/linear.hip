@@ -367,13 +367,14 @@ __device__ __forceinline__ void meet() {
 
 // A workgroup's tile of c is BI x BJ, WI x WJ wavefronts with 32 x 32 pieces of it each, WS times over: those share the quarters of a
 // step, and their sums are added at the end.  STAGES steps of both operands lie in LDS or are on their way there;
-// what goes through registers does so HOLD steps ahead.
+// what goes through registers does so HOLD steps ahead, LONG: without a branch in sums of more than kLongSteps steps.
+constexpr int kLongSteps = 8;
 template <int BI, int BJ, int WI, int WJ, int WS, int STAGES>
 constexpr int product_lds() {
     constexpr int kStages = STAGES * (BI + BJ) * kStepBytes, kOut = 32 * (32 * (BJ / WJ / 32) * 4 + 16) * WI * WJ * WS;
     return kStages > kOut ? kStages : kOut;
 }
-template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool ACROSS_I, bool ACROSS_J>
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG, bool ACROSS_I, bool ACROSS_J>
 __device__ __forceinline__ void product(const ProductParams& p, int block, char* lds) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
     constexpr int kThreads = 64 * WI * WJ * WS, NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec, kQuarters = 4 / WS;
@@ -539,14 +540,13 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
                 if constexpr (HOLD == 4) f(integral_constant<int, 1>()), f(integral_constant<int, 2>()), f(integral_constant<int, 3>());
             };
             static_assert(HOLD == 1 || HOLD == 4, "");
-            each([&](auto k) {
-                if (k.value < steps) request_i(0, k.value, k), request_j(0, k.value, k);
-            });
-            hand_over(0, 0, slot0);
-            if (HOLD < steps) request_i(0, HOLD, slot0), request_j(0, HOLD, slot0);
-            fragments(0, 0, 0);
+            auto request_both = [&](int step, auto slot) { request_i(0, step, slot), request_j(0, step, slot); };
             // `slot`: step % HOLD
-            auto advance = [&](int step, auto slot) {
+            enum { NOTHING, IF_ANY, ALWAYS };
+            constexpr integral_constant<int, NOTHING> nothing;
+            constexpr integral_constant<int, IF_ANY> if_any;
+            constexpr integral_constant<int, ALWAYS> always;
+            auto advance = [&](int step, auto slot, auto more) {
                 const int next = stage ^ 1;
                 constexpr integral_constant<int, (slot.value + 1) % HOLD> next_slot;
 #pragma unroll
@@ -555,9 +555,9 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
                     multiply(k & 1);
                     interleave(reads, slot0);
                 }
-                if (step + 1 < steps) {
+                if (more.value == ALWAYS || step + 1 < steps) {
                     hand_over(next, step + 1, next_slot);
-                    if (step + 1 + HOLD < steps) request_i(0, step + 1 + HOLD, next_slot), request_j(0, step + 1 + HOLD, next_slot);
+                    if (more.value == ALWAYS || (more.value == IF_ANY && step + 1 + HOLD < steps)) request_both(min(step + 1 + HOLD, steps - 1), next_slot);
                     fragments(kQuarters & 1, next, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -571,10 +571,31 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
                 }
                 stage = next;
             };
-            for (int step = 0; step < steps; step += HOLD)
+            // LONG: in long sums every step requests another without a branch, the last ones the last step again.  Where a request may or
+            // may not have been made the compiler does not know how many came after the one that it waits for, and waits for
+            // them all.
+            int step = 0;
+            if (LONG && steps > kLongSteps) {
+                each([&](auto k) { request_both(k.value, k); });
+                hand_over(0, 0, slot0);
+                request_both(HOLD, slot0);
+                fragments(0, 0, 0);
+                for (; step + HOLD < steps; step += HOLD) each([&](auto k) { advance(step + k.value, k, always); });
                 each([&](auto k) {
-                    if (step + k.value < steps) advance(step + k.value, k);
+                    if (step + k.value < steps) advance(step + k.value, k, nothing);
                 });
+            } else {
+                each([&](auto k) {
+                    if (k.value < steps) request_both(k.value, k);
+                });
+                hand_over(0, 0, slot0);
+                if (HOLD < steps) request_both(HOLD, slot0);
+                fragments(0, 0, 0);
+                for (; step < steps; step += HOLD)
+                    each([&](auto k) {
+                        if (step + k.value < steps) advance(step + k.value, k, if_any);
+                    });
+            }
         }
     }
     __syncthreads();
@@ -645,10 +666,10 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
     }
 #endif
 }
-template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool ACROSS_I, bool ACROSS_J>
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG, bool ACROSS_I, bool ACROSS_J>
 __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const ProductParams p) {
     __shared__ __align__(1024) char lds[product_lds<BI, BJ, WI, WJ, WS, STAGES>()];
-    product<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, ACROSS_I, ACROSS_J>(p, blockIdx.x, lds);
+    product<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, LONG, ACROSS_I, ACROSS_J>(p, blockIdx.x, lds);
 }
 
 // the sums of all splits and what follows them
@@ -873,9 +894,9 @@ template <typename T, Access ACCESS, int STAGES, int HOLD>
 __global__ __launch_bounds__(256) void small_gradients_kernel(const ProductParams dx, const ProductParams dw, int blocks_dx) {
     __shared__ __align__(1024) char lds[product_lds<32, 32, 1, 1, 4, STAGES>()];
     if ((int)blockIdx.x < blocks_dx)
-        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, false, true>(dx, blockIdx.x, lds);
+        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, false, false, true>(dx, blockIdx.x, lds);
     else
-        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, true, true>(dw, blockIdx.x - blocks_dx, lds);
+        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, false, true, true>(dw, blockIdx.x - blocks_dx, lds);
 }
 
 // The tile that a product is cut into, how often its sum is split, and its launch.
@@ -892,11 +913,11 @@ struct CutCost {
 // Measured in tiles of 256 / 128 / 128 deep / 64 / 32, rows x inputs x outputs, 16-bit types: 8192 x 4096 x 4096 220 / 274 / 310 / 458 / -,
 // 8192 x 4096 x 1024 108 / 79 / 86 / 127 / 216, 4096 x 8192 x 1024 195 / 113 / 78 / 121 / 204, 2048^3 51 / 29 / 23 / 32 / 62, 1024^3 34 / 18 / 14 / 8.5 /
 // 12.6, 64 x 4096 x 4096 69 / 44 / 29 / 19 / 11, 512^3 25 / 11 / 11 / 6.1 / 4.7.  fp32: 4000 x 2000 x 2000 482 / 259 / 266 / 280 / -, 1000^3 256 / 78 /
-// 72 / 25 / 30, 64 x 1024 x 1024 244 / 77 / 71 / 23 / 11.  Rows that lie anywhere: 8192 x 4096 x 4096 - / 358 / - / 593 / 974, 77 x 1023 x 1537 - /
-// 22 / - / 13 / 10.
+// 72 / 25 / 30, 64 x 1024 x 1024 244 / 77 / 71 / 23 / 11.  Rows that lie anywhere: 8192 x 4096 x 4096 - / 358 / - / 593 / 974, 4001 x
+// 1999 x 1001 - / 40 / - / 55 / 86, 1000 x 1001 x 999 - / 24 / - / 10.6 / 16, 77 x 1023 x 1537 - / 22 / - / 10 / 6.6.
 constexpr CutCost kCuts16[CUTS] = {{256, 9.0f, 4.0f, 1.4f, 1.6f}, {128, 6.0f, 1.5f, 0.8f, 0.52f}, {128, 6.0f, 3.0f, 0.4f, 0.55f}, {64, 3.5f, 1.0f, 0.27f, 0.21f}, {32, 3.2f, 0.5f, 0.135f, 0.11f}};
 constexpr CutCost kCuts32[CUTS] = {{256, 12.0f, 4.0f, 7.4f, 7.4f}, {128, 6.0f, 1.5f, 2.2f, 1.95f}, {128, 6.0f, 3.0f, 2.0f, 2.05f}, {64, 3.5f, 1.0f, 0.67f, 0.55f}, {32, 3.2f, 0.5f, 0.25f, 0.22f}};
-constexpr CutCost kCutsAnywhere[CUTS] = {{}, {128, 6.0f, 0.0f, 1.0f, 0.7f}, {}, {64, 3.2f, 0.0f, 0.6f, 0.29f}, {32, 3.2f, 0.0f, 0.45f, 0.17f}};
+constexpr CutCost kCutsAnywhere[CUTS] = {{}, {128, 6.0f, 0.0f, 1.0f, 0.7f}, {}, {64, 3.2f, 1.2f, 0.42f, 0.33f}, {32, 3.2f, 0.5f, 0.18f, 0.165f}};
 constexpr float kReadRate = 5.5e6f;  // bytes of operands in a us that no tile exceeds where they are read once
 struct Plan {
     Cut cut;
@@ -927,7 +948,7 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
 // costs a wavefront a latency, and the compute unit its requests where several workgroups have one; the rows of x are read again by every
 // workgroup.  Measured, this kernel / tiles, 16-bit types: 1 x 4096 x 4096 8.4 / 14.9, 16 x 4096 x 4096 10.4 / 10.8, 4 x 8192 x 28672 80 / 85,
 // 16 x 8192 x 28672 108 / 88, 1 x 2048 x 8192 9.8 / 8.2, 1 x 16384 x 512 20 / 16; fp32: 8 x 2048 x 1024 8.7 / 11.7, 8 x 16384 x 64 48 / 24;
-// rows that lie anywhere: 8 x 999 x 1001 6.2 / 8.7, 8 x 4095 x 4097 32 / 23, 4 x 8191 x 20001 184 / 109.
+// rows that lie anywhere: 1 x 999 x 1001 5.0 / 6.0, 8 x 4095 x 4097 32 / 15, 4 x 8191 x 20001 184 / 110.
 inline int few_shares(int cols, int sum, int size) { return sum * size <= 1024 && cols > 64 * (kComputeUnits - 1) ? 2 : 8; }
 inline float few_time(int rows, int cols, int sum, int size, bool vectors) {
     const int shares = few_shares(cols, sum, size), outputs = kFewOutputs * kFewWaves / shares;
@@ -974,6 +995,14 @@ bool launch_small_gradients(ProductParams dx, ProductParams dw, hipStream_t stre
     return true;
 }
 
+// Tiles of 64 whose rows lie anywhere: the loop for long sums takes registers that a third workgroup of a compute unit would have
+// (bf16, with that loop / without: 1000 x 1001 x 999, one tile a compute unit, 10.6 us / 14.2; 2000 x 777 x 1111, three, 25.1 / 20.2).
+template <typename T>
+bool long_sums(const ProductParams& p, const Plan& plan) {
+    const long long tiles = (long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) * plan.splits;
+    return tiles <= 2 * kComputeUnits && (long long)p.sum * sizeof(T) > (long long)kLongSteps * kStepBytes * plan.splits;
+}
+
 // (tiles of single elements are for memory where addresses do not fit; they are slower in any size)
 template <typename T>
 bool few_rows(const ProductParams& p, Access access, const Plan& plan) {
@@ -995,7 +1024,8 @@ void product_name(const ProductParams& p, size_t workspace_bytes, char* buf, siz
         {"", "128, 128, 2, 2, 1, 2", "", "64, 64, 2, 2, 2, 2", "32, 32, 1, 1, 4, 2"},
         {"32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2"}};
     const int hold = access == ANYWHERE && plan.cut != CUT_128 ? 4 : 1;
-    snprintf(buf, len, "product_kernel<%s, %s, (Access)%d, %d, false, false>%s", type, shape[access][plan.cut], (int)access, hold,
+    const bool keep = hold == 4 && (plan.cut != CUT_64 || long_sums<T>(p, plan));
+    snprintf(buf, len, "product_kernel<%s, %s, (Access)%d, %d, %s, false, false>%s", type, shape[access][plan.cut], (int)access, hold, keep ? "true" : "false",
              plan.splits > 1 && access != ELEMENTS ? " + product_join_kernel" : "");
 }
 
@@ -1016,11 +1046,12 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
             return TCBNN_OK;
         }
     }
-    auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold) {
+    auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
         constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value, H = hold.value;
+        constexpr bool L = keep.value;
         cut_product(p, B, kStepBytes / (int)sizeof(T), plan.splits, workspace);
         const long long units = (long long)p.tiles_i * p.tiles_j * p.splits;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, ACROSS_I, ACROSS_J>), dim3((unsigned)units),
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, L, ACROSS_I, ACROSS_J>), dim3((unsigned)units),
                            dim3(64 * WI * WJ * WS), 0, stream, p);
         if (p.splits > 1) {
             const long long vectors_out = (long long)p.rows * ((p.cols + Elem<T>::kVec - 1) / Elem<T>::kVec);
@@ -1035,25 +1066,32 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
     constexpr std::integral_constant<int, 2> two;
     constexpr std::integral_constant<int, 4> four;
     constexpr std::integral_constant<int, 8> eight;
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
     constexpr std::integral_constant<Access, WHOLE_PIECES> pieces;
     constexpr std::integral_constant<Access, ANYWHERE> anywhere;
     constexpr std::integral_constant<Access, ELEMENTS> elements;
     if (access == WHOLE_PIECES) {
         switch (plan.cut) {
-            case CUT_256: go(n256, two, four, one, two, pieces, one); break;
-            case CUT_128: go(n128, two, two, one, two, pieces, one); break;
-            case CUT_128_DEEP: go(n128, two, two, two, four, pieces, one); break;
-            case CUT_64: go(n64, two, two, two, four, pieces, one); break;
-            default: go(n32, one, one, four, eight, pieces, one); break;
+            case CUT_256: go(n256, two, four, one, two, pieces, one, no); break;
+            case CUT_128: go(n128, two, two, one, two, pieces, one, no); break;
+            case CUT_128_DEEP: go(n128, two, two, two, four, pieces, one, no); break;
+            case CUT_64: go(n64, two, two, two, four, pieces, one, no); break;
+            default: go(n32, one, one, four, eight, pieces, one, no); break;
         }
     } else if (access == ANYWHERE) {
         switch (plan.cut) {
-            case CUT_128: go(n128, two, two, one, two, anywhere, one); break;
-            case CUT_64: go(n64, two, two, two, two, anywhere, four); break;
-            default: go(n32, one, one, four, two, anywhere, four); break;
+            case CUT_128: go(n128, two, two, one, two, anywhere, one, no); break;
+            case CUT_64:
+                if (long_sums<T>(p, plan))
+                    go(n64, two, two, two, two, anywhere, four, yes);
+                else
+                    go(n64, two, two, two, two, anywhere, four, no);
+                break;
+            default: go(n32, one, one, four, two, anywhere, four, yes); break;
         }
     } else {
-        go(n32, one, one, four, two, elements, one);
+        go(n32, one, one, four, two, elements, one, no);
     }
     TCBNN_LAUNCH_CHECK("product_kernel");
     return TCBNN_OK;
