@@ -388,8 +388,8 @@ int tcbnn_avgpool_fc_forward(const tcbnn_avgpool_fc_desc* d, void* stream);
  * one element.  Activations, weights and logits have the type `dtype` names; bias, gamma, beta, statistics, log
  * probabilities and the gradients of bias, gamma and beta are fp32.  Sums are held in fp32 and every output is rounded
  * once.  A call with rows = 0 launches nothing (the gradients of parameters become 0); other sizes are positive.
- * Outputs may not overlap inputs or each other except where noted.  Results do not depend on what else runs: no atomics,
- * the same sums in the same order in every call of the same sizes. */
+ * Outputs may not overlap inputs or each other except where noted.  Results do not depend on what else runs: the
+ * same sums in the same order in every call of the same sizes and workspace. */
 #define TCBNN_F32 0
 #define TCBNN_BF16 1
 #define TCBNN_F16 2
