@@ -785,14 +785,16 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
 constexpr int kDzThreads = 256;
 // Rows that one thread takes, and the parts that a column's sum falls into (a part a workgroup).
 inline int dz_lanes(int vectors) { return vectors >= kDzThreads ? kDzThreads : vectors; }  // of a workgroup, side by side
-inline int dz_rows(int rows, int vectors) {
+inline int dz_rows(int rows, int vectors, bool active) {
     const long long threads = 1024LL * kComputeUnits;  // four workgroups a compute unit
     const int each = (int)std::max(8LL, ((long long)rows * vectors + threads - 1) / threads), deep = kDzThreads / dz_lanes(vectors);
-    // one part needs no join: 16 rows a thread take less time than that launch
-    return rows <= 16 * deep ? std::max(each, (rows + deep - 1) / deep) : each;
+    // one part needs no join: 16 rows a thread with their activation's slopes, 32 without, take less time than that launch (one
+    // workgroup with 32 rows of GELU a thread: gradients of 64 x 1024 -> 1024 29.7 us, 19.7 with a join; 36 x 860 -> 489
+    // fp32 without an activation 14.2 in one part, 17.7 with a join)
+    return rows <= (active ? 16 : 32) * deep ? std::max(each, (rows + deep - 1) / deep) : each;
 }
-inline int dz_parts(int rows, int vectors) {
-    const int deep = kDzThreads / dz_lanes(vectors) * dz_rows(rows, vectors);
+inline int dz_parts(int rows, int vectors, bool active) {
+    const int deep = kDzThreads / dz_lanes(vectors) * dz_rows(rows, vectors, active);
     return (rows + deep - 1) / deep;
 }
 
@@ -888,15 +890,17 @@ __global__ __launch_bounds__(kDzThreads) void column_join_kernel(const float* __
     }
 }
 
-// ---- both products of small gradients in one launch: the first workgroups have dx, the others dw.  A launch more takes as long as
-// these products do (102 x 24 -> 21 f16 with its dz: 15.9 us in three launches, 9.8 in two).
+// ---- both products of small gradients in one launch.  A launch more takes as long as these products do (102 x 24 -> 21 f16 with its dz:
+// 15.9 us in three launches, 9.8 in two; 128 x 1024 -> 512 18.3 and 15.7).  The first `blocks` workgroups have the product with the longer sum:
+// started last, they would run on alone (1024 x 1024 -> 10 fp32 21.5 us, 19.4 so).
 template <typename T, Access ACCESS, int STAGES, int HOLD>
-__global__ __launch_bounds__(256) void small_gradients_kernel(const ProductParams dx, const ProductParams dw, int blocks_dx) {
+__global__ __launch_bounds__(256) void small_gradients_kernel(const ProductParams dx, const ProductParams dw, int blocks, bool dw_first) {
     __shared__ __align__(1024) char lds[product_lds<32, 32, 1, 1, 4, STAGES>()];
-    if ((int)blockIdx.x < blocks_dx)
-        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, false, false, true>(dx, blockIdx.x, lds);
+    const int second = (int)blockIdx.x >= blocks, block = (int)blockIdx.x - (second ? blocks : 0);
+    if (second == dw_first)
+        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, ACCESS == ANYWHERE, false, true>(dx, block, lds);
     else
-        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, false, true, true>(dw, blockIdx.x - blocks_dx, lds);
+        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, ACCESS == ANYWHERE, true, true>(dw, block, lds);
 }
 
 // The tile that a product is cut into, how often its sum is split, and its launch.
@@ -924,11 +928,11 @@ struct Plan {
     int splits;
     float time;
 };
-inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, size_t workspace_bytes) {
+inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, size_t workspace_bytes, Cut largest = CUT_256) {
     const int steps = (int)(((long long)sum * size + kStepBytes - 1) / kStepBytes);
     const float read = ((float)rows + (float)cols) * (float)sum * (float)size / kReadRate;
     Plan best = {CUT_32, 1, 0.0f};
-    for (int c = 0; c < CUTS; ++c) {
+    for (int c = largest; c < CUTS; ++c) {
         CutCost cost = vectors ? (size == 4 ? kCuts32[c] : kCuts16[c]) : kCutsAnywhere[c];
         if (cost.size == 0) continue;
         if (!vectors && size == 4) cost.step = std::max(cost.step, kCuts32[c].step), cost.more = std::max(cost.more, kCuts32[c].more);
@@ -976,22 +980,29 @@ inline void cut_product(ProductParams& p, int size, int steps_size, int splits, 
     p.partial = workspace;
 }
 
-// dx and dw, where both are products of 32 x 32 tiles, four a compute unit at most; false: nothing is launched
+// dx and dw in one launch, where in tiles of 32 x 32, four a compute unit at most, they are estimated to take less time together than
+// apart in tiles and splits of their own; false: nothing is launched
 template <typename T>
-bool launch_small_gradients(ProductParams dx, ProductParams dw, hipStream_t stream) {
-    const Access access = std::max(access_of<T, false, true>(dx), access_of<T, true, true>(dw));
-    auto small = [&](const ProductParams& p) {
-        const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0);
-        return plan.cut == CUT_32 && (long long)((p.rows + 31) / 32) * ((p.cols + 31) / 32) <= 4 * kComputeUnits;
-    };
-    if (access == ELEMENTS || !small(dx) || !small(dw)) return false;
+bool launch_small_gradients(ProductParams dx, ProductParams dw, size_t workspace_bytes, hipStream_t stream) {
+    const Access access_dx = access_of<T, false, true>(dx), access_dw = access_of<T, true, true>(dw), access = std::max(access_dx, access_dw);
+    float together = -kCuts16[CUT_32].start, apart = 0.0f;
+    for (const ProductParams* p : {&dx, &dw}) {
+        if ((long long)((p->rows + 31) / 32) * ((p->cols + 31) / 32) > 4 * kComputeUnits) return false;
+        together += plan_product(p->rows, p->cols, p->sum, (int)sizeof(T), access == WHOLE_PIECES, 0, CUT_32).time;
+        apart += plan_product(p->rows, p->cols, p->sum, (int)sizeof(T), (p == &dx ? access_dx : access_dw) == WHOLE_PIECES, workspace_bytes).time;
+    }
+    if (access == ELEMENTS || together >= apart) return false;
     cut_product(dx, 32, kStepBytes / (int)sizeof(T), 1, nullptr);
     cut_product(dw, 32, kStepBytes / (int)sizeof(T), 1, nullptr);
-    const int blocks_dx = dx.tiles_i * dx.tiles_j, blocks = blocks_dx + dw.tiles_i * dw.tiles_j;
+    const int blocks_dx = dx.tiles_i * dx.tiles_j, blocks_dw = dw.tiles_i * dw.tiles_j;
+    const bool dw_first = dw.sum > dx.sum;
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks_dx + blocks_dw)), dim3(256), 0, stream, dx, dw, dw_first ? blocks_dw : blocks_dx, dw_first);
+    };
     if (access == WHOLE_PIECES)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(small_gradients_kernel<T, WHOLE_PIECES, 8, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, dx, dw, blocks_dx);
+        go(small_gradients_kernel<T, WHOLE_PIECES, 8, 1>);
     else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(small_gradients_kernel<T, ANYWHERE, 2, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, dx, dw, blocks_dx);
+        go(small_gradients_kernel<T, ANYWHERE, 2, 4>);
     return true;
 }
 
@@ -1176,7 +1187,7 @@ static size_t dz_bytes(int rows, int out_features, int dtype) { return whole_lin
 static int out_vectors(int out_features, int dtype) { return (out_features + (int)(16 / dtype_bytes(dtype)) - 1) / (int)(16 / dtype_bytes(dtype)); }
 
 static size_t sum_bytes(int rows, int out_features, int dtype) {
-    return rows == 0 ? 0 : whole_lines(sizeof(float) * dz_parts(rows, out_vectors(out_features, dtype)) * (size_t)out_features);
+    return rows == 0 ? 0 : whole_lines(sizeof(float) * dz_parts(rows, out_vectors(out_features, dtype), true) * (size_t)out_features);
 }
 extern "C" size_t tcbnn_linear_grad_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
     if (rows <= 0 || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
@@ -1207,14 +1218,14 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
     return by_dtype(d->dtype, [&](auto t) -> int {
         using T = decltype(t);
         if (active || d->grad_bias) {
-            const int vectors = out_vectors(d->out_features, d->dtype), lanes = dz_lanes(vectors), parts = dz_parts(d->rows, vectors);
+            const int vectors = out_vectors(d->out_features, d->dtype), lanes = dz_lanes(vectors), parts = dz_parts(d->rows, vectors, active);
             float* sums = d->grad_bias ? (float*)((char*)d->workspace + dz_bytes(d->rows, d->out_features, d->dtype)) : nullptr;
             if (d->grad_bias && parts == 1 && d->rows > 0) sums = d->grad_bias;
             if (d->rows > 0)
                 by_activation(d->activation, [&](auto act) {
                     hipLaunchKernelGGL(HIP_KERNEL_NAME(dz_kernel<T, act.value>), dim3((unsigned)((vectors + lanes - 1) / lanes), (unsigned)parts),
                                        dim3(kDzThreads), 0, (hipStream_t)stream, (const T*)d->grad_output, (const T*)d->preact,
-                                       (T*)d->workspace, sums, d->rows, d->out_features, lanes, dz_rows(d->rows, vectors), dy_ld, z_ld);
+                                       (T*)d->workspace, sums, d->rows, d->out_features, lanes, dz_rows(d->rows, vectors, active), dy_ld, z_ld);
                 });
             if (d->grad_bias && sums != d->grad_bias)
                 hipLaunchKernelGGL(column_join_kernel, dim3((unsigned)((d->out_features + kJoinColumns - 1) / kJoinColumns)), dim3(kDzThreads), 0,
@@ -1239,7 +1250,7 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
         dw.sum = d->rows;
         dw.out = d->grad_weight;
         dw.out_ld = dw_ld;
-        if (d->grad_input && d->grad_weight && d->rows > 0 && launch_small_gradients<T>(dx, dw, (hipStream_t)stream)) {
+        if (d->grad_input && d->grad_weight && d->rows > 0 && launch_small_gradients<T>(dx, dw, partial_bytes, (hipStream_t)stream)) {
             TCBNN_LAUNCH_CHECK("small_gradients_kernel");
             return TCBNN_OK;
         }

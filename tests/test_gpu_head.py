@@ -20,7 +20,8 @@ def rng(*seed):
 LINEAR = [(1, 1, 1), (1, 16, 10), (1, 4096, 512), (1, 1025, 33), (2, 8, 3), (3, 17, 5), (5, 1032, 264), (7, 33, 1000),
           (8, 512, 64), (15, 31, 65), (16, 64, 16), (17, 72, 130), (31, 2048, 96), (32, 256, 129), (33, 100, 127),
           (64, 4096, 48), (65, 65, 65), (77, 1023, 129), (127, 200, 128), (128, 128, 128), (129, 136, 257),
-          (256, 512, 1000), (300, 64, 8), (255, 1000, 511), (513, 96, 300), (1000, 24, 1030), (4, 1023, 4099), (8, 16385, 33), (1000, 1001, 999)]
+          (256, 512, 1000), (300, 64, 8), (255, 1000, 511), (513, 96, 300), (1000, 24, 1030), (4, 1023, 4099), (8, 16385, 33), (1000, 1001, 999),
+          (36, 860, 489), (200, 304, 16), (128, 520, 512)]
 
 
 def _linear(gpu, m, k, n, dtype, activation, bias=True, residual=True, preact=True, gap=0, in_place=False, stream=None, shift=1):
