@@ -7,7 +7,7 @@
 // Bound by memory: every value is read once and kept in registers as fp32 (the variance is summed about the mean, which one
 // pass over the memory allows because the row is still there).  A row belongs to a team of W wavefronts whose lanes hold R
 // vectors of 16 bytes each; teams go from row to row, so gamma, beta and the gradient's sums over rows stay in registers too.
-// 16384 x 4096 bf16: 50 us forward (268 MB, 5.3 TB/s); 8192 x 4096: 49 us backward (201 MB and the sums, 4.1 TB/s).  A row
+// 16384 x 4096 bf16: 50 us forward (268 MB, 5.3 TB/s); 8192 x 4096: 46 us backward (201 MB and the sums, 4.4 TB/s).  A row
 // alone (1 x 4096) takes 3.2 us: the launch, one latency of memory and two sums over a team.
 #include "head.h"
 
@@ -207,9 +207,12 @@ __global__ __launch_bounds__(kGradThreads) void layernorm_grad_kernel(const T* _
     const int lane = threadIdx.x % (64 * W), wave = lane >> 6, team = threadIdx.x / (64 * W);
     Slice g, s, d, dg, db;
     typename Slice::Raw raw_x, raw_dy;
+    float next_mean, next_rstd;
     const long long stride = (long long)gridDim.x * kTeams;
     auto request = [&](long long first) {
         const long long row = min(first + team, (long long)rows - 1);
+        next_mean = mean_in[row];
+        next_rstd = rstd_in[row];
         Slice::request(x + row * x_ld, lane, n, raw_x);
         Slice::request(dy + row * dy_ld, lane, n, raw_dy);
     };
@@ -226,8 +229,8 @@ __global__ __launch_bounds__(kGradThreads) void layernorm_grad_kernel(const T* _
         const long long row = min(first + team, (long long)rows - 1);
         s.take(raw_x);
         d.take(raw_dy);
+        const float mean = next_mean, rstd = next_rstd;
         if (first + stride < rows) request(first + stride);
-        const float mean = mean_in[row], rstd = rstd_in[row];
         float sg = 0.0f, sgx = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -372,7 +375,7 @@ __global__ __launch_bounds__(kJoinThreads) void layernorm_join_kernel(const floa
 }
 
 // The team of wavefronts that keeps a row of so many vectors of 16 bytes: one vector a lane, two in the longest (8192 x 4096 bf16 in
-// teams of 8 wavefronts 26.4 us forward and 49 backward; 4, two vectors a lane, 28.0 and 63; 16, half of them idle, 34.7 and 61).
+// teams of 8 wavefronts 26.2 us forward and 46 backward; 4, two vectors a lane, 28.0 and 71; 16, half of them idle, 34.0 and 61).
 inline int row_vectors(int n, int per_vector) { return (n + per_vector - 1) / per_vector; }
 constexpr int kMaxVectors = 2 * 16 * 64;
 template <typename F>
