@@ -912,7 +912,7 @@ __global__ __launch_bounds__(256) void small_gradients_kernel(const ProductParam
 //
 // The plan is the one with the shortest estimate, from what the tiles measured (us): a step of the sum takes `step` when a
 // compute unit has one tile to work on (latency, then), `more` for each when it has several, `tile` besides for every tile after
-// the first, and a launch `start`.  A split sum is joined by a kernel of its own: 4.5 (6, where splits of rows that lie anywhere start)
+// the first, and a launch `start`.  A split sum is joined by a kernel of its own: 2.3 (3, where splits of rows that lie anywhere start)
 // and the partial sums' bytes, out and back in, at 4 TB/s.
 enum Cut : int { CUT_256, CUT_128, CUT_128_DEEP, CUT_64, CUT_32, CUTS };
 struct CutCost {
@@ -946,7 +946,7 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
             const size_t partial = k > 1 ? (size_t)k * rows * cols * sizeof(float) : 0;
             if (partial > workspace_bytes) break;
             const float rounds = std::ceil(tiles * (float)k / (float)kComputeUnits), each = std::max(cost.step, rounds * cost.more);
-            const float time = cost.start + (rounds - 1.0f) * cost.tile + std::max((float)((steps + k - 1) / k) * each, read) + (k > 1 ? (vectors ? 4.5f : 6.0f) + (float)partial * 2.0f / 4.0e6f : 0.0f);
+            const float time = cost.start + (rounds - 1.0f) * cost.tile + std::max((float)((steps + k - 1) / k) * each, read) + (k > 1 ? (vectors ? 2.3f : 3.0f) + (float)partial * 2.0f / 4.0e6f : 0.0f);
             if (best.time == 0.0f || time < best.time) best = {(Cut)c, k, time};
         }
     }
