@@ -955,9 +955,9 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
 
 // The kernel for few rows instead: the wavefronts' shares of a sum, and the estimate to compare with a plan's.  A chunk of 64 bytes
 // costs a wavefront a latency, and the compute unit its requests where several workgroups have one; the rows of x are read again by every
-// workgroup.  Measured, this kernel / tiles, 16-bit types: 1 x 4096 x 4096 8.4 / 14.9, 16 x 4096 x 4096 10.4 / 10.8, 4 x 8192 x 28672 80 / 85,
-// 16 x 8192 x 28672 108 / 88, 1 x 2048 x 8192 9.8 / 8.2, 1 x 16384 x 512 20 / 16; fp32: 8 x 2048 x 1024 8.7 / 11.7, 8 x 16384 x 64 48 / 24;
-// rows that lie anywhere: 1 x 999 x 1001 5.0 / 6.0, 8 x 4095 x 4097 32 / 15, 4 x 8191 x 20001 184 / 110.
+// workgroup.  Measured, this kernel / tiles, 16-bit types: 1 x 4096 x 4096 8.2 / 10.1, 16 x 4096 x 4096 10.4 / 10.8, 4 x 8192 x 28672 80 / 88,
+// 16 x 8192 x 28672 108 / 88, 1 x 2048 x 8192 9.8 / 8.2, 1 x 16384 x 512 20 / 9.6; fp32: 1 x 4096 x 4096 16.3 / 21.8, 8 x 16384 x 64 48 / 21;
+// rows that lie anywhere: 1 x 999 x 1001 5.1 / 6.0, 8 x 4095 x 4097 32 / 15, 4 x 8191 x 20001 184 / 110.
 inline int few_shares(int cols, int sum, int size) { return sum * size <= 1024 && cols > 64 * (kComputeUnits - 1) ? 2 : 8; }
 inline float few_time(int rows, int cols, int sum, int size, bool vectors) {
     const int shares = few_shares(cols, sum, size), outputs = kFewOutputs * kFewWaves / shares;
