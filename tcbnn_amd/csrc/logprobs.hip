@@ -16,6 +16,7 @@ namespace {
 using namespace head;
 
 constexpr int kMaxTop = 64;
+constexpr float kNear = 65536.0f;  // |m| up to which sums of exp(x - m) are taken about m log2 e, rounded
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 
 // The order of classes as one number: larger logits first (NaN before all, -0 with +0), lower indices first among equals.
@@ -201,9 +202,9 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
     }
     Part part = {wave_max(lane_max), 0.0f, 0.0f, 0};
     // ---- sums about it, and what goes before the given class.
-    // exp(x - m) = 2^u, u = x log2 e - c with c = m log2 e rounded: one fused multiply-add, as exact as a difference of x and
-    // m, but about c.  `off`, what c was rounded by, takes the sums back to m.  u is held above -250, where 2^u is 0 anyway: 0
-    // times -inf is NaN.
+    // exp(x - m) = 2^u, u = x log2 e - c with c = m log2 e rounded: one fused multiply-add, but about c.  `off`, what c was rounded by,
+    // takes the sums back to m while it is small: it is 2^-8 at most up to kNear, and grows with m.  u is held above -250, where 2^u is
+    // 0 anyway: 0 times -inf is NaN.
     // Before the class go larger logits and equal ones of lower index: whole vectors below it compare with the next lower
     // number, the equal ones in the class's own vector are counted afterwards.
     const float m = part.m == -INFINITY ? 0.0f : part.m, c = m * kLog2e, off = __builtin_fmaf(m, kLog2e, -c);
@@ -231,13 +232,17 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
         if (r + 1 < R) asm volatile("" : "+v"(raw[r + 1]));
         __builtin_amdgcn_sched_barrier(0);
     }
-    if (fabsf(m) > 1e38f) {  // log2 e times that is infinite; neighbours are so far apart that only equal logits count
-        const float one = m < INFINITY ? 1.0f : NAN;
+    if (fabsf(m) > kNear) {  // the row once more (from the cache), every logit's difference to m first: exact beside m, whatever m is
         part.s = part.sx = 0.0f;
 #pragma unroll 1
-        for (int j = tid; j < n; j += kTeam) {
-            const float v = (float)x[j];
-            part.s += v == m ? one : (v != v ? v : 0.0f);
+        for (int j = tid * V; j < n; j += kStep) {
+            const Words w = j + V <= n ? load_words(x + j) : load_rest(x + j, n - j);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float d = value<T>(w, e) - m, ex = __builtin_amdgcn_exp2f(d * kLog2e);
+                part.s += ex;
+                part.sx = __builtin_fmaf(ex, fmaxf(d, -200.0f), part.sx);
+            }
         }
     } else {
         part.sx = __builtin_fmaf(-off, part.s, part.sx) * kLn2;

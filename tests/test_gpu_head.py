@@ -501,6 +501,75 @@ def test_logprobs_of_rows_that_are_hard_to_rank(gpu, m, n, top, kind, dtype):
     _logprobs(m, n, top, dtype, kind, gap=GAPS[dtype] if n % 2 else 8)
 
 
+# one wavefront a row (dealt, and in vectors), four, and rows in several chunks
+SHAPES = [(4, 100, 20), (3, 1000, 20), (2, 4099, 33), (2, 24255, 33), (3, 33001, 20), (2, 140000, 64)]
+
+
+def _about_the_largest(x, t, top):
+    """ho.logprobs() of a row of finite logits, with log probabilities as (x - m) - log sum: x - logsumexp loses the sum's
+    logarithm in any type once the logits are large enough."""
+    _, _, _, rank, best, _ = ho.logprobs(x, t, top)
+    d = x - x.max()
+    log_sum = np.log(np.exp(d).sum())
+    p = np.exp(d - log_sum)
+    lp = d - log_sum
+    return lp[t], -(p * np.where(p > 0, lp, 0.0)).sum(), x.max() + log_sum, rank, best, lp[best]
+
+
+def _against_definition(x, t, top, dtype):
+    """forward() of rows given as a Matrix, with tolerances that do not grow with the logits: exp and log are good to two units, the
+    argument of exp adds 1.5 of its size, whose mean under the distribution is below log n; sums over at least 64 lanes; x - m
+    and a log probability are rounded once each.  A logsumexp's own rounding is of its size."""
+    from tcbnn_amd import head
+    m, n = x.shape
+    layer = head.LogProbsLayerParam("logprobs", m, n, top, dtype).initialize(x.view, ho.vector(t, np.int32))
+    layer.forward()
+    ho.sync()
+    got = layer.download_output()
+    want = [_about_the_largest(x.values[i], int(t[i]), top) for i in range(m)]
+    np.testing.assert_array_equal(got["rank"], [w[3] for w in want])
+    np.testing.assert_array_equal(got["top_index"], np.stack([w[4] for w in want]))
+    depth, log_n = n / 64 + 24, np.log(n)
+    base = ho.U32 * (depth + 8 + 4 * log_n)
+    lp, lse, ent, best = (np.array([w[k] for w in want]) for k in (0, 2, 1, 5))
+    ho.check(got["logprob"], lp, base + 2 * ho.U32 * np.abs(lp), "logprob")
+    ho.check(got["top_logprob"], best, base + 2 * ho.U32 * np.abs(best), "top_logprob")
+    ho.check(got["logsumexp"], lse, base + 1.01 * ho.U32 * np.abs(lse), "logsumexp")
+    ho.check(got["entropy"], ent, (2 * depth + 24) * ho.U32 * (log_n + 2 + ent), "entropy")
+    layer.release()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,top", SHAPES)
+def test_logprobs_far_from_zero(gpu, m, n, top, dtype):
+    """Finite logits about any value: spread as far as the type's neighbours are there, and all equal."""
+    r = rng(m, n, 21)
+    for about in (1e5, 1e6, -1e6, 1e7, 1e9, -1e9, 1e20, -1e30, 1e37, 3e38):
+        v = about + 3.0 * r.standard_normal((m, n))
+        v[-1] = about
+        v[0] *= 1.0 - 2.0 ** -8 * r.integers(0, 3, n)
+        _against_definition(ho.Matrix(v, dtype), r.integers(0, n, m).astype(np.int32), top, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [-1e9, -1e10, -1e30, "lowest"])
+@pytest.mark.parametrize("m,n,top", SHAPES)
+def test_logprobs_of_finite_masks(gpu, m, n, top, value, dtype):
+    """A finite value in the place of forbidden classes: behind the allowed ones (whole wavefronts' shares and chunks), before them,
+    in all places but one, in all."""
+    if value == "lowest":
+        value = {"f32": -3.4028234663852886e38, "bf16": -3.3895313892515355e38}[dtype]
+    r = rng(m, n, 22)
+    for first, last in ((n // 3, n), (0, n - n // 5), (0, n), (n // 2 + 1, n)):
+        v = 3.0 * r.standard_normal((m, n))
+        v[:, first:last] = value
+        if last - first < n // 2:
+            v[:, :first - 1] = value
+        t = r.integers(0, n, m).astype(np.int32)
+        t[0] = first - 1 if first else (last if last < n else 0)
+        _against_definition(ho.Matrix(v, dtype), t, top, dtype)
+
+
 def test_logprobs_outputs_are_optional(gpu):
     """What is not asked for is not needed: entropy alone, the best classes alone."""
     import ctypes as C
