@@ -202,9 +202,9 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
     }
     Part part = {wave_max(lane_max), 0.0f, 0.0f, 0};
     // ---- sums about it, and what goes before the given class.
-    // exp(x - m) = 2^u, u = x log2 e - c with c = m log2 e rounded: one fused multiply-add, but about c.  `off`, what c was rounded by,
-    // takes the sums back to m while it is small: it is 2^-8 at most up to kNear, and grows with m.  u is held above -250, where 2^u is
-    // 0 anyway: 0 times -inf is NaN.
+    // exp(x - m) = 2^u, u = x log2 e - c with c = m log2 e rounded: one fused multiply-add, but about c: every term is
+    // 2^off too large and every u off, where `off` is what c was rounded by (known exactly; 2^-8 at most up to kNear, as exact then as
+    // differences of x and m).  u is held above -250, where 2^u is 0 anyway: 0 times -inf is NaN.
     // Before the class go larger logits and equal ones of lower index: whole vectors below it compare with the next lower
     // number, the equal ones in the class's own vector are counted afterwards.
     const float m = part.m == -INFINITY ? 0.0f : part.m, c = m * kLog2e, off = __builtin_fmaf(m, kLog2e, -c);
@@ -245,8 +245,9 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
             }
         }
     } else {
-        part.sx = __builtin_fmaf(-off, part.s, part.sx) * kLn2;
-        part.s = __builtin_fmaf(-off * kLn2, part.s, part.s);
+        const float back = __builtin_amdgcn_exp2f(-off);
+        part.sx = __builtin_fmaf(-off, part.s, part.sx) * (back * kLn2);
+        part.s *= back;
     }
     if (!kDealt && wave == 0 && t >= 0 && t < n && lane < t % V) part.before += (float)x[t - 1 - lane] == xt;
     part.before = wave_sum_int(part.before);

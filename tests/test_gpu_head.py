@@ -551,6 +551,15 @@ def test_logprobs_far_from_zero(gpu, m, n, top, dtype):
         _against_definition(ho.Matrix(v, dtype), r.integers(0, n, m).astype(np.int32), top, dtype)
 
 
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,n,top", SHAPES)
+def test_logprobs_at_ordinary_offsets(gpu, m, n, top, dtype):
+    """Entropies and log probabilities as good about 60000 as about 0."""
+    r = rng(m, n, 23)
+    for about in (-30.0, 100.0, -1000.0, 3000.0, 20000.0, -60000.0, 60000.0):
+        _against_definition(ho.Matrix(about + 2.5 * r.standard_normal((m, n)), dtype), r.integers(0, n, m).astype(np.int32), top, dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("value", [-1e9, -1e10, -1e30, "lowest"])
 @pytest.mark.parametrize("m,n,top", SHAPES)
