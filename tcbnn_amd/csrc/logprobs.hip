@@ -188,7 +188,7 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
     const int target = p.targets ? p.targets[row] : -1;
     const bool given = target >= 0 && target < p.classes;
     const int t = target - base;  // within the chunk, before it or behind it
-    const float xt = given ? (float)x[t] : 0.0f;
+    const float xt = given ? (float)x[t] + 0.0f : 0.0f;  // (+0 for -0: the sign of +0 - +0 and of +0 - -0 is clear)
     if (tid == 0) lds.count = 0;
 
     // ---- the largest logit of each vector, of the lane, of the wavefront

@@ -579,6 +579,36 @@ def test_logprobs_of_finite_masks(gpu, m, n, top, value, dtype):
         _against_definition(ho.Matrix(v, dtype), t, top, dtype)
 
 
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,n,top", SHAPES)
+def test_logprobs_of_negative_zeros(gpu, m, n, top, dtype):
+    """-0 and +0 are equal logits: a target that holds either has the rank that its index among them says, and is where the best
+    classes say."""
+    from tcbnn_amd import head
+    r = rng(m, n, 24)
+    for share in (0.0, 0.5, 1.0):  # of -0 among the classes besides the target
+        v = np.where(r.random((m, n)) < share, -0.0, 0.0)
+        v[1, r.integers(0, n, n // 4)] = -1.0
+        v[-1, r.integers(0, n, 3)] = 1.0
+        for sign in (-0.0, 0.0):
+            for at in (0, 5, n // 2, n - 1, n // 3 + 1):
+                t = np.full(m, at, np.int32)
+                w = v.copy()
+                w[:, at] = sign
+                x = ho.Matrix(w, dtype)
+                layer = head.LogProbsLayerParam("logprobs", m, n, top, dtype).initialize(x.view, ho.vector(t, np.int32))
+                layer.forward()
+                ho.sync()
+                got = layer.download_output()
+                want = [ho.logprobs(row, at, top) for row in x.values]
+                np.testing.assert_array_equal(got["rank"], [a[3] for a in want])
+                np.testing.assert_array_equal(got["top_index"], np.stack([a[4] for a in want]))
+                for i in range(m):
+                    if got["rank"][i] < top:
+                        assert got["top_index"][i, got["rank"][i]] == at
+                layer.release()
+
+
 def test_logprobs_outputs_are_optional(gpu):
     """What is not asked for is not needed: entropy alone, the best classes alone."""
     import ctypes as C
