@@ -68,9 +68,12 @@ class DeviceView:
 
     @classmethod
     def of(cls, tensor):
-        """A torch tensor of one or two dimensions whose rows are contiguous."""
-        if tensor.dim() > 2 or (tensor.shape[-1] > 1 and tensor.stride(-1) != 1):
+        """A torch tensor of one or two dimensions whose rows are contiguous and apart (an expanded one's are not: they
+        are one piece of memory, and a layer would go past it)."""
+        if tensor.dim() not in (1, 2) or (tensor.shape[-1] > 1 and tensor.stride(-1) != 1):
             raise _lib.TcbnnError("a layer takes vectors and matrices with contiguous rows")
+        if tensor.dim() == 2 and tensor.shape[0] > 1 and tensor.stride(0) < tensor.shape[1]:
+            raise _lib.TcbnnError("a layer takes matrices whose rows do not share memory")
         ld = tensor.stride(0) if tensor.dim() == 2 and tensor.shape[0] > 1 else 0
         return cls(tensor.data_ptr(), tensor.numel() * tensor.element_size(), ld, tensor)
 

@@ -168,6 +168,17 @@ def test_views_of_tensors():
             DeviceView.of(bad)
 
 
+def test_views_of_broadcast_tensors():
+    """Rows that share memory are fewer bytes than a layer would read or write."""
+    torch = pytest.importorskip("torch")
+    from tcbnn_amd.device import DeviceView
+    row = torch.zeros(8)
+    for bad in (row.expand(1000, 8), row[:1].expand(4, 1), torch.zeros((40,)).as_strided((5, 8), (4, 1)), row[:1].expand(8), torch.zeros(())):
+        with pytest.raises(_lib().TcbnnError):
+            DeviceView.of(bad)
+    assert DeviceView.of(row.expand(1, 8)).nbytes == 32 and DeviceView.of(torch.zeros((0, 8))).nbytes == 0
+
+
 def test_encode_rounds_to_nearest_even():
     from tcbnn_amd import head
     torch = pytest.importorskip("torch")
