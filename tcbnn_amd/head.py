@@ -39,6 +39,9 @@ def storage(dtype):
     return {"f32": np.float32, "bf16": np.uint16, "f16": np.float16}[dtype]
 
 
+ITEMSIZE = {"f32": 4, "bf16": 2, "f16": 2, "i32": 4}
+
+
 def _ptr(buf):
     return None if buf is None else buf.ptr
 
@@ -59,9 +62,6 @@ class _HeadLayer:
     def _not_initialized(self, handle):
         raise _lib.TcbnnError("Error: %s: not initialized" % self.name)
 
-    def _itemsize(self):
-        return 4 if self.dtype == "f32" else 2
-
     def _buffer(self, nbytes):
         buf = DeviceBuffer(nbytes)
         self._owned.append(buf)
@@ -75,9 +75,14 @@ class _HeadLayer:
         self._owned.append(buf)
         return buf
 
-    def _sized(self, buf, what, count, itemsize):
-        if buf is not None and buf.nbytes < count * itemsize:
-            raise _lib.TcbnnError("Error: %s: %s holds %d bytes, %d needed" % (self.name, what, buf.nbytes, count * itemsize))
+    def _sized(self, buf, what, count, dtype):
+        """`buf`, which holds `count` elements of `dtype` (a buffer that does not say its type is taken at its size)."""
+        if buf is None:
+            return buf
+        if getattr(buf, "dtype", None) not in (None, dtype):
+            raise _lib.TcbnnError("Error: %s: %s is %s, not %s" % (self.name, what, buf.dtype, dtype))
+        if buf.nbytes < count * ITEMSIZE[dtype]:
+            raise _lib.TcbnnError("Error: %s: %s holds %d bytes, %d needed" % (self.name, what, buf.nbytes, count * ITEMSIZE[dtype]))
         return buf
 
     def _required(self, buf, what):
@@ -124,15 +129,15 @@ class LinearLayerParam(_HeadLayer):
     def initialize(self, weight, bias, input_gpu, residual_gpu=None, output_gpu=None, preact_gpu=None, save_preact=False):
         """save_preact: keep the values before the activation, which backward() of a layer with one needs, in a buffer of
         the layer's own (or give `preact_gpu`)."""
-        m, k, n, size = self.rows, self.in_features, self.out_features, self._itemsize()
-        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", m * k, size)
-        self.weight_gpu = self._sized(self._parameter(self._required(weight, "weight"), self.dtype, (n, k)), "weight", n * k, size)
-        self.bias_gpu = self._sized(self._parameter(bias, "f32", (n,)), "bias", n, 4)
-        self.residual_gpu = self._sized(residual_gpu, "residual", m * n, size)
-        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * size), "output", m * n, size)
+        m, k, n, dt = self.rows, self.in_features, self.out_features, self.dtype
+        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", m * k, dt)
+        self.weight_gpu = self._sized(self._parameter(self._required(weight, "weight"), self.dtype, (n, k)), "weight", n * k, dt)
+        self.bias_gpu = self._sized(self._parameter(bias, "f32", (n,)), "bias", n, "f32")
+        self.residual_gpu = self._sized(residual_gpu, "residual", m * n, dt)
+        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * ITEMSIZE[dt]), "output", m * n, dt)
         if preact_gpu is None and save_preact:
-            preact_gpu = self._buffer(m * n * size)
-        self.preact_gpu = self._sized(preact_gpu, "preact", m * n, size)
+            preact_gpu = self._buffer(m * n * ITEMSIZE[dt])
+        self.preact_gpu = self._sized(preact_gpu, "preact", m * n, dt)
         nbytes = lib.tcbnn_linear_workspace_bytes(m, k, n, _lib.DTYPES[self.dtype])
         ws = self._buffer(nbytes) if nbytes else None
         self._desc = _lib.LinearDesc(
@@ -144,13 +149,13 @@ class LinearLayerParam(_HeadLayer):
 
     def initialize_backward(self, grad_output_gpu, grad_input_gpu=None, grad_weight_gpu=None, grad_bias_gpu=None):
         """After initialize().  Gradients are written where a buffer is given."""
-        m, k, n, size = self.rows, self.in_features, self.out_features, self._itemsize()
+        m, k, n, dt = self.rows, self.in_features, self.out_features, self.dtype
         if self.activation != "none":
             self._required(self.preact_gpu, "preact")
-        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", m * n, size)
-        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", m * k, size)
-        self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", n * k, size)
-        self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", n, 4)
+        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", m * n, dt)
+        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", m * k, dt)
+        self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", n * k, dt)
+        self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", n, "f32")
         nbytes = lib.tcbnn_linear_grad_workspace_bytes(m, k, n, _lib.DTYPES[self.dtype])
         ws = self._buffer(nbytes) if nbytes else None
         self._grad_desc = _lib.LinearGradDesc(
@@ -177,13 +182,13 @@ class LayerNormLayerParam(_HeadLayer):
         self.rows, self.features, self.eps = rows, features, eps
 
     def initialize(self, gamma, beta, input_gpu, output_gpu=None, mean_gpu=None, rstd_gpu=None):
-        m, n, size = self.rows, self.features, self._itemsize()
-        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", m * n, size)
-        self.gamma_gpu = self._sized(self._parameter(gamma, "f32", (n,)), "gamma", n, 4)
-        self.beta_gpu = self._sized(self._parameter(beta, "f32", (n,)), "beta", n, 4)
-        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * size), "output", m * n, size)
-        self.mean_gpu = self._sized(mean_gpu if mean_gpu is not None else self._buffer(4 * m), "mean", m, 4)
-        self.rstd_gpu = self._sized(rstd_gpu if rstd_gpu is not None else self._buffer(4 * m), "rstd", m, 4)
+        m, n, dt = self.rows, self.features, self.dtype
+        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", m * n, dt)
+        self.gamma_gpu = self._sized(self._parameter(gamma, "f32", (n,)), "gamma", n, "f32")
+        self.beta_gpu = self._sized(self._parameter(beta, "f32", (n,)), "beta", n, "f32")
+        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * ITEMSIZE[dt]), "output", m * n, dt)
+        self.mean_gpu = self._sized(mean_gpu if mean_gpu is not None else self._buffer(4 * m), "mean", m, "f32")
+        self.rstd_gpu = self._sized(rstd_gpu if rstd_gpu is not None else self._buffer(4 * m), "rstd", m, "f32")
         self._desc = _lib.LayerNormDesc(
             self.input_gpu.ptr, _ptr(self.gamma_gpu), _ptr(self.beta_gpu), self.output_gpu.ptr, self.mean_gpu.ptr, self.rstd_gpu.ptr,
             m, n, _lib.DTYPES[self.dtype], self.eps, _ld(self.input_gpu), _ld(self.output_gpu))
@@ -192,11 +197,11 @@ class LayerNormLayerParam(_HeadLayer):
 
     def initialize_backward(self, grad_output_gpu, grad_input_gpu=None, grad_gamma_gpu=None, grad_beta_gpu=None):
         """After initialize().  Gradients are written where a buffer is given; mean and rstd are those of forward()."""
-        m, n, size = self.rows, self.features, self._itemsize()
-        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", m * n, size)
-        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", m * n, size)
-        self.grad_gamma_gpu = self._sized(grad_gamma_gpu, "grad_gamma", n, 4)
-        self.grad_beta_gpu = self._sized(grad_beta_gpu, "grad_beta", n, 4)
+        m, n, dt = self.rows, self.features, self.dtype
+        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", m * n, dt)
+        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", m * n, dt)
+        self.grad_gamma_gpu = self._sized(grad_gamma_gpu, "grad_gamma", n, "f32")
+        self.grad_beta_gpu = self._sized(grad_beta_gpu, "grad_beta", n, "f32")
         nbytes = lib.tcbnn_layernorm_grad_workspace_bytes(m, n)
         ws = self._buffer(nbytes) if nbytes else None
         self._grad_desc = _lib.LayerNormGradDesc(
@@ -225,18 +230,18 @@ class LogProbsLayerParam(_HeadLayer):
                    top_index_gpu=None, top_logprob_gpu=None):
         """Without `targets_gpu` (int32, -1: none) no log probabilities and ranks of given classes are computed."""
         m, n, k = self.rows, self.classes, self.top
-        self.logits_gpu = self._sized(self._required(logits_gpu, "logits"), "logits", m * n, self._itemsize())
-        self.targets_gpu = self._sized(targets_gpu, "targets", m, 4)
+        self.logits_gpu = self._sized(self._required(logits_gpu, "logits"), "logits", m * n, self.dtype)
+        self.targets_gpu = self._sized(targets_gpu, "targets", m, "i32")
 
-        def out(buf, what, count, wanted=True):
-            return self._sized(buf if buf is not None or not wanted else self._buffer(4 * count), what, count, 4)
+        def out(buf, what, count, wanted=True, dtype="f32"):
+            return self._sized(buf if buf is not None or not wanted else self._buffer(4 * count), what, count, dtype)
 
         given = targets_gpu is not None
         self.logprob_gpu = out(logprob_gpu, "logprob", m, given)
         self.entropy_gpu = out(entropy_gpu, "entropy", m)
         self.logsumexp_gpu = out(logsumexp_gpu, "logsumexp", m)
-        self.rank_gpu = out(rank_gpu, "rank", m, given)
-        self.top_index_gpu = out(top_index_gpu, "top_index", m * k, k > 0)
+        self.rank_gpu = out(rank_gpu, "rank", m, given, "i32")
+        self.top_index_gpu = out(top_index_gpu, "top_index", m * k, k > 0, "i32")
         self.top_logprob_gpu = out(top_logprob_gpu, "top_logprob", m * k, k > 0)
         nbytes = lib.tcbnn_logprobs_workspace_bytes(m, n, k, _lib.DTYPES[self.dtype])
         ws = self._buffer(nbytes) if nbytes else None
@@ -252,9 +257,9 @@ class LogProbsLayerParam(_HeadLayer):
         m, n = self.rows, self.classes
         if grad_logprob_gpu is not None:
             self._required(self.targets_gpu, "targets")
-        self.grad_logprob_gpu = self._sized(grad_logprob_gpu, "grad_logprob", m, 4)
-        self.grad_entropy_gpu = self._sized(grad_entropy_gpu, "grad_entropy", m, 4)
-        self.grad_logits_gpu = self._sized(self._required(grad_logits_gpu, "grad_logits"), "grad_logits", m * n, self._itemsize())
+        self.grad_logprob_gpu = self._sized(grad_logprob_gpu, "grad_logprob", m, "f32")
+        self.grad_entropy_gpu = self._sized(grad_entropy_gpu, "grad_entropy", m, "f32")
+        self.grad_logits_gpu = self._sized(self._required(grad_logits_gpu, "grad_logits"), "grad_logits", m * n, self.dtype)
         self._grad_desc = _lib.LogProbsGradDesc(
             self.logits_gpu.ptr, _ptr(self.targets_gpu), self.logsumexp_gpu.ptr, self.entropy_gpu.ptr, _ptr(grad_logprob_gpu),
             _ptr(grad_entropy_gpu), grad_logits_gpu.ptr, m, n, _lib.DTYPES[self.dtype], _ld(self.logits_gpu), _ld(grad_logits_gpu))

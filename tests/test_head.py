@@ -179,6 +179,40 @@ def test_views_of_broadcast_tensors():
     assert DeviceView.of(row.expand(1, 8)).nbytes == 32 and DeviceView.of(torch.zeros((0, 8))).nbytes == 0
 
 
+def test_layers_refuse_other_element_types():
+    """A view of a tensor knows its type: enough bytes of another one are not what a layer reads."""
+    torch = pytest.importorskip("torch")
+    from tcbnn_amd import head
+    from tcbnn_amd.device import DeviceView
+    E = _lib().TcbnnError
+
+    def view(dtype, *shape):
+        v = DeviceView.of(torch.zeros(shape, dtype=dtype))
+        return DeviceView(P, v.nbytes, v.ld, dtype=v.dtype)
+
+    f32, bf16, raw = view(torch.float32, 8, 8), view(torch.bfloat16, 8, 8), DeviceView(P, 256)
+    assert (f32.dtype, bf16.dtype, view(torch.float16, 1).dtype, view(torch.int32, 1).dtype, raw.dtype) == ("f32", "bf16", "f16", "i32", None)
+    with pytest.raises(E, match="input.*f32.*bf16"):
+        head.LinearLayerParam("l", 8, 8, 8, "bf16").initialize(bf16, None, f32, output_gpu=bf16)
+    with pytest.raises(E, match="weight"):
+        head.LinearLayerParam("l", 8, 8, 8, "f32").initialize(view(torch.float64, 8, 8), None, f32, output_gpu=f32)
+    with pytest.raises(E, match="bias"):
+        head.LinearLayerParam("l", 8, 8, 8, "bf16").initialize(bf16, view(torch.bfloat16, 16), bf16, output_gpu=bf16)
+    with pytest.raises(E, match="gamma"):
+        head.LayerNormLayerParam("n", 8, 8, "f16").initialize(view(torch.float16, 16), None, view(torch.float16, 8, 8), output_gpu=raw)
+    lp = head.LogProbsLayerParam("p", 8, 8)
+    lp._buffer = lambda nbytes: DeviceView(P, nbytes)
+    with pytest.raises(E, match="targets.*int64.*i32"):
+        lp.initialize(f32, view(torch.int64, 8))
+    with pytest.raises(E, match="rank"):
+        lp.initialize(f32, view(torch.int32, 8), rank_gpu=view(torch.float32, 8))
+    lp.initialize(f32, view(torch.int32, 8), rank_gpu=view(torch.int32, 8), entropy_gpu=view(torch.float32, 8))
+    with pytest.raises(E, match="grad_logits"):
+        lp.initialize_backward(raw, None, view(torch.float64, 8, 8))
+    linear = head.LinearLayerParam("l", 8, 8, 8, "f32")  # (what does not say its type is taken at its size, as before)
+    linear.initialize(raw, raw, raw, output_gpu=f32)
+
+
 def test_encode_rounds_to_nearest_even():
     from tcbnn_amd import head
     torch = pytest.importorskip("torch")
