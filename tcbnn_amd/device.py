@@ -62,13 +62,13 @@ class DeviceBuffer:
 class DeviceView:
     """Device memory that something else owns, as a layer's input or output: `nbytes` at `ptr`, rows of a matrix `ld`
     elements apart (0: without gaps).  `dtype` is the elements' type ("f32", "bf16", "f16", "i32", or the name of another; None:
-    not known, whatever a layer reads), which layers compare with theirs.  `owner` is kept alive with the view; free() leaves
-    the memory alone."""
+    not known, whatever a layer reads), which layers compare with theirs.  `on_host`: pageable host memory, which they refuse.  `owner` is
+    kept alive with the view; free() leaves the memory alone."""
 
     _TYPES = {"float32": "f32", "bfloat16": "bf16", "float16": "f16", "int32": "i32"}
 
-    def __init__(self, ptr, nbytes, ld=0, owner=None, dtype=None):
-        self.ptr, self.nbytes, self.ld, self.owner, self.dtype = ptr, int(nbytes), int(ld), owner, dtype
+    def __init__(self, ptr, nbytes, ld=0, owner=None, dtype=None, on_host=False):
+        self.ptr, self.nbytes, self.ld, self.owner, self.dtype, self.on_host = ptr, int(nbytes), int(ld), owner, dtype, on_host
 
     @classmethod
     def of(cls, tensor):
@@ -80,7 +80,8 @@ class DeviceView:
             raise _lib.TcbnnError("a layer takes matrices whose rows do not share memory")
         ld = tensor.stride(0) if tensor.dim() == 2 and tensor.shape[0] > 1 else 0
         name = str(tensor.dtype).rpartition(".")[2]
-        return cls(tensor.data_ptr(), tensor.numel() * tensor.element_size(), ld, tensor, cls._TYPES.get(name, name))
+        return cls(tensor.data_ptr(), tensor.numel() * tensor.element_size(), ld, tensor, cls._TYPES.get(name, name),
+                   not tensor.is_cuda and not tensor.is_pinned())
 
     to_numpy = DeviceBuffer.to_numpy
 

@@ -79,6 +79,8 @@ class _HeadLayer:
         """`buf`, which holds `count` elements of `dtype` (a buffer that does not say its type is taken at its size)."""
         if buf is None:
             return buf
+        if getattr(buf, "on_host", False):
+            raise _lib.TcbnnError("Error: %s: %s lies in host memory" % (self.name, what))
         if getattr(buf, "dtype", None) not in (None, dtype):
             raise _lib.TcbnnError("Error: %s: %s is %s, not %s" % (self.name, what, buf.dtype, dtype))
         if buf.nbytes < count * ITEMSIZE[dtype]:

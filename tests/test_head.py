@@ -213,6 +213,22 @@ def test_layers_refuse_other_element_types():
     linear.initialize(raw, raw, raw, output_gpu=f32)
 
 
+def test_layers_refuse_host_tensors():
+    """A kernel does not follow a pointer into pageable host memory."""
+    torch = pytest.importorskip("torch")
+    from tcbnn_amd import head
+    from tcbnn_amd.device import DeviceView
+    E = _lib().TcbnnError
+    buf, host = DeviceView(P, 256), DeviceView.of(torch.zeros(8, 8))
+    assert host.on_host and not buf.on_host
+    with pytest.raises(E, match="input.*host"):
+        head.LinearLayerParam("l", 8, 8, 8).initialize(buf, None, host, output_gpu=buf)
+    with pytest.raises(E, match="bias.*host"):
+        head.LinearLayerParam("l", 8, 8, 8).initialize(buf, DeviceView.of(torch.zeros(8)), buf, output_gpu=buf)
+    with pytest.raises(E, match="grad_output.*host"):
+        head.LinearLayerParam("l", 8, 8, 8).initialize(buf, None, buf, output_gpu=buf).initialize_backward(host)
+
+
 def test_encode_rounds_to_nearest_even():
     from tcbnn_amd import head
     torch = pytest.importorskip("torch")
