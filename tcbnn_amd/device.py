@@ -61,14 +61,15 @@ class DeviceBuffer:
 
 class DeviceView:
     """Device memory that something else owns, as a layer's input or output: `nbytes` at `ptr`, rows of a matrix `ld`
-    elements apart (0: without gaps).  `dtype` is the elements' type ("f32", "bf16", "f16", "i32", or the name of another; None:
-    not known, whatever a layer reads), which layers compare with theirs.  `on_host`: pageable host memory, which they refuse.  `owner` is
-    kept alive with the view; free() leaves the memory alone."""
+    elements apart (0: without gaps).  Layers refuse what they know not to be theirs: `dtype` is the elements' type ("f32",
+    "bf16", "f16", "i32", or the name of another), `shape` how many rows there are and how long (None: not known, each), `on_host`
+    says that it is pageable host memory.  `owner` is kept alive with the view; free() leaves the memory alone."""
 
     _TYPES = {"float32": "f32", "bfloat16": "bf16", "float16": "f16", "int32": "i32"}
 
-    def __init__(self, ptr, nbytes, ld=0, owner=None, dtype=None, on_host=False):
-        self.ptr, self.nbytes, self.ld, self.owner, self.dtype, self.on_host = ptr, int(nbytes), int(ld), owner, dtype, on_host
+    def __init__(self, ptr, nbytes, ld=0, owner=None, dtype=None, on_host=False, shape=None):
+        self.ptr, self.nbytes, self.ld, self.owner = ptr, int(nbytes), int(ld), owner
+        self.dtype, self.on_host, self.shape = dtype, on_host, shape
 
     @classmethod
     def of(cls, tensor):
@@ -81,7 +82,7 @@ class DeviceView:
         ld = tensor.stride(0) if tensor.dim() == 2 and tensor.shape[0] > 1 else 0
         name = str(tensor.dtype).rpartition(".")[2]
         return cls(tensor.data_ptr(), tensor.numel() * tensor.element_size(), ld, tensor, cls._TYPES.get(name, name),
-                   not tensor.is_cuda and not tensor.is_pinned())
+                   not tensor.is_cuda and not tensor.is_pinned(), tuple(tensor.shape))
 
     to_numpy = DeviceBuffer.to_numpy
 

@@ -75,16 +75,27 @@ class _HeadLayer:
         self._owned.append(buf)
         return buf
 
-    def _sized(self, buf, what, count, dtype):
-        """`buf`, which holds `count` elements of `dtype` (a buffer that does not say its type is taken at its size)."""
+    def _sized(self, buf, what, shape, dtype, gaps=True):
+        """`buf`, which holds a matrix or a vector of `shape` in `dtype` (what does not say its type is taken at its size).
+        `gaps`: whether rows may be further apart than they are long."""
         if buf is None:
             return buf
         if getattr(buf, "on_host", False):
             raise _lib.TcbnnError("Error: %s: %s lies in host memory" % (self.name, what))
         if getattr(buf, "dtype", None) not in (None, dtype):
             raise _lib.TcbnnError("Error: %s: %s is %s, not %s" % (self.name, what, buf.dtype, dtype))
-        if buf.nbytes < count * ITEMSIZE[dtype]:
-            raise _lib.TcbnnError("Error: %s: %s holds %d bytes, %d needed" % (self.name, what, buf.nbytes, count * ITEMSIZE[dtype]))
+        rows, cols = shape if len(shape) == 2 else (1, shape[0])
+        if buf.nbytes < rows * cols * ITEMSIZE[dtype]:
+            raise _lib.TcbnnError("Error: %s: %s holds %d bytes, %d needed" % (self.name, what, buf.nbytes, rows * cols * ITEMSIZE[dtype]))
+        ld, there = _ld(buf), getattr(buf, "shape", None)
+        if rows * cols == 0:
+            pass
+        elif ld and (len(shape) == 1 or not gaps):
+            if ld != (there[1] if there else cols):
+                raise _lib.TcbnnError("Error: %s: %s has gaps between rows" % (self.name, what))
+        elif ld and (there[0] < rows or there[1] < cols if there else
+                     ((rows - 1) * ld + cols) * ITEMSIZE[dtype] > buf.nbytes):
+            raise _lib.TcbnnError("Error: %s: %s is not %d rows of %d, %d apart" % (self.name, what, rows, cols, ld))
         return buf
 
     def _required(self, buf, what):
@@ -132,14 +143,14 @@ class LinearLayerParam(_HeadLayer):
         """save_preact: keep the values before the activation, which backward() of a layer with one needs, in a buffer of
         the layer's own (or give `preact_gpu`)."""
         m, k, n, dt = self.rows, self.in_features, self.out_features, self.dtype
-        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", m * k, dt)
-        self.weight_gpu = self._sized(self._parameter(self._required(weight, "weight"), self.dtype, (n, k)), "weight", n * k, dt)
-        self.bias_gpu = self._sized(self._parameter(bias, "f32", (n,)), "bias", n, "f32")
-        self.residual_gpu = self._sized(residual_gpu, "residual", m * n, dt)
-        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * ITEMSIZE[dt]), "output", m * n, dt)
+        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", (m, k), dt)
+        self.weight_gpu = self._sized(self._parameter(self._required(weight, "weight"), self.dtype, (n, k)), "weight", (n, k), dt)
+        self.bias_gpu = self._sized(self._parameter(bias, "f32", (n,)), "bias", (n,), "f32")
+        self.residual_gpu = self._sized(residual_gpu, "residual", (m, n), dt)
+        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * ITEMSIZE[dt]), "output", (m, n), dt)
         if preact_gpu is None and save_preact:
             preact_gpu = self._buffer(m * n * ITEMSIZE[dt])
-        self.preact_gpu = self._sized(preact_gpu, "preact", m * n, dt)
+        self.preact_gpu = self._sized(preact_gpu, "preact", (m, n), dt)
         nbytes = lib.tcbnn_linear_workspace_bytes(m, k, n, _lib.DTYPES[self.dtype])
         ws = self._buffer(nbytes) if nbytes else None
         self._desc = _lib.LinearDesc(
@@ -154,10 +165,10 @@ class LinearLayerParam(_HeadLayer):
         m, k, n, dt = self.rows, self.in_features, self.out_features, self.dtype
         if self.activation != "none":
             self._required(self.preact_gpu, "preact")
-        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", m * n, dt)
-        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", m * k, dt)
-        self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", n * k, dt)
-        self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", n, "f32")
+        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", (m, n), dt)
+        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", (m, k), dt)
+        self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", (n, k), dt)
+        self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", (n,), "f32")
         nbytes = lib.tcbnn_linear_grad_workspace_bytes(m, k, n, _lib.DTYPES[self.dtype])
         ws = self._buffer(nbytes) if nbytes else None
         self._grad_desc = _lib.LinearGradDesc(
@@ -185,12 +196,12 @@ class LayerNormLayerParam(_HeadLayer):
 
     def initialize(self, gamma, beta, input_gpu, output_gpu=None, mean_gpu=None, rstd_gpu=None):
         m, n, dt = self.rows, self.features, self.dtype
-        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", m * n, dt)
-        self.gamma_gpu = self._sized(self._parameter(gamma, "f32", (n,)), "gamma", n, "f32")
-        self.beta_gpu = self._sized(self._parameter(beta, "f32", (n,)), "beta", n, "f32")
-        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * ITEMSIZE[dt]), "output", m * n, dt)
-        self.mean_gpu = self._sized(mean_gpu if mean_gpu is not None else self._buffer(4 * m), "mean", m, "f32")
-        self.rstd_gpu = self._sized(rstd_gpu if rstd_gpu is not None else self._buffer(4 * m), "rstd", m, "f32")
+        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", (m, n), dt)
+        self.gamma_gpu = self._sized(self._parameter(gamma, "f32", (n,)), "gamma", (n,), "f32")
+        self.beta_gpu = self._sized(self._parameter(beta, "f32", (n,)), "beta", (n,), "f32")
+        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * ITEMSIZE[dt]), "output", (m, n), dt)
+        self.mean_gpu = self._sized(mean_gpu if mean_gpu is not None else self._buffer(4 * m), "mean", (m,), "f32")
+        self.rstd_gpu = self._sized(rstd_gpu if rstd_gpu is not None else self._buffer(4 * m), "rstd", (m,), "f32")
         self._desc = _lib.LayerNormDesc(
             self.input_gpu.ptr, _ptr(self.gamma_gpu), _ptr(self.beta_gpu), self.output_gpu.ptr, self.mean_gpu.ptr, self.rstd_gpu.ptr,
             m, n, _lib.DTYPES[self.dtype], self.eps, _ld(self.input_gpu), _ld(self.output_gpu))
@@ -200,10 +211,10 @@ class LayerNormLayerParam(_HeadLayer):
     def initialize_backward(self, grad_output_gpu, grad_input_gpu=None, grad_gamma_gpu=None, grad_beta_gpu=None):
         """After initialize().  Gradients are written where a buffer is given; mean and rstd are those of forward()."""
         m, n, dt = self.rows, self.features, self.dtype
-        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", m * n, dt)
-        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", m * n, dt)
-        self.grad_gamma_gpu = self._sized(grad_gamma_gpu, "grad_gamma", n, "f32")
-        self.grad_beta_gpu = self._sized(grad_beta_gpu, "grad_beta", n, "f32")
+        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", (m, n), dt)
+        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", (m, n), dt)
+        self.grad_gamma_gpu = self._sized(grad_gamma_gpu, "grad_gamma", (n,), "f32")
+        self.grad_beta_gpu = self._sized(grad_beta_gpu, "grad_beta", (n,), "f32")
         nbytes = lib.tcbnn_layernorm_grad_workspace_bytes(m, n)
         ws = self._buffer(nbytes) if nbytes else None
         self._grad_desc = _lib.LayerNormGradDesc(
@@ -232,19 +243,19 @@ class LogProbsLayerParam(_HeadLayer):
                    top_index_gpu=None, top_logprob_gpu=None):
         """Without `targets_gpu` (int32, -1: none) no log probabilities and ranks of given classes are computed."""
         m, n, k = self.rows, self.classes, self.top
-        self.logits_gpu = self._sized(self._required(logits_gpu, "logits"), "logits", m * n, self.dtype)
-        self.targets_gpu = self._sized(targets_gpu, "targets", m, "i32")
+        self.logits_gpu = self._sized(self._required(logits_gpu, "logits"), "logits", (m, n), self.dtype)
+        self.targets_gpu = self._sized(targets_gpu, "targets", (m,), "i32")
 
-        def out(buf, what, count, wanted=True, dtype="f32"):
-            return self._sized(buf if buf is not None or not wanted else self._buffer(4 * count), what, count, dtype)
+        def out(buf, what, shape, wanted=True, dtype="f32"):
+            return self._sized(buf if buf is not None or not wanted else self._buffer(4 * int(np.prod(shape))), what, shape, dtype, gaps=False)
 
         given = targets_gpu is not None
-        self.logprob_gpu = out(logprob_gpu, "logprob", m, given)
-        self.entropy_gpu = out(entropy_gpu, "entropy", m)
-        self.logsumexp_gpu = out(logsumexp_gpu, "logsumexp", m)
-        self.rank_gpu = out(rank_gpu, "rank", m, given, "i32")
-        self.top_index_gpu = out(top_index_gpu, "top_index", m * k, k > 0, "i32")
-        self.top_logprob_gpu = out(top_logprob_gpu, "top_logprob", m * k, k > 0)
+        self.logprob_gpu = out(logprob_gpu, "logprob", (m,), given)
+        self.entropy_gpu = out(entropy_gpu, "entropy", (m,))
+        self.logsumexp_gpu = out(logsumexp_gpu, "logsumexp", (m,))
+        self.rank_gpu = out(rank_gpu, "rank", (m,), given, "i32")
+        self.top_index_gpu = out(top_index_gpu, "top_index", (m, k), k > 0, "i32")
+        self.top_logprob_gpu = out(top_logprob_gpu, "top_logprob", (m, k), k > 0)
         nbytes = lib.tcbnn_logprobs_workspace_bytes(m, n, k, _lib.DTYPES[self.dtype])
         ws = self._buffer(nbytes) if nbytes else None
         self._desc = _lib.LogProbsDesc(
@@ -259,9 +270,9 @@ class LogProbsLayerParam(_HeadLayer):
         m, n = self.rows, self.classes
         if grad_logprob_gpu is not None:
             self._required(self.targets_gpu, "targets")
-        self.grad_logprob_gpu = self._sized(grad_logprob_gpu, "grad_logprob", m, "f32")
-        self.grad_entropy_gpu = self._sized(grad_entropy_gpu, "grad_entropy", m, "f32")
-        self.grad_logits_gpu = self._sized(self._required(grad_logits_gpu, "grad_logits"), "grad_logits", m * n, self.dtype)
+        self.grad_logprob_gpu = self._sized(grad_logprob_gpu, "grad_logprob", (m,), "f32")
+        self.grad_entropy_gpu = self._sized(grad_entropy_gpu, "grad_entropy", (m,), "f32")
+        self.grad_logits_gpu = self._sized(self._required(grad_logits_gpu, "grad_logits"), "grad_logits", (m, n), self.dtype)
         self._grad_desc = _lib.LogProbsGradDesc(
             self.logits_gpu.ptr, _ptr(self.targets_gpu), self.logsumexp_gpu.ptr, self.entropy_gpu.ptr, _ptr(grad_logprob_gpu),
             _ptr(grad_entropy_gpu), grad_logits_gpu.ptr, m, n, _lib.DTYPES[self.dtype], _ld(self.logits_gpu), _ld(grad_logits_gpu))

@@ -229,6 +229,46 @@ def test_layers_refuse_host_tensors():
         head.LinearLayerParam("l", 8, 8, 8).initialize(buf, None, buf, output_gpu=buf).initialize_backward(host)
 
 
+def test_layers_refuse_rows_that_are_not_there():
+    """Rows some elements apart: as many, as long as a layer has, in memory that holds them; vectors without gaps."""
+    torch = pytest.importorskip("torch")
+    from tcbnn_amd import head
+    from tcbnn_amd.device import DeviceView
+    E = _lib().TcbnnError
+
+    def view(rows, cols, wide):
+        v = DeviceView.of(torch.zeros((rows, wide))[:, :cols])
+        return DeviceView(P, v.nbytes, v.ld, shape=v.shape)
+
+    buf, raw = DeviceView(P, 4096), DeviceView(P, 4 * (7 * 12 + 8), 12)  # (raw: eight rows of eight, twelve apart, and no byte more)
+    linear = lambda x, w=buf, b=None, y=buf: head.LinearLayerParam("l", 8, 8, 8).initialize(w, b, x, output_gpu=y)  # noqa: E731
+    assert view(8, 8, 12).shape == (8, 8) and raw.shape is None
+    for good in (view(8, 8, 12), view(9, 9, 12), view(8, 8, 8), view(1, 64, 64), raw):
+        linear(good)
+        linear(buf, w=good, y=good)
+    with pytest.raises(E, match="input.*rows"):
+        linear(view(2, 32, 40))  # 64 values, but eight rows of 40 would go past them
+    with pytest.raises(E, match="input.*rows"):
+        linear(view(4, 16, 16))
+    with pytest.raises(E, match="input.*rows"):
+        linear(view(16, 4, 12))  # eight values of its rows are there, four of them in the gap
+    with pytest.raises(E, match="weight.*rows"):
+        linear(buf, w=DeviceView(P, 4 * (7 * 12 + 7), 12))
+    with pytest.raises(E, match="output.*rows"):
+        linear(buf, y=view(4, 16, 24))
+    with pytest.raises(E, match="bias.*gaps"):
+        linear(buf, b=view(8, 1, 12))  # a column
+    linear(buf, b=view(8, 1, 1))
+    linear(buf, b=view(2, 4, 4))
+    with pytest.raises(E, match="gamma.*gaps"):
+        head.LayerNormLayerParam("n", 4, 8).initialize(DeviceView(P, 64, 2), None, buf, output_gpu=buf, mean_gpu=buf, rstd_gpu=buf)
+    outs = dict(logprob_gpu=buf, entropy_gpu=buf, logsumexp_gpu=buf, rank_gpu=buf)
+    best = head.LogProbsLayerParam("p", 8, 64, top=4)
+    best.initialize(buf, buf, **outs, top_index_gpu=view(8, 4, 4), top_logprob_gpu=view(1, 32, 32))
+    with pytest.raises(E, match="top_index.*gaps"):
+        best.initialize(buf, buf, **outs, top_index_gpu=view(8, 4, 6), top_logprob_gpu=buf)
+
+
 def test_encode_rounds_to_nearest_even():
     from tcbnn_amd import head
     torch = pytest.importorskip("torch")
