@@ -103,6 +103,11 @@ class _HeadLayer:
             raise _lib.TcbnnError("Error: NULL pointer (%s: %s)" % (self.name, what))
         return buf
 
+    def _download(self, buf, rows, cols):
+        if _ld(buf) not in (0, cols):
+            raise _lib.TcbnnError("Error: %s: output has gaps between rows" % self.name)
+        return decode(buf.to_numpy(storage(self.dtype), (rows, cols)), self.dtype)
+
     @staticmethod
     def _call(entry, desc):
         """A call of the entry point with this descriptor, on a stream's handle (what does not change is made once: a small
@@ -184,7 +189,7 @@ class LinearLayerParam(_HeadLayer):
 
     def download_output(self):
         """fp32 [rows][out_features] of a buffer without gaps between rows."""
-        return decode(self.output_gpu.to_numpy(storage(self.dtype), (self.rows, self.out_features)), self.dtype)
+        return self._download(self.output_gpu, self.rows, self.out_features)
 
 
 class LayerNormLayerParam(_HeadLayer):
@@ -229,7 +234,7 @@ class LayerNormLayerParam(_HeadLayer):
 
     def download_output(self):
         """fp32 [rows][features] of a buffer without gaps between rows."""
-        return decode(self.output_gpu.to_numpy(storage(self.dtype), (self.rows, self.features)), self.dtype)
+        return self._download(self.output_gpu, self.rows, self.features)
 
 
 class LogProbsLayerParam(_HeadLayer):

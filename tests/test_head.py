@@ -269,6 +269,28 @@ def test_layers_refuse_rows_that_are_not_there():
         best.initialize(buf, buf, **outs, top_index_gpu=view(8, 4, 6), top_logprob_gpu=buf)
 
 
+def test_downloads_refuse_gaps():
+    """download_output() copies one piece of memory: not where its rows have others between them."""
+    from tcbnn_amd import head
+    from tcbnn_amd.device import DeviceView
+    copied = []
+
+    class View(DeviceView):
+        def to_numpy(self, dtype, shape):
+            copied.append(shape)
+            return np.zeros(shape, dtype)
+
+    buf = View(P, 4096)
+    linear = lambda y: head.LinearLayerParam("l", 8, 8, 8).initialize(buf, None, buf, output_gpu=y)  # noqa: E731
+    norm = lambda y: head.LayerNormLayerParam("n", 8, 8).initialize(None, None, buf, output_gpu=y, mean_gpu=buf, rstd_gpu=buf)  # noqa: E731
+    for layer in (linear, norm):
+        with pytest.raises(_lib().TcbnnError, match="gaps"):
+            layer(View(P, 4096, 12)).download_output()
+        assert not copied
+        for y in (buf, View(P, 4096, 8)):
+            assert layer(y).download_output().shape == (8, 8) and copied.pop() == (8, 8)
+
+
 def test_encode_rounds_to_nearest_even():
     from tcbnn_amd import head
     torch = pytest.importorskip("torch")
