@@ -104,7 +104,7 @@ class _HeadLayer:
         return buf
 
     def _download(self, buf, rows, cols):
-        if _ld(buf) not in (0, cols):
+        if rows > 1 and _ld(buf) not in (0, cols):
             raise _lib.TcbnnError("Error: %s: output has gaps between rows" % self.name)
         return decode(buf.to_numpy(storage(self.dtype), (rows, cols)), self.dtype)
 

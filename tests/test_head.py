@@ -289,6 +289,8 @@ def test_downloads_refuse_gaps():
         assert not copied
         for y in (buf, View(P, 4096, 8)):
             assert layer(y).download_output().shape == (8, 8) and copied.pop() == (8, 8)
+    one = head.LinearLayerParam("l", 1, 8, 8).initialize(buf, None, buf, output_gpu=View(P, 4096, 12))  # (one row has none)
+    assert one.download_output().shape == (1, 8)
 
 
 def test_encode_rounds_to_nearest_even():
