@@ -55,7 +55,11 @@ class _HeadLayer:
         if dtype not in _lib.DTYPES:
             raise _lib.TcbnnError("Error: %s: unknown dtype %r" % (name, dtype))
         self.name, self.dtype = name, dtype
-        self._owned = []
+        self._forget()
+
+    def _forget(self):
+        """As before initialize().  What the layer owned lives on where something else still holds it."""
+        self._owned, self._grad_workspace = [], None
         self._desc = self._grad_desc = None  # kept by the calls below
         self._forward = self._backward = self._not_initialized
 
@@ -66,6 +70,13 @@ class _HeadLayer:
         buf = DeviceBuffer(nbytes)
         self._owned.append(buf)
         return buf
+
+    def _grad_buffer(self, nbytes):
+        """The backward pass' workspace, in the place of an earlier one."""
+        self._backward = self._not_initialized
+        self._owned = [buf for buf in self._owned if buf is not self._grad_workspace]
+        self._grad_workspace = self._buffer(nbytes) if nbytes else None
+        return self._grad_workspace
 
     def _parameter(self, p, dtype, shape):
         """A parameter's device buffer: what the caller holds, or an upload of a host array."""
@@ -130,9 +141,7 @@ class _HeadLayer:
     def release(self):
         for buf in self._owned:
             buf.free()
-        self._owned = []
-        self._desc = self._grad_desc = None
-        self._forward = self._backward = self._not_initialized
+        self._forget()
 
 
 class LinearLayerParam(_HeadLayer):
@@ -147,6 +156,7 @@ class LinearLayerParam(_HeadLayer):
     def initialize(self, weight, bias, input_gpu, residual_gpu=None, output_gpu=None, preact_gpu=None, save_preact=False):
         """save_preact: keep the values before the activation, which backward() of a layer with one needs, in a buffer of
         the layer's own (or give `preact_gpu`)."""
+        self._forget()
         m, k, n, dt = self.rows, self.in_features, self.out_features, self.dtype
         self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", (m, k), dt)
         self.weight_gpu = self._sized(self._parameter(self._required(weight, "weight"), self.dtype, (n, k)), "weight", (n, k), dt)
@@ -175,7 +185,7 @@ class LinearLayerParam(_HeadLayer):
         self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", (n, k), dt)
         self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", (n,), "f32")
         nbytes = lib.tcbnn_linear_grad_workspace_bytes(m, k, n, _lib.DTYPES[self.dtype])
-        ws = self._buffer(nbytes) if nbytes else None
+        ws = self._grad_buffer(nbytes)
         self._grad_desc = _lib.LinearGradDesc(
             self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.preact_gpu), self.grad_output_gpu.ptr, _ptr(grad_input_gpu),
             _ptr(grad_weight_gpu), _ptr(grad_bias_gpu), m, k, n, _lib.DTYPES[self.dtype], _lib.ACTIVATIONS[self.activation],
@@ -200,6 +210,7 @@ class LayerNormLayerParam(_HeadLayer):
         self.rows, self.features, self.eps = rows, features, eps
 
     def initialize(self, gamma, beta, input_gpu, output_gpu=None, mean_gpu=None, rstd_gpu=None):
+        self._forget()
         m, n, dt = self.rows, self.features, self.dtype
         self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", (m, n), dt)
         self.gamma_gpu = self._sized(self._parameter(gamma, "f32", (n,)), "gamma", (n,), "f32")
@@ -221,7 +232,7 @@ class LayerNormLayerParam(_HeadLayer):
         self.grad_gamma_gpu = self._sized(grad_gamma_gpu, "grad_gamma", (n,), "f32")
         self.grad_beta_gpu = self._sized(grad_beta_gpu, "grad_beta", (n,), "f32")
         nbytes = lib.tcbnn_layernorm_grad_workspace_bytes(m, n)
-        ws = self._buffer(nbytes) if nbytes else None
+        ws = self._grad_buffer(nbytes)
         self._grad_desc = _lib.LayerNormGradDesc(
             self.input_gpu.ptr, _ptr(self.gamma_gpu), self.mean_gpu.ptr, self.rstd_gpu.ptr, self.grad_output_gpu.ptr,
             _ptr(grad_input_gpu), _ptr(grad_gamma_gpu), _ptr(grad_beta_gpu), m, n, _lib.DTYPES[self.dtype], _ld(self.input_gpu),
@@ -247,6 +258,7 @@ class LogProbsLayerParam(_HeadLayer):
     def initialize(self, logits_gpu, targets_gpu=None, logprob_gpu=None, entropy_gpu=None, logsumexp_gpu=None, rank_gpu=None,
                    top_index_gpu=None, top_logprob_gpu=None):
         """Without `targets_gpu` (int32, -1: none) no log probabilities and ranks of given classes are computed."""
+        self._forget()
         m, n, k = self.rows, self.classes, self.top
         self.logits_gpu = self._sized(self._required(logits_gpu, "logits"), "logits", (m, n), self.dtype)
         self.targets_gpu = self._sized(targets_gpu, "targets", (m,), "i32")

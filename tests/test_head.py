@@ -293,6 +293,51 @@ def test_downloads_refuse_gaps():
     assert one.download_output().shape == (1, 8)
 
 
+def test_layers_are_initialized_anew():
+    """initialize() once more: no call of the layer still uses the buffers of before, and it keeps none of its own from there."""
+    from tcbnn_amd import head
+    from tcbnn_amd.device import DeviceView
+    E, alive = _lib().TcbnnError, []
+
+    class Own(DeviceView):
+        def __init__(self, nbytes):
+            super().__init__(P, nbytes)
+            alive.append(self)
+
+    def fill(layer):
+        layer._buffer = lambda nbytes: layer._owned.append(Own(nbytes)) or layer._owned[-1]
+        return layer
+
+    def started(layer):
+        args = {"l": (buf, None, buf), "n": (None, None, buf), "p": (buf, buf)}[layer.name]
+        return layer.initialize(*args)
+
+    buf, short = DeviceView(P, 4096), DeviceView(P, 16)
+    layers = [fill(head.LinearLayerParam("l", 8, 8, 8)), fill(head.LayerNormLayerParam("n", 8, 8)), fill(head.LogProbsLayerParam("p", 8, 8))]
+    grads = {"l": (buf, buf, buf, buf), "n": (buf, buf, buf, buf), "p": (buf, buf, buf)}
+    for layer in layers:
+        for _ in range(2):
+            started(layer)
+            with pytest.raises(E, match="not initialized"):
+                layer.backward()
+            own = len(alive)
+            layer.initialize_backward(*grads[layer.name])
+            layer.initialize_backward(*grads[layer.name])
+            assert {id(b) for b in layer._owned} <= {id(b) for b in alive} and len(layer._owned) <= own + 1
+            first = list(alive)
+            alive.clear()
+            started(layer)
+            assert not {id(b) for b in layer._owned} & {id(b) for b in first}
+            alive.clear()
+        bad = {"l": (buf, None, short), "n": (None, None, short), "p": (short, buf)}[layer.name]
+        started(layer).initialize_backward(*grads[layer.name])
+        with pytest.raises(E, match="holds"):
+            layer.initialize(*bad)
+        for call in (layer.forward, layer.backward):
+            with pytest.raises(E, match="not initialized"):
+                call()
+
+
 def test_encode_rounds_to_nearest_even():
     from tcbnn_amd import head
     torch = pytest.importorskip("torch")
