@@ -1042,7 +1042,7 @@ void product_name(const ProductParams& p, size_t workspace_bytes, char* buf, siz
     const int hold = access == ANYWHERE && plan.cut != CUT_128 ? 4 : 1;
     const bool keep = hold == 4 && (plan.cut != CUT_64 || long_sums<T>(p, plan));
     snprintf(buf, len, "product_kernel<%s, %s, (Access)%d, %d, %s, false, false>%s", type, shape[access][plan.cut], (int)access, hold, keep ? "true" : "false",
-             plan.splits > 1 && access != ELEMENTS ? " + product_join_kernel" : "");
+             plan.splits > 1 ? " + product_join_kernel" : "");
 }
 
 template <typename T, bool ACROSS_I, bool ACROSS_J>

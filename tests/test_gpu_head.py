@@ -277,6 +277,28 @@ def test_offsets_past_32_bits(gpu, rows, ld):
     x.buf.free()
 
 
+def test_linear_split_sums_of_far_rows(gpu):
+    """A long sum, split among workgroups, over weight rows that are read element by element; the gradients of such a layer."""
+    from tcbnn_amd import head
+    m, k, n = 40, 16390, 24
+    r = rng(m, k, n)
+    w = _Apart((r.standard_normal((n, k)) / np.sqrt(k)).astype(np.float32), "bf16", (1 << 22) + 8)
+    x, dy = ho.Matrix(r.standard_normal((m, k)), "bf16"), ho.Matrix(r.standard_normal((m, n)), "bf16")
+    y, dx, dw = ho.Matrix(None, "bf16", 0, m, n), ho.Matrix(None, "bf16", 0, m, k), ho.Matrix(None, "bf16", 0, n, k)
+    layer = head.LinearLayerParam("linear", m, k, n, "bf16").initialize(w.view, None, x.view, output_gpu=y.view)
+    layer.initialize_backward(dy.view, dx.view, dw.view)
+    assert layer._desc.workspace_bytes > 0
+    layer.forward()
+    layer.backward()
+    ho.sync()
+    for got, a, b in ((y, x.values, w.values.T), (dx, dy.values, w.values), (dw, dy.values.T, x.values)):
+        exact, terms = a @ b, np.abs(a) @ np.abs(b)
+        err = (a.shape[1] + 1) * ho.U32 * terms
+        ho.check(got.get(), exact, err + ho.U["bf16"] * (np.abs(exact) + err) + ho.TINY["bf16"])
+    layer.release()
+    w.buf.free()
+
+
 def test_linear_without_rows(gpu):
     from tcbnn_amd import head
     x, w = ho.Matrix(None, "bf16", 0, 0, 24), ho.Matrix(np.ones((16, 24)), "bf16")

@@ -131,6 +131,17 @@ def test_kernel_names():
     assert lib.tcbnn_linear_kernel_name(None, C.create_string_buffer(8), 8) == ENULL
 
 
+def test_kernel_name_of_a_split_sum_of_far_rows():
+    """Rows too far apart for a tile's 32-bit offsets: a long sum of few tiles is split, and joined, there too."""
+    lib = _lib().lib
+    need = lib.tcbnn_linear_workspace_bytes(64, 16384, 64, 1)
+    buf = C.create_string_buffer(160)
+    for workspace, joined in ((need, True), (0, False)):
+        d = _linear(rows=64, in_features=16384, out_features=64, weight_ld=1 << 24, workspace=P if workspace else 0, workspace_bytes=workspace)[1]
+        assert lib.tcbnn_linear_kernel_name(C.byref(d), buf, 160) == 0
+        assert "(Access)2" in buf.value.decode() and ("product_join_kernel" in buf.value.decode()) == joined
+
+
 def test_layers_refuse():
     from tcbnn_amd import head
     from tcbnn_amd.device import DeviceView
