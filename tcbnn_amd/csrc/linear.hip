@@ -1213,12 +1213,10 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
         if (active) TCBNN_NOTNULL(d->preact);
         if (d->grad_weight) TCBNN_NOTNULL(d->input);
         if (d->grad_input) TCBNN_NOTNULL(d->weight);
-        if (active || d->grad_bias) {
-            TCBNN_NOTNULL(d->workspace);
-            TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "linear: the workspace is not aligned to 16 bytes");
-            TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_linear_grad_workspace_bytes(d->rows, d->in_features, d->out_features, d->dtype),
-                          "linear: workspace too small");
-        }
+        TCBNN_NOTNULL(d->workspace);
+        TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "linear: the workspace is not aligned to 16 bytes");
+        TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_linear_grad_workspace_bytes(d->rows, d->in_features, d->out_features, d->dtype),
+                      "linear: workspace too small");
     }
     return by_dtype(d->dtype, [&](auto t) -> int {
         using T = decltype(t);
@@ -1238,8 +1236,8 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
         }
         TCBNN_LAUNCH_CHECK("dz_kernel");
         const size_t before = dz_bytes(d->rows, d->out_features, d->dtype) + sum_bytes(d->rows, d->out_features, d->dtype);
-        float* partials = d->workspace && d->workspace_bytes > before ? (float*)((char*)d->workspace + before) : nullptr;
-        const size_t partial_bytes = partials ? d->workspace_bytes - before : 0;
+        float* partials = d->rows > 0 ? (float*)((char*)d->workspace + before) : nullptr;
+        const size_t partial_bytes = d->rows > 0 ? d->workspace_bytes - before : 0;
         const Operand dz = active ? Operand{d->workspace, d->out_features} : Operand{d->grad_output, dy_ld};
         ProductParams dx = {}, dw = {};
         dx.i = dw.i = dz;

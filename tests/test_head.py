@@ -89,6 +89,18 @@ def test_refusals(make, change, code, message):
     assert message in lib.tcbnn_last_error().decode()
 
 
+@pytest.mark.parametrize("change", [dict(), dict(activation=0), dict(activation=0, grad_bias=0), dict(activation=0, grad_bias=0, grad_weight=0),
+                                    dict(activation=0, grad_bias=0, grad_input=0)])
+def test_linear_gradients_need_their_workspace(change):
+    """The whole of it, whichever gradients are asked for: how a sum is split does not go by what is there."""
+    lib = _lib().lib
+    need = lib.tcbnn_linear_grad_workspace_bytes(4, 8, 8, 1)
+    for workspace, code in ((dict(workspace=0), ENULL), (dict(workspace_bytes=need - 1), EINVAL), (dict(workspace=P + 4), EINVAL)):
+        entry, d = _linear_grad(**{**change, **workspace})
+        assert getattr(lib, entry)(C.byref(d), None) == code
+        assert "workspace" in lib.tcbnn_last_error().decode()
+
+
 def test_no_rows_and_null_descriptors():
     lib = _lib().lib
     for entry, d in (_linear(rows=0, input=0, output=0), _norm(rows=0, input=0, output=0), _logprobs(rows=0, logits=0),
