@@ -402,7 +402,7 @@ int tcbnn_avgpool_fc_forward(const tcbnn_avgpool_fc_desc* d, void* stream);
 /* z = input * weight^T + bias;  output = act(z) + residual.  `output` may be `residual` (same pointer and stride).
  * `preact` receives z, rounded to dtype: what tcbnn_linear_backward needs of a layer with an activation.
  * `workspace` (tcbnn_linear_workspace_bytes; may be NULL) lets products of few rows and outputs share a long sum over
- * inputs among workgroups.  in_features <= 1048576, out_features <= 2^28. */
+ * inputs among workgroups.  rows <= 2^31 - 2^22, in_features <= 1048576, out_features <= 2^28. */
 typedef struct tcbnn_linear_desc {
     const void* input;     /* [rows][in_features]                     */
     const void* weight;    /* [out_features][in_features]             */

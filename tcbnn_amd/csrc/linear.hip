@@ -19,7 +19,8 @@ namespace {
 
 using namespace head;
 
-constexpr int kMaxIn = 1 << 20, kMaxOut = 1 << 28;
+// Rows: sums over them, and what is requested ahead of them, are counted in 32 bits.
+constexpr int kMaxIn = 1 << 20, kMaxOut = 1 << 28, kMaxRows = 0x7fffffff - (1 << 22) + 1;
 
 // ---- activations.  fp32 uses the library's erf and exp.  In 16-bit types, whose rounding is 2^-9 or 2^-12 of a result, they
 // cost as much as a quarter of a large product; there exp is 2^x of the hardware, a quotient its reciprocal (each good to
@@ -1123,6 +1124,7 @@ static int check_linear(int rows, int in_features, int out_features, int dtype, 
     TCBNN_REQUIRE(dtype_known(dtype), "linear: unknown dtype");
     TCBNN_REQUIRE(activation >= TCBNN_ACT_NONE && activation <= TCBNN_ACT_SILU, "linear: unknown activation");
     TCBNN_REQUIRE(rows >= 0 && in_features > 0 && out_features > 0, "linear: bad shape");
+    TCBNN_REQUIRE(rows <= kMaxRows, "linear: at most %d rows", kMaxRows);
     TCBNN_REQUIRE(in_features <= kMaxIn, "linear: at most %d inputs", kMaxIn);
     TCBNN_REQUIRE(out_features <= kMaxOut, "linear: at most %d outputs", kMaxOut);
     return TCBNN_OK;
@@ -1140,7 +1142,7 @@ static size_t split_bytes(int rows, int cols, int sum, int dtype, bool forward) 
 }
 
 extern "C" size_t tcbnn_linear_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
-    if (rows <= 0 || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
+    if (rows <= 0 || rows > kMaxRows || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
     return split_bytes(rows, out_features, in_features, dtype, true);
 }
 
@@ -1195,7 +1197,7 @@ static size_t sum_bytes(int rows, int out_features, int dtype) {
     return rows == 0 ? 0 : whole_lines(sizeof(float) * dz_parts(rows, out_vectors(out_features, dtype), true) * (size_t)out_features);
 }
 extern "C" size_t tcbnn_linear_grad_workspace_bytes(int rows, int in_features, int out_features, int dtype) {
-    if (rows <= 0 || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
+    if (rows <= 0 || rows > kMaxRows || in_features <= 0 || out_features <= 0 || !dtype_known(dtype)) return 0;
     return dz_bytes(rows, out_features, dtype) + sum_bytes(rows, out_features, dtype) +
            std::max(split_bytes(rows, in_features, out_features, dtype, false), split_bytes(out_features, in_features, rows, dtype, false));
 }

@@ -101,6 +101,18 @@ def test_linear_gradients_need_their_workspace(change):
         assert "workspace" in lib.tcbnn_last_error().decode()
 
 
+@pytest.mark.parametrize("rows", [(1 << 31) - 1, (1 << 31) - 600, (1 << 31) - (1 << 22) + 1])
+def test_linear_refuses_rows_that_its_sums_do_not_count(rows):
+    """The gradient of the weight sums over the rows, a step at a time past the last one: within 32 bits."""
+    lib = _lib().lib
+    for entry, d in (_linear(rows=rows), _linear_grad(rows=rows, workspace_bytes=1 << 62), _linear_grad(rows=rows, workspace_bytes=1 << 62, grad_input=0)):
+        assert getattr(lib, entry)(C.byref(d), None) == EINVAL
+        assert "rows" in lib.tcbnn_last_error().decode()
+    d = _linear(rows=rows)[1]
+    assert lib.tcbnn_linear_kernel_name(C.byref(d), C.create_string_buffer(160), 160) == EINVAL
+    assert lib.tcbnn_linear_workspace_bytes(rows, 8, 8, 1) == lib.tcbnn_linear_grad_workspace_bytes(rows, 8, 8, 1) == 0
+
+
 def test_no_rows_and_null_descriptors():
     lib = _lib().lib
     for entry, d in (_linear(rows=0, input=0, output=0), _norm(rows=0, input=0, output=0), _logprobs(rows=0, logits=0),
