@@ -89,5 +89,9 @@ __device__ __forceinline__ float wave_max(float v) {
 // of a workspace is asked for before a device is chosen.
 constexpr int kComputeUnits = 256;
 
+// A launch's threads along one axis are counted in 32 bits, without an error: what would be more is cut into several launches, taken
+// by fewer workgroups, or refused.
+constexpr long long kMaxThreads = 0xffffffffLL;
+
 }  // namespace head
 }  // namespace tcbnn

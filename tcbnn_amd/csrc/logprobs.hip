@@ -588,31 +588,37 @@ extern "C" int tcbnn_logprobs_forward(const tcbnn_logprobs_desc* d, void* stream
     const int top = d->top_index || d->top_logprob ? d->top : 0;
     const Shape shape = shape_of(d->rows, d->classes, (int)(16 / dtype_bytes(d->dtype)));
     const long long units = (long long)d->rows * shape.chunks;
-    TCBNN_REQUIRE(units <= 0x7fffffffLL, "logprobs: grid too large");
-    LogProbsParams p = {d->targets, d->logprob, d->entropy, d->logsumexp, d->top_logprob, d->rank, d->top_index, d->rows, d->classes, top,
-                        shape.chunks, ld, nullptr, nullptr};
+    Part* parts = nullptr;
+    uint64_t* keys = nullptr;
     if (shape.chunks > 1) {
         TCBNN_NOTNULL(d->workspace);
         TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_logprobs_workspace_bytes(d->rows, d->classes, top, d->dtype), "logprobs: workspace too small");
         TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "logprobs: the workspace is not aligned to 16 bytes");
-        p.parts = (Part*)d->workspace;
-        p.keys = (uint64_t*)(p.parts + units);
+        parts = (Part*)d->workspace;
+        keys = (uint64_t*)(parts + units);
     }
     by_dtype(d->dtype, [&](auto e) {
         using T = decltype(e);
         by_shape(shape, [&](auto w, auto r) {
             constexpr int W = w.value, R = r.value, kTeams = team_threads(W) / (64 * W);
-            const dim3 grid((unsigned)((units + kTeams - 1) / kTeams));
-            if constexpr (W > 1)
-                if (shape.chunks > 1) {
-                    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_kernel<T, W, R, true>), grid, dim3(team_threads(W)), 0, (hipStream_t)stream,
-                                       (const T*)d->logits, p);
-                    hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)((d->rows + kJoinRows - 1) / kJoinRows)), dim3(64 * kJoinRows),
-                                       0, (hipStream_t)stream, (const T*)d->logits, p);
-                    return;
-                }
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_kernel<T, W, R, false>), grid, dim3(team_threads(W)), 0, (hipStream_t)stream,
-                               (const T*)d->logits, p);
+            const long long at_once = kMaxThreads / team_threads(W) * kTeams / shape.chunks;
+            for (long long row = 0; row < d->rows; row += at_once) {
+                auto from = [&](auto* q, long long each) { return q ? q + row * each : q; };
+                const int rows = (int)std::min(at_once, d->rows - row);
+                const LogProbsParams p = {from(d->targets, 1), from(d->logprob, 1), from(d->entropy, 1), from(d->logsumexp, 1), from(d->top_logprob, top),
+                                          from(d->rank, 1), from(d->top_index, top), rows, d->classes, top, shape.chunks, ld, from(parts, shape.chunks),
+                                          from(keys, (long long)shape.chunks * top)};
+                const T* x = (const T*)d->logits + row * ld;
+                const dim3 grid((unsigned)(((long long)rows * shape.chunks + kTeams - 1) / kTeams));
+                if constexpr (W > 1)
+                    if (shape.chunks > 1) {
+                        hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_kernel<T, W, R, true>), grid, dim3(team_threads(W)), 0, (hipStream_t)stream, x, p);
+                        hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)((rows + kJoinRows - 1) / kJoinRows)), dim3(64 * kJoinRows), 0,
+                                           (hipStream_t)stream, x, p);
+                        continue;
+                    }
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_kernel<T, W, R, false>), grid, dim3(team_threads(W)), 0, (hipStream_t)stream, x, p);
+            }
         });
     });
     TCBNN_LAUNCH_CHECK("logprobs_kernel");
@@ -634,12 +640,15 @@ extern "C" int tcbnn_logprobs_backward(const tcbnn_logprobs_grad_desc* d, void* 
     TCBNN_REQUIRE(d->grad_logits != d->logits || d->rows == 1 || x_ld == dx_ld, "logprobs: a gradient over the logits has their stride");
     const long long piece = kGradThreads * kGradVectors * (long long)(16 / dtype_bytes(d->dtype));
     const long long pieces = (d->classes + piece - 1) / piece;
-    TCBNN_REQUIRE(pieces * d->rows <= 0x7fffffffLL, "logprobs: grid too large");
+    const long long at_once = kMaxThreads / kGradThreads / pieces;
     by_dtype(d->dtype, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(logprobs_grad_kernel<T>, dim3((unsigned)(pieces * d->rows)), dim3(kGradThreads), 0, (hipStream_t)stream,
-                           (const T*)d->logits, d->targets, d->logsumexp, d->entropy, d->grad_logprob, d->grad_entropy,
-                           (T*)d->grad_logits, d->classes, (int)pieces, x_ld, dx_ld);
+        for (long long row = 0; row < d->rows; row += at_once) {
+            auto from = [&](auto* q) { return q ? q + row : q; };
+            hipLaunchKernelGGL(logprobs_grad_kernel<T>, dim3((unsigned)(pieces * std::min(at_once, d->rows - row))), dim3(kGradThreads), 0, (hipStream_t)stream,
+                               (const T*)d->logits + row * x_ld, from(d->targets), from(d->logsumexp), from(d->entropy), from(d->grad_logprob),
+                               from(d->grad_entropy), (T*)d->grad_logits + row * dx_ld, d->classes, (int)pieces, x_ld, dx_ld);
+        }
     });
     TCBNN_LAUNCH_CHECK("logprobs_grad_kernel");
     return TCBNN_OK;

@@ -711,6 +711,47 @@ def test_logprobs_grad_of_special_rows(gpu, m, n, kind, dtype):
     _logprobs_grad(m, n, dtype, kind)
 
 
+def test_logprobs_of_more_rows_than_a_launch_has(gpu):
+    """A grid has fewer than 2^32 threads: 2^26 rows of few classes forward, 2^24 backward.  The rows repeat with an odd period."""
+    from tcbnn_amd import head
+    n, period = 2, 4099
+    r = rng(31)
+    values = r.standard_normal((period, n)).astype(np.float16)
+    targets, g = r.integers(-1, n, period).astype(np.int32), r.standard_normal(period).astype(np.float32)
+    want = [ho.logprobs(v.astype(np.float64), int(t), 1) for v, t in zip(values, targets)]
+
+    def rows(a, m):
+        return ho.DeviceBuffer.from_numpy(np.resize(a, (m,) + a.shape[1:]))
+
+    def repeats(got, a, tol):
+        wide = np.resize(np.asarray(a, np.float32), (got.shape[0],) + np.shape(a)[1:])
+        worst = np.abs(got.astype(np.float32) - wide).max()
+        assert worst <= tol, worst
+
+    m = (1 << 26) + 77
+    layer = head.LogProbsLayerParam("logprobs", m, n, 1, "f16").initialize(rows(values, m), rows(targets, m))
+    layer.forward()
+    ho.sync()
+    for name, k in (("logprob", 0), ("entropy", 1), ("logsumexp", 2), ("rank", 3), ("top_index", 4), ("top_logprob", 5)):
+        buf = getattr(layer, name + "_gpu")
+        whole = name in ("rank", "top_index")
+        got = buf.to_numpy(np.int32 if whole else np.float32, (m,))
+        repeats(got, [np.ravel(w[k])[0] for w in want], 0 if whole else 1e-5)
+    layer.release()
+    m = (1 << 24) + 77
+    layer = head.LogProbsLayerParam("logprobs", m, n, 0, "f16").initialize(rows(values, m), rows(targets, m))
+    dx = ho.DeviceBuffer(2 * m * n)
+    dx.fill(0x7f)
+    layer.initialize_backward(rows(g, m), None, dx)
+    layer.forward()
+    layer.backward()
+    ho.sync()
+    lse = np.array([w[2] for w in want])
+    hot = (np.arange(n) == targets[:, None]) - np.exp(values.astype(np.float64) - lse[:, None])
+    repeats(dx.to_numpy(np.float16, (m, n)), np.where(targets[:, None] < 0, 0.0, g[:, None] * hot), 2 * ho.U["f16"] * 4 + 1e-5)
+    layer.release()
+
+
 # --------------------------------------------------------------------------- gradients against differences
 def _slope_along(f, x, v):
     h = 1e-5
