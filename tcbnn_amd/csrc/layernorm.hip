@@ -157,34 +157,38 @@ __global__ __launch_bounds__(forward_threads(W)) void layernorm_kernel(const T* 
     }
 }
 
-// Rows that a workgroup's registers do not hold: a workgroup a row, which is read three times (twice from the cache).
+// Rows that a workgroup's registers do not hold: a workgroup a row, which is read three times (twice from the cache).  Rows beyond
+// the workgroups of a launch are taken by the same ones afterwards (with two workgroups a compute unit from the start 20000 x 8196 fp32 takes
+// 520 us, 498 with one a row); between two sums into one slot lies the barrier of the other's.
 constexpr int kLongThreads = 1024;
+inline int long_blocks(int rows) { return (int)std::min((long long)rows, kMaxThreads / kLongThreads); }
 __device__ __forceinline__ float long_sum(float v, float* slot) { return team_sum<kLongThreads / 64>(v, slot, threadIdx.x >> 6); }
 
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void layernorm_long_kernel(const T* x, const float* __restrict__ gamma,
                                                                       const float* __restrict__ beta, T* y,
                                                                       float* __restrict__ mean_out, float* __restrict__ rstd_out,
-                                                                      int n, float eps, long long x_ld, long long y_ld) {
+                                                                      int rows, int n, float eps, long long x_ld, long long y_ld) {
     __shared__ float slots[2][kLongThreads / 64];
-    const long long row = blockIdx.x;
-    x += row * x_ld;
-    y += row * y_ld;
-    float s = 0.0f;
-    for (int i = threadIdx.x; i < n; i += kLongThreads) s += (float)x[i];
-    const float mean = long_sum(s, slots[0]) / (float)n;
-    s = 0.0f;
-    for (int i = threadIdx.x; i < n; i += kLongThreads) {
-        const float d = (float)x[i] - mean;
-        s = __builtin_fmaf(d, d, s);
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* from = x + row * x_ld;
+        T* to = y + row * y_ld;
+        float s = 0.0f;
+        for (int i = threadIdx.x; i < n; i += kLongThreads) s += (float)from[i];
+        const float mean = long_sum(s, slots[0]) / (float)n;
+        s = 0.0f;
+        for (int i = threadIdx.x; i < n; i += kLongThreads) {
+            const float d = (float)from[i] - mean;
+            s = __builtin_fmaf(d, d, s);
+        }
+        const float rstd = 1.0f / sqrtf(long_sum(s, slots[1]) / (float)n + eps);
+        if (threadIdx.x == 0) {
+            if (mean_out) mean_out[row] = mean;
+            if (rstd_out) rstd_out[row] = rstd;
+        }
+        for (int i = threadIdx.x; i < n; i += kLongThreads)
+            to[i] = (T)__builtin_fmaf(((float)from[i] - mean) * rstd, gamma ? gamma[i] : 1.0f, beta ? beta[i] : 0.0f);
     }
-    const float rstd = 1.0f / sqrtf(long_sum(s, slots[1]) / (float)n + eps);
-    if (threadIdx.x == 0) {
-        if (mean_out) mean_out[row] = mean;
-        if (rstd_out) rstd_out[row] = rstd;
-    }
-    for (int i = threadIdx.x; i < n; i += kLongThreads)
-        y[i] = (T)__builtin_fmaf(((float)x[i] - mean) * rstd, gamma ? gamma[i] : 1.0f, beta ? beta[i] : 0.0f);
 }
 
 // ---- gradient.  A workgroup of 16 wavefronts is 16 / W teams; all of them take the same number of steps (a team without a
@@ -303,25 +307,25 @@ __global__ __launch_bounds__(kGradThreads) void layernorm_grad_kernel(const T* _
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void layernorm_long_grad_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
                                                                            const float* __restrict__ mean_in,
-                                                                           const float* __restrict__ rstd_in, const T* dy, T* dx,
+                                                                           const float* __restrict__ rstd_in, const T* dy, T* dx, int rows,
                                                                            int n, long long x_ld, long long dy_ld, long long dx_ld) {
     __shared__ float slots[2][kLongThreads / 64];
-    const long long row = blockIdx.x;
-    x += row * x_ld;
-    dy += row * dy_ld;
-    dx += row * dx_ld;
-    const float mean = mean_in[row], rstd = rstd_in[row];
-    float sg = 0.0f, sgx = 0.0f;
-    for (int i = threadIdx.x; i < n; i += kLongThreads) {
-        const float g = (float)dy[i] * (gamma ? gamma[i] : 1.0f);
-        sg += g;
-        sgx = __builtin_fmaf(g, ((float)x[i] - mean) * rstd, sgx);
-    }
-    sg = long_sum(sg, slots[0]) / (float)n;
-    sgx = long_sum(sgx, slots[1]) / (float)n;
-    for (int i = threadIdx.x; i < n; i += kLongThreads) {
-        const float g = (float)dy[i] * (gamma ? gamma[i] : 1.0f);
-        dx[i] = (T)((g - sg - ((float)x[i] - mean) * rstd * sgx) * rstd);
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *from = x + row * x_ld, *dy_row = dy + row * dy_ld;
+        T* to = dx + row * dx_ld;
+        const float mean = mean_in[row], rstd = rstd_in[row];
+        float sg = 0.0f, sgx = 0.0f;
+        for (int i = threadIdx.x; i < n; i += kLongThreads) {
+            const float g = (float)dy_row[i] * (gamma ? gamma[i] : 1.0f);
+            sg += g;
+            sgx = __builtin_fmaf(g, ((float)from[i] - mean) * rstd, sgx);
+        }
+        sg = long_sum(sg, slots[0]) / (float)n;
+        sgx = long_sum(sgx, slots[1]) / (float)n;
+        for (int i = threadIdx.x; i < n; i += kLongThreads) {
+            const float g = (float)dy_row[i] * (gamma ? gamma[i] : 1.0f);
+            to[i] = (T)((g - sg - ((float)from[i] - mean) * rstd * sgx) * rstd);
+        }
     }
 }
 
@@ -392,7 +396,7 @@ void by_team(int vectors, F&& f) {
 // Workgroups whose sums over rows are joined afterwards.  Up to four rows a team they are one: the launch that joins them takes as
 // long as those rows (bf16, us in one launch / two: 16 x 512 3.9 / 4.2, 32 x 512 4.7 / 6.0, 4 x 4096 7.8 / 9.1, 64 x 512 6.7 / 6.5).
 inline int grad_parts(int rows, int teams) {
-    const int steps = (rows + teams - 1) / teams;
+    const int steps = (int)((rows + teams - 1LL) / teams);
     return steps <= 4 ? 1 : std::min(steps, kComputeUnits);
 }
 
@@ -423,15 +427,15 @@ extern "C" int tcbnn_layernorm_forward(const tcbnn_layernorm_desc* d, void* stre
         using T = decltype(t);
         const int vectors = row_vectors(d->features, Elem<T>::kVec);
         if (vectors > kMaxVectors) {
-            hipLaunchKernelGGL(layernorm_long_kernel<T>, dim3((unsigned)d->rows), dim3(kLongThreads), 0, (hipStream_t)stream,
-                               (const T*)d->input, d->gamma, d->beta, (T*)d->output, d->mean, d->rstd, d->features, d->eps, x_ld, y_ld);
+            hipLaunchKernelGGL(layernorm_long_kernel<T>, dim3((unsigned)long_blocks(d->rows)), dim3(kLongThreads), 0, (hipStream_t)stream,
+                               (const T*)d->input, d->gamma, d->beta, (T*)d->output, d->mean, d->rstd, d->rows, d->features, d->eps, x_ld, y_ld);
             return;
         }
         by_team(vectors, [&](auto w, auto r) {
             constexpr int W = w.value, R = r.value;
             const int teams = forward_threads(W) / (64 * W);
             // the registers of 2048 threads a compute unit, more where rows are left
-            const int blocks = std::min((d->rows + teams - 1) / teams, kComputeUnits * 2048 / forward_threads(W));
+            const int blocks = (int)std::min((d->rows + teams - 1LL) / teams, kComputeUnits * 2048LL / forward_threads(W));
             hipLaunchKernelGGL(HIP_KERNEL_NAME(layernorm_kernel<T, W, R>), dim3((unsigned)blocks), dim3(forward_threads(W)), 0,
                                (hipStream_t)stream, (const T*)d->input, d->gamma, d->beta, (T*)d->output, d->mean, d->rstd, d->rows,
                                d->features, d->eps, x_ld, y_ld);
@@ -481,14 +485,14 @@ extern "C" int tcbnn_layernorm_backward(const tcbnn_layernorm_grad_desc* d, void
                                        (const T*)d->grad_output, partial, d->rows, d->features, x_ld, dy_ld);
                 }
                 if (d->grad_input)
-                    hipLaunchKernelGGL(layernorm_long_grad_kernel<T>, dim3((unsigned)d->rows), dim3(kLongThreads), 0, (hipStream_t)stream,
-                                       (const T*)d->input, d->gamma, d->mean, d->rstd, (const T*)d->grad_output, (T*)d->grad_input,
-                                       d->features, x_ld, dy_ld, dx_ld);
+                    hipLaunchKernelGGL(layernorm_long_grad_kernel<T>, dim3((unsigned)long_blocks(d->rows)), dim3(kLongThreads), 0,
+                                       (hipStream_t)stream, (const T*)d->input, d->gamma, d->mean, d->rstd, (const T*)d->grad_output,
+                                       (T*)d->grad_input, d->rows, d->features, x_ld, dy_ld, dx_ld);
                 return;
             }
             by_team(vectors, [&](auto w, auto r) {
                 constexpr int W = w.value, R = r.value, kTeams = kGradThreads / (64 * W);
-                parts = params ? grad_parts(d->rows, kTeams) : std::min((d->rows + kTeams - 1) / kTeams, kComputeUnits);
+                parts = params ? grad_parts(d->rows, kTeams) : (int)std::min((d->rows + kTeams - 1LL) / kTeams, (long long)kComputeUnits);
                 auto launch = [&](auto kernel) {
                     hipLaunchKernelGGL(kernel, dim3((unsigned)parts), dim3(kGradThreads), 0, (hipStream_t)stream, (const T*)d->input,
                                        d->gamma, d->mean, d->rstd, (const T*)d->grad_output, (T*)d->grad_input, partial, d->grad_gamma,

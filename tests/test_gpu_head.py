@@ -423,6 +423,45 @@ def test_layernorm_grad_single_outputs_and_in_place(gpu, m, n, dtype):
     _norm_grad(m, n, dtype, 8, in_place=True)
 
 
+@pytest.mark.parametrize("dtype,n", [("f32", 8195), ("bf16", 16392)])
+def test_layernorm_of_many_long_rows(gpu, dtype, n):
+    """Rows that a workgroup's registers do not hold, more of them than workgroups run at a time."""
+    from tcbnn_amd import head
+    m = 1100
+    r, x, gamma, beta = _norm_inputs(m, n, dtype, 0)
+    layer = head.LayerNormLayerParam("norm", m, n, dtype, EPS).initialize(gamma, beta, x.view, output_gpu=x.view)
+    want = x.values
+    layer.forward()
+    ho.sync()
+    _check_norm(want, gamma.astype(np.float64), beta.astype(np.float64), x.get(), layer.mean_gpu.to_numpy(np.float32, (m,)),
+                layer.rstd_gpu.to_numpy(np.float32, (m,)), dtype)
+    layer.release()
+    _norm_grad(m, n, dtype, in_place=True)
+
+
+def test_layernorm_of_more_long_rows_than_a_launch_has(gpu):
+    """2^22 workgroups of 1024 threads are more than a grid has: equal values become beta in every row, the last ones too."""
+    import ctypes as C
+    from tcbnn_amd import _lib, head
+    m, n = (1 << 22) + 5, 8193
+    free, total = C.c_size_t(0), C.c_size_t(0)
+    _lib.hip.hipMemGetInfo(C.byref(free), C.byref(total))
+    if free.value < 4 * m * n + (8 << 30):
+        pytest.skip("needs %d GB of device memory" % (4 * m * n >> 30))
+    x, beta = ho.DeviceBuffer(4 * m * n), np.arange(n, dtype=np.float32)
+    x.fill(0x3c)
+    layer = head.LayerNormLayerParam("norm", m, n, "f32", EPS).initialize(None, beta, x, output_gpu=x)
+    layer.forward()
+    ho.sync()
+    value = np.uint32(0x3c3c3c3c).view(np.float32)
+    for first in (0, 5, m // 2, m - 8):
+        got = ho.DeviceView(x.ptr + 4 * first * n, 4 * 8 * n).to_numpy(np.float32, (8, n))
+        # the mean's error beside the value, times rstd
+        np.testing.assert_allclose(got, np.tile(beta, (8, 1)), rtol=2 * ho.U32, atol=(n / 64 + 24) * ho.U32 * value / np.sqrt(EPS))
+    layer.release()
+    x.free()
+
+
 def test_layernorm_without_rows(gpu):
     from tcbnn_amd import head
     x, dg, db, one = ho.Matrix(None, "f32", 0, 0, 40), ho.empty(40), ho.empty(40), ho.empty(1)
