@@ -871,28 +871,31 @@ __global__ __launch_bounds__(kDzThreads) void dz_kernel(const T* __restrict__ dy
     }
 }
 
-// the sums of all parts: 16 columns a workgroup, 16 threads to a column
+// the sums of all parts: 16 columns a workgroup (and 16 more where there are more than a launch has threads for), 16 threads to a column
 constexpr int kJoinColumns = 16;
 __global__ __launch_bounds__(kDzThreads) void column_join_kernel(const float* __restrict__ sums, float* __restrict__ db, int parts, int n) {
     constexpr int kStep = kDzThreads / kJoinColumns;
     __shared__ float lds[kStep][kJoinColumns];
-    const int c = threadIdx.x % kJoinColumns, part = threadIdx.x / kJoinColumns, j = blockIdx.x * kJoinColumns + c;
-    float s = 0.0f;
-    if (j < n)
-        for (int k = part; k < parts; k += 8 * kStep) {
-            float v[8];  // (requests of their own, one wait)
+    const int c = threadIdx.x % kJoinColumns, part = threadIdx.x / kJoinColumns;
+    for (int j = blockIdx.x * kJoinColumns + c; j - c < n; j += gridDim.x * kJoinColumns) {
+        float s = 0.0f;
+        if (j < n)
+            for (int k = part; k < parts; k += 8 * kStep) {
+                float v[8];  // (requests of their own, one wait)
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = k + u * kStep < parts ? sums[(size_t)(k + u * kStep) * n + j] : 0.0f;
+                for (int u = 0; u < 8; ++u) v[u] = k + u * kStep < parts ? sums[(size_t)(k + u * kStep) * n + j] : 0.0f;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) s += v[u];
+                for (int u = 0; u < 8; ++u) s += v[u];
+            }
+        lds[part][c] = s;
+        __syncthreads();
+        if (part == 0 && j < n) {
+            s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kStep; ++k) s += lds[k][c];
+            db[j] = s;
         }
-    lds[part][c] = s;
-    __syncthreads();
-    if (part == 0 && j < n) {
-        s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kStep; ++k) s += lds[k][c];
-        db[j] = s;
+        __syncthreads();
     }
 }
 
@@ -1048,7 +1051,6 @@ void product_name(const ProductParams& p, size_t workspace_bytes, char* buf, siz
 
 template <typename T, bool ACROSS_I, bool ACROSS_J>
 int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
-    TCBNN_REQUIRE((long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) <= 0x7fffffffLL, "linear: grid too large");
     const Access access = access_of<T, ACROSS_I, ACROSS_J>(p);
     const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
     if constexpr (!ACROSS_I && !ACROSS_J) {
@@ -1066,13 +1068,24 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
     auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
         constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value, H = hold.value;
         constexpr bool L = keep.value;
+        constexpr int kThreads = 64 * WI * WJ * WS;
+        // rows beyond a launch's threads (2^29 rows, where they are too short for larger tiles than 32) have one of their own
         cut_product(p, B, kStepBytes / (int)sizeof(T), plan.splits, workspace);
-        const long long units = (long long)p.tiles_i * p.tiles_j * p.splits;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, L, ACROSS_I, ACROSS_J>), dim3((unsigned)units),
-                           dim3(64 * WI * WJ * WS), 0, stream, p);
-        if (p.splits > 1) {
-            const long long vectors_out = (long long)p.rows * ((p.cols + kJoinVector - 1) / kJoinVector);
-            hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)((vectors_out + 255) / 256)), dim3(256), 0, stream, p);
+        const long long at_once = kMaxThreads / kThreads / ((long long)p.tiles_j * p.splits) * B;
+        for (long long first = 0; first < p.rows; first += at_once) {
+            ProductParams q = p;
+            q.rows = (int)std::min(at_once, p.rows - first);
+            q.i.p = (const T*)p.i.p + (ACROSS_I ? first : first * p.i.ld);
+            q.residual = p.residual ? (const T*)p.residual + first * p.residual_ld : nullptr;
+            q.out = (T*)p.out + first * p.out_ld;
+            q.preact = p.preact ? (T*)p.preact + first * p.preact_ld : nullptr;
+            cut_product(q, B, kStepBytes / (int)sizeof(T), plan.splits, workspace);
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, L, ACROSS_I, ACROSS_J>),
+                               dim3((unsigned)((long long)q.tiles_i * q.tiles_j * q.splits)), dim3(kThreads), 0, stream, q);
+            if (q.splits > 1) {
+                const long long vectors_out = (long long)q.rows * ((q.cols + kJoinVector - 1) / kJoinVector);
+                hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)((vectors_out + 255) / 256)), dim3(256), 0, stream, q);
+            }
         }
     };
     constexpr std::integral_constant<int, 256> n256;
@@ -1233,8 +1246,8 @@ extern "C" int tcbnn_linear_backward(const tcbnn_linear_grad_desc* d, void* stre
                                        (T*)d->workspace, sums, d->rows, d->out_features, lanes, dz_rows(d->rows, vectors, active), dy_ld, z_ld);
                 });
             if (d->grad_bias && sums != d->grad_bias)
-                hipLaunchKernelGGL(column_join_kernel, dim3((unsigned)((d->out_features + kJoinColumns - 1) / kJoinColumns)), dim3(kDzThreads), 0,
-                                   (hipStream_t)stream, sums, d->grad_bias, d->rows > 0 ? parts : 0, d->out_features);
+                hipLaunchKernelGGL(column_join_kernel, dim3((unsigned)std::min((d->out_features + kJoinColumns - 1LL) / kJoinColumns, kMaxThreads / kDzThreads)),
+                                   dim3(kDzThreads), 0, (hipStream_t)stream, sums, d->grad_bias, d->rows > 0 ? parts : 0, d->out_features);
         }
         TCBNN_LAUNCH_CHECK("dz_kernel");
         const size_t before = dz_bytes(d->rows, d->out_features, d->dtype) + sum_bytes(d->rows, d->out_features, d->dtype);

@@ -299,6 +299,42 @@ def test_linear_split_sums_of_far_rows(gpu):
     w.buf.free()
 
 
+def test_linear_of_more_rows_than_a_launch_has(gpu):
+    """Rows shorter than 16 bytes go through tiles of 32 whatever their number: 2^29 of them are 2^32 threads."""
+    from tcbnn_amd import head
+    m, k, n = (1 << 29) + 77, 4, 4
+    x, y = ho.DeviceBuffer(2 * m * k), ho.DeviceBuffer(2 * m * n)
+    x.fill(0x3c)
+    y.fill(0x7f)
+    value = np.float64(np.uint16(0x3c3c).view(np.float16))
+    w = np.arange(1, 17, dtype=np.float32).reshape(n, k) / 16
+    layer = head.LinearLayerParam("linear", m, k, n, "f16").initialize(w, None, x, output_gpu=y)
+    layer.initialize_backward(x, y)
+    for run, sums in ((layer.forward, w.sum(1)), (layer.backward, w.sum(0))):
+        y.fill(0x7f)
+        run()
+        ho.sync()
+        for first in (0, 77, m // 2, m - 100):
+            got = ho.DeviceView(y.ptr + 2 * n * first, 2 * n * 100).to_numpy(np.float16, (100, n)).astype(np.float64)
+            np.testing.assert_allclose(got, np.tile(value * sums, (100, 1)), rtol=2 * ho.U["f16"])
+    layer.release()
+    x.free()
+    y.free()
+
+
+def test_bias_gradients_of_most_outputs_without_rows(gpu):
+    import ctypes as C
+    from tcbnn_amd import _lib
+    n = 1 << 28
+    db = ho.DeviceBuffer(4 * n)
+    db.fill(0x7f)
+    d = _lib.LinearGradDesc(grad_bias=db.ptr, rows=0, in_features=1, out_features=n, dtype=1)
+    _lib.check(_lib.lib.tcbnn_linear_backward(C.byref(d), None))
+    ho.sync()
+    assert not db.to_numpy(np.uint32, (n,)).any()
+    db.free()
+
+
 def test_linear_without_rows(gpu):
     from tcbnn_amd import head
     x, w = ho.Matrix(None, "bf16", 0, 0, 24), ho.Matrix(np.ones((16, 24)), "bf16")
