@@ -329,6 +329,8 @@ class FloatHead:
 
     def initialize(self, features_gpu, targets, seed=0):
         """features_gpu: [rows][features] in the head's dtype; targets: int32 [rows], -1 for rows without a class."""
+        if np.size(targets) != self.rows:
+            raise _lib.TcbnnError("Error: %d targets for %d rows" % (np.size(targets), self.rows))
         rng = np.random.default_rng(seed)
         k, h, c, m = self.features, self.hidden, self.classes, self.rows
         self.params = {"gamma1": np.ones(k, np.float32), "beta1": np.zeros(k, np.float32),

@@ -373,6 +373,15 @@ def test_layers_are_initialized_anew():
                 call()
 
 
+@pytest.mark.parametrize("count", [7, 9, 16])
+def test_head_refuses_other_than_a_target_a_row(count):
+    """More targets than rows would be counted in the mean of the rows' cross entropy."""
+    from tcbnn_amd import head
+    from tcbnn_amd.device import DeviceView
+    with pytest.raises(_lib().TcbnnError, match="targets"):
+        head.FloatHead(8, 16, 16, 4).initialize(DeviceView(P, 4 * 8 * 16), np.zeros(count, np.int32))
+
+
 def test_encode_rounds_to_nearest_even():
     from tcbnn_amd import head
     torch = pytest.importorskip("torch")
