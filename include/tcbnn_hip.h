@@ -517,6 +517,8 @@ int tcbnn_logprobs_forward(const tcbnn_logprobs_desc* d, void* stream);
  * grad_logits_j = grad_logprob * ([j = t] - p_j) - grad_entropy * p_j * (log p_j + entropy).  `logsumexp` and `entropy`
  * are the forward call's; grad_logprob or grad_entropy may be NULL (0).  Without a given class (t < 0) grad_logprob
  * counts as 0; with t >= classes the row is NaN unless grad_logprob is NULL; a row whose classes are all forbidden gets 0.
+ * p_j carries the rounding of `logsumexp` to fp32, |logsumexp| 2^-24 of it: rows of very large logits are better shifted first
+ * (the forward call's log probabilities and entropy do not depend on it).
  * The mean cross entropy of n rows is grad_logprob = -1 / n.  `grad_logits` may be `logits` (same pointer and stride). */
 typedef struct tcbnn_logprobs_grad_desc {
     const void* logits;         /* [rows][classes]           */

@@ -1,5 +1,5 @@
 // What the float head's kernels (linear.hip, layernorm.hip, logprobs.hip) share: element types, vector loads and stores at
-// any alignment, sums over wavefronts and workgroups, activations, and the choice of a kernel by type.
+// any alignment, sums over wavefronts, the choice of a kernel by type, and the sizes of grids.
 #pragma once
 
 #include <algorithm>

@@ -394,7 +394,7 @@ void by_team(int vectors, F&& f) {
 }
 
 // Workgroups whose sums over rows are joined afterwards.  Up to four rows a team they are one: the launch that joins them takes as
-// long as those rows (bf16, us in one launch / two: 16 x 512 3.9 / 4.2, 32 x 512 4.7 / 6.0, 4 x 4096 7.8 / 9.1, 64 x 512 6.7 / 6.5).
+// long as those rows (bf16, us in one launch / two: 16 x 512 3.7 / 3.7, 32 x 512 4.7 / 6.3, 4 x 4096 7.8 / 9.0, 64 x 512 6.8 / 6.5).
 inline int grad_parts(int rows, int teams) {
     const int steps = (int)((rows + teams - 1LL) / teams);
     return steps <= 4 ? 1 : std::min(steps, kComputeUnits);

@@ -5,10 +5,10 @@
 // sum (x and w of the forward product: rows of s) or across it (w of dx, dz and x of dw: a row for every s).
 //
 // Large products are bound by the matrix instructions, as far as power and the barriers between steps let them run: 8192 x 4096 x
-// 4096 in bf16 takes 218 us (1.26 PFLOP/s), 250 with bias, GELU, residual and z kept, because 134 MB more of traffic and the
-// activations follow the tiles' last steps; 8192^3 815 us (1.35 PFLOP/s); fp32 4096^3 960 us (143 TFLOP/s).  Of the gradients
+// 4096 in bf16 takes 222 us (1.24 PFLOP/s), 254 with bias, GELU, residual and z kept, because 134 MB more of traffic and the
+// activations follow the tiles' last steps; 8192^3 811 us (1.36 PFLOP/s); fp32 4096^3 949 us (145 TFLOP/s).  Of the gradients
 // of 8192 x 4096 x 1024 dx takes 83 us and dw 86 (0.8 PFLOP/s): operands across the sum need twice the LDS requests.  Rows that lie
-// anywhere go through registers, 358 us instead of 218.  Small products are bound by a launch and the latency of their steps,
+// anywhere go through registers, 348 us instead of 222.  Small products are bound by a launch and the latency of their steps,
 // products of few rows by the weights' bytes.
 #include <cmath>
 
@@ -27,7 +27,8 @@ constexpr int kMaxIn = 1 << 20, kMaxOut = 1 << 28, kMaxRows = 0x7fffffff - (1 <<
 // one unit in the last place of fp32), and the normal distribution's tail
 //   h(z) = erfc(|z| / sqrt 2) / 2 = exp(-z^2 / 2) Q(1 / (1 + 0.3 |z|)),
 // Q a polynomial of degree 8 without a constant term, fitted here for the least relative error of h over 0 <= |z| <= 13 (a Lawson
-// iteration: least squares, weights multiplied by the errors): 1.2e-7, evaluated in fp32 4.5e-7.
+// iteration: least squares, weights multiplied by the errors): 1.2e-7.  Evaluated in fp32 it is good to 5e-7 up to |z| = 2, 2e-6
+// up to 6 and 8e-6 at 13, where the rounding of the exponential's argument counts.
 constexpr float kLog2e = 1.44269504088896341f;
 template <typename T>
 __device__ __forceinline__ float exp_of(float x) {
@@ -387,7 +388,6 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
     // a wavefront's 32 rows of c on their way out, 16 bytes between rows
     constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
     static_assert(ALIGNED || STAGES == 2, "what registers hold needs two tiles");
-    static_assert(ALIGNED || STAGES == 2, "what registers hold needs two tiles");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // Workgroups go to the 8 XCDs in turn: each XCD gets a run of tiles, and a run covers 8 tiles of i after 8 tiles of i, so that what
@@ -707,8 +707,8 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
 // ---- few rows (16 at most): bound by the weights' bytes.  A wavefront has 16 outputs and a share of the sum; 64 bytes of 16 weight
 // rows are one request of it and one matrix instruction (four in fp32), and eight requests of each operand are under way at a
 // time.  A workgroup's 8 wavefronts are SHARES of the sum by 8 / SHARES groups of outputs: 8, or 2 where a sum is so short that eight
-// requests are half of it (1 x 512 x 32768 in 16 bits 8.2 us instead of 10.8, 1 x 128 x 65536 5.8 instead of 12.6).  Nothing goes
-// through LDS but the wavefronts' sums, and rows may lie anywhere.  1 x 4096 x 4096 bf16 8.3 us (33.6 MB, half of it the launch and the
+// requests are half of it (1 x 512 x 32768 in 16 bits 7.4 us instead of 10.7, 1 x 128 x 65536 6.4 instead of 12.2).  Nothing goes
+// through LDS but the wavefronts' sums, and rows may lie anywhere.  1 x 4096 x 4096 bf16 8.1 us (33.6 MB, half of it the launch and the
 // first requests' latency), 1 x 8192 x 28672 77 us (6.1 TB/s).
 constexpr int kFewRows = 16, kFewWaves = 8, kFewOutputs = 16, kFewAtOnce = 8;
 typedef float Acc4 __attribute__((ext_vector_type(4)));
@@ -795,8 +795,8 @@ inline int dz_rows(int rows, int vectors, bool active) {
     const long long threads = 1024LL * kComputeUnits;  // four workgroups a compute unit
     const int each = (int)std::max(8LL, ((long long)rows * vectors + threads - 1) / threads), deep = kDzThreads / dz_lanes(vectors);
     // one part needs no join: 16 rows a thread with their activation's slopes, 32 without, take less time than that launch (one
-    // workgroup with 32 rows of GELU a thread: gradients of 64 x 1024 -> 1024 29.7 us, 19.7 with a join; 36 x 860 -> 489
-    // fp32 without an activation 14.2 in one part, 17.7 with a join)
+    // workgroup with 32 rows of GELU a thread: gradients of 64 x 1024 -> 1024 30.5 us, 18.9 with a join; 36 x 860 -> 489
+    // fp32 without an activation 13.3 in one part, 13.9 with a join, 32 x 512 -> 1024 bf16 11.8 and 13.1)
     return rows <= (active ? 16 : 32) * deep ? std::max(each, (rows + deep - 1) / deep) : each;
 }
 inline int dz_parts(int rows, int vectors, bool active) {
@@ -900,8 +900,8 @@ __global__ __launch_bounds__(kDzThreads) void column_join_kernel(const float* __
 }
 
 // ---- both products of small gradients in one launch.  A launch more takes as long as these products do (102 x 24 -> 21 f16 with its dz:
-// 15.9 us in three launches, 9.8 in two; 128 x 1024 -> 512 18.3 and 15.7).  The first `blocks` workgroups have the product with the longer sum:
-// started last, they would run on alone (1024 x 1024 -> 10 fp32 21.5 us, 19.4 so).
+// 13.0 us in three launches, 9.9 in two; 128 x 1024 -> 512 18.8 and 16.3).  The first `blocks` workgroups have the product with the longer sum:
+// started last, they would run on alone (1024 x 1024 -> 10 bf16 15.1 us, 12.6 so).
 template <typename T, Access ACCESS, int STAGES, int HOLD>
 __global__ __launch_bounds__(256) void small_gradients_kernel(const ProductParams dx, const ProductParams dw, int blocks, bool dw_first) {
     __shared__ __align__(1024) char lds[product_lds<32, 32, 1, 1, 4, STAGES>()];
@@ -923,11 +923,12 @@ struct CutCost {
     int size;
     float start, tile, step, more;
 };
-// Measured in tiles of 256 / 128 / 128 deep / 64 / 32, rows x inputs x outputs, 16-bit types: 8192 x 4096 x 4096 220 / 274 / 310 / 458 / -,
-// 8192 x 4096 x 1024 108 / 79 / 86 / 127 / 216, 4096 x 8192 x 1024 195 / 113 / 78 / 121 / 204, 2048^3 51 / 29 / 23 / 32 / 62, 1024^3 34 / 18 / 14 / 8.5 /
-// 12.6, 64 x 4096 x 4096 69 / 44 / 29 / 19 / 11, 512^3 25 / 11 / 11 / 6.1 / 4.7.  fp32: 4000 x 2000 x 2000 482 / 259 / 266 / 280 / -, 1000^3 256 / 78 /
-// 72 / 25 / 30, 64 x 1024 x 1024 244 / 77 / 71 / 23 / 11.  Rows that lie anywhere: 8192 x 4096 x 4096 - / 358 / - / 593 / 974, 4001 x
-// 1999 x 1001 - / 40 / - / 55 / 86, 1000 x 1001 x 999 - / 24 / - / 10.6 / 16, 77 x 1023 x 1537 - / 22 / - / 10 / 6.6.
+// Measured in tiles of 256 / 128 / 128 deep / 64 / 32, rows x inputs x outputs, 16-bit types: 8192 x 4096 x 4096 221 / 279 / 315 / 455 / 786,
+// 8192 x 4096 x 1024 100 / 74 / 82 / 123 / 210, 4096 x 8192 x 1024 187 / 110 / 76 / 120 / 203, 2048^3 43 / 27 / 23 / 32 / 59, 1024^3 26 / 15 / 12 / 7.9 /
+// 11.7, 64 x 4096 x 4096 67 / 42 / 27 / 19 / 11, 512^3 17 / 8.9 / 9.0 / 5.5 / 4.4.  fp32: 4000 x 2000 x 2000 471 / 253 / 261 / 278 / 372, 1000^3 243 / 72 /
+// 69 / 24 / 29, 64 x 1024 x 1024 238 / 71 / 68 / 22 / 11.  Rows that lie anywhere: 8192 x 4096 x 4096 - / 346 / - / 584 / 943, 4001 x
+// 1999 x 1001 - / 38 / - / 55 / 86, 1000 x 1001 x 999 - / 21 / - / 9.9 / 16, 77 x 1023 x 1537 - / 19 / - / 9.1 / 6.2.  (The estimates take no
+// account of what the tiles write: the gradients of fp32 59 x 7192 -> 4060, 117 MB of them the weight's, take 124 us.)
 constexpr CutCost kCuts16[CUTS] = {{256, 9.0f, 4.0f, 1.4f, 1.6f}, {128, 6.0f, 1.5f, 0.8f, 0.52f}, {128, 6.0f, 3.0f, 0.4f, 0.55f}, {64, 3.5f, 1.0f, 0.27f, 0.21f}, {32, 3.2f, 0.5f, 0.135f, 0.11f}};
 constexpr CutCost kCuts32[CUTS] = {{256, 12.0f, 4.0f, 7.4f, 7.4f}, {128, 6.0f, 1.5f, 2.2f, 1.95f}, {128, 6.0f, 3.0f, 2.0f, 2.05f}, {64, 3.5f, 1.0f, 0.67f, 0.55f}, {32, 3.2f, 0.5f, 0.25f, 0.22f}};
 constexpr CutCost kCutsAnywhere[CUTS] = {{}, {128, 6.0f, 0.0f, 1.0f, 0.7f}, {}, {64, 3.2f, 1.2f, 0.42f, 0.33f}, {32, 3.2f, 0.5f, 0.18f, 0.165f}};
@@ -959,9 +960,9 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
 
 // The kernel for few rows instead: the wavefronts' shares of a sum, and the estimate to compare with a plan's.  A chunk of 64 bytes
 // costs a wavefront a latency, and the compute unit its requests where several workgroups have one; the rows of x are read again by every
-// workgroup.  Measured, this kernel / tiles, 16-bit types: 1 x 4096 x 4096 8.2 / 10.1, 16 x 4096 x 4096 10.4 / 10.8, 4 x 8192 x 28672 80 / 88,
-// 16 x 8192 x 28672 108 / 88, 1 x 2048 x 8192 9.8 / 8.2, 1 x 16384 x 512 20 / 9.6; fp32: 1 x 4096 x 4096 16.3 / 21.8, 8 x 16384 x 64 48 / 21;
-// rows that lie anywhere: 1 x 999 x 1001 5.1 / 6.0, 8 x 4095 x 4097 32 / 15, 4 x 8191 x 20001 184 / 110.
+// workgroup.  Measured, this kernel / tiles, 16-bit types: 1 x 4096 x 4096 8.1 / 9.9, 16 x 4096 x 4096 10.3 / 10.5, 4 x 8192 x 28672 80 / 91,
+// 16 x 8192 x 28672 108 / 89, 1 x 2048 x 8192 9.8 / 7.8, 1 x 16384 x 512 19.5 / 9.5; fp32: 1 x 4096 x 4096 15.8 / 21.3, 8 x 16384 x 64 47 / 21;
+// rows that lie anywhere: 1 x 999 x 1001 4.9 / 5.6, 8 x 4095 x 4097 31 / 15, 4 x 8191 x 20001 182 / 109.
 inline int few_shares(int cols, int sum, int size) { return sum * size <= 1024 && cols > 64 * (kComputeUnits - 1) ? 2 : 8; }
 inline float few_time(int rows, int cols, int sum, int size, bool vectors) {
     const int shares = few_shares(cols, sum, size), outputs = kFewOutputs * kFewWaves / shares;
@@ -1016,7 +1017,7 @@ bool launch_small_gradients(ProductParams dx, ProductParams dw, size_t workspace
 }
 
 // Tiles of 64 whose rows lie anywhere: the loop for long sums takes registers that a third workgroup of a compute unit would have
-// (bf16, with that loop / without: 1000 x 1001 x 999, one tile a compute unit, 10.6 us / 14.2; 2000 x 777 x 1111, three, 25.1 / 20.2).
+// (bf16, with that loop / without: 1000 x 1001 x 999, one tile a compute unit, 9.8 us / 13.5; 2000 x 777 x 1111, three, 24.4 / 19.6).
 template <typename T>
 bool long_sums(const ProductParams& p, const Plan& plan) {
     const long long tiles = (long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) * plan.splits;
