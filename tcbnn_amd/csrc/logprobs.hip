@@ -28,6 +28,7 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 __device__ __forceinline__ uint64_t key_of(float x, int j) { return ((uint64_t)ordered(x) << 32) | (uint32_t)~j; }
 __device__ __forceinline__ int class_of(uint64_t key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ uint64_t next_key(uint64_t key) { return key == 0 ? 0 : key - 1; }  // the largest that comes behind it
 __device__ __forceinline__ float logit_of(uint64_t key) {
     const uint32_t u = (uint32_t)(key >> 32);
     return u == 0xffffffffu ? NAN : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
@@ -381,14 +382,14 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
             for (int i = count + tid; i < top; i += kTeam) emit(i, 0);
         return;
     }
-    uint64_t last = ~0ull;
+    uint64_t most = ~0ull;  // (a NaN in class 0 has that key)
 #pragma unroll 1
     for (int i = 0; i < top; ++i) {
         uint64_t best = 0;
 #pragma unroll 1
         for (int j = tid; j < n; j += kTeam) {
             const uint64_t key = key_of((float)x[j], j);
-            if (key < last) best = max(best, key);
+            if (key <= most) best = max(best, key);
         }
         best = wave_max_key(best);
         if constexpr (W > 1) {
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(team_threads(W)) void logprobs_kernel(const T* __re
             for (int w = 0; w < W; ++w) best = max(best, lds.best[w]);
         }
         if (tid == 0) emit(i, best);
-        last = best;
+        most = next_key(best);
     }
 }
 
@@ -472,14 +473,15 @@ __global__ __launch_bounds__(64 * kJoinRows) void logprobs_join_kernel(const T* 
         }
         return;
     }
-    uint64_t last = ~0ull;
+    uint64_t most = ~0ull;
     for (int i = 0; i < p.top; ++i) {
         best = 0;
         each_key([&](uint64_t key) {
-            if (key < last) best = max(best, key);
+            if (key <= most) best = max(best, key);
         });
-        last = wave_max_key(best);
-        if (lane == 0) write_top(p, row, answer, i, last);
+        best = wave_max_key(best);
+        if (lane == 0) write_top(p, row, answer, i, best);
+        most = next_key(best);
     }
 }
 

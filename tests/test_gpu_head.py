@@ -706,6 +706,29 @@ def test_logprobs_of_negative_zeros(gpu, m, n, top, dtype):
                 layer.release()
 
 
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,n,top", SHAPES + [(2, 1, 1), (3, 64, 64), (2, 70000, 20)])
+def test_logprobs_of_nans_in_first_places(gpu, m, n, top, dtype):
+    """NaN goes before every number wherever it is: in class 0, in the first class of a wavefront's share or a chunk, in all."""
+    from tcbnn_amd import head
+    r = rng(m, n, 25)
+    for places in (slice(0, 1), slice(0, n, 4096), slice(0, n, 32768), slice(n - 1, n), slice(0, n)):
+        v = r.standard_normal((m, n))
+        v[:, places] = np.nan
+        t = np.zeros(m, np.int32)
+        t[-1] = n - 1
+        x = ho.Matrix(v, dtype)
+        layer = head.LogProbsLayerParam("logprobs", m, n, top, dtype).initialize(x.view, ho.vector(t, np.int32))
+        layer.forward()
+        ho.sync()
+        got = layer.download_output()
+        want = [ho.logprobs(x.values[i], int(t[i]), top) for i in range(m)]
+        np.testing.assert_array_equal(got["rank"], [w[3] for w in want])
+        np.testing.assert_array_equal(got["top_index"], np.stack([w[4] for w in want]))
+        assert np.isnan(got["logprob"]).all() and np.isnan(got["top_logprob"]).all() and np.isnan(got["entropy"]).all()
+        layer.release()
+
+
 def test_logprobs_outputs_are_optional(gpu):
     """What is not asked for is not needed: entropy alone, the best classes alone."""
     import ctypes as C
