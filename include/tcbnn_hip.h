@@ -485,6 +485,118 @@ typedef struct tcbnn_layernorm_grad_desc {
 size_t tcbnn_layernorm_grad_workspace_bytes(int rows, int features);
 int tcbnn_layernorm_backward(const tcbnn_layernorm_grad_desc* d, void* stream);
 
+/* The norms after and before a block, with its gate, its scale and the residual stream between them:
+ *   u = norm_after(block);  stream_out = stream_in + scale * gate * u;  output = norm_before(stream_out)
+ * norm(x) = (x - mean) * rstd * gamma + beta with the mean and variance of a row's features (TCBNN_NORM_LAYER), x * rstd * gamma with
+ * the mean of x^2 for the variance (TCBNN_NORM_RMS), x (TCBNN_NORM_NONE); rstd = 1 / sqrt(variance + eps).  Nothing is rounded between
+ * the two norms.  Without a `block` the stream is stream_in (after = TCBNN_NORM_NONE, no gate).  `stream_out` may be `stream_in` or
+ * `block`, `output` any of the three that is not wanted afterwards (same pointer and stride).  A beta belongs to a layer norm, a gamma to either.
+ * The statistics may be NULL; tcbnn_blocknorm_backward needs them.  features <= 65536. */
+#define TCBNN_NORM_NONE 0
+#define TCBNN_NORM_RMS 1
+#define TCBNN_NORM_LAYER 2
+typedef struct tcbnn_blocknorm_desc {
+    const void* stream_in;     /* [rows][features]                         */
+    const void* block;         /* [rows][features], or NULL                */
+    const float* gate;         /* [features], or NULL (1)                  */
+    const float* after_gamma;  /* [features], or NULL (1)                  */
+    const float* after_beta;   /* [features], or NULL (0)                  */
+    const float* before_gamma; /* [features], or NULL (1)                  */
+    const float* before_beta;  /* [features], or NULL (0)                  */
+    void* stream_out;          /* [rows][features], or NULL                */
+    void* output;              /* [rows][features]; NULL without a norm before */
+    float* after_mean;         /* [rows] each, or NULL; means of layer norms only */
+    float* after_rstd;
+    float* before_mean;
+    float* before_rstd;
+    int rows, features;
+    int dtype;
+    int after, before;         /* TCBNN_NORM_*                             */
+    float scale;
+    float eps;                 /* >= 0                                     */
+    long long stream_in_ld, block_ld, stream_out_ld, output_ld;
+} tcbnn_blocknorm_desc;
+int tcbnn_blocknorm_forward(const tcbnn_blocknorm_desc* d, void* stream);
+
+/* With g = grad_output * before_gamma, xh = (stream_out - mean) * rstd:
+ *   grad_stream_in = grad_stream_out + rstd * (g - mean of g - xh * mean of g * xh)   (no mean of g in an RMS norm),
+ *   grad_u = scale * gate * grad_stream_in, and grad_block from it through norm_after in the same way;
+ *   grad_gate = sums over the rows of scale * grad_stream_in * u, grad_after_gamma and _beta of grad_u * yh and grad_u (yh: the block's
+ *   output, normed), grad_before_gamma and _beta of grad_output * xh and grad_output.
+ * grad_stream_in is rounded where it is written only.  Any gradient that is written may be NULL; grad_output or grad_stream_out may be NULL (0).
+ * grad_stream_in may be grad_output or grad_stream_out, grad_block one of them or `block` (same pointer and stride, and not both the same).
+ * The stream and the statistics are the forward call's.  `workspace` holds tcbnn_blocknorm_grad_workspace_bytes. */
+typedef struct tcbnn_blocknorm_grad_desc {
+    const void* stream_out;       /* [rows][features]; NULL without a norm before         */
+    const void* block;            /* [rows][features], or NULL                            */
+    const float* gate;            /* [features], or NULL (1)                              */
+    const float* after_gamma;     /* [features], or NULL (1)                              */
+    const float* after_beta;      /* [features], or NULL (0)                              */
+    const float* before_gamma;    /* [features], or NULL (1)                              */
+    const float* after_mean;      /* [rows] each, where the norm has them                 */
+    const float* after_rstd;
+    const float* before_mean;
+    const float* before_rstd;
+    const void* grad_output;      /* [rows][features], or NULL                            */
+    const void* grad_stream_out;  /* [rows][features], or NULL                            */
+    void* grad_stream_in;         /* [rows][features]                                     */
+    void* grad_block;             /* [rows][features]                                     */
+    float* grad_gate;             /* [features] each                                      */
+    float* grad_after_gamma;
+    float* grad_after_beta;
+    float* grad_before_gamma;
+    float* grad_before_beta;
+    int rows, features;
+    int dtype;
+    int after, before;
+    float scale;
+    long long stream_out_ld, block_ld, grad_output_ld, grad_stream_out_ld, grad_stream_in_ld, grad_block_ld;
+    void* workspace;
+    size_t workspace_bytes;
+} tcbnn_blocknorm_grad_desc;
+size_t tcbnn_blocknorm_grad_workspace_bytes(int rows, int features, int dtype);
+int tcbnn_blocknorm_backward(const tcbnn_blocknorm_grad_desc* d, void* stream);
+
+/* A gated feed-forward product: z = input * weight^T + bias with 2 * features columns, the gate's first;
+ * output = act(z of the gate) * (z of the rest).  `preact` receives z, rounded to dtype: what tcbnn_gated_backward needs.
+ * rows <= 2^31 - 2^22, in_features <= 1048576, features <= 2^27. */
+typedef struct tcbnn_gated_desc {
+    const void* input;   /* [rows][in_features]         */
+    const void* weight;  /* [2 * features][in_features] */
+    const float* bias;   /* [2 * features], or NULL     */
+    void* output;        /* [rows][features]            */
+    void* preact;        /* [rows][2 * features], or NULL */
+    int rows, in_features, features;
+    int dtype;
+    int activation;      /* TCBNN_ACT_*                 */
+    long long input_ld, weight_ld, output_ld, preact_ld;
+} tcbnn_gated_desc;
+int tcbnn_gated_forward(const tcbnn_gated_desc* d, void* stream);
+/* Name of the kernel that tcbnn_gated_forward launches for this descriptor; nothing is launched, no pointer followed. */
+int tcbnn_gated_kernel_name(const tcbnn_gated_desc* d, char* buf, size_t len);
+
+/* With z as the forward call wrote it, dz of the gate = grad_output * (z of the rest) * act'(z of the gate), dz of the rest =
+ * grad_output * act(z of the gate):  grad_input = dz * weight, grad_weight = dz^T * input, grad_bias = sums of dz over the rows.  Each of
+ * the three may be NULL; what is given is overwritten.  relu'(0) = 0.  In 16-bit types dz is rounded to dtype before the two products;
+ * grad_bias sums it unrounded.  `workspace` holds tcbnn_gated_grad_workspace_bytes. */
+typedef struct tcbnn_gated_grad_desc {
+    const void* input;        /* [rows][in_features]; NULL where grad_weight is          */
+    const void* weight;       /* [2 * features][in_features]; NULL where grad_input is   */
+    const void* preact;       /* [rows][2 * features]                                    */
+    const void* grad_output;  /* [rows][features]                                        */
+    void* grad_input;         /* [rows][in_features]                                     */
+    void* grad_weight;        /* [2 * features][in_features]                             */
+    float* grad_bias;         /* [2 * features]                                          */
+    int rows, in_features, features;
+    int dtype;
+    int activation;
+    long long input_ld, weight_ld, preact_ld, grad_output_ld, grad_input_ld, grad_weight_ld;
+    void* workspace;
+    size_t workspace_bytes;
+} tcbnn_gated_grad_desc;
+size_t tcbnn_gated_grad_workspace_bytes(int rows, int in_features, int features, int dtype);
+int tcbnn_gated_backward(const tcbnn_gated_grad_desc* d, void* stream);
+
 /* Of every row of logits x: logsumexp = log(sum exp(x_j)); logprob = x_t - logsumexp of the given class t = targets[row];
  * entropy = -sum p_j log p_j with p_j = exp(x_j - logsumexp) (in nats); rank = the number of classes before t in the order
  * "larger logit first, lower index among equals" (0: t is the best); top_index, top_logprob = the first `top` classes of

@@ -113,6 +113,46 @@ class LayerNormGradDesc(C.Structure):
                 ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
+class BlockNormDesc(C.Structure):
+    _fields_ = [("stream_in", c_void_p), ("block", c_void_p), ("gate", c_void_p), ("after_gamma", c_void_p),
+                ("after_beta", c_void_p), ("before_gamma", c_void_p), ("before_beta", c_void_p),
+                ("stream_out", c_void_p), ("output", c_void_p), ("after_mean", c_void_p), ("after_rstd", c_void_p),
+                ("before_mean", c_void_p), ("before_rstd", c_void_p), ("rows", c_int), ("features", c_int),
+                ("dtype", c_int), ("after", c_int), ("before", c_int), ("scale", C.c_float), ("eps", C.c_float),
+                ("stream_in_ld", C.c_longlong), ("block_ld", C.c_longlong), ("stream_out_ld", C.c_longlong),
+                ("output_ld", C.c_longlong)]
+
+
+class BlockNormGradDesc(C.Structure):
+    _fields_ = [("stream_out", c_void_p), ("block", c_void_p), ("gate", c_void_p), ("after_gamma", c_void_p),
+                ("after_beta", c_void_p), ("before_gamma", c_void_p), ("after_mean", c_void_p),
+                ("after_rstd", c_void_p), ("before_mean", c_void_p), ("before_rstd", c_void_p),
+                ("grad_output", c_void_p), ("grad_stream_out", c_void_p), ("grad_stream_in", c_void_p),
+                ("grad_block", c_void_p), ("grad_gate", c_void_p), ("grad_after_gamma", c_void_p),
+                ("grad_after_beta", c_void_p), ("grad_before_gamma", c_void_p), ("grad_before_beta", c_void_p),
+                ("rows", c_int), ("features", c_int), ("dtype", c_int), ("after", c_int), ("before", c_int),
+                ("scale", C.c_float), ("stream_out_ld", C.c_longlong), ("block_ld", C.c_longlong),
+                ("grad_output_ld", C.c_longlong), ("grad_stream_out_ld", C.c_longlong),
+                ("grad_stream_in_ld", C.c_longlong), ("grad_block_ld", C.c_longlong), ("workspace", c_void_p),
+                ("workspace_bytes", c_size_t)]
+
+
+class GatedDesc(C.Structure):
+    _fields_ = [("input", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("output", c_void_p),
+                ("preact", c_void_p), ("rows", c_int), ("in_features", c_int), ("features", c_int), ("dtype", c_int),
+                ("activation", c_int), ("input_ld", C.c_longlong), ("weight_ld", C.c_longlong),
+                ("output_ld", C.c_longlong), ("preact_ld", C.c_longlong)]
+
+
+class GatedGradDesc(C.Structure):
+    _fields_ = [("input", c_void_p), ("weight", c_void_p), ("preact", c_void_p), ("grad_output", c_void_p),
+                ("grad_input", c_void_p), ("grad_weight", c_void_p), ("grad_bias", c_void_p), ("rows", c_int),
+                ("in_features", c_int), ("features", c_int), ("dtype", c_int), ("activation", c_int),
+                ("input_ld", C.c_longlong), ("weight_ld", C.c_longlong), ("preact_ld", C.c_longlong),
+                ("grad_output_ld", C.c_longlong), ("grad_input_ld", C.c_longlong), ("grad_weight_ld", C.c_longlong),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
 class LogProbsDesc(C.Structure):
     _fields_ = [("logits", c_void_p), ("targets", c_void_p), ("logprob", c_void_p), ("entropy", c_void_p),
                 ("logsumexp", c_void_p), ("rank", c_void_p), ("top_index", c_void_p), ("top_logprob", c_void_p),
@@ -184,6 +224,13 @@ ABI = {
     "tcbnn_layernorm_forward": (c_int, [C.POINTER(LayerNormDesc), c_void_p]),
     "tcbnn_layernorm_grad_workspace_bytes": (c_size_t, [c_int] * 2),
     "tcbnn_layernorm_backward": (c_int, [C.POINTER(LayerNormGradDesc), c_void_p]),
+    "tcbnn_blocknorm_forward": (c_int, [C.POINTER(BlockNormDesc), c_void_p]),
+    "tcbnn_blocknorm_grad_workspace_bytes": (c_size_t, [c_int] * 3),
+    "tcbnn_blocknorm_backward": (c_int, [C.POINTER(BlockNormGradDesc), c_void_p]),
+    "tcbnn_gated_forward": (c_int, [C.POINTER(GatedDesc), c_void_p]),
+    "tcbnn_gated_kernel_name": (c_int, [C.POINTER(GatedDesc), C.c_char_p, c_size_t]),
+    "tcbnn_gated_grad_workspace_bytes": (c_size_t, [c_int] * 4),
+    "tcbnn_gated_backward": (c_int, [C.POINTER(GatedGradDesc), c_void_p]),
     "tcbnn_logprobs_workspace_bytes": (c_size_t, [c_int] * 4),
     "tcbnn_logprobs_forward": (c_int, [C.POINTER(LogProbsDesc), c_void_p]),
     "tcbnn_logprobs_backward": (c_int, [C.POINTER(LogProbsGradDesc), c_void_p]),
@@ -209,6 +256,7 @@ VARIANTS = {"auto": 0, "popc": 1, "mfma_i8": 2, "mfma_f4": 3}
 RES_I32, RES_I16, RES_I12 = 0, 1, 2
 INCONV_INPUT_NCHW, INCONV_INPUT_PACKED = 0, 1
 DTYPES = {"f32": 0, "bf16": 1, "f16": 2}
+NORMS = {"none": 0, "rms": 1, "layer": 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 INT32_MAX = 2 ** 31 - 1
 

@@ -1,0 +1,422 @@
+// The gated feed-forward product and its gradients (tcbnn_gated_forward / _backward):  z = x w^T + b with 2 n columns, the gate's first;
+// h = act(g) u of its halves g and u;  dg = dh u act'(g),  du = dh act(g),  dx = [dg du] w,  dw = [dg du]^T x,  db = column sums.
+//
+// Forward, both projections are one product: a tile's columns alternate between 16 rows of the gate's weights and the same 16 of the
+// rest, so that g and u of a column are in one lane's registers when the sum is done, and z leaves only where it is asked for.
+// Backward, [dg du] is one matrix of 2 n columns, as w is one of 2 n rows: a pass makes it, and two products of the linear layer's follow.
+#include "product.h"
+
+namespace tcbnn {
+namespace {
+
+using namespace head;
+
+constexpr int kMaxFeatures = kMaxOut / 2;
+
+// their z -> the outputs: C neighbouring columns of a row, of which `n` exist
+template <typename T, int C>
+__device__ __forceinline__ void finish(const ProductParams& p, long long i, int j, int n, const float* bias_g, const float* bias_u, float* g, float* u) {
+#pragma unroll
+    for (int e = 0; e < C; ++e) g[e] += bias_g[e], u[e] += bias_u[e];
+    if (p.preact) {
+        put_columns<T, C>(p.preact, p.preact_ld, i, j, n, g);
+        put_columns<T, C>((T*)p.preact + p.cols, p.preact_ld, i, j, n, u);
+    }
+    by_activation(p.activation, [&](auto act) {
+#pragma unroll
+        for (int e = 0; e < C; ++e) g[e] = activate<T, act.value>(g[e]) * u[e];
+    });
+    put_columns<T, C>(p.out, p.out_ld, i, j, n, g);
+}
+
+// `p.cols` is n; a workgroup's tile is BI rows by BJ / 2 columns of either half.
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG>
+__global__ __launch_bounds__(64 * WI * WJ * WS) void gated_product_kernel(const ProductParams p) {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
+    __shared__ __align__(1024) char lds[product_lds<BI, BJ, WI, WJ, WS, STAGES>()];
+    constexpr int NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec;
+    constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
+    Acc acc[NI][NJ];
+    Spot spot;
+    product_sums<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, LONG, false, false, true>(p, blockIdx.x, lds, acc, spot);
+    const int lane = spot.lane, share = spot.share;
+
+    // ---- out: 32 rows of the wavefront at a time through LDS (16 columns of g, 16 of u and so on), shared among wavefronts that shared the sum
+    char* mine = lds + spot.wave * kOutWave;
+    const char* first_share = lds + spot.wave % (WI * WJ) * kOutWave;
+    constexpr int kPerRow = 16 * NJ / V, kShareRows = 32 / WS;  // lanes to a row, rows of a wavefront
+    constexpr int kRowsAtOnce = 64 / kPerRow < kShareRows ? 64 / kPerRow : kShareRows, kTimes = kShareRows / kRowsAtOnce;
+    const int col = (lane % kPerRow) * V, j = (int)spot.j0 + spot.wj / 2 + col, n = lane / kPerRow < kRowsAtOnce ? min(V, p.cols - j) : 0;
+    const int at = (col / kPairedRows * 2 * kPairedRows + col % kPairedRows) * 4;
+    float bias_g[V], bias_u[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        bias_g[e] = p.bias && e < n ? p.bias[j + e] : 0.0f;
+        bias_u[e] = p.bias && e < n ? p.bias[(long long)p.cols + j + e] : 0.0f;
+    }
+#pragma unroll 1
+    for (int a = 0; a < NI; ++a) {
+        const int row0 = share * kShareRows + lane / kPerRow % kRowsAtOnce;
+        const long long first = spot.i0 + spot.wi + 32 * a + row0;
+#pragma unroll
+        for (int k = 0; k < NI; ++k)  // (registers have no index: one of NI pieces of code)
+            if (k == a) {
+#pragma unroll
+                for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<float4*>(mine + (lane & 31) * kOutRow + (32 * b + 8 * q + 4 * (lane >> 5)) * 4) =
+                            make_float4(acc[k][b][4 * q], acc[k][b][4 * q + 1], acc[k][b][4 * q + 2], acc[k][b][4 * q + 3]);
+            }
+        if constexpr (WS > 1)
+            __syncthreads();
+        else
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int r = 0; r < kTimes; ++r) {
+            const long long i = first + r * kRowsAtOnce;
+            const char* from = first_share + (row0 + r * kRowsAtOnce) * kOutRow + at;
+            float z[2][V];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int e = 0; e < V; e += 4) {
+                    float4 q = *reinterpret_cast<const float4*>(from + (half * kPairedRows + e) * 4);
+#pragma unroll
+                    for (int w = 1; w < WS; ++w) {
+                        const float4 o = *reinterpret_cast<const float4*>(from + w * (WI * WJ * kOutWave) + (half * kPairedRows + e) * 4);
+                        q.x += o.x, q.y += o.y, q.z += o.z, q.w += o.w;
+                    }
+                    z[half][e] = q.x, z[half][e + 1] = q.y, z[half][e + 2] = q.z, z[half][e + 3] = q.w;
+                }
+            if (i < p.rows && n > 0) finish<T, V>(p, i, j, n, bias_g, bias_u, z[0], z[1]);
+        }
+        if constexpr (WS > 1) {
+            if (NI > 1) __syncthreads();
+        } else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    }
+#endif
+}
+
+// few rows: 8 rows of the gate's weights and the same 8 of the rest are a wavefront's 16
+constexpr int kFewPairs = kFewOutputs / 2;
+template <typename T, int SHARES>
+__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 4))) void gated_few_rows_kernel(const ProductParams p) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = wave % SHARES;
+    const long long j0 = ((long long)blockIdx.x * (kFewWaves / SHARES) + wave / SHARES) * kFewPairs;
+    // rows past the last one are read as the last one; nothing of them is kept
+    const T* w = (const T*)p.j.p + (min(j0 + lane % kFewPairs, (long long)p.cols - 1) + (lane & kFewPairs ? p.cols : 0)) * p.j.ld;
+    const T* x = (const T*)p.i.p + (long long)min(lane & 15, p.rows - 1) * p.i.ld;
+    const Acc4 acc = few_rows_sums<T, SHARES>(p, w, x);
+    if (share != 0) return;
+    float g[4], u[4], bias_g[4], bias_u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        g[e] = acc[e];
+        u[e] = __shfl_xor(acc[e], 32);
+    }
+    const int i = lane & 15;
+    const long long j = j0 + 4 * (lane >> 4);
+    const int n = (int)min(4LL, p.cols - j);
+    if (lane >= 32 || i >= p.rows || n <= 0) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bias_g[e] = p.bias && e < n ? p.bias[j + e] : 0.0f;
+        bias_u[e] = p.bias && e < n ? p.bias[p.cols + j + e] : 0.0f;
+    }
+    finish<T, 4>(p, i, (int)j, n, bias_g, bias_u, g, u);
+}
+
+// ---- [dg du] in the operands' type, and its column sums in fp32, unrounded.  Bound by memory, and built as the linear layer's pass is: a thread has
+// one vector of 16 bytes of columns, of both halves, and goes down its share of the rows.
+template <typename T, int ACT>
+__global__ __launch_bounds__(kDzThreads) void gated_dz_kernel(const T* __restrict__ dh, const T* __restrict__ z, T* __restrict__ dz,
+                                                              float* __restrict__ sums, int rows, int n, int lanes, int each, long long dh_ld,
+                                                              long long z_ld) {
+    constexpr int V = Elem<T>::kVec, kAtOnce = 2;
+    __shared__ float lds[2][kDzThreads * V];
+    const int deep = kDzThreads / lanes, lane = threadIdx.x % lanes, depth = threadIdx.x / lanes;
+    const int j = (blockIdx.x * lanes + lane) * V, left = n - j;
+    const long long first = (long long)blockIdx.y * deep * each;
+    const long long last = min((long long)rows, first + (long long)deep * each);
+    float s[2][V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[0][e] = s[1][e] = 0.0f;
+    if (depth < deep && left > 0) {
+        auto get = [&](const T* p) {
+            if (left >= V) return load_vec(p);
+            Vec<T> v;
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = e < left ? p[e] : (T)0.0f;
+            return v;
+        };
+        auto put = [&](T* to, const float* d) {
+            if (left >= V) {
+                Vec<T> v;
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = (T)d[e];
+                store_vec(to, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e < left) to[e] = (T)d[e];
+            }
+        };
+        for (long long r = first + depth; r < last; r += kAtOnce * deep) {
+            Vec<T> d[kAtOnce], g[kAtOnce], u[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const long long at = min(r + k * deep, last - 1);  // (rows past the end are read once more and not used)
+                d[k] = get(dh + at * dh_ld + j);
+                g[k] = get(z + at * z_ld + j);
+                u[k] = get(z + at * z_ld + n + j);
+            }
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                if (r + k * deep >= last) break;
+                float dg[V], du[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float gate = (float)g[k][e], out = (float)d[k][e];
+                    dg[e] = out * (float)u[k][e] * slope<T, ACT>(gate);
+                    du[e] = out * activate<T, ACT>(gate);
+                    s[0][e] += dg[e];
+                    s[1][e] += du[e];
+                }
+                T* to = dz + (r + k * deep) * 2 * n + j;
+                put(to, dg);
+                put(to + n, du);
+            }
+        }
+    }
+    if (sums == nullptr) return;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int e = 0; e < V; ++e) lds[half][e * kDzThreads + threadIdx.x] = s[half][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < lanes * V; c += kDzThreads) {
+        const int l = c / V, e = c % V, col = (blockIdx.x * lanes + l) * V + e;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float t = 0.0f;
+            for (int d = 0; d < deep; ++d) t += lds[half][e * kDzThreads + d * lanes + l];
+            if (col < n) sums[((size_t)blockIdx.y * 2 + half) * n + col] = t;
+        }
+    }
+}
+
+// The tile is the one that the linear layer's estimates would take for a product of 2 n columns; sums are not split.
+template <typename T>
+struct GatedPlan {
+    Access access;
+    Plan plan;
+    bool few;
+};
+template <typename T>
+GatedPlan<T> plan_gated(const ProductParams& p) {
+    GatedPlan<T> g;
+    g.access = access_of<T, false, false>(p);
+    const bool vectors = g.access == WHOLE_PIECES;
+    g.plan = plan_product(p.rows, 2 * p.cols, p.sum, (int)sizeof(T), vectors, 0);
+    g.few = p.rows <= kFewRows && (g.access == ELEMENTS || few_time(p.rows, 2 * p.cols, p.sum, (int)sizeof(T), vectors) < g.plan.time);
+    return g;
+}
+
+template <typename T>
+int launch_gated(const ProductParams& p, hipStream_t stream) {
+    const GatedPlan<T> g = plan_gated<T>(p);
+    if (g.few) {
+        const int shares = few_shares(2 * p.cols, p.sum, (int)sizeof(T)), outputs = kFewPairs * kFewWaves / shares;
+        const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
+        if (shares == 8)
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_few_rows_kernel<T, 8>), grid, dim3(64 * kFewWaves), 0, stream, p);
+        else
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_few_rows_kernel<T, 2>), grid, dim3(64 * kFewWaves), 0, stream, p);
+        TCBNN_LAUNCH_CHECK("gated_few_rows_kernel");
+        return TCBNN_OK;
+    }
+    auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
+        constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value, H = hold.value;
+        constexpr bool L = keep.value;
+        constexpr int kThreads = 64 * WI * WJ * WS;
+        // rows beyond a launch's threads have one of their own
+        const long long tiles_j = (p.cols + B / 2 - 1) / (B / 2), at_once = std::max(1LL, kMaxThreads / kThreads / tiles_j) * B;
+        for (long long first = 0; first < p.rows; first += at_once) {
+            ProductParams q = p;
+            q.rows = (int)std::min(at_once, p.rows - first);
+            q.i.p = (const T*)p.i.p + first * p.i.ld;
+            q.out = (T*)p.out + first * p.out_ld;
+            q.preact = p.preact ? (T*)p.preact + first * p.preact_ld : nullptr;
+            cut_product(q, B, kStepBytes / (int)sizeof(T), 1, nullptr);
+            q.tiles_j = (int)tiles_j;
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, L>),
+                               dim3((unsigned)((long long)q.tiles_i * q.tiles_j)), dim3(kThreads), 0, stream, q);
+        }
+    };
+    constexpr std::integral_constant<int, 256> n256;
+    constexpr std::integral_constant<int, 128> n128;
+    constexpr std::integral_constant<int, 64> n64;
+    constexpr std::integral_constant<int, 32> n32;
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 4> four;
+    constexpr std::integral_constant<int, 8> eight;
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    constexpr std::integral_constant<Access, WHOLE_PIECES> pieces;
+    constexpr std::integral_constant<Access, ANYWHERE> anywhere;
+    constexpr std::integral_constant<Access, ELEMENTS> elements;
+    if (g.access == WHOLE_PIECES) {
+        switch (g.plan.cut) {
+            case CUT_256: go(n256, two, four, one, two, pieces, one, no); break;
+            case CUT_128: go(n128, two, two, one, two, pieces, one, no); break;
+            case CUT_128_DEEP: go(n128, two, two, two, four, pieces, one, no); break;
+            case CUT_64: go(n64, two, two, two, four, pieces, one, no); break;
+            default: go(n32, one, one, four, eight, pieces, one, no); break;
+        }
+    } else if (g.access == ANYWHERE) {
+        switch (g.plan.cut) {
+            case CUT_128: go(n128, two, two, one, two, anywhere, one, no); break;
+            case CUT_64: go(n64, two, two, two, two, anywhere, four, no); break;
+            default: go(n32, one, one, four, two, anywhere, four, yes); break;
+        }
+    } else {
+        go(n32, one, one, four, two, elements, one, no);
+    }
+    TCBNN_LAUNCH_CHECK("gated_product_kernel");
+    return TCBNN_OK;
+}
+
+// the kernel that launch_gated takes, as a profiler lists it
+template <typename T>
+void gated_name(const ProductParams& p, char* buf, size_t len) {
+    const char* type = std::is_same_v<T, float> ? "float" : (std::is_same_v<T, _Float16> ? "_Float16" : "__bf16");
+    const GatedPlan<T> g = plan_gated<T>(p);
+    if (g.few) {
+        snprintf(buf, len, "gated_few_rows_kernel<%s, %d>", type, few_shares(2 * p.cols, p.sum, (int)sizeof(T)));
+        return;
+    }
+    static const char* const shape[3][CUTS] = {
+        {"256, 256, 2, 4, 1, 2", "128, 128, 2, 2, 1, 2", "128, 128, 2, 2, 2, 4", "64, 64, 2, 2, 2, 4", "32, 32, 1, 1, 4, 8"},
+        {"", "128, 128, 2, 2, 1, 2", "", "64, 64, 2, 2, 2, 2", "32, 32, 1, 1, 4, 2"},
+        {"32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2"}};
+    const int hold = g.access == ANYWHERE && g.plan.cut != CUT_128 ? 4 : 1;
+    snprintf(buf, len, "gated_product_kernel<%s, %s, (Access)%d, %d, %s>", type, shape[g.access][g.plan.cut], (int)g.access, hold,
+             hold == 4 && g.plan.cut != CUT_64 ? "true" : "false");
+}
+
+int check_gated(int rows, int in_features, int features, int dtype, int activation) {
+    TCBNN_REQUIRE(dtype_known(dtype), "gated: unknown dtype");
+    TCBNN_REQUIRE(activation >= TCBNN_ACT_NONE && activation <= TCBNN_ACT_SILU, "gated: unknown activation");
+    TCBNN_REQUIRE(rows >= 0 && in_features > 0 && features > 0, "gated: bad shape");
+    TCBNN_REQUIRE(rows <= kMaxRows, "gated: at most %d rows", kMaxRows);
+    TCBNN_REQUIRE(in_features <= kMaxIn, "gated: at most %d inputs", kMaxIn);
+    TCBNN_REQUIRE(features <= kMaxFeatures, "gated: at most %d features", kMaxFeatures);
+    return TCBNN_OK;
+}
+
+ProductParams gated_product(const tcbnn_gated_desc* d) {
+    ProductParams p = {};
+    p.i = {d->input, row_stride(d->input_ld, d->in_features)};
+    p.j = {d->weight, row_stride(d->weight_ld, d->in_features)};
+    p.rows = d->rows;
+    p.cols = d->features;
+    p.sum = d->in_features;
+    p.activation = d->activation;
+    p.bias = d->bias;
+    p.out = d->output;
+    p.preact = d->preact;
+    p.out_ld = row_stride(d->output_ld, d->features);
+    p.preact_ld = row_stride(d->preact_ld, 2LL * d->features);
+    return p;
+}
+
+// What the gradients need of a workspace: dz in dtype, then the parts of the column sums (whole 256 bytes each).
+size_t dz_bytes(int rows, int features, int dtype) { return whole_lines((size_t)rows * 2 * features * dtype_bytes(dtype)); }
+size_t sum_bytes(int rows, int features, int dtype) {
+    return rows == 0 ? 0 : whole_lines(sizeof(float) * dz_parts(rows, out_vectors(features, dtype), true) * 2 * (size_t)features);
+}
+
+}  // namespace
+}  // namespace tcbnn
+
+using namespace tcbnn;
+using namespace tcbnn::head;
+
+extern "C" int tcbnn_gated_kernel_name(const tcbnn_gated_desc* d, char* buf, size_t len) {
+    TCBNN_NOTNULL(d);
+    TCBNN_NOTNULL(buf);
+    if (int rc = check_gated(d->rows, d->in_features, d->features, d->dtype, d->activation)) return rc;
+    by_dtype(d->dtype, [&](auto t) { gated_name<decltype(t)>(gated_product(d), buf, len); });
+    return TCBNN_OK;
+}
+
+extern "C" int tcbnn_gated_forward(const tcbnn_gated_desc* d, void* stream) {
+    TCBNN_NOTNULL(d);
+    if (int rc = check_gated(d->rows, d->in_features, d->features, d->dtype, d->activation)) return rc;
+    const ProductParams p = gated_product(d);
+    TCBNN_REQUIRE(p.i.ld > 0 && p.j.ld > 0 && p.out_ld > 0 && p.preact_ld > 0, "gated: rows overlap");
+    if (d->rows == 0) return TCBNN_OK;
+    TCBNN_NOTNULL(d->input);
+    TCBNN_NOTNULL(d->weight);
+    TCBNN_NOTNULL(d->output);
+    return by_dtype(d->dtype, [&](auto t) { return launch_gated<decltype(t)>(p, (hipStream_t)stream); });
+}
+
+extern "C" size_t tcbnn_gated_grad_workspace_bytes(int rows, int in_features, int features, int dtype) {
+    if (rows <= 0 || rows > kMaxRows || in_features <= 0 || in_features > kMaxIn || features <= 0 || features > tcbnn::kMaxFeatures || !dtype_known(dtype)) return 0;
+    return dz_bytes(rows, features, dtype) + sum_bytes(rows, features, dtype) + gradient_product_bytes(rows, in_features, 2 * features, dtype);
+}
+
+extern "C" int tcbnn_gated_backward(const tcbnn_gated_grad_desc* d, void* stream) {
+    TCBNN_NOTNULL(d);
+    if (int rc = check_gated(d->rows, d->in_features, d->features, d->dtype, d->activation)) return rc;
+    const long long x_ld = row_stride(d->input_ld, d->in_features), w_ld = row_stride(d->weight_ld, d->in_features),
+                    z_ld = row_stride(d->preact_ld, 2LL * d->features), dh_ld = row_stride(d->grad_output_ld, d->features),
+                    dx_ld = row_stride(d->grad_input_ld, d->in_features), dw_ld = row_stride(d->grad_weight_ld, d->in_features);
+    TCBNN_REQUIRE(x_ld > 0 && w_ld > 0 && z_ld > 0 && dh_ld > 0 && dx_ld > 0 && dw_ld > 0, "gated: rows overlap");
+    if (d->rows > 0) {
+        TCBNN_NOTNULL(d->grad_output);
+        TCBNN_NOTNULL(d->preact);
+        if (d->grad_weight) TCBNN_NOTNULL(d->input);
+        if (d->grad_input) TCBNN_NOTNULL(d->weight);
+        TCBNN_NOTNULL(d->workspace);
+        TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "gated: the workspace is not aligned to 16 bytes");
+        TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_gated_grad_workspace_bytes(d->rows, d->in_features, d->features, d->dtype), "gated: workspace too small");
+    }
+    if (!d->grad_input && !d->grad_weight && !d->grad_bias) return TCBNN_OK;
+    const int vectors = out_vectors(d->features, d->dtype), lanes = dz_lanes(vectors), parts = d->rows > 0 ? dz_parts(d->rows, vectors, true) : 0;
+    float* sums = d->grad_bias ? (float*)((char*)d->workspace + dz_bytes(d->rows, d->features, d->dtype)) : nullptr;
+    if (d->grad_bias && parts == 1) sums = d->grad_bias;
+    if (d->rows > 0)
+        by_dtype(d->dtype, [&](auto t) {
+            using T = decltype(t);
+            by_activation(d->activation, [&](auto act) {
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_dz_kernel<T, act.value>), dim3((unsigned)((vectors + lanes - 1) / lanes), (unsigned)parts), dim3(kDzThreads),
+                                   0, (hipStream_t)stream, (const T*)d->grad_output, (const T*)d->preact, (T*)d->workspace, sums, d->rows, d->features, lanes,
+                                   dz_rows(d->rows, vectors, true), dh_ld, z_ld);
+            });
+        });
+    if (d->grad_bias && sums != d->grad_bias) launch_column_join(sums, d->grad_bias, parts, 2 * d->features, (hipStream_t)stream);
+    TCBNN_LAUNCH_CHECK("gated_dz_kernel");
+    const size_t before = dz_bytes(d->rows, d->features, d->dtype) + sum_bytes(d->rows, d->features, d->dtype);
+    ProductParams dx = {}, dw = {};
+    dx.i = dw.i = {d->workspace, 2LL * d->features};
+    dx.j = {d->weight, w_ld};
+    dx.rows = d->rows;
+    dx.cols = d->in_features;
+    dx.sum = 2 * d->features;
+    dx.out = d->grad_input;
+    dx.out_ld = dx_ld;
+    dw.j = {d->input, x_ld};
+    dw.rows = 2 * d->features;
+    dw.cols = d->in_features;
+    dw.sum = d->rows;
+    dw.out = d->grad_weight;
+    dw.out_ld = dw_ld;
+    return launch_gradient_products(d->dtype, dx, dw, d->rows > 0 ? (float*)((char*)d->workspace + before) : nullptr,
+                                    d->rows > 0 ? d->workspace_bytes - before : 0, (hipStream_t)stream);
+}

@@ -17,9 +17,6 @@ namespace {
 
 using namespace head;
 
-// Rows: sums over them, and what is requested ahead of them, are counted in 32 bits.
-constexpr int kMaxIn = 1 << 20, kMaxOut = 1 << 28, kMaxRows = 0x7fffffff - (1 << 22) + 1;
-
 template <typename T, int C>
 __device__ __forceinline__ void finish(const ProductParams& p, long long i, int j, int n, const float* bias, Columns<T, C> residual, float* z) {
     if constexpr (std::is_same_v<T, _Float16>) {

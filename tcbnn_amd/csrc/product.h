@@ -12,6 +12,9 @@
 namespace tcbnn {
 namespace head {
 
+// Rows: sums over them, and what is requested ahead of them, are counted in 32 bits.
+constexpr int kMaxIn = 1 << 20, kMaxOut = 1 << 28, kMaxRows = 0x7fffffff - (1 << 22) + 1;
+
 // ---- activations.  fp32 uses the library's erf and exp.  In 16-bit types, whose rounding is 2^-9 or 2^-12 of a result, they
 // cost as much as a quarter of a large product; there exp is 2^x of the hardware, a quotient its reciprocal (each good to
 // one unit in the last place of fp32), and the normal distribution's tail
@@ -130,7 +133,7 @@ struct Tile {
     static_assert(kEach * THREADS == kPieces, "whole pieces a thread");
 
     const T* base;
-    const T* second;  // PAIRED: the same place of the second matrix
+    long long apart;  // PAIRED: elements between a place of the first matrix and the same place of the second
     int offset[kEach];  // bytes from the tile's first element in memory, at the first step
     Words held[SLOTS][ACCESS == WHOLE_PIECES ? 1 : kEach];
     long long ld;
@@ -151,7 +154,7 @@ struct Tile {
     static __device__ __forceinline__ int source(int row) { return PAIRED ? row / (2 * kPairedRows) * kPairedRows + row % kPairedRows : row; }
     __device__ __forceinline__ const T* matrix(int e) const {
         if constexpr (!PAIRED) return base;
-        return (e * THREADS + wave_first()) / (8 * kPairedRows) % 2 ? second : base;
+        return base + ((e * THREADS + wave_first()) / (8 * kPairedRows) % 2 ? apart : 0);  // (a choice of pointers would put the tile into memory)
     }
     // rows first .. of `total` rows (i or j; of each matrix).  What lies past the last row is some other row's: nothing of it is kept.
     __device__ __forceinline__ void init(const Operand& o, long long first, long long total) {
@@ -161,7 +164,7 @@ struct Tile {
         // columns than that: offsets count from there and are never negative.
         const int lead = ACROSS && ACCESS == ANYWHERE ? max(0, V - valid) : 0;
         base = (const T*)o.p + (ACROSS ? first - lead : first * ld);
-        if constexpr (PAIRED) second = base + total * ld;
+        if constexpr (PAIRED) apart = total * ld;
         if constexpr (ACCESS != ELEMENTS) {
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {

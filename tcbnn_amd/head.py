@@ -248,6 +248,146 @@ class LayerNormLayerParam(_HeadLayer):
         return self._download(self.output_gpu, self.rows, self.features)
 
 
+class GatedLayerParam(_HeadLayer):
+    """output = act(gate) * up with [gate up] = input * weight^T + bias; input [rows][in_features], weight [2 * features]
+    [in_features], the gate's rows first, output [rows][features]."""
+
+    def __init__(self, name, rows, in_features, features, dtype="f32", activation="silu"):
+        super().__init__(name, dtype)
+        if activation not in _lib.ACTIVATIONS:
+            raise _lib.TcbnnError("Error: %s: unknown activation %r" % (name, activation))
+        self.rows, self.in_features, self.features, self.activation = rows, in_features, features, activation
+
+    def initialize(self, weight, bias, input_gpu, output_gpu=None, preact_gpu=None, save_preact=False):
+        """save_preact: keep [gate up], which backward() needs, in a buffer of the layer's own (or give `preact_gpu`,
+        [rows][2 * features])."""
+        self._forget()
+        m, k, n, dt = self.rows, self.in_features, self.features, self.dtype
+        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", (m, k), dt)
+        self.weight_gpu = self._sized(self._parameter(self._required(weight, "weight"), dt, (2 * n, k)), "weight", (2 * n, k), dt)
+        self.bias_gpu = self._sized(self._parameter(bias, "f32", (2 * n,)), "bias", (2 * n,), "f32")
+        self.output_gpu = self._sized(output_gpu if output_gpu is not None else self._buffer(m * n * ITEMSIZE[dt]), "output", (m, n), dt)
+        if preact_gpu is None and save_preact:
+            preact_gpu = self._buffer(2 * m * n * ITEMSIZE[dt])
+        self.preact_gpu = self._sized(preact_gpu, "preact", (m, 2 * n), dt)
+        self._desc = _lib.GatedDesc(
+            self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), self.output_gpu.ptr, _ptr(self.preact_gpu), m, k, n,
+            _lib.DTYPES[dt], _lib.ACTIVATIONS[self.activation], _ld(self.input_gpu), _ld(self.weight_gpu), _ld(self.output_gpu),
+            _ld(self.preact_gpu))
+        self._forward = self._call(lib.tcbnn_gated_forward, self._desc)
+        return self
+
+    def initialize_backward(self, grad_output_gpu, grad_input_gpu=None, grad_weight_gpu=None, grad_bias_gpu=None):
+        """After initialize().  Gradients are written where a buffer is given."""
+        m, k, n, dt = self.rows, self.in_features, self.features, self.dtype
+        self._required(self.preact_gpu, "preact")
+        self.grad_output_gpu = self._sized(self._required(grad_output_gpu, "grad_output"), "grad_output", (m, n), dt)
+        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", (m, k), dt)
+        self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", (2 * n, k), dt)
+        self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", (2 * n,), "f32")
+        nbytes = lib.tcbnn_gated_grad_workspace_bytes(m, k, n, _lib.DTYPES[dt])
+        ws = self._grad_buffer(nbytes)
+        self._grad_desc = _lib.GatedGradDesc(
+            self.input_gpu.ptr, self.weight_gpu.ptr, self.preact_gpu.ptr, self.grad_output_gpu.ptr, _ptr(grad_input_gpu),
+            _ptr(grad_weight_gpu), _ptr(grad_bias_gpu), m, k, n, _lib.DTYPES[dt], _lib.ACTIVATIONS[self.activation],
+            _ld(self.input_gpu), _ld(self.weight_gpu), _ld(self.preact_gpu), _ld(grad_output_gpu), _ld(grad_input_gpu),
+            _ld(grad_weight_gpu), _ptr(ws), nbytes)
+        self._backward = self._call(lib.tcbnn_gated_backward, self._grad_desc)
+        return self
+
+    def get_output_gpu(self):
+        return self.output_gpu
+
+    def download_output(self):
+        """fp32 [rows][features] of a buffer without gaps between rows."""
+        return self._download(self.output_gpu, self.rows, self.features)
+
+
+class BlockNormLayerParam(_HeadLayer):
+    """The norms after and before a block, with the residual stream between them:
+    new_stream = stream + scale * gate * norm_after(block);  output = norm_before(new_stream).
+
+    `after` and `before` are "rms", "layer" or "none".  Without a block the stream stays as it is (the norm before a first
+    block)."""
+
+    def __init__(self, name, rows, features, dtype="f32", after="none", before="rms", scale=1.0, eps=1e-5):
+        super().__init__(name, dtype)
+        for kind in (after, before):
+            if kind not in _lib.NORMS:
+                raise _lib.TcbnnError("Error: %s: unknown norm %r" % (name, kind))
+        self.rows, self.features, self.after, self.before, self.scale, self.eps = rows, features, after, before, scale, eps
+
+    def initialize(self, stream_gpu, block_gpu=None, gate=None, after_gamma=None, after_beta=None, before_gamma=None,
+                   before_beta=None, new_stream_gpu=None, output_gpu=None, after_mean_gpu=None, after_rstd_gpu=None,
+                   before_mean_gpu=None, before_rstd_gpu=None):
+        """`new_stream_gpu` may be `stream_gpu`.  gate, gammas and betas are fp32 [features]; a beta belongs to a layer norm."""
+        self._forget()
+        m, n, dt = self.rows, self.features, self.dtype
+        self.stream_gpu = self._sized(self._required(stream_gpu, "stream"), "stream", (m, n), dt)
+        self.block_gpu = self._sized(block_gpu, "block", (m, n), dt)
+        self.gate_gpu, self.after_gamma_gpu, self.after_beta_gpu, self.before_gamma_gpu, self.before_beta_gpu = (
+            self._sized(self._parameter(p, "f32", (n,)), what, (n,), "f32")
+            for p, what in ((gate, "gate"), (after_gamma, "after_gamma"), (after_beta, "after_beta"),
+                            (before_gamma, "before_gamma"), (before_beta, "before_beta")))
+
+        def matrix(buf, what, wanted):
+            return self._sized(buf if buf is not None or not wanted else self._buffer(m * n * ITEMSIZE[dt]), what, (m, n), dt)
+
+        def statistic(buf, what, wanted):
+            return self._sized(buf if buf is not None or not wanted else self._buffer(4 * m), what, (m,), "f32")
+
+        written = matrix(new_stream_gpu, "new_stream", block_gpu is not None)
+        self.new_stream_gpu = self.stream_gpu if written is None else written
+        self.output_gpu = matrix(output_gpu, "output", self.before != "none")
+        self.after_mean_gpu = statistic(after_mean_gpu, "after_mean", self.after == "layer")
+        self.after_rstd_gpu = statistic(after_rstd_gpu, "after_rstd", self.after != "none")
+        self.before_mean_gpu = statistic(before_mean_gpu, "before_mean", self.before == "layer")
+        self.before_rstd_gpu = statistic(before_rstd_gpu, "before_rstd", self.before != "none")
+        self._desc = _lib.BlockNormDesc(
+            self.stream_gpu.ptr, _ptr(self.block_gpu), _ptr(self.gate_gpu), _ptr(self.after_gamma_gpu), _ptr(self.after_beta_gpu),
+            _ptr(self.before_gamma_gpu), _ptr(self.before_beta_gpu), _ptr(written), _ptr(self.output_gpu), _ptr(self.after_mean_gpu),
+            _ptr(self.after_rstd_gpu), _ptr(self.before_mean_gpu), _ptr(self.before_rstd_gpu), m, n, _lib.DTYPES[dt],
+            _lib.NORMS[self.after], _lib.NORMS[self.before], self.scale, self.eps, _ld(self.stream_gpu), _ld(self.block_gpu),
+            _ld(written), _ld(self.output_gpu))
+        self._forward = self._call(lib.tcbnn_blocknorm_forward, self._desc)
+        return self
+
+    def initialize_backward(self, grad_output_gpu=None, grad_new_stream_gpu=None, grad_stream_gpu=None, grad_block_gpu=None,
+                            grad_gate_gpu=None, grad_after_gamma_gpu=None, grad_after_beta_gpu=None, grad_before_gamma_gpu=None,
+                            grad_before_beta_gpu=None):
+        """After initialize().  Of the first two, None counts as 0; the other gradients are written where a buffer is given.
+        The new stream and the statistics are those of forward()."""
+        m, n, dt = self.rows, self.features, self.dtype
+        self.grad_output_gpu, self.grad_new_stream_gpu, self.grad_stream_gpu, self.grad_block_gpu = (
+            self._sized(buf, what, (m, n), dt)
+            for buf, what in ((grad_output_gpu, "grad_output"), (grad_new_stream_gpu, "grad_new_stream"),
+                              (grad_stream_gpu, "grad_stream"), (grad_block_gpu, "grad_block")))
+        self.grad_gate_gpu, self.grad_after_gamma_gpu, self.grad_after_beta_gpu, self.grad_before_gamma_gpu, self.grad_before_beta_gpu = (
+            self._sized(buf, what, (n,), "f32")
+            for buf, what in ((grad_gate_gpu, "grad_gate"), (grad_after_gamma_gpu, "grad_after_gamma"),
+                              (grad_after_beta_gpu, "grad_after_beta"), (grad_before_gamma_gpu, "grad_before_gamma"),
+                              (grad_before_beta_gpu, "grad_before_beta")))
+        nbytes = lib.tcbnn_blocknorm_grad_workspace_bytes(m, n, _lib.DTYPES[dt])
+        ws = self._grad_buffer(nbytes)
+        self._grad_desc = _lib.BlockNormGradDesc(
+            self.new_stream_gpu.ptr, _ptr(self.block_gpu), _ptr(self.gate_gpu), _ptr(self.after_gamma_gpu), _ptr(self.after_beta_gpu),
+            _ptr(self.before_gamma_gpu), _ptr(self.after_mean_gpu), _ptr(self.after_rstd_gpu), _ptr(self.before_mean_gpu),
+            _ptr(self.before_rstd_gpu), _ptr(grad_output_gpu), _ptr(grad_new_stream_gpu), _ptr(grad_stream_gpu), _ptr(grad_block_gpu),
+            _ptr(grad_gate_gpu), _ptr(grad_after_gamma_gpu), _ptr(grad_after_beta_gpu), _ptr(grad_before_gamma_gpu),
+            _ptr(grad_before_beta_gpu), m, n, _lib.DTYPES[dt], _lib.NORMS[self.after], _lib.NORMS[self.before], self.scale,
+            _ld(self.new_stream_gpu), _ld(self.block_gpu), _ld(grad_output_gpu), _ld(grad_new_stream_gpu), _ld(grad_stream_gpu),
+            _ld(grad_block_gpu), _ptr(ws), nbytes)
+        self._backward = self._call(lib.tcbnn_blocknorm_backward, self._grad_desc)
+        return self
+
+    def get_output_gpu(self):
+        return self.output_gpu
+
+    def download_output(self):
+        """fp32 [rows][features] of a buffer without gaps between rows."""
+        return self._download(self._required(self.output_gpu, "output"), self.rows, self.features)
+
+
 class LogProbsLayerParam(_HeadLayer):
     """Of every row of logits: log probability and rank of a given class, entropy, the `top` best classes."""
 
