@@ -646,6 +646,54 @@ typedef struct tcbnn_logprobs_grad_desc {
 } tcbnn_logprobs_grad_desc;
 int tcbnn_logprobs_backward(const tcbnn_logprobs_grad_desc* d, void* stream);
 
+/* The softmax cross entropy of a linear classifier, which keeps no logits: z = input * weight^T + bias, of every row logsumexp =
+ * log(sum exp(z_j)) and loss = logsumexp - z_t of the given class t = targets[row].  Logits are in fp32 and are not rounded.
+ *   t < 0        : a row without a class: loss 0.   t >= classes: loss NaN.
+ *   bias_j = -inf: a forbidden class; z_t = -inf: loss +inf; every z_j = -inf: logsumexp -inf.
+ *   NaN, +inf    : the row's logsumexp and loss are NaN.
+ * `workspace` holds tcbnn_linear_loss_workspace_bytes.  rows <= 2^31 - 2^22, in_features <= 1048576, classes <= 2^28. */
+typedef struct tcbnn_linear_loss_desc {
+    const void* input;       /* [rows][in_features]      */
+    const void* weight;      /* [classes][in_features]   */
+    const float* bias;       /* [classes], or NULL       */
+    const int32_t* targets;  /* [rows]; NULL where loss is */
+    float* loss;             /* [rows], or NULL          */
+    float* logsumexp;        /* [rows], or NULL          */
+    int rows, in_features, classes;
+    int dtype;
+    long long input_ld, weight_ld;
+    void* workspace;
+    size_t workspace_bytes;
+} tcbnn_linear_loss_desc;
+size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, int classes, int dtype);
+int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream);
+
+/* The gradient of sum over rows of grad_loss * loss.  With d_j = grad_loss * (exp(z_j - logsumexp) - [j = t]), and d = 0 in rows without
+ * a class and in rows whose classes are all forbidden (t >= classes: NaN):  grad_input = d * weight, grad_weight = d^T * input,
+ * grad_bias = sums of d over the rows.  Each of the three may be NULL; what is given is overwritten.  The logits are made again, a piece
+ * of the classes at a time; in 16-bit types d is rounded to dtype before the two products (in f16 times a power of two that keeps small
+ * ones from getting lost); grad_bias sums it unrounded.  `logsumexp` is the forward call's; exp carries its rounding, |logsumexp| 2^-24.
+ * A row without a class still has to hold finite inputs: grad_weight sums 0 times them.  `workspace` holds
+ * tcbnn_linear_loss_grad_workspace_bytes. */
+typedef struct tcbnn_linear_loss_grad_desc {
+    const void* input;       /* [rows][in_features]      */
+    const void* weight;      /* [classes][in_features]   */
+    const float* bias;       /* [classes], or NULL       */
+    const int32_t* targets;  /* [rows]                   */
+    const float* logsumexp;  /* [rows]                   */
+    const float* grad_loss;  /* [rows]                   */
+    void* grad_input;        /* [rows][in_features]      */
+    void* grad_weight;       /* [classes][in_features]   */
+    float* grad_bias;        /* [classes]                */
+    int rows, in_features, classes;
+    int dtype;
+    long long input_ld, weight_ld, grad_input_ld, grad_weight_ld;
+    void* workspace;
+    size_t workspace_bytes;
+} tcbnn_linear_loss_grad_desc;
+size_t tcbnn_linear_loss_grad_workspace_bytes(int rows, int in_features, int classes, int dtype);
+int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, void* stream);
+
 /* ------------------------------------------------ standalone GEMM / conv */
 /* C[m][n] = K - 2*popc(A[m,:] xor B[n,:]), int32 row major [M][N].  A: [K/32][M]
  * (tcbnn_pack_rows output), B: [N][K/32] (tcbnn_pack_cols output: each column of the

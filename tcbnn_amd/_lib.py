@@ -153,6 +153,22 @@ class GatedGradDesc(C.Structure):
                 ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
+class LinearLossDesc(C.Structure):
+    _fields_ = [("input", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("targets", c_void_p),
+                ("loss", c_void_p), ("logsumexp", c_void_p), ("rows", c_int), ("in_features", c_int),
+                ("classes", c_int), ("dtype", c_int), ("input_ld", C.c_longlong), ("weight_ld", C.c_longlong),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class LinearLossGradDesc(C.Structure):
+    _fields_ = [("input", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("targets", c_void_p),
+                ("logsumexp", c_void_p), ("grad_loss", c_void_p), ("grad_input", c_void_p),
+                ("grad_weight", c_void_p), ("grad_bias", c_void_p), ("rows", c_int), ("in_features", c_int),
+                ("classes", c_int), ("dtype", c_int), ("input_ld", C.c_longlong), ("weight_ld", C.c_longlong),
+                ("grad_input_ld", C.c_longlong), ("grad_weight_ld", C.c_longlong), ("workspace", c_void_p),
+                ("workspace_bytes", c_size_t)]
+
+
 class LogProbsDesc(C.Structure):
     _fields_ = [("logits", c_void_p), ("targets", c_void_p), ("logprob", c_void_p), ("entropy", c_void_p),
                 ("logsumexp", c_void_p), ("rank", c_void_p), ("top_index", c_void_p), ("top_logprob", c_void_p),
@@ -231,6 +247,10 @@ ABI = {
     "tcbnn_gated_kernel_name": (c_int, [C.POINTER(GatedDesc), C.c_char_p, c_size_t]),
     "tcbnn_gated_grad_workspace_bytes": (c_size_t, [c_int] * 4),
     "tcbnn_gated_backward": (c_int, [C.POINTER(GatedGradDesc), c_void_p]),
+    "tcbnn_linear_loss_workspace_bytes": (c_size_t, [c_int] * 4),
+    "tcbnn_linear_loss_forward": (c_int, [C.POINTER(LinearLossDesc), c_void_p]),
+    "tcbnn_linear_loss_grad_workspace_bytes": (c_size_t, [c_int] * 4),
+    "tcbnn_linear_loss_backward": (c_int, [C.POINTER(LinearLossGradDesc), c_void_p]),
     "tcbnn_logprobs_workspace_bytes": (c_size_t, [c_int] * 4),
     "tcbnn_logprobs_forward": (c_int, [C.POINTER(LogProbsDesc), c_void_p]),
     "tcbnn_logprobs_backward": (c_int, [C.POINTER(LogProbsGradDesc), c_void_p]),

@@ -238,7 +238,7 @@ int launch_gated(const ProductParams& p, hipStream_t stream) {
         TCBNN_LAUNCH_CHECK("gated_few_rows_kernel");
         return TCBNN_OK;
     }
-    auto go = [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
+    by_tile(g.access, g.plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
         constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value, H = hold.value;
         constexpr bool L = keep.value;
         constexpr int kThreads = 64 * WI * WJ * WS;
@@ -255,37 +255,7 @@ int launch_gated(const ProductParams& p, hipStream_t stream) {
             hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, L>),
                                dim3((unsigned)((long long)q.tiles_i * q.tiles_j)), dim3(kThreads), 0, stream, q);
         }
-    };
-    constexpr std::integral_constant<int, 256> n256;
-    constexpr std::integral_constant<int, 128> n128;
-    constexpr std::integral_constant<int, 64> n64;
-    constexpr std::integral_constant<int, 32> n32;
-    constexpr std::integral_constant<int, 1> one;
-    constexpr std::integral_constant<int, 2> two;
-    constexpr std::integral_constant<int, 4> four;
-    constexpr std::integral_constant<int, 8> eight;
-    constexpr std::true_type yes;
-    constexpr std::false_type no;
-    constexpr std::integral_constant<Access, WHOLE_PIECES> pieces;
-    constexpr std::integral_constant<Access, ANYWHERE> anywhere;
-    constexpr std::integral_constant<Access, ELEMENTS> elements;
-    if (g.access == WHOLE_PIECES) {
-        switch (g.plan.cut) {
-            case CUT_256: go(n256, two, four, one, two, pieces, one, no); break;
-            case CUT_128: go(n128, two, two, one, two, pieces, one, no); break;
-            case CUT_128_DEEP: go(n128, two, two, two, four, pieces, one, no); break;
-            case CUT_64: go(n64, two, two, two, four, pieces, one, no); break;
-            default: go(n32, one, one, four, eight, pieces, one, no); break;
-        }
-    } else if (g.access == ANYWHERE) {
-        switch (g.plan.cut) {
-            case CUT_128: go(n128, two, two, one, two, anywhere, one, no); break;
-            case CUT_64: go(n64, two, two, two, two, anywhere, four, no); break;
-            default: go(n32, one, one, four, two, anywhere, four, yes); break;
-        }
-    } else {
-        go(n32, one, one, four, two, elements, one, no);
-    }
+    });
     TCBNN_LAUNCH_CHECK("gated_product_kernel");
     return TCBNN_OK;
 }

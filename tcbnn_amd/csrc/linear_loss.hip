@@ -1,0 +1,584 @@
+// The softmax cross entropy of a linear classifier without its logits (tcbnn_linear_loss_forward / _backward):  z = x w^T + b,
+// logsumexp = log sum exp z_j,  loss = logsumexp - z_t;  d_j = dloss (exp(z_j - logsumexp) - [j = t]),  dx = d w,  dw = d^T x,  db = column sums of d.
+//
+// Forward, a tile of z stays in the registers that its sums end in: what leaves is the largest logit m of a row of the tile and the sum of
+// exp(z - m), 8 bytes for a tile's width of logits, and z_t from the one lane that has it.  A second launch joins them.
+// Backward, z is made again, a piece of the classes at a time, and becomes d where it lies; d goes to the workspace in the operands' type and from
+// there through two products.  dx is summed over the pieces in fp32.  With pieces of kPieceBytes that are read back from the cache, four products
+// (8 rows classes inputs operations a step) are nearly all of the time.
+#include "product.h"
+
+namespace tcbnn {
+namespace {
+
+using namespace head;
+
+struct LossParams {
+    const int32_t* targets;
+    float2* parts;          // [parts][rows_there] largest logit, sum of exponentials about it
+    float* given;           // [rows] z_t
+    long long rows_there;
+};
+struct LossGradParams {
+    const int32_t* targets;
+    const float *lse, *dloss, *scale;  // (scale: of d in f16)
+    float* sums;                       // [tiles of i][cols], or NULL
+    int first, classes;                // the piece's first class
+};
+
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+// exp(m - to) s: what a sum of exponentials about m is about `to`, m <= to
+__device__ __forceinline__ float about(float m, float s, float to) { return m == to ? s : s * exp_fast(m - to); }
+// f(v, v of the lane 32 away)
+template <typename F>
+__device__ __forceinline__ float across_halves(float v, F f) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float((uint32_t)a[0]), __uint_as_float((uint32_t)a[1]));
+}
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+
+// bias added to a wavefront's sums; what lies past the last column is -inf.  Register v of lane l is column 8 (v / 4) + 4 (l / 32) + v % 4 of a piece of 32.
+template <int NI, int NJ>
+__device__ __forceinline__ void add_bias(Acc (&acc)[NI][NJ], const ProductParams& p, long long j0, int lane) {
+#pragma unroll
+    for (int b = 0; b < NJ; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const long long j = j0 + 32 * b + 8 * q + 4 * (lane >> 5);
+            if (p.bias) {
+                const Columns<float, 4> c = get_columns<float, 4>(p.bias, 0, 0, (int)j, (int)min(4LL, p.cols - j));
+#pragma unroll
+                for (int a = 0; a < NI; ++a)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[a][b][4 * q + e] += c[e];
+            }
+            if (j0 + 32 * NJ > p.cols) {
+#pragma unroll
+                for (int a = 0; a < NI; ++a)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[a][b][4 * q + e] = j + e < p.cols ? acc[a][b][4 * q + e] : -INFINITY;
+            }
+        }
+}
+
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG>
+__global__ __launch_bounds__(64 * WI * WJ * WS) void loss_product_kernel(const ProductParams p, const LossParams l) {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
+    __shared__ __align__(1024) char lds[product_lds<BI, BJ, WI, WJ, WS, STAGES>()];
+    constexpr int NI = BI / WI / 32, NJ = BJ / WJ / 32;
+    Acc acc[NI][NJ];
+    Spot spot;
+    product_sums<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, LONG, false, false>(p, blockIdx.x, lds, acc, spot);
+    join_shares<WI, WJ, WS>(acc, lds, spot);
+    float2* rows = reinterpret_cast<float2*>(lds);  // [WJ][BI]
+    if (spot.share == 0) {
+        const long long j0 = spot.j0 + spot.wj;
+        add_bias(acc, p, j0, spot.lane);
+#pragma unroll
+        for (int a = 0; a < NI; ++a) {
+            const int row = spot.wi + 32 * a + (spot.lane & 31);
+            float m = -INFINITY, s = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[a][b][v]);
+            m = across_halves(m, larger);
+            const float c = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s += exp_fast(acc[a][b][v] - c);
+            s = across_halves(s, add);
+            if (spot.lane < 32) rows[spot.wj / (32 * NJ) * BI + row] = make_float2(m, s);
+            const long long i = spot.i0 + row;
+            const long long t = l.targets && i < p.rows ? l.targets[i] - j0 : -1;
+            if (__any(t >= 0 && t < 32 * NJ && t + j0 < p.cols)) {
+                const int at = (int)(t - 4 * (spot.lane >> 5));
+#pragma unroll
+                for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (t >= 0 && t + j0 < p.cols && at == 32 * b + 8 * (v / 4) + v % 4) l.given[i] = acc[a][b][v];
+            }
+        }
+    }
+    __syncthreads();
+    for (int row = threadIdx.x; row < BI; row += 64 * WI * WJ * WS) {
+        float2 r = rows[row];
+#pragma unroll
+        for (int w = 1; w < WJ; ++w) {
+            const float2 o = rows[w * BI + row];
+            const float m = fmaxf(r.x, o.x);
+            r = make_float2(m, about(r.x, r.y, m) + about(o.x, o.y, m));
+        }
+        if (spot.i0 + row < p.rows) l.parts[spot.tile_j * l.rows_there + spot.i0 + row] = r;
+    }
+#endif
+}
+
+// few rows: a wavefront's 16 classes are a part
+template <typename T, int SHARES>
+__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 4))) void loss_few_rows_kernel(const ProductParams p, const LossParams l) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = wave % SHARES;
+    const long long part = (long long)blockIdx.x * (kFewWaves / SHARES) + wave / SHARES, j0 = part * kFewOutputs;
+    // rows past the last one are read as the last one; nothing of them is kept
+    const T* w = (const T*)p.j.p + min(j0 + (lane & 15), (long long)p.cols - 1) * p.j.ld;
+    const T* x = (const T*)p.i.p + (long long)min(lane & 15, p.rows - 1) * p.i.ld;
+    Acc4 acc = few_rows_sums<T, SHARES>(p, w, x);
+    if (share != 0 || j0 >= p.cols) return;
+    const int i = lane & 15;
+    const long long j = j0 + 4 * (lane >> 4);
+    const int t = l.targets && i < p.rows ? l.targets[i] : -1;
+    float m = -INFINITY, s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        acc[e] = j + e < p.cols ? acc[e] + (p.bias ? p.bias[j + e] : 0.0f) : -INFINITY;
+        if (j + e == t && j + e < p.cols) l.given[i] = acc[e];
+        m = fmaxf(m, acc[e]);
+    }
+    m = __uint_as_float(across_rows(__float_as_uint(m), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+    const float c = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += exp_fast(acc[e] - c);
+    s = __uint_as_float(across_rows(__float_as_uint(s), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+    if (lane < 16 && i < p.rows) l.parts[part * l.rows_there + i] = make_float2(m, s);
+}
+
+// A row's parts joined, always in the same order: R rows a workgroup side by side, 1024 / R threads to a row.
+constexpr int kLossJoinThreads = 1024;
+template <int R>
+__global__ __launch_bounds__(kLossJoinThreads) void loss_join_kernel(const LossParams l, float* __restrict__ loss, float* __restrict__ lse, int rows,
+                                                                     int classes, int parts) {
+    constexpr int kStep = kLossJoinThreads / R, kWaves = kLossJoinThreads / 64;
+    static_assert(R == 1 || R == 32, "");
+    __shared__ float2 lds[kWaves][R];
+    const int r = threadIdx.x % R, first = threadIdx.x / R;
+    for (long long row0 = (long long)blockIdx.x * R; row0 < rows; row0 += (long long)gridDim.x * R) {
+        const long long row = min(row0 + r, (long long)rows - 1);
+        float m = -INFINITY, s = 0.0f;
+        for (int k = first; k < parts; k += 4 * kStep) {
+            float2 v[4];  // (requests of their own, one wait)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = k + u * kStep < parts ? l.parts[(long long)(k + u * kStep) * l.rows_there + row] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float to = fmaxf(m, v[u].x);
+                s = about(m, s, to) + about(v[u].x, v[u].y, to);
+                m = to;
+            }
+        }
+        const float to = R == 1 ? wave_max(m) : across_halves(m, larger);
+        s = about(m, s, to);
+        s = R == 1 ? wave_sum(s) : across_halves(s, add);
+        if ((threadIdx.x & 63) < R) lds[threadIdx.x >> 6][r] = make_float2(to, s);
+        __syncthreads();
+        if (first == 0 && row0 + r < rows) {
+            m = -INFINITY;
+            s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds[w][r].x);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) s += about(lds[w][r].x, lds[w][r].y, m);
+            const float log_s = logf(s);
+            const bool none = m == -INFINITY && s == 0.0f;  // every class is forbidden
+            if (lse) lse[row] = none ? -INFINITY : m + log_s;
+            if (loss) {
+                const int t = l.targets[row];
+                loss[row] = t < 0 ? 0.0f : t >= classes ? NAN : none ? INFINITY : (m - l.given[row]) + log_s;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- gradient
+// A power of two that brings the largest |dloss| to 2^14 .. 2^15: d is no larger, and what is 2^-28 of it is still a normal number in f16.
+// scale[0] is the factor, scale[1] its inverse.
+constexpr int kScaleThreads = 1024;
+__global__ __launch_bounds__(kScaleThreads) void loss_scale_kernel(const float* __restrict__ dloss, const int32_t* __restrict__ targets, float* __restrict__ scale, int rows) {
+    __shared__ float lds[kScaleThreads / 64];
+    float m = 0.0f;
+    for (long long i = threadIdx.x; i < rows; i += kScaleThreads) {
+        const float g = fabsf(dloss[i]);
+        if (targets[i] >= 0 && g < INFINITY) m = fmaxf(m, g);
+    }
+    m = wave_max(m);
+    lds[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kScaleThreads / 64; ++w) m = fmaxf(m, lds[w]);
+        const int e = m > 0.0f ? min(14 - ilogbf(m), 120) : 0;
+        scale[0] = ldexpf(1.0f, e);
+        scale[1] = ldexpf(1.0f, -e);
+    }
+}
+
+// the sum over the 32 lanes of a half, in the lanes whose number ends in 0
+__device__ __forceinline__ float half_sum(float v) {
+    v += __uint_as_float(dpp<kSwapPairs>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<kSwapTwos>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<kMirrorHalf>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<kMirrorRow>(__float_as_uint(v)));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((uint32_t)a[0]) + __uint_as_float((uint32_t)a[1]);
+}
+
+// d of a piece of the classes: p.out [rows][out_ld], the columns behind the last one of 16 bytes 0
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG>
+__global__ __launch_bounds__(64 * WI * WJ * WS) void loss_grad_product_kernel(const ProductParams p, const LossGradParams l) {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
+    __shared__ __align__(1024) char lds[product_lds<BI, BJ, WI, WJ, WS, STAGES>()];
+    constexpr int NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec, kThreads = 64 * WI * WJ * WS;
+    constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
+    Acc acc[NI][NJ];
+    Spot spot;
+    product_sums<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, LONG, false, false>(p, blockIdx.x, lds, acc, spot);
+    join_shares<WI, WJ, WS>(acc, lds, spot);
+    const int lane = spot.lane;
+    const long long j0 = spot.j0 + spot.wj;
+    if (spot.share == 0) {
+        add_bias(acc, p, j0, lane);
+#pragma unroll
+        for (int a = 0; a < NI; ++a) {
+            const long long i = spot.i0 + spot.wi + 32 * a + (lane & 31), row = min(i, (long long)p.rows - 1);
+            const int t = l.targets[row];
+            const float lse = l.lse[row];
+            const bool none = i >= p.rows || t < 0 || lse == -INFINITY;
+            const float g = t < l.classes ? l.dloss[row] : NAN;
+#pragma unroll
+            for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[a][b][v] = none ? 0.0f : g * exp_fast(acc[a][b][v] - lse);
+            const long long at = (long long)t - l.first - j0 - 4 * (lane >> 5);
+            if (__any(!none && at >= 0 && at < 32 * NJ)) {
+#pragma unroll
+                for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (!none && at == 32 * b + 8 * (v / 4) + v % 4) acc[a][b][v] -= g;
+            }
+        }
+    }
+    if (l.sums) {
+        float* columns = reinterpret_cast<float*>(lds);  // [WI][BJ]
+        if (spot.share == 0) {
+#pragma unroll
+            for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float s[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[e] = acc[0][b][4 * q + e];
+#pragma unroll
+                        for (int a = 1; a < NI; ++a) s[e] += acc[a][b][4 * q + e];
+                        s[e] = half_sum(s[e]);
+                    }
+                    if ((lane & 31) == 0)
+                        *reinterpret_cast<float4*>(columns + spot.wi / (32 * NI) * BJ + spot.wj + 32 * b + 8 * q + 4 * (lane >> 5)) = make_float4(s[0], s[1], s[2], s[3]);
+                }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < BJ; c += kThreads) {
+            float s = columns[c];
+#pragma unroll
+            for (int w = 1; w < WI; ++w) s += columns[w * BJ + c];
+            if (spot.j0 + c < p.cols) l.sums[(long long)spot.tile_i * p.cols + spot.j0 + c] = s;
+        }
+        __syncthreads();
+    }
+    if (spot.share != 0) return;
+    // ---- out: 32 rows of the wavefront at a time through LDS, so that a row leaves in whole runs of 64 bytes or more
+    char* mine = lds + spot.wave * kOutWave;
+    constexpr int kPerRow = 32 * NJ / V, kRowsAtOnce = 64 / kPerRow < 32 ? 64 / kPerRow : 32, kTimes = 32 / kRowsAtOnce;
+    const int col = (lane % kPerRow) * V, row0 = lane / kPerRow % kRowsAtOnce;
+    const long long j = j0 + col;
+    const float scale = l.scale ? l.scale[0] : 1.0f;
+    const bool there = j < p.cols && lane / kPerRow < kRowsAtOnce;
+#pragma unroll 1
+    for (int a = 0; a < NI; ++a) {
+        const long long first = spot.i0 + spot.wi + 32 * a + row0;
+#pragma unroll
+        for (int k = 0; k < NI; ++k)  // (registers have no index: one of NI pieces of code)
+            if (k == a) {
+#pragma unroll
+                for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<float4*>(mine + (lane & 31) * kOutRow + (32 * b + 8 * q + 4 * (lane >> 5)) * 4) =
+                            make_float4(acc[k][b][4 * q], acc[k][b][4 * q + 1], acc[k][b][4 * q + 2], acc[k][b][4 * q + 3]);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int r = 0; r < kTimes; ++r) {
+            const long long i = first + r * kRowsAtOnce;
+            const char* from = mine + (row0 + r * kRowsAtOnce) * kOutRow + col * 4;
+            Vec<T> d;
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(from + e * 4);
+                d[e] = (T)(q.x * scale), d[e + 1] = (T)(q.y * scale), d[e + 2] = (T)(q.z * scale), d[e + 3] = (T)(q.w * scale);
+            }
+            if (j + V > p.cols) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[e] = j + e < p.cols ? d[e] : (T)0.0f;
+            }
+            if (there && i < p.rows) *reinterpret_cast<Vec<T>*>((T*)p.out + i * p.out_ld + j) = d;  // (rows of whole 16 bytes)
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#endif
+}
+
+// ---- plans
+// The forward call's kernel: its tile, or the one for few rows; the number of parts that it leaves of a row.
+struct LossPlan {
+    Plan plan;
+    bool few;
+    int parts;
+};
+inline LossPlan plan_loss(int rows, int classes, int sum, int size, Access access) {
+    const bool vectors = access == WHOLE_PIECES;
+    LossPlan l;
+    l.plan = plan_product(rows, classes, sum, size, vectors, 0);
+    l.few = rows <= kFewRows && (access == ELEMENTS || few_time(rows, classes, sum, size, vectors) < l.plan.time);
+    const int width = l.few ? kFewOutputs : access == ELEMENTS ? 32 : (vectors ? kCuts16 : kCutsAnywhere)[l.plan.cut].size;
+    l.parts = (classes - 1) / width + 1;
+    return l;
+}
+
+// A piece of the classes whose d is in the workspace at a time: as many as kPieceBytes hold, pieces of about the same size.
+constexpr size_t kPieceBytes = (size_t)256 << 20;
+constexpr int kPieceUnit = 256;
+inline int piece_classes(int rows, int classes, int size) {
+    const long long most = std::max<long long>(kPieceUnit, (long long)(kPieceBytes / ((size_t)rows * size)) / kPieceUnit * kPieceUnit);
+    if (classes <= most) return classes;
+    const long long pieces = (classes + most - 1) / most;
+    return (int)(((classes + pieces - 1) / pieces + kPieceUnit - 1) / kPieceUnit * kPieceUnit);
+}
+// elements between rows of d
+inline long long piece_ld(int piece, int size) { return ((long long)piece * size + 15) / 16 * 16 / size; }
+// The splits of dx's sum over a whole piece, where there are several.  Where the weights lie is not known when a workspace is asked for: the splits are
+// those of rows at whole 16 bytes, which are no fewer.
+inline int carried_splits(int rows, int in_features, int piece, int size) {
+    const int splits = plan_product(rows, in_features, piece, size, true, ~(size_t)0).splits;
+    const int steps = (int)(((long long)piece * size + kStepBytes - 1) / kStepBytes), each = (steps + splits - 1) / splits;
+    return (steps + each - 1) / each;  // (as cut_product cuts a whole piece: every part is written by the first)
+}
+
+struct LossWorkspace {
+    size_t scale, d, sums, dx, split, total;  // offsets, in order
+    int piece, splits;
+};
+inline LossWorkspace loss_workspace(int rows, int in_features, int classes, int dtype) {
+    const int size = (int)dtype_bytes(dtype);
+    LossWorkspace w = {};
+    w.piece = piece_classes(rows, classes, size);
+    const bool carried = w.piece < classes;
+    w.splits = carried ? carried_splits(rows, in_features, w.piece, size) : 1;
+    w.d = 256;
+    w.sums = w.d + whole_lines((size_t)rows * piece_ld(w.piece, size) * size);
+    w.dx = w.sums + whole_lines((size_t)((rows + 31) / 32) * w.piece * sizeof(float));
+    w.split = w.dx + (carried ? whole_lines((size_t)w.splits * rows * in_features * sizeof(float)) : 0);
+    w.total = w.split + gradient_product_bytes(rows, in_features, w.piece, dtype);
+    return w;
+}
+
+int check_loss(int rows, int in_features, int classes, int dtype) {
+    TCBNN_REQUIRE(dtype_known(dtype), "linear loss: unknown dtype");
+    TCBNN_REQUIRE(rows >= 0 && in_features > 0 && classes > 0, "linear loss: bad shape");
+    TCBNN_REQUIRE(rows <= kMaxRows, "linear loss: at most %d rows", kMaxRows);
+    TCBNN_REQUIRE(in_features <= kMaxIn, "linear loss: at most %d inputs", kMaxIn);
+    TCBNN_REQUIRE(classes <= kMaxOut, "linear loss: at most %d classes", kMaxOut);
+    return TCBNN_OK;
+}
+// rows that are so far apart that 32 bits do not hold a tile
+bool too_far(long long ld, int dtype) { return ld * 256 * (long long)dtype_bytes(dtype) > 0x7fffffffLL; }
+
+}  // namespace
+}  // namespace tcbnn
+
+using namespace tcbnn;
+using namespace tcbnn::head;
+
+extern "C" size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, int classes, int dtype) {
+    if (rows <= 0 || rows > kMaxRows || in_features <= 0 || in_features > kMaxIn || classes <= 0 || classes > kMaxOut || !dtype_known(dtype)) return 0;
+    size_t parts = 0;
+    const int size = (int)dtype_bytes(dtype);
+    for (Access access : {WHOLE_PIECES, ANYWHERE, ELEMENTS})  // (where the operands will lie is not known here)
+        if ((access == ELEMENTS) == (in_features * size < 16)) parts = std::max(parts, (size_t)plan_loss(rows, classes, in_features, size, access).parts);
+    return whole_lines(parts * rows * sizeof(float2)) + (size_t)rows * sizeof(float);
+}
+
+extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream) {
+    TCBNN_NOTNULL(d);
+    if (int rc = check_loss(d->rows, d->in_features, d->classes, d->dtype)) return rc;
+    ProductParams p = {};
+    p.i = {d->input, row_stride(d->input_ld, d->in_features)};
+    p.j = {d->weight, row_stride(d->weight_ld, d->in_features)};
+    TCBNN_REQUIRE(p.i.ld > 0 && p.j.ld > 0, "linear loss: rows overlap");
+    TCBNN_REQUIRE(!too_far(p.i.ld, d->dtype) && !too_far(p.j.ld, d->dtype), "linear loss: rows too far apart");
+    if (d->rows == 0 || (!d->loss && !d->logsumexp)) return TCBNN_OK;
+    TCBNN_NOTNULL(d->input);
+    TCBNN_NOTNULL(d->weight);
+    if (d->loss) TCBNN_NOTNULL(d->targets);
+    TCBNN_NOTNULL(d->workspace);
+    TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "linear loss: the workspace is not aligned to 16 bytes");
+    TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_linear_loss_workspace_bytes(d->rows, d->in_features, d->classes, d->dtype), "linear loss: workspace too small");
+    p.rows = d->rows;
+    p.cols = d->classes;
+    p.sum = d->in_features;
+    p.bias = d->bias;
+    hipStream_t s = (hipStream_t)stream;
+    return by_dtype(d->dtype, [&](auto type) -> int {
+        using T = decltype(type);
+        const Access access = access_of<T, false, false>(p);
+        const LossPlan plan = plan_loss(p.rows, p.cols, p.sum, (int)sizeof(T), access);
+        LossParams l = {d->loss ? d->targets : nullptr, (float2*)d->workspace, (float*)((char*)d->workspace + whole_lines((size_t)plan.parts * p.rows * sizeof(float2))),
+                        p.rows};
+        if (plan.few) {
+            const int shares = few_shares(p.cols, p.sum, (int)sizeof(T)), outputs = kFewOutputs * kFewWaves / shares;
+            const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
+            if (shares == 8)
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_few_rows_kernel<T, 8>), grid, dim3(64 * kFewWaves), 0, s, p, l);
+            else
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_few_rows_kernel<T, 2>), grid, dim3(64 * kFewWaves), 0, s, p, l);
+        } else {
+            by_tile(access, plan.plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
+                constexpr int B = size.value, kThreads = 64 * wi.value * wj.value * ws.value;
+                // rows beyond a launch's threads have one of their own
+                const long long at_once = std::max(1LL, kMaxThreads / kThreads / plan.parts) * B;
+                for (long long first = 0; first < p.rows; first += at_once) {
+                    ProductParams q = p;
+                    LossParams part = l;
+                    q.rows = (int)std::min(at_once, p.rows - first);
+                    q.i.p = (const T*)p.i.p + first * p.i.ld;
+                    part.targets = l.targets ? l.targets + first : nullptr;
+                    part.parts += first;
+                    part.given += first;
+                    cut_product(q, B, kStepBytes / (int)sizeof(T), 1, nullptr);
+                    hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_product_kernel<T, B, B, wi.value, wj.value, ws.value, stages.value, how.value, hold.value, keep.value>),
+                                       dim3((unsigned)((long long)q.tiles_i * q.tiles_j)), dim3(kThreads), 0, s, q, part);
+                }
+            });
+        }
+        TCBNN_LAUNCH_CHECK("loss_product_kernel");
+        if (p.rows <= kFewRows)
+            hipLaunchKernelGGL(loss_join_kernel<1>, dim3((unsigned)p.rows), dim3(kLossJoinThreads), 0, s, l, d->loss, d->logsumexp, p.rows, p.cols, plan.parts);
+        else
+            hipLaunchKernelGGL(loss_join_kernel<32>, dim3((unsigned)std::min((p.rows + 31LL) / 32, kMaxThreads / kLossJoinThreads)), dim3(kLossJoinThreads), 0, s, l,
+                               d->loss, d->logsumexp, p.rows, p.cols, plan.parts);
+        TCBNN_LAUNCH_CHECK("loss_join_kernel");
+        return TCBNN_OK;
+    });
+}
+
+extern "C" size_t tcbnn_linear_loss_grad_workspace_bytes(int rows, int in_features, int classes, int dtype) {
+    if (rows <= 0 || rows > kMaxRows || in_features <= 0 || in_features > kMaxIn || classes <= 0 || classes > kMaxOut || !dtype_known(dtype)) return 0;
+    return loss_workspace(rows, in_features, classes, dtype).total;
+}
+
+extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, void* stream) {
+    TCBNN_NOTNULL(d);
+    if (int rc = check_loss(d->rows, d->in_features, d->classes, d->dtype)) return rc;
+    const long long x_ld = row_stride(d->input_ld, d->in_features), w_ld = row_stride(d->weight_ld, d->in_features),
+                    dx_ld = row_stride(d->grad_input_ld, d->in_features), dw_ld = row_stride(d->grad_weight_ld, d->in_features);
+    TCBNN_REQUIRE(x_ld > 0 && w_ld > 0 && dx_ld > 0 && dw_ld > 0, "linear loss: rows overlap");
+    TCBNN_REQUIRE(!too_far(x_ld, d->dtype) && !too_far(w_ld, d->dtype), "linear loss: rows too far apart");
+    if (!d->grad_input && !d->grad_weight && !d->grad_bias) return TCBNN_OK;
+    hipStream_t s = (hipStream_t)stream;
+    if (d->rows == 0) {  // the parameters' gradients are sums of nothing
+        ProductParams dx = {}, dw = {};
+        dw.rows = d->classes;
+        dw.cols = d->in_features;
+        dw.i.ld = d->classes;
+        dw.j.ld = x_ld;
+        dw.out = d->grad_weight;
+        dw.out_ld = dw_ld;
+        if (d->grad_bias) launch_column_join(nullptr, d->grad_bias, 0, d->classes, s);
+        TCBNN_LAUNCH_CHECK("column_join_kernel");
+        return launch_gradient_products(d->dtype, dx, dw, nullptr, 0, s);
+    }
+    TCBNN_NOTNULL(d->input);
+    TCBNN_NOTNULL(d->weight);
+    TCBNN_NOTNULL(d->targets);
+    TCBNN_NOTNULL(d->logsumexp);
+    TCBNN_NOTNULL(d->grad_loss);
+    TCBNN_NOTNULL(d->workspace);
+    TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "linear loss: the workspace is not aligned to 16 bytes");
+    const LossWorkspace w = loss_workspace(d->rows, d->in_features, d->classes, d->dtype);
+    TCBNN_REQUIRE(d->workspace_bytes >= w.total, "linear loss: workspace too small");
+    char* base = (char*)d->workspace;
+    float* scale = d->dtype == TCBNN_F16 ? (float*)base : nullptr;
+    if (scale) hipLaunchKernelGGL(loss_scale_kernel, dim3(1), dim3(kScaleThreads), 0, s, d->grad_loss, d->targets, scale, d->rows);
+    const bool carried = w.piece < d->classes;
+    return by_dtype(d->dtype, [&](auto type) -> int {
+        using T = decltype(type);
+        ProductParams dx = {};
+        for (int first = 0; first < d->classes; first += w.piece) {
+            const int classes = std::min(w.piece, d->classes - first);
+            const T* weight = (const T*)d->weight + first * w_ld;
+            ProductParams p = {};
+            p.i = {d->input, x_ld};
+            p.j = {weight, w_ld};
+            p.rows = d->rows;
+            p.cols = classes;
+            p.sum = d->in_features;
+            p.bias = d->bias ? d->bias + first : nullptr;
+            p.out = base + w.d;
+            p.out_ld = piece_ld(w.piece, (int)sizeof(T));
+            const LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes};
+            const Access access = access_of<T, false, false>(p);
+            const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0);
+            int tiles_i = 0;
+            by_tile(access, plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
+                constexpr int B = size.value, kThreads = 64 * wi.value * wj.value * ws.value;
+                tiles_i = (p.rows - 1) / B + 1;
+                // rows beyond a launch's threads have one of their own
+                const long long tiles_j = (p.cols - 1) / B + 1, at_once = std::max(1LL, kMaxThreads / kThreads / tiles_j) * B;
+                for (long long row = 0; row < p.rows; row += at_once) {
+                    ProductParams q = p;
+                    LossGradParams part = l;
+                    q.rows = (int)std::min(at_once, p.rows - row);
+                    q.i.p = (const T*)p.i.p + row * p.i.ld;
+                    q.out = (T*)p.out + row * p.out_ld;
+                    part.targets += row;
+                    part.lse += row;
+                    part.dloss += row;
+                    if (part.sums) part.sums += row / B * p.cols;
+                    cut_product(q, B, kStepBytes / (int)sizeof(T), 1, nullptr);
+                    hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_grad_product_kernel<T, B, B, wi.value, wj.value, ws.value, stages.value, how.value, hold.value, keep.value>),
+                                       dim3((unsigned)((long long)q.tiles_i * q.tiles_j)), dim3(kThreads), 0, s, q, part);
+                }
+            });
+            if (d->grad_bias) launch_column_join(l.sums, d->grad_bias + first, tiles_i, classes, s);
+            TCBNN_LAUNCH_CHECK("loss_grad_product_kernel");
+            ProductParams dw = {};
+            dx.i = dw.i = {p.out, p.out_ld};
+            dx.padded = dw.padded = classes >= Elem<T>::kVec;
+            dx.factor = dw.factor = scale ? scale + 1 : nullptr;
+            dx.j = {weight, w_ld};
+            dx.rows = d->rows;
+            dx.cols = d->in_features;
+            dx.sum = classes;
+            dx.out = d->grad_input;
+            dx.out_ld = dx_ld;
+            if (carried) {
+                dx.carry = first == 0 ? CARRY_FIRST : CARRY_ON;
+                dx.splits = w.splits;
+                dx.partial = (float*)(base + w.dx);
+                dx.partial_stride = (long long)d->rows * d->in_features;
+            }
+            dw.j = {d->input, x_ld};
+            dw.rows = classes;
+            dw.cols = d->in_features;
+            dw.sum = d->rows;
+            dw.out = d->grad_weight ? (T*)d->grad_weight + first * dw_ld : nullptr;
+            dw.out_ld = dw_ld;
+            if (int rc = launch_gradient_products(d->dtype, dx, dw, (float*)(base + w.split), w.total - w.split, s)) return rc;
+        }
+        if (carried && d->grad_input) return launch_carried_sum(d->dtype, dx, s);
+        return TCBNN_OK;
+    });
+}

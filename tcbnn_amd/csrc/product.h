@@ -322,6 +322,7 @@ struct ProductParams {
     long long partial_stride;  // from one split's to the next one's
     int carry;             // the sum goes on in `partial`: CARRY_FIRST writes it, CARRY_ON adds to what is there
     const float* factor;   // of the sums, or NULL (a power of two: nothing is rounded by it)
+    bool padded;           // I's rows, 16 bytes or more, go on with zeros to whole 16 bytes
 };
 enum Carry : int { NO_CARRY, CARRY_FIRST, CARRY_ON };
 
@@ -400,7 +401,8 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
 
     TileI ti;
     TileJ tj;
-    ti.init(p.i, i0, p.rows);
+    constexpr int V = Elem<T>::kVec;
+    ti.init(p.i, i0, ACROSS_I && p.padded ? ((long long)p.rows + V - 1) / V * V : (long long)p.rows);
     tj.init(p.j, j0, p.cols);
     const int s0 = split * p.split_sum, s1 = min(p.sum, s0 + p.split_sum);
     const int share = wave / (WI * WJ), wi = wave / WJ % WI * (32 * NI), wj = wave % WJ * (32 * NJ);
@@ -730,12 +732,45 @@ inline float few_time(int rows, int cols, int sum, int size, bool vectors) {
 
 template <typename T, bool ACROSS_I, bool ACROSS_J>
 Access access_of(const ProductParams& p) {
-    auto of = [](const Operand& o, int rows, int sum, bool across) {
-        const int row = across ? rows : sum;
+    auto of = [](const Operand& o, int rows, int sum, bool across, bool padded) {
+        int row = across ? rows : sum;
+        if (padded) row = (row + Elem<T>::kVec - 1) / Elem<T>::kVec * Elem<T>::kVec;
         if (row < Elem<T>::kVec || o.ld * 256 * (long long)sizeof(T) > 0x7fffffffLL) return ELEMENTS;
         return (uintptr_t)o.p % 16 == 0 && o.ld * sizeof(T) % 16 == 0 && row % Elem<T>::kVec == 0 ? WHOLE_PIECES : ANYWHERE;
     };
-    return std::max(of(p.i, p.rows, p.sum, ACROSS_I), of(p.j, p.cols, p.sum, ACROSS_J));
+    return std::max(of(p.i, p.rows, p.sum, ACROSS_I, p.padded), of(p.j, p.cols, p.sum, ACROSS_J, false));
+}
+// f(tile, wavefronts of i, of j, of the sum, stages, access, steps held, long sums) with the constants of a tile's kernel (product_sums)
+template <typename F>
+void by_tile(Access access, Cut cut, F&& f) {
+    constexpr std::integral_constant<int, 256> n256;
+    constexpr std::integral_constant<int, 128> n128;
+    constexpr std::integral_constant<int, 64> n64;
+    constexpr std::integral_constant<int, 32> n32;
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 4> four;
+    constexpr std::integral_constant<int, 8> eight;
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    constexpr std::integral_constant<Access, WHOLE_PIECES> pieces;
+    constexpr std::integral_constant<Access, ANYWHERE> anywhere;
+    constexpr std::integral_constant<Access, ELEMENTS> elements;
+    if (access == WHOLE_PIECES) {
+        switch (cut) {
+            case CUT_256: return f(n256, two, four, one, two, pieces, one, no);
+            case CUT_128: return f(n128, two, two, one, two, pieces, one, no);
+            case CUT_128_DEEP: return f(n128, two, two, two, four, pieces, one, no);
+            case CUT_64: return f(n64, two, two, two, four, pieces, one, no);
+            default: return f(n32, one, one, four, eight, pieces, one, no);
+        }
+    }
+    if (access == ELEMENTS) return f(n32, one, one, four, two, elements, one, no);
+    switch (cut) {
+        case CUT_128: return f(n128, two, two, one, two, anywhere, one, no);
+        case CUT_64: return f(n64, two, two, two, two, anywhere, four, no);
+        default: return f(n32, one, one, four, two, anywhere, four, yes);
+    }
 }
 inline void cut_product(ProductParams& p, int size, int steps_size, int splits, float* workspace) {
     p.tiles_i = (p.rows + size - 1) / size;
@@ -745,6 +780,40 @@ inline void cut_product(ProductParams& p, int size, int steps_size, int splits, 
     p.splits = std::max(1, (p.sum + p.split_sum - 1) / p.split_sum);
     p.partial = workspace;
     p.partial_stride = (long long)p.rows * p.cols;
+}
+
+// The sums of wavefronts that shared a tile's sum, in those of share 0; all of the workgroup call it.
+template <int WI, int WJ, int WS, int NI, int NJ>
+__device__ __forceinline__ void join_shares(Acc (&acc)[NI][NJ], char* lds, const Spot& spot) {
+    if constexpr (WS > 1) {
+        float4* mine = reinterpret_cast<float4*>(lds) + spot.wave % (WI * WJ) * (4 * NI * NJ * 64) + spot.lane;
+        constexpr int kShare = WI * WJ * 4 * NI * NJ * 64;
+        if (spot.share > 0) {
+#pragma unroll
+            for (int a = 0; a < NI; ++a)
+#pragma unroll
+                for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        mine[(spot.share - 1) * kShare + ((a * NJ + b) * 4 + q) * 64] =
+                            make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
+        }
+        __syncthreads();
+        if (spot.share == 0) {
+#pragma unroll
+            for (int w = 0; w + 1 < WS; ++w)
+#pragma unroll
+                for (int a = 0; a < NI; ++a)
+#pragma unroll
+                    for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float4 o = mine[w * kShare + ((a * NJ + b) * 4 + q) * 64];
+                            acc[a][b][4 * q] += o.x, acc[a][b][4 * q + 1] += o.y, acc[a][b][4 * q + 2] += o.z, acc[a][b][4 * q + 3] += o.w;
+                        }
+        }
+        __syncthreads();
+    }
 }
 
 // ---- passes over an output's gradient (dz): a thread has one vector of 16 bytes of columns and goes down its share of the rows; the workgroups' column

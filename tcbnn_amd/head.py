@@ -449,6 +449,55 @@ class LogProbsLayerParam(_HeadLayer):
         return out
 
 
+class LinearLossLayerParam(_HeadLayer):
+    """loss = logsumexp(z) - z[target] of every row of z = input * weight^T + bias: the softmax cross entropy of a linear
+    classifier that keeps no logits; input [rows][in_features], weight [classes][in_features]."""
+
+    def __init__(self, name, rows, in_features, classes, dtype="f32"):
+        super().__init__(name, dtype)
+        self.rows, self.in_features, self.classes = rows, in_features, classes
+
+    def initialize(self, weight, bias, input_gpu, targets_gpu, loss_gpu=None, logsumexp_gpu=None):
+        """targets: int32 [rows], -1 for rows without a class (loss 0, no gradient)."""
+        self._forget()
+        m, k, n, dt = self.rows, self.in_features, self.classes, self.dtype
+        self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", (m, k), dt)
+        self.weight_gpu = self._sized(self._parameter(self._required(weight, "weight"), dt, (n, k)), "weight", (n, k), dt)
+        self.bias_gpu = self._sized(self._parameter(bias, "f32", (n,)), "bias", (n,), "f32")
+        self.targets_gpu = self._sized(self._required(targets_gpu, "targets"), "targets", (m,), "i32")
+        self.loss_gpu, self.logsumexp_gpu = (
+            self._sized(buf if buf is not None else self._buffer(4 * m), what, (m,), "f32")
+            for buf, what in ((loss_gpu, "loss"), (logsumexp_gpu, "logsumexp")))
+        nbytes = lib.tcbnn_linear_loss_workspace_bytes(m, k, n, _lib.DTYPES[dt])
+        ws = self._buffer(nbytes) if nbytes else None
+        self._desc = _lib.LinearLossDesc(
+            self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), self.targets_gpu.ptr, self.loss_gpu.ptr,
+            self.logsumexp_gpu.ptr, m, k, n, _lib.DTYPES[dt], _ld(self.input_gpu), _ld(self.weight_gpu), _ptr(ws), nbytes)
+        self._forward = self._call(lib.tcbnn_linear_loss_forward, self._desc)
+        return self
+
+    def initialize_backward(self, grad_loss_gpu, grad_input_gpu=None, grad_weight_gpu=None, grad_bias_gpu=None):
+        """After initialize().  grad_loss: fp32 [rows] (1 / n for the mean of n rows).  Gradients are written where a buffer is
+        given; logsumexp is that of forward()."""
+        m, k, n, dt = self.rows, self.in_features, self.classes, self.dtype
+        self.grad_loss_gpu = self._sized(self._required(grad_loss_gpu, "grad_loss"), "grad_loss", (m,), "f32")
+        self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", (m, k), dt)
+        self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", (n, k), dt)
+        self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", (n,), "f32")
+        nbytes = lib.tcbnn_linear_loss_grad_workspace_bytes(m, k, n, _lib.DTYPES[dt])
+        ws = self._grad_buffer(nbytes)
+        self._grad_desc = _lib.LinearLossGradDesc(
+            self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), self.targets_gpu.ptr, self.logsumexp_gpu.ptr,
+            self.grad_loss_gpu.ptr, _ptr(grad_input_gpu), _ptr(grad_weight_gpu), _ptr(grad_bias_gpu), m, k, n, _lib.DTYPES[dt],
+            _ld(self.input_gpu), _ld(self.weight_gpu), _ld(grad_input_gpu), _ld(grad_weight_gpu), _ptr(ws), nbytes)
+        self._backward = self._call(lib.tcbnn_linear_loss_backward, self._grad_desc)
+        return self
+
+    def download_output(self):
+        """dict of the host arrays of what forward() wrote."""
+        return {"loss": self.loss_gpu.to_numpy(np.float32, (self.rows,)), "logsumexp": self.logsumexp_gpu.to_numpy(np.float32, (self.rows,))}
+
+
 class FloatHead:
     """A float head on `features` values a row, as on the last binary layer of a network:
     norm -> linear (GELU), + the features where there are as many hidden values -> norm -> linear -> log probabilities of

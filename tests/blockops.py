@@ -104,3 +104,55 @@ def norms_grad(stream, block, gate, ag, ab, bg, stats, dy, ds, after, before, sc
     out["after_gamma"] = scale * gate * A, np.abs(scale * gate) * (Aerr + 4 * U * np.abs(A))
     out["after_beta"] = scale * gate * B, np.abs(scale * gate) * (Berr + 4 * U * np.abs(B))
     return out
+
+
+def loss(x, w, b, t, g=None):
+    """Loss, logsumexp and (g given) {name: (gradient, its error)}, with the errors of the first two, of fp32 logits; rows of finite logits, or
+    whose bias forbids classes (-inf)."""
+    k, n = x.shape[1], len(w)
+    bias = 0.0 if b is None else b
+    z = x @ w.T + bias
+    shared = np.where(np.isfinite(bias), np.abs(bias), 0.0)
+    zerr = (k + 1) * U * (np.abs(x) @ np.abs(w).T + shared)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        m = z.max(1)
+        safe = np.where(m == -np.inf, 0.0, m)
+        e = np.exp(z - safe[:, None])
+        lse = safe + np.log(e.sum(1))
+        p = np.exp(z - np.where(lse == -np.inf, 0.0, lse)[:, None])
+        given = (t >= 0) & (t < n)
+        at = np.where(given, t, 0)
+        zt, rows = z[np.arange(len(x)), at], np.arange(len(x))
+        out = np.where(t < 0, 0.0, np.where(t >= n, np.nan, np.where(zt == -np.inf, np.inf, lse - zt)))
+    # exp's argument is off by its rounding and by the logits' error, exp by some units, the sum by one a term; the logarithm by that relative error
+    far = np.where(np.isfinite(z), np.abs(z - safe[:, None]), 0.0)
+    rel = zerr + U * (4 * far + 6)
+    serr = (p * rel).sum(1) + (n + 8) * U
+    lse_err = 1.1 * (serr + 4 * U * (np.abs(np.where(np.isfinite(lse), lse, 0)) + np.abs(np.log(n + 1.0))))
+    loss_err = lse_err + zerr[rows, at] + 4 * U * (np.abs(safe - np.where(np.isfinite(zt), zt, safe)) + np.log(n + 1.0))
+    if g is None:
+        return out, loss_err, lse, lse_err
+    return out, loss_err, lse, lse_err, z, zerr, p
+
+
+def loss_grads(x, w, t, g, z, zerr, p, lse, lse_err, dtype):
+    """{name: (gradient, error)}: d as the products read it is off by its own rounding and by what its logits and logsumexp are off by"""
+    m, k = x.shape
+    n = len(w)
+    none = (t < 0) | (lse == -np.inf)
+    g = np.where(none, 0.0, g)
+    one = np.zeros((m, n))
+    one[np.arange(m), np.where(t < 0, 0, t)] = 1.0
+    d = g[:, None] * (p - one)
+    zabs = np.where(np.isfinite(z), np.abs(z), 0.0)
+    derr = np.abs(g)[:, None] * (p * (zerr + lse_err[:, None] + U * (4 * zabs + 4 * np.abs(np.where(np.isfinite(lse), lse, 0))[:, None] + 6)) + U * np.abs(p - one)) * 1.1
+    # f16: d is scaled, so that what lies below the normal numbers is less than 2^-38 of the largest |g|
+    tiny = {"f32": 2.0 ** -126, "bf16": 2.0 ** -126, "f16": 2.0 ** -38 * np.abs(g).max()}[dtype]
+    used = derr + ho.U[dtype] * (np.abs(d) + derr) + tiny
+    out = {}
+    terms, exact = np.abs(d) @ np.abs(w), d @ w
+    out["input"] = exact, used @ np.abs(w) + (n + 32) * U * 1.01 * terms
+    terms, exact = np.abs(d).T @ np.abs(x), d.T @ x
+    out["weight"] = exact, used.T @ np.abs(x) + m * U * 1.01 * terms
+    out["bias"] = d.sum(0), derr.sum(0) + m * U * 1.01 * np.abs(d).sum(0)
+    return out

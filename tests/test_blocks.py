@@ -39,7 +39,29 @@ def _gated_grad(**kw):
     return "tcbnn_gated_backward", _lib().GatedGradDesc(**{**d, **kw})
 
 
+def _loss(**kw):
+    d = dict(input=P, weight=P, targets=P, loss=P, logsumexp=P, rows=4, in_features=8, classes=8, dtype=1, workspace=P, workspace_bytes=1 << 30)
+    return "tcbnn_linear_loss_forward", _lib().LinearLossDesc(**{**d, **kw})
+
+
+def _loss_grad(**kw):
+    d = dict(input=P, weight=P, targets=P, logsumexp=P, grad_loss=P, grad_input=P, grad_weight=P, grad_bias=P, rows=4, in_features=8, classes=8, dtype=1,
+             workspace=P, workspace_bytes=1 << 30)
+    return "tcbnn_linear_loss_backward", _lib().LinearLossGradDesc(**{**d, **kw})
+
+
 @pytest.mark.parametrize("make,change,code,message", [
+    (_loss, dict(dtype=3), EINVAL, "dtype"), (_loss, dict(rows=-1), EINVAL, "shape"), (_loss, dict(in_features=0), EINVAL, "shape"),
+    (_loss, dict(classes=0), EINVAL, "shape"), (_loss, dict(in_features=(1 << 20) + 1), EINVAL, "inputs"), (_loss, dict(classes=(1 << 28) + 1), EINVAL, "classes"),
+    (_loss, dict(rows=(1 << 31) - 1), EINVAL, "rows"), (_loss, dict(input_ld=7), EINVAL, "overlap"), (_loss, dict(weight_ld=-8), EINVAL, "overlap"),
+    (_loss, dict(weight_ld=1 << 23), EINVAL, "apart"), (_loss, dict(input_ld=1 << 40), EINVAL, "apart"), (_loss, dict(input=0), ENULL, "input"),
+    (_loss, dict(weight=0), ENULL, "weight"), (_loss, dict(targets=0), ENULL, "targets"), (_loss, dict(workspace=0), ENULL, "workspace"),
+    (_loss, dict(workspace=P + 8), EINVAL, "aligned"), (_loss, dict(workspace_bytes=16), EINVAL, "workspace"),
+    (_loss_grad, dict(dtype=-1), EINVAL, "dtype"), (_loss_grad, dict(rows=-3), EINVAL, "shape"), (_loss_grad, dict(grad_input_ld=4), EINVAL, "overlap"),
+    (_loss_grad, dict(grad_weight_ld=4), EINVAL, "overlap"), (_loss_grad, dict(weight_ld=1 << 23), EINVAL, "apart"), (_loss_grad, dict(input=0), ENULL, "input"),
+    (_loss_grad, dict(weight=0), ENULL, "weight"), (_loss_grad, dict(targets=0), ENULL, "targets"), (_loss_grad, dict(logsumexp=0), ENULL, "logsumexp"),
+    (_loss_grad, dict(grad_loss=0), ENULL, "grad_loss"), (_loss_grad, dict(workspace=0), ENULL, "workspace"),
+    (_loss_grad, dict(workspace=P + 4), EINVAL, "aligned"), (_loss_grad, dict(workspace_bytes=64), EINVAL, "workspace"),
     (_gated, dict(dtype=3), EINVAL, "dtype"), (_gated, dict(activation=4), EINVAL, "activation"), (_gated, dict(rows=-1), EINVAL, "shape"),
     (_gated, dict(in_features=0), EINVAL, "shape"), (_gated, dict(features=0), EINVAL, "shape"), (_gated, dict(in_features=(1 << 20) + 1), EINVAL, "inputs"),
     (_gated, dict(features=(1 << 27) + 1), EINVAL, "features"), (_gated, dict(rows=(1 << 31) - 1), EINVAL, "rows"),
@@ -87,9 +109,11 @@ def test_refusals(make, change, code, message):
 
 def test_no_rows_and_null_descriptors():
     lib = _lib().lib
-    for entry, d in (_norms(rows=0, stream_in=0, output=0), _gated(rows=0, input=0, output=0)):
+    for entry, d in (_norms(rows=0, stream_in=0, output=0), _gated(rows=0, input=0, output=0),
+                     _loss(rows=0, input=0, workspace=0), _loss(loss=0, logsumexp=0, input=0, workspace=0)):
         assert getattr(lib, entry)(C.byref(d), None) == 0
-    for entry in ("tcbnn_blocknorm_forward", "tcbnn_blocknorm_backward", "tcbnn_gated_forward", "tcbnn_gated_backward"):
+    for entry in ("tcbnn_blocknorm_forward", "tcbnn_blocknorm_backward", "tcbnn_gated_forward", "tcbnn_gated_backward",
+                  "tcbnn_linear_loss_forward", "tcbnn_linear_loss_backward"):
         assert getattr(lib, entry)(None, None) == ENULL
 
 
@@ -98,6 +122,8 @@ def test_workspaces_of_refused_sizes_are_empty():
     assert lib.tcbnn_blocknorm_grad_workspace_bytes(0, 8, 0) == lib.tcbnn_blocknorm_grad_workspace_bytes(4, 65537, 0) == 0
     assert lib.tcbnn_blocknorm_grad_workspace_bytes(4, 8, 5) == 0
     assert lib.tcbnn_gated_grad_workspace_bytes(0, 8, 8, 0) == lib.tcbnn_gated_grad_workspace_bytes(4, 8, 0, 0) == 0
+    for f in (lib.tcbnn_linear_loss_workspace_bytes, lib.tcbnn_linear_loss_grad_workspace_bytes):
+        assert f(0, 8, 8, 0) == f(4, 0, 8, 0) == f(4, 8, -1, 0) == f(4, 8, 8, 3) == f(4, (1 << 20) + 1, 8, 0) == f(4, 8, (1 << 28) + 1, 0) == 0
     assert lib.tcbnn_gated_grad_workspace_bytes(4, 8, (1 << 27) + 1, 0) == lib.tcbnn_gated_grad_workspace_bytes(4, 8, 8, 3) == 0
 
 
@@ -158,6 +184,45 @@ def test_gated_layer_refuses():
     layer.initialize(w, None, x, output_gpu=x)
     with pytest.raises(TcbnnError, match="preact"):
         layer.initialize_backward(x)
+
+
+def test_loss_layer_refuses():
+    from tcbnn_amd import head
+    from tcbnn_amd._lib import TcbnnError
+    from tcbnn_amd.device import DeviceView
+    layer = head.LinearLossLayerParam("loss", 4, 8, 16, "bf16")
+    x, w, t = DeviceView(P, 64), DeviceView(P, 256), DeviceView(P, 16)
+    with pytest.raises(TcbnnError, match="targets"):
+        layer.initialize(w, None, x, None)
+    with pytest.raises(TcbnnError, match="targets is i64"):
+        layer.initialize(w, None, x, DeviceView(P, 32, dtype="i64"))
+    with pytest.raises(TcbnnError, match="weight holds"):
+        layer.initialize(x, None, x, t)
+
+
+def test_loss_keeps_no_logits():
+    """Workspaces of a large vocabulary: forward 8 bytes a row and tile, backward a piece of the classes and the sum of the inputs' gradient."""
+    lib = _lib().lib
+    rows, classes = 8192, 131072
+    logits = 2 * rows * classes
+    assert lib.tcbnn_linear_loss_workspace_bytes(rows, 1024, classes, 1) < logits / 16
+    assert lib.tcbnn_linear_loss_grad_workspace_bytes(rows, 1024, classes, 1) < logits / 4
+
+
+def test_loss_gradient_is_the_definitions():
+    r = np.random.default_rng(6)
+    m, k, n = 4, 5, 9
+    x, w, b, g = r.standard_normal((m, k)), r.standard_normal((n, k)), r.standard_normal(n), r.standard_normal(m)
+    t = np.array([3, -1, 8, 0])
+
+    def total(x, w, b):
+        return (g * bo.loss(x, w, b, t)[0]).sum()
+
+    _, _, lse, lse_err, z, zerr, p = bo.loss(x, w, b, t, g)
+    got = bo.loss_grads(x, w, t, g, z, zerr, p, lse, lse_err, "f32")
+    for name, at in (("input", lambda v: total(x + v, w, b)), ("weight", lambda v: total(x, w + v, b)), ("bias", lambda v: total(x, w, b + v))):
+        v = r.standard_normal(got[name][0].shape)
+        assert abs((at(1e-5 * v) - at(-1e-5 * v)) / 2e-5 - (got[name][0] * v).sum()) < 1e-7, name
 
 
 @pytest.mark.parametrize("after", bo.KINDS)

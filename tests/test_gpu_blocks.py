@@ -1,5 +1,5 @@
-"""The gated block's operators on the GPU against definitions in 64 bits: the norms after and before a block, the gated product, and
-their gradients; sizes around those where the kernels change, odd sizes, strides, buffers over one another, empty and degenerate
+"""The gated block's operators on the GPU against definitions in 64 bits: the norms after and before a block, the gated product, the
+loss of a linear classifier, and their gradients; sizes around those where the kernels change, odd sizes, strides, buffers over one another, empty and degenerate
 inputs."""
 import numpy as np
 import pytest
@@ -331,6 +331,174 @@ def test_gated_without_rows(gpu):
     x, dw, db = ho.Matrix(None, "bf16", 0, 32, 8), ho.Matrix(None, "bf16", 0, 32, 8), ho.empty(32)
     layer = head.GatedLayerParam("gated", 0, 8, 16, "bf16").initialize(x.view, None, x.view, output_gpu=x.view, preact_gpu=x.view)
     layer.initialize_backward(x.view, x.view, dw.view, db)
+    layer.forward()
+    layer.backward()
+    ho.sync()
+    assert np.isnan(x.get()).all()
+    assert (dw.get() == 0).all() and (db.to_numpy(np.float32, (32,)) == 0).all()
+
+
+# --------------------------------------------------------------------------- linear loss
+# (rows, inputs, classes): one value; one row; a part of 16, a tile and one to each side; few rows and long sums; classes in several pieces are below
+LOSS = [(1, 1, 1), (1, 16, 10), (1, 4096, 512), (1, 1025, 3), (2, 8, 17), (3, 17, 5), (5, 1032, 1264), (7, 33, 1000), (16, 64, 16), (17, 72, 2), (31, 2048, 96),
+        (32, 256, 129), (33, 100, 127), (64, 4096, 48), (65, 65, 65), (77, 1023, 129), (128, 128, 128), (129, 136, 257), (256, 512, 1000), (300, 64, 7),
+        (255, 1000, 511), (513, 96, 300), (4, 1023, 4099), (1000, 1001, 999), (3, 5, 4000), (40, 7, 30), (9, 512, 16392), (2100, 64, 40)]
+
+
+def _loss(gpu, m, k, n, dtype, bias=True, gap=0, shift=1, stream=None, want=("input", "weight", "bias"), scale=1.0, forbidden=(), t=None, targets=True):
+    from tcbnn_amd import head
+    r = rng(m, k, n, len(dtype), 4)
+    wv = 2.5 * r.standard_normal((n, k)) / np.sqrt(k)
+    if t is None:
+        t = r.integers(0, n, m).astype(np.int32)
+        t[r.random(m) < 0.1] = -1
+    xv = r.standard_normal((m, k)) + np.where(r.random(m) < 0.5, 1.0, 0.0)[:, None] * wv[np.clip(t, 0, n - 1)]
+    x, w = ho.Matrix(xv, dtype, gap, shift=shift), ho.Matrix(wv, dtype, gap, shift=shift)
+    b = r.standard_normal(n).astype(np.float32) if bias else None
+    if len(forbidden):
+        b[forbidden] = -np.inf
+    g = (scale * (0.5 + r.random(m))).astype(np.float32)
+    dx, dw, db = ho.Matrix(None, dtype, gap, m, k), ho.Matrix(None, dtype, gap, n, k), ho.empty(n)
+    layer = head.LinearLossLayerParam("loss", m, k, n, dtype)
+    layer.initialize(w.view, b, x.view, ho.vector(t, np.int32))
+    layer.forward(stream)
+    ho.sync()
+    b64 = b.astype(np.float64) if bias else None
+    loss, loss_err, lse, lse_err, z, zerr, p = bo.loss(x.values, w.values, b64, t, g)
+    got = layer.download_output()
+    ho.check(got["logsumexp"], lse, lse_err, "logsumexp")
+    ho.check(got["loss"], loss, loss_err, "loss")
+    if want:
+        layer.initialize_backward(ho.vector(g), dx.view if "input" in want else None, dw.view if "weight" in want else None, db if "bias" in want else None)
+        layer.backward(stream)
+        ho.sync()
+        exact = bo.loss_grads(x.values, w.values, t, g.astype(np.float64), z, zerr, p, lse, lse_err, dtype)
+        for name, buf in (("input", dx), ("weight", dw)):
+            if name in want:
+                e, err = exact[name]
+                ho.check(buf.get(), e, bo.out_error(e, err, dtype), "grad of " + name)
+        if "bias" in want:
+            e, err = exact["bias"]
+            ho.check(db.to_numpy(np.float32, (n,)), e, 1.1 * err + ho.TINY["f32"], "grad of bias")
+    layer.release()
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n", LOSS)
+def test_loss(gpu, m, k, n, dtype):
+    _loss(gpu, m, k, n, dtype, bias=(m + k + n) % 3 > 0)
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 64, 40), (19, 128, 72), (130, 264, 136), (300, 61, 77), (40, 24, 1003)])
+def test_loss_strides_and_single_outputs(gpu, m, k, n, dtype):
+    _loss(gpu, m, k, n, dtype, gap=GAPS[dtype])
+    _loss(gpu, m, k, n, dtype, gap=8, shift=0)
+    for want in (("input",), ("weight",), ("bias",), ("weight", "bias"), ()):
+        _loss(gpu, m, k, n, dtype, want=want, shift=0)
+
+
+# rows at whole 16 bytes: every tile, whole and ragged
+@pytest.mark.parametrize("m,k,n", [(17, 1048, 36), (33, 8, 8), (100, 520, 304), (64, 2048, 2048), (1024, 512, 1024), (1000, 72, 1500), (2040, 136, 1020),
+                                   (2048, 512, 1024), (2040, 72, 2052), (2048, 64, 2048), (2000, 200, 2044)])
+def test_loss_of_whole_pieces(gpu, m, k, n):
+    for dtype in ho.DTYPES:
+        _loss(gpu, m, k, n, dtype, shift=0)
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+def test_loss_in_pieces(gpu, dtype, monkeypatch):
+    """Classes whose gradients the workspace does not hold at a time, the last piece a short one."""
+    from tcbnn_amd import _lib
+    m, k, n = 40000, 24, 1700 if dtype == "f32" else 3400
+    assert _lib.lib.tcbnn_linear_loss_grad_workspace_bytes(m, k, n, _lib.DTYPES[dtype]) < 1.4 * 2 ** 28
+    from tcbnn_amd import head
+    r = rng(n)
+    x, w = ho.Matrix(r.standard_normal((m, k)), dtype, shift=0), ho.Matrix(r.standard_normal((n, k)) / 4, dtype, shift=0)
+    t = r.integers(-1, n, m).astype(np.int32)
+    g = (0.5 + r.random(m)).astype(np.float32)
+    dx, dw, db = ho.Matrix(None, dtype, 0, m, k), ho.Matrix(None, dtype, 0, n, k), ho.empty(n)
+    layer = head.LinearLossLayerParam("loss", m, k, n, dtype).initialize(w.view, None, x.view, ho.vector(t, np.int32))
+    layer.initialize_backward(ho.vector(g), dx.view, dw.view, db)
+    layer.forward()
+    layer.backward()
+    ho.sync()
+    got, dxv, dwv, dbv = layer.download_output(), dx.get(), dw.get(), db.to_numpy(np.float32, (n,))
+    dw_exact = dw_err = db_exact = db_err = 0.0
+    for i in range(0, m, 4000):
+        rows = slice(i, i + 4000)
+        loss, loss_err, lse, lse_err, z, zerr, p = bo.loss(x.values[rows], w.values, None, t[rows], g[rows])
+        ho.check(got["loss"][rows], loss, loss_err, "loss")
+        e = bo.loss_grads(x.values[rows], w.values, t[rows], g[rows].astype(np.float64), z, zerr, p, lse, lse_err, dtype)
+        ho.check(dxv[rows], e["input"][0], bo.out_error(*e["input"], dtype), "grad of input")
+        dw_exact, dw_err = dw_exact + e["weight"][0], dw_err + 10 * e["weight"][1]  # (a sum ten times as long)
+        db_exact, db_err = db_exact + e["bias"][0], db_err + 10 * e["bias"][1]
+    ho.check(dwv, dw_exact, bo.out_error(dw_exact, dw_err, dtype), "grad of weight")
+    ho.check(dbv, db_exact, 1.1 * db_err, "grad of bias")
+    layer.release()
+
+
+def test_loss_of_forbidden_classes(gpu):
+    """A bias of -inf: no share in the sums, no gradient; a row whose class is forbidden."""
+    for dtype in ho.DTYPES:
+        for m, k, n in ((1, 64, 100), (12, 40, 700), (150, 72, 1000)):
+            r = rng(m, n)
+            t = r.integers(n // 2, n, m).astype(np.int32)
+            t[::5] = -1
+            _loss(gpu, m, k, n, dtype, forbidden=np.arange(n // 2), t=t)
+
+
+def test_loss_of_degenerate_rows(gpu):
+    """Every class forbidden; a forbidden class given; a class that there is not; a NaN and an infinite logit; rows without a class."""
+    from tcbnn_amd import head
+    for dtype in ho.DTYPES:
+        for m, k, n in ((8, 24, 40), (40, 24, 300)):
+            for all_forbidden in (False, True):
+                r = rng(m, n)
+                xv, wv = r.standard_normal((m, k)), r.standard_normal((n, k))
+                xv[0, 3], xv[1, 3] = np.nan, np.inf
+                wv[:, 3] = np.abs(wv[:, 3]) + 0.1
+                b = np.zeros(n, np.float32)
+                b[:3] = -np.inf
+                if all_forbidden:
+                    b[:] = -np.inf
+                    xv[:2] = 1.0
+                t = r.integers(3, n, m).astype(np.int32)
+                t[2], t[3], t[4], t[5] = 1, n, -1, -7
+                x, w = ho.Matrix(xv, dtype), ho.Matrix(wv, dtype)
+                dx = ho.Matrix(None, dtype, 0, m, k)
+                layer = head.LinearLossLayerParam("loss", m, k, n, dtype).initialize(w.view, b, x.view, ho.vector(t, np.int32))
+                layer.initialize_backward(ho.vector(np.ones(m)), dx.view)
+                layer.forward()
+                layer.backward()
+                ho.sync()
+                out, d = layer.download_output(), dx.get()
+                if all_forbidden:
+                    assert (out["logsumexp"] == -np.inf).all()
+                    want = np.full(m, np.inf)
+                    want[3], want[4:6] = np.nan, 0
+                    np.testing.assert_array_equal(out["loss"], want)
+                    d = np.delete(d, 3, 0)  # (a class that there is not is told by its loss)
+                    assert (d == 0).all()
+                    continue
+                assert np.isnan(out["loss"][:2]).all() and np.isnan(out["logsumexp"][:2]).all() and np.isnan(d[:2]).all()
+                assert out["loss"][2] == np.inf and np.isnan(out["loss"][3]) and np.isfinite(out["logsumexp"][2:]).all()
+                assert np.isnan(d[3]).all() and (out["loss"][4:6] == 0).all() and (d[4:6] == 0).all()
+                assert np.isfinite(out["loss"][6:]).all() and np.isfinite(d[6:]).all() and np.isfinite(d[2]).all()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -40, 2.0 ** -20, 1.0 / 8192, 100.0])
+def test_loss_gradients_of_any_size(gpu, scale):
+    """f16: what d is scaled by does not show, but in what leaves as f16."""
+    for dtype in ("f16", "bf16"):
+        _loss(gpu, 70, 64, 500, dtype, scale=scale)
+
+
+def test_loss_without_rows(gpu):
+    from tcbnn_amd import head
+    x, dw, db = ho.Matrix(None, "bf16", 0, 32, 8), ho.Matrix(None, "bf16", 0, 32, 8), ho.empty(32)
+    layer = head.LinearLossLayerParam("loss", 0, 8, 32, "bf16").initialize(x.view, None, x.view, ho.empty(1))
+    layer.initialize_backward(db, x.view, dw.view, db)
     layer.forward()
     layer.backward()
     ho.sync()
