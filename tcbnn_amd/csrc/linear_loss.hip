@@ -24,6 +24,7 @@ struct LossGradParams {
     const float *lse, *dloss, *scale;  // (scale: of d in f16)
     float* sums;                       // [tiles of i][cols], or NULL
     int first, classes;                // the piece's first class
+    long long low;                     // elements from d to what its rounding left of it, or 0
 };
 
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
@@ -192,6 +193,28 @@ __global__ __launch_bounds__(kLossJoinThreads) void loss_join_kernel(const LossP
     }
 }
 
+// ---- rows of the input in the workspace, at whole 16 bytes, `copies` times over
+constexpr int kPackThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kPackThreads) void loss_pack_kernel(const T* __restrict__ x, T* __restrict__ to, int rows, int n, int copies, long long x_ld,
+                                                                 long long to_ld) {
+    constexpr int V = Elem<T>::kVec;
+    const int vectors = (n + V - 1) / V;
+    for (long long at = (long long)blockIdx.x * kPackThreads + threadIdx.x; at < (long long)rows * vectors; at += (long long)gridDim.x * kPackThreads) {
+        const long long row = at / vectors;
+        const int i = (int)(at - row * vectors) * V;
+        const T* from = x + row * x_ld + i;
+        Vec<T> v;
+        if (i + V <= n) {
+            v = load_vec(from);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = i + e < n ? from[e] : (T)0.0f;
+        }
+        for (int c = 0; c < copies; ++c) *reinterpret_cast<Vec<T>*>(to + (row + (long long)c * rows) * to_ld + i) = v;
+    }
+}
+
 // ---- gradient
 // A power of two that brings the largest |dloss| to 2^14 .. 2^15: d is no larger, and what is 2^-28 of it is still a normal number in f16.
 // scale[0] is the factor, scale[1] its inverse.
@@ -325,6 +348,11 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void loss_grad_product_kernel(co
                 for (int e = 0; e < V; ++e) d[e] = j + e < p.cols ? d[e] : (T)0.0f;
             }
             if (there && i < p.rows) *reinterpret_cast<Vec<T>*>((T*)p.out + i * p.out_ld + j) = d;  // (rows of whole 16 bytes)
+            if (l.low) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[e] = j + e < p.cols ? (T)(*reinterpret_cast<const float*>(from + e * 4) * scale - (float)d[e]) : (T)0.0f;
+                if (there && i < p.rows) *reinterpret_cast<Vec<T>*>((T*)p.out + l.low + i * p.out_ld + j) = d;
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
@@ -361,26 +389,38 @@ inline int piece_classes(int rows, int classes, int size) {
 inline long long piece_ld(int piece, int size) { return ((long long)piece * size + 15) / 16 * 16 / size; }
 // The splits of dx's sum over a whole piece, where there are several.  Where the weights lie is not known when a workspace is asked for: the splits are
 // those of rows at whole 16 bytes, which are no fewer.
-inline int carried_splits(int rows, int in_features, int piece, int size) {
-    const int splits = plan_product(rows, in_features, piece, size, true, ~(size_t)0).splits;
+inline int carried_splits(int rows, int in_features, int piece, int size, int most) {
+    const int splits = std::min(most, plan_product(rows, in_features, piece, size, true, ~(size_t)0).splits);
     const int steps = (int)(((long long)piece * size + kStepBytes - 1) / kStepBytes), each = (steps + splits - 1) / splits;
     return (steps + each - 1) / each;  // (as cut_product cuts a whole piece: every part is written by the first)
 }
 
+// In 16 bits d is rounded before it is multiplied.  A row of d, and a column, is often little else than its given class' value, whose rounding then is that
+// of all that it is multiplied with.  Over many rows these errors, like those of the sums' other terms, come to sqrt 2 of what rounding the results
+// leaves (8192 rows bf16: 0.0024 of them, 0.0017 the rounding); a few rows may be off by twice that.  Up to kTwoPlaneRows rows, where the
+// products are bound by the weights' bytes, d is kept in two planes, its rounding and what that left: rows of their own in dx, summed
+// afterwards, and more rows to sum over in dw, where the input's rows are there twice.
+constexpr int kTwoPlaneRows = 128;
+inline int loss_planes(int rows, int dtype) { return dtype != TCBNN_F32 && rows <= kTwoPlaneRows ? 2 : 1; }
+
 struct LossWorkspace {
-    size_t scale, d, sums, dx, split, total;  // offsets, in order
-    int piece, splits;
+    size_t scale, x, d, sums, dx, split, total;  // offsets, in order
+    int planes, piece, splits;
+    bool carried;
 };
 inline LossWorkspace loss_workspace(int rows, int in_features, int classes, int dtype) {
     const int size = (int)dtype_bytes(dtype);
     LossWorkspace w = {};
+    w.planes = loss_planes(rows, dtype);
+    rows *= w.planes;
     w.piece = piece_classes(rows, classes, size);
-    const bool carried = w.piece < classes;
-    w.splits = carried ? carried_splits(rows, in_features, w.piece, size) : 1;
-    w.d = 256;
+    w.carried = w.piece < classes || w.planes > 1;
+    w.splits = w.carried ? carried_splits(rows, in_features, w.piece, size, kMaxSplits / w.planes) : 1;
+    w.x = 256;
+    w.d = w.x + whole_lines((size_t)rows * piece_ld(in_features, size) * size);
     w.sums = w.d + whole_lines((size_t)rows * piece_ld(w.piece, size) * size);
     w.dx = w.sums + whole_lines((size_t)((rows + 31) / 32) * w.piece * sizeof(float));
-    w.split = w.dx + (carried ? whole_lines((size_t)w.splits * rows * in_features * sizeof(float)) : 0);
+    w.split = w.dx + (w.carried ? whole_lines((size_t)w.splits * rows * in_features * sizeof(float)) : 0);
     w.total = w.split + gradient_product_bytes(rows, in_features, w.piece, dtype);
     return w;
 }
@@ -392,6 +432,16 @@ int check_loss(int rows, int in_features, int classes, int dtype) {
     TCBNN_REQUIRE(in_features <= kMaxIn, "linear loss: at most %d inputs", kMaxIn);
     TCBNN_REQUIRE(classes <= kMaxOut, "linear loss: at most %d classes", kMaxOut);
     return TCBNN_OK;
+}
+// Rows of the input that do not lie at whole 16 bytes while those of the weights do are copied first.
+template <typename T>
+bool apart(const Operand& o, int n) { return n % Elem<T>::kVec != 0 || (uintptr_t)o.p % 16 != 0 || o.ld * sizeof(T) % 16 != 0; }
+template <typename T>
+Operand pack(const Operand& x, void* to, int rows, int n, int copies, hipStream_t stream) {
+    const long long ld = piece_ld(n, (int)sizeof(T)), vectors = rows * (ld / Elem<T>::kVec);
+    hipLaunchKernelGGL(loss_pack_kernel<T>, dim3((unsigned)std::min((vectors + kPackThreads - 1) / kPackThreads, 8LL * kComputeUnits)), dim3(kPackThreads), 0, stream,
+                       (const T*)x.p, (T*)to, rows, n, copies, x.ld, ld);
+    return {to, ld};
 }
 // rows that are so far apart that 32 bits do not hold a tile
 bool too_far(long long ld, int dtype) { return ld * 256 * (long long)dtype_bytes(dtype) > 0x7fffffffLL; }
@@ -408,7 +458,7 @@ extern "C" size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, i
     const int size = (int)dtype_bytes(dtype);
     for (Access access : {WHOLE_PIECES, ANYWHERE, ELEMENTS})  // (where the operands will lie is not known here)
         if ((access == ELEMENTS) == (in_features * size < 16)) parts = std::max(parts, (size_t)plan_loss(rows, classes, in_features, size, access).parts);
-    return whole_lines(parts * rows * sizeof(float2)) + (size_t)rows * sizeof(float);
+    return whole_lines(parts * rows * sizeof(float2)) + whole_lines((size_t)rows * sizeof(float)) + (size_t)rows * piece_ld(in_features, size) * size;
 }
 
 extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream) {
@@ -433,6 +483,8 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(d->dtype, [&](auto type) -> int {
         using T = decltype(type);
+        if (p.rows > kFewRows && apart<T>(p.i, p.sum) && !apart<T>(p.j, p.sum))
+            p.i = pack<T>(p.i, (char*)d->workspace + d->workspace_bytes / 16 * 16 - (size_t)p.rows * piece_ld(p.sum, (int)sizeof(T)) * sizeof(T), p.rows, p.sum, 1, s);
         const Access access = access_of<T, false, false>(p);
         const LossPlan plan = plan_loss(p.rows, p.cols, p.sum, (int)sizeof(T), access);
         LossParams l = {d->loss ? d->targets : nullptr, (float2*)d->workspace, (float*)((char*)d->workspace + whole_lines((size_t)plan.parts * p.rows * sizeof(float2))),
@@ -512,23 +564,27 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
     char* base = (char*)d->workspace;
     float* scale = d->dtype == TCBNN_F16 ? (float*)base : nullptr;
     if (scale) hipLaunchKernelGGL(loss_scale_kernel, dim3(1), dim3(kScaleThreads), 0, s, d->grad_loss, d->targets, scale, d->rows);
-    const bool carried = w.piece < d->classes;
     return by_dtype(d->dtype, [&](auto type) -> int {
         using T = decltype(type);
         ProductParams dx = {};
+        Operand x = {d->input, x_ld};
+        const bool packed = apart<T>(x, d->in_features) && !apart<T>({d->weight, w_ld}, d->in_features);
+        if (packed || (w.planes > 1 && d->grad_weight)) x = pack<T>(x, base + w.x, d->rows, d->in_features, w.planes, s);
+        const long long d_ld = piece_ld(w.piece, (int)sizeof(T));
         for (int first = 0; first < d->classes; first += w.piece) {
             const int classes = std::min(w.piece, d->classes - first);
             const T* weight = (const T*)d->weight + first * w_ld;
             ProductParams p = {};
-            p.i = {d->input, x_ld};
+            p.i = x;
             p.j = {weight, w_ld};
             p.rows = d->rows;
             p.cols = classes;
             p.sum = d->in_features;
             p.bias = d->bias ? d->bias + first : nullptr;
             p.out = base + w.d;
-            p.out_ld = piece_ld(w.piece, (int)sizeof(T));
-            const LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes};
+            p.out_ld = d_ld;
+            const LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes,
+                                      w.planes > 1 ? d->rows * d_ld : 0};
             const Access access = access_of<T, false, false>(p);
             const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0);
             int tiles_i = 0;
@@ -559,26 +615,30 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             dx.padded = dw.padded = classes >= Elem<T>::kVec;
             dx.factor = dw.factor = scale ? scale + 1 : nullptr;
             dx.j = {weight, w_ld};
-            dx.rows = d->rows;
+            dx.rows = w.planes * d->rows;
             dx.cols = d->in_features;
             dx.sum = classes;
             dx.out = d->grad_input;
             dx.out_ld = dx_ld;
-            if (carried) {
+            if (w.carried) {
                 dx.carry = first == 0 ? CARRY_FIRST : CARRY_ON;
                 dx.splits = w.splits;
                 dx.partial = (float*)(base + w.dx);
-                dx.partial_stride = (long long)d->rows * d->in_features;
             }
-            dw.j = {d->input, x_ld};
+            dw.j = x;
             dw.rows = classes;
             dw.cols = d->in_features;
-            dw.sum = d->rows;
+            dw.sum = w.planes * d->rows;
             dw.out = d->grad_weight ? (T*)d->grad_weight + first * dw_ld : nullptr;
             dw.out_ld = dw_ld;
             if (int rc = launch_gradient_products(d->dtype, dx, dw, (float*)(base + w.split), w.total - w.split, s)) return rc;
         }
-        if (carried && d->grad_input) return launch_carried_sum(d->dtype, dx, s);
+        if (w.carried && d->grad_input) {
+            dx.rows = d->rows;
+            dx.splits = w.splits * w.planes;  // (a split's planes lie one behind the other)
+            dx.partial_stride = (long long)d->rows * d->in_features;
+            return launch_carried_sum(d->dtype, dx, s);
+        }
         return TCBNN_OK;
     });
 }
