@@ -41,7 +41,7 @@ __device__ __forceinline__ void finish(const ProductParams& p, long long i, int 
 }
 
 // A tile of a linear layer's product or of its gradients'
-template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG, bool ACROSS_I, bool ACROSS_J>
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG, bool ACROSS_I, bool ACROSS_J, bool PLANES>
 __device__ __forceinline__ void product(const ProductParams& p, int block, char* lds) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
     constexpr int NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec;
@@ -49,7 +49,7 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
     constexpr int kOutRow = 32 * NJ * 4 + 16, kOutWave = 32 * kOutRow;
     Acc acc[NI][NJ];
     Spot spot;
-    product_sums<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, LONG, ACROSS_I, ACROSS_J>(p, block, lds, acc, spot);
+    product_sums<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, LONG, ACROSS_I, ACROSS_J, false, PLANES>(p, block, lds, acc, spot);
     const auto [split, tile_i, tile_j, share, wi, wj, wave, lane, i0, j0] = spot;
 
     // ---- out: 32 rows of the wavefront at a time through LDS, so that a row leaves in whole runs of 64 bytes or more.  Wavefronts
@@ -126,10 +126,10 @@ __device__ __forceinline__ void product(const ProductParams& p, int block, char*
     }
 #endif
 }
-template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG, bool ACROSS_I, bool ACROSS_J>
+template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG, bool ACROSS_I, bool ACROSS_J, bool PLANES>
 __global__ __launch_bounds__(64 * WI * WJ * WS) void product_kernel(const ProductParams p) {
     __shared__ __align__(1024) char lds[product_lds<BI, BJ, WI, WJ, WS, STAGES>()];
-    product<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, LONG, ACROSS_I, ACROSS_J>(p, blockIdx.x, lds);
+    product<T, BI, BJ, WI, WJ, WS, STAGES, ACCESS, HOLD, LONG, ACROSS_I, ACROSS_J, PLANES>(p, blockIdx.x, lds);
 }
 
 // The sums of a split product's parts, always in the same order, and what follows them: four columns of a row a thread, all parts requested
@@ -288,14 +288,14 @@ __global__ __launch_bounds__(kDzThreads) void column_join_kernel(const float* __
 // ---- both products of small gradients in one launch.  A launch more takes as long as these products do (102 x 24 -> 21 f16 with its dz:
 // 13.0 us in three launches, 9.9 in two; 128 x 1024 -> 512 18.8 and 16.3).  The first `blocks` workgroups have the product with the longer sum:
 // started last, they would run on alone (1024 x 1024 -> 10 bf16 15.1 us, 12.6 so).
-template <typename T, Access ACCESS, int STAGES, int HOLD>
+template <typename T, Access ACCESS, int STAGES, int HOLD, bool PLANES>
 __global__ __launch_bounds__(256) void small_gradients_kernel(const ProductParams dx, const ProductParams dw, int blocks, bool dw_first) {
     __shared__ __align__(1024) char lds[product_lds<32, 32, 1, 1, 4, STAGES>()];
     const int second = (int)blockIdx.x >= blocks, block = (int)blockIdx.x - (second ? blocks : 0);
     if (second == dw_first)
-        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, ACCESS == ANYWHERE, false, true>(dx, block, lds);
+        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, ACCESS == ANYWHERE, false, true, PLANES>(dx, block, lds);
     else
-        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, ACCESS == ANYWHERE, true, true>(dw, block, lds);
+        product<T, 32, 32, 1, 1, 4, STAGES, ACCESS, HOLD, ACCESS == ANYWHERE, true, true, PLANES>(dw, block, lds);
 }
 
 // dx and dw in one launch, where in tiles of 32 x 32, four a compute unit at most, they are estimated to take less time together than
@@ -306,21 +306,30 @@ bool launch_small_gradients(ProductParams dx, ProductParams dw, size_t workspace
     float together = -kCuts16[CUT_32].start, apart = 0.0f;
     for (const ProductParams* p : {&dx, &dw}) {
         if ((long long)((p->rows + 31) / 32) * ((p->cols + 31) / 32) > 4 * kComputeUnits) return false;
-        together += plan_product(p->rows, p->cols, p->sum, (int)sizeof(T), access == WHOLE_PIECES, 0, CUT_32).time;
-        apart += plan_product(p->rows, p->cols, p->sum, (int)sizeof(T), (p == &dx ? access_dx : access_dw) == WHOLE_PIECES, workspace_bytes).time;
+        together += plan_product(p->rows, p->cols, p->plane + p->sum, (int)sizeof(T), access == WHOLE_PIECES, 0, CUT_32).time;
+        apart += plan_product(p->rows, p->cols, p->plane + p->sum, (int)sizeof(T), (p == &dx ? access_dx : access_dw) == WHOLE_PIECES, workspace_bytes).time;
     }
     if (access == ELEMENTS || together >= apart) return false;
     cut_product(dx, 32, kStepBytes / (int)sizeof(T), 1, nullptr);
     cut_product(dw, 32, kStepBytes / (int)sizeof(T), 1, nullptr);
     const int blocks_dx = dx.tiles_i * dx.tiles_j, blocks_dw = dw.tiles_i * dw.tiles_j;
-    const bool dw_first = dw.sum > dx.sum;
+    const bool dw_first = dw.plane + dw.sum > dx.plane + dx.sum;
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks_dx + blocks_dw)), dim3(256), 0, stream, dx, dw, dw_first ? blocks_dw : blocks_dx, dw_first);
     };
+    if constexpr (sizeof(T) == 2) {
+        if (dx.plane) {
+            if (access == WHOLE_PIECES)
+                go(small_gradients_kernel<T, WHOLE_PIECES, 8, 1, true>);
+            else
+                go(small_gradients_kernel<T, ANYWHERE, 2, 4, true>);
+            return true;
+        }
+    }
     if (access == WHOLE_PIECES)
-        go(small_gradients_kernel<T, WHOLE_PIECES, 8, 1>);
+        go(small_gradients_kernel<T, WHOLE_PIECES, 8, 1, false>);
     else
-        go(small_gradients_kernel<T, ANYWHERE, 2, 4>);
+        go(small_gradients_kernel<T, ANYWHERE, 2, 4, false>);
     return true;
 }
 
@@ -329,7 +338,7 @@ bool launch_small_gradients(ProductParams dx, ProductParams dw, size_t workspace
 template <typename T>
 bool long_sums(const ProductParams& p, const Plan& plan) {
     const long long tiles = (long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) * plan.splits;
-    return tiles <= 2 * kComputeUnits && (long long)p.sum * sizeof(T) > (long long)kLongSteps * kStepBytes * plan.splits;
+    return tiles <= 2 * kComputeUnits && ((long long)p.plane + p.sum) * sizeof(T) > (long long)kLongSteps * kStepBytes * plan.splits;
 }
 
 // (tiles of single elements are for memory where addresses do not fit; they are slower in any size)
@@ -354,7 +363,7 @@ void product_name(const ProductParams& p, size_t workspace_bytes, char* buf, siz
         {"32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2"}};
     const int hold = access == ANYWHERE && plan.cut != CUT_128 ? 4 : 1;
     const bool keep = hold == 4 && (plan.cut != CUT_64 || long_sums<T>(p, plan));
-    snprintf(buf, len, "product_kernel<%s, %s, (Access)%d, %d, %s, false, false>%s", type, shape[access][plan.cut], (int)access, hold, keep ? "true" : "false",
+    snprintf(buf, len, "product_kernel<%s, %s, (Access)%d, %d, %s, false, false, false>%s", type, shape[access][plan.cut], (int)access, hold, keep ? "true" : "false",
              plan.splits > 1 ? " + product_join_kernel" : "");
 }
 
@@ -377,7 +386,7 @@ void launch_join(const ProductParams& p, hipStream_t stream) {
 template <typename T, bool ACROSS_I, bool ACROSS_J>
 int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
     const Access access = access_of<T, ACROSS_I, ACROSS_J>(p);
-    Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
+    Plan plan = plan_product(p.rows, p.cols, p.plane + p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
     if (p.carry) plan.splits = p.splits;
     if constexpr (!ACROSS_I && !ACROSS_J) {
         if (few_rows<T>(p, access, plan)) {
@@ -410,8 +419,15 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
                 q.partial = workspace + first * p.cols;
                 q.partial_stride = (long long)p.rows * p.cols;
             }
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, L, ACROSS_I, ACROSS_J>),
-                               dim3((unsigned)((long long)q.tiles_i * q.tiles_j * q.splits)), dim3(kThreads), 0, stream, q);
+            const dim3 grid((unsigned)((long long)q.tiles_i * q.tiles_j * q.splits));
+            if constexpr (sizeof(T) == 2 && ACROSS_J) {
+                if (p.plane)
+                    hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, L, ACROSS_I, ACROSS_J, true>), grid, dim3(kThreads), 0,
+                                       stream, q);
+            }
+            if (!p.plane)
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, B, B, WI, WJ, WS, S, how.value, H, L, ACROSS_I, ACROSS_J, false>), grid, dim3(kThreads), 0,
+                                   stream, q);
             if (q.splits > 1 && !q.carry) launch_join<T>(q, stream);
         }
     };

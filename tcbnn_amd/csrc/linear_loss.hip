@@ -193,25 +193,16 @@ __global__ __launch_bounds__(kLossJoinThreads) void loss_join_kernel(const LossP
     }
 }
 
-// ---- rows of the input in the workspace, at whole 16 bytes, `copies` times over
+// ---- rows of the input in the workspace, at whole 16 bytes
 constexpr int kPackThreads = 256;
 template <typename T>
-__global__ __launch_bounds__(kPackThreads) void loss_pack_kernel(const T* __restrict__ x, T* __restrict__ to, int rows, int n, int copies, long long x_ld,
-                                                                 long long to_ld) {
-    constexpr int V = Elem<T>::kVec;
-    const int vectors = (n + V - 1) / V;
+__global__ __launch_bounds__(kPackThreads) void loss_pack_kernel(const T* __restrict__ x, T* __restrict__ to, int rows, int n, long long x_ld, long long to_ld) {
+    constexpr int V = Elem<T>::kVec;  // (n is a multiple of it)
+    const int vectors = n / V;
     for (long long at = (long long)blockIdx.x * kPackThreads + threadIdx.x; at < (long long)rows * vectors; at += (long long)gridDim.x * kPackThreads) {
         const long long row = at / vectors;
         const int i = (int)(at - row * vectors) * V;
-        const T* from = x + row * x_ld + i;
-        Vec<T> v;
-        if (i + V <= n) {
-            v = load_vec(from);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = i + e < n ? from[e] : (T)0.0f;
-        }
-        for (int c = 0; c < copies; ++c) *reinterpret_cast<Vec<T>*>(to + (row + (long long)c * rows) * to_ld + i) = v;
+        *reinterpret_cast<Vec<T>*>(to + row * to_ld + i) = load_vec(x + row * x_ld + i);
     }
 }
 
@@ -360,6 +351,8 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void loss_grad_product_kernel(co
 }
 
 // ---- plans
+// rows and columns of a tile (by_tile)
+inline int cut_size(Access access, Cut cut) { return access == ELEMENTS ? 32 : (access == WHOLE_PIECES ? kCuts16 : kCutsAnywhere)[cut].size; }
 // The forward call's kernel: its tile, or the one for few rows; the number of parts that it leaves of a row.
 struct LossPlan {
     Plan plan;
@@ -371,7 +364,7 @@ inline LossPlan plan_loss(int rows, int classes, int sum, int size, Access acces
     LossPlan l;
     l.plan = plan_product(rows, classes, sum, size, vectors, 0);
     l.few = rows <= kFewRows && (access == ELEMENTS || few_time(rows, classes, sum, size, vectors) < l.plan.time);
-    const int width = l.few ? kFewOutputs : access == ELEMENTS ? 32 : (vectors ? kCuts16 : kCutsAnywhere)[l.plan.cut].size;
+    const int width = l.few ? kFewOutputs : cut_size(access, l.plan.cut);
     l.parts = (classes - 1) / width + 1;
     return l;
 }
@@ -389,39 +382,37 @@ inline int piece_classes(int rows, int classes, int size) {
 inline long long piece_ld(int piece, int size) { return ((long long)piece * size + 15) / 16 * 16 / size; }
 // The splits of dx's sum over a whole piece, where there are several.  Where the weights lie is not known when a workspace is asked for: the splits are
 // those of rows at whole 16 bytes, which are no fewer.
-inline int carried_splits(int rows, int in_features, int piece, int size, int most) {
-    const int splits = std::min(most, plan_product(rows, in_features, piece, size, true, ~(size_t)0).splits);
+inline int carried_splits(int rows, int in_features, int piece, int size) {
+    const int splits = plan_product(rows, in_features, piece, size, true, ~(size_t)0).splits;
     const int steps = (int)(((long long)piece * size + kStepBytes - 1) / kStepBytes), each = (steps + splits - 1) / splits;
     return (steps + each - 1) / each;  // (as cut_product cuts a whole piece: every part is written by the first)
 }
 
 // In 16 bits d is rounded before it is multiplied.  A row of d, and a column, is often little else than its given class' value, whose rounding then is that
 // of all that it is multiplied with.  Over many rows these errors, like those of the sums' other terms, come to sqrt 2 of what rounding the results
-// leaves (8192 rows bf16: 0.0024 of them, 0.0017 the rounding); a few rows may be off by twice that.  Up to kTwoPlaneRows rows, where the
-// products are bound by the weights' bytes, d is kept in two planes, its rounding and what that left: rows of their own in dx, summed
-// afterwards, and more rows to sum over in dw, where the input's rows are there twice.
-constexpr int kTwoPlaneRows = 128;
-inline int loss_planes(int rows, int dtype) { return dtype != TCBNN_F32 && rows <= kTwoPlaneRows ? 2 : 1; }
+// leaves (8192 rows bf16: 0.0024 of them, 0.0017 the rounding); few rows may be off by twice that.  Up to kTwoPlaneRows rows d is kept in
+// two planes, its rounding and what that left, and both products sum over both.  (@@)
+constexpr int kTwoPlaneRows = 256;
+inline bool two_planes(int rows, int dtype) { return dtype != TCBNN_F32 && rows <= kTwoPlaneRows; }
+// where the second plane of a sum of n begins: whole steps
+inline int plane_of(int n, int size) { return (n + kStepBytes / size - 1) / (kStepBytes / size) * (kStepBytes / size); }
 
 struct LossWorkspace {
     size_t scale, x, d, sums, dx, split, total;  // offsets, in order
-    int planes, piece, splits;
-    bool carried;
+    int piece, splits;
 };
 inline LossWorkspace loss_workspace(int rows, int in_features, int classes, int dtype) {
-    const int size = (int)dtype_bytes(dtype);
+    const int size = (int)dtype_bytes(dtype), planes = two_planes(rows, dtype) ? 2 : 1;
     LossWorkspace w = {};
-    w.planes = loss_planes(rows, dtype);
-    rows *= w.planes;
-    w.piece = piece_classes(rows, classes, size);
-    w.carried = w.piece < classes || w.planes > 1;
-    w.splits = w.carried ? carried_splits(rows, in_features, w.piece, size, kMaxSplits / w.planes) : 1;
+    w.piece = piece_classes(rows * planes, classes, size);
+    const bool carried = w.piece < classes;
+    w.splits = carried ? carried_splits(rows, in_features, (planes - 1) * plane_of(w.piece, size) + w.piece, size) : 1;
     w.x = 256;
     w.d = w.x + whole_lines((size_t)rows * piece_ld(in_features, size) * size);
-    w.sums = w.d + whole_lines((size_t)rows * piece_ld(w.piece, size) * size);
+    w.sums = w.d + whole_lines((size_t)rows * planes * piece_ld(w.piece, size) * size);
     w.dx = w.sums + whole_lines((size_t)((rows + 31) / 32) * w.piece * sizeof(float));
-    w.split = w.dx + (w.carried ? whole_lines((size_t)w.splits * rows * in_features * sizeof(float)) : 0);
-    w.total = w.split + gradient_product_bytes(rows, in_features, w.piece, dtype);
+    w.split = w.dx + (carried ? whole_lines((size_t)w.splits * rows * in_features * sizeof(float)) : 0);
+    w.total = w.split + gradient_product_bytes(rows * planes, in_features, w.piece * planes, dtype);
     return w;
 }
 
@@ -437,10 +428,10 @@ int check_loss(int rows, int in_features, int classes, int dtype) {
 template <typename T>
 bool apart(const Operand& o, int n) { return n % Elem<T>::kVec != 0 || (uintptr_t)o.p % 16 != 0 || o.ld * sizeof(T) % 16 != 0; }
 template <typename T>
-Operand pack(const Operand& x, void* to, int rows, int n, int copies, hipStream_t stream) {
+Operand pack(const Operand& x, void* to, int rows, int n, hipStream_t stream) {
     const long long ld = piece_ld(n, (int)sizeof(T)), vectors = rows * (ld / Elem<T>::kVec);
     hipLaunchKernelGGL(loss_pack_kernel<T>, dim3((unsigned)std::min((vectors + kPackThreads - 1) / kPackThreads, 8LL * kComputeUnits)), dim3(kPackThreads), 0, stream,
-                       (const T*)x.p, (T*)to, rows, n, copies, x.ld, ld);
+                       (const T*)x.p, (T*)to, rows, n, x.ld, ld);
     return {to, ld};
 }
 // rows that are so far apart that 32 bits do not hold a tile
@@ -484,7 +475,7 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
     return by_dtype(d->dtype, [&](auto type) -> int {
         using T = decltype(type);
         if (p.rows > kFewRows && apart<T>(p.i, p.sum) && !apart<T>(p.j, p.sum))
-            p.i = pack<T>(p.i, (char*)d->workspace + d->workspace_bytes / 16 * 16 - (size_t)p.rows * piece_ld(p.sum, (int)sizeof(T)) * sizeof(T), p.rows, p.sum, 1, s);
+            p.i = pack<T>(p.i, (char*)d->workspace + d->workspace_bytes / 16 * 16 - (size_t)p.rows * piece_ld(p.sum, (int)sizeof(T)) * sizeof(T), p.rows, p.sum, s);
         const Access access = access_of<T, false, false>(p);
         const LossPlan plan = plan_loss(p.rows, p.cols, p.sum, (int)sizeof(T), access);
         LossParams l = {d->loss ? d->targets : nullptr, (float2*)d->workspace, (float*)((char*)d->workspace + whole_lines((size_t)plan.parts * p.rows * sizeof(float2))),
@@ -568,9 +559,9 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
         using T = decltype(type);
         ProductParams dx = {};
         Operand x = {d->input, x_ld};
-        const bool packed = apart<T>(x, d->in_features) && !apart<T>({d->weight, w_ld}, d->in_features);
-        if (packed || (w.planes > 1 && d->grad_weight)) x = pack<T>(x, base + w.x, d->rows, d->in_features, w.planes, s);
-        const long long d_ld = piece_ld(w.piece, (int)sizeof(T));
+        if (apart<T>(x, d->in_features) && !apart<T>({d->weight, w_ld}, d->in_features)) x = pack<T>(x, base + w.x, d->rows, d->in_features, s);
+        const bool planes = two_planes(d->rows, d->dtype);
+        const long long d_ld = piece_ld(w.piece, (int)sizeof(T)), low = planes ? d->rows * d_ld : 0;
         for (int first = 0; first < d->classes; first += w.piece) {
             const int classes = std::min(w.piece, d->classes - first);
             const T* weight = (const T*)d->weight + first * w_ld;
@@ -583,14 +574,13 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             p.bias = d->bias ? d->bias + first : nullptr;
             p.out = base + w.d;
             p.out_ld = d_ld;
-            const LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes,
-                                      w.planes > 1 ? d->rows * d_ld : 0};
+            LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes, low};
             const Access access = access_of<T, false, false>(p);
             const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0);
-            int tiles_i = 0;
+            const int tiles_i = (p.rows - 1) / cut_size(access, plan.cut) + 1;
+            if (l.sums && tiles_i == 1) l.sums = d->grad_bias + first;
             by_tile(access, plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
                 constexpr int B = size.value, kThreads = 64 * wi.value * wj.value * ws.value;
-                tiles_i = (p.rows - 1) / B + 1;
                 // rows beyond a launch's threads have one of their own
                 const long long tiles_j = (p.cols - 1) / B + 1, at_once = std::max(1LL, kMaxThreads / kThreads / tiles_j) * B;
                 for (long long row = 0; row < p.rows; row += at_once) {
@@ -608,19 +598,22 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
                                        dim3((unsigned)((long long)q.tiles_i * q.tiles_j)), dim3(kThreads), 0, s, q, part);
                 }
             });
-            if (d->grad_bias) launch_column_join(l.sums, d->grad_bias + first, tiles_i, classes, s);
+            if (d->grad_bias && tiles_i > 1) launch_column_join(l.sums, d->grad_bias + first, tiles_i, classes, s);
             TCBNN_LAUNCH_CHECK("loss_grad_product_kernel");
             ProductParams dw = {};
             dx.i = dw.i = {p.out, p.out_ld};
             dx.padded = dw.padded = classes >= Elem<T>::kVec;
             dx.factor = dw.factor = scale ? scale + 1 : nullptr;
             dx.j = {weight, w_ld};
-            dx.rows = w.planes * d->rows;
+            dx.i_low = dw.i_low = low;
+            dx.plane = planes ? plane_of(classes, (int)sizeof(T)) : 0;
+            dw.plane = planes ? plane_of(d->rows, (int)sizeof(T)) : 0;
+            dx.rows = d->rows;
             dx.cols = d->in_features;
             dx.sum = classes;
             dx.out = d->grad_input;
             dx.out_ld = dx_ld;
-            if (w.carried) {
+            if (w.piece < d->classes) {
                 dx.carry = first == 0 ? CARRY_FIRST : CARRY_ON;
                 dx.splits = w.splits;
                 dx.partial = (float*)(base + w.dx);
@@ -628,14 +621,12 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             dw.j = x;
             dw.rows = classes;
             dw.cols = d->in_features;
-            dw.sum = w.planes * d->rows;
+            dw.sum = d->rows;
             dw.out = d->grad_weight ? (T*)d->grad_weight + first * dw_ld : nullptr;
             dw.out_ld = dw_ld;
             if (int rc = launch_gradient_products(d->dtype, dx, dw, (float*)(base + w.split), w.total - w.split, s)) return rc;
         }
-        if (w.carried && d->grad_input) {
-            dx.rows = d->rows;
-            dx.splits = w.splits * w.planes;  // (a split's planes lie one behind the other)
+        if (w.piece < d->classes && d->grad_input) {
             dx.partial_stride = (long long)d->rows * d->in_features;
             return launch_carried_sum(d->dtype, dx, s);
         }

@@ -177,13 +177,13 @@ struct Tile {
             }
         }
     }
-    // requests a piece of the step that begins at `s` of `sum` into LDS
-    __device__ __forceinline__ void request_piece(char* lds, int s, int sum, int e) {
+    // requests a piece of the step that begins at `s` of `sum` into LDS (`plane`: elements to the plane of the sum that the step lies in)
+    __device__ __forceinline__ void request_piece(char* lds, int s, int sum, long long plane, int e) {
         int row, piece;
         where(e, row, piece);
         const int at = s + (ACROSS ? row : piece * V) < sum ? offset[e] : kOutOfRange;
         char* to = lds + (e * THREADS + wave_first()) * 16;
-        const T* from = ACROSS ? base + s * ld : matrix(e);
+        const T* from = ACROSS ? base + plane + s * ld : matrix(e) + plane;
         if constexpr (HIDDEN) {
             // The builtin makes the compiler wait for it before every transposing read of LDS, whichever tile that reads; what is in
             // LDS is for meet() to wait for.  (m0, which the compiler sets itself right before each use of its own: where in LDS.  Nothing comes back into registers.)
@@ -202,17 +202,17 @@ struct Tile {
     }
     // requests the tile of a step: into LDS at once, or into the registers of a slot
     template <int SLOT>
-    __device__ __forceinline__ void request(char* lds, int s, int sum) {
+    __device__ __forceinline__ void request(char* lds, int s, int sum, long long plane) {
         if constexpr (ACCESS == WHOLE_PIECES) {
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) request_piece(lds, s, sum, e);
+            for (int e = 0; e < kEach; ++e) request_piece(lds, s, sum, plane, e);
         } else if constexpr (ACCESS == ANYWHERE) {
             // (no branches: then the requests of several steps can be told apart by their number)
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
                 int row, piece;
                 where(e, row, piece);
-                const char* from = reinterpret_cast<const char*>(ACROSS ? base + s * ld : matrix(e));
+                const char* from = reinterpret_cast<const char*>(ACROSS ? base + plane + s * ld : matrix(e) + plane);
                 int at = offset[e];
                 if constexpr (ACROSS) {
                     at -= max(0, s + row - (sum - 1)) * (int)(ld * (int)sizeof(T));  // rows past the sum: the last one
@@ -227,7 +227,7 @@ struct Tile {
             for (int e = 0; e < kEach; ++e) {
                 int row, piece;
                 where(e, row, piece);
-                const T* p = ACROSS ? base + (s + row) * ld + piece * V : matrix(e) + min(source(row), valid - 1) * ld + s + piece * V;
+                const T* p = plane + (ACROSS ? base + (s + row) * ld + piece * V : matrix(e) + min(source(row), valid - 1) * ld + s + piece * V);
                 const int n = ACROSS ? (s + row < sum ? valid - piece * V : 0) : sum - (s + piece * V);
                 Vec<T> v;
 #pragma unroll
@@ -322,6 +322,10 @@ struct ProductParams {
     long long partial_stride;  // from one split's to the next one's
     int carry;             // the sum goes on in `partial`: CARRY_FIRST writes it, CARRY_ON adds to what is there
     const float* factor;   // of the sums, or NULL (a power of two: nothing is rounded by it)
+    // I in two planes whose products are added: the sum goes over the first, `sum` long, and from `plane` on over the second, which lies i_low
+    // elements behind it; J is the same for both.  0: one plane.
+    int plane;
+    long long i_low;
     bool padded;           // I's rows, 16 bytes or more, go on with zeros to whole 16 bytes
 };
 enum Carry : int { NO_CARRY, CARRY_FIRST, CARRY_ON };
@@ -378,7 +382,7 @@ struct Spot {
 };
 // The sums of workgroup `block`'s tile, in registers as the matrix instructions leave them; LDS is free afterwards.
 template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG, bool ACROSS_I, bool ACROSS_J,
-          bool PAIRED = false>
+          bool PAIRED = false, bool PLANES = false>
 __device__ __forceinline__ void product_sums(const ProductParams& p, int block, char* lds, Acc (&acc)[BI / WI / 32][BJ / WJ / 32], Spot& spot) {
     constexpr int kThreads = 64 * WI * WJ * WS, NI = BI / WI / 32, NJ = BJ / WJ / 32, kQuarters = 4 / WS;
     constexpr bool ALIGNED = ACCESS == WHOLE_PIECES;
@@ -404,7 +408,7 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
     constexpr int V = Elem<T>::kVec;
     ti.init(p.i, i0, ACROSS_I && p.padded ? ((long long)p.rows + V - 1) / V * V : (long long)p.rows);
     tj.init(p.j, j0, p.cols);
-    const int s0 = split * p.split_sum, s1 = min(p.sum, s0 + p.split_sum);
+    const int s0 = split * p.split_sum, s1 = min(PLANES ? p.plane + p.sum : p.sum, s0 + p.split_sum);
     const int share = wave / (WI * WJ), wi = wave / WJ % WI * (32 * NI), wj = wave % WJ * (32 * NJ);
     spot = {split, tile_i, tile_j, share, wi, wj, wave, lane, i0, j0};
 
@@ -419,14 +423,30 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
     constexpr integral_constant<int, 0> slot0;
     const int steps = (s1 - s0 + TileI::kSteps - 1) / TileI::kSteps;
     // (a step past the last one: requests that touch no memory)
-    auto request_i = [&](int stage, int step, auto slot) { ti.template request<slot.value>(lds + stage * kStage, s0 + step * TileI::kSteps, s1); };
+    // where a step begins: in the sum of its plane, that plane's end (or the split's), the plane
+    struct Step {
+        int s, end;
+        long long i_plane;
+    };
+    auto where = [&](int step) -> Step {
+        const int s = s0 + step * TileI::kSteps;
+        if constexpr (!PLANES) return {s, s1, 0};
+        const int before = s >= p.plane ? p.plane : 0;
+        return {s - before, min(p.sum, s1 - before), before ? p.i_low : 0};
+    };
+    auto request_i = [&](int stage, int step, auto slot) {
+        const Step at = where(step);
+        ti.template request<slot.value>(lds + stage * kStage, at.s, at.end, at.i_plane);
+    };
     auto request_j = [&](int stage, int step, auto slot) {
-        tj.template request<slot.value>(lds + stage * kStage + TileI::kBytes, s0 + step * TileI::kSteps, s1);
+        const Step at = where(step);
+        tj.template request<slot.value>(lds + stage * kStage + TileI::kBytes, at.s, at.end, 0);
     };
     // (registers only) a slot's step goes to LDS, for all to read
     auto hand_over = [&](int stage, int step, auto slot) {
-        ti.template store<slot.value>(lds + stage * kStage, s0 + step * TileI::kSteps, s1);
-        tj.template store<slot.value>(lds + stage * kStage + TileI::kBytes, s0 + step * TileI::kSteps, s1);
+        const Step at = where(step);
+        ti.template store<slot.value>(lds + stage * kStage, at.s, at.end);
+        tj.template store<slot.value>(lds + stage * kStage + TileI::kBytes, at.s, at.end);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (requests into registers stay under way)
     };
     // A step's fragments come a quarter ahead of their instructions, the first quarter's from the next step's tiles: so the barrier
@@ -502,11 +522,12 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int k = 0; k + 1 < kQuarters; ++k) {
-                    const int last = stage == 0 ? STAGES - 1 : stage - 1, s = s0 + (step + STAGES - 1) * TileI::kSteps;
+                    const int last = stage == 0 ? STAGES - 1 : stage - 1;
+                    const Step at = where(step + STAGES - 1);
                     if (kApart && k == 0 && !kHidden) request_i(last, step + STAGES - 1, slot0);
                     fragments((k + 1) & 1, stage, k + 1);
                     if (kApart && k == 0 && kHidden) {
-                        multiply_and(0, requests_i, [&](int e) { ti.request_piece(lds + last * kStage, s, s1, e); });
+                        multiply_and(0, requests_i, [&](int e) { ti.request_piece(lds + last * kStage, at.s, at.end, at.i_plane, e); });
                     } else {
                         multiply(k & 1);
                         if (kApart && k == 0)
@@ -520,8 +541,9 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
                 if (!kApart) request_i(stage, step + STAGES, slot0);
                 fragments(kQuarters & 1, next, 0);
                 if constexpr (kHidden && kApart) {
+                    const Step at = where(step + STAGES);
                     multiply_and((kQuarters - 1) & 1, requests_j, [&](int e) {
-                        tj.request_piece(lds + stage * kStage + TileI::kBytes, s0 + (step + STAGES) * TileI::kSteps, s1, e);
+                        tj.request_piece(lds + stage * kStage + TileI::kBytes, at.s, at.end, 0, e);
                     });
                 } else {
                     multiply((kQuarters - 1) & 1);
@@ -775,9 +797,9 @@ void by_tile(Access access, Cut cut, F&& f) {
 inline void cut_product(ProductParams& p, int size, int steps_size, int splits, float* workspace) {
     p.tiles_i = (p.rows + size - 1) / size;
     p.tiles_j = (p.cols + size - 1) / size;
-    const int steps = (p.sum + steps_size - 1) / steps_size;
+    const int steps = (p.plane + p.sum + steps_size - 1) / steps_size;
     p.split_sum = std::max(1, (steps + splits - 1) / splits) * steps_size;
-    p.splits = std::max(1, (p.sum + p.split_sum - 1) / p.split_sum);
+    p.splits = std::max(1, (p.plane + p.sum + p.split_sum - 1) / p.split_sum);
     p.partial = workspace;
     p.partial_stride = (long long)p.rows * p.cols;
 }

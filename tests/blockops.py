@@ -148,8 +148,8 @@ def loss_grads(x, w, t, g, z, zerr, p, lse, lse_err, dtype):
     derr = np.abs(g)[:, None] * (p * (zerr + lse_err[:, None] + U * (4 * zabs + 4 * np.abs(np.where(np.isfinite(lse), lse, 0))[:, None] + 6)) + U * np.abs(p - one)) * 1.1
     # f16: d is scaled, so that what lies below the normal numbers is less than 2^-38 of the largest |g|
     tiny = {"f32": 2.0 ** -126, "bf16": 2.0 ** -126, "f16": 2.0 ** -38 * np.abs(g).max()}[dtype]
-    # (of 128 rows at most d is kept in two planes: its rounding, and what that left, rounded)
-    step = ho.U[dtype] ** 2 if dtype != "f32" and m <= 128 else ho.U[dtype]
+    # (of 256 rows at most d is kept in two planes: its rounding, and what that left, rounded)
+    step = ho.U[dtype] ** 2 if dtype != "f32" and m <= 256 else ho.U[dtype]
     used = derr + step * (np.abs(d) + derr) + tiny
     out = {}
     terms, exact = np.abs(d) @ np.abs(w), d @ w
