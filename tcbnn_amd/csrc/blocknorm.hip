@@ -39,21 +39,33 @@ __device__ __forceinline__ float after_factor(const P& p, int i) { return times(
 template <typename P>
 __device__ __forceinline__ float after_shift(const P& p, int i) { return p.after_beta ? times(p.scale, p.gate, i) * p.after_beta[i] : 0.0f; }
 
-// a lane's P or Q, 0 past the row
-template <typename Slice, typename F>
-__device__ __forceinline__ void each_feature(Slice& s, int lane, int n, F f) {
+// a lane's P (of after_gamma) or Q (of after_beta), 0 past the row
+template <typename P, typename Slice>
+__device__ __forceinline__ void load_after(const P& p, const float* vector, Slice& s, int lane, int n) {
+    Slice gate;
+    s.load_param(vector, lane, n, 1.0f);
+    gate.load_param(p.gate, lane, n, 1.0f);
 #pragma unroll
     for (int r = 0; r < (int)(sizeof(s.v) / sizeof(s.v[0])); ++r)
 #pragma unroll
         for (int e = 0; e < Slice::V; ++e) {
-            const int i = r * Slice::kStep + lane * Slice::V + e;
-            s.v[r][e] = i < n ? f(i) : 0.0f;
+            const bool in = (r + 1) * Slice::kStep <= n || r * Slice::kStep + lane * Slice::V + e < n;
+            s.v[r][e] = in ? p.scale * gate.v[r][e] * s.v[r][e] : 0.0f;
         }
+}
+
+// Rows of more bytes than the caches hold are requested and stored past them (PASSING): 16384 x 4096 bf16 100 us, 106 through them; gradients of 8192 x
+// 4096 85 us and 91.
+constexpr long long kPassingBytes = 256LL << 20;
+template <typename F>
+void by_passing(long long bytes, F&& f) {
+    if (bytes > kPassingBytes) return f(std::true_type());
+    f(std::false_type());
 }
 
 // LAYER: either norm may have means.  All teams of a workgroup take the same number of steps; one without a row of its own computes on the
 // last one and keeps nothing.  Two sets of slots in turn: between two sums into one slot lies the barrier of a row in between.
-template <typename T, int W, int R, bool LAYER>
+template <typename T, int W, int R, bool LAYER, bool PASSING>
 __global__ __launch_bounds__(forward_threads(W)) void blocknorm_kernel(const NormsParams p) {
     constexpr int kTeams = forward_threads(W) / (64 * W);
     using Slice = RowSlice<T, W, R>;
@@ -66,13 +78,22 @@ __global__ __launch_bounds__(forward_threads(W)) void blocknorm_kernel(const Nor
     const long long stride = (long long)gridDim.x * kTeams;
     auto request = [&](long long first) {
         const long long row = min(first + team, (long long)p.rows - 1);
-        Slice::request((const T*)p.in + row * p.in_ld, lane, n, raw_s);
-        if (p.block) Slice::request((const T*)p.block + row * p.block_ld, lane, n, raw_u);
+        Slice::template request<PASSING>((const T*)p.in + row * p.in_ld, lane, n, raw_s);
+        if (p.block) Slice::template request<PASSING>((const T*)p.block + row * p.block_ld, lane, n, raw_u);
     };
     request((long long)blockIdx.x * kTeams);
     auto parameters_after = [&] {
-        each_feature(P, lane, n, [&](int i) { return after_factor(p, i); });
-        if constexpr (LAYER) each_feature(Q, lane, n, [&](int i) { return after_shift(p, i); });
+        load_after(p, p.after_gamma, P, lane, n);
+        if constexpr (LAYER) {
+            if (p.after_beta) {
+                load_after(p, p.after_beta, Q, lane, n);
+            } else {
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) Q.v[r][e] = 0.0f;
+            }
+        }
     };
     auto parameters_before = [&] {
         g.load_param(p.before_gamma, lane, n, 1.0f);
@@ -135,7 +156,7 @@ __global__ __launch_bounds__(forward_threads(W)) void blocknorm_kernel(const Nor
                     s.v[r][e] = __builtin_fmaf(u.v[r][e] * rstd, P.v[r][e], s.v[r][e]);
                 }
         }
-        if (mine && p.out) s.store((T*)p.out + row * p.out_ld, lane, n);
+        if (mine && p.out) s.template store<PASSING>((T*)p.out + row * p.out_ld, lane, n);
         if (!p.before) continue;
         rstd = normalize(s, p.before, mean, slot[2], slot[3]);
         if (!mine) continue;
@@ -148,7 +169,7 @@ __global__ __launch_bounds__(forward_threads(W)) void blocknorm_kernel(const Nor
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int e = 0; e < V; ++e) s.v[r][e] = __builtin_fmaf(s.v[r][e] * rstd, g.v[r][e], LAYER ? b.v[r][e] : 0.0f);
-        s.store((T*)p.y + row * p.y_ld, lane, n);
+        s.template store<PASSING>((T*)p.y + row * p.y_ld, lane, n);
     }
 }
 
@@ -225,8 +246,8 @@ __device__ __forceinline__ void put_parameters(const NormsGradParams& p, int i, 
 }
 
 // A workgroup of 16 wavefronts is 16 / W teams, and keeps its rows' sums; a workgroup that has all rows writes the parameters' gradients themselves.
-// BETAS: the sums B and D, and means.
-template <typename T, int W, int R, bool LAYER>
+// LAYER: the sums B and D, and means.
+template <typename T, int W, int R, bool LAYER, bool PASSING>
 __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const NormsGradParams p) {
     constexpr int kTeams = kGradThreads / (64 * W);
     using Slice = RowSlice<T, W, R>;
@@ -241,21 +262,21 @@ __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const Norm
     const long long stride = (long long)gridDim.x * kTeams;
     auto request = [&](long long first) {
         const long long row = min(first + team, (long long)p.rows - 1);
-        if (p.ds) Slice::request((const T*)p.ds + row * p.ds_ld, lane, n, raw_ds);
+        if (p.ds) Slice::template request<PASSING>((const T*)p.ds + row * p.ds_ld, lane, n, raw_ds);
         if (p.dy) {
             next[2] = LAYER && p.before == TCBNN_NORM_LAYER ? p.before_mean[row] : 0.0f;
             next[3] = p.before_rstd[row];
-            Slice::request((const T*)p.dy + row * p.dy_ld, lane, n, raw_dy);
-            Slice::request((const T*)p.stream + row * p.stream_ld, lane, n, raw_s);
+            Slice::template request<PASSING>((const T*)p.dy + row * p.dy_ld, lane, n, raw_dy);
+            Slice::template request<PASSING>((const T*)p.stream + row * p.stream_ld, lane, n, raw_s);
         }
         if (with_block) {
             next[0] = LAYER && p.after == TCBNN_NORM_LAYER ? p.after_mean[row] : 0.0f;
             next[1] = p.after ? p.after_rstd[row] : 1.0f;
-            Slice::request((const T*)p.block + row * p.block_ld, lane, n, raw_u);
+            Slice::template request<PASSING>((const T*)p.block + row * p.block_ld, lane, n, raw_u);
         }
     };
     request((long long)blockIdx.x * kTeams);
-    each_feature(P, lane, n, [&](int i) { return after_factor(p, i); });
+    load_after(p, p.after_gamma, P, lane, n);
     g.load_param(p.before_gamma, lane, n, 1.0f);
 #pragma unroll
     for (int k = 0; k < kSums; ++k)
@@ -327,7 +348,7 @@ __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const Norm
                     d.v[r][e] = __builtin_fmaf(v, rstd2, d.v[r][e]);
                 }
         }
-        if (mine && p.dr) d.store((T*)p.dr + row * p.dr_ld, lane, n);
+        if (mine && p.dr) d.template store<PASSING>((T*)p.dr + row * p.dr_ld, lane, n);
         if (!with_block) continue;
         float sg = 0.0f, sgx = 0.0f;
 #pragma unroll
@@ -355,7 +376,7 @@ __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const Norm
                     d.v[r][e] = v * rstd1;
                 }
         }
-        if (mine && p.db) d.store((T*)p.db + row * p.db_ld, lane, n);
+        if (mine && p.db) d.template store<PASSING>((T*)p.db + row * p.db_ld, lane, n);
     }
     if (!p.params) return;
     const bool last = gridDim.x == 1;
@@ -366,7 +387,8 @@ __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const Norm
             put_parameters(p, i, t);
         } else {
 #pragma unroll
-            for (int k = 0; k < kSums; ++k) to[(size_t)k * n + i] = t[k];
+            for (int k = 0; k < kSums; ++k)
+                if (LAYER || k % 2 == 0) to[(size_t)k * n + i] = t[k];
         }
     };
 #pragma unroll
@@ -379,9 +401,10 @@ __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const Norm
             }
         } else {
             constexpr int kEach = (Slice::kStep + kGradThreads - 1) / kGradThreads;
-            float t[kEach][kSums];
+            float t[kEach][kSums] = {};
 #pragma unroll
             for (int k = 0; k < kSums; ++k) {
+                if (!LAYER && k % 2) continue;
                 __syncthreads();
 #pragma unroll
                 for (int e = 0; e < V; ++e) sums[(team * V + e) * 64 * W + lane] = acc[k].v[r][e];  // (lanes side by side: no bank twice)
@@ -503,6 +526,7 @@ constexpr int kJoinThreads = 256, kJoinFeatures = 16;
 __global__ __launch_bounds__(kJoinThreads) void blocknorm_join_kernel(const NormsGradParams p, int parts) {
     constexpr int kStep = kJoinThreads / kJoinFeatures;
     __shared__ float lds[kSums][kStep][kJoinFeatures];
+    const bool all = p.after == TCBNN_NORM_LAYER || p.before == TCBNN_NORM_LAYER;  // (otherwise B and D are not there)
     const int c = threadIdx.x % kJoinFeatures, part = threadIdx.x / kJoinFeatures, i = blockIdx.x * kJoinFeatures + c;
     float t[kSums] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (i < p.n)
@@ -511,7 +535,7 @@ __global__ __launch_bounds__(kJoinThreads) void blocknorm_join_kernel(const Norm
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int w = 0; w < kSums; ++w) v[u][w] = k + u * kStep < parts ? p.partial[((size_t)(k + u * kStep) * kSums + w) * p.n + i] : 0.0f;
+                for (int w = 0; w < kSums; ++w) v[u][w] = (all || w % 2 == 0) && k + u * kStep < parts ? p.partial[((size_t)(k + u * kStep) * kSums + w) * p.n + i] : 0.0f;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -586,12 +610,18 @@ extern "C" int tcbnn_blocknorm_forward(const tcbnn_blocknorm_desc* d, void* stre
         by_team(vectors, [&](auto w, auto r) {
             constexpr int W = w.value, R = r.value;
             const int teams = forward_threads(W) / (64 * W);
-            // the registers of 2048 threads a compute unit, more where rows are left
-            const dim3 blocks((unsigned)std::min((p.rows + teams - 1LL) / teams, kComputeUnits * 2048LL / forward_threads(W)));
-            if (p.after == TCBNN_NORM_LAYER || p.before == TCBNN_NORM_LAYER)
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(blocknorm_kernel<T, W, R, true>), blocks, dim3(forward_threads(W)), 0, (hipStream_t)stream, p);
-            else
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(blocknorm_kernel<T, W, R, false>), blocks, dim3(forward_threads(W)), 0, (hipStream_t)stream, p);
+            const bool layer = p.after == TCBNN_NORM_LAYER || p.before == TCBNN_NORM_LAYER;
+            // As many workgroups as a compute unit has registers for, more where rows are left: 16384 x 4096 bf16 with a fourth of 512 threads, which
+            // begins when the others end, 132 us, three 106.
+            const long long threads = R * Elem<T>::kVec > kHeld ? 1024 : layer ? 1280 : 1536;
+            const dim3 blocks((unsigned)std::min((p.rows + teams - 1LL) / teams, kComputeUnits * (threads / forward_threads(W))));
+            const long long bytes = (long long)p.rows * p.n * sizeof(T) * (1 + (p.block != nullptr) + (p.out != nullptr) + (p.y != nullptr));
+            by_passing(bytes, [&](auto passing) {
+                if (layer)
+                    hipLaunchKernelGGL(HIP_KERNEL_NAME(blocknorm_kernel<T, W, R, true, passing.value>), blocks, dim3(forward_threads(W)), 0, (hipStream_t)stream, p);
+                else
+                    hipLaunchKernelGGL(HIP_KERNEL_NAME(blocknorm_kernel<T, W, R, false, passing.value>), blocks, dim3(forward_threads(W)), 0, (hipStream_t)stream, p);
+            });
         });
     });
     TCBNN_LAUNCH_CHECK("blocknorm_kernel");
@@ -672,10 +702,16 @@ extern "C" int tcbnn_blocknorm_backward(const tcbnn_blocknorm_grad_desc* d, void
                 if constexpr (R * Elem<T>::kVec <= kHeld) {
                     parts = p.params ? grad_parts(p.rows, kTeams) : (int)std::min((p.rows + kTeams - 1LL) / kTeams, (long long)kComputeUnits);
                     joined = p.params && parts == 1;
-                    if (p.after == TCBNN_NORM_LAYER || p.before == TCBNN_NORM_LAYER)
-                        hipLaunchKernelGGL(HIP_KERNEL_NAME(blocknorm_grad_kernel<T, W, R, true>), dim3((unsigned)parts), dim3(kGradThreads), 0, (hipStream_t)stream, p);
-                    else
-                        hipLaunchKernelGGL(HIP_KERNEL_NAME(blocknorm_grad_kernel<T, W, R, false>), dim3((unsigned)parts), dim3(kGradThreads), 0, (hipStream_t)stream, p);
+                    const long long bytes = (long long)p.rows * p.n * sizeof(T) * ((p.block != nullptr) + 2 * (p.dy != nullptr) + (p.ds != nullptr) +
+                                                                                  (p.dr != nullptr) + (p.db != nullptr));
+                    by_passing(bytes, [&](auto passing) {
+                        if (p.after == TCBNN_NORM_LAYER || p.before == TCBNN_NORM_LAYER)
+                            hipLaunchKernelGGL(HIP_KERNEL_NAME(blocknorm_grad_kernel<T, W, R, true, passing.value>), dim3((unsigned)parts), dim3(kGradThreads), 0,
+                                               (hipStream_t)stream, p);
+                        else
+                            hipLaunchKernelGGL(HIP_KERNEL_NAME(blocknorm_grad_kernel<T, W, R, false, passing.value>), dim3((unsigned)parts), dim3(kGradThreads), 0,
+                                               (hipStream_t)stream, p);
+                    });
                 }
             });
         });

@@ -16,14 +16,15 @@ struct RowSlice {
     static constexpr int kStep = 64 * W * V;  // elements that one vector of every lane covers
     float v[R][V];
 
-    // A row's vectors are requested a step before they are taken up: what lies past the row is 0.
+    // A row's vectors are requested a step before they are taken up: what lies past the row is 0.  PASSING: nothing of the row stays in the caches.
     using Raw = Vec<T>[R];
+    template <bool PASSING = false>
     static __device__ __forceinline__ void request(const T* __restrict__ row, int lane, int n, Raw& raw) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int i = r * kStep + lane * V;
             if ((r + 1) * kStep <= n || i + V <= n) {
-                raw[r] = load_vec(row + i);
+                raw[r] = PASSING ? __builtin_nontemporal_load(reinterpret_cast<const VecAnywhere<T>*>(row + i)) : load_vec(row + i);
             } else {
 #pragma unroll
                 for (int e = 0; e < V; ++e) raw[r][e] = i + e < n ? row[i + e] : (T)0.0f;
@@ -36,6 +37,7 @@ struct RowSlice {
 #pragma unroll
             for (int e = 0; e < V; ++e) v[r][e] = (float)raw[r][e];
     }
+    template <bool PASSING = false>
     __device__ __forceinline__ void store(T* __restrict__ row, int lane, int n) const {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -44,7 +46,10 @@ struct RowSlice {
                 Vec<T> x;
 #pragma unroll
                 for (int e = 0; e < V; ++e) x[e] = (T)v[r][e];
-                store_vec(row + i, x);
+                if constexpr (PASSING)
+                    __builtin_nontemporal_store(x, reinterpret_cast<VecAnywhere<T>*>(row + i));
+                else
+                    store_vec(row + i, x);
             } else {
 #pragma unroll
                 for (int e = 0; e < V; ++e)
