@@ -63,10 +63,18 @@ void by_passing(long long bytes, F&& f) {
     f(std::false_type());
 }
 
+// Wavefronts a SIMD that the forward kernel's registers are to do for.  Two teams of 16 wavefronts a compute unit with RMS norms (3000 x 8000 bf16 46 us), one
+// with layer norms, whose parameters take the registers (63 us; two that read their parameters anew for every row 103).  Of smaller teams
+// three workgroups of 8 wavefronts with RMS norms and two with layer norms (8000 x 4000 67 us, three 79 with registers in memory).
+constexpr int waves_wanted(int w, int values, bool layer) {
+    if (values > kHeld) return 4;
+    if (w == 16) return values <= (layer ? kHeld / 2 : kHeld) ? 8 : 4;
+    return layer ? 5 : 6;
+}
 // LAYER: either norm may have means.  All teams of a workgroup take the same number of steps; one without a row of its own computes on the
 // last one and keeps nothing.  Two sets of slots in turn: between two sums into one slot lies the barrier of a row in between.
 template <typename T, int W, int R, bool LAYER, bool PASSING>
-__global__ __launch_bounds__(forward_threads(W)) void blocknorm_kernel(const NormsParams p) {
+__global__ __launch_bounds__(forward_threads(W)) __attribute__((amdgpu_waves_per_eu(waves_wanted(W, R * Elem<T>::kVec, LAYER)))) void blocknorm_kernel(const NormsParams p) {
     constexpr int kTeams = forward_threads(W) / (64 * W);
     using Slice = RowSlice<T, W, R>;
     constexpr int V = Slice::V;
@@ -260,22 +268,32 @@ __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const Norm
     float next[4];
     const bool with_block = p.block != nullptr;
     const long long stride = (long long)gridDim.x * kTeams;
-    auto request = [&](long long first) {
-        const long long row = min(first + team, (long long)p.rows - 1);
-        if (p.ds) Slice::template request<PASSING>((const T*)p.ds + row * p.ds_ld, lane, n, raw_ds);
+    // What a phase of a row reads is requested when the phase of the row before has taken its own: less lies in registers at a time.
+    auto row_of = [&](long long first) { return min(first + team, (long long)p.rows - 1); };
+    auto request_dy = [&](long long row) {
         if (p.dy) {
             next[2] = LAYER && p.before == TCBNN_NORM_LAYER ? p.before_mean[row] : 0.0f;
             next[3] = p.before_rstd[row];
             Slice::template request<PASSING>((const T*)p.dy + row * p.dy_ld, lane, n, raw_dy);
             Slice::template request<PASSING>((const T*)p.stream + row * p.stream_ld, lane, n, raw_s);
         }
+    };
+    auto request_ds = [&](long long row) {
+        if (p.ds) Slice::template request<PASSING>((const T*)p.ds + row * p.ds_ld, lane, n, raw_ds);
+    };
+    auto request_block = [&](long long row) {
         if (with_block) {
             next[0] = LAYER && p.after == TCBNN_NORM_LAYER ? p.after_mean[row] : 0.0f;
             next[1] = p.after ? p.after_rstd[row] : 1.0f;
             Slice::template request<PASSING>((const T*)p.block + row * p.block_ld, lane, n, raw_u);
         }
     };
-    request((long long)blockIdx.x * kTeams);
+    {
+        const long long row = row_of((long long)blockIdx.x * kTeams);
+        request_dy(row);
+        request_ds(row);
+        request_block(row);
+    }
     load_after(p, p.after_gamma, P, lane, n);
     g.load_param(p.before_gamma, lane, n, 1.0f);
 #pragma unroll
@@ -307,23 +325,16 @@ __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const Norm
     int parity = 0;
     for (long long first = (long long)blockIdx.x * kTeams; first < p.rows; first += stride, parity ^= 1) {
         const bool mine = first + team < p.rows;
-        const long long row = min(first + team, (long long)p.rows - 1);
+        const long long row = row_of(first);
         float (*slot)[W] = slots[parity][team];
-        const float mean1 = next[0], rstd1 = next[1], mean2 = next[2], rstd2 = next[3];
-        Slice e_, y;  // dy, the block's output
-        if (p.ds) {
-            d.take(raw_ds);
-        } else {
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int e = 0; e < V; ++e) d.v[r][e] = 0.0f;
-        }
+        const bool more = first + stride < p.rows;
+        const long long next_row = row_of(first + stride);
+        const float mean2 = next[2], rstd2 = next[3];
+        Slice e_;  // dy
         if (p.dy) e_.take(raw_dy), x.take(raw_s);
-        if (with_block) y.take(raw_u);
-        if (first + stride < p.rows) request(first + stride);
+        if (more) request_dy(next_row);
+        float sg = 0.0f, sgx = 0.0f;
         if (p.dy) {
-            float sg = 0.0f, sgx = 0.0f;
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -339,6 +350,17 @@ __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const Norm
                     sgx = __builtin_fmaf(gv, xh, sgx);
                 }
             row_sums(slot, p.before, sg, sgx);
+        }
+        if (p.ds) {
+            d.take(raw_ds);
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int e = 0; e < V; ++e) d.v[r][e] = 0.0f;
+        }
+        if (more) request_ds(next_row);
+        if (p.dy) {
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -350,7 +372,11 @@ __global__ __launch_bounds__(kGradThreads) void blocknorm_grad_kernel(const Norm
         }
         if (mine && p.dr) d.template store<PASSING>((T*)p.dr + row * p.dr_ld, lane, n);
         if (!with_block) continue;
-        float sg = 0.0f, sgx = 0.0f;
+        const float mean1 = next[0], rstd1 = next[1];
+        Slice& y = x;  // the block's output
+        y.take(raw_u);
+        if (more) request_block(next_row);
+        sg = sgx = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -613,7 +639,7 @@ extern "C" int tcbnn_blocknorm_forward(const tcbnn_blocknorm_desc* d, void* stre
             const bool layer = p.after == TCBNN_NORM_LAYER || p.before == TCBNN_NORM_LAYER;
             // As many workgroups as a compute unit has registers for, more where rows are left: 16384 x 4096 bf16 with a fourth of 512 threads, which
             // begins when the others end, 132 us, three 106.
-            const long long threads = R * Elem<T>::kVec > kHeld ? 1024 : layer ? 1280 : 1536;
+            const long long threads = 256 * waves_wanted(W, R * Elem<T>::kVec, layer);
             const dim3 blocks((unsigned)std::min((p.rows + teams - 1LL) / teams, kComputeUnits * (threads / forward_threads(W))));
             const long long bytes = (long long)p.rows * p.n * sizeof(T) * (1 + (p.block != nullptr) + (p.out != nullptr) + (p.y != nullptr));
             by_passing(bytes, [&](auto passing) {
