@@ -388,5 +388,5 @@ extern "C" int tcbnn_gated_backward(const tcbnn_gated_grad_desc* d, void* stream
     dw.out = d->grad_weight;
     dw.out_ld = dw_ld;
     return launch_gradient_products(d->dtype, dx, dw, d->rows > 0 ? (float*)((char*)d->workspace + before) : nullptr,
-                                    d->rows > 0 ? d->workspace_bytes - before : 0, (hipStream_t)stream);
+                                    d->rows > 0 ? d->workspace_bytes - before : 0, (hipStream_t)stream, true);
 }

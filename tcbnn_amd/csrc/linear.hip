@@ -333,6 +333,42 @@ bool launch_small_gradients(ProductParams dx, ProductParams dw, size_t workspace
     return true;
 }
 
+// ---- both products of large gradients in one launch, where neither has a tile of 256 for every compute unit: the first `blocks` workgroups have the one with
+// the longer sum.  (Gated product of 8192 x 1024 -> 2 x 4096 bf16 with its pass over dz: 303 us, 372 in launches of their own.)
+template <typename T>
+__global__ __launch_bounds__(512) void large_gradients_kernel(const ProductParams dx, const ProductParams dw, int blocks, bool dw_first) {
+    __shared__ __align__(1024) char lds[product_lds<256, 256, 2, 4, 1, 2>()];
+    const int second = (int)blockIdx.x >= blocks, block = (int)blockIdx.x - (second ? blocks : 0);
+    if (second == dw_first)
+        product<T, 256, 256, 2, 4, 1, 2, WHOLE_PIECES, 1, false, false, true, false>(dx, block, lds);
+    else
+        product<T, 256, 256, 2, 4, 1, 2, WHOLE_PIECES, 1, false, true, true, false>(dw, block, lds);
+}
+// A step of a tile of 256 across the sum, where every compute unit has one: 1.75 us measured in both (as long products alone have it, 1.6, and the plans).
+template <typename T>
+bool launch_large_gradients(ProductParams dx, ProductParams dw, size_t workspace_bytes, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2) {
+        if (dx.plane || dx.carry || access_of<T, false, true>(dx) != WHOLE_PIECES || access_of<T, true, true>(dw) != WHOLE_PIECES) return false;
+        constexpr float kStep = 1.75f;
+        cut_product(dx, 256, kStepBytes / (int)sizeof(T), 1, nullptr);
+        cut_product(dw, 256, kStepBytes / (int)sizeof(T), 1, nullptr);
+        const long long blocks_dx = (long long)dx.tiles_i * dx.tiles_j, blocks_dw = (long long)dw.tiles_i * dw.tiles_j;
+        if (blocks_dx + blocks_dw > 2 * kComputeUnits) return false;
+        const float steps_dx = (float)(dx.split_sum / (kStepBytes / (int)sizeof(T))), steps_dw = (float)(dw.split_sum / (kStepBytes / (int)sizeof(T)));
+        // in one round the longer sum; otherwise what is left over begins when the first are done
+        const float longest = std::max(steps_dx, steps_dw), work = ((float)blocks_dx * steps_dx + (float)blocks_dw * steps_dw) / (float)kComputeUnits;
+        const float together = kCuts16[CUT_256].start + kStep * (blocks_dx + blocks_dw <= kComputeUnits ? longest : longest + work);
+        float apart = 0.0f;
+        for (const ProductParams* p : {&dx, &dw}) apart += plan_product(p->rows, p->cols, p->sum, (int)sizeof(T), true, workspace_bytes).time;
+        if (together >= apart) return false;
+        const bool dw_first = steps_dw > steps_dx;
+        hipLaunchKernelGGL(large_gradients_kernel<T>, dim3((unsigned)(blocks_dx + blocks_dw)), dim3(512), 0, stream, dx, dw, (int)(dw_first ? blocks_dw : blocks_dx),
+                           dw_first);
+        return true;
+    }
+    return false;
+}
+
 // Tiles of 64 whose rows lie anywhere: the loop for long sums takes registers that a third workgroup of a compute unit would have
 // (bf16, with that loop / without: 1000 x 1001 x 999, one tile a compute unit, 9.8 us / 13.5; 2000 x 777 x 1111, three, 24.4 / 19.6).
 template <typename T>
@@ -489,11 +525,16 @@ size_t gradient_product_bytes(int rows, int in_features, int out_features, int d
     return std::max(split_bytes(rows, in_features, out_features, dtype, false), split_bytes(out_features, in_features, rows, dtype, false));
 }
 
-int launch_gradient_products(int dtype, const ProductParams& dx, const ProductParams& dw, float* workspace, size_t workspace_bytes, hipStream_t stream) {
+int launch_gradient_products(int dtype, const ProductParams& dx, const ProductParams& dw, float* workspace, size_t workspace_bytes, hipStream_t stream,
+                             bool together) {
     return by_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
         if (dx.out && dw.out && dx.rows > 0 && !dx.carry && launch_small_gradients<T>(dx, dw, workspace_bytes, stream)) {
             TCBNN_LAUNCH_CHECK("small_gradients_kernel");
+            return TCBNN_OK;
+        }
+        if (together && dx.out && dw.out && dx.rows > 0 && launch_large_gradients<T>(dx, dw, workspace_bytes, stream)) {
+            TCBNN_LAUNCH_CHECK("large_gradients_kernel");
             return TCBNN_OK;
         }
         if (dx.out && dx.rows > 0)

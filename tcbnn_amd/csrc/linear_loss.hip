@@ -391,7 +391,7 @@ inline int carried_splits(int rows, int in_features, int piece, int size) {
 // In 16 bits d is rounded before it is multiplied.  A row of d, and a column, is often little else than its given class' value, whose rounding then is that
 // of all that it is multiplied with.  Over many rows these errors, like those of the sums' other terms, come to sqrt 2 of what rounding the results
 // leaves (8192 rows bf16: 0.0024 of them, 0.0017 the rounding); few rows may be off by twice that.  Up to kTwoPlaneRows rows d is kept in
-// two planes, its rounding and what that left, and both products sum over both.  (@@)
+// two planes, its rounding and what that left, and both products sum over both.
 constexpr int kTwoPlaneRows = 256;
 inline bool two_planes(int rows, int dtype) { return dtype != TCBNN_F32 && rows <= kTwoPlaneRows; }
 // where the second plane of a sum of n begins: whole steps
@@ -624,7 +624,7 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             dw.sum = d->rows;
             dw.out = d->grad_weight ? (T*)d->grad_weight + first * dw_ld : nullptr;
             dw.out_ld = dw_ld;
-            if (int rc = launch_gradient_products(d->dtype, dx, dw, (float*)(base + w.split), w.total - w.split, s)) return rc;
+            if (int rc = launch_gradient_products(d->dtype, dx, dw, (float*)(base + w.split), w.total - w.split, s, true)) return rc;
         }
         if (w.piece < d->classes && d->grad_input) {
             dx.partial_stride = (long long)d->rows * d->in_features;

@@ -322,8 +322,8 @@ struct ProductParams {
     long long partial_stride;  // from one split's to the next one's
     int carry;             // the sum goes on in `partial`: CARRY_FIRST writes it, CARRY_ON adds to what is there
     const float* factor;   // of the sums, or NULL (a power of two: nothing is rounded by it)
-    // I in two planes whose products are added: the sum goes over the first, `sum` long, and from `plane` on over the second, which lies i_low
-    // elements behind it; J is the same for both.  0: one plane.
+    // I in two planes whose products are added, the second i_low elements behind the first: the sum goes over a step of the first and the same step of the
+    // second in turn, so that J's steps are in the cache when they are read again.  `plane`: the sum in whole steps (0: one plane).
     int plane;
     long long i_low;
     bool padded;           // I's rows, 16 bytes or more, go on with zeros to whole 16 bytes
@@ -408,7 +408,7 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
     constexpr int V = Elem<T>::kVec;
     ti.init(p.i, i0, ACROSS_I && p.padded ? ((long long)p.rows + V - 1) / V * V : (long long)p.rows);
     tj.init(p.j, j0, p.cols);
-    const int s0 = split * p.split_sum, s1 = min(PLANES ? p.plane + p.sum : p.sum, s0 + p.split_sum);
+    const int s0 = split * p.split_sum, s1 = min(PLANES ? 2 * p.plane : p.sum, s0 + p.split_sum);
     const int share = wave / (WI * WJ), wi = wave / WJ % WI * (32 * NI), wj = wave % WJ * (32 * NJ);
     spot = {split, tile_i, tile_j, share, wi, wj, wave, lane, i0, j0};
 
@@ -423,7 +423,7 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
     constexpr integral_constant<int, 0> slot0;
     const int steps = (s1 - s0 + TileI::kSteps - 1) / TileI::kSteps;
     // (a step past the last one: requests that touch no memory)
-    // where a step begins: in the sum of its plane, that plane's end (or the split's), the plane
+    // where a step begins: in the sum of its plane, the sum's end (or the split's), the plane
     struct Step {
         int s, end;
         long long i_plane;
@@ -431,8 +431,8 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
     auto where = [&](int step) -> Step {
         const int s = s0 + step * TileI::kSteps;
         if constexpr (!PLANES) return {s, s1, 0};
-        const int before = s >= p.plane ? p.plane : 0;
-        return {s - before, min(p.sum, s1 - before), before ? p.i_low : 0};
+        const int nth = s / TileI::kSteps;
+        return {nth / 2 * TileI::kSteps, s < s1 ? p.sum : 0, nth % 2 ? p.i_low : 0};
     };
     auto request_i = [&](int stage, int step, auto slot) {
         const Step at = where(step);
@@ -797,9 +797,9 @@ void by_tile(Access access, Cut cut, F&& f) {
 inline void cut_product(ProductParams& p, int size, int steps_size, int splits, float* workspace) {
     p.tiles_i = (p.rows + size - 1) / size;
     p.tiles_j = (p.cols + size - 1) / size;
-    const int steps = (p.plane + p.sum + steps_size - 1) / steps_size;
+    const int steps = p.plane ? 2 * p.plane / steps_size : (p.sum + steps_size - 1) / steps_size;
     p.split_sum = std::max(1, (steps + splits - 1) / splits) * steps_size;
-    p.splits = std::max(1, (p.plane + p.sum + p.split_sum - 1) / p.split_sum);
+    p.splits = std::max(1, ((p.plane ? 2 * p.plane : p.sum) + p.split_sum - 1) / p.split_sum);
     p.partial = workspace;
     p.partial_stride = (long long)p.rows * p.cols;
 }
@@ -861,7 +861,9 @@ inline size_t whole_lines(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // ---- (linear.hip)  dx = d w and dw = d^T x, each where it has an `out`; with dx.carry its sum stays in its `partial`, whose number of splits is
 // dx.splits.  The workspace is for split sums (gradient_product_bytes; without one none is split).
 size_t gradient_product_bytes(int rows, int in_features, int out_features, int dtype);
-int launch_gradient_products(int dtype, const ProductParams& dx, const ProductParams& dw, float* workspace, size_t workspace_bytes, hipStream_t stream);
+// `together`: both in one launch of large tiles too, where that is estimated to take less time.
+int launch_gradient_products(int dtype, const ProductParams& dx, const ProductParams& dw, float* workspace, size_t workspace_bytes, hipStream_t stream,
+                             bool together = false);
 // a carried sum -> dx.out
 int launch_carried_sum(int dtype, const ProductParams& dx, hipStream_t stream);
 // out[n] = the sums of `parts` rows of n, in one order
