@@ -1,4 +1,5 @@
-"""The floating point end of a network: linear layers, layer norms and log probabilities, forward and backward.
+"""The floating point end of a network: linear layers, layer norms, log probabilities, gated products, norms around a residual block and
+the loss of a linear classifier, forward and backward.
 
 The layers are objects like those of layers.py: a constructor with the sizes, `initialize` with parameters and buffers,
 `forward(stream)` and `backward(stream)` as stream-ordered launches that allocate nothing, `download_*` and `release`.
@@ -498,7 +499,35 @@ class LinearLossLayerParam(_HeadLayer):
         return {"loss": self.loss_gpu.to_numpy(np.float32, (self.rows,)), "logsumexp": self.logsumexp_gpu.to_numpy(np.float32, (self.rows,))}
 
 
-class FloatHead:
+class _Head:
+    """What heads share: `params` (fp32 host arrays by name, those of weights beginning with w), `_devices` and `_grads` (their buffers and
+    their gradients' by the same names), `layers` in the order that forward() takes them."""
+
+    def forward(self, stream=None):
+        for layer in self.layers:
+            layer.forward(stream)
+
+    def backward(self, stream=None):
+        """The gradients of all parameters, of the mean cross entropy of the last forward()."""
+        for layer in reversed(self.layers):
+            layer.backward(stream)
+
+    def gradients(self):
+        """fp32 host arrays of the last backward()'s gradients, by parameter."""
+        _lib.device_synchronize()
+        out = {}
+        for name, a in self.params.items():
+            dt = self.dtype if name[0] == "w" else "f32"
+            out[name] = decode(self._grads[name].to_numpy(storage(dt), a.shape), dt)
+        return out
+
+    def step(self, rate):
+        for name, g in self.gradients().items():
+            self.params[name] -= np.float32(rate) * g
+            self._devices[name].upload(encode(self.params[name], self.dtype if name[0] == "w" else "f32"))
+
+
+class FloatHead(_Head):
     """A float head on `features` values a row, as on the last binary layer of a network:
     norm -> linear (GELU), + the features where there are as many hidden values -> norm -> linear -> log probabilities of
     `classes`.  The features are given (the network below them is frozen): they get no gradient.
@@ -550,36 +579,117 @@ class FloatHead:
                          "gamma2": n2.gamma_gpu, "beta2": n2.beta_gpu, "w2": l2.weight_gpu, "b2": l2.bias_gpu}
         return self
 
-    def forward(self, stream=None):
-        for layer in self.layers:
-            layer.forward(stream)
-
-    def backward(self, stream=None):
-        """The gradients of all parameters, of the mean cross entropy of the last forward()."""
-        for layer in reversed(self.layers):
-            layer.backward(stream)
-
     def loss(self):
         """The mean cross entropy of the last forward()."""
         _lib.device_synchronize()
         return -float(self.logprobs.logprob_gpu.to_numpy(np.float32, (self.rows,)).astype(np.float64).sum()) / self._given
 
-    def gradients(self):
-        """fp32 host arrays of the last backward()'s gradients, by parameter."""
-        _lib.device_synchronize()
-        out = {}
-        for name, a in self.params.items():
-            dt = self.dtype if name[0] == "w" else "f32"
-            out[name] = decode(self._grads[name].to_numpy(storage(dt), a.shape), dt)
-        return out
-
-    def step(self, rate):
-        for name, g in self.gradients().items():
-            self.params[name] -= np.float32(rate) * g
-            self._devices[name].upload(encode(self.params[name], self.dtype if name[0] == "w" else "f32"))
-
     def release(self):
         for layer in self.layers:
+            layer.release()
+        for buf in [self._targets, self._loss] + self._flows + list(self._grads.values()):
+            buf.free()
+
+
+class GatedHead(_Head):
+    """A float head of gated residual blocks on `features` values a row:
+    norm -> [gated product (SiLU) -> linear, normed, gated and added to the stream, norm] x blocks -> linear loss over `classes`,
+    with RMS norms.  The features are given (the network below them is frozen): they get no gradient.
+
+    forward() computes the rows' losses, without logits; backward() leaves the gradient of the mean cross entropy in the layers' gradient
+    buffers; step() takes a step of gradient descent; score() ranks the best classes of the last forward()."""
+
+    def __init__(self, rows, features, hidden, classes, dtype="f32", blocks=1, scale=0.5, top=5):
+        if blocks < 1:
+            raise _lib.TcbnnError("Error: a gated head of %d blocks" % blocks)
+        self.rows, self.features, self.hidden, self.classes, self.dtype, self.blocks = rows, features, hidden, classes, dtype, blocks
+        self.norm = BlockNormLayerParam("Norm", rows, features, dtype)
+        self.gated = [GatedLayerParam("Gated%d" % i, rows, features, hidden, dtype) for i in range(blocks)]
+        self.down = [LinearLayerParam("Down%d" % i, rows, hidden, features, dtype) for i in range(blocks)]
+        self.norms = [BlockNormLayerParam("Norms%d" % i, rows, features, dtype, after="rms", scale=scale) for i in range(blocks)]
+        self.linear_loss = LinearLossLayerParam("Loss", rows, features, classes, dtype)
+        self.classifier = LinearLayerParam("Classifier", rows, features, classes, dtype)
+        self.logprobs = LogProbsLayerParam("LogProbs", rows, classes, min(top, classes), dtype)
+        self.layers = [self.norm]
+        for block in zip(self.gated, self.down, self.norms):
+            self.layers += block
+        self.layers.append(self.linear_loss)
+        self._score = None
+
+    def initialize(self, features_gpu, targets, seed=0):
+        """features_gpu: [rows][features] in the head's dtype; targets: int32 [rows], -1 for rows without a class."""
+        if np.size(targets) != self.rows:
+            raise _lib.TcbnnError("Error: %d targets for %d rows" % (np.size(targets), self.rows))
+        rng = np.random.default_rng(seed)
+        k, h, c, m, size = self.features, self.hidden, self.classes, self.rows, 4 if self.dtype == "f32" else 2
+
+        def weight(out, inp):
+            return rng.normal(0, inp ** -0.5, (out, inp)).astype(np.float32)
+
+        p = self.params = {"gamma": np.ones(k, np.float32)}
+        for i in range(self.blocks):
+            p.update({"w_gated%d" % i: weight(2 * h, k), "b_gated%d" % i: np.zeros(2 * h, np.float32), "w_down%d" % i: weight(k, h),
+                      "gate%d" % i: np.ones(k, np.float32), "gamma_after%d" % i: np.ones(k, np.float32),
+                      "gamma_before%d" % i: np.ones(k, np.float32)})
+        p.update({"w_class": weight(c, k), "b_class": np.zeros(c, np.float32)})
+        targets = np.ascontiguousarray(targets, np.int32)
+        self._given = max(1, int((targets >= 0).sum()))
+        self._targets = DeviceBuffer.from_numpy(targets)
+        self._loss = DeviceBuffer.from_numpy(np.where(targets >= 0, np.float32(1.0 / self._given), np.float32(0)))
+        g = self._grads = {name: DeviceBuffer(a.size * (size if name[0] == "w" else 4)) for name, a in p.items()}
+        self._flows = []
+
+        def flow(cols):
+            self._flows.append(DeviceBuffer(m * cols * size))
+            return self._flows[-1]
+
+        self.norm.initialize(features_gpu, before_gamma=p["gamma"])
+        stream, y = features_gpu, self.norm.output_gpu
+        for i, (gated, down, norms) in enumerate(zip(self.gated, self.down, self.norms)):
+            gated.initialize(p["w_gated%d" % i], p["b_gated%d" % i], y, save_preact=True)
+            down.initialize(p["w_down%d" % i], None, gated.output_gpu)
+            norms.initialize(stream, down.output_gpu, gate=p["gate%d" % i], after_gamma=p["gamma_after%d" % i], before_gamma=p["gamma_before%d" % i])
+            stream, y = norms.new_stream_gpu, norms.output_gpu
+        self.linear_loss.initialize(p["w_class"], p["b_class"], y, self._targets)
+        d_y, d_stream = flow(k), None
+        self.linear_loss.initialize_backward(self._loss, d_y, g["w_class"], g["b_class"])
+        for i in reversed(range(self.blocks)):
+            d_block, d_hidden, before = flow(k), flow(h), flow(k) if i else None  # (the features get no gradient)
+            self.norms[i].initialize_backward(d_y, d_stream, before, d_block, g["gate%d" % i], g["gamma_after%d" % i],
+                                              grad_before_gamma_gpu=g["gamma_before%d" % i])
+            self.down[i].initialize_backward(d_block, d_hidden, g["w_down%d" % i])
+            d_y = flow(k)
+            self.gated[i].initialize_backward(d_hidden, d_y, g["w_gated%d" % i], g["b_gated%d" % i])
+            d_stream = before
+        self.norm.initialize_backward(d_y, grad_before_gamma_gpu=g["gamma"])
+        self._devices = {"gamma": self.norm.before_gamma_gpu, "w_class": self.linear_loss.weight_gpu, "b_class": self.linear_loss.bias_gpu}
+        for i in range(self.blocks):
+            self._devices.update({"w_gated%d" % i: self.gated[i].weight_gpu, "b_gated%d" % i: self.gated[i].bias_gpu,
+                                  "w_down%d" % i: self.down[i].weight_gpu, "gate%d" % i: self.norms[i].gate_gpu,
+                                  "gamma_after%d" % i: self.norms[i].after_gamma_gpu, "gamma_before%d" % i: self.norms[i].before_gamma_gpu})
+        self._score = None
+        return self
+
+    def loss(self):
+        """The mean cross entropy of the last forward()."""
+        _lib.device_synchronize()
+        return float(self.linear_loss.loss_gpu.to_numpy(np.float32, (self.rows,)).astype(np.float64).sum()) / self._given
+
+    def score(self, stream=None):
+        """Log probabilities, ranks and best classes of the last forward()'s rows (LogProbsLayerParam's outputs): with logits, which the
+        first call makes room for."""
+        if self._score is None:
+            last = self.linear_loss
+            self.classifier.initialize(last.weight_gpu, last.bias_gpu, last.input_gpu)
+            self.logprobs.initialize(self.classifier.output_gpu, self._targets)
+            self._score = [self.classifier, self.logprobs]
+        for layer in self._score:
+            layer.forward(stream)
+        _lib.device_synchronize()
+        return self.logprobs.download_output()
+
+    def release(self):
+        for layer in self.layers + [self.classifier, self.logprobs]:
             layer.release()
         for buf in [self._targets, self._loss] + self._flows + list(self._grads.values()):
             buf.free()

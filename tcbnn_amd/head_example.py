@@ -2,6 +2,9 @@
 labels, then used to score a batch.
 
     python -m tcbnn_amd.head_example [--batch 1024] [--hidden 1024] [--classes 10] [--steps 40] [--rate 0.02] [--dtype f32]
+                                      [--head float|gated] [--blocks 1]
+
+--head gated takes gated residual blocks and a loss that keeps no logits in place of the two linear layers.
 
 The labels are those of a random linear rule on the images, so the loss falls from log(classes)."""
 import argparse
@@ -11,7 +14,7 @@ import numpy as np
 from . import _lib, nets
 from ._lib import check, lib
 from .device import DeviceBuffer
-from .head import FloatHead, encode
+from .head import FloatHead, GatedHead, encode
 
 
 def binary_features(batch, width=1024, seed=0):
@@ -34,6 +37,8 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=40)
     ap.add_argument("--rate", type=float, default=0.02)
     ap.add_argument("--dtype", choices=sorted(_lib.DTYPES), default="f32")
+    ap.add_argument("--head", choices=["float", "gated"], default="float")
+    ap.add_argument("--blocks", type=int, default=1)
     a = ap.parse_args(argv)
     features, images, trunk = binary_features(a.batch, a.hidden)
     rule = np.random.default_rng(1).standard_normal((images.shape[1], a.classes)).astype(np.float32)
@@ -41,7 +46,10 @@ def main(argv=None):
     if a.dtype != "f32":  # +-1 is exact in every type
         bits = encode(features.to_numpy(np.float32, (a.batch, a.hidden)), a.dtype)
         features = DeviceBuffer.from_numpy(bits)
-    head = FloatHead(a.batch, a.hidden, a.hidden, a.classes, a.dtype).initialize(features, targets)
+    if a.head == "gated":
+        head = GatedHead(a.batch, a.hidden, a.hidden, a.classes, a.dtype, a.blocks).initialize(features, targets)
+    else:
+        head = FloatHead(a.batch, a.hidden, a.hidden, a.classes, a.dtype).initialize(features, targets)
     losses = []
     for step in range(a.steps + 1):
         head.forward()
@@ -49,7 +57,7 @@ def main(argv=None):
         if step < a.steps:
             head.backward()
             head.step(a.rate)
-    scores = head.logprobs.download_output()
+    scores = head.score() if a.head == "gated" else head.logprobs.download_output()
     k = head.logprobs.top
     print("loss %.4f -> %.4f in %d steps; top-1 %.1f %%, top-%d %.1f %%, mean entropy %.3f nats" % (
         losses[0], losses[-1], a.steps, 100 * (scores["rank"] == 0).mean(), k, 100 * (scores["rank"] < k).mean(),

@@ -258,3 +258,13 @@ def test_norms_gradient_is_the_definitions(after, before):
             return total(x, b, {**p, names[name]: p[names[name]] + t * v})
         h = 1e-5
         assert abs((at(h) - at(-h)) / (2 * h) - (g * v).sum()) < 1e-6, name
+
+
+def test_gated_head_refuses():
+    from tcbnn_amd._lib import TcbnnError
+    from tcbnn_amd.device import DeviceView
+    from tcbnn_amd.head import GatedHead
+    with pytest.raises(TcbnnError, match="blocks"):
+        GatedHead(4, 8, 8, 3, blocks=0)
+    with pytest.raises(TcbnnError, match="targets"):
+        GatedHead(4, 8, 8, 3).initialize(DeviceView(P, 128), np.zeros(3, np.int32))
