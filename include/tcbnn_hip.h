@@ -672,7 +672,7 @@ int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream);
  * a class and in rows whose classes are all forbidden (t >= classes: NaN):  grad_input = d * weight, grad_weight = d^T * input,
  * grad_bias = sums of d over the rows.  Each of the three may be NULL; what is given is overwritten.  The logits are made again, a piece
  * of the classes at a time; in 16-bit types d is rounded to dtype before the two products (in f16 times a power of two that keeps small
- * ones from getting lost); grad_bias sums it unrounded.  `logsumexp` is the forward call's; exp carries its rounding, |logsumexp| 2^-24.
+ * ones from getting lost); grad_bias sums it unrounded.  `logsumexp` is the forward call's; exp carries its rounding and one more like it, |logsumexp| 2^-23.
  * A row without a class still has to hold finite inputs: grad_weight sums 0 times them.  `workspace` holds
  * tcbnn_linear_loss_grad_workspace_bytes. */
 typedef struct tcbnn_linear_loss_grad_desc {

@@ -85,12 +85,13 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void loss_product_kernel(const P
 #pragma unroll
                 for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[a][b][v]);
             m = across_halves(m, larger);
-            const float c = m == -INFINITY ? 0.0f : m;
+            // (one fused multiply-add a logit: exponents about m log2 e as it is rounded, and the sum scaled back by what that rounding was)
+            const float base = m == -INFINITY ? 0.0f : m, c = base * kLog2e;
 #pragma unroll
             for (int b = 0; b < NJ; ++b)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) s += exp_fast(acc[a][b][v] - c);
-            s = across_halves(s, add);
+                for (int v = 0; v < 16; ++v) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][v], kLog2e, -c));
+            s = across_halves(s, add) * __builtin_amdgcn_exp2f(-__builtin_fmaf(base, kLog2e, -c));
             if (spot.lane < 32) rows[spot.wj / (32 * NJ) * BI + row] = make_float2(m, s);
             const long long i = spot.i0 + row;
             const long long t = l.targets && i < p.rows ? l.targets[i] - j0 : -1;
@@ -260,10 +261,18 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void loss_grad_product_kernel(co
             const float lse = l.lse[row];
             const bool none = i >= p.rows || t < 0 || lse == -INFINITY;
             const float g = t < l.classes ? l.dloss[row] : NAN;
+            // (about logsumexp log2 e as it is rounded: no more than logsumexp's own rounding)
+            const float c = lse * kLog2e;
 #pragma unroll
             for (int b = 0; b < NJ; ++b)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) acc[a][b][v] = none ? 0.0f : g * exp_fast(acc[a][b][v] - lse);
+                for (int v = 0; v < 16; ++v) acc[a][b][v] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][v], kLog2e, -c));
+            if (__any(none)) {
+#pragma unroll
+                for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) acc[a][b][v] = none ? 0.0f : acc[a][b][v];
+            }
             const long long at = (long long)t - l.first - j0 - 4 * (lane >> 5);
             if (__any(!none && at >= 0 && at < 32 * NJ)) {
 #pragma unroll
