@@ -559,7 +559,8 @@ int tcbnn_blocknorm_backward(const tcbnn_blocknorm_grad_desc* d, void* stream);
 
 /* A gated feed-forward product: z = input * weight^T + bias with 2 * features columns, the gate's first;
  * output = act(z of the gate) * (z of the rest).  `preact` receives z, rounded to dtype: what tcbnn_gated_backward needs.
- * rows <= 2^31 - 2^22, in_features <= 1048576, features <= 2^27. */
+ * `workspace` (tcbnn_gated_workspace_bytes; may be NULL) is for copies of operands whose rows do not lie at whole 16 bytes, where these are
+ * faster.  rows <= 2^31 - 2^22, in_features <= 1048576, features <= 2^27. */
 typedef struct tcbnn_gated_desc {
     const void* input;   /* [rows][in_features]         */
     const void* weight;  /* [2 * features][in_features] */
@@ -570,7 +571,10 @@ typedef struct tcbnn_gated_desc {
     int dtype;
     int activation;      /* TCBNN_ACT_*                 */
     long long input_ld, weight_ld, output_ld, preact_ld;
+    void* workspace;
+    size_t workspace_bytes;
 } tcbnn_gated_desc;
+size_t tcbnn_gated_workspace_bytes(int rows, int in_features, int features, int dtype);
 int tcbnn_gated_forward(const tcbnn_gated_desc* d, void* stream);
 /* Name of the kernel that tcbnn_gated_forward launches for this descriptor; nothing is launched, no pointer followed. */
 int tcbnn_gated_kernel_name(const tcbnn_gated_desc* d, char* buf, size_t len);
@@ -578,7 +582,8 @@ int tcbnn_gated_kernel_name(const tcbnn_gated_desc* d, char* buf, size_t len);
 /* With z as the forward call wrote it, dz of the gate = grad_output * (z of the rest) * act'(z of the gate), dz of the rest =
  * grad_output * act(z of the gate):  grad_input = dz * weight, grad_weight = dz^T * input, grad_bias = sums of dz over the rows.  Each of
  * the three may be NULL; what is given is overwritten.  relu'(0) = 0.  In 16-bit types dz is rounded to dtype before the two products;
- * grad_bias sums it unrounded.  `workspace` holds tcbnn_gated_grad_workspace_bytes. */
+ * grad_bias sums it unrounded.  `workspace` holds tcbnn_gated_grad_workspace_bytes; with `anywhere` these are enough for copies of operands whose
+ * rows do not lie at whole 16 bytes, where these are faster (without, such operands are read as they lie). */
 typedef struct tcbnn_gated_grad_desc {
     const void* input;        /* [rows][in_features]; NULL where grad_weight is          */
     const void* weight;       /* [2 * features][in_features]; NULL where grad_input is   */
@@ -594,7 +599,7 @@ typedef struct tcbnn_gated_grad_desc {
     void* workspace;
     size_t workspace_bytes;
 } tcbnn_gated_grad_desc;
-size_t tcbnn_gated_grad_workspace_bytes(int rows, int in_features, int features, int dtype);
+size_t tcbnn_gated_grad_workspace_bytes(int rows, int in_features, int features, int dtype, int anywhere);
 int tcbnn_gated_backward(const tcbnn_gated_grad_desc* d, void* stream);
 
 /* Of every row of logits x: logsumexp = log(sum exp(x_j)); logprob = x_t - logsumexp of the given class t = targets[row];
@@ -651,7 +656,8 @@ int tcbnn_logprobs_backward(const tcbnn_logprobs_grad_desc* d, void* stream);
  *   t < 0        : a row without a class: loss 0.   t >= classes: loss NaN.
  *   bias_j = -inf: a forbidden class; z_t = -inf: loss +inf; every z_j = -inf: logsumexp -inf.
  *   NaN, +inf    : the row's logsumexp and loss are NaN.
- * `workspace` holds tcbnn_linear_loss_workspace_bytes.  rows <= 2^31 - 2^22, in_features <= 1048576, classes <= 2^28. */
+ * `workspace` holds tcbnn_linear_loss_workspace_bytes; with `anywhere` these are enough for copies of operands whose rows do not lie at whole 16
+ * bytes, where these are faster (without, such operands are read as they lie).  rows <= 2^31 - 2^22, in_features <= 1048576, classes <= 2^28. */
 typedef struct tcbnn_linear_loss_desc {
     const void* input;       /* [rows][in_features]      */
     const void* weight;      /* [classes][in_features]   */
@@ -665,7 +671,7 @@ typedef struct tcbnn_linear_loss_desc {
     void* workspace;
     size_t workspace_bytes;
 } tcbnn_linear_loss_desc;
-size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, int classes, int dtype);
+size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, int classes, int dtype, int anywhere);
 int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream);
 
 /* The gradient of sum over rows of grad_loss * loss.  With d_j = grad_loss * (exp(z_j - logsumexp) - [j = t]), and d = 0 in rows without
@@ -674,7 +680,7 @@ int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream);
  * of the classes at a time; in 16-bit types d is rounded to dtype before the two products (in f16 times a power of two that keeps small
  * ones from getting lost); grad_bias sums it unrounded.  `logsumexp` is the forward call's; exp carries its rounding and one more like it, |logsumexp| 2^-23.
  * A row without a class still has to hold finite inputs: grad_weight sums 0 times them.  `workspace` holds
- * tcbnn_linear_loss_grad_workspace_bytes. */
+ * tcbnn_linear_loss_grad_workspace_bytes, `anywhere` as in the forward call. */
 typedef struct tcbnn_linear_loss_grad_desc {
     const void* input;       /* [rows][in_features]      */
     const void* weight;      /* [classes][in_features]   */
@@ -691,7 +697,7 @@ typedef struct tcbnn_linear_loss_grad_desc {
     void* workspace;
     size_t workspace_bytes;
 } tcbnn_linear_loss_grad_desc;
-size_t tcbnn_linear_loss_grad_workspace_bytes(int rows, int in_features, int classes, int dtype);
+size_t tcbnn_linear_loss_grad_workspace_bytes(int rows, int in_features, int classes, int dtype, int anywhere);
 int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, void* stream);
 
 /* ------------------------------------------------ standalone GEMM / conv */

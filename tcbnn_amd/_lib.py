@@ -141,7 +141,8 @@ class GatedDesc(C.Structure):
     _fields_ = [("input", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("output", c_void_p),
                 ("preact", c_void_p), ("rows", c_int), ("in_features", c_int), ("features", c_int), ("dtype", c_int),
                 ("activation", c_int), ("input_ld", C.c_longlong), ("weight_ld", C.c_longlong),
-                ("output_ld", C.c_longlong), ("preact_ld", C.c_longlong)]
+                ("output_ld", C.c_longlong), ("preact_ld", C.c_longlong),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
 class GatedGradDesc(C.Structure):
@@ -243,13 +244,14 @@ ABI = {
     "tcbnn_blocknorm_forward": (c_int, [C.POINTER(BlockNormDesc), c_void_p]),
     "tcbnn_blocknorm_grad_workspace_bytes": (c_size_t, [c_int] * 3),
     "tcbnn_blocknorm_backward": (c_int, [C.POINTER(BlockNormGradDesc), c_void_p]),
+    "tcbnn_gated_workspace_bytes": (c_size_t, [c_int] * 4),
     "tcbnn_gated_forward": (c_int, [C.POINTER(GatedDesc), c_void_p]),
     "tcbnn_gated_kernel_name": (c_int, [C.POINTER(GatedDesc), C.c_char_p, c_size_t]),
-    "tcbnn_gated_grad_workspace_bytes": (c_size_t, [c_int] * 4),
+    "tcbnn_gated_grad_workspace_bytes": (c_size_t, [c_int] * 5),
     "tcbnn_gated_backward": (c_int, [C.POINTER(GatedGradDesc), c_void_p]),
-    "tcbnn_linear_loss_workspace_bytes": (c_size_t, [c_int] * 4),
+    "tcbnn_linear_loss_workspace_bytes": (c_size_t, [c_int] * 5),
     "tcbnn_linear_loss_forward": (c_int, [C.POINTER(LinearLossDesc), c_void_p]),
-    "tcbnn_linear_loss_grad_workspace_bytes": (c_size_t, [c_int] * 4),
+    "tcbnn_linear_loss_grad_workspace_bytes": (c_size_t, [c_int] * 5),
     "tcbnn_linear_loss_backward": (c_int, [C.POINTER(LinearLossGradDesc), c_void_p]),
     "tcbnn_logprobs_workspace_bytes": (c_size_t, [c_int] * 4),
     "tcbnn_logprobs_forward": (c_int, [C.POINTER(LogProbsDesc), c_void_p]),

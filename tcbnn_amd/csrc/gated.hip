@@ -147,7 +147,7 @@ inline int gated_dz_parts(int rows, int vectors) {
 template <typename T, int ACT>
 __global__ __launch_bounds__(kDzThreads) void gated_dz_kernel(const T* __restrict__ dh, const T* __restrict__ z, T* __restrict__ dz,
                                                               float* __restrict__ sums, int rows, int n, int lanes, int each, long long dh_ld,
-                                                              long long z_ld) {
+                                                              long long z_ld, long long dz_ld) {
     constexpr int V = Elem<T>::kVec, kAtOnce = kGatedAtOnce;
     __shared__ float lds[2][kDzThreads * V];
     const int deep = kDzThreads / lanes, lane = threadIdx.x % lanes, depth = threadIdx.x / lanes;
@@ -198,9 +198,12 @@ __global__ __launch_bounds__(kDzThreads) void gated_dz_kernel(const T* __restric
                     s[0][e] += dg[e];
                     s[1][e] += du[e];
                 }
-                T* to = dz + (r + k * deep) * 2 * n + j;
+                T* to = dz + (r + k * deep) * dz_ld + j;
                 put(to, dg);
                 put(to + n, du);
+                if (left <= V) {  // (zeros to the row's whole 16 bytes)
+                    for (long long e = 2LL * n; e < dz_ld; ++e) dz[(r + k * deep) * dz_ld + e] = (T)0.0f;
+                }
             }
         }
     }
@@ -221,26 +224,36 @@ __global__ __launch_bounds__(kDzThreads) void gated_dz_kernel(const T* __restric
     }
 }
 
-// The tile is the one that the linear layer's estimates would take for a product of 2 n columns; sums are not split.
-template <typename T>
+// The tile is the one that the linear layer's estimates would take for a product of 2 n columns; sums are not split.  Operands that lie anywhere are
+// copied where the product of the copies and the copying are estimated to take less time, and the workspace holds them.
 struct GatedPlan {
     Access access;
     Plan plan;
-    bool few;
+    bool few, pack_i, pack_j;
 };
+inline GatedPlan plan_gated(int rows, int cols, int sum, int size, Access access, bool i_anywhere, bool j_anywhere, size_t workspace_bytes) {
+    const bool vectors = access == WHOLE_PIECES;
+    GatedPlan g = {access, plan_product(rows, 2 * cols, sum, size, vectors, 0), false, false, false};
+    g.few = rows <= kFewRows && (access == ELEMENTS || few_time(rows, 2 * cols, sum, size, vectors) < g.plan.time);
+    if (g.few || access != ANYWHERE) return g;
+    const Plan whole = plan_product(rows, 2 * cols, sum, size, true, 0);
+    const size_t i_bytes = i_anywhere ? packed_bytes(rows, sum, size) : 0, j_bytes = j_anywhere ? packed_bytes(2LL * cols, sum, size) : 0;
+    if (i_bytes + j_bytes > workspace_bytes) return g;
+    if (whole.time + (i_anywhere ? pack_time(i_bytes) : 0.0f) + (j_anywhere ? pack_time(j_bytes) : 0.0f) >= g.plan.time) return g;
+    return {WHOLE_PIECES, whole, false, i_anywhere, j_anywhere};
+}
 template <typename T>
-GatedPlan<T> plan_gated(const ProductParams& p) {
-    GatedPlan<T> g;
-    g.access = access_of<T, false, false>(p);
-    const bool vectors = g.access == WHOLE_PIECES;
-    g.plan = plan_product(p.rows, 2 * p.cols, p.sum, (int)sizeof(T), vectors, 0);
-    g.few = p.rows <= kFewRows && (g.access == ELEMENTS || few_time(p.rows, 2 * p.cols, p.sum, (int)sizeof(T), vectors) < g.plan.time);
-    return g;
+GatedPlan plan_gated(const ProductParams& p, size_t workspace_bytes) {
+    return plan_gated(p.rows, p.cols, p.sum, (int)sizeof(T), access_of<T, false, false>(p), lies_anywhere<T>(p.i, p.sum), lies_anywhere<T>(p.j, p.sum), workspace_bytes);
 }
 
 template <typename T>
-int launch_gated(const ProductParams& p, hipStream_t stream) {
-    const GatedPlan<T> g = plan_gated<T>(p);
+int launch_gated(ProductParams p, int dtype, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    const GatedPlan g = plan_gated<T>(p, workspace_bytes);
+    if (g.pack_i) p.i = launch_pack(dtype, p.i, p.rows, p.sum, workspace, stream);
+    if (g.pack_j) p.j = launch_pack(dtype, p.j, 2LL * p.cols, p.sum, (char*)workspace + (g.pack_i ? packed_bytes(p.rows, p.sum, (int)sizeof(T)) : 0), stream);
+    p.padded_i = g.pack_i;
+    p.padded_j = g.pack_j;
     if (g.few) {
         const int shares = few_shares(2 * p.cols, p.sum, (int)sizeof(T)), outputs = kFewPairs * kFewWaves / shares;
         const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
@@ -275,9 +288,9 @@ int launch_gated(const ProductParams& p, hipStream_t stream) {
 
 // the kernel that launch_gated takes, as a profiler lists it
 template <typename T>
-void gated_name(const ProductParams& p, char* buf, size_t len) {
+void gated_name(const ProductParams& p, size_t workspace_bytes, char* buf, size_t len) {
     const char* type = std::is_same_v<T, float> ? "float" : (std::is_same_v<T, _Float16> ? "_Float16" : "__bf16");
-    const GatedPlan<T> g = plan_gated<T>(p);
+    const GatedPlan g = plan_gated<T>(p, workspace_bytes);
     if (g.few) {
         snprintf(buf, len, "gated_few_rows_kernel<%s, %d>", type, few_shares(2 * p.cols, p.sum, (int)sizeof(T)));
         return;
@@ -317,10 +330,28 @@ ProductParams gated_product(const tcbnn_gated_desc* d) {
     return p;
 }
 
-// What the gradients need of a workspace: dz in dtype, then the parts of the column sums (whole 256 bytes each).
-size_t dz_bytes(int rows, int features, int dtype) { return whole_lines((size_t)rows * 2 * features * dtype_bytes(dtype)); }
-size_t sum_bytes(int rows, int features, int dtype) {
-    return rows == 0 ? 0 : whole_lines(sizeof(float) * gated_dz_parts(rows, out_vectors(features, dtype)) * 2 * (size_t)features);
+// What the gradients need of a workspace: dz in dtype, rows at whole 16 bytes, the parts of the column sums, copies of weights and input that lie
+// anywhere where the products' estimates say so, and what split sums need.
+struct GatedGradWorkspace {
+    size_t sums, weight, input, split, total;
+    bool pack_weight, pack_input;
+};
+GatedGradWorkspace grad_workspace(int rows, int in_features, int features, int dtype, bool anywhere) {
+    const int size = (int)dtype_bytes(dtype), n = 2 * features;
+    auto worth = [&](int i, int sum, size_t bytes) {
+        return anywhere && in_features * size >= 16 &&
+               plan_product(i, in_features, sum, size, true, 0).time + pack_time(bytes) < plan_product(i, in_features, sum, size, false, 0).time;
+    };
+    const size_t weight = packed_bytes(n, in_features, size), input = packed_bytes(rows, in_features, size);
+    GatedGradWorkspace w = {};
+    w.pack_weight = worth(rows, n, weight);
+    w.pack_input = worth(n, rows, input);
+    w.sums = packed_bytes(rows, n, size);
+    w.weight = w.sums + whole_lines(sizeof(float) * gated_dz_parts(rows, out_vectors(features, dtype)) * n);
+    w.input = w.weight + (w.pack_weight ? weight : 0);
+    w.split = w.input + (w.pack_input ? input : 0);
+    w.total = w.split + gradient_product_bytes(rows, in_features, n, dtype);
+    return w;
 }
 
 }  // namespace
@@ -329,11 +360,24 @@ size_t sum_bytes(int rows, int features, int dtype) {
 using namespace tcbnn;
 using namespace tcbnn::head;
 
+extern "C" size_t tcbnn_gated_workspace_bytes(int rows, int in_features, int features, int dtype) {
+    if (rows <= 0 || rows > kMaxRows || in_features <= 0 || in_features > kMaxIn || features <= 0 || features > tcbnn::kMaxFeatures || !dtype_known(dtype)) return 0;
+    const int size = (int)dtype_bytes(dtype);
+    if (in_features * size < 16) return 0;
+    size_t need = 0;
+    for (bool i : {false, true})  // (where the operands will lie is not known here)
+        for (bool j : {false, true}) {
+            const GatedPlan g = plan_gated(rows, features, in_features, size, ANYWHERE, i, j, ~(size_t)0);
+            need = std::max(need, (g.pack_i ? packed_bytes(rows, in_features, size) : 0) + (g.pack_j ? packed_bytes(2LL * features, in_features, size) : 0));
+        }
+    return need;
+}
+
 extern "C" int tcbnn_gated_kernel_name(const tcbnn_gated_desc* d, char* buf, size_t len) {
     TCBNN_NOTNULL(d);
     TCBNN_NOTNULL(buf);
     if (int rc = check_gated(d->rows, d->in_features, d->features, d->dtype, d->activation)) return rc;
-    by_dtype(d->dtype, [&](auto t) { gated_name<decltype(t)>(gated_product(d), buf, len); });
+    by_dtype(d->dtype, [&](auto t) { gated_name<decltype(t)>(gated_product(d), d->workspace ? d->workspace_bytes : 0, buf, len); });
     return TCBNN_OK;
 }
 
@@ -346,12 +390,15 @@ extern "C" int tcbnn_gated_forward(const tcbnn_gated_desc* d, void* stream) {
     TCBNN_NOTNULL(d->input);
     TCBNN_NOTNULL(d->weight);
     TCBNN_NOTNULL(d->output);
-    return by_dtype(d->dtype, [&](auto t) { return launch_gated<decltype(t)>(p, (hipStream_t)stream); });
+    TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "gated: the workspace is not aligned to 16 bytes");
+    return by_dtype(d->dtype, [&](auto t) {
+        return launch_gated<decltype(t)>(p, d->dtype, d->workspace, d->workspace ? d->workspace_bytes : 0, (hipStream_t)stream);
+    });
 }
 
-extern "C" size_t tcbnn_gated_grad_workspace_bytes(int rows, int in_features, int features, int dtype) {
+extern "C" size_t tcbnn_gated_grad_workspace_bytes(int rows, int in_features, int features, int dtype, int anywhere) {
     if (rows <= 0 || rows > kMaxRows || in_features <= 0 || in_features > kMaxIn || features <= 0 || features > tcbnn::kMaxFeatures || !dtype_known(dtype)) return 0;
-    return dz_bytes(rows, features, dtype) + sum_bytes(rows, features, dtype) + gradient_product_bytes(rows, in_features, 2 * features, dtype);
+    return grad_workspace(rows, in_features, features, dtype, anywhere != 0).total;
 }
 
 extern "C" int tcbnn_gated_backward(const tcbnn_gated_grad_desc* d, void* stream) {
@@ -368,38 +415,53 @@ extern "C" int tcbnn_gated_backward(const tcbnn_gated_grad_desc* d, void* stream
         if (d->grad_input) TCBNN_NOTNULL(d->weight);
         TCBNN_NOTNULL(d->workspace);
         TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "gated: the workspace is not aligned to 16 bytes");
-        TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_gated_grad_workspace_bytes(d->rows, d->in_features, d->features, d->dtype), "gated: workspace too small");
+        TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_gated_grad_workspace_bytes(d->rows, d->in_features, d->features, d->dtype, 0), "gated: workspace too small");
     }
     if (!d->grad_input && !d->grad_weight && !d->grad_bias) return TCBNN_OK;
     const int vectors = out_vectors(d->features, d->dtype), lanes = dz_lanes(vectors), parts = d->rows > 0 ? gated_dz_parts(d->rows, vectors) : 0;
-    float* sums = d->grad_bias ? (float*)((char*)d->workspace + dz_bytes(d->rows, d->features, d->dtype)) : nullptr;
-    if (d->grad_bias && parts == 1) sums = d->grad_bias;
+    const int n = 2 * d->features, size = (int)dtype_bytes(d->dtype);
+    const bool copies = d->workspace_bytes >= tcbnn_gated_grad_workspace_bytes(d->rows, d->in_features, d->features, d->dtype, 1);
+    const GatedGradWorkspace w = d->rows > 0 ? grad_workspace(d->rows, d->in_features, d->features, d->dtype, copies) : GatedGradWorkspace{};
+    const long long dz_ld = packed_ld(n, size);
+    char* base = (char*)d->workspace;
+    float* sums = d->grad_bias ? (parts == 1 ? d->grad_bias : (float*)(base + w.sums)) : nullptr;
     if (d->rows > 0)
         by_dtype(d->dtype, [&](auto t) {
             using T = decltype(t);
             by_activation(d->activation, [&](auto act) {
                 hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_dz_kernel<T, act.value>), dim3((unsigned)((vectors + lanes - 1) / lanes), (unsigned)parts), dim3(kDzThreads),
                                    0, (hipStream_t)stream, (const T*)d->grad_output, (const T*)d->preact, (T*)d->workspace, sums, d->rows, d->features, lanes,
-                                   gated_dz_rows(d->rows, vectors), dh_ld, z_ld);
+                                   gated_dz_rows(d->rows, vectors), dh_ld, z_ld, dz_ld);
             });
         });
-    if (d->grad_bias && sums != d->grad_bias) launch_column_join(sums, d->grad_bias, parts, 2 * d->features, (hipStream_t)stream);
+    if (d->grad_bias && sums != d->grad_bias) launch_column_join(sums, d->grad_bias, parts, n, (hipStream_t)stream);
     TCBNN_LAUNCH_CHECK("gated_dz_kernel");
-    const size_t before = dz_bytes(d->rows, d->features, d->dtype) + sum_bytes(d->rows, d->features, d->dtype);
     ProductParams dx = {}, dw = {};
-    dx.i = dw.i = {d->workspace, 2LL * d->features};
+    dx.i = dw.i = {d->workspace, dz_ld};
+    dx.padded_i = dw.padded_i = n * size >= 16;
     dx.j = {d->weight, w_ld};
+    dw.j = {d->input, x_ld};
+    by_dtype(d->dtype, [&](auto t) {
+        using T = decltype(t);
+        if (d->grad_input && w.pack_weight && lies_anywhere<T>(dx.j, d->in_features)) {
+            dx.j = launch_pack(d->dtype, dx.j, n, d->in_features, base + w.weight, (hipStream_t)stream);
+            dx.padded_j = true;
+        }
+        if (d->grad_weight && w.pack_input && lies_anywhere<T>(dw.j, d->in_features)) {
+            dw.j = launch_pack(d->dtype, dw.j, d->rows, d->in_features, base + w.input, (hipStream_t)stream);
+            dw.padded_j = true;
+        }
+    });
     dx.rows = d->rows;
     dx.cols = d->in_features;
-    dx.sum = 2 * d->features;
+    dx.sum = n;
     dx.out = d->grad_input;
     dx.out_ld = dx_ld;
-    dw.j = {d->input, x_ld};
-    dw.rows = 2 * d->features;
+    dw.rows = n;
     dw.cols = d->in_features;
     dw.sum = d->rows;
     dw.out = d->grad_weight;
     dw.out_ld = dw_ld;
-    return launch_gradient_products(d->dtype, dx, dw, d->rows > 0 ? (float*)((char*)d->workspace + before) : nullptr,
-                                    d->rows > 0 ? d->workspace_bytes - before : 0, (hipStream_t)stream, true);
+    return launch_gradient_products(d->dtype, dx, dw, d->rows > 0 ? (float*)(base + w.split) : nullptr, d->rows > 0 ? d->workspace_bytes - w.split : 0,
+                                    (hipStream_t)stream, true);
 }

@@ -506,6 +506,26 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
     return TCBNN_OK;
 }
 
+constexpr int kPackThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kPackThreads) void pack_rows_kernel(const T* __restrict__ x, T* __restrict__ to, long long rows, int n, long long x_ld, long long to_ld) {
+    constexpr int V = Elem<T>::kVec;
+    const int vectors = (n + V - 1) / V;
+    for (long long at = (long long)blockIdx.x * kPackThreads + threadIdx.x; at < rows * vectors; at += (long long)gridDim.x * kPackThreads) {
+        const long long row = at / vectors;
+        const int i = (int)(at - row * vectors) * V;
+        const T* from = x + row * x_ld + i;
+        Vec<T> v;
+        if (i + V <= n) {
+            v = load_vec(from);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = i + e < n ? from[e] : (T)0.0f;
+        }
+        *reinterpret_cast<Vec<T>*>(to + row * to_ld + i) = v;
+    }
+}
+
 // the partial sums of a split product
 size_t split_bytes(int rows, int cols, int sum, int dtype, bool forward) {
     const int size = (int)dtype_bytes(dtype);
@@ -549,6 +569,17 @@ int launch_carried_sum(int dtype, const ProductParams& dx, hipStream_t stream) {
     by_dtype(dtype, [&](auto t) { launch_join<decltype(t)>(dx, stream); });
     TCBNN_LAUNCH_CHECK("product_join_kernel");
     return TCBNN_OK;
+}
+
+Operand launch_pack(int dtype, const Operand& o, long long rows, int n, void* to, hipStream_t stream) {
+    const long long ld = packed_ld(n, (int)dtype_bytes(dtype));
+    by_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const long long vectors = rows * (ld / Elem<T>::kVec);
+        hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((unsigned)std::min((vectors + kPackThreads - 1) / kPackThreads, 8LL * kComputeUnits)), dim3(kPackThreads), 0,
+                           stream, (const T*)o.p, (T*)to, rows, n, o.ld, ld);
+    });
+    return {to, ld};
 }
 
 void launch_column_join(const float* sums, float* out, int parts, int n, hipStream_t stream) {

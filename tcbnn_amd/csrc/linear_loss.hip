@@ -18,6 +18,7 @@ struct LossParams {
     float2* parts;          // [parts][rows_there] largest logit, sum of exponentials about it
     float* given;           // [rows] z_t
     long long rows_there;
+    int first;              // the first class of the call
 };
 struct LossGradParams {
     const int32_t* targets;
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void loss_product_kernel(const P
             s = across_halves(s, add) * __builtin_amdgcn_exp2f(-__builtin_fmaf(base, kLog2e, -c));
             if (spot.lane < 32) rows[spot.wj / (32 * NJ) * BI + row] = make_float2(m, s);
             const long long i = spot.i0 + row;
-            const long long t = l.targets && i < p.rows ? l.targets[i] - j0 : -1;
+            const long long t = l.targets && i < p.rows ? (long long)l.targets[i] - l.first - j0 : -1;
             if (__any(t >= 0 && t < 32 * NJ && t + j0 < p.cols)) {
                 const int at = (int)(t - 4 * (spot.lane >> 5));
 #pragma unroll
@@ -191,19 +192,6 @@ __global__ __launch_bounds__(kLossJoinThreads) void loss_join_kernel(const LossP
             }
         }
         __syncthreads();
-    }
-}
-
-// ---- rows of the input in the workspace, at whole 16 bytes
-constexpr int kPackThreads = 256;
-template <typename T>
-__global__ __launch_bounds__(kPackThreads) void loss_pack_kernel(const T* __restrict__ x, T* __restrict__ to, int rows, int n, long long x_ld, long long to_ld) {
-    constexpr int V = Elem<T>::kVec;  // (n is a multiple of it)
-    const int vectors = n / V;
-    for (long long at = (long long)blockIdx.x * kPackThreads + threadIdx.x; at < (long long)rows * vectors; at += (long long)gridDim.x * kPackThreads) {
-        const long long row = at / vectors;
-        const int i = (int)(at - row * vectors) * V;
-        *reinterpret_cast<Vec<T>*>(to + row * to_ld + i) = load_vec(x + row * x_ld + i);
     }
 }
 
@@ -364,18 +352,32 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void loss_grad_product_kernel(co
 inline int cut_size(Access access, Cut cut) { return access == ELEMENTS ? 32 : (access == WHOLE_PIECES ? kCuts16 : kCutsAnywhere)[cut].size; }
 // The forward call's kernel: its tile, or the one for few rows; the number of parts that it leaves of a row.
 struct LossPlan {
+    Access access;
     Plan plan;
     bool few;
     int parts;
+    bool pack_x, pack_w;
 };
 inline LossPlan plan_loss(int rows, int classes, int sum, int size, Access access) {
     const bool vectors = access == WHOLE_PIECES;
-    LossPlan l;
+    LossPlan l = {};
+    l.access = access;
     l.plan = plan_product(rows, classes, sum, size, vectors, 0);
     l.few = rows <= kFewRows && (access == ELEMENTS || few_time(rows, classes, sum, size, vectors) < l.plan.time);
     const int width = l.few ? kFewOutputs : cut_size(access, l.plan.cut);
     l.parts = (classes - 1) / width + 1;
     return l;
+}
+// ... with operands that lie anywhere copied where that and the product of the copies are estimated to take less time
+inline LossPlan plan_loss(int rows, int classes, int sum, int size, Access access, bool x_anywhere, bool w_anywhere, bool copies_fit) {
+    const LossPlan l = plan_loss(rows, classes, sum, size, access);
+    if (l.few || access != ANYWHERE || !copies_fit) return l;
+    LossPlan whole = plan_loss(rows, classes, sum, size, WHOLE_PIECES);
+    const float copies = (x_anywhere ? pack_time(packed_bytes(rows, sum, size)) : 0.0f) + (w_anywhere ? pack_time(packed_bytes(classes, sum, size)) : 0.0f);
+    if (whole.few || whole.plan.time + copies >= l.plan.time) return l;
+    whole.pack_x = x_anywhere;
+    whole.pack_w = w_anywhere;
+    return whole;
 }
 
 // A piece of the classes whose d is in the workspace at a time: as many as kPieceBytes hold, pieces of about the same size.
@@ -387,8 +389,11 @@ inline int piece_classes(int rows, int classes, int size) {
     const long long pieces = (classes + most - 1) / most;
     return (int)(((classes + pieces - 1) / pieces + kPieceUnit - 1) / kPieceUnit * kPieceUnit);
 }
-// elements between rows of d
-inline long long piece_ld(int piece, int size) { return ((long long)piece * size + 15) / 16 * 16 / size; }
+// classes whose weights are copied at a time
+inline int packed_classes(int classes, int in_features, int size) {
+    const long long most = std::max<long long>(kPieceUnit, (long long)(kPieceBytes / (packed_ld(in_features, size) * size)) / kPieceUnit * kPieceUnit);
+    return (int)std::min<long long>(classes, most);
+}
 // The splits of dx's sum over a whole piece, where there are several.  Where the weights lie is not known when a workspace is asked for: the splits are
 // those of rows at whole 16 bytes, which are no fewer.
 inline int carried_splits(int rows, int in_features, int piece, int size) {
@@ -406,19 +411,50 @@ inline bool two_planes(int rows, int dtype) { return dtype != TCBNN_F32 && rows 
 // where the second plane of a sum of n begins: whole steps
 inline int plane_of(int n, int size) { return (n + kStepBytes / size - 1) / (kStepBytes / size) * (kStepBytes / size); }
 
+// Which of a step's operands to copy (linear_loss_backward's three products a piece), where they lie anywhere.
+struct LossPacking {
+    bool x, w;
+};
+inline LossPacking loss_packing(int rows, int in_features, int piece, int classes, int size, bool planes, bool x_anywhere, bool w_anywhere) {
+    if (in_features * size < 16) return {false, false};
+    const int pieces = (classes - 1) / piece + 1;
+    auto time = [&](int i, int j, int sum, bool whole) { return plan_product(i, j, sum, size, whole, 0).time; };
+    LossPacking best = {false, false};
+    float best_time = 0.0f;
+    for (bool x : {false, true})
+        for (bool w : {false, true}) {
+            if ((x && !x_anywhere) || (w && !w_anywhere)) continue;
+            const bool x_whole = x || !x_anywhere, w_whole = w || !w_anywhere;
+            const float each = time(rows, piece, in_features, x_whole && w_whole) + time(rows, in_features, planes ? plane_of(piece, size) + piece : piece, w_whole) +
+                               time(piece, in_features, planes ? plane_of(rows, size) + rows : rows, x_whole) +
+                               (w ? pack_time(packed_bytes(piece, in_features, size)) : 0.0f);
+            const float total = (float)pieces * each + (x ? pack_time(packed_bytes(rows, in_features, size)) : 0.0f);
+            if (best_time == 0.0f || total < best_time) best = {x, w}, best_time = total;
+        }
+    return best;
+}
+
 struct LossWorkspace {
-    size_t scale, x, d, sums, dx, split, total;  // offsets, in order
+    size_t scale, x, w, d, sums, dx, split, total;  // offsets, in order
     int piece, splits;
 };
-inline LossWorkspace loss_workspace(int rows, int in_features, int classes, int dtype) {
+inline LossWorkspace loss_workspace(int rows, int in_features, int classes, int dtype, bool anywhere) {
     const int size = (int)dtype_bytes(dtype), planes = two_planes(rows, dtype) ? 2 : 1;
     LossWorkspace w = {};
     w.piece = piece_classes(rows * planes, classes, size);
     const bool carried = w.piece < classes;
     w.splits = carried ? carried_splits(rows, in_features, (planes - 1) * plane_of(w.piece, size) + w.piece, size) : 1;
+    bool pack_x = false, pack_w = false;
+    for (bool x : {false, anywhere})  // (which of the operands is not known here)
+        for (bool v : {false, anywhere}) {
+            const LossPacking packing = loss_packing(rows, in_features, w.piece, classes, size, planes > 1, x, v);
+            pack_x |= packing.x;
+            pack_w |= packing.w;
+        }
     w.x = 256;
-    w.d = w.x + whole_lines((size_t)rows * piece_ld(in_features, size) * size);
-    w.sums = w.d + whole_lines((size_t)rows * planes * piece_ld(w.piece, size) * size);
+    w.w = w.x + (pack_x ? packed_bytes(rows, in_features, size) : 0);
+    w.d = w.w + (pack_w ? packed_bytes(w.piece, in_features, size) : 0);
+    w.sums = w.d + packed_bytes((long long)rows * planes, w.piece, size);
     w.dx = w.sums + whole_lines((size_t)((rows + 31) / 32) * w.piece * sizeof(float));
     w.split = w.dx + (carried ? whole_lines((size_t)w.splits * rows * in_features * sizeof(float)) : 0);
     w.total = w.split + gradient_product_bytes(rows * planes, in_features, w.piece * planes, dtype);
@@ -433,16 +469,6 @@ int check_loss(int rows, int in_features, int classes, int dtype) {
     TCBNN_REQUIRE(classes <= kMaxOut, "linear loss: at most %d classes", kMaxOut);
     return TCBNN_OK;
 }
-// Rows of the input that do not lie at whole 16 bytes while those of the weights do are copied first.
-template <typename T>
-bool apart(const Operand& o, int n) { return n % Elem<T>::kVec != 0 || (uintptr_t)o.p % 16 != 0 || o.ld * sizeof(T) % 16 != 0; }
-template <typename T>
-Operand pack(const Operand& x, void* to, int rows, int n, hipStream_t stream) {
-    const long long ld = piece_ld(n, (int)sizeof(T)), vectors = rows * (ld / Elem<T>::kVec);
-    hipLaunchKernelGGL(loss_pack_kernel<T>, dim3((unsigned)std::min((vectors + kPackThreads - 1) / kPackThreads, 8LL * kComputeUnits)), dim3(kPackThreads), 0, stream,
-                       (const T*)x.p, (T*)to, rows, n, x.ld, ld);
-    return {to, ld};
-}
 // rows that are so far apart that 32 bits do not hold a tile
 bool too_far(long long ld, int dtype) { return ld * 256 * (long long)dtype_bytes(dtype) > 0x7fffffffLL; }
 
@@ -452,13 +478,18 @@ bool too_far(long long ld, int dtype) { return ld * 256 * (long long)dtype_bytes
 using namespace tcbnn;
 using namespace tcbnn::head;
 
-extern "C" size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, int classes, int dtype) {
+extern "C" size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, int classes, int dtype, int anywhere) {
     if (rows <= 0 || rows > kMaxRows || in_features <= 0 || in_features > kMaxIn || classes <= 0 || classes > kMaxOut || !dtype_known(dtype)) return 0;
-    size_t parts = 0;
     const int size = (int)dtype_bytes(dtype);
-    for (Access access : {WHOLE_PIECES, ANYWHERE, ELEMENTS})  // (where the operands will lie is not known here)
-        if ((access == ELEMENTS) == (in_features * size < 16)) parts = std::max(parts, (size_t)plan_loss(rows, classes, in_features, size, access).parts);
-    return whole_lines(parts * rows * sizeof(float2)) + whole_lines((size_t)rows * sizeof(float)) + (size_t)rows * piece_ld(in_features, size) * size;
+    size_t parts = 0, copies = 0;
+    for (bool x : {false, true})  // (which of the operands is not known here; parts are there for rows that lie anywhere in any case)
+        for (bool w : {false, true}) {
+            const LossPlan l = plan_loss(rows, classes, in_features, size, in_features * size < 16 ? ELEMENTS : x || w ? ANYWHERE : WHOLE_PIECES, x, w, anywhere != 0);
+            parts = std::max(parts, (size_t)l.parts);
+            copies = std::max(copies, (l.pack_x ? packed_bytes(rows, in_features, size) : 0) +
+                                          (l.pack_w ? packed_bytes(packed_classes(classes, in_features, size), in_features, size) : 0));
+        }
+    return copies + whole_lines(parts * rows * sizeof(float2)) + whole_lines((size_t)rows * sizeof(float));
 }
 
 extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream) {
@@ -475,7 +506,8 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
     if (d->loss) TCBNN_NOTNULL(d->targets);
     TCBNN_NOTNULL(d->workspace);
     TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "linear loss: the workspace is not aligned to 16 bytes");
-    TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_linear_loss_workspace_bytes(d->rows, d->in_features, d->classes, d->dtype), "linear loss: workspace too small");
+    TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_linear_loss_workspace_bytes(d->rows, d->in_features, d->classes, d->dtype, 0), "linear loss: workspace too small");
+    const bool copies = d->workspace_bytes >= tcbnn_linear_loss_workspace_bytes(d->rows, d->in_features, d->classes, d->dtype, 1);
     p.rows = d->rows;
     p.cols = d->classes;
     p.sum = d->in_features;
@@ -483,12 +515,18 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(d->dtype, [&](auto type) -> int {
         using T = decltype(type);
-        if (p.rows > kFewRows && apart<T>(p.i, p.sum) && !apart<T>(p.j, p.sum))
-            p.i = pack<T>(p.i, (char*)d->workspace + d->workspace_bytes / 16 * 16 - (size_t)p.rows * piece_ld(p.sum, (int)sizeof(T)) * sizeof(T), p.rows, p.sum, s);
-        const Access access = access_of<T, false, false>(p);
-        const LossPlan plan = plan_loss(p.rows, p.cols, p.sum, (int)sizeof(T), access);
-        LossParams l = {d->loss ? d->targets : nullptr, (float2*)d->workspace, (float*)((char*)d->workspace + whole_lines((size_t)plan.parts * p.rows * sizeof(float2))),
-                        p.rows};
+        const LossPlan plan = plan_loss(p.rows, p.cols, p.sum, (int)sizeof(T), access_of<T, false, false>(p), lies_anywhere<T>(p.i, p.sum), lies_anywhere<T>(p.j, p.sum),
+                                        copies);
+        char* at = (char*)d->workspace;
+        if (plan.pack_x) {
+            p.i = launch_pack(d->dtype, p.i, p.rows, p.sum, at, s);
+            p.padded_i = true;
+            at += packed_bytes(p.rows, p.sum, (int)sizeof(T));
+        }
+        char* copy = at;
+        const int piece = plan.pack_w ? packed_classes(p.cols, p.sum, (int)sizeof(T)) : p.cols;
+        if (plan.pack_w) at += packed_bytes(piece, p.sum, (int)sizeof(T));
+        LossParams l = {d->loss ? d->targets : nullptr, (float2*)at, (float*)(at + whole_lines((size_t)plan.parts * p.rows * sizeof(float2))), p.rows, 0};
         if (plan.few) {
             const int shares = few_shares(p.cols, p.sum, (int)sizeof(T)), outputs = kFewOutputs * kFewWaves / shares;
             const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
@@ -497,21 +535,30 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
             else
                 hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_few_rows_kernel<T, 2>), grid, dim3(64 * kFewWaves), 0, s, p, l);
         } else {
-            by_tile(access, plan.plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
+            by_tile(plan.access, plan.plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
                 constexpr int B = size.value, kThreads = 64 * wi.value * wj.value * ws.value;
                 // rows beyond a launch's threads have one of their own
                 const long long at_once = std::max(1LL, kMaxThreads / kThreads / plan.parts) * B;
-                for (long long first = 0; first < p.rows; first += at_once) {
-                    ProductParams q = p;
-                    LossParams part = l;
-                    q.rows = (int)std::min(at_once, p.rows - first);
-                    q.i.p = (const T*)p.i.p + first * p.i.ld;
-                    part.targets = l.targets ? l.targets + first : nullptr;
-                    part.parts += first;
-                    part.given += first;
-                    cut_product(q, B, kStepBytes / (int)sizeof(T), 1, nullptr);
-                    hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_product_kernel<T, B, B, wi.value, wj.value, ws.value, stages.value, how.value, hold.value, keep.value>),
-                                       dim3((unsigned)((long long)q.tiles_i * q.tiles_j)), dim3(kThreads), 0, s, q, part);
+                for (int c = 0; c < p.cols; c += piece) {
+                    ProductParams r = p;
+                    r.cols = std::min(piece, p.cols - c);
+                    r.j.p = (const T*)p.j.p + c * p.j.ld;
+                    r.bias = p.bias ? p.bias + c : nullptr;
+                    if (plan.pack_w) r.j = launch_pack(d->dtype, r.j, r.cols, r.sum, copy, s);
+                    r.padded_j = plan.pack_w;
+                    for (long long first = 0; first < p.rows; first += at_once) {
+                        ProductParams q = r;
+                        LossParams part = l;
+                        q.rows = (int)std::min(at_once, p.rows - first);
+                        q.i.p = (const T*)p.i.p + first * p.i.ld;
+                        part.targets = l.targets ? l.targets + first : nullptr;
+                        part.parts += first + c / B * l.rows_there;  // (a piece is whole tiles)
+                        part.given += first;
+                        part.first = c;
+                        cut_product(q, B, kStepBytes / (int)sizeof(T), 1, nullptr);
+                        hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_product_kernel<T, B, B, wi.value, wj.value, ws.value, stages.value, how.value, hold.value, keep.value>),
+                                           dim3((unsigned)((long long)q.tiles_i * q.tiles_j)), dim3(kThreads), 0, s, q, part);
+                    }
                 }
             });
         }
@@ -526,9 +573,9 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
     });
 }
 
-extern "C" size_t tcbnn_linear_loss_grad_workspace_bytes(int rows, int in_features, int classes, int dtype) {
+extern "C" size_t tcbnn_linear_loss_grad_workspace_bytes(int rows, int in_features, int classes, int dtype, int anywhere) {
     if (rows <= 0 || rows > kMaxRows || in_features <= 0 || in_features > kMaxIn || classes <= 0 || classes > kMaxOut || !dtype_known(dtype)) return 0;
-    return loss_workspace(rows, in_features, classes, dtype).total;
+    return loss_workspace(rows, in_features, classes, dtype, anywhere != 0).total;
 }
 
 extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, void* stream) {
@@ -559,8 +606,9 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
     TCBNN_NOTNULL(d->grad_loss);
     TCBNN_NOTNULL(d->workspace);
     TCBNN_REQUIRE((uintptr_t)d->workspace % 16 == 0, "linear loss: the workspace is not aligned to 16 bytes");
-    const LossWorkspace w = loss_workspace(d->rows, d->in_features, d->classes, d->dtype);
-    TCBNN_REQUIRE(d->workspace_bytes >= w.total, "linear loss: workspace too small");
+    TCBNN_REQUIRE(d->workspace_bytes >= loss_workspace(d->rows, d->in_features, d->classes, d->dtype, false).total, "linear loss: workspace too small");
+    const bool copies = d->workspace_bytes >= loss_workspace(d->rows, d->in_features, d->classes, d->dtype, true).total;
+    const LossWorkspace w = loss_workspace(d->rows, d->in_features, d->classes, d->dtype, copies);
     char* base = (char*)d->workspace;
     float* scale = d->dtype == TCBNN_F16 ? (float*)base : nullptr;
     if (scale) hipLaunchKernelGGL(loss_scale_kernel, dim3(1), dim3(kScaleThreads), 0, s, d->grad_loss, d->targets, scale, d->rows);
@@ -568,15 +616,20 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
         using T = decltype(type);
         ProductParams dx = {};
         Operand x = {d->input, x_ld};
-        if (apart<T>(x, d->in_features) && !apart<T>({d->weight, w_ld}, d->in_features)) x = pack<T>(x, base + w.x, d->rows, d->in_features, s);
         const bool planes = two_planes(d->rows, d->dtype);
-        const long long d_ld = piece_ld(w.piece, (int)sizeof(T)), low = planes ? d->rows * d_ld : 0;
+        const LossPacking packing = loss_packing(d->rows, d->in_features, w.piece, d->classes, (int)sizeof(T), planes,
+                                                 copies && lies_anywhere<T>(x, d->in_features), copies && lies_anywhere<T>({d->weight, w_ld}, d->in_features));
+        if (packing.x) x = launch_pack(d->dtype, x, d->rows, d->in_features, base + w.x, s);
+        const long long d_ld = packed_ld(w.piece, (int)sizeof(T)), low = planes ? d->rows * d_ld : 0;
         for (int first = 0; first < d->classes; first += w.piece) {
             const int classes = std::min(w.piece, d->classes - first);
-            const T* weight = (const T*)d->weight + first * w_ld;
+            Operand weight = {(const T*)d->weight + first * w_ld, w_ld};
+            if (packing.w) weight = launch_pack(d->dtype, weight, classes, d->in_features, base + w.w, s);
             ProductParams p = {};
             p.i = x;
-            p.j = {weight, w_ld};
+            p.j = weight;
+            p.padded_i = packing.x;
+            p.padded_j = packing.w;
             p.rows = d->rows;
             p.cols = classes;
             p.sum = d->in_features;
@@ -611,9 +664,11 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             TCBNN_LAUNCH_CHECK("loss_grad_product_kernel");
             ProductParams dw = {};
             dx.i = dw.i = {p.out, p.out_ld};
-            dx.padded = dw.padded = classes >= Elem<T>::kVec;
+            dx.padded_i = dw.padded_i = classes >= Elem<T>::kVec;
             dx.factor = dw.factor = scale ? scale + 1 : nullptr;
-            dx.j = {weight, w_ld};
+            dx.j = weight;
+            dx.padded_j = packing.w;
+            dw.padded_j = packing.x;
             dx.i_low = dw.i_low = low;
             dx.plane = planes ? plane_of(classes, (int)sizeof(T)) : 0;
             dw.plane = planes ? plane_of(d->rows, (int)sizeof(T)) : 0;

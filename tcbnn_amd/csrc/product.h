@@ -326,7 +326,7 @@ struct ProductParams {
     // second in turn, so that J's steps are in the cache when they are read again.  `plane`: the sum in whole steps (0: one plane).
     int plane;
     long long i_low;
-    bool padded;           // I's rows, 16 bytes or more, go on with zeros to whole 16 bytes
+    bool padded_i, padded_j;  // the operand's rows, 16 bytes or more, go on with zeros to whole 16 bytes
 };
 enum Carry : int { NO_CARRY, CARRY_FIRST, CARRY_ON };
 
@@ -406,8 +406,8 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
     TileI ti;
     TileJ tj;
     constexpr int V = Elem<T>::kVec;
-    ti.init(p.i, i0, ACROSS_I && p.padded ? ((long long)p.rows + V - 1) / V * V : (long long)p.rows);
-    tj.init(p.j, j0, p.cols);
+    ti.init(p.i, i0, ACROSS_I && p.padded_i ? ((long long)p.rows + V - 1) / V * V : (long long)p.rows);
+    tj.init(p.j, j0, ACROSS_J && p.padded_j ? ((long long)p.cols + V - 1) / V * V : (long long)p.cols);
     const int s0 = split * p.split_sum, s1 = min(PLANES ? 2 * p.plane : p.sum, s0 + p.split_sum);
     const int share = wave / (WI * WJ), wi = wave / WJ % WI * (32 * NI), wj = wave % WJ * (32 * NJ);
     spot = {split, tile_i, tile_j, share, wi, wj, wave, lane, i0, j0};
@@ -760,7 +760,7 @@ Access access_of(const ProductParams& p) {
         if (row < Elem<T>::kVec || o.ld * 256 * (long long)sizeof(T) > 0x7fffffffLL) return ELEMENTS;
         return (uintptr_t)o.p % 16 == 0 && o.ld * sizeof(T) % 16 == 0 && row % Elem<T>::kVec == 0 ? WHOLE_PIECES : ANYWHERE;
     };
-    return std::max(of(p.i, p.rows, p.sum, ACROSS_I, p.padded), of(p.j, p.cols, p.sum, ACROSS_J, false));
+    return std::max(of(p.i, p.rows, p.sum, ACROSS_I, p.padded_i), of(p.j, p.cols, p.sum, ACROSS_J, p.padded_j));
 }
 // f(tile, wavefronts of i, of j, of the sum, stages, access, steps held, long sums) with the constants of a tile's kernel (product_sums)
 template <typename F>
@@ -857,6 +857,16 @@ inline int dz_parts(int rows, int vectors, bool active) {
 }
 inline int out_vectors(int out_features, int dtype) { return (out_features + (int)(16 / dtype_bytes(dtype)) - 1) / (int)(16 / dtype_bytes(dtype)); }
 inline size_t whole_lines(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// ---- copies of rows that lie anywhere.  A tile of such rows takes 1.6 times as long, so that a large product is faster on a copy at whole 16 bytes, zeros
+// behind the rows' ends: bf16 @@
+template <typename T>
+bool lies_anywhere(const Operand& o, int n) { return n % Elem<T>::kVec != 0 || (uintptr_t)o.p % 16 != 0 || o.ld * (long long)sizeof(T) % 16 != 0; }
+inline long long packed_ld(int n, int size) { return ((long long)n * size + 15) / 16 * 16 / size; }
+inline size_t packed_bytes(long long rows, int n, int size) { return whole_lines((size_t)rows * packed_ld(n, size) * size); }
+inline float pack_time(size_t bytes) { return 2.5f + (float)bytes * 2.0f / 4.0e6f; }
+// (linear.hip)  the copy
+Operand launch_pack(int dtype, const Operand& o, long long rows, int n, void* to, hipStream_t stream);
 
 // ---- (linear.hip)  dx = d w and dw = d^T x, each where it has an `out`; with dx.carry its sum stays in its `partial`, whose number of splits is
 // dx.splits.  The workspace is for split sums (gradient_product_bytes; without one none is split).

@@ -51,6 +51,12 @@ def _ld(buf):
     return getattr(buf, "ld", 0)
 
 
+def _anywhere(dtype, cols, *buffers):
+    """Whether rows of one of these matrices do not lie at whole 16 bytes."""
+    size = ITEMSIZE[dtype]
+    return int(any(b.ptr % 16 or (_ld(b) or cols) * size % 16 or cols * size % 16 for b in buffers))
+
+
 class _HeadLayer:
     def __init__(self, name, dtype):
         if dtype not in _lib.DTYPES:
@@ -271,10 +277,12 @@ class GatedLayerParam(_HeadLayer):
         if preact_gpu is None and save_preact:
             preact_gpu = self._buffer(2 * m * n * ITEMSIZE[dt])
         self.preact_gpu = self._sized(preact_gpu, "preact", (m, 2 * n), dt)
+        nbytes = lib.tcbnn_gated_workspace_bytes(m, k, n, _lib.DTYPES[dt]) if _anywhere(dt, k, self.input_gpu, self.weight_gpu) else 0
+        ws = self._buffer(nbytes) if nbytes else None
         self._desc = _lib.GatedDesc(
             self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), self.output_gpu.ptr, _ptr(self.preact_gpu), m, k, n,
             _lib.DTYPES[dt], _lib.ACTIVATIONS[self.activation], _ld(self.input_gpu), _ld(self.weight_gpu), _ld(self.output_gpu),
-            _ld(self.preact_gpu))
+            _ld(self.preact_gpu), _ptr(ws), nbytes)
         self._forward = self._call(lib.tcbnn_gated_forward, self._desc)
         return self
 
@@ -286,7 +294,7 @@ class GatedLayerParam(_HeadLayer):
         self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", (m, k), dt)
         self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", (2 * n, k), dt)
         self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", (2 * n,), "f32")
-        nbytes = lib.tcbnn_gated_grad_workspace_bytes(m, k, n, _lib.DTYPES[dt])
+        nbytes = lib.tcbnn_gated_grad_workspace_bytes(m, k, n, _lib.DTYPES[dt], _anywhere(dt, k, self.input_gpu, self.weight_gpu))
         ws = self._grad_buffer(nbytes)
         self._grad_desc = _lib.GatedGradDesc(
             self.input_gpu.ptr, self.weight_gpu.ptr, self.preact_gpu.ptr, self.grad_output_gpu.ptr, _ptr(grad_input_gpu),
@@ -469,7 +477,7 @@ class LinearLossLayerParam(_HeadLayer):
         self.loss_gpu, self.logsumexp_gpu = (
             self._sized(buf if buf is not None else self._buffer(4 * m), what, (m,), "f32")
             for buf, what in ((loss_gpu, "loss"), (logsumexp_gpu, "logsumexp")))
-        nbytes = lib.tcbnn_linear_loss_workspace_bytes(m, k, n, _lib.DTYPES[dt])
+        nbytes = lib.tcbnn_linear_loss_workspace_bytes(m, k, n, _lib.DTYPES[dt], _anywhere(dt, k, self.input_gpu, self.weight_gpu))
         ws = self._buffer(nbytes) if nbytes else None
         self._desc = _lib.LinearLossDesc(
             self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), self.targets_gpu.ptr, self.loss_gpu.ptr,
@@ -485,7 +493,7 @@ class LinearLossLayerParam(_HeadLayer):
         self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", (m, k), dt)
         self.grad_weight_gpu = self._sized(grad_weight_gpu, "grad_weight", (n, k), dt)
         self.grad_bias_gpu = self._sized(grad_bias_gpu, "grad_bias", (n,), "f32")
-        nbytes = lib.tcbnn_linear_loss_grad_workspace_bytes(m, k, n, _lib.DTYPES[dt])
+        nbytes = lib.tcbnn_linear_loss_grad_workspace_bytes(m, k, n, _lib.DTYPES[dt], _anywhere(dt, k, self.input_gpu, self.weight_gpu))
         ws = self._grad_buffer(nbytes)
         self._grad_desc = _lib.LinearLossGradDesc(
             self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), self.targets_gpu.ptr, self.logsumexp_gpu.ptr,

@@ -121,10 +121,12 @@ def test_workspaces_of_refused_sizes_are_empty():
     lib = _lib().lib
     assert lib.tcbnn_blocknorm_grad_workspace_bytes(0, 8, 0) == lib.tcbnn_blocknorm_grad_workspace_bytes(4, 65537, 0) == 0
     assert lib.tcbnn_blocknorm_grad_workspace_bytes(4, 8, 5) == 0
-    assert lib.tcbnn_gated_grad_workspace_bytes(0, 8, 8, 0) == lib.tcbnn_gated_grad_workspace_bytes(4, 8, 0, 0) == 0
+    assert lib.tcbnn_gated_workspace_bytes(0, 8, 8, 0) == lib.tcbnn_gated_workspace_bytes(4, 8, 0, 0) == lib.tcbnn_gated_workspace_bytes(4, 8, 8, 5) == 0
+    assert lib.tcbnn_gated_grad_workspace_bytes(0, 8, 8, 0, 1) == lib.tcbnn_gated_grad_workspace_bytes(4, 8, 0, 0, 0) == 0
     for f in (lib.tcbnn_linear_loss_workspace_bytes, lib.tcbnn_linear_loss_grad_workspace_bytes):
-        assert f(0, 8, 8, 0) == f(4, 0, 8, 0) == f(4, 8, -1, 0) == f(4, 8, 8, 3) == f(4, (1 << 20) + 1, 8, 0) == f(4, 8, (1 << 28) + 1, 0) == 0
-    assert lib.tcbnn_gated_grad_workspace_bytes(4, 8, (1 << 27) + 1, 0) == lib.tcbnn_gated_grad_workspace_bytes(4, 8, 8, 3) == 0
+        for a in (0, 1):
+            assert f(0, 8, 8, 0, a) == f(4, 0, 8, 0, a) == f(4, 8, -1, 0, a) == f(4, 8, 8, 3, a) == f(4, (1 << 20) + 1, 8, 0, a) == f(4, 8, (1 << 28) + 1, 0, a) == 0
+    assert lib.tcbnn_gated_grad_workspace_bytes(4, 8, (1 << 27) + 1, 0, 1) == lib.tcbnn_gated_grad_workspace_bytes(4, 8, 8, 3, 0) == 0
 
 
 def test_layers_refuse():
@@ -200,13 +202,23 @@ def test_loss_layer_refuses():
         layer.initialize(x, None, x, t)
 
 
+def test_copies_are_made_where_they_are_faster():
+    """Room for them is asked for by sizes, and only for operands that lie anywhere."""
+    lib = _lib().lib
+    assert lib.tcbnn_gated_workspace_bytes(64, 1023, 512, 1) == 0  # (a launch more takes longer than it gains)
+    assert lib.tcbnn_gated_workspace_bytes(8192, 4095, 4096, 1) >= 2 * 4096 * (8192 + 8192)
+    for f in (lib.tcbnn_gated_grad_workspace_bytes, lib.tcbnn_linear_loss_workspace_bytes, lib.tcbnn_linear_loss_grad_workspace_bytes):
+        assert f(64, 1023, 512, 1, 0) == f(64, 1023, 512, 1, 1)
+        assert f(8192, 4095, 4096, 1, 1) >= f(8192, 4095, 4096, 1, 0) + 2 * 4096 * 8192
+
+
 def test_loss_keeps_no_logits():
     """Workspaces of a large vocabulary: forward 8 bytes a row and tile, backward a piece of the classes and the sum of the inputs' gradient."""
     lib = _lib().lib
     rows, classes = 8192, 131072
     logits = 2 * rows * classes
-    assert lib.tcbnn_linear_loss_workspace_bytes(rows, 1024, classes, 1) < logits / 16
-    assert lib.tcbnn_linear_loss_grad_workspace_bytes(rows, 1024, classes, 1) < logits / 4
+    assert lib.tcbnn_linear_loss_workspace_bytes(rows, 1024, classes, 1, 0) < logits / 16
+    assert lib.tcbnn_linear_loss_grad_workspace_bytes(rows, 1024, classes, 1, 0) < logits / 4
 
 
 def test_loss_gradient_is_the_definitions():

@@ -326,6 +326,23 @@ def test_gated_grad_strides_and_single_outputs(gpu, m, k, n, dtype):
         _gated_grad(gpu, m, k, n, dtype, "silu", want=want)
 
 
+# large enough that copies of operands that lie anywhere are taken: odd inputs, rows out of wider arrays, odd features, each operand alone
+@pytest.mark.parametrize("m,k,n,gap,shift", [(4096, 1023, 1024, 0, 0), (4096, 1024, 1024, 3, 0), (4096, 1024, 1024, 8, 1), (4000, 1025, 1001, 0, 1),
+                                             (4096, 2047, 1500, 0, 0), (4096, 2047, 2048, 0, 0)])
+def test_gated_on_copies(gpu, m, k, n, gap, shift):
+    from tcbnn_amd import _lib
+    lib = _lib.lib
+    for dtype in ("bf16", "f16"):
+        dt = _lib.DTYPES[dtype]
+        assert lib.tcbnn_gated_grad_workspace_bytes(m, k, n, dt, 1) > lib.tcbnn_gated_grad_workspace_bytes(m, k, n, dt, 0)
+        assert n < 1500 or lib.tcbnn_gated_workspace_bytes(m, k, n, dt) > 0
+        assert n < 2048 or lib.tcbnn_gated_workspace_bytes(m, k, n, dt) >= 2 * (k + 1) * (m + 2 * n)  # (both operands')
+        _gated(gpu, m, k, n, dtype, "silu", gap=gap, shift=shift)
+        _gated_grad(gpu, m, k, n, dtype, "gelu", gap=gap, shift=shift)
+    if not gap:
+        _gated_grad(gpu, m, k, n, "f32", "silu", shift=shift)
+
+
 def test_gated_without_rows(gpu):
     from tcbnn_amd import head
     x, dw, db = ho.Matrix(None, "bf16", 0, 32, 8), ho.Matrix(None, "bf16", 0, 32, 8), ho.empty(32)
@@ -411,7 +428,7 @@ def test_loss_in_pieces(gpu, dtype, monkeypatch):
     """Classes whose gradients the workspace does not hold at a time, the last piece a short one."""
     from tcbnn_amd import _lib
     m, k, n = 40000, 24, 1700 if dtype == "f32" else 3400
-    assert _lib.lib.tcbnn_linear_loss_grad_workspace_bytes(m, k, n, _lib.DTYPES[dtype]) < 1.4 * 2 ** 28
+    assert _lib.lib.tcbnn_linear_loss_grad_workspace_bytes(m, k, n, _lib.DTYPES[dtype], 0) < 1.4 * 2 ** 28
     from tcbnn_amd import head
     r = rng(n)
     x, w = ho.Matrix(r.standard_normal((m, k)), dtype, shift=0), ho.Matrix(r.standard_normal((n, k)) / 4, dtype, shift=0)
@@ -436,6 +453,39 @@ def test_loss_in_pieces(gpu, dtype, monkeypatch):
     ho.check(dwv, dw_exact, bo.out_error(dw_exact, dw_err, dtype), "grad of weight")
     ho.check(dbv, db_exact, 1.1 * db_err, "grad of bias")
     layer.release()
+
+
+@pytest.mark.parametrize("m,k,n,gap,shift", [(2048, 1023, 4100, 0, 0), (2048, 1024, 4100, 3, 0), (2047, 1024, 4099, 8, 1), (250, 2047, 8001, 0, 1)])
+def test_loss_on_copies(gpu, m, k, n, gap, shift):
+    from tcbnn_amd import _lib
+    lib = _lib.lib
+    for dtype in ("bf16", "f16"):
+        assert lib.tcbnn_linear_loss_grad_workspace_bytes(m, k, n, _lib.DTYPES[dtype], 1) > lib.tcbnn_linear_loss_grad_workspace_bytes(m, k, n, _lib.DTYPES[dtype], 0)
+        _loss(gpu, m, k, n, dtype, gap=gap, shift=shift)
+
+
+def test_loss_on_copies_of_pieces(gpu):
+    """Weights whose copy is made a piece at a time, forward and backward: against the same values at whole 16 bytes."""
+    from tcbnn_amd import head
+    m, k, n, dtype = 600, 2047, 70001, "bf16"
+    r = rng(k, n)
+    xv = r.standard_normal((m, k)).astype(np.float32)
+    wv = (r.standard_normal((n, k)) / 20).astype(np.float32)
+    t, g = ho.vector(r.integers(-1, n, m), np.int32), ho.vector(np.ones(m))
+    out = []
+    for pad in (0, 1):  # (a column of zeros more is at whole 16 bytes)
+        x, w = (ho.Matrix(np.pad(v, ((0, 0), (0, pad))), dtype, shift=0) for v in (xv, wv))
+        dx, dw = ho.Matrix(None, dtype, 0, m, k + pad, shift=0), ho.Matrix(None, dtype, 0, n, k + pad, shift=0)
+        layer = head.LinearLossLayerParam("loss", m, k + pad, n, dtype).initialize(w.view, None, x.view, t)
+        layer.initialize_backward(g, dx.view, dw.view)
+        layer.forward()
+        layer.backward()
+        ho.sync()
+        got = layer.download_output()
+        out.append((got["loss"], got["logsumexp"], dx.get()[:, :k], dw.get()[:, :k]))
+        layer.release()
+    for a, b in zip(*out):
+        np.testing.assert_array_equal(a, b)
 
 
 def test_loss_of_forbidden_classes(gpu):
