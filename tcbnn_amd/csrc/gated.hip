@@ -224,6 +224,33 @@ __global__ __launch_bounds__(kDzThreads) void gated_dz_kernel(const T* __restric
     }
 }
 
+// few rows: [dg du] in fp32 as launch_few_gradients takes it, and its sums; a lane has a column
+template <typename T, int ACT>
+__global__ __launch_bounds__(kDzThreads) void gated_dz_few_rows_kernel(const T* __restrict__ dh, const T* __restrict__ z, float* __restrict__ dz,
+                                                                       float* __restrict__ db, int rows, int n, long long dh_ld, long long z_ld) {
+    const int j = blockIdx.x * kDzThreads + threadIdx.x;
+    if (j >= n) return;
+    float d[2][kFewGradientRows];
+#pragma unroll
+    for (int i = 0; i < kFewGradientRows; ++i) {
+        const long long r = min(i, rows - 1);
+        const float out = (float)dh[r * dh_ld + j], gate = (float)z[r * z_ld + j], up = (float)z[r * z_ld + n + j];
+        d[0][i] = i < rows ? out * up * slope<T, ACT>(gate) : 0.0f;
+        d[1][i] = i < rows ? out * activate<T, ACT>(gate) : 0.0f;
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        float* to = dz + ((long long)half * n + j) * kFewGradientRows;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kFewGradientRows; i += 4) {
+            *reinterpret_cast<float4*>(to + i) = make_float4(d[half][i], d[half][i + 1], d[half][i + 2], d[half][i + 3]);
+            s += d[half][i] + d[half][i + 1] + d[half][i + 2] + d[half][i + 3];
+        }
+        if (db) db[half * n + j] = s;
+    }
+}
+
 // The tile is the one that the linear layer's estimates would take for a product of 2 n columns; sums are not split.  Operands that lie anywhere are
 // copied where the product of the copies and the copying are estimated to take less time, and the workspace holds them.
 struct GatedPlan {
@@ -346,6 +373,12 @@ GatedGradWorkspace grad_workspace(int rows, int in_features, int features, int d
     GatedGradWorkspace w = {};
     w.pack_weight = worth(rows, n, weight);
     w.pack_input = worth(n, rows, input);
+    if (rows <= kFewGradientRows) {
+        w.split = whole_lines((size_t)n * kFewGradientRows * sizeof(float));
+        w.total = w.split + few_gradients_bytes(rows, in_features, n, dtype);
+        w.pack_weight = w.pack_input = false;
+        return w;
+    }
     w.sums = packed_bytes(rows, n, size);
     w.weight = w.sums + whole_lines(sizeof(float) * gated_dz_parts(rows, out_vectors(features, dtype)) * n);
     w.input = w.weight + (w.pack_weight ? weight : 0);
@@ -418,6 +451,20 @@ extern "C" int tcbnn_gated_backward(const tcbnn_gated_grad_desc* d, void* stream
         TCBNN_REQUIRE(d->workspace_bytes >= tcbnn_gated_grad_workspace_bytes(d->rows, d->in_features, d->features, d->dtype, 0), "gated: workspace too small");
     }
     if (!d->grad_input && !d->grad_weight && !d->grad_bias) return TCBNN_OK;
+    if (d->rows > 0 && d->rows <= kFewGradientRows) {
+        const int n = 2 * d->features;
+        float* dz = (float*)d->workspace;
+        by_dtype(d->dtype, [&](auto t) {
+            using T = decltype(t);
+            by_activation(d->activation, [&](auto act) {
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_dz_few_rows_kernel<T, act.value>), dim3((unsigned)((d->features - 1) / kDzThreads + 1)), dim3(kDzThreads), 0,
+                                   (hipStream_t)stream, (const T*)d->grad_output, (const T*)d->preact, dz, d->grad_bias, d->rows, d->features, dh_ld, z_ld);
+            });
+        });
+        TCBNN_LAUNCH_CHECK("gated_dz_few_rows_kernel");
+        return launch_few_gradients(d->dtype, dz, d->rows, d->in_features, n, {d->weight, w_ld}, {d->input, x_ld}, d->grad_input, dx_ld, d->grad_weight, dw_ld,
+                                    (float*)((char*)d->workspace + whole_lines((size_t)n * kFewGradientRows * sizeof(float))), (hipStream_t)stream);
+    }
     const int vectors = out_vectors(d->features, d->dtype), lanes = dz_lanes(vectors), parts = d->rows > 0 ? gated_dz_parts(d->rows, vectors) : 0;
     const int n = 2 * d->features, size = (int)dtype_bytes(d->dtype);
     const bool copies = d->workspace_bytes >= tcbnn_gated_grad_workspace_bytes(d->rows, d->in_features, d->features, d->dtype, 1);

@@ -347,6 +347,64 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void loss_grad_product_kernel(co
 #endif
 }
 
+// few rows: a wavefront has 16 classes.  p.out: d in T as above, or (FLOAT) in fp32 as launch_few_gradients takes it
+template <typename T, int SHARES, bool FLOAT>
+__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 4))) void loss_grad_few_rows_kernel(const ProductParams p, const LossGradParams l) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = wave % SHARES;
+    const long long j0 = ((long long)blockIdx.x * (kFewWaves / SHARES) + wave / SHARES) * kFewOutputs;
+    // rows past the last one are read as the last one; nothing of them is kept
+    const T* w = (const T*)p.j.p + min(j0 + (lane & 15), (long long)p.cols - 1) * p.j.ld;
+    const T* x = (const T*)p.i.p + (long long)min(lane & 15, p.rows - 1) * p.i.ld;
+    const Acc4 acc = few_rows_sums<T, SHARES>(p, w, x);
+    if (share != 0 || j0 >= p.cols) return;
+    const int i = lane & 15, row = min(i, p.rows - 1), t = l.targets[row];
+    const long long j = j0 + 4 * (lane >> 4);
+    const float lse = l.lse[row], c = lse * kLog2e, g = t < l.classes ? l.dloss[row] : NAN;
+    const bool none = i >= p.rows || t < 0 || lse == -INFINITY;
+    float d[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const bool there = j + e < p.cols;
+        d[e] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[e] + (p.bias && there ? p.bias[j + e] : 0.0f), kLog2e, -c));
+        d[e] = none || !there ? 0.0f : l.first + j + e == t ? d[e] - g : d[e];
+        if (l.sums) {
+            float s = d[e];
+            s += __uint_as_float(dpp<kSwapPairs>(__float_as_uint(s)));
+            s += __uint_as_float(dpp<kSwapTwos>(__float_as_uint(s)));
+            s += __uint_as_float(dpp<kMirrorHalf>(__float_as_uint(s)));
+            s += __uint_as_float(dpp<kMirrorRow>(__float_as_uint(s)));
+            if (i == 0 && there) l.sums[j + e] = s;
+        }
+    }
+    if constexpr (FLOAT) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i < kFewGradientRows && j + e < p.cols) ((float*)p.out)[(j + e) * kFewGradientRows + i] = d[e];
+    } else {
+        if (i >= p.rows || j >= p.out_ld) return;  // (rows end at whole 16 bytes: where they go on, four columns do)
+        const float f = l.scale ? l.scale[0] : 1.0f;
+        Columns<T, 4> v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(d[e] * f);
+        T* to = (T*)p.out + i * p.out_ld + j;
+        *reinterpret_cast<Columns<T, 4>*>(to) = v;
+        if (l.low) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(d[e] * f - (float)v[e]);
+            *reinterpret_cast<Columns<T, 4>*>(to + l.low) = v;
+        }
+    }
+}
+template <typename T, bool FLOAT>
+void launch_grad_few_rows(const ProductParams& p, const LossGradParams& l, hipStream_t stream) {
+    const int shares = few_shares(p.cols, p.sum, (int)sizeof(T)), outputs = kFewOutputs * kFewWaves / shares;
+    const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
+    if (shares == 8)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_grad_few_rows_kernel<T, 8, FLOAT>), grid, dim3(64 * kFewWaves), 0, stream, p, l);
+    else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_grad_few_rows_kernel<T, 2, FLOAT>), grid, dim3(64 * kFewWaves), 0, stream, p, l);
+}
+
 // ---- plans
 // rows and columns of a tile (by_tile)
 inline int cut_size(Access access, Cut cut) { return access == ELEMENTS ? 32 : (access == WHOLE_PIECES ? kCuts16 : kCutsAnywhere)[cut].size; }
@@ -441,6 +499,12 @@ struct LossWorkspace {
 inline LossWorkspace loss_workspace(int rows, int in_features, int classes, int dtype, bool anywhere) {
     const int size = (int)dtype_bytes(dtype), planes = two_planes(rows, dtype) ? 2 : 1;
     LossWorkspace w = {};
+    if (rows <= kFewGradientRows) {
+        w.piece = classes;
+        w.split = whole_lines((size_t)classes * kFewGradientRows * sizeof(float));
+        w.total = w.split + few_gradients_bytes(rows, in_features, classes, dtype);
+        return w;
+    }
     w.piece = piece_classes(rows * planes, classes, size);
     const bool carried = w.piece < classes;
     w.splits = carried ? carried_splits(rows, in_features, (planes - 1) * plane_of(w.piece, size) + w.piece, size) : 1;
@@ -610,6 +674,23 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
     const bool copies = d->workspace_bytes >= loss_workspace(d->rows, d->in_features, d->classes, d->dtype, true).total;
     const LossWorkspace w = loss_workspace(d->rows, d->in_features, d->classes, d->dtype, copies);
     char* base = (char*)d->workspace;
+    if (d->rows <= kFewGradientRows) {
+        by_dtype(d->dtype, [&](auto type) {
+            using T = decltype(type);
+            ProductParams p = {};
+            p.i = {d->input, x_ld};
+            p.j = {d->weight, w_ld};
+            p.rows = d->rows;
+            p.cols = d->classes;
+            p.sum = d->in_features;
+            p.bias = d->bias;
+            p.out = base;
+            launch_grad_few_rows<T, true>(p, {d->targets, d->logsumexp, d->grad_loss, nullptr, d->grad_bias, 0, d->classes, 0}, s);
+        });
+        TCBNN_LAUNCH_CHECK("loss_grad_few_rows_kernel");
+        return launch_few_gradients(d->dtype, (float*)base, d->rows, d->in_features, d->classes, {d->weight, w_ld}, {d->input, x_ld}, d->grad_input, dx_ld,
+                                    d->grad_weight, dw_ld, (float*)(base + w.split), s);
+    }
     float* scale = d->dtype == TCBNN_F16 ? (float*)base : nullptr;
     if (scale) hipLaunchKernelGGL(loss_scale_kernel, dim3(1), dim3(kScaleThreads), 0, s, d->grad_loss, d->targets, scale, d->rows);
     return by_dtype(d->dtype, [&](auto type) -> int {
@@ -639,9 +720,11 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes, low};
             const Access access = access_of<T, false, false>(p);
             const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0);
-            const int tiles_i = (p.rows - 1) / cut_size(access, plan.cut) + 1;
+            const bool few = p.rows <= kFewRows && (access == ELEMENTS || few_time(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES) < plan.time);
+            const int tiles_i = few ? 1 : (p.rows - 1) / cut_size(access, plan.cut) + 1;
             if (l.sums && tiles_i == 1) l.sums = d->grad_bias + first;
-            by_tile(access, plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
+            if (few) launch_grad_few_rows<T, false>(p, l, s);
+            if (!few) by_tile(access, plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
                 constexpr int B = size.value, kThreads = 64 * wi.value * wj.value * ws.value;
                 // rows beyond a launch's threads have one of their own
                 const long long tiles_j = (p.cols - 1) / B + 1, at_once = std::max(1LL, kMaxThreads / kThreads / tiles_j) * B;

@@ -874,7 +874,13 @@ size_t gradient_product_bytes(int rows, int in_features, int out_features, int d
 // `together`: both in one launch of large tiles too, where that is estimated to take less time.
 int launch_gradient_products(int dtype, const ProductParams& dx, const ProductParams& dw, float* workspace, size_t workspace_bytes, hipStream_t stream,
                              bool together = false);
-// a carried sum -> dx.out
+// ---- (few_gradients.hip)  the same for kFewGradientRows rows at most and d in fp32, [outs][kFewGradientRows] with zeros behind the last row; `partial` holds few_gradients_bytes
+constexpr int kFewGradientRows = 4;
+size_t few_gradients_bytes(int rows, int in_features, int outs, int dtype);
+int launch_few_gradients(int dtype, const float* d, int rows, int in_features, int outs, const Operand& weight, const Operand& input, void* dx, long long dx_ld,
+                         void* dw, long long dw_ld, float* partial, hipStream_t stream);
+
+// ---- (linear.hip)  a carried sum -> dx.out
 int launch_carried_sum(int dtype, const ProductParams& dx, hipStream_t stream);
 // out[n] = the sums of `parts` rows of n, in one order
 void launch_column_join(const float* sums, float* out, int parts, int n, hipStream_t stream);
