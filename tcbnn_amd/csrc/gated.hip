@@ -383,7 +383,7 @@ GatedGradWorkspace grad_workspace(int rows, int in_features, int features, int d
     w.weight = w.sums + whole_lines(sizeof(float) * gated_dz_parts(rows, out_vectors(features, dtype)) * n);
     w.input = w.weight + (w.pack_weight ? weight : 0);
     w.split = w.input + (w.pack_input ? input : 0);
-    w.total = w.split + gradient_product_bytes(rows, in_features, n, dtype);
+    w.total = w.split + gradient_product_bytes(rows, in_features, n, dtype, true);
     return w;
 }
 

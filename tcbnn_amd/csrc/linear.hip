@@ -143,9 +143,12 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
     if (i >= p.rows) return;
     const int j = (int)(v - i * per_row) * C, n = min(C, p.cols - j);
     Columns<float, C> part[kMaxSplits];
+    auto get = [&](int first) {
 #pragma unroll
-    for (int k = 0; k < kMaxSplits; ++k)
-        if (k < p.splits) part[k] = get_columns<float, C>(p.partial + k * p.partial_stride, p.cols, i, j, n);
+        for (int k = 0; k < kMaxSplits; ++k)
+            if (first + k < p.splits) part[k] = get_columns<float, C>(p.partial + (first + k) * p.partial_stride, p.cols, i, j, n);
+    };
+    get(0);
     float z[C], bias[C];
 #pragma unroll
     for (int e = 0; e < C; ++e) {
@@ -154,12 +157,16 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
     }
     Columns<T, C> residual = {};
     if (p.residual) residual = get_columns<T, C>(p.residual, p.residual_ld, i, j, n);
+    for (int first = 0;; get(first)) {
 #pragma unroll
-    for (int k = 0; k < kMaxSplits; ++k)
-        if (k < p.splits) {
+        for (int k = 0; k < kMaxSplits; ++k)
+            if (first + k < p.splits) {
 #pragma unroll
-            for (int e = 0; e < C; ++e) z[e] += part[k][e];
-        }
+                for (int e = 0; e < C; ++e) z[e] += part[k][e];
+            }
+        first += kMaxSplits;
+        if (first >= p.splits) break;
+    }
     finish<T, C>(p, i, j, n, bias, residual, z);
 }
 
@@ -418,6 +425,52 @@ void launch_join(const ProductParams& p, hipStream_t stream) {
     }
 }
 
+// ---- dx of few rows: tiles of 32 or 64 rows by 256 columns, so that a row of the weights is read in runs of 512 bytes, and a sum that all compute units share
+// (16 x 131072 classes -> 4096 bf16, both planes: 176 us, 6.1 TB/s of the weights, 467 in tiles of 32; small products are faster in small tiles: the gradients
+// of 64 x 512 -> 2000 classes 29 us, 32 with wide ones, which the estimates below tell apart).
+template <typename T, int BI, int STAGES, bool PLANES>
+__global__ __launch_bounds__(256) void wide_product_kernel(const ProductParams p) {
+    __shared__ __align__(1024) char lds[product_lds<BI, 256, 1, 4, 1, STAGES>()];
+    product<T, BI, 256, 1, 4, 1, STAGES, WHOLE_PIECES, 1, false, false, true, PLANES>(p, blockIdx.x, lds);
+}
+constexpr int kWideRows = 64, kWideSplits = 64;
+struct WidePlan {
+    int splits;
+    float time;
+};
+inline WidePlan plan_wide(int rows, int cols, int sum, int size, bool planes) {
+    const int tiles = (cols - 1) / 256 + 1, steps = (int)(((long long)sum * size + kStepBytes - 1) / kStepBytes);
+    const int splits = std::max(1, std::min({kWideSplits, kComputeUnits / tiles, steps / 4})), each = (steps + splits - 1) / splits;
+    const float read = (float)cols * (float)sum * (float)size / (planes ? 12.0e6f : 6.0e6f), rounds = std::ceil((float)(tiles * splits) / (float)kComputeUnits);
+    const float partial = splits > 1 ? 2.3f + (float)splits * (float)rows * (float)cols * 8.0f / 4.0e6f : 0.0f;
+    return {(steps + each - 1) / each, 3.0f + std::max(rounds * (float)each * 0.35f, read) + partial};
+}
+inline size_t wide_bytes(int rows, int cols, int sum, int size) {
+    const WidePlan w = plan_wide(rows, cols, sum, size, false);
+    return size == 2 && rows <= kWideRows && w.splits > 1 ? (size_t)w.splits * rows * cols * sizeof(float) : 0;
+}
+template <typename T>
+bool launch_wide(ProductParams dx, float* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2) {
+        if (dx.rows > kWideRows || dx.carry || access_of<T, false, true>(dx) != WHOLE_PIECES) return false;
+        const int sum = dx.plane + dx.sum;
+        const WidePlan w = plan_wide(dx.rows, dx.cols, sum, (int)sizeof(T), dx.plane != 0);
+        if (wide_bytes(dx.rows, dx.cols, sum, (int)sizeof(T)) > workspace_bytes) return false;
+        if (w.time >= plan_product(dx.rows, dx.cols, sum, (int)sizeof(T), true, workspace_bytes).time) return false;
+        cut_product(dx, 256, kStepBytes / (int)sizeof(T), w.splits, workspace);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(dx.tiles_j * dx.splits)), dim3(256), 0, stream, dx);
+        };
+        if (dx.rows <= 32)
+            dx.plane ? go(wide_product_kernel<T, 32, 4, true>) : go(wide_product_kernel<T, 32, 4, false>);
+        else
+            dx.plane ? go(wide_product_kernel<T, 64, 3, true>) : go(wide_product_kernel<T, 64, 3, false>);
+        if (dx.splits > 1) launch_join<T>(dx, stream);
+        return true;
+    }
+    return false;
+}
+
 // A carried sum has the splits that it began with.
 template <typename T, bool ACROSS_I, bool ACROSS_J>
 int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
@@ -541,8 +594,9 @@ size_t split_bytes(int rows, int cols, int sum, int dtype, bool forward) {
 
 namespace head {
 
-size_t gradient_product_bytes(int rows, int in_features, int out_features, int dtype) {
-    return std::max(split_bytes(rows, in_features, out_features, dtype, false), split_bytes(out_features, in_features, rows, dtype, false));
+size_t gradient_product_bytes(int rows, int in_features, int out_features, int dtype, bool together) {
+    const size_t wide = together ? wide_bytes(rows, in_features, out_features, (int)dtype_bytes(dtype)) : 0;
+    return std::max(wide, std::max(split_bytes(rows, in_features, out_features, dtype, false), split_bytes(out_features, in_features, rows, dtype, false)));
 }
 
 int launch_gradient_products(int dtype, const ProductParams& dx, const ProductParams& dw, float* workspace, size_t workspace_bytes, hipStream_t stream,
@@ -557,7 +611,9 @@ int launch_gradient_products(int dtype, const ProductParams& dx, const ProductPa
             TCBNN_LAUNCH_CHECK("large_gradients_kernel");
             return TCBNN_OK;
         }
-        if (dx.out && dx.rows > 0)
+        const bool wide = together && dx.out && dx.rows > 0 && launch_wide<T>(dx, workspace, workspace_bytes, stream);
+        TCBNN_LAUNCH_CHECK("wide_product_kernel");
+        if (dx.out && dx.rows > 0 && !wide)
             if (int rc = launch_product<T, false, true>(dx, dx.carry ? dx.partial : workspace, workspace_bytes, stream)) return rc;
         if (dw.out)
             if (int rc = launch_product<T, true, true>(dw, workspace, workspace_bytes, stream)) return rc;

@@ -521,7 +521,8 @@ inline LossWorkspace loss_workspace(int rows, int in_features, int classes, int 
     w.sums = w.d + packed_bytes((long long)rows * planes, w.piece, size);
     w.dx = w.sums + whole_lines((size_t)((rows + 31) / 32) * w.piece * sizeof(float));
     w.split = w.dx + (carried ? whole_lines((size_t)w.splits * rows * in_features * sizeof(float)) : 0);
-    w.total = w.split + gradient_product_bytes(rows * planes, in_features, w.piece * planes, dtype);
+    w.total = w.split + std::max(gradient_product_bytes(rows, in_features, planes > 1 ? plane_of(w.piece, size) + w.piece : w.piece, dtype, true),
+                                 gradient_product_bytes(planes > 1 ? plane_of(rows, size) + rows : rows, in_features, w.piece, dtype));
     return w;
 }
 
