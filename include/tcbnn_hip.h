@@ -656,6 +656,7 @@ int tcbnn_logprobs_backward(const tcbnn_logprobs_grad_desc* d, void* stream);
  *   t < 0        : a row without a class: loss 0.   t >= classes: loss NaN.
  *   bias_j = -inf: a forbidden class; z_t = -inf: loss +inf; every z_j = -inf: logsumexp -inf.
  *   NaN, +inf    : the row's logsumexp and loss are NaN.
+ * Finite masks, the type's lowest value too, are logits like others.  Rows of either operand are less than 2^31 / 256 bytes apart.
  * `workspace` holds tcbnn_linear_loss_workspace_bytes; with `anywhere` these are enough for copies of operands whose rows do not lie at whole 16
  * bytes, where these are faster (without, such operands are read as they lie).  rows <= 2^31 - 2^22, in_features <= 1048576, classes <= 2^28. */
 typedef struct tcbnn_linear_loss_desc {

@@ -29,6 +29,8 @@ struct LossGradParams {
 };
 
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+// Past it a finite logit times log2 e has no place in fp32, as a mask of the type's lowest value has none: exponents of such rows are taken of the difference.
+constexpr float kFarLogit = 0x1p126f;
 // exp(m - to) s: what a sum of exponentials about m is about `to`, m <= to
 __device__ __forceinline__ float about(float m, float s, float to) { return m == to ? s : s * exp_fast(m - to); }
 // f(v, v of the lane 32 away)
@@ -93,6 +95,15 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void loss_product_kernel(const P
 #pragma unroll
                 for (int v = 0; v < 16; ++v) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][v], kLog2e, -c));
             s = across_halves(s, add) * __builtin_amdgcn_exp2f(-__builtin_fmaf(base, kLog2e, -c));
+            if (__any(fabsf(base) > kFarLogit)) {
+                float far = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) far += exp_fast(acc[a][b][v] - base);
+                far = across_halves(far, add);
+                s = fabsf(base) > kFarLogit ? far : s;
+            }
             if (spot.lane < 32) rows[spot.wj / (32 * NJ) * BI + row] = make_float2(m, s);
             const long long i = spot.i0 + row;
             const long long t = l.targets && i < p.rows ? (long long)l.targets[i] - l.first - j0 : -1;
@@ -251,10 +262,18 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) void loss_grad_product_kernel(co
             const float g = t < l.classes ? l.dloss[row] : NAN;
             // (about logsumexp log2 e as it is rounded: no more than logsumexp's own rounding)
             const float c = lse * kLog2e;
+            if (__any(fabsf(lse) > kFarLogit)) {
+                const bool far = fabsf(lse) > kFarLogit;
 #pragma unroll
-            for (int b = 0; b < NJ; ++b)
+                for (int b = 0; b < NJ; ++b)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) acc[a][b][v] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][v], kLog2e, -c));
+                    for (int v = 0; v < 16; ++v) acc[a][b][v] = g * (far ? exp_fast(acc[a][b][v] - lse) : __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][v], kLog2e, -c)));
+            } else {
+#pragma unroll
+                for (int b = 0; b < NJ; ++b)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) acc[a][b][v] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][v], kLog2e, -c));
+            }
             if (__any(none)) {
 #pragma unroll
                 for (int b = 0; b < NJ; ++b)
@@ -365,7 +384,8 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const bool there = j + e < p.cols;
-        d[e] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[e] + (p.bias && there ? p.bias[j + e] : 0.0f), kLog2e, -c));
+        const float z = acc[e] + (p.bias && there ? p.bias[j + e] : 0.0f);
+        d[e] = g * (fabsf(lse) > kFarLogit ? exp_fast(z - lse) : __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -c)));
         d[e] = none || !there ? 0.0f : l.first + j + e == t ? d[e] - g : d[e];
         if (l.sums) {
             float s = d[e];

@@ -362,7 +362,7 @@ LOSS = [(1, 1, 1), (1, 16, 10), (1, 4096, 512), (1, 1025, 3), (2, 8, 17), (3, 17
         (255, 1000, 511), (513, 96, 300), (4, 1023, 4099), (1000, 1001, 999), (3, 5, 4000), (40, 7, 30), (9, 512, 16392), (2100, 64, 40)]
 
 
-def _loss(gpu, m, k, n, dtype, bias=True, gap=0, shift=1, stream=None, want=("input", "weight", "bias"), scale=1.0, forbidden=(), t=None, targets=True):
+def _loss(gpu, m, k, n, dtype, bias=True, gap=0, shift=1, stream=None, want=("input", "weight", "bias"), scale=1.0, forbidden=(), t=None, mask=-np.inf):
     from tcbnn_amd import head
     r = rng(m, k, n, len(dtype), 4)
     wv = 2.5 * r.standard_normal((n, k)) / np.sqrt(k)
@@ -373,7 +373,7 @@ def _loss(gpu, m, k, n, dtype, bias=True, gap=0, shift=1, stream=None, want=("in
     x, w = ho.Matrix(xv, dtype, gap, shift=shift), ho.Matrix(wv, dtype, gap, shift=shift)
     b = r.standard_normal(n).astype(np.float32) if bias else None
     if len(forbidden):
-        b[forbidden] = -np.inf
+        b[forbidden] = mask
     g = (scale * (0.5 + r.random(m))).astype(np.float32)
     dx, dw, db = ho.Matrix(None, dtype, gap, m, k), ho.Matrix(None, dtype, gap, n, k), ho.empty(n)
     layer = head.LinearLossLayerParam("loss", m, k, n, dtype)
@@ -496,6 +496,36 @@ def test_loss_of_forbidden_classes(gpu):
             t = r.integers(n // 2, n, m).astype(np.int32)
             t[::5] = -1
             _loss(gpu, m, k, n, dtype, forbidden=np.arange(n // 2), t=t)
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n,shift", [(1, 64, 100, 1), (3, 40, 70, 0), (12, 40, 700, 1), (40, 24, 130, 0), (150, 72, 1000, 1), (1024, 64, 1024, 0), (2048, 64, 2048, 0)])
+def test_loss_of_classes_masked_by_the_lowest_value(gpu, m, k, n, shift, dtype):
+    """A bias of the lowest finite value, over whole tiles: as good as -inf."""
+    _loss(gpu, m, k, n, dtype, shift=shift, forbidden=np.arange(n - n // 2, n), t=rng(m, n).integers(-1, n - n // 2, m).astype(np.int32), mask=np.finfo(np.float32).min)
+
+
+@pytest.mark.parametrize("m,k,n", [(2, 24, 40), (9, 24, 40), (40, 24, 300), (2048, 64, 2048)])
+def test_loss_of_rows_far_from_0(gpu, m, k, n):
+    """Every class at the lowest finite value, or at the highest: log(classes), and gradients that are numbers."""
+    from tcbnn_amd import head
+    for dtype in ho.DTYPES:
+        for value in (np.finfo(np.float32).min, 3e38):
+            r = rng(m, n)
+            x, w = (ho.Matrix(r.standard_normal((rows, k)), dtype, shift=0) for rows in (m, n))
+            dx, dw, db = ho.Matrix(None, dtype, 0, m, k, shift=0), ho.Matrix(None, dtype, 0, n, k, shift=0), ho.empty(n)
+            layer = head.LinearLossLayerParam("loss", m, k, n, dtype)
+            layer.initialize(w.view, np.full(n, value, np.float32), x.view, ho.vector(r.integers(0, n, m), np.int32))
+            layer.initialize_backward(ho.vector(np.full(m, 1.0 / n)), dx.view, dw.view, db)
+            layer.forward()
+            layer.backward()
+            ho.sync()
+            out = layer.download_output()
+            assert (out["logsumexp"] == np.float32(value)).all()
+            # (the sum is of n ones, its logarithm off by a few units)
+            np.testing.assert_allclose(out["loss"], np.log(n), rtol=2.0 ** -20)
+            assert np.isfinite(dx.get()).all() and np.isfinite(dw.get()).all() and np.isfinite(db.to_numpy(np.float32, (n,))).all()
+            layer.release()
 
 
 def test_loss_of_degenerate_rows(gpu):
