@@ -260,10 +260,10 @@ struct GatedPlan {
 };
 inline GatedPlan plan_gated(int rows, int cols, int sum, int size, Access access, bool i_anywhere, bool j_anywhere, size_t workspace_bytes) {
     const bool vectors = access == WHOLE_PIECES;
-    GatedPlan g = {access, plan_product(rows, 2 * cols, sum, size, vectors, 0), false, false, false};
+    GatedPlan g = {access, plan_product(rows, 2 * cols, sum, size, vectors, 0, CUT_256, true), false, false, false};
     g.few = rows <= kFewRows && (access == ELEMENTS || few_time(rows, 2 * cols, sum, size, vectors) < g.plan.time);
     if (g.few || access != ANYWHERE) return g;
-    const Plan whole = plan_product(rows, 2 * cols, sum, size, true, 0);
+    const Plan whole = plan_product(rows, 2 * cols, sum, size, true, 0, CUT_256, true);
     const size_t i_bytes = i_anywhere ? packed_bytes(rows, sum, size) : 0, j_bytes = j_anywhere ? packed_bytes(2LL * cols, sum, size) : 0;
     if (i_bytes + j_bytes > workspace_bytes) return g;
     if (whole.time + (i_anywhere ? pack_time(i_bytes) : 0.0f) + (j_anywhere ? pack_time(j_bytes) : 0.0f) >= g.plan.time) return g;

@@ -440,7 +440,7 @@ inline LossPlan plan_loss(int rows, int classes, int sum, int size, Access acces
     const bool vectors = access == WHOLE_PIECES;
     LossPlan l = {};
     l.access = access;
-    l.plan = plan_product(rows, classes, sum, size, vectors, 0);
+    l.plan = plan_product(rows, classes, sum, size, vectors, 0, CUT_256, true);
     l.few = rows <= kFewRows && (access == ELEMENTS || few_time(rows, classes, sum, size, vectors) < l.plan.time);
     const int width = l.few ? kFewOutputs : cut_size(access, l.plan.cut);
     l.parts = (classes - 1) / width + 1;
@@ -740,7 +740,7 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             p.out_ld = d_ld;
             LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes, low};
             const Access access = access_of<T, false, false>(p);
-            const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0);
+            const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0, CUT_256, true);
             const bool few = p.rows <= kFewRows && (access == ELEMENTS || few_time(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES) < plan.time);
             const int tiles_i = few ? 1 : (p.rows - 1) / cut_size(access, plan.cut) + 1;
             if (l.sums && tiles_i == 1) l.sums = d->grad_bias + first;

@@ -718,7 +718,10 @@ struct Plan {
     int splits;
     float time;
 };
-inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, size_t workspace_bytes, Cut largest = CUT_256) {
+// `pairs`: a compute unit has two workgroups at a time of all tiles but the two that take its shared memory, so that of an odd number of them the last
+// one works alone (losses, bf16: 300 x 4096 -> 32000 classes 135 us in tiles of 128, three a compute unit, 105 in tiles of 256; 333 x 1024 -> 32000 39
+// and 33; 2000 x 512 -> 5000 23.0 and 21.0).
+inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, size_t workspace_bytes, Cut largest = CUT_256, bool pairs = false) {
     const int steps = (int)(((long long)sum * size + kStepBytes - 1) / kStepBytes);
     const float read = ((float)rows + (float)cols) * (float)sum * (float)size / kReadRate;
     Plan best = {CUT_32, 1, 0.0f};
@@ -730,7 +733,9 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
         for (int k = 1; k <= kMaxSplits && (k == 1 || steps >= 4 * k); k *= 2) {
             const size_t partial = k > 1 ? (size_t)k * rows * cols * sizeof(float) : 0;
             if (partial > workspace_bytes) break;
-            const float rounds = std::ceil(tiles * (float)k / (float)kComputeUnits), each = std::max(cost.step, rounds * cost.more);
+            const float rounds = std::ceil(tiles * (float)k / (float)kComputeUnits);
+            const bool alone = pairs && rounds > 1.0f && std::fmod(rounds, 2.0f) == 1.0f && c != CUT_256 && c != CUT_128_DEEP;
+            const float each = std::max(cost.step, rounds * cost.more) + (alone ? std::max(0.0f, cost.step - cost.more) : 0.0f);
             const float time = cost.start + (rounds - 1.0f) * cost.tile + std::max((float)((steps + k - 1) / k) * each, read) + (k > 1 ? (vectors ? 2.3f : 3.0f) + (float)partial * 2.0f / 4.0e6f : 0.0f);
             if (best.time == 0.0f || time < best.time) best = {(Cut)c, k, time};
         }
