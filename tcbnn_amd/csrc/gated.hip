@@ -35,7 +35,7 @@ __device__ __forceinline__ void finish(const ProductParams& p, long long i, int 
 
 // `p.cols` is n; a workgroup's tile is BI rows by BJ / 2 columns of either half.
 template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG>
-__global__ __launch_bounds__(64 * WI * WJ * WS) void gated_product_kernel(const ProductParams p) {
+__global__ __launch_bounds__(64 * WI * WJ * WS) __attribute__((amdgpu_waves_per_eu(short_waves(WI * WJ * WS, STAGES)))) void gated_product_kernel(const ProductParams p) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
     __shared__ __align__(1024) char lds[product_lds<BI, BJ, WI, WJ, WS, STAGES>()];
     constexpr int NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec;
@@ -257,21 +257,25 @@ __global__ __launch_bounds__(kDzThreads) void gated_dz_few_rows_kernel(const T* 
 
 // The tile is the one that the linear layer's estimates would take for a product of 2 n columns; sums are not split.  Operands that lie anywhere are
 // copied where the product of the copies and the copying are estimated to take less time, and the workspace holds them.
+// (Tiles for short sums: 8192 x 256 -> 2 x 4096 bf16 with z kept, 4 steps, 86 us, 101 in tiles of 256; 8192 x 384 -> 2 x 512, 6 steps, 15.2 and 16.0; 8192 x 512 -> 2 x 2048, 8
+// steps, 60 and 58.)
+constexpr int kGatedShortSteps = 6;
 struct GatedPlan {
     Access access;
     Plan plan;
-    bool few, pack_i, pack_j;
+    bool few, brief, pack_i, pack_j;
 };
 inline GatedPlan plan_gated(int rows, int cols, int sum, int size, Access access, bool i_anywhere, bool j_anywhere, size_t workspace_bytes) {
     const bool vectors = access == WHOLE_PIECES;
-    GatedPlan g = {access, plan_product(rows, 2 * cols, sum, size, vectors, 0, CUT_256, true), false, false, false};
+    GatedPlan g = {access, plan_product(rows, 2 * cols, sum, size, vectors, 0, CUT_256, true), false, false, false, false};
     g.few = rows <= kFewRows && (access == ELEMENTS || few_time(rows, 2 * cols, sum, size, vectors) < g.plan.time);
+    g.brief = !g.few && short_sum(access, rows, 2 * cols, sum, size, kGatedShortSteps);
     if (g.few || access != ANYWHERE) return g;
     const Plan whole = plan_product(rows, 2 * cols, sum, size, true, 0, CUT_256, true);
     const size_t i_bytes = i_anywhere ? packed_bytes(rows, sum, size) : 0, j_bytes = j_anywhere ? packed_bytes(2LL * cols, sum, size) : 0;
     if (i_bytes + j_bytes > workspace_bytes) return g;
     if (whole.time + (i_anywhere ? pack_time(i_bytes) : 0.0f) + (j_anywhere ? pack_time(j_bytes) : 0.0f) >= g.plan.time) return g;
-    return {WHOLE_PIECES, whole, false, i_anywhere, j_anywhere};
+    return {WHOLE_PIECES, whole, false, short_sum(WHOLE_PIECES, rows, 2 * cols, sum, size, kGatedShortSteps), i_anywhere, j_anywhere};
 }
 template <typename T>
 GatedPlan plan_gated(const ProductParams& p, size_t workspace_bytes) {
@@ -295,7 +299,7 @@ int launch_gated(ProductParams p, int dtype, void* workspace, size_t workspace_b
         TCBNN_LAUNCH_CHECK("gated_few_rows_kernel");
         return TCBNN_OK;
     }
-    by_tile(g.access, g.plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
+    by_tile(g.access, g.plan.cut, g.brief, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
         constexpr int B = size.value, WI = wi.value, WJ = wj.value, WS = ws.value, S = stages.value, H = hold.value;
         constexpr bool L = keep.value;
         constexpr int kThreads = 64 * WI * WJ * WS;
@@ -331,7 +335,7 @@ void gated_name(const ProductParams& p, size_t workspace_bytes, char* buf, size_
         {"", "128, 128, 2, 2, 1, 2", "", "64, 64, 2, 2, 2, 2", "32, 32, 1, 1, 4, 2"},
         {"32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2", "32, 32, 1, 1, 4, 2"}};
     const int hold = g.access == ANYWHERE && g.plan.cut != CUT_128 ? 4 : 1;
-    snprintf(buf, len, "gated_product_kernel<%s, %s, (Access)%d, %d, %s>", type, shape[g.access][g.plan.cut], (int)g.access, hold,
+    snprintf(buf, len, "gated_product_kernel<%s, %s, (Access)%d, %d, %s>", type, g.brief ? "128, 128, 2, 2, 1, 1" : shape[g.access][g.plan.cut], (int)g.access, hold,
              hold == 4 && g.plan.cut != CUT_64 ? "true" : "false");
 }
 

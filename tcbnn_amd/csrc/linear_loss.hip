@@ -69,7 +69,7 @@ __device__ __forceinline__ void add_bias(Acc (&acc)[NI][NJ], const ProductParams
 }
 
 template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG>
-__global__ __launch_bounds__(64 * WI * WJ * WS) void loss_product_kernel(const ProductParams p, const LossParams l) {
+__global__ __launch_bounds__(64 * WI * WJ * WS) __attribute__((amdgpu_waves_per_eu(short_waves(WI * WJ * WS, STAGES)))) void loss_product_kernel(const ProductParams p, const LossParams l) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
     __shared__ __align__(1024) char lds[product_lds<BI, BJ, WI, WJ, WS, STAGES>()];
     constexpr int NI = BI / WI / 32, NJ = BJ / WJ / 32;
@@ -242,7 +242,7 @@ __device__ __forceinline__ float half_sum(float v) {
 
 // d of a piece of the classes: p.out [rows][out_ld], the columns behind the last one of 16 bytes 0
 template <typename T, int BI, int BJ, int WI, int WJ, int WS, int STAGES, Access ACCESS, int HOLD, bool LONG>
-__global__ __launch_bounds__(64 * WI * WJ * WS) void loss_grad_product_kernel(const ProductParams p, const LossGradParams l) {
+__global__ __launch_bounds__(64 * WI * WJ * WS) __attribute__((amdgpu_waves_per_eu(short_waves(WI * WJ * WS, STAGES)))) void loss_grad_product_kernel(const ProductParams p, const LossGradParams l) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass leaves a kernel's stub out where it instantiates a tile's requests twice)
     __shared__ __align__(1024) char lds[product_lds<BI, BJ, WI, WJ, WS, STAGES>()];
     constexpr int NI = BI / WI / 32, NJ = BJ / WJ / 32, V = Elem<T>::kVec, kThreads = 64 * WI * WJ * WS;
@@ -429,12 +429,12 @@ void launch_grad_few_rows(const ProductParams& p, const LossGradParams& l, hipSt
 
 // ---- plans
 // rows and columns of a tile (by_tile)
-inline int cut_size(Access access, Cut cut) { return access == ELEMENTS ? 32 : (access == WHOLE_PIECES ? kCuts16 : kCutsAnywhere)[cut].size; }
+inline int cut_size(Access access, Cut cut, bool brief) { return brief ? 128 : access == ELEMENTS ? 32 : (access == WHOLE_PIECES ? kCuts16 : kCutsAnywhere)[cut].size; }
 // The forward call's kernel: its tile, or the one for few rows; the number of parts that it leaves of a row.
 struct LossPlan {
     Access access;
     Plan plan;
-    bool few;
+    bool few, brief;
     int parts;
     bool pack_x, pack_w;
 };
@@ -444,7 +444,8 @@ inline LossPlan plan_loss(int rows, int classes, int sum, int size, Access acces
     l.access = access;
     l.plan = plan_product(rows, classes, sum, size, vectors, 0, CUT_256, true);
     l.few = rows <= kFewRows && (access == ELEMENTS || few_time(rows, classes, sum, size, vectors) < l.plan.time);
-    const int width = l.few ? kFewOutputs : cut_size(access, l.plan.cut);
+    l.brief = !l.few && short_sum(access, rows, classes, sum, size);
+    const int width = l.few ? kFewOutputs : cut_size(access, l.plan.cut, l.brief);
     l.parts = (classes - 1) / width + 1;
     return l;
 }
@@ -623,7 +624,7 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
             else
                 hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_few_rows_kernel<T, 2>), grid, dim3(64 * kFewWaves), 0, s, p, l);
         } else {
-            by_tile(plan.access, plan.plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
+            by_tile(plan.access, plan.plan.cut, plan.brief, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
                 constexpr int B = size.value, kThreads = 64 * wi.value * wj.value * ws.value;
                 // rows beyond a launch's threads have one of their own
                 const long long at_once = std::max(1LL, kMaxThreads / kThreads / plan.parts) * B;
@@ -745,10 +746,11 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             const Access access = access_of<T, false, false>(p);
             const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0, CUT_256, true);
             const bool few = p.rows <= kFewRows && (access == ELEMENTS || few_time(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES) < plan.time);
-            const int tiles_i = few ? 1 : (p.rows - 1) / cut_size(access, plan.cut) + 1;
+            const bool brief = !few && short_sum(access, p.rows, p.cols, p.sum, (int)sizeof(T));
+            const int tiles_i = few ? 1 : (p.rows - 1) / cut_size(access, plan.cut, brief) + 1;
             if (l.sums && tiles_i == 1) l.sums = d->grad_bias + first;
             if (few) launch_grad_few_rows<T, false>(p, l, s);
-            if (!few) by_tile(access, plan.cut, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
+            if (!few) by_tile(access, plan.cut, brief, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
                 constexpr int B = size.value, kThreads = 64 * wi.value * wj.value * ws.value;
                 // rows beyond a launch's threads have one of their own
                 const long long tiles_j = (p.cols - 1) / B + 1, at_once = std::max(1LL, kMaxThreads / kThreads / tiles_j) * B;

@@ -391,6 +391,7 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
     using TileJ = Tile<T, BJ, ACROSS_J, ACCESS, kThreads, HOLD, kHidden, PAIRED>;
     constexpr int kStage = TileI::kBytes + TileJ::kBytes;
     static_assert(ALIGNED || STAGES == 2, "what registers hold needs two tiles");
+    static_assert(STAGES > 1 || WS == 1, "");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // Workgroups go to the 8 XCDs in turn: each XCD gets a run of tiles, and a run covers 8 tiles of i after 8 tiles of i, so that what
@@ -506,7 +507,21 @@ __device__ __forceinline__ void product_sums(const ProductParams& p, int block, 
     constexpr int kRequests = TileI::kEach + TileJ::kEach;
     int stage = 0;
     if (steps > 0) {
-        if constexpr (ALIGNED) {
+        if constexpr (STAGES == 1) {  // (a workgroup waits for its step, others beside it work)
+            for (int step = 0; step < steps; ++step) {
+                if (step > 0) meet<0>();
+                request_j(0, step, slot0);
+                request_i(0, step, slot0);
+                meet<0>();
+                fragments(0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < kQuarters; ++k) {
+                    if (k + 1 < kQuarters) fragments((k + 1) & 1, 0, k + 1);
+                    multiply(k & 1);
+                }
+            }
+            meet<0>();
+        } else if constexpr (ALIGNED) {
             // Step t + STAGES is requested into the tiles of step t as soon as these are done with: J's with the last quarter of step
             // t, I's with the first of step t + 1 (where a wavefront has a quarter alone, both at once).
             constexpr bool kApart = kQuarters > 1;
@@ -768,8 +783,18 @@ Access access_of(const ProductParams& p) {
     return std::max(of(p.i, p.rows, p.sum, ACROSS_I, p.padded_i), of(p.j, p.cols, p.sum, ACROSS_J, p.padded_j));
 }
 // f(tile, wavefronts of i, of j, of the sum, stages, access, steps held, long sums) with the constants of a tile's kernel (product_sums)
+// Short sums of many tiles: a tile's life is its launch, its first requests and what follows its sums rather than these, and so several workgroups a compute unit do more
+// than steps under way.  Tiles of 128 with one step in LDS, four of them at a time (losses, bf16: 3043 x 32 -> 17021 classes 23 us, 32 in tiles
+// of 256; 4096 x 512 -> 65536, 8 steps, 272 and 282; 8192 x 1024 -> 32768, 16 steps, 495 and 472; 200 x 512 -> 20000, 314 tiles, 16.7 and 16.1).
+constexpr int kShortSteps = 8, kShortTiles = 3 * kComputeUnits / 2;
+inline bool short_sum(Access access, int rows, int cols, int sum, int size, int steps = kShortSteps) {
+    const long long tiles = ((rows - 1) / 128 + 1LL) * ((cols - 1) / 128 + 1);
+    return access == WHOLE_PIECES && (long long)sum * size <= steps * kStepBytes && tiles >= kShortTiles;
+}
+constexpr int short_waves(int waves, int stages) { return stages == 1 ? 4 : (waves + 3) / 4; }  // wavefronts a SIMD that registers do for
+
 template <typename F>
-void by_tile(Access access, Cut cut, F&& f) {
+void by_tile(Access access, Cut cut, bool brief, F&& f) {
     constexpr std::integral_constant<int, 256> n256;
     constexpr std::integral_constant<int, 128> n128;
     constexpr std::integral_constant<int, 64> n64;
@@ -784,6 +809,7 @@ void by_tile(Access access, Cut cut, F&& f) {
     constexpr std::integral_constant<Access, ANYWHERE> anywhere;
     constexpr std::integral_constant<Access, ELEMENTS> elements;
     if (access == WHOLE_PIECES) {
+        if (brief) return f(n128, two, two, one, one, pieces, one, no);
         switch (cut) {
             case CUT_256: return f(n256, two, four, one, two, pieces, one, no);
             case CUT_128: return f(n128, two, two, one, two, pieces, one, no);

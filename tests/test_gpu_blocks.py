@@ -250,7 +250,8 @@ def _gated_kernel(m, k, n, dtype):
 GATED_WHOLE = [((1, 64, 64), "few_rows_kernel<__bf16, 8>"), ((16, 1048, 72), "few_rows_kernel<__bf16, 8>"), ((3, 264, 8204), "few_rows_kernel<__bf16, 2>"),
                ((17, 1048, 36), "32, 32"), ((33, 8, 4), "32, 32"), ((100, 520, 152), "32, 32"), ((64, 2048, 1024), "32, 32"), ((1024, 512, 512), "64, 64"),
                ((1000, 72, 1500), "64, 64"), ((2040, 136, 1020), "128, 128, 2, 2, 2, 4"), ((2048, 512, 1024), "128, 128, 2, 2, 2, 4"),
-               ((2040, 72, 1028), "128, 128, 2, 2, 1, 2"), ((2040, 72, 2052), "256, 256"), ((4096, 64, 2048), "256, 256"), ((4000, 200, 2044), "256, 256")]
+               ((2040, 72, 1028), "128, 128, 2, 2, 1, 2"), ((2040, 72, 2052), "128, 128, 2, 2, 1, 1"), ((4096, 64, 2048), "128, 128, 2, 2, 1, 1"),
+               ((4000, 200, 2044), "128, 128, 2, 2, 1, 1"), ((4096, 392, 2048), "256, 256"), ((4000, 400, 2044), "256, 256")]
 
 
 @pytest.mark.parametrize("shape,kernel", GATED_WHOLE)
@@ -324,6 +325,13 @@ def test_gated_grad_strides_and_single_outputs(gpu, m, k, n, dtype):
     _gated_grad(gpu, m, k, n, dtype, "none", gap=8, shift=0)
     for want in (("x",), ("w",), ("b",), ("w", "b")):
         _gated_grad(gpu, m, k, n, dtype, "silu", want=want)
+
+
+# weights' gradients of short sums and many tiles, odd columns among them
+@pytest.mark.parametrize("m,k,n", [(16, 2048, 2000), (70, 1024, 3200), (33, 1024, 3203), (500, 520, 5000)])
+def test_gated_grad_of_short_sums(gpu, m, k, n):
+    for dtype in ho.DTYPES:
+        _gated_grad(gpu, m, k, n, dtype, "silu", shift=0)
 
 
 # large enough that copies of operands that lie anywhere are taken: odd inputs, rows out of wider arrays, odd features, each operand alone
@@ -496,6 +504,13 @@ def test_loss_of_forbidden_classes(gpu):
             t = r.integers(n // 2, n, m).astype(np.int32)
             t[::5] = -1
             _loss(gpu, m, k, n, dtype, forbidden=np.arange(n // 2), t=t)
+
+
+# short sums and many tiles, of the logits and of the weights' gradients; the largest tiles
+@pytest.mark.parametrize("m,k,n", [(16, 2048, 4000), (40, 1024, 8000), (40, 1024, 8003), (300, 520, 12500), (2048, 64, 4096), (2040, 72, 4100), (1100, 504, 6000), (4096, 1040, 2048)])
+def test_loss_of_short_sums(gpu, m, k, n):
+    for dtype in ho.DTYPES:
+        _loss(gpu, m, k, n, dtype, shift=0)
 
 
 @pytest.mark.parametrize("dtype", ho.DTYPES)
