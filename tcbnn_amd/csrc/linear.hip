@@ -425,7 +425,7 @@ void launch_join(const ProductParams& p, hipStream_t stream) {
     }
 }
 
-// ---- dx of few rows: tiles of 32 or 64 rows by 256 columns, so that a row of the weights is read in runs of 512 bytes, and a sum that all compute units share
+// ---- dx of few rows: tiles of 32, 64 or 128 rows (78 x 2488 -> 43155 classes, the loss's step 298 us, 313 in tiles of 128) by 256 columns, so that a row of the weights is read in runs of 512 bytes, and a sum that all compute units share
 // (16 x 131072 classes -> 4096 bf16, both planes: 176 us, 6.1 TB/s of the weights, 467 in tiles of 32; small products are faster in small tiles: the gradients
 // of 64 x 512 -> 2000 classes 29 us, 32 with wide ones, which the estimates below tell apart).
 template <typename T, int BI, int STAGES, bool PLANES>
@@ -433,7 +433,37 @@ __global__ __launch_bounds__(256) void wide_product_kernel(const ProductParams p
     __shared__ __align__(1024) char lds[product_lds<BI, 256, 1, 4, 1, STAGES>()];
     product<T, BI, 256, 1, 4, 1, STAGES, WHOLE_PIECES, 1, false, false, true, PLANES>(p, blockIdx.x, lds);
 }
-constexpr int kWideRows = 64, kWideSplits = 64;
+constexpr int kWideRows = 128, kWideSplits = 64;
+// Its join: 16 vectors a workgroup, 16 threads to a vector, always in the same order (64 splits of 5 x 554 21 us with a thread to a vector).
+constexpr int kWideJoined = 16, kWideJoinThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kWideJoinThreads) void wide_join_kernel(const ProductParams p) {
+    constexpr int C = kJoinVector, kParts = kWideJoinThreads / kWideJoined, kAtOnce = 4;
+    __shared__ Columns<float, C> lds[kParts][kWideJoined];
+    const int per_row = (p.cols + C - 1) / C, lane = threadIdx.x % kWideJoined, part = threadIdx.x / kWideJoined;
+    const long long v = (long long)blockIdx.x * kWideJoined + lane, i = v / per_row;
+    const int j = (int)(v - i * per_row) * C, n = i < p.rows ? min(C, p.cols - j) : 0;
+    Columns<float, C> z = {};
+    if (n > 0)
+        for (int k = part; k < p.splits; k += kAtOnce * kParts) {
+            Columns<float, C> s[kAtOnce];  // (requests of their own, one wait)
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                s[u] = k + u * kParts < p.splits ? get_columns<float, C>(p.partial + (k + u * kParts) * p.partial_stride, p.cols, i, j, n) : Columns<float, C>{};
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) z += s[u];
+        }
+    lds[part][lane] = z;
+    __syncthreads();
+    if (part != 0 || n <= 0) return;
+#pragma unroll
+    for (int k = 1; k < kParts; ++k) z += lds[k][lane];
+    float sum[C];
+#pragma unroll
+    for (int e = 0; e < C; ++e) sum[e] = z[e];
+    const float bias[C] = {};
+    finish<T, C>(p, i, j, n, bias, Columns<T, C>{}, sum);
+}
 struct WidePlan {
     int splits;
     float time;
@@ -443,7 +473,7 @@ inline WidePlan plan_wide(int rows, int cols, int sum, int size, bool planes) {
     const int splits = std::max(1, std::min({kWideSplits, kComputeUnits / tiles, steps / 4})), each = (steps + splits - 1) / splits;
     const float read = (float)cols * (float)sum * (float)size / (planes ? 12.0e6f : 6.0e6f), rounds = std::ceil((float)(tiles * splits) / (float)kComputeUnits);
     const float partial = splits > 1 ? 2.3f + (float)splits * (float)rows * (float)cols * 8.0f / 4.0e6f : 0.0f;
-    return {(steps + each - 1) / each, 3.0f + std::max(rounds * (float)each * 0.35f, read) + partial};
+    return {(steps + each - 1) / each, 3.0f + std::max(rounds * (float)each * (rows > 64 ? 0.9f : 0.35f), read) + partial};
 }
 inline size_t wide_bytes(int rows, int cols, int sum, int size) {
     const WidePlan w = plan_wide(rows, cols, sum, size, false);
@@ -461,11 +491,16 @@ bool launch_wide(ProductParams dx, float* workspace, size_t workspace_bytes, hip
         auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)(dx.tiles_j * dx.splits)), dim3(256), 0, stream, dx);
         };
-        if (dx.rows <= 32)
+        if (dx.rows > 64)
+            dx.plane ? go(wide_product_kernel<T, 128, 3, true>) : go(wide_product_kernel<T, 128, 3, false>);
+        else if (dx.rows <= 32)
             dx.plane ? go(wide_product_kernel<T, 32, 4, true>) : go(wide_product_kernel<T, 32, 4, false>);
         else
             dx.plane ? go(wide_product_kernel<T, 64, 3, true>) : go(wide_product_kernel<T, 64, 3, false>);
-        if (dx.splits > 1) launch_join<T>(dx, stream);
+        if (dx.splits > kMaxSplits)
+            hipLaunchKernelGGL(wide_join_kernel<T>, dim3((unsigned)((dx.rows * (long long)((dx.cols - 1) / kJoinVector + 1) - 1) / kWideJoined + 1)), dim3(kWideJoinThreads), 0, stream, dx);
+        else if (dx.splits > 1)
+            launch_join<T>(dx, stream);
         return true;
     }
     return false;

@@ -506,6 +506,14 @@ def test_loss_of_forbidden_classes(gpu):
             _loss(gpu, m, k, n, dtype, forbidden=np.arange(n // 2), t=t)
 
 
+# input gradients of few rows and long sums, in many parts
+@pytest.mark.parametrize("m,k,n", [(5, 560, 20889), (21, 80, 17700), (60, 304, 30000), (64, 1024, 4000), (65, 160, 22985), (100, 2488, 9000), (128, 520, 20003)])
+def test_loss_of_few_rows_and_many_classes(gpu, m, k, n):
+    for dtype in ho.DTYPES:
+        _loss(gpu, m, k, n, dtype, shift=0)
+    _loss(gpu, m, k, n, "bf16", gap=8, shift=0, want=("input",))
+
+
 # short sums and many tiles, of the logits and of the weights' gradients; the largest tiles
 @pytest.mark.parametrize("m,k,n", [(16, 2048, 4000), (40, 1024, 8000), (40, 1024, 8003), (300, 520, 12500), (2048, 64, 4096), (2040, 72, 4100), (1100, 504, 6000), (4096, 1040, 2048)])
 def test_loss_of_short_sums(gpu, m, k, n):
