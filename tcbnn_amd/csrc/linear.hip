@@ -366,7 +366,7 @@ bool launch_large_gradients(ProductParams dx, ProductParams dw, size_t workspace
         const float longest = std::max(steps_dx, steps_dw), work = ((float)blocks_dx * steps_dx + (float)blocks_dw * steps_dw) / (float)kComputeUnits;
         const float together = kCuts16[CUT_256].start + kStep * (blocks_dx + blocks_dw <= kComputeUnits ? longest : longest + work);
         float apart = 0.0f;
-        for (const ProductParams* p : {&dx, &dw}) apart += plan_product(p->rows, p->cols, p->sum, (int)sizeof(T), true, workspace_bytes).time;
+        for (const ProductParams* p : {&dx, &dw}) apart += plan_product(p->rows, p->cols, p->sum, (int)sizeof(T), true, workspace_bytes, CUT_256, true).time;
         if (together >= apart) return false;
         const bool dw_first = steps_dw > steps_dx;
         hipLaunchKernelGGL(large_gradients_kernel<T>, dim3((unsigned)(blocks_dx + blocks_dw)), dim3(512), 0, stream, dx, dw, (int)(dw_first ? blocks_dw : blocks_dx),
@@ -486,7 +486,7 @@ bool launch_wide(ProductParams dx, float* workspace, size_t workspace_bytes, hip
         const int sum = dx.plane + dx.sum;
         const WidePlan w = plan_wide(dx.rows, dx.cols, sum, (int)sizeof(T), dx.plane != 0);
         if (wide_bytes(dx.rows, dx.cols, sum, (int)sizeof(T)) > workspace_bytes) return false;
-        if (w.time >= plan_product(dx.rows, dx.cols, sum, (int)sizeof(T), true, workspace_bytes).time) return false;
+        if (w.time >= plan_product(dx.rows, dx.cols, sum, (int)sizeof(T), true, workspace_bytes, CUT_256, true).time) return false;
         cut_product(dx, 256, kStepBytes / (int)sizeof(T), w.splits, workspace);
         auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)(dx.tiles_j * dx.splits)), dim3(256), 0, stream, dx);
@@ -533,9 +533,9 @@ bool launch_short(ProductParams dw, hipStream_t stream) {
 
 // A carried sum has the splits that it began with.
 template <typename T, bool ACROSS_I, bool ACROSS_J>
-int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream) {
+int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hipStream_t stream, bool fine = false) {
     const Access access = access_of<T, ACROSS_I, ACROSS_J>(p);
-    Plan plan = plan_product(p.rows, p.cols, p.plane + p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes);
+    Plan plan = plan_product(p.rows, p.cols, p.plane + p.sum, (int)sizeof(T), access == WHOLE_PIECES, workspace_bytes, CUT_256, fine);
     if (p.carry) plan.splits = p.splits;
     if constexpr (!ACROSS_I && !ACROSS_J) {
         if (few_rows<T>(p, access, plan)) {
@@ -640,11 +640,11 @@ __global__ __launch_bounds__(kPackThreads) void pack_rows_kernel(const T* __rest
 }
 
 // the partial sums of a split product
-size_t split_bytes(int rows, int cols, int sum, int dtype, bool forward) {
+size_t split_bytes(int rows, int cols, int sum, int dtype, bool forward, bool fine = false) {
     const int size = (int)dtype_bytes(dtype);
     int splits = 1;
     for (bool vectors : {false, true}) {  // (where the operands will lie is not known here)
-        const Plan plan = plan_product(rows, cols, sum, size, vectors, ~(size_t)0);
+        const Plan plan = plan_product(rows, cols, sum, size, vectors, ~(size_t)0, CUT_256, fine);
         if (!forward || rows > kFewRows || few_time(rows, cols, sum, size, vectors) >= plan.time) splits = std::max(splits, plan.splits);
     }
     return splits > 1 ? (size_t)splits * rows * cols * sizeof(float) : 0;
@@ -656,7 +656,8 @@ namespace head {
 
 size_t gradient_product_bytes(int rows, int in_features, int out_features, int dtype, bool together) {
     const size_t wide = together ? wide_bytes(rows, in_features, out_features, (int)dtype_bytes(dtype)) : 0;
-    return std::max(wide, std::max(split_bytes(rows, in_features, out_features, dtype, false), split_bytes(out_features, in_features, rows, dtype, false)));
+    return std::max(wide, std::max(split_bytes(rows, in_features, out_features, dtype, false, together),
+                                   split_bytes(out_features, in_features, rows, dtype, false, together)));
 }
 
 int launch_gradient_products(int dtype, const ProductParams& dx, const ProductParams& dw, float* workspace, size_t workspace_bytes, hipStream_t stream,
@@ -674,11 +675,11 @@ int launch_gradient_products(int dtype, const ProductParams& dx, const ProductPa
         const bool wide = together && dx.out && dx.rows > 0 && launch_wide<T>(dx, workspace, workspace_bytes, stream);
         TCBNN_LAUNCH_CHECK("wide_product_kernel");
         if (dx.out && dx.rows > 0 && !wide)
-            if (int rc = launch_product<T, false, true>(dx, dx.carry ? dx.partial : workspace, workspace_bytes, stream)) return rc;
+            if (int rc = launch_product<T, false, true>(dx, dx.carry ? dx.partial : workspace, workspace_bytes, stream, together)) return rc;
         const bool brief = together && dw.out && launch_short<T>(dw, stream);
         TCBNN_LAUNCH_CHECK("short_product_kernel");
         if (dw.out && !brief)
-            if (int rc = launch_product<T, true, true>(dw, workspace, workspace_bytes, stream)) return rc;
+            if (int rc = launch_product<T, true, true>(dw, workspace, workspace_bytes, stream, together)) return rc;
         return TCBNN_OK;
     });
 }

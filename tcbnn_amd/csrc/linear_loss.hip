@@ -479,7 +479,7 @@ inline int packed_classes(int classes, int in_features, int size) {
 // The splits of dx's sum over a whole piece, where there are several.  Where the weights lie is not known when a workspace is asked for: the splits are
 // those of rows at whole 16 bytes, which are no fewer.
 inline int carried_splits(int rows, int in_features, int piece, int size) {
-    const int splits = plan_product(rows, in_features, piece, size, true, ~(size_t)0).splits;
+    const int splits = plan_product(rows, in_features, piece, size, true, ~(size_t)0, CUT_256, true).splits;
     const int steps = (int)(((long long)piece * size + kStepBytes - 1) / kStepBytes), each = (steps + splits - 1) / splits;
     return (steps + each - 1) / each;  // (as cut_product cuts a whole piece: every part is written by the first)
 }
@@ -546,7 +546,7 @@ inline LossWorkspace loss_workspace(int rows, int in_features, int classes, int 
     w.dx = w.sums + whole_lines((size_t)((rows + 31) / 32) * w.piece * sizeof(float));
     w.split = w.dx + (carried ? whole_lines((size_t)w.splits * rows * in_features * sizeof(float)) : 0);
     w.total = w.split + std::max(gradient_product_bytes(rows, in_features, planes > 1 ? plane_of(w.piece, size) + w.piece : w.piece, dtype, true),
-                                 gradient_product_bytes(planes > 1 ? plane_of(rows, size) + rows : rows, in_features, w.piece, dtype));
+                                 gradient_product_bytes(planes > 1 ? plane_of(rows, size) + rows : rows, in_features, w.piece, dtype, true));
     return w;
 }
 

@@ -733,10 +733,11 @@ struct Plan {
     int splits;
     float time;
 };
-// `pairs`: a compute unit has two workgroups at a time of all tiles but the two that take its shared memory, so that of an odd number of them the last
-// one works alone (losses, bf16: 300 x 4096 -> 32000 classes 135 us in tiles of 128, three a compute unit, 105 in tiles of 256; 333 x 1024 -> 32000 39
-// and 33; 2000 x 512 -> 5000 23.0 and 21.0).
-inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, size_t workspace_bytes, Cut largest = CUT_256, bool pairs = false) {
+// `fine`, for what the linear layer does not launch: a compute unit has two workgroups at a time of all tiles but the two that take its shared memory, so that
+// of an odd number of them the last one works alone (losses, bf16: 300 x 4096 -> 32000 classes 135 us in tiles of 128, three a compute unit, 105 in
+// tiles of 256; 333 x 1024 -> 32000 39 and 33; 2000 x 512 -> 5000 23.0 and 21.0); and a sum may be split into any number of parts (loss's
+// step of 3630 x 1072 -> 38878 bf16 1445 us, 1580 with powers of two; gradients of gated 1500 x 2048 -> 2 x 5600 205 and 224).
+inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, size_t workspace_bytes, Cut largest = CUT_256, bool fine = false) {
     const int steps = (int)(((long long)sum * size + kStepBytes - 1) / kStepBytes);
     const float read = ((float)rows + (float)cols) * (float)sum * (float)size / kReadRate;
     Plan best = {CUT_32, 1, 0.0f};
@@ -745,11 +746,11 @@ inline Plan plan_product(int rows, int cols, int sum, int size, bool vectors, si
         if (cost.size == 0) continue;
         if (!vectors && size == 4) cost.step = std::max(cost.step, kCuts32[c].step), cost.more = std::max(cost.more, kCuts32[c].more);
         const float tiles = (float)((rows + cost.size - 1) / cost.size) * (float)((cols + cost.size - 1) / cost.size);
-        for (int k = 1; k <= kMaxSplits && (k == 1 || steps >= 4 * k); k *= 2) {
+        for (int k = 1; k <= kMaxSplits && (k == 1 || steps >= 4 * k); k = fine ? k + 1 : 2 * k) {
             const size_t partial = k > 1 ? (size_t)k * rows * cols * sizeof(float) : 0;
             if (partial > workspace_bytes) break;
             const float rounds = std::ceil(tiles * (float)k / (float)kComputeUnits);
-            const bool alone = pairs && rounds > 1.0f && std::fmod(rounds, 2.0f) == 1.0f && c != CUT_256 && c != CUT_128_DEEP;
+            const bool alone = fine && rounds > 1.0f && std::fmod(rounds, 2.0f) == 1.0f && c != CUT_256 && c != CUT_128_DEEP;
             const float each = std::max(cost.step, rounds * cost.more) + (alone ? std::max(0.0f, cost.step - cost.more) : 0.0f);
             const float time = cost.start + (rounds - 1.0f) * cost.tile + std::max((float)((steps + k - 1) / k) * each, read) + (k > 1 ? (vectors ? 2.3f : 3.0f) + (float)partial * 2.0f / 4.0e6f : 0.0f);
             if (best.time == 0.0f || time < best.time) best = {(Cut)c, k, time};
