@@ -680,6 +680,7 @@ int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream);
  * grad_bias = sums of d over the rows.  Each of the three may be NULL; what is given is overwritten.  The logits are made again, a piece
  * of the classes at a time; in 16-bit types d is rounded to dtype before the two products (in f16 times a power of two that keeps small
  * ones from getting lost); grad_bias sums it unrounded.  `logsumexp` is the forward call's; exp carries its rounding and one more like it, |logsumexp| 2^-23.
+ * With the forward call's `loss` the given class' d is grad_loss * (exp(-loss) - 1) instead, which is good where the class is nearly certain.
  * A row without a class still has to hold finite inputs: grad_weight sums 0 times them.  `workspace` holds
  * tcbnn_linear_loss_grad_workspace_bytes, `anywhere` as in the forward call. */
 typedef struct tcbnn_linear_loss_grad_desc {
@@ -688,6 +689,7 @@ typedef struct tcbnn_linear_loss_grad_desc {
     const float* bias;       /* [classes], or NULL       */
     const int32_t* targets;  /* [rows]                   */
     const float* logsumexp;  /* [rows]                   */
+    const float* loss;       /* [rows], or NULL          */
     const float* grad_loss;  /* [rows]                   */
     void* grad_input;        /* [rows][in_features]      */
     void* grad_weight;       /* [classes][in_features]   */

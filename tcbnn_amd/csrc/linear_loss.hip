@@ -25,6 +25,7 @@ struct LossParams {
 struct LossGradParams {
     const int32_t* targets;
     const float *lse, *dloss, *scale;  // (scale: of d in f16)
+    const float* loss;                 // [rows], or NULL
     float* sums;                       // [tiles of i][cols], or NULL
     int first, classes;                // the piece's first class
     long long low;                     // elements from d to what its rounding left of it, or 0
@@ -230,6 +231,13 @@ __global__ __launch_bounds__(kScaleThreads) void loss_scale_kernel(const float* 
     }
 }
 
+// exp(-loss) - 1: what the given class' p - 1 is, good where p is near 1 too
+__device__ __forceinline__ float given_d(float loss) {
+    const float x = -loss;
+    const float near = x * __builtin_fmaf(x, __builtin_fmaf(x, __builtin_fmaf(x, __builtin_fmaf(x, __builtin_fmaf(x, 1.0f / 720, 1.0f / 120), 1.0f / 24), 1.0f / 6), 0.5f), 1.0f);
+    return x > -0.25f ? near : exp_fast(x) - 1.0f;
+}
+
 // the sum over the 32 lanes of a half, in the lanes whose number ends in 0
 __device__ __forceinline__ float half_sum(float v) {
     v += __uint_as_float(dpp<kSwapPairs>(__float_as_uint(v)));
@@ -284,11 +292,12 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) __attribute__((amdgpu_waves_per_
             }
             const long long at = (long long)t - l.first - j0 - 4 * (lane >> 5);
             if (__any(!none && at >= 0 && at < 32 * NJ)) {
+                const float given = l.loss ? g * given_d(l.loss[row]) : 0.0f;
 #pragma unroll
                 for (int b = 0; b < NJ; ++b)
 #pragma unroll
                     for (int v = 0; v < 16; ++v)
-                        if (!none && at == 32 * b + 8 * (v / 4) + v % 4) acc[a][b][v] -= g;
+                        if (!none && at == 32 * b + 8 * (v / 4) + v % 4) acc[a][b][v] = l.loss ? given : acc[a][b][v] - g;
             }
         }
     }
@@ -382,13 +391,14 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
     const long long j = j0 + 4 * (lane >> 4);
     const float lse = l.lse[row], c = lse * kLog2e, g = t < l.classes ? l.dloss[row] : NAN;
     const bool none = i >= p.rows || t < 0 || lse == -INFINITY;
+    const float given = l.loss ? g * given_d(l.loss[row]) : 0.0f;
     float d[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const bool there = j + e < p.cols;
         const float z = acc[e] + (p.bias && there ? p.bias[j + e] : 0.0f);
         d[e] = g * (fabsf(lse) > kFarLogit ? exp_fast(z - lse) : __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -c)));
-        d[e] = none || !there ? 0.0f : l.first + j + e == t ? d[e] - g : d[e];
+        d[e] = none || !there ? 0.0f : l.first + j + e == t ? (l.loss ? given : d[e] - g) : d[e];
         if (l.sums) {
             float s = d[e];
             s += __uint_as_float(dpp<kSwapPairs>(__float_as_uint(s)));
@@ -710,7 +720,7 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             p.sum = d->in_features;
             p.bias = d->bias;
             p.out = base;
-            launch_grad_few_rows<T, true>(p, {d->targets, d->logsumexp, d->grad_loss, nullptr, d->grad_bias, 0, d->classes, 0}, s);
+            launch_grad_few_rows<T, true>(p, {d->targets, d->logsumexp, d->grad_loss, nullptr, d->loss, d->grad_bias, 0, d->classes, 0}, s);
         });
         TCBNN_LAUNCH_CHECK("loss_grad_few_rows_kernel");
         return launch_few_gradients(d->dtype, (float*)base, d->rows, d->in_features, d->classes, {d->weight, w_ld}, {d->input, x_ld}, d->grad_input, dx_ld,
@@ -742,7 +752,7 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             p.bias = d->bias ? d->bias + first : nullptr;
             p.out = base + w.d;
             p.out_ld = d_ld;
-            LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes, low};
+            LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->loss, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes, low};
             const Access access = access_of<T, false, false>(p);
             const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0, CUT_256, true);
             const bool few = p.rows <= kFewRows && (access == ELEMENTS || few_time(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES) < plan.time);
@@ -763,6 +773,7 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
                     part.targets += row;
                     part.lse += row;
                     part.dloss += row;
+                    if (part.loss) part.loss += row;
                     if (part.sums) part.sums += row / B * p.cols;
                     cut_product(q, B, kStepBytes / (int)sizeof(T), 1, nullptr);
                     hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_grad_product_kernel<T, B, B, wi.value, wj.value, ws.value, stages.value, how.value, hold.value, keep.value>),

@@ -487,7 +487,7 @@ class LinearLossLayerParam(_HeadLayer):
 
     def initialize_backward(self, grad_loss_gpu, grad_input_gpu=None, grad_weight_gpu=None, grad_bias_gpu=None):
         """After initialize().  grad_loss: fp32 [rows] (1 / n for the mean of n rows).  Gradients are written where a buffer is
-        given; logsumexp is that of forward()."""
+        given; loss and logsumexp are those of forward()."""
         m, k, n, dt = self.rows, self.in_features, self.classes, self.dtype
         self.grad_loss_gpu = self._sized(self._required(grad_loss_gpu, "grad_loss"), "grad_loss", (m,), "f32")
         self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", (m, k), dt)
@@ -497,7 +497,7 @@ class LinearLossLayerParam(_HeadLayer):
         ws = self._grad_buffer(nbytes)
         self._grad_desc = _lib.LinearLossGradDesc(
             self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), self.targets_gpu.ptr, self.logsumexp_gpu.ptr,
-            self.grad_loss_gpu.ptr, _ptr(grad_input_gpu), _ptr(grad_weight_gpu), _ptr(grad_bias_gpu), m, k, n, _lib.DTYPES[dt],
+            self.loss_gpu.ptr, self.grad_loss_gpu.ptr, _ptr(grad_input_gpu), _ptr(grad_weight_gpu), _ptr(grad_bias_gpu), m, k, n, _lib.DTYPES[dt],
             _ld(self.input_gpu), _ld(self.weight_gpu), _ld(grad_input_gpu), _ld(grad_weight_gpu), _ptr(ws), nbytes)
         self._backward = self._call(lib.tcbnn_linear_loss_backward, self._grad_desc)
         return self

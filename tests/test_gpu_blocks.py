@@ -551,6 +551,40 @@ def test_loss_of_rows_far_from_0(gpu, m, k, n):
             layer.release()
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 24, 14), (4, 64, 300), (12, 64, 40), (70, 64, 500), (2048, 64, 4096)])
+def test_loss_gradient_of_a_nearly_certain_class(gpu, m, k, n):
+    """p - 1 of a given class whose p is about 1 - e^-7: with the loss it carries that one's error, without it logsumexp's."""
+    import ctypes as C
+    from tcbnn_amd import _lib, head
+    r = rng(m, k, n)
+    t = np.full(m, n // 3, np.int32)
+    # two inputs of whole sixteenths: logits are exact in fp32
+    wv, xv = np.zeros((n, k)), np.zeros((m, k))
+    wv[:, 0], xv[:, 0] = r.integers(0, 16, n) / 16.0, 1.0
+    wv[t, 1], xv[:, 1] = 1.0, np.round(16 * (8 + np.log(n))) / 16
+    x, w = ho.Matrix(xv, "f32", shift=0), ho.Matrix(wv, "f32", shift=0)
+    z = x.values @ w.values.T
+    given = np.arange(n)[None, :] == t[:, None]
+    e = np.exp(z - z.max(1, keepdims=True))
+    d = e / e.sum(1, keepdims=True)
+    d[given] = -np.where(given, 0.0, e).sum(1) / e.sum(1)
+    lse = np.log(e.sum(1, keepdims=True)) + z.max(1, keepdims=True)
+    layer = head.LinearLossLayerParam("loss", m, k, n, "f32").initialize(w.view, None, x.view, ho.vector(t, np.int32))
+    for with_loss in (True, False):
+        db = ho.empty(n)
+        layer.initialize_backward(ho.vector(np.ones(m)), None, None, db)
+        layer.forward()
+        desc = layer._grad_desc
+        desc.loss = desc.loss if with_loss else None
+        _lib.check(_lib.lib.tcbnn_linear_loss_backward(C.byref(desc), None))
+        ho.sync()
+        # of the other classes: logsumexp's rounding and one like it, exp's argument and some units; of the given one: the loss is the logarithm of a
+        # sum a little above 1, to which at most 128 roundings of its size go on the way
+        units = np.where(given, 128 + (0 if with_loss else 4 * lse + 16), np.abs(d) * (160 + 4 * lse + 4 * np.abs(z - lse)))
+        ho.check(db.to_numpy(np.float32, (n,)), d.sum(0), ho.U32 * (units.sum(0) + (m + 4) * np.abs(d).sum(0)), "with the loss" if with_loss else "without")
+    layer.release()
+
+
 def test_loss_of_degenerate_rows(gpu):
     """Every class forbidden; a forbidden class given; a class that there is not; a NaN and an infinite logit; rows without a class."""
     from tcbnn_amd import head
