@@ -7,7 +7,7 @@
 // there through two products.  dx is summed over the pieces in fp32.  With pieces of kPieceBytes that are read back from the cache, four products
 // (8 rows classes inputs operations a step) are nearly all of the time: 8192 x 1024 -> 131072 bf16 7.9 ms, z 1.84 (1.20 PFLOP/s), d 2.33, dx 1.91, dw
 // 1.86.  Single rows are bound by the weights' bytes, 1 x 4096 -> 131072 173 us (6.2 TB/s); small steps by their launches one after
-// the other, 256 x 512 -> 1000 fp32 36 us; weights' gradients of few rows by what they write, 333 x 1000 -> 32003 f16 47 us of the step's 178.
+// the other, 256 x 512 -> 1000 fp32 36 us; weights' gradients of few rows by what they write, 333 x 1000 -> 32003 f16 42 us of the step's 173.
 #include "product.h"
 
 namespace tcbnn {
