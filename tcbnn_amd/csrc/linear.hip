@@ -425,9 +425,10 @@ void launch_join(const ProductParams& p, hipStream_t stream) {
     }
 }
 
-// ---- dx of few rows: tiles of 32, 64 or 128 rows (78 x 2488 -> 43155 classes, the loss's step 298 us, 313 in tiles of 128) by 256 columns, so that a row of the weights is read in runs of 512 bytes, and a sum that all compute units share
-// (16 x 131072 classes -> 4096 bf16, both planes: 176 us, 6.1 TB/s of the weights, 467 in tiles of 32; small products are faster in small tiles: the gradients
-// of 64 x 512 -> 2000 classes 29 us, 32 with wide ones, which the estimates below tell apart).
+// ---- dx of few rows: tiles of 32, 64 or 128 rows by 256 columns, so that a row of the weights is read in runs of 512 bytes, and a sum that all compute
+// units share (16 x 131072 classes -> 4096 bf16, both planes: 176 us, 6.1 TB/s of the weights, 467 in tiles of 32; the loss's step of 78 x 2488 -> 43155
+// classes 298 us, 313 in tiles of 128; small products are faster in small tiles: the gradients of 64 x 512 -> 2000 classes 29 us, 32 with
+// wide ones, which the estimates below tell apart).
 template <typename T, int BI, int STAGES, bool PLANES>
 __global__ __launch_bounds__(256) void wide_product_kernel(const ProductParams p) {
     __shared__ __align__(1024) char lds[product_lds<BI, 256, 1, 4, 1, STAGES>()];

@@ -904,7 +904,7 @@ Operand launch_pack(int dtype, const Operand& o, long long rows, int n, void* to
 // ---- (linear.hip)  dx = d w and dw = d^T x, each where it has an `out`; with dx.carry its sum stays in its `partial`, whose number of splits is
 // dx.splits.  The workspace is for split sums (gradient_product_bytes; without one none is split).
 size_t gradient_product_bytes(int rows, int in_features, int out_features, int dtype, bool together = false);
-// `together`: both in one launch of large tiles, and wide tiles for few rows, too, where these are estimated to take less time.
+// `together`: both in one launch of large tiles, wide tiles for few rows, tiles for short sums and fine plans, too, where these take less time.
 int launch_gradient_products(int dtype, const ProductParams& dx, const ProductParams& dw, float* workspace, size_t workspace_bytes, hipStream_t stream,
                              bool together = false);
 // ---- (few_gradients.hip)  the same for kFewGradientRows rows at most and d in fp32, [outs][kFewGradientRows] with zeros behind the last row; `partial` holds few_gradients_bytes
