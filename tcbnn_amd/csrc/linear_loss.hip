@@ -32,7 +32,11 @@ struct LossGradParams {
 };
 
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
-// Past it a finite logit times log2 e has no place in fp32, as a mask of the type's lowest value has none: exponents of such rows are taken of the difference.
+// Up to it exponents of a row are taken about m log2 e, rounded: one fused multiply-add a logit, and what the rounding was (2^-8 at most) scales the
+// sum back.  Beyond, that would be any number of powers of two, inf or 0 from 2^31 on, and nothing at all where m log2 e has no place in fp32 (a mask of the
+// type's lowest value): there logits' differences to m are taken first, which are exact beside m.
+constexpr float kNear = 65536.0f;
+// the gradient's
 constexpr float kFarLogit = 0x1p126f;
 // exp(m - to) s: what a sum of exponentials about m is about `to`, m <= to
 __device__ __forceinline__ float about(float m, float s, float to) { return m == to ? s : s * exp_fast(m - to); }
@@ -91,21 +95,20 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) __attribute__((amdgpu_waves_per_
 #pragma unroll
                 for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[a][b][v]);
             m = across_halves(m, larger);
-            // (one fused multiply-add a logit: exponents about m log2 e as it is rounded, and the sum scaled back by what that rounding was)
             const float base = m == -INFINITY ? 0.0f : m, c = base * kLog2e;
 #pragma unroll
             for (int b = 0; b < NJ; ++b)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][v], kLog2e, -c));
             s = across_halves(s, add) * __builtin_amdgcn_exp2f(-__builtin_fmaf(base, kLog2e, -c));
-            if (__any(fabsf(base) > kFarLogit)) {
+            if (__any(fabsf(base) > kNear)) {
                 float far = 0.0f;
 #pragma unroll
                 for (int b = 0; b < NJ; ++b)
 #pragma unroll
                     for (int v = 0; v < 16; ++v) far += exp_fast(acc[a][b][v] - base);
                 far = across_halves(far, add);
-                s = fabsf(base) > kFarLogit ? far : s;
+                s = fabsf(base) > kNear ? far : s;
             }
             if (spot.lane < 32) rows[spot.wj / (32 * NJ) * BI + row] = make_float2(m, s);
             const long long i = spot.i0 + row;

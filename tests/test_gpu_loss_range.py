@@ -1,0 +1,76 @@
+"""The linear loss where logits are far from 0: finite masks of every size over whole tiles and over a wavefront's columns, and rows all of whose
+logits are there.  Inputs are whole numbers, so that logits are known to the bit."""
+import numpy as np
+import pytest
+
+from tests import headops as ho
+from tests.test_gpu_blocks import _loss, rng
+
+pytestmark = pytest.mark.gpu
+
+MASKS = [-1e5, -1e9, -1e10, -1e20, -1e30, -8e37]
+# few rows, one row that takes tiles, and every tile: 32, 64, 128, 128 deep, 128 with one step in LDS, 256; rows that lie anywhere
+SIZES = [(1, 64, 200, 0), (1, 2048, 8192, 0), (12, 40, 700, 1), (33, 72, 300, 0), (100, 61, 304, 1), (1024, 72, 1500, 0), (1000, 71, 1500, 1), (2040, 72, 2052, 0),
+         (2040, 72, 2052, 1), (2048, 64, 2048, 0), (2048, 64, 3100, 0)]
+
+
+def _masked(gpu, m, k, n, dtype, shift, mask, want=()):
+    allowed = n - n // 2
+    t = rng(m, n).integers(-1, allowed, m).astype(np.int32)
+    _loss(gpu, m, k, n, dtype, shift=shift, forbidden=np.arange(allowed, n), t=t, mask=mask, want=want)
+    # one wavefront's 32 or 64 columns, with classes on both sides
+    first = n // 2 // 64 * 64
+    t[t >= first] -= first
+    _loss(gpu, m, k, n, dtype, shift=shift, forbidden=np.arange(first, min(n, first + 64)), t=t, mask=mask, want=want)
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n,shift", SIZES)
+def test_loss_of_classes_masked_by_any_value(gpu, m, k, n, shift, dtype):
+    for mask in MASKS if m * n < 1 << 20 else [-1e10, -1e30]:
+        _masked(gpu, m, k, n, dtype, shift, mask)
+    _masked(gpu, m, k, n, dtype, shift, -1e20, ("input", "weight", "bias"))
+
+
+@pytest.mark.parametrize("m,k,n,dtype", [(1500, 520, 6000, "bf16"), (4096, 256, 4096, "f32")])
+def test_loss_of_masked_classes_in_the_largest_tiles(gpu, m, k, n, dtype):
+    _masked(gpu, m, k, n, dtype, 0, -1e10)
+
+
+def _whole(r, rows, k, dtype, shift):
+    """A matrix of -1, 0 and 1, of which any product is exact."""
+    return ho.Matrix(r.integers(-1, 2, (rows, k)).astype(np.float64), dtype, shift=shift)
+
+
+def _logits(x, w, b):
+    """As fp32 holds them: the products are whole numbers, the bias is added once."""
+    return ((x.values @ w.values.T).astype(np.float32) + b[None, :]).astype(np.float64)
+
+
+# what all logits of a row are about
+FAR = [3e4, -3e4, 1e6, -1e6, 1e9, -1e9, 1e10, -1e10, 1e12, 1e20, -1e20, -1e30, 1e37, -8e37]
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n,shift", SIZES)
+def test_loss_of_rows_all_far_from_0(gpu, m, k, n, shift, dtype):
+    from tcbnn_amd import head
+    r = rng(m, k, n)
+    x, w = _whole(r, m, k, dtype, shift), _whole(r, n, k, dtype, shift)
+    t = r.integers(0, n, m).astype(np.int32)
+    for value in FAR if m * n < 1 << 20 else FAR[::3]:
+        b = np.full(n, value, np.float32)
+        layer = head.LinearLossLayerParam("loss", m, k, n, dtype).initialize(w.view, b, x.view, ho.vector(t, np.int32))
+        layer.forward()
+        ho.sync()
+        z = _logits(x, w, b)
+        top = z.max(1, keepdims=True)
+        e = np.exp(z - top)
+        s = e.sum(1)
+        lse, loss = top[:, 0] + np.log(s), top[:, 0] - z[np.arange(m), t] + np.log(s)
+        # exp's argument, exp by some units and the sum of n; the logarithm of it, and one rounding of each difference
+        err = (e / s[:, None] * (4 * (top - z) + 6)).sum(1) + n + 8 + 4 * np.log(n + 1.0)
+        got = layer.download_output()
+        ho.check(got["logsumexp"], lse, 1.1 * ho.U32 * (err + 2 * np.abs(lse)), "logsumexp at %g" % value)
+        ho.check(got["loss"], loss, 1.1 * ho.U32 * (err + 4 * np.abs(loss)), "loss at %g" % value)
+        layer.release()
