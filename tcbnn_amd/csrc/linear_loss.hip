@@ -36,8 +36,6 @@ __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp
 // sum back.  Beyond, that would be any number of powers of two, inf or 0 from 2^31 on, and nothing at all where m log2 e has no place in fp32 (a mask of the
 // type's lowest value): there logits' differences to m are taken first, which are exact beside m.
 constexpr float kNear = 65536.0f;
-// the gradient's
-constexpr float kFarLogit = 0x1p126f;
 // exp(m - to) s: what a sum of exponentials about m is about `to`, m <= to
 __device__ __forceinline__ float about(float m, float s, float to) { return m == to ? s : s * exp_fast(m - to); }
 // f(v, v of the lane 32 away)
@@ -273,10 +271,10 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) __attribute__((amdgpu_waves_per_
             const float lse = l.lse[row];
             const bool none = i >= p.rows || t < 0 || lse == -INFINITY;
             const float g = t < l.classes ? l.dloss[row] : NAN;
-            // (about logsumexp log2 e as it is rounded: no more than logsumexp's own rounding)
+            // (about logsumexp log2 e as it is rounded: up to kNear no more than logsumexp's own rounding, and differences beyond)
             const float c = lse * kLog2e;
-            if (__any(fabsf(lse) > kFarLogit)) {
-                const bool far = fabsf(lse) > kFarLogit;
+            if (__any(fabsf(lse) > kNear)) {
+                const bool far = fabsf(lse) > kNear;
 #pragma unroll
                 for (int b = 0; b < NJ; ++b)
 #pragma unroll
@@ -400,7 +398,7 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
     for (int e = 0; e < 4; ++e) {
         const bool there = j + e < p.cols;
         const float z = acc[e] + (p.bias && there ? p.bias[j + e] : 0.0f);
-        d[e] = g * (fabsf(lse) > kFarLogit ? exp_fast(z - lse) : __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -c)));
+        d[e] = g * (fabsf(lse) > kNear ? exp_fast(z - lse) : __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -c)));
         d[e] = none || !there ? 0.0f : l.first + j + e == t ? (l.loss ? given : d[e] - g) : d[e];
         if (l.sums) {
             float s = d[e];

@@ -3,6 +3,7 @@ logits are there.  Inputs are whole numbers, so that logits are known to the bit
 import numpy as np
 import pytest
 
+from tests import blockops as bo
 from tests import headops as ho
 from tests.test_gpu_blocks import _loss, rng
 
@@ -73,4 +74,40 @@ def test_loss_of_rows_all_far_from_0(gpu, m, k, n, shift, dtype):
         got = layer.download_output()
         ho.check(got["logsumexp"], lse, 1.1 * ho.U32 * (err + 2 * np.abs(lse)), "logsumexp at %g" % value)
         ho.check(got["loss"], loss, 1.1 * ho.U32 * (err + 4 * np.abs(loss)), "loss at %g" % value)
+        layer.release()
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n,shift", [(1, 64, 200, 0), (3, 24, 70, 1), (12, 40, 700, 1), (40, 72, 300, 0), (300, 61, 304, 1), (1024, 72, 1500, 0), (2040, 72, 2052, 0),
+                                         (2048, 64, 3100, 0)])
+def test_loss_gradient_of_a_certain_class_far_from_0(gpu, m, k, n, shift, dtype):
+    """One class of every row is alone at `value`: its p is 1, the others' 0, whatever logsumexp's size."""
+    from tcbnn_amd import head
+    r = rng(m, k, n)
+    x, w = _whole(r, m, k, dtype, shift), _whole(r, n, k, dtype, shift)
+    t = r.integers(-1, n, m).astype(np.int32)
+    t[0], best = n - 1, n // 3
+    if m > 2:
+        t[2] = best
+    g = (0.5 + r.random(m)).astype(np.float32)
+    for value in [1e5, -1e5, 3e9, -3e9, 1e10, -1e10, 1e12, -1e12, 1e20, -1e30, 1e37, -8e37]:
+        b = np.full(n, 0.0 if value > 0 else 4 * value, np.float32)
+        b[best] = value
+        dx, dw, db = ho.Matrix(None, dtype, 0, m, k, shift=0), ho.Matrix(None, dtype, 0, n, k, shift=0), ho.empty(n)
+        layer = head.LinearLossLayerParam("loss", m, k, n, dtype).initialize(w.view, b, x.view, ho.vector(t, np.int32))
+        layer.initialize_backward(ho.vector(g), dx.view, dw.view, db)
+        layer.forward()
+        layer.backward()
+        ho.sync()
+        z = _logits(x, w, b)
+        p = np.zeros((m, n))
+        p[:, best] = 1.0
+        # (p is that of logits about logsumexp: exp's argument is 0, and off by less than 65536 2^-23 where it is that of a rounded product)
+        near = np.where(np.abs(z[:, best]) > 65536.0, 0.0, ho.U32 * 2 * 65536)
+        exact = bo.loss_grads(x.values, w.values, t, g.astype(np.float64), z - z[:, best:best + 1], 0.0, p, np.zeros(m), near, dtype)
+        for name, buf in (("input", dx), ("weight", dw)):
+            e, err = exact[name]
+            ho.check(buf.get(), e, bo.out_error(e, err, dtype), "grad of %s at %g" % (name, value))
+        e, err = exact["bias"]
+        ho.check(db.to_numpy(np.float32, (n,)), e, 1.1 * err + ho.TINY["f32"], "grad of bias at %g" % value)
         layer.release()
