@@ -671,6 +671,7 @@ typedef struct tcbnn_linear_loss_desc {
     long long input_ld, weight_ld;
     void* workspace;
     size_t workspace_bytes;
+    float* logsumexp_rest;   /* [rows], or NULL: what rounding to fp32 left of logsumexp */
 } tcbnn_linear_loss_desc;
 size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, int classes, int dtype, int anywhere);
 int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream);
@@ -679,8 +680,9 @@ int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream);
  * a class and in rows whose classes are all forbidden (t >= classes: NaN):  grad_input = d * weight, grad_weight = d^T * input,
  * grad_bias = sums of d over the rows.  Each of the three may be NULL; what is given is overwritten.  The logits are made again, a piece
  * of the classes at a time; in 16-bit types d is rounded to dtype before the two products (in f16 times a power of two that keeps small
- * ones from getting lost); grad_bias sums it unrounded.  `logsumexp` is the forward call's; exp carries its rounding and one more like it, |logsumexp| 2^-23.
- * With the forward call's `loss` the given class' d is grad_loss * (exp(-loss) - 1) instead, which is good where the class is nearly certain.
+ * ones from getting lost); grad_bias sums it unrounded.  `logsumexp` and `logsumexp_rest` are the forward call's; without the rest exp carries logsumexp's
+ * rounding, a relative |logsumexp| 2^-24 (of rows whose logits are all far beyond 2^24 logsumexp is the largest one, and exp of it 1 however many
+ * classes have it).  With the forward call's `loss` the given class' d is grad_loss * (exp(-loss) - 1) instead, which is good where the class is nearly certain.
  * A row without a class still has to hold finite inputs: grad_weight sums 0 times them.  `workspace` holds
  * tcbnn_linear_loss_grad_workspace_bytes, `anywhere` as in the forward call. */
 typedef struct tcbnn_linear_loss_grad_desc {
@@ -699,6 +701,7 @@ typedef struct tcbnn_linear_loss_grad_desc {
     long long input_ld, weight_ld, grad_input_ld, grad_weight_ld;
     void* workspace;
     size_t workspace_bytes;
+    const float* logsumexp_rest; /* [rows], or NULL (0)  */
 } tcbnn_linear_loss_grad_desc;
 size_t tcbnn_linear_loss_grad_workspace_bytes(int rows, int in_features, int classes, int dtype, int anywhere);
 int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, void* stream);

@@ -158,7 +158,7 @@ class LinearLossDesc(C.Structure):
     _fields_ = [("input", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("targets", c_void_p),
                 ("loss", c_void_p), ("logsumexp", c_void_p), ("rows", c_int), ("in_features", c_int),
                 ("classes", c_int), ("dtype", c_int), ("input_ld", C.c_longlong), ("weight_ld", C.c_longlong),
-                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("logsumexp_rest", c_void_p)]
 
 
 class LinearLossGradDesc(C.Structure):
@@ -167,7 +167,7 @@ class LinearLossGradDesc(C.Structure):
                 ("grad_weight", c_void_p), ("grad_bias", c_void_p), ("rows", c_int), ("in_features", c_int),
                 ("classes", c_int), ("dtype", c_int), ("input_ld", C.c_longlong), ("weight_ld", C.c_longlong),
                 ("grad_input_ld", C.c_longlong), ("grad_weight_ld", C.c_longlong), ("workspace", c_void_p),
-                ("workspace_bytes", c_size_t)]
+                ("workspace_bytes", c_size_t), ("logsumexp_rest", c_void_p)]
 
 
 class LogProbsDesc(C.Structure):

@@ -25,7 +25,7 @@ struct LossParams {
 struct LossGradParams {
     const int32_t* targets;
     const float *lse, *dloss, *scale;  // (scale: of d in f16)
-    const float* loss;                 // [rows], or NULL
+    const float *loss, *rest;          // [rows] each, or NULL (rest: what fp32 left of lse)
     float* sums;                       // [tiles of i][cols], or NULL
     int first, classes;                // the piece's first class
     long long low;                     // elements from d to what its rounding left of it, or 0
@@ -163,11 +163,17 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
     if (lane < 16 && i < p.rows) l.parts[part * l.rows_there + i] = make_float2(m, s);
 }
 
+// a + b = (float)(a + b) + what this gives (Knuth's sum of two)
+__device__ __forceinline__ float rest_of_sum(float a, float b) {
+    const float sum = a + b, of_b = sum - a;
+    return (a - (sum - of_b)) + (b - of_b);
+}
+
 // A row's parts joined, always in the same order: R rows a workgroup side by side, 1024 / R threads to a row.
 constexpr int kLossJoinThreads = 1024;
 template <int R>
-__global__ __launch_bounds__(kLossJoinThreads) void loss_join_kernel(const LossParams l, float* __restrict__ loss, float* __restrict__ lse, int rows,
-                                                                     int classes, int parts) {
+__global__ __launch_bounds__(kLossJoinThreads) void loss_join_kernel(const LossParams l, float* __restrict__ loss, float* __restrict__ lse,
+                                                                     float* __restrict__ rest, int rows, int classes, int parts) {
     constexpr int kStep = kLossJoinThreads / R, kWaves = kLossJoinThreads / 64;
     static_assert(R == 1 || R == 32, "");
     __shared__ float2 lds[kWaves][R];
@@ -201,6 +207,10 @@ __global__ __launch_bounds__(kLossJoinThreads) void loss_join_kernel(const LossP
             const float log_s = logf(s);
             const bool none = m == -INFINITY && s == 0.0f;  // every class is forbidden
             if (lse) lse[row] = none ? -INFINITY : m + log_s;
+            if (rest) {
+                const float r = rest_of_sum(m, log_s);
+                rest[row] = fabsf(r) < INFINITY ? r : 0.0f;
+            }
             if (loss) {
                 const int t = l.targets[row];
                 loss[row] = t < 0 ? 0.0f : t >= classes ? NAN : none ? INFINITY : (m - l.given[row]) + log_s;
@@ -231,6 +241,18 @@ __global__ __launch_bounds__(kScaleThreads) void loss_scale_kernel(const float* 
         scale[1] = ldexpf(1.0f, -e);
     }
 }
+
+// exp(z - logsumexp) of a row's logits, logsumexp = lse + rest, as `factor` times near(z), or beyond(z) where lse is beyond kNear.  About c, lse log2 e as it is
+// rounded, it is one fused multiply-add a logit; the factor is what that rounding and the rest make of it.
+struct RowExp {
+    float lse, rest, c, factor;
+    bool far;
+    __device__ __forceinline__ RowExp(float lse, float rest) : lse(lse), rest(rest), c(lse * kLog2e), far(fabsf(lse) > kNear) {
+        factor = far ? 1.0f : __builtin_amdgcn_exp2f(-__builtin_fmaf(rest, kLog2e, __builtin_fmaf(lse, kLog2e, -c)));
+    }
+    __device__ __forceinline__ float near(float z) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -c)); }
+    __device__ __forceinline__ float beyond(float z) const { return exp_fast((z - lse) - rest); }
+};
 
 // exp(-loss) - 1: what the given class' p - 1 is, good where p is near 1 too
 __device__ __forceinline__ float given_d(float loss) {
@@ -271,19 +293,18 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) __attribute__((amdgpu_waves_per_
             const float lse = l.lse[row];
             const bool none = i >= p.rows || t < 0 || lse == -INFINITY;
             const float g = t < l.classes ? l.dloss[row] : NAN;
-            // (about logsumexp log2 e as it is rounded: up to kNear no more than logsumexp's own rounding, and differences beyond)
-            const float c = lse * kLog2e;
-            if (__any(fabsf(lse) > kNear)) {
-                const bool far = fabsf(lse) > kNear;
+            const RowExp e(lse, l.rest ? l.rest[row] : 0.0f);
+            const float gf = g * e.factor;
+            if (__any(e.far)) {
 #pragma unroll
                 for (int b = 0; b < NJ; ++b)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) acc[a][b][v] = g * (far ? exp_fast(acc[a][b][v] - lse) : __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][v], kLog2e, -c)));
+                    for (int v = 0; v < 16; ++v) acc[a][b][v] = gf * (e.far ? e.beyond(acc[a][b][v]) : e.near(acc[a][b][v]));
             } else {
 #pragma unroll
                 for (int b = 0; b < NJ; ++b)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) acc[a][b][v] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][v], kLog2e, -c));
+                    for (int v = 0; v < 16; ++v) acc[a][b][v] = gf * e.near(acc[a][b][v]);
             }
             if (__any(none)) {
 #pragma unroll
@@ -390,7 +411,8 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
     if (share != 0 || j0 >= p.cols) return;
     const int i = lane & 15, row = min(i, p.rows - 1), t = l.targets[row];
     const long long j = j0 + 4 * (lane >> 4);
-    const float lse = l.lse[row], c = lse * kLog2e, g = t < l.classes ? l.dloss[row] : NAN;
+    const float lse = l.lse[row], g = t < l.classes ? l.dloss[row] : NAN;
+    const RowExp of(lse, l.rest ? l.rest[row] : 0.0f);
     const bool none = i >= p.rows || t < 0 || lse == -INFINITY;
     const float given = l.loss ? g * given_d(l.loss[row]) : 0.0f;
     float d[4];
@@ -398,7 +420,7 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
     for (int e = 0; e < 4; ++e) {
         const bool there = j + e < p.cols;
         const float z = acc[e] + (p.bias && there ? p.bias[j + e] : 0.0f);
-        d[e] = g * (fabsf(lse) > kNear ? exp_fast(z - lse) : __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -c)));
+        d[e] = g * of.factor * (of.far ? of.beyond(z) : of.near(z));
         d[e] = none || !there ? 0.0f : l.first + j + e == t ? (l.loss ? given : d[e] - g) : d[e];
         if (l.sums) {
             float s = d[e];
@@ -600,7 +622,7 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
     p.j = {d->weight, row_stride(d->weight_ld, d->in_features)};
     TCBNN_REQUIRE(p.i.ld > 0 && p.j.ld > 0, "linear loss: rows overlap");
     TCBNN_REQUIRE(!too_far(p.i.ld, d->dtype) && !too_far(p.j.ld, d->dtype), "linear loss: rows too far apart");
-    if (d->rows == 0 || (!d->loss && !d->logsumexp)) return TCBNN_OK;
+    if (d->rows == 0 || (!d->loss && !d->logsumexp && !d->logsumexp_rest)) return TCBNN_OK;
     TCBNN_NOTNULL(d->input);
     TCBNN_NOTNULL(d->weight);
     if (d->loss) TCBNN_NOTNULL(d->targets);
@@ -664,10 +686,11 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
         }
         TCBNN_LAUNCH_CHECK("loss_product_kernel");
         if (p.rows <= kFewRows)
-            hipLaunchKernelGGL(loss_join_kernel<1>, dim3((unsigned)p.rows), dim3(kLossJoinThreads), 0, s, l, d->loss, d->logsumexp, p.rows, p.cols, plan.parts);
+            hipLaunchKernelGGL(loss_join_kernel<1>, dim3((unsigned)p.rows), dim3(kLossJoinThreads), 0, s, l, d->loss, d->logsumexp, d->logsumexp_rest, p.rows, p.cols,
+                               plan.parts);
         else
             hipLaunchKernelGGL(loss_join_kernel<32>, dim3((unsigned)std::min((p.rows + 31LL) / 32, kMaxThreads / kLossJoinThreads)), dim3(kLossJoinThreads), 0, s, l,
-                               d->loss, d->logsumexp, p.rows, p.cols, plan.parts);
+                               d->loss, d->logsumexp, d->logsumexp_rest, p.rows, p.cols, plan.parts);
         TCBNN_LAUNCH_CHECK("loss_join_kernel");
         return TCBNN_OK;
     });
@@ -721,7 +744,7 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             p.sum = d->in_features;
             p.bias = d->bias;
             p.out = base;
-            launch_grad_few_rows<T, true>(p, {d->targets, d->logsumexp, d->grad_loss, nullptr, d->loss, d->grad_bias, 0, d->classes, 0}, s);
+            launch_grad_few_rows<T, true>(p, {d->targets, d->logsumexp, d->grad_loss, nullptr, d->loss, d->logsumexp_rest, d->grad_bias, 0, d->classes, 0}, s);
         });
         TCBNN_LAUNCH_CHECK("loss_grad_few_rows_kernel");
         return launch_few_gradients(d->dtype, (float*)base, d->rows, d->in_features, d->classes, {d->weight, w_ld}, {d->input, x_ld}, d->grad_input, dx_ld,
@@ -753,7 +776,7 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
             p.bias = d->bias ? d->bias + first : nullptr;
             p.out = base + w.d;
             p.out_ld = d_ld;
-            LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->loss, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes, low};
+            LossGradParams l = {d->targets, d->logsumexp, d->grad_loss, scale, d->loss, d->logsumexp_rest, d->grad_bias ? (float*)(base + w.sums) : nullptr, first, d->classes, low};
             const Access access = access_of<T, false, false>(p);
             const Plan plan = plan_product(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES, 0, CUT_256, true);
             const bool few = p.rows <= kFewRows && (access == ELEMENTS || few_time(p.rows, p.cols, p.sum, (int)sizeof(T), access == WHOLE_PIECES) < plan.time);
@@ -775,6 +798,7 @@ extern "C" int tcbnn_linear_loss_backward(const tcbnn_linear_loss_grad_desc* d, 
                     part.lse += row;
                     part.dloss += row;
                     if (part.loss) part.loss += row;
+                    if (part.rest) part.rest += row;
                     if (part.sums) part.sums += row / B * p.cols;
                     cut_product(q, B, kStepBytes / (int)sizeof(T), 1, nullptr);
                     hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_grad_product_kernel<T, B, B, wi.value, wj.value, ws.value, stages.value, how.value, hold.value, keep.value>),

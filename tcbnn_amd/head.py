@@ -466,28 +466,30 @@ class LinearLossLayerParam(_HeadLayer):
         super().__init__(name, dtype)
         self.rows, self.in_features, self.classes = rows, in_features, classes
 
-    def initialize(self, weight, bias, input_gpu, targets_gpu, loss_gpu=None, logsumexp_gpu=None):
-        """targets: int32 [rows], -1 for rows without a class (loss 0, no gradient)."""
+    def initialize(self, weight, bias, input_gpu, targets_gpu, loss_gpu=None, logsumexp_gpu=None, logsumexp_rest_gpu=None):
+        """targets: int32 [rows], -1 for rows without a class (loss 0, no gradient).  logsumexp_rest: what rounding left of
+        logsumexp, for backward()."""
         self._forget()
         m, k, n, dt = self.rows, self.in_features, self.classes, self.dtype
         self.input_gpu = self._sized(self._required(input_gpu, "input"), "input", (m, k), dt)
         self.weight_gpu = self._sized(self._parameter(self._required(weight, "weight"), dt, (n, k)), "weight", (n, k), dt)
         self.bias_gpu = self._sized(self._parameter(bias, "f32", (n,)), "bias", (n,), "f32")
         self.targets_gpu = self._sized(self._required(targets_gpu, "targets"), "targets", (m,), "i32")
-        self.loss_gpu, self.logsumexp_gpu = (
+        self.loss_gpu, self.logsumexp_gpu, self.logsumexp_rest_gpu = (
             self._sized(buf if buf is not None else self._buffer(4 * m), what, (m,), "f32")
-            for buf, what in ((loss_gpu, "loss"), (logsumexp_gpu, "logsumexp")))
+            for buf, what in ((loss_gpu, "loss"), (logsumexp_gpu, "logsumexp"), (logsumexp_rest_gpu, "logsumexp_rest")))
         nbytes = lib.tcbnn_linear_loss_workspace_bytes(m, k, n, _lib.DTYPES[dt], _anywhere(dt, k, self.input_gpu, self.weight_gpu))
         ws = self._buffer(nbytes) if nbytes else None
         self._desc = _lib.LinearLossDesc(
             self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), self.targets_gpu.ptr, self.loss_gpu.ptr,
-            self.logsumexp_gpu.ptr, m, k, n, _lib.DTYPES[dt], _ld(self.input_gpu), _ld(self.weight_gpu), _ptr(ws), nbytes)
+            self.logsumexp_gpu.ptr, m, k, n, _lib.DTYPES[dt], _ld(self.input_gpu), _ld(self.weight_gpu), _ptr(ws), nbytes,
+            self.logsumexp_rest_gpu.ptr)
         self._forward = self._call(lib.tcbnn_linear_loss_forward, self._desc)
         return self
 
     def initialize_backward(self, grad_loss_gpu, grad_input_gpu=None, grad_weight_gpu=None, grad_bias_gpu=None):
         """After initialize().  grad_loss: fp32 [rows] (1 / n for the mean of n rows).  Gradients are written where a buffer is
-        given; loss and logsumexp are those of forward()."""
+        given; loss, logsumexp and its rest are those of forward()."""
         m, k, n, dt = self.rows, self.in_features, self.classes, self.dtype
         self.grad_loss_gpu = self._sized(self._required(grad_loss_gpu, "grad_loss"), "grad_loss", (m,), "f32")
         self.grad_input_gpu = self._sized(grad_input_gpu, "grad_input", (m, k), dt)
@@ -498,7 +500,8 @@ class LinearLossLayerParam(_HeadLayer):
         self._grad_desc = _lib.LinearLossGradDesc(
             self.input_gpu.ptr, self.weight_gpu.ptr, _ptr(self.bias_gpu), self.targets_gpu.ptr, self.logsumexp_gpu.ptr,
             self.loss_gpu.ptr, self.grad_loss_gpu.ptr, _ptr(grad_input_gpu), _ptr(grad_weight_gpu), _ptr(grad_bias_gpu), m, k, n, _lib.DTYPES[dt],
-            _ld(self.input_gpu), _ld(self.weight_gpu), _ld(grad_input_gpu), _ld(grad_weight_gpu), _ptr(ws), nbytes)
+            _ld(self.input_gpu), _ld(self.weight_gpu), _ld(grad_input_gpu), _ld(grad_weight_gpu), _ptr(ws), nbytes,
+            self.logsumexp_rest_gpu.ptr)
         self._backward = self._call(lib.tcbnn_linear_loss_backward, self._grad_desc)
         return self
 

@@ -111,3 +111,39 @@ def test_loss_gradient_of_a_certain_class_far_from_0(gpu, m, k, n, shift, dtype)
         e, err = exact["bias"]
         ho.check(db.to_numpy(np.float32, (n,)), e, 1.1 * err + ho.TINY["f32"], "grad of bias at %g" % value)
         layer.release()
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n,shift", [(1, 64, 200, 0), (3, 24, 70, 1), (12, 40, 700, 1), (40, 72, 300, 0), (300, 61, 304, 1), (1024, 72, 1500, 0), (2040, 72, 2052, 0),
+                                         (2048, 64, 3100, 0)])
+def test_loss_gradients_of_rows_all_far_from_0(gpu, m, k, n, shift, dtype):
+    """A row whose mask, or whose size, leaves no class near 0: classes share p as their differences say."""
+    from tcbnn_amd import head
+    r = rng(m, k, n, 2)
+    x, w = _whole(r, m, k, dtype, shift), _whole(r, n, k, dtype, shift)
+    t = r.integers(-1, n, m).astype(np.int32)
+    g = (0.5 + r.random(m)).astype(np.float32)
+    for value in [0.0, *FAR, np.finfo(np.float32).min] if m * n < 1 << 20 else [3e4, -1e6, 1e9, -1e30]:
+        b = np.full(n, value, np.float32)
+        dx, dw, db = ho.Matrix(None, dtype, 0, m, k, shift=0), ho.Matrix(None, dtype, 0, n, k, shift=0), ho.empty(n)
+        layer = head.LinearLossLayerParam("loss", m, k, n, dtype).initialize(w.view, b, x.view, ho.vector(t, np.int32))
+        layer.initialize_backward(ho.vector(g), dx.view, dw.view, db)
+        layer.forward()
+        layer.backward()
+        ho.sync()
+        z = _logits(x, w, b)
+        top = z.max(1, keepdims=True)
+        z = z - top
+        e = np.exp(z)
+        s = e.sum(1)
+        p, lse = e / s[:, None], np.log(s)
+        lse_err = 1.1 * ho.U32 * ((p * (4 * np.abs(z) + 6)).sum(1) + n + 8 + 4 * np.log(n + 1.0))
+        whole, rest = layer.logsumexp_gpu.to_numpy(np.float32, (m,)).astype(np.float64), layer.logsumexp_rest_gpu.to_numpy(np.float32, (m,))
+        ho.check(whole - top[:, 0] + rest, lse, lse_err + ho.U32 * np.abs(rest), "logsumexp and its rest at %g" % value)
+        exact = bo.loss_grads(x.values, w.values, t, g.astype(np.float64), z, 0.0, p, lse, lse_err, dtype)
+        for name, buf in (("input", dx), ("weight", dw)):
+            e, err = exact[name]
+            ho.check(buf.get(), e, bo.out_error(e, err, dtype), "grad of %s at %g" % (name, value))
+        e, err = exact["bias"]
+        ho.check(db.to_numpy(np.float32, (n,)), e, 1.1 * err + ho.TINY["f32"], "grad of bias at %g" % value)
+        layer.release()
