@@ -251,7 +251,11 @@ struct RowExp {
         factor = far ? 1.0f : __builtin_amdgcn_exp2f(-__builtin_fmaf(rest, kLog2e, __builtin_fmaf(lse, kLog2e, -c)));
     }
     __device__ __forceinline__ float near(float z) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -c)); }
-    __device__ __forceinline__ float beyond(float z) const { return exp_fast((z - lse) - rest); }
+    // (no more than 1: the logit is made again, perhaps in another order, and so far from 0 one unit of it may be any number of powers of e; NaN stays)
+    __device__ __forceinline__ float beyond(float z) const {
+        const float d = (z - lse) - rest;
+        return exp_fast(d > 0.0f ? 0.0f : d);
+    }
 };
 
 // exp(-loss) - 1: what the given class' p - 1 is, good where p is near 1 too

@@ -147,3 +147,31 @@ def test_loss_gradients_of_rows_all_far_from_0(gpu, m, k, n, shift, dtype):
         e, err = exact["bias"]
         ho.check(db.to_numpy(np.float32, (n,)), e, 1.1 * err + ho.TINY["f32"], "grad of bias at %g" % value)
         layer.release()
+
+
+# (one row of the first takes tiles forward and the kernel for few rows backward)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k,n", [(1, 2048, 8192), (4, 2048, 8192), (12, 4096, 640), (40, 2048, 300), (300, 1000, 777)])
+def test_loss_gradients_of_logits_that_are_known_to_no_unit(gpu, m, k, n, dtype):
+    """Sums so large that their rounding in another order is many units: p is still no more than 1."""
+    from tcbnn_amd import head
+    r = rng(m, k, n, 3)
+    x, w = (ho.Matrix(3e4 * r.standard_normal((rows, k)), dtype, shift=0) for rows in (m, n))
+    g = (0.5 + r.random(m)).astype(np.float32)
+    for sign in (1, -1):
+        dx, dw, db = ho.Matrix(None, dtype, 0, m, k, shift=0), ho.Matrix(None, dtype, 0, n, k, shift=0), ho.empty(n)
+        b = np.full(n, 4e11 * sign, np.float32)
+        layer = head.LinearLossLayerParam("loss", m, k, n, dtype).initialize(w.view, b, x.view, ho.vector(r.integers(-1, n, m), np.int32))
+        layer.initialize_backward(ho.vector(g), dx.view, dw.view, db)
+        layer.forward()
+        layer.backward()
+        ho.sync()
+        out = layer.download_output()
+        assert np.isfinite(out["loss"]).all() and np.isfinite(out["logsumexp"]).all()
+        # |d| is |g| at most, but for roundings of the loss' exponential and of the sums
+        limit = (1 + 2.0 ** -7) * g.sum()
+        assert (np.abs(db.to_numpy(np.float32, (n,))) <= limit).all()
+        assert (np.abs(dw.get()) <= limit * np.abs(x.values).max()).all()
+        # (a class that has the largest logit, and the given one)
+        assert np.isfinite(dx.get()).all()
+        layer.release()
