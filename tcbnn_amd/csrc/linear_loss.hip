@@ -604,18 +604,24 @@ bool too_far(long long ld, int dtype) { return ld * 256 * (long long)dtype_bytes
 using namespace tcbnn;
 using namespace tcbnn::head;
 
-extern "C" size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, int classes, int dtype, int anywhere) {
-    if (rows <= 0 || rows > kMaxRows || in_features <= 0 || in_features > kMaxIn || classes <= 0 || classes > kMaxOut || !dtype_known(dtype)) return 0;
+// what a forward call needs, with room for copies or without
+static size_t loss_forward_bytes(int rows, int in_features, int classes, int dtype, bool room) {
     const int size = (int)dtype_bytes(dtype);
     size_t parts = 0, copies = 0;
     for (bool x : {false, true})  // (which of the operands is not known here; parts are there for rows that lie anywhere in any case)
         for (bool w : {false, true}) {
-            const LossPlan l = plan_loss(rows, classes, in_features, size, in_features * size < 16 ? ELEMENTS : x || w ? ANYWHERE : WHOLE_PIECES, x, w, anywhere != 0);
+            const LossPlan l = plan_loss(rows, classes, in_features, size, in_features * size < 16 ? ELEMENTS : x || w ? ANYWHERE : WHOLE_PIECES, x, w, room);
             parts = std::max(parts, (size_t)l.parts);
             copies = std::max(copies, (l.pack_x ? packed_bytes(rows, in_features, size) : 0) +
                                           (l.pack_w ? packed_bytes(packed_classes(classes, in_features, size), in_features, size) : 0));
         }
     return copies + whole_lines(parts * rows * sizeof(float2)) + whole_lines((size_t)rows * sizeof(float));
+}
+extern "C" size_t tcbnn_linear_loss_workspace_bytes(int rows, int in_features, int classes, int dtype, int anywhere) {
+    if (rows <= 0 || rows > kMaxRows || in_features <= 0 || in_features > kMaxIn || classes <= 0 || classes > kMaxOut || !dtype_known(dtype)) return 0;
+    // (no less with room for copies: these are multiplied in wider tiles, which leave fewer parts, and every call asks for the size without)
+    const size_t without = loss_forward_bytes(rows, in_features, classes, dtype, false);
+    return anywhere ? std::max(without, loss_forward_bytes(rows, in_features, classes, dtype, true)) : without;
 }
 
 extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* stream) {
