@@ -109,7 +109,7 @@ constexpr int kFewPairs = kFewOutputs / 2;
 template <typename T, int SHARES>
 __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 4))) void gated_few_rows_kernel(const ProductParams p) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = wave % SHARES;
-    const long long j0 = ((long long)blockIdx.x * (kFewWaves / SHARES) + wave / SHARES) * kFewPairs;
+    const long long j0 = p.first + ((long long)blockIdx.x * (kFewWaves / SHARES) + wave / SHARES) * kFewPairs;
     // rows past the last one are read as the last one; nothing of them is kept
     const T* w = (const T*)p.j.p + (min(j0 + lane % kFewPairs, (long long)p.cols - 1) + (lane & kFewPairs ? p.cols : 0)) * p.j.ld;
     const T* x = (const T*)p.i.p + (long long)min(lane & 15, p.rows - 1) * p.i.ld;
@@ -290,12 +290,10 @@ int launch_gated(ProductParams p, int dtype, void* workspace, size_t workspace_b
     p.padded_i = g.pack_i;
     p.padded_j = g.pack_j;
     if (g.few) {
-        const int shares = few_shares(2 * p.cols, p.sum, (int)sizeof(T)), outputs = kFewPairs * kFewWaves / shares;
-        const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
-        if (shares == 8)
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_few_rows_kernel<T, 8>), grid, dim3(64 * kFewWaves), 0, stream, p);
-        else
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_few_rows_kernel<T, 2>), grid, dim3(64 * kFewWaves), 0, stream, p);
+        const int shares = few_shares(2 * p.cols, p.sum, (int)sizeof(T));
+        by_few_columns(p, shares, kFewPairs * kFewWaves / shares, [&](auto s, dim3 grid, const ProductParams& q) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_few_rows_kernel<T, s.value>), grid, dim3(64 * kFewWaves), 0, stream, q);
+        });
         TCBNN_LAUNCH_CHECK("gated_few_rows_kernel");
         return TCBNN_OK;
     }

@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
 template <typename T, int SHARES>
 __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 4))) void few_rows_kernel(const ProductParams p) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = wave % SHARES;
-    const int j0 = (blockIdx.x * (kFewWaves / SHARES) + wave / SHARES) * kFewOutputs;
+    const int j0 = p.first + (blockIdx.x * (kFewWaves / SHARES) + wave / SHARES) * kFewOutputs;
     // rows past the last one are read as the last one; nothing of them is kept
     const T* w = (const T*)p.j.p + (long long)min(j0 + (lane & 15), p.cols - 1) * p.j.ld;
     const T* x = (const T*)p.i.p + (long long)min(lane & 15, p.rows - 1) * p.i.ld;
@@ -540,12 +540,10 @@ int launch_product(ProductParams p, float* workspace, size_t workspace_bytes, hi
     if (p.carry) plan.splits = p.splits;
     if constexpr (!ACROSS_I && !ACROSS_J) {
         if (few_rows<T>(p, access, plan)) {
-            const int shares = few_shares(p.cols, p.sum, (int)sizeof(T)), outputs = kFewOutputs * kFewWaves / shares;
-            const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
-            if (shares == 8)
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, 8>), grid, dim3(64 * kFewWaves), 0, stream, p);
-            else
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, 2>), grid, dim3(64 * kFewWaves), 0, stream, p);
+            const int shares = few_shares(p.cols, p.sum, (int)sizeof(T));
+            by_few_columns(p, shares, kFewOutputs * kFewWaves / shares, [&](auto s, dim3 grid, const ProductParams& q) {
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, s.value>), grid, dim3(64 * kFewWaves), 0, stream, q);
+            });
             TCBNN_LAUNCH_CHECK("few_rows_kernel");
             return TCBNN_OK;
         }

@@ -139,7 +139,7 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) __attribute__((amdgpu_waves_per_
 template <typename T, int SHARES>
 __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 4))) void loss_few_rows_kernel(const ProductParams p, const LossParams l) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = wave % SHARES;
-    const long long part = (long long)blockIdx.x * (kFewWaves / SHARES) + wave / SHARES, j0 = part * kFewOutputs;
+    const long long part = p.first / kFewOutputs + (long long)blockIdx.x * (kFewWaves / SHARES) + wave / SHARES, j0 = part * kFewOutputs;
     // rows past the last one are read as the last one; nothing of them is kept
     const T* w = (const T*)p.j.p + min(j0 + (lane & 15), (long long)p.cols - 1) * p.j.ld;
     const T* x = (const T*)p.i.p + (long long)min(lane & 15, p.rows - 1) * p.i.ld;
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(64 * WI * WJ * WS) __attribute__((amdgpu_waves_per_
 template <typename T, int SHARES, bool FLOAT>
 __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 4))) void loss_grad_few_rows_kernel(const ProductParams p, const LossGradParams l) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = wave % SHARES;
-    const long long j0 = ((long long)blockIdx.x * (kFewWaves / SHARES) + wave / SHARES) * kFewOutputs;
+    const long long j0 = p.first + ((long long)blockIdx.x * (kFewWaves / SHARES) + wave / SHARES) * kFewOutputs;
     // rows past the last one are read as the last one; nothing of them is kept
     const T* w = (const T*)p.j.p + min(j0 + (lane & 15), (long long)p.cols - 1) * p.j.ld;
     const T* x = (const T*)p.i.p + (long long)min(lane & 15, p.rows - 1) * p.i.ld;
@@ -456,12 +456,10 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
 }
 template <typename T, bool FLOAT>
 void launch_grad_few_rows(const ProductParams& p, const LossGradParams& l, hipStream_t stream) {
-    const int shares = few_shares(p.cols, p.sum, (int)sizeof(T)), outputs = kFewOutputs * kFewWaves / shares;
-    const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
-    if (shares == 8)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_grad_few_rows_kernel<T, 8, FLOAT>), grid, dim3(64 * kFewWaves), 0, stream, p, l);
-    else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_grad_few_rows_kernel<T, 2, FLOAT>), grid, dim3(64 * kFewWaves), 0, stream, p, l);
+    const int shares = few_shares(p.cols, p.sum, (int)sizeof(T));
+    by_few_columns(p, shares, kFewOutputs * kFewWaves / shares, [&](auto s, dim3 grid, const ProductParams& q) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_grad_few_rows_kernel<T, s.value, FLOAT>), grid, dim3(64 * kFewWaves), 0, stream, q, l);
+    });
 }
 
 // ---- plans
@@ -660,12 +658,10 @@ extern "C" int tcbnn_linear_loss_forward(const tcbnn_linear_loss_desc* d, void* 
         if (plan.pack_w) at += packed_bytes(piece, p.sum, (int)sizeof(T));
         LossParams l = {d->loss ? d->targets : nullptr, (float2*)at, (float*)(at + whole_lines((size_t)plan.parts * p.rows * sizeof(float2))), p.rows, 0};
         if (plan.few) {
-            const int shares = few_shares(p.cols, p.sum, (int)sizeof(T)), outputs = kFewOutputs * kFewWaves / shares;
-            const dim3 grid((unsigned)(p.cols / outputs + (p.cols % outputs != 0)));
-            if (shares == 8)
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_few_rows_kernel<T, 8>), grid, dim3(64 * kFewWaves), 0, s, p, l);
-            else
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_few_rows_kernel<T, 2>), grid, dim3(64 * kFewWaves), 0, s, p, l);
+            const int shares = few_shares(p.cols, p.sum, (int)sizeof(T));
+            by_few_columns(p, shares, kFewOutputs * kFewWaves / shares, [&](auto n, dim3 grid, const ProductParams& q) {
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(loss_few_rows_kernel<T, n.value>), grid, dim3(64 * kFewWaves), 0, s, q, l);
+            });
         } else {
             by_tile(plan.access, plan.plan.cut, plan.brief, [&](auto size, auto wi, auto wj, auto ws, auto stages, auto how, auto hold, auto keep) {
                 constexpr int B = size.value, kThreads = 64 * wi.value * wj.value * ws.value;

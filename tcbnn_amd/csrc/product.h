@@ -327,6 +327,7 @@ struct ProductParams {
     int plane;
     long long i_low;
     bool padded_i, padded_j;  // the operand's rows, 16 bytes or more, go on with zeros to whole 16 bytes
+    int first;                // the first column of a launch for few rows
 };
 enum Carry : int { NO_CARRY, CARRY_FIRST, CARRY_ON };
 
@@ -771,6 +772,21 @@ inline float few_time(int rows, int cols, int sum, int size, bool vectors) {
     const float chunks = std::ceil((float)sum * (float)size / (64.0f * (float)shares)), n = (float)rows;
     const float latency = vectors ? 0.25f + 0.01f * n : 0.45f + 0.035f * n, more = vectors ? 0.2875f + 0.0095f * n : 0.85f + 0.1f * n;
     return 2.4f + chunks * std::max(latency, blocks * more) + blocks * (shares == 2 ? 0.7f : 1.4f);
+}
+
+// A product of few rows whose workgroups have `outputs` columns each: go(shares, grid, its parameters), columns beyond a launch's threads (2^27 with 16 a workgroup) in
+// launches of their own.
+template <typename F>
+void by_few_columns(ProductParams p, int shares, int outputs, F&& go) {
+    const int blocks = p.cols / outputs + (p.cols % outputs != 0), most = (int)(kMaxThreads / (64 * kFewWaves));
+    for (int first = 0; first < blocks; first += most) {
+        p.first = first * outputs;
+        const dim3 grid((unsigned)std::min(most, blocks - first));
+        if (shares == 8)
+            go(std::integral_constant<int, 8>(), grid, p);
+        else
+            go(std::integral_constant<int, 2>(), grid, p);
+    }
 }
 
 template <typename T, bool ACROSS_I, bool ACROSS_J>
