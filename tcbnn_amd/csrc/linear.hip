@@ -143,12 +143,9 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
     if (i >= p.rows) return;
     const int j = (int)(v - i * per_row) * C, n = min(C, p.cols - j);
     Columns<float, C> part[kMaxSplits];
-    auto get = [&](int first) {
 #pragma unroll
-        for (int k = 0; k < kMaxSplits; ++k)
-            if (first + k < p.splits) part[k] = get_columns<float, C>(p.partial + (first + k) * p.partial_stride, p.cols, i, j, n);
-    };
-    get(0);
+    for (int k = 0; k < kMaxSplits; ++k)
+        if (k < p.splits) part[k] = get_columns<float, C>(p.partial + k * p.partial_stride, p.cols, i, j, n);
     float z[C], bias[C];
 #pragma unroll
     for (int e = 0; e < C; ++e) {
@@ -157,16 +154,12 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductParams p
     }
     Columns<T, C> residual = {};
     if (p.residual) residual = get_columns<T, C>(p.residual, p.residual_ld, i, j, n);
-    for (int first = 0;; get(first)) {
 #pragma unroll
-        for (int k = 0; k < kMaxSplits; ++k)
-            if (first + k < p.splits) {
+    for (int k = 0; k < kMaxSplits; ++k)
+        if (k < p.splits) {
 #pragma unroll
-                for (int e = 0; e < C; ++e) z[e] += part[k][e];
-            }
-        first += kMaxSplits;
-        if (first >= p.splits) break;
-    }
+            for (int e = 0; e < C; ++e) z[e] += part[k][e];
+        }
     finish<T, C>(p, i, j, n, bias, residual, z);
 }
 

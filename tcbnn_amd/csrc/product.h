@@ -308,11 +308,15 @@ struct Tile {
     }
 };
 
+// (A kernel's parameters come in lines of 64 bytes, whose first reading a small call waits for: what a kernel begins with is in the first, what it ends
+// with in the second, and partial sums and planes behind them.)
 struct ProductParams {
     Operand i, j;
     int rows, cols, sum;  // c is rows x cols
     int tiles_i, tiles_j, splits, split_sum;
+    int first;             // the first column of a launch for few rows
     int activation;
+    int carry;             // the sum goes on in `partial`: CARRY_FIRST writes it, CARRY_ON adds to what is there
     const float* bias;     // [cols], or NULL
     const void* residual;  // or NULL
     void* out;
@@ -320,14 +324,12 @@ struct ProductParams {
     long long residual_ld, out_ld, preact_ld;
     float* partial;        // splits > 1 or a carry: [splits][rows][cols]
     long long partial_stride;  // from one split's to the next one's
-    int carry;             // the sum goes on in `partial`: CARRY_FIRST writes it, CARRY_ON adds to what is there
     const float* factor;   // of the sums, or NULL (a power of two: nothing is rounded by it)
     // I in two planes whose products are added, the second i_low elements behind the first: the sum goes over a step of the first and the same step of the
     // second in turn, so that J's steps are in the cache when they are read again.  `plane`: the sum in whole steps (0: one plane).
     int plane;
     long long i_low;
     bool padded_i, padded_j;  // the operand's rows, 16 bytes or more, go on with zeros to whole 16 bytes
-    int first;                // the first column of a launch for few rows
 };
 enum Carry : int { NO_CARRY, CARRY_FIRST, CARRY_ON };
 
