@@ -581,8 +581,8 @@ int tcbnn_gated_kernel_name(const tcbnn_gated_desc* d, char* buf, size_t len);
 
 /* With z as the forward call wrote it, dz of the gate = grad_output * (z of the rest) * act'(z of the gate), dz of the rest =
  * grad_output * act(z of the gate):  grad_input = dz * weight, grad_weight = dz^T * input, grad_bias = sums of dz over the rows.  Each of
- * the three may be NULL; what is given is overwritten.  relu'(0) = 0.  In 16-bit types dz is rounded to dtype before the two products;
- * grad_bias sums it unrounded.  `workspace` holds tcbnn_gated_grad_workspace_bytes; with `anywhere` these are enough for copies of operands whose
+ * the three may be NULL; what is given is overwritten.  relu'(0) = 0.  In 16-bit types dz is rounded to dtype before the two products (f16: a dz
+ * beyond 65504 is infinite there); grad_bias sums it unrounded.  `workspace` holds tcbnn_gated_grad_workspace_bytes; with `anywhere` these are enough for copies of operands whose
  * rows do not lie at whole 16 bytes, where these are faster (without, such operands are read as they lie). */
 typedef struct tcbnn_gated_grad_desc {
     const void* input;        /* [rows][in_features]; NULL where grad_weight is          */

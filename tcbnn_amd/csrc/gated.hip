@@ -5,8 +5,8 @@
 // rest, so that g and u of a column are in one lane's registers when the sum is done, and z leaves only where it is asked for.
 // Backward, [dg du] is one matrix of 2 n columns, as w is one of 2 n rows: a pass makes it, and two products of the linear layer's follow.
 //
-// Large products are bound by the matrix instructions, 8192 x 4096 -> 2 x 8192 bf16 with z kept 880 us (1.25 PFLOP/s), gradients of 8192 x 1024 -> 2 x 4096
-// 289 us, of which the products take 226 (1.22 PFLOP/s) and the pass 58 (5.8 TB/s); single rows by the weights' bytes, 1 x 4096 -> 2 x 8192
+// Large products are bound by the matrix instructions, 8192 x 4096 -> 2 x 8192 bf16 with z kept 877 to 929 us from card to card (1.25 to 1.18 PFLOP/s), gradients of 8192 x
+// 1024 -> 2 x 4096 289 to 311 us, of which the products take 225 to 250 (1.22 to 1.10 PFLOP/s) and the pass 58 (5.8 TB/s); single rows by the weights' bytes, 1 x 4096 -> 2 x 8192
 // 26 us (5.1 TB/s, the launch included); 77 x 1023 -> 2 x 1537 f16 takes 8.5 us, steps of the sum one after the other.
 #include "product.h"
 

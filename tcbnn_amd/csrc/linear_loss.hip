@@ -5,9 +5,9 @@
 // exp(z - m), 8 bytes for a tile's width of logits, and z_t from the one lane that has it.  A second launch joins them.
 // Backward, z is made again, a piece of the classes at a time, and becomes d where it lies; d goes to the workspace in the operands' type and from
 // there through two products.  dx is summed over the pieces in fp32.  With pieces of kPieceBytes that are read back from the cache, four products
-// (8 rows classes inputs operations a step) are nearly all of the time: 8192 x 1024 -> 131072 bf16 7.9 ms, z 1.84 (1.20 PFLOP/s), d 2.33, dx 1.91, dw
+// (8 rows classes inputs operations a step) are nearly all of the time: 8192 x 1024 -> 131072 bf16 7.9 to 8.6 ms from card to card, in the former z 1.84 (1.20 PFLOP/s), d 2.35, dx 1.93, dw
 // 1.86.  Single rows are bound by the weights' bytes, 1 x 4096 -> 131072 173 us (6.2 TB/s); small steps by their launches one after
-// the other, 256 x 512 -> 1000 fp32 36 us; weights' gradients of few rows by what they write, 333 x 1000 -> 32003 f16 42 us of the step's 173.
+// the other, 256 x 512 -> 1000 fp32 37 us; weights' gradients of few rows by what they write, 333 x 1000 -> 32003 f16 42 us of the step's 174 to 191.
 #include "product.h"
 
 namespace tcbnn {
