@@ -175,3 +175,41 @@ def test_loss_gradients_of_logits_that_are_known_to_no_unit(gpu, m, k, n, dtype)
         # (a class that has the largest logit, and the given one)
         assert np.isfinite(dx.get()).all()
         layer.release()
+
+
+@pytest.mark.parametrize("dtype", ho.DTYPES)
+@pytest.mark.parametrize("m,k,n", [(2, 64, 300), (12, 40, 700), (300, 61, 304)])
+def test_loss_without_what_may_be_missing(gpu, m, k, n, dtype):
+    """Each output of the forward call alone; gradients from logsumexp alone."""
+    from tcbnn_amd import head
+    r = rng(m, k, n, 5)
+    x, w = (ho.Matrix(r.standard_normal((rows, k)), dtype) for rows in (m, n))
+    t, g = r.integers(-1, n, m).astype(np.int32), (0.5 + r.random(m)).astype(np.float32)
+    b = (30 + r.standard_normal(n)).astype(np.float32)
+    dx, dw, db = ho.Matrix(None, dtype, 0, m, k), ho.Matrix(None, dtype, 0, n, k), ho.empty(n)
+    layer = head.LinearLossLayerParam("loss", m, k, n, dtype).initialize(w.view, b, x.view, ho.vector(t, np.int32))
+    layer.initialize_backward(ho.vector(g), dx.view, dw.view, db)
+    layer.forward()
+    names = ("loss", "logsumexp", "logsumexp_rest")
+    buffers = [getattr(layer, name + "_gpu") for name in names]
+    all_at_once = [buf.to_numpy(np.float32, (m,)) for buf in buffers]
+    for i, name in enumerate(names):
+        for other in names:
+            setattr(layer._desc, other, None)
+        alone = ho.empty(m)
+        setattr(layer._desc, name, alone.ptr)
+        layer._desc.targets = layer.targets_gpu.ptr if name == "loss" else None
+        layer.forward()
+        ho.sync()
+        np.testing.assert_array_equal(alone.to_numpy(np.float32, (m,)), all_at_once[i])
+    layer._grad_desc.loss = layer._grad_desc.logsumexp_rest = None
+    layer.backward()
+    ho.sync()
+    _, _, lse, lse_err, z, zerr, p = bo.loss(x.values, w.values, b.astype(np.float64), t, g)
+    exact = bo.loss_grads(x.values, w.values, t, g.astype(np.float64), z, zerr, p, lse, lse_err, dtype)
+    for name, buf in (("input", dx), ("weight", dw)):
+        e, err = exact[name]
+        ho.check(buf.get(), e, bo.out_error(e, err, dtype), "grad of " + name)
+    e, err = exact["bias"]
+    ho.check(db.to_numpy(np.float32, (n,)), e, 1.1 * err + ho.TINY["f32"], "grad of bias")
+    layer.release()
